@@ -179,8 +179,8 @@ int32_t b200_event_elapsed_ms(void *start, void *end, float *ms);
 int32_t b200_event_destroy(void *event);
 
 /* Sticky device-side error bits of the library's kernels on `device` (bit 0: a bounded
- * mbarrier / flag wait gave up and the kernel returned early). Synchronous; `clear` != 0
- * resets them. Replaces the sticky `failure` of runtime/ops_dx12.py:171,195-198. */
+ * mbarrier / flag wait gave up and the kernel returned early; bit 1: a slot, page or position
+ * of a cache call lay outside its table). Synchronous; `clear` != 0 resets them. Replaces the sticky `failure` of runtime/ops_dx12.py:171,195-198. */
 int32_t b200_device_status(int32_t device, uint32_t *flags, int32_t clear);
 
 /* Device-side bounded wait (failure detection without a GPU fault): a one-thread kernel
@@ -249,6 +249,99 @@ int32_t b200_peer_allreduce_add_rmsnorm(const void *const *partials, uint32_t *c
 int32_t b200_ipc_get_handle(void *dev_ptr, void *handle64);
 int32_t b200_ipc_open(const void *handle64, void **dev_ptr);
 int32_t b200_ipc_close(void *dev_ptr);
+
+/* ---- attention over a packed key/value cache -------------------------------------------
+ * No counterpart in the reference, whose packed path ends at one matmul. Keys and values are
+ * held as codes with block scales, in pages that requests name in tables:
+ *   codes   [pages, kv_heads, page_size, head_dim * bits / 8], lowest bits first
+ *   scales  [pages, kv_heads, page_size, head_dim / block_size], bfloat16 or E8M0
+ * of any strides with contiguous rows: heads before tokens or tokens before heads.
+ * A block's scale is s = bf16(max|x| * (1 / QMAX)), or the smallest power of two not below
+ * max|x| * (1 / QMAX) for E8M0, held within [2^-100, 2^100]; x is stored as the code nearest to
+ * x * (1 / s), ties to even (QMAX: 127, 448, 7, 6). A NaN makes its block's scale NaN. Cell
+ * (page, offset) is slot page * page_size + offset. */
+#define B200_CACHE_INT8 0
+#define B200_CACHE_FP8E4M3 1
+#define B200_CACHE_INT4 2
+#define B200_CACHE_FP4_E2M1 3
+typedef struct b200_cache_desc {
+  void *k, *v;               /* codes, 16-byte aligned                                  */
+  void *k_scales, *v_scales; /* scales, 16-byte aligned                                 */
+  int64_t pages;
+  int32_t page_size;         /* a power of two, at least 16                             */
+  int32_t kv_heads;
+  int32_t head_dim;          /* 64, 128 or 256                                          */
+  int32_t block_size;        /* 32 or head_dim                                          */
+  int32_t format;            /* B200_CACHE_*                                            */
+  int32_t scale_dtype;       /* B200_DT_BF16 or B200_DT_E8M0                            */
+  int64_t strides[3];        /* of k and v: page, head, token, in bytes, multiples of 16 */
+  int64_t scale_strides[3];  /* of the scales: page, head, token, in elements           */
+} b200_cache_desc;
+
+/* Tables of cosines and sines, fp32 [rows, rotary_dim / 2], contiguous: row p turns position p. */
+typedef struct b200_rotary_desc {
+  const float *cos, *sin;
+  int64_t rows;
+  int32_t rotary_dim;   /* even, at most head_dim: the values behind it are not turned  */
+  int32_t interleaved;  /* pairs (2i, 2i + 1) instead of (i, i + rotary_dim / 2)        */
+} b200_rotary_desc;
+
+/* y = x turned by its positions: pair (a, b) becomes (a cos - b sin, b cos + a sin); `transpose`
+ * takes -sin (the gradient). x, y: [batch, tokens, heads, head_dim] of F16, BF16 or F32, unit
+ * stride along head_dim, element strides of the other axes in x_strides / y_strides (3 each);
+ * y may be x with equal strides. positions: batch * tokens contiguous I32 or I64. A position
+ * outside the table gives NaN and sets bit 1 of b200_device_status. */
+int32_t b200_rotary(const void *x, int32_t dtype, int64_t batch, int64_t tokens, int32_t heads, int32_t head_dim,
+                    const int64_t *x_strides, void *y, const int64_t *y_strides, const b200_rotary_desc *table,
+                    const void *positions, int32_t positions_dtype, int32_t transpose, void *stream);
+
+/* Store tokens' keys (turned first when `table` is given) and values in the cells `slots` names
+ * (I32 or I64; negative: not stored; beyond the cache: not stored, bit 1 of b200_device_status).
+ * k, v: [tokens, kv_heads, head_dim] with element strides (token, head), F16, BF16 or F32. With
+ * `q` ([tokens, q_heads, head_dim], same type) the turned queries go to q_out (contiguous, 16-byte
+ * aligned). Two tokens of one call must not name one slot. */
+int32_t b200_cache_write(const b200_cache_desc *cache, const void *k, const void *v, int32_t dtype, int64_t tokens,
+                         const int64_t *k_strides, const int64_t *v_strides, const void *slots, int32_t slots_dtype,
+                         const b200_rotary_desc *table, const void *positions, int32_t positions_dtype, const void *q,
+                         int32_t q_heads, const int64_t *q_strides, void *q_out, void *stream);
+
+/* The values that the cells `slots` hold, as `dtype` (F16, BF16, F32), contiguous [tokens, kv_heads,
+ * head_dim], 16-byte aligned. Negative slots and slots beyond the cache (bit 1 of
+ * b200_device_status) read zeros. */
+int32_t b200_cache_read(const b200_cache_desc *cache, const void *slots, int32_t slots_dtype, int64_t tokens,
+                        void *k_out, void *v_out, int32_t dtype, void *stream);
+
+/* Softmax attention of `queries` tokens per request over its cached keys and values. Request b has
+ * min(max(lengths[b], 0), max_pages * page_size) keys, key i at offset i % page_size of page
+ * tables[b * table_stride + i / page_size]; its tokens are the last of them, so query j sees keys
+ * 0 .. lengths[b] - queries + j. With prefix_length > 0 every query first sees that many keys of
+ * the pages `prefix`, shared by the batch and read once for all. Rows that see no key give zeros
+ * (lse: -inf). A page outside the cache counts as absent keys and sets bit 1 of
+ * b200_device_status. q: F16 or BF16, element strides (request, token, head), unit along head_dim;
+ * out: contiguous [batch, queries, heads, head_dim] of q's type; lse: fp32 [batch, queries, heads]
+ * natural logarithms of the softmax sums, or NULL. `scratch` holds b200_cache_attention_scratch()
+ * bytes (prefix only). Allocates a workspace (10 MiB) on the first call per (device, stream); when
+ * that first call is captured into a graph it runs without one, with less parallelism. */
+typedef struct b200_attention_args {
+  const void *q;
+  int64_t q_strides[3];
+  const int32_t *tables;
+  const int32_t *lengths;
+  const int32_t *prefix;
+  void *out;
+  float *lse;
+  void *scratch;
+  int64_t batch, queries;
+  int64_t table_stride, max_pages;
+  int64_t prefix_pages, prefix_length;
+  int32_t q_dtype;
+  int32_t heads;  /* a multiple of kv_heads: head h reads key head h / (heads / kv_heads) */
+  float scale;    /* multiplies q . k */
+  int32_t reserved;
+} b200_attention_args;
+int64_t b200_cache_attention_scratch(int64_t batch, int64_t queries, int32_t heads, int32_t head_dim,
+                                     int64_t prefix_length);
+int32_t b200_cache_attention(const b200_cache_desc *cache, const b200_attention_args *args, void *stream);
 
 #ifdef __cplusplus
 }

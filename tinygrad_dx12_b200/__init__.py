@@ -8,8 +8,10 @@ from .compat import register as register
 from .packed import FORMATS, FP8_CANDIDATES, PackedTensor, matrix_intermediate
 from .linalg import Estimates, choose_matrix, estimates, matmul, matvec, set_profile_hook
 from .graph import GraphStep
+from .attention import PackedCache, RotaryTable, cache_attention, cache_read, cache_write, rotary
 
 register()
 
 __all__ = ["register", "FORMATS", "FP8_CANDIDATES", "PackedTensor", "matrix_intermediate", "matmul", "matvec",
-           "choose_matrix", "Estimates", "estimates", "set_profile_hook", "GraphStep"]
+           "choose_matrix", "Estimates", "estimates", "set_profile_hook", "GraphStep", "PackedCache",
+           "RotaryTable", "cache_attention", "cache_read", "cache_write", "rotary"]

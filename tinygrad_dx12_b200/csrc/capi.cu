@@ -45,6 +45,8 @@ static int32_t injected() {
   return 0;
 }
 
+int32_t b200_injected() { return injected(); }
+
 using namespace b200;
 
 static int32_t validate_desc(const b200_packed_desc *w) {
@@ -302,8 +304,11 @@ int32_t b200_device_status(int32_t device, uint32_t *flags, int32_t clear) {
   if (int32_t rc = stackops_device_error(&z, clear != 0)) return rc;
   if (int32_t rc = gemm_dense_device_error(&dd, clear != 0)) return rc;
   if (int32_t rc = mx_device_error(&mxe, clear != 0)) return rc;
-  *flags = v | u | w | z | dd | mxe;
-  if (clear != 0 && *flags != 0)  // a kernel gave up mid-way: its split-tile tickets may be half counted
+  unsigned int co = 0, ca = 0;
+  if (int32_t rc = cache_ops_device_error(&co, clear != 0)) return rc;
+  if (int32_t rc = cache_attn_device_error(&ca, clear != 0)) return rc;
+  *flags = v | u | w | z | dd | mxe | co | ca;
+  if (clear != 0 && (*flags & 1u) != 0)  // a kernel gave up mid-way: its split-tile tickets may be half counted
     if (int32_t rc = mx_reset_tickets()) return rc;
   return B200_OK;
 }

@@ -90,4 +90,12 @@ int32_t stackops_device_error(unsigned int *v, bool clear);
 int32_t launch_gate_mul(const void *gu, int gdt, void *out, int odt, int64_t M, int64_t I, cudaStream_t stream);
 int32_t launch_wait_flag(const int32_t *flag, int32_t expect, int64_t max_spins, int32_t *status, cudaStream_t stream);
 
+
+// packed key/value cache: rotary positions, writing, reading (cache_ops.cu), attention (cache_attn.cu)
+int32_t check_cache(const b200_cache_desc *c);
+int32_t cache_ops_device_error(unsigned int *v, bool clear);
+int32_t cache_attn_device_error(unsigned int *v, bool clear);
+
 }  // namespace b200
+
+int32_t b200_injected();  // non-zero (the code) when this compute entry call should fail (capi.cu)
