@@ -14,18 +14,23 @@
 //
 // m16n8k16 takes keys as its 16 rows and query rows (heads that share a key head, and the tokens of
 // a short block) as its 8 columns: s^T = K q^T, out^T = V^T p^T. Which value of the head sits at
-// which k of an instruction is free as long as both operands agree, so a lane reads 16 consecutive
-// bytes of a key row and q is laid out to match; a lane reads four values' worth of tokens of V^T
-// at its 16 (8, 32) values of the head, and pairs of tokens are joined by byte permutes before
-// the codes become fp16. p is turned with movmatrix. Keys therefore go from memory to registers
-// to the tensor core: no shared memory, no barrier on the way. A warp works alone on units of 16
-// or 32 keys, issues the loads of its next keys as soon as the registers are free, and 16 warps of
-// an SM hide the latency.
+// which k of an instruction is free as long as both operands agree: lane t of four holds values
+// 8t .. 8t + 7 of each 32, so that a k step stays within one scale block, whose sum is multiplied by
+// its scale in fp32. For V^T a lane reads its D / 8 neighbouring values of four keys; pairs of keys
+// are joined by byte permutes before the codes become fp16. p is turned with movmatrix.
 //
-// The units of all (request, key head, row tile) are laid end to end and cut into equal runs, one
-// per CTA, from the lengths on the device: ragged batches balance, and the launch (a CUDA graph)
-// does not depend on the lengths. A CTA's warps take its units in turn and join in shared memory;
-// a segment cut over several CTAs is joined by the CTA that finishes last, always in the same order.
+// Every warp works alone: it copies units of 16 to 64 keys (4 KB of codes) into a ring of its own
+// with cp.async, 16 bytes a lane, two units ahead, chunks xor-ed by their row so that both operands'
+// reads spread over the banks; a lane loads the scales of one key three units ahead and leaves what
+// the scores need of them beside the ring. Page numbers are read one unit earlier still. 16 warps of
+// an SM keep up to 128 KB in flight, and no barrier stands between a segment's units.
+//
+// The units of all (request, key head, row tile) segments are laid end to end in rounds (a unit for
+// each warp) and cut into equal runs, one per CTA, from the lengths on the device: ragged batches
+// balance, and the launch (a CUDA graph) does not depend on the lengths. Where there is little work,
+// segments start on run boundaries instead, so that short ones are not cut. A CTA's warps join in
+// shared memory; a segment cut over several CTAs is joined by the CTA that finishes last, always in
+// the same order.
 #include <map>
 #include <mutex>
 
@@ -44,9 +49,10 @@ namespace cattn {
 
 using namespace cache;
 
-constexpr int WARPS = 8, THREADS = WARPS * 32;
-constexpr int MAX_ENTRIES = 4096;  // (request, row tile) pairs of one launch
-constexpr float LAZY = 4.f;         // u may pass the running maximum by this before it moves
+constexpr int WARPS = 8, THREADS = WARPS * 32, STAGES = 2;
+constexpr int MAX_ENTRIES = 1024;    // (request, row tile) pairs of one launch
+constexpr int SHORT = 4;             // rounds that a segment is not cut below where work is scarce
+constexpr float LAZY = 4.f;          // u may pass the running maximum by this before it moves
 constexpr float BIAS = 15.f - LAZY;  // p = 2^(u - m + BIAS) uses fp16 up to 2^15, so small weights keep their bits
 
 struct Params {
@@ -55,7 +61,7 @@ struct Params {
   const uint8_t *k, *v;
   const void *ks, *vs;
   int64_t cp, ch, ct, sp, sh, st;  // strides of codes (bytes) and scales: page, head, token
-  int e8m0;
+  int e8m0, scale_vec, q_vec;
   int64_t pages;
   int page_shift, kv_heads, group;
   const int32_t *tables;
@@ -78,24 +84,47 @@ struct Params {
   uint32_t *tickets;
 };
 
-template <int F, int D, int NT>
+template <int F, int D, int NT, bool BLK>
 struct Cfg {
   static constexpr int bits = CFmt<F>::bits;
-  static constexpr int RB = D * bits / 8;                       // bytes of a row
-  static constexpr int KCB = RB / 4 < 16 ? RB / 4 : 16;         // bytes of a lane's key chunk
-  static constexpr int KCH = RB / 4 / KCB, KCW = KCB / 4;       // chunks, words of one
-  static constexpr int KEC = KCB * 8 / bits;                    // values of one
-  static constexpr int VCB = RB / 8 < 16 ? RB / 8 : 16;
-  static constexpr int VCH = RB / 8 / VCB, VCW = VCB / 4;
-  static constexpr int VEC = VCB * 8 / bits;
-  static constexpr int KS = D / 16;                             // k steps of q K^T
-  static constexpr int MT = D / 16;                             // tiles of V^T
-  static constexpr int M2 = RB >= 128 ? 1 : 2;                  // blocks of 16 keys in a unit
+  static constexpr int RB = D * bits / 8;                              // bytes of a row
+  static constexpr int T = RB == 32 ? 64 : RB == 64 ? 32 : 16;         // keys of a unit
+  static constexpr int CPR = RB / 16;                                  // 16-byte chunks of a row
+  static constexpr int RPI = 32 / CPR;                                 // rows that 32 lanes copy at once
+  static constexpr int NB = D / 32;                                    // blocks of 32 values
+  static constexpr int KNB = BLK ? NB : 1;                             // scales of a row
+  static constexpr int VCB = RB / 8 < 16 ? RB / 8 : 16;                // bytes of a lane's value chunk
+  static constexpr int VCH = RB / 8 / VCB, VCW = VCB / 4;              // chunks, words of one
+  static constexpr int VEC = VCB * 8 / bits;                           // values of one
+  static constexpr int MT = D / 16;                                    // tiles of V^T
   static constexpr int ROWS = 8 * NT;
-  static constexpr int Q_BYTES = NT * KS * 32 * 8;
-  static constexpr int ORS = D + 4;                             // row pitch of a warp's numerators (floats)
-  static constexpr int JOIN_BYTES = WARPS * ROWS * ORS * 4;
-  static constexpr int SMEM = Q_BYTES + JOIN_BYTES + WARPS * ROWS * 8 + ROWS * 16;
+  static constexpr int STAGE = 2 * T * RB;                             // codes of a unit
+  // what the scores need of a unit's scales: (log2 of the value scale, its inverse) per key, key
+  // scales, and in blocks the ratios of the value scales to their row's
+  static constexpr int LVI = T * 8, KSB = T * KNB * 4, VRB = BLK ? T * NB * 2 : 0;
+  static constexpr int SLOT = LVI + KSB + VRB;
+  static constexpr int HALF = D / 2, ORS = HALF + 4;                   // values and row pitch of a join pass
+  static constexpr int JOIN = WARPS * ROWS * ORS * 4;
+  static constexpr int SMEM = WARPS * STAGES * (STAGE + SLOT) + JOIN + 2 * WARPS * ROWS * 4;
+  static constexpr int CTAS = D == 256 || NT == 2 ? 1 : 2;             // per SM
+
+  // key of a unit's 16 that row r of an instruction's first 8 rows holds (row r + 8: the same + 8),
+  // chosen with chunk() so that a read of 32 lanes meets no bank twice
+  __device__ static __forceinline__ int key_of(int r) {
+    if constexpr (bits == 4) return r;
+    else if constexpr (RB == 64) return (r & 1) | ((r & 2) << 1) | ((r & 4) >> 1);
+    else return 2 * (r & 3) + (r >> 2);
+  }
+  __device__ static __forceinline__ int row_of(int k) {  // the inverse
+    if constexpr (bits == 4) return k;
+    else if constexpr (RB == 64) return (k & 1) | ((k & 4) >> 1) | ((k & 2) << 1);
+    else return (k >> 1) | ((k & 1) << 2);
+  }
+  // byte of chunk c of row `row` in a tile
+  __device__ static __forceinline__ int chunk(int row, int c) {
+    const int x = RB == 32 ? c ^ ((row >> 2) & 1) : RB == 64 ? c ^ ((row >> 1) & 3) : c ^ (row & 7);
+    return row * RB + x * 16;
+  }
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -121,16 +150,23 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
   const __half2 r = __hmul2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
   return *reinterpret_cast<const uint32_t *>(&r);
 }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool in) {  // zeros where not `in`
+  const int n = in ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 template <int BYTES>
-__device__ __forceinline__ void load_words(const uint8_t *p, uint32_t *w) {
+__device__ __forceinline__ void lds(const uint8_t *p, uint32_t *w) {
   if constexpr (BYTES == 16) {
-    const uint4 x = __ldg(reinterpret_cast<const uint4 *>(p));
+    const uint4 x = *reinterpret_cast<const uint4 *>(p);
     w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
   } else if constexpr (BYTES == 8) {
-    const uint2 x = __ldg(reinterpret_cast<const uint2 *>(p));
+    const uint2 x = *reinterpret_cast<const uint2 *>(p);
     w[0] = x.x, w[1] = x.y;
   } else {
-    w[0] = __ldg(reinterpret_cast<const uint32_t *>(p));
+    w[0] = *reinterpret_cast<const uint32_t *>(p);
   }
 }
 
@@ -144,88 +180,6 @@ struct RowRef {
   __device__ static __forceinline__ float value(int e) { return __uint_as_float((uint32_t)e << 23); }
 };
 
-// A scale's bits, nothing for NaN: the NaN of a row travels in its denominator, which only rows that
-// see the key take.
-__device__ __forceinline__ uint32_t number(uint32_t bits) { return bits > 0x7F80u ? 0u : bits; }
-
-// Where 16 keys' codes and scales begin.
-struct At {
-  int64_t code, scale;
-};
-
-// The codes and scales of 16 keys as a lane holds them.
-template <int F, int D, int NT, bool BLK>
-struct Keys {
-  using C = Cfg<F, D, NT>;
-  static constexpr int NB = D / 32;
-  uint32_t k[2][C::KCH * C::KCW];
-  uint32_t v[4][C::VCH * C::VCW];
-  uint32_t ks[2][BLK ? C::KCH : 1];  // bfloat16 bits
-  uint32_t vs[2];                    // of the two keys of this lane's scores (blocks: the largest)
-  uint32_t kt[2];                    // blocks: the largest of the two keys'
-  uint32_t vb[BLK ? 4 : 1][BLK ? C::VCH : 1];
-};
-
-template <int F, int D, int NT, bool BLK>
-__device__ __forceinline__ void load_k(Keys<F, D, NT, BLK> &x, const Params &p, At at, int valid, int g, int t) {
-  using C = Cfg<F, D, NT>;
-  constexpr int NB = D / 32;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int tok = 4 * (g >> 1) + (g & 1) + 2 * i;
-    const bool in = tok < valid;
-    const int64_t r = at.scale + tok * p.st;
-    if (in) {
-#pragma unroll
-      for (int c = 0; c < C::KCH; ++c)
-        load_words<C::KCB>(p.k + at.code + tok * p.ct + (t + 4 * c) * C::KCB, &x.k[i][c * C::KCW]);
-    } else {
-#pragma unroll
-      for (int c = 0; c < C::KCH * C::KCW; ++c) x.k[i][c] = 0;
-    }
-    if constexpr (!BLK) {
-      x.ks[i][0] = in ? scale_bits(p.ks, r, p.e8m0) : 0x3F80u;
-      x.vs[i] = in ? scale_bits(p.vs, r, p.e8m0) : 0x3F80u;
-    } else {
-      uint32_t kt = 0, vt = 0;  // the largest over this lane's share of the blocks, then over the quad
-#pragma unroll
-      for (int c = 0; c < C::KCH; ++c)
-        x.ks[i][c] = in ? scale_bits(p.ks, r + (t + 4 * c) * C::KEC / 32, p.e8m0) : 0u;
-#pragma unroll
-      for (int b = 0; b < (NB + 3) / 4; ++b) {
-        const int nb = min(t + 4 * b, NB - 1);
-        if (in) {
-          kt = max(kt, scale_bits(p.ks, r + nb, p.e8m0));
-          vt = max(vt, scale_bits(p.vs, r + nb, p.e8m0));
-        }
-      }
-      x.kt[i] = kt, x.vs[i] = vt;
-    }
-  }
-}
-template <int F, int D, int NT, bool BLK>
-__device__ __forceinline__ void load_v(Keys<F, D, NT, BLK> &x, const Params &p, At at, int valid, int g, int t) {
-  using C = Cfg<F, D, NT>;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int tok = 4 * t + i;
-    if (tok < valid) {
-#pragma unroll
-      for (int c = 0; c < C::VCH; ++c) {
-        load_words<C::VCB>(p.v + at.code + tok * p.ct + (g + 8 * c) * C::VCB, &x.v[i][c * C::VCW]);
-        if constexpr (BLK)
-          x.vb[i][c] = scale_bits(p.vs, at.scale + tok * p.st + (g + 8 * c) * C::VEC / 32, p.e8m0);
-      }
-    } else {  // nothing of a key that is not there: its codes may be anything
-#pragma unroll
-      for (int c = 0; c < C::VCH * C::VCW; ++c) x.v[i][c] = 0;
-      if constexpr (BLK)
-#pragma unroll
-        for (int c = 0; c < C::VCH; ++c) x.vb[i][c] = 0;
-    }
-  }
-}
-
 // Query row r of (entry, key head h): its offset in q, and its place among all rows of out.
 struct RowAt {
   int64_t q, out;
@@ -235,22 +189,6 @@ __device__ __forceinline__ RowAt row_at(const Params &p, int b, int h, int r) {
   const int rq = tok / p.per_request, qi = tok - rq * p.per_request;
   const int64_t req = b + rq;
   return {req * p.qsr + qi * p.qsb + head * p.qsh, (req * p.per_request + qi) * p.q_heads + head};
-}
-
-// Half index in shared memory of value d of query row n: the order in which a lane's codes of a
-// key row come out of their decoding.
-template <int F, int D, int NT>
-__device__ __forceinline__ int q_index(int n, int d) {
-  using C = Cfg<F, D, NT>;
-  const int chunk = d / C::KEC, t = chunk & 3, c = chunk >> 2, w = d % C::KEC;
-  int step, reg, half;
-  if constexpr (F == B200_CACHE_INT4) {  // words of 8: pairs (i, i + 4)
-    const int pi = w & 3;
-    step = (w >> 3) * 2 + (pi >> 1), reg = pi & 1, half = (w >> 2) & 1;
-  } else {
-    step = w >> 2, reg = (w >> 1) & 1, half = w & 1;
-  }
-  return ((((n >> 3) * C::KS + c * (C::KEC / 4) + step) * 32 + (n & 7) * 4 + t) * 2 + reg) * 2 + half;
 }
 
 template <typename T>
@@ -282,68 +220,137 @@ __device__ __forceinline__ void finish(const Params &p, int64_t row, int d, floa
   if (p.lse != nullptr && d == 0) p.lse[row] = l == 0.f ? -INFINITY : (m - BIAS + log2f(l)) * 0.69314718055994531f;
 }
 
+// A run of units of one segment, as a warp walks it.
+struct Walk {
+  uint32_t u, seg1;   // the round it stands at, and where its segment ends (both in the run's numbering)
+  int e, h;           // entry and key head
+  int b, keys;        // request, keys that the segment reads
+  uint32_t seg0;
+};
+
+// NB scales of a row as bfloat16 bits.
+template <int NB>
+__device__ __forceinline__ void load_scales(const void *base, int64_t at, bool e8m0, bool vec, uint32_t (&raw)[(NB + 1) / 2]) {
+  if constexpr (NB == 1) {
+    raw[0] = e8m0 ? ((const uint8_t *)base)[at] : ((const uint16_t *)base)[at];
+  } else {
+    if (vec && !e8m0) {
+#pragma unroll
+      for (int i = 0; i < NB / 2; ++i) raw[i] = 0;
+      if constexpr (NB == 2) raw[0] = *(const uint32_t *)((const uint16_t *)base + at);
+      if constexpr (NB == 4) {
+        const uint2 x = *(const uint2 *)((const uint16_t *)base + at);
+        raw[0] = x.x, raw[1] = x.y;
+      }
+      if constexpr (NB == 8) {
+        const uint4 x = *(const uint4 *)((const uint16_t *)base + at);
+        raw[0] = x.x, raw[1] = x.y, raw[2] = x.z, raw[3] = x.w;
+      }
+    } else if (vec) {  // bytes, left as they are: scale_at() widens them
+      if constexpr (NB == 2) raw[0] = *(const uint16_t *)((const uint8_t *)base + at);
+      if constexpr (NB == 4) raw[0] = *(const uint32_t *)((const uint8_t *)base + at);
+      if constexpr (NB == 8) {
+        const uint2 x = *(const uint2 *)((const uint8_t *)base + at);
+        raw[0] = x.x, raw[1] = x.y;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < (NB + 1) / 2; ++i) raw[i] = 0;
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        if (e8m0) raw[i / 4] |= (uint32_t)((const uint8_t *)base)[at + i] << (8 * (i % 4));
+        else raw[i / 2] |= (uint32_t)((const uint16_t *)base)[at + i] << (16 * (i % 2));
+      }
+    }
+  }
+}
+// Scale i of load_scales' words as bfloat16 bits.
+template <int NB>
+__device__ __forceinline__ uint32_t scale_at(const uint32_t (&raw)[(NB + 1) / 2], int i, bool e8m0) {
+  if (e8m0) {
+    const uint32_t b = NB == 1 ? raw[0] : (raw[i / 4] >> (8 * (i % 4))) & 0xFFu;
+    return b == 0 ? 0x40u : b == 255 ? 0x7FC0u : b << 7;
+  }
+  return NB == 1 ? raw[0] : (raw[i / 2] >> (16 * (i % 2))) & 0xFFFFu;
+}
+
 template <typename T, int F, int D, int NT, bool BLK>
-__global__ void __launch_bounds__(THREADS, D == 256 || NT == 2 ? 1 : 2) attn_kernel(const Params p) {
-  using C = Cfg<F, D, NT>;
-  extern __shared__ __align__(16) uint8_t smem[];
-  uint32_t *qf = (uint32_t *)smem;
-  float *join_o = (float *)(smem + C::Q_BYTES);
-  float *join_m = (float *)(smem + C::Q_BYTES + C::JOIN_BYTES), *join_l = join_m + WARPS * C::ROWS;
-  float *qs_s = join_l + WARPS * C::ROWS;  // [ROWS] multiplier of a row's scores
-  int *lim_s = (int *)(qs_s + C::ROWS);    // [ROWS] keys that a row sees
-  __shared__ uint32_t prefix[MAX_ENTRIES + 1];
-  __shared__ uint32_t scan[WARPS];
+__global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel(const Params p) {
+  using C = Cfg<F, D, NT, BLK>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint32_t prefix[MAX_ENTRIES + 1];  // rounds of a key head before each entry
+  __shared__ uint32_t scan[2 * WARPS];
   __shared__ uint32_t last;
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int entries = p.batch * p.row_tiles;
-  constexpr int UNIT = 16 * C::M2;
+  uint8_t *ring = smem + warp * STAGES * C::STAGE;
+  uint8_t *slots = smem + WARPS * STAGES * C::STAGE + warp * STAGES * C::SLOT;
+  float *join_o = (float *)(smem + WARPS * STAGES * (C::STAGE + C::SLOT));
+  float *join_m = join_o + WARPS * C::ROWS * C::ORS, *join_l = join_m + WARPS * C::ROWS;
+  const int entries = p.batch * p.row_tiles, heads = p.kv_heads;
+  constexpr uint32_t ROUND = C::T * WARPS;
   const int64_t cap = (int64_t)p.max_pages << p.page_shift;
+  const bool split = p.ws_o != nullptr;
 
-  auto length_of = [&](int b) -> int64_t {
+  auto length_of = [&](int b) -> int {
     const int64_t n = p.lengths != nullptr ? p.lengths[b] : p.fixed;
-    return n < 0 ? 0 : n > cap ? cap : n;
+    return (int)(n < 0 ? 0 : n > cap ? cap : n);
   };
   // keys that the last row of an entry's tile sees
-  auto keys_of = [&](int e) -> int64_t {
-    const int b = e / p.row_tiles, rt = e - b * p.row_tiles;
-    const int64_t n = length_of(b);
-    if (!p.causal) return n;
-    const int r1 = min(p.rows, (rt + 1) * C::ROWS) - 1;
-    const int64_t lim = n - p.queries + r1 / p.group + 1;
-    return lim < 0 ? 0 : lim;
+  auto keys_of = [&](int e) -> int {
+    const int b = p.row_tiles == 1 ? e : e / p.row_tiles;
+    const int n = length_of(b);
+    if (!p.causal || p.queries == 1) return n;
+    const int r1 = min(p.rows, (e - b * p.row_tiles + 1) * C::ROWS) - 1;
+    return max(0, n - p.queries + r1 / p.group + 1);
   };
+  auto rounds_of = [&](int keys) -> uint32_t { return ((uint32_t)keys + ROUND - 1) / ROUND; };
+  auto aligned = [&](uint32_t r) -> uint32_t { return (r + SHORT - 1) / SHORT * SHORT; };
 
-  // units of the entries, summed up
+  // rounds of the entries, summed up: as they are, and with segments padded to SHORT
+  uint32_t per;
+  bool pad;
   {
-    const int per = (entries + THREADS - 1) / THREADS, e0 = tid * per;
-    uint32_t sum = 0;
-    for (int i = 0; i < per; ++i)
-      if (e0 + i < entries) sum += (uint32_t)((keys_of(e0 + i) + UNIT - 1) / UNIT);
-    uint32_t inc = sum;
+    const int each = (entries + THREADS - 1) / THREADS, e0 = tid * each;
+    uint32_t sum = 0, psum = 0;
+    for (int i = 0; i < each; ++i)
+      if (e0 + i < entries) {
+        const uint32_t r = rounds_of(keys_of(e0 + i));
+        prefix[e0 + i] = r;
+        sum += r, psum += aligned(r);
+      }
+    uint32_t inc = sum, pinc = psum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
-      if (lane >= o) inc += v;
+      const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, inc, o), w = __shfl_up_sync(0xFFFFFFFFu, pinc, o);
+      if (lane >= o) inc += v, pinc += w;
     }
-    if (lane == 31) scan[warp] = inc;
+    if (lane == 31) scan[warp] = inc, scan[WARPS + warp] = pinc;
     __syncthreads();
-    uint32_t base = 0;
-    for (int w = 0; w < warp; ++w) base += scan[w];
-    uint32_t run = base + inc - sum;
-    for (int i = 0; i < per; ++i)
+    uint32_t base = 0, pbase = 0, total = 0, ptotal = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      if (w < warp) base += scan[w], pbase += scan[WARPS + w];
+      total += scan[w], ptotal += scan[WARPS + w];
+    }
+    per = (uint32_t)(((uint64_t)total * heads + gridDim.x - 1) / gridDim.x);
+    pad = split && per <= 1;
+    if (pad) per = aligned((uint32_t)(((uint64_t)ptotal * heads + gridDim.x - 1) / gridDim.x));
+    if (per == 0) per = 1;
+    uint32_t run = pad ? pbase + pinc - psum : base + inc - sum;
+    for (int i = 0; i < each; ++i)
       if (e0 + i < entries) {
+        const uint32_t r = prefix[e0 + i];
         prefix[e0 + i] = run;
-        run += (uint32_t)((keys_of(e0 + i) + UNIT - 1) / UNIT);
+        run += pad ? aligned(r) : r;
         if (e0 + i == entries - 1) prefix[entries] = run;
       }
     __syncthreads();
   }
-  const int heads = p.kv_heads;
-  const int64_t total = (int64_t)prefix[entries] * heads;
+  const uint32_t total = prefix[entries] * (uint32_t)heads;
 
   // rows without a key: zeros (or what the prefix gave)
   for (int e = blockIdx.x; e < entries; e += gridDim.x) {
@@ -357,73 +364,225 @@ __global__ void __launch_bounds__(THREADS, D == 256 || NT == 2 ? 1 : 2) attn_ker
     }
   }
 
-  // this CTA's run of units; without a workspace, whole segments in turn
-  const bool split = p.ws_o != nullptr;
-  int64_t per = (total + gridDim.x - 1) / gridDim.x;
-  if (per < 2 * WARPS) per = 2 * WARPS;
-  int64_t u = split ? (int64_t)blockIdx.x * per : 0;
-  const int64_t u_end = split ? min(total, u + per) : total;
-  int64_t skip = split ? 0 : blockIdx.x;  // segments to pass over
-  int e = 0;
-  while (u < u_end) {
-    {  // the entry of unit u
-      int lo = 0, hi = entries;
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if ((int64_t)prefix[mid] * heads <= u) lo = mid;
-        else hi = mid;
+  // this CTA's run of rounds; without a workspace, whole segments in turn
+  const uint32_t u0 = split ? min(total, blockIdx.x * per) : 0, u_end = split ? min(total, u0 + per) : total;
+
+  auto enter = [&](Walk &w) {  // reads the segment that w.e, w.h name
+    const uint32_t n = prefix[w.e + 1] - prefix[w.e];
+    w.seg0 = prefix[w.e] * heads + w.h * n;
+    w.seg1 = w.seg0 + n;
+    w.b = p.row_tiles == 1 ? w.e : w.e / p.row_tiles;
+    w.keys = keys_of(w.e);
+  };
+  auto next_segment = [&](Walk &w) {  // w.u stands at its end
+    do {
+      w.u = w.seg1;
+      if (w.u >= u_end) return;
+      if (++w.h == heads) {
+        w.h = 0;
+        do ++w.e;
+        while (prefix[w.e + 1] == prefix[w.e]);
       }
-      e = lo;
+      enter(w);
+    } while (!split && (w.e * (uint32_t)heads + w.h) % gridDim.x != blockIdx.x);
+  };
+  Walk c;
+  c.u = u0, c.e = 0, c.h = 0;
+  if (u0 < u_end) {
+    int lo = 0, hi = entries;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (prefix[mid] * heads <= u0) lo = mid;
+      else hi = mid;
     }
-    const int units = (int)(prefix[e + 1] - prefix[e]);
-    const int64_t first = (int64_t)prefix[e] * heads;
-    const int h = (int)((u - first) / units);
-    const int64_t seg0 = first + (int64_t)h * units, seg1 = seg0 + units;
-    if (skip > 0) {
-      --skip;
-      u = seg1;
+    c.e = lo;
+    c.h = (int)((u0 - prefix[lo] * heads) / (prefix[lo + 1] - prefix[lo]));
+    enter(c);
+    if (!split && (c.e * (uint32_t)heads + c.h) % gridDim.x != blockIdx.x) next_segment(c);
+  }
+
+  // ---- what is on its way: pages of one unit, scales of the one before, codes of the one before that
+  constexpr int BPU = C::T / 16;                 // blocks of 16 keys in a unit
+  constexpr int KPL = (C::T + 31) / 32;          // keys of a lane
+  constexpr int SW = (C::KNB + 1) / 2;
+  Walk a = c;                                    // the unit whose pages are being read
+  int32_t page[BPU];
+  int64_t code[BPU];                             // of the unit whose scales are being read
+  int left = 0;                                  // its keys, none if there is no such unit
+  uint32_t bad = 0;                              // its blocks on pages outside the cache
+  uint32_t rk[KPL][SW], rv[KPL][SW];
+  const int page_blocks = p.page_shift - 4;
+
+  auto read_pages = [&]() {
+    if (a.u >= u_end) return;
+    const int first = ((int)(a.u - a.seg0) * WARPS + warp) * BPU;
+    const int32_t *table = p.tables + a.b * p.table_stride;
+#pragma unroll
+    for (int j = 0; j < BPU; ++j)
+      page[j] = (first + j) * 16 < a.keys ? __ldg(table + ((first + j) >> page_blocks)) : 0;
+  };
+  auto read_scales = [&]() {  // of a's unit, whose pages are here; then a moves on and its next pages are asked for
+    left = 0, bad = 0;
+    if (a.u >= u_end) return;
+    const int first = (int)(a.u - a.seg0) * WARPS + warp;
+    left = a.keys - first * C::T;
+    int64_t at[BPU];
+#pragma unroll
+    for (int j = 0; j < BPU; ++j) {
+      const bool in = 16 * j < left;
+      const bool ok = (uint32_t)page[j] < (uint64_t)p.pages;
+      if (in && !ok) {
+        bad |= 1u << j;
+        if (lane == 0) atomicOr(&g_device_error, DEVERR_BAD_INDEX);
+      }
+      const int64_t pg = in && ok ? page[j] : 0;
+      const int64_t off = (int64_t)((first * BPU + j) & ((1 << page_blocks) - 1)) << 4;
+      code[j] = pg * p.cp + a.h * p.ch + off * p.ct;
+      at[j] = pg * p.sp + a.h * p.sh + off * p.st;
+    }
+#pragma unroll
+    for (int k = 0; k < KPL; ++k) {
+      const int key = lane + 32 * k, j = key >> 4;
+      int64_t row = at[0];
+#pragma unroll
+      for (int i = 1; i < BPU; ++i)
+        if (j == i) row = at[i];
+      row += (key & 15) * p.st;
+      if (key < C::T && key < left && !((bad >> j) & 1)) {
+        load_scales<C::KNB>(p.ks, row, p.e8m0, p.scale_vec, rk[k]);
+        load_scales<C::KNB>(p.vs, row, p.e8m0, p.scale_vec, rv[k]);
+      }
+    }
+    if (++a.u == a.seg1) next_segment(a);
+    read_pages();
+  };
+  // the codes of the unit whose scales were read last, and those scales, into stage s
+  auto fill = [&](int s) {
+    if (left > 0) {
+      const uint32_t kd = smem_u32(ring + s * C::STAGE), vd = kd + C::T * C::RB;
+      const int lr = lane / C::CPR, lc = lane % C::CPR;
+#pragma unroll
+      for (int i = 0; i < C::T / C::RPI; ++i) {
+        const int row = lr + i * C::RPI, j = (i * C::RPI) >> 4;
+        const bool in = row < left && !((bad >> j) & 1);
+        const int64_t src = code[j] + (int64_t)(row & 15) * p.ct + lc * 16;
+        cp_async16(kd + C::chunk(row, lc), p.k + src, in);
+        cp_async16(vd + C::chunk(row, lc), p.v + src, in);
+      }
+      float2 *lvi = (float2 *)(slots + s * C::SLOT);
+      float *ks = (float *)(slots + s * C::SLOT + C::LVI);
+      __half *vr = (__half *)(slots + s * C::SLOT + C::LVI + C::KSB);
+#pragma unroll
+      for (int k = 0; k < KPL; ++k) {
+        const int key = lane + 32 * k;
+        if (C::T < 32 && key >= C::T) continue;
+        const bool in = key < left && !((bad >> (key >> 4)) & 1);
+        if constexpr (!BLK) {
+          float vsc = __uint_as_float(scale_at<1>(rv[k], 0, p.e8m0) << 16);
+          vsc = vsc < 0x1p-120f ? 0x1p-120f : vsc;  // a scale of zero: weight without a value
+          lvi[key] = in ? make_float2(lg2(vsc), __frcp_rn(vsc)) : make_float2(-INFINITY, 0.f);
+          ks[key] = in ? __uint_as_float(scale_at<1>(rk[k], 0, p.e8m0) << 16) : 0.f;
+        } else {
+          uint32_t top = 0, vb[C::NB];
+          float kb[C::NB];
+#pragma unroll
+          for (int i = 0; i < C::NB; ++i) {
+            vb[i] = scale_at<C::NB>(rv[k], i, p.e8m0);
+            kb[i] = in ? __uint_as_float(scale_at<C::NB>(rk[k], i, p.e8m0) << 16) : 0.f;
+            top = max(top, vb[i]);
+          }
+          const int e = RowRef<F>::exponent(top);
+          const bool nan = top > 0x7F80u;  // the row's NaN travels in its denominator, which only rows that see it take
+          lvi[key] = in ? make_float2((float)(e - 127), nan ? __uint_as_float(0x7FC00000u) : RowRef<F>::inverse(e))
+                        : make_float2(-INFINITY, 0.f);
+#pragma unroll
+          for (int i = 0; i < C::NB; ++i) {
+            ks[key * C::NB + i] = kb[i];
+            // ratios in the order of the instruction's rows
+            vr[i * C::T + (key & ~7) + C::row_of(key & 7)] =
+                __float2half_rn(in && vb[i] <= 0x7F80u && !nan ? __uint_as_float(vb[i] << 16) * RowRef<F>::inverse(e) : 0.f);
+          }
+        }
+      }
+    }
+    cp_async_commit();
+  };
+
+  read_pages();
+#pragma unroll
+  for (int s = 0; s < STAGES; ++s) {
+    read_scales();
+    fill(s);
+  }
+  read_scales();
+  int stage = 0;
+
+  while (c.u < u_end) {
+    const uint32_t real = rounds_of(c.keys), from = c.u - c.seg0, to = min(u_end, c.seg1) - c.seg0;
+    const uint32_t upto = min(to, real);
+    if (from >= real) {  // padding alone: the ring goes on
+      for (uint32_t i = from; i < to; ++i) {
+        fill(stage);
+        read_scales();
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
+      }
+      c.u = c.seg0 + to;
+      if (c.u == c.seg1) next_segment(c);
       continue;
     }
-    if (!split) skip = gridDim.x - 1;
-    const int b = e / p.row_tiles, rt = e - b * p.row_tiles, r0 = rt * C::ROWS;
-    const int from = (int)(u - seg0), to = (int)(min(u_end, seg1) - seg0);
-    const int n_rows = min(C::ROWS, p.rows - r0);
-    const int64_t len = length_of(b), keys = keys_of(e);
+    const int rt = c.e - c.b * p.row_tiles, r0 = rt * C::ROWS, n_rows = min(C::ROWS, p.rows - r0);
+    const int len = length_of(c.b);
 
-    // q: fp16, each row scaled by a power of two, in the order of the keys' fragments
-    __syncthreads();
-    for (int n = warp; n < C::ROWS; n += WARPS) {
-      constexpr int E = D / 32;
-      float x[E], top = 0.f;
-      bool bad = false;
-      const bool in = n < n_rows;
-      const T *src = in ? (const T *)p.q + row_at(p, b, h, r0 + n).q : nullptr;
-#pragma unroll
-      for (int i = 0; i < E; ++i) {
-        x[i] = in ? to_f32<T>(src[i * 32 + lane]) : 0.f;
-        top = fmaxf(top, fabsf(x[i]));
-        bad |= x[i] != x[i];
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-      const int ex = min(max((int)(__float_as_uint(top) >> 23), 1), 253);
-      const float down = __uint_as_float((uint32_t)(254 - ex) << 23);
-#pragma unroll
-      for (int i = 0; i < E; ++i) ((__half *)qf)[q_index<F, D, NT>(n, i * 32 + lane)] = __float2half_rn(x[i] * down);
-      if (lane == 0) {
-        qs_s[n] = p.scale * __uint_as_float((uint32_t)ex << 23);
-        const int64_t lim = !p.causal ? len : len - p.queries + (r0 + n) / p.group + 1;
-        lim_s[n] = in ? (int)max((int64_t)0, lim) : 0;
-      }
-    }
-    __syncthreads();
-
+    // q as the second operand: fp16, each row scaled by a power of two, lane (g, t) of tile n holding
+    // values 8t .. 8t + 7 of every block of 32 of row 8n + g, paired as the codes come out decoded
+    uint32_t q[NT][C::NB][4];
     float qs[NT][2];
     int lim[NT][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n) {
+      const int r = n * 8 + g;
+      const bool in = r < n_rows;
+      const T *src = in ? (const T *)p.q + row_at(p, c.b, c.h, r0 + r).q + 8 * t : nullptr;
+      uint32_t raw[C::NB][4];
+      float top = 0.f;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) qs[n][c] = qs_s[n * 8 + 2 * t + c], lim[n][c] = lim_s[n * 8 + 2 * t + c];
+      for (int b = 0; b < C::NB; ++b) {
+        if (in && p.q_vec) lds<16>((const uint8_t *)(src + 32 * b), raw[b]);
+        else if (in)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            raw[b][i] = (uint32_t)*(const uint16_t *)(src + 32 * b + 2 * i) | ((uint32_t)*(const uint16_t *)(src + 32 * b + 2 * i + 1) << 16);
+        else raw[b][0] = raw[b][1] = raw[b][2] = raw[b][3] = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const T *v = reinterpret_cast<const T *>(&raw[b][i]);
+          top = fmaxf(top, fmaxf(fabsf(to_f32(v[0])), fabsf(to_f32(v[1]))));
+        }
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+      const int ex = min(max((int)(__float_as_uint(top) >> 23), 1), 253);
+      const float down = __uint_as_float((uint32_t)(254 - ex) << 23);
+#pragma unroll
+      for (int b = 0; b < C::NB; ++b) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const T *v = reinterpret_cast<const T *>(&raw[b][i]);
+          x[2 * i] = to_f32(v[0]) * down, x[2 * i + 1] = to_f32(v[1]) * down;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          q[n][b][i] = F == B200_CACHE_INT4 ? pack_f16(x[i], x[i + 4]) : pack_f16(x[2 * i], x[2 * i + 1]);
+      }
+      const float mine = p.scale * __uint_as_float((uint32_t)ex << 23);
+#pragma unroll
+      for (int col = 0; col < 2; ++col) {
+        qs[n][col] = __shfl_sync(0xFFFFFFFFu, mine, (2 * t + col) * 4);
+        const int rc = n * 8 + 2 * t + col;
+        lim[n][col] = rc >= n_rows ? 0 : p.causal ? len - p.queries + (r0 + rc) / p.group + 1 : len;
+      }
+    }
 
     float o[NT][C::MT][4], m[NT][2], l[NT][2];
 #pragma unroll
@@ -432,200 +591,133 @@ __global__ void __launch_bounds__(THREADS, D == 256 || NT == 2 ? 1 : 2) attn_ker
 #pragma unroll
       for (int i = 0; i < C::MT; ++i)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) o[n][i][c] = 0.f;
+        for (int x = 0; x < 4; ++x) o[n][i][x] = 0.f;
     }
 
-    const int32_t *table = p.tables + (int64_t)b * p.table_stride;
-    const int page_blocks = p.page_shift - 4;  // blocks of 16 keys of a page, as a shift
-    // where block blk (16 keys) is in the cache, and how many of its keys there are
-    auto locate = [&](int blk, At &at, int &valid) {
-      const int64_t left = keys - (int64_t)blk * 16;
-      valid = left > 16 ? 16 : left < 0 ? 0 : (int)left;
-      at = {0, 0};
-      if (valid > 0) {
-        const int32_t page = __ldg(table + (blk >> page_blocks));
-        if (page < 0 || page >= p.pages) {
-          if (lane == 0) atomicOr(&g_device_error, DEVERR_BAD_INDEX);
-          valid = 0;
-        } else {
-          const int64_t offset = (int64_t)(blk & ((1 << page_blocks) - 1)) << 4;
-          at = {page * p.cp + h * p.ch + offset * p.ct, page * p.sp + h * p.sh + offset * p.st};
-        }
-      }
-    };
-
-    Keys<F, D, NT, BLK> x[C::M2];
-    At row[C::M2];
-    int valid[C::M2], unit = from + warp;
-    if (unit < to) {
-#pragma unroll
-      for (int j = 0; j < C::M2; ++j) {
-        locate(unit * C::M2 + j, row[j], valid[j]);
-        load_k<F, D, NT, BLK>(x[j], p, row[j], valid[j], g, t);
-      }
-#pragma unroll
-      for (int j = 0; j < C::M2; ++j) load_v<F, D, NT, BLK>(x[j], p, row[j], valid[j], g, t);
-    }
-    for (; unit < to; unit += WARPS) {
-      float s[C::M2][NT][4], iv[C::M2][2], lv[C::M2][2];
-      int ve[C::M2][2], seen[C::M2];
-#pragma unroll
-      for (int j = 0; j < C::M2; ++j) {
-        seen[j] = valid[j];
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) s[j][n][c] = 0.f;
-        float krow[2];
-        uint32_t kr[2][BLK ? C::KCH : 1];
-        if constexpr (BLK) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            uint32_t pk = x[j].kt[i] | (x[j].vs[i] << 16);
-#pragma unroll
-            for (int q = 1; q < 4; q <<= 1) {
-              const uint32_t other = __shfl_xor_sync(0xFFFFFFFFu, pk, q);
-              asm("max.u16x2 %0, %0, %1;" : "+r"(pk) : "r"(other));
-            }
-            const uint32_t kt = pk & 0xFFFFu, vt = pk >> 16;
-            const int ke = RowRef<F>::exponent(kt);
-            ve[j][i] = RowRef<F>::exponent(vt);
-            // a NaN scale makes the whole row NaN
-            krow[i] = kt > 0x7F80u ? __uint_as_float(0x7FC00000u) : RowRef<F>::value(ke);
-            iv[j][i] = vt > 0x7F80u ? __uint_as_float(0x7FC00000u) : RowRef<F>::inverse(ve[j][i]);
-            lv[j][i] = (float)(ve[j][i] - 127);
-#pragma unroll
-            for (int c = 0; c < C::KCH; ++c) {
-              const float r = __uint_as_float(x[j].ks[i][c] << 16) * RowRef<F>::inverse(ke);
-              kr[i][c] = pack_f16(r, r);
-            }
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            krow[i] = __uint_as_float(x[j].ks[i][0] << 16);
-            float vsc = __uint_as_float(x[j].vs[i] << 16);
-            vsc = vsc < 0x1p-120f ? 0x1p-120f : vsc;  // a scale of zero: weight without a value
-            iv[j][i] = 1.f / vsc;
-            lv[j][i] = lg2(vsc);
-          }
-        }
+    for (uint32_t round = from; round < to; ++round) {
+      const int first = ((int)round * WARPS + warp) * C::T;  // the unit's first key
+      cp_async_wait<STAGES - 1>();
+      __syncwarp();
+      const uint8_t *kt = ring + stage * C::STAGE, *vt = kt + C::T * C::RB;
+      const float2 *lvi_s = (const float2 *)(slots + stage * C::SLOT);
+      const float *ks_s = (const float *)(slots + stage * C::SLOT + C::LVI);
+      const uint8_t *vr_s = slots + stage * C::SLOT + C::LVI + C::KSB;
+#pragma unroll 1
+      for (int sb = 0; sb < C::T && first + sb < c.keys; sb += 16) {
+        const int k0 = sb + C::key_of(g), k1 = k0 + 8;  // this lane's two keys
         // s^T = K q^T
-#pragma unroll
-        for (int c = 0; c < C::KCH; ++c)
-#pragma unroll
-          for (int w = 0; w < C::KCW; ++w) {
-            constexpr int STEPS = C::bits == 8 ? 1 : 2;
-            uint32_t a[2][4];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const uint32_t word = x[j].k[i][c * C::KCW + w];
-              if constexpr (C::bits == 8) decode4_8bit<F>(word, a[i][0], a[i][1]);
-              else decode8_4<F>(word, a[i]);
-              if constexpr (BLK)
-#pragma unroll
-                for (int y = 0; y < 2 * STEPS; ++y) a[i][y] = hmul2(a[i][y], kr[i][c]);
-            }
-#pragma unroll
-            for (int st = 0; st < STEPS; ++st) {
-              const uint32_t frag[4] = {a[0][2 * st], a[1][2 * st], a[0][2 * st + 1], a[1][2 * st + 1]};
-#pragma unroll
-              for (int n = 0; n < NT; ++n) {
-                const uint2 bq = *reinterpret_cast<const uint2 *>(
-                    &qf[((n * C::KS + c * (C::KEC / 4) + w * STEPS + st) * 32 + lane) * 2]);
-                gemv::mma16816(s[j][n], frag, bq.x, bq.y);
-              }
-            }
-          }
+        float s[NT][4], s2[NT][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) s[j][n][c] *= krow[c >> 1];
-      }
-      // the next keys: their registers are free
-      const int next = unit + WARPS;
-      At nrow[C::M2];
-      int nvalid[C::M2];
-      if (next < to) {
+          for (int x = 0; x < 4; ++x) s[n][x] = 0.f, s2[n][x] = 0.f;
 #pragma unroll
-        for (int j = 0; j < C::M2; ++j) {
-          locate(next * C::M2 + j, nrow[j], nvalid[j]);
-          load_k<F, D, NT, BLK>(x[j], p, nrow[j], nvalid[j], g, t);
+        for (int b = 0; b < C::NB; ++b) {
+          uint32_t f[2][4];  // [key][pairs of two k steps]
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int row = i ? k1 : k0;
+            if constexpr (C::bits == 8) {
+              uint32_t w[2];
+              lds<8>(kt + C::chunk(row, 2 * b + (t >> 1)) + 8 * (t & 1), w);
+              decode4_8bit<F>(w[0], f[i][0], f[i][1]);
+              decode4_8bit<F>(w[1], f[i][2], f[i][3]);
+            } else {
+              uint32_t w[1];
+              lds<4>(kt + C::chunk(row, b) + 4 * t, w);
+              decode8_4<F>(w[0], f[i]);
+            }
+          }
+          const uint32_t f0[4] = {f[0][0], f[1][0], f[0][1], f[1][1]}, f1[4] = {f[0][2], f[1][2], f[0][3], f[1][3]};
+          if constexpr (BLK) {
+            const float sk0 = ks_s[k0 * C::NB + b], sk1 = ks_s[k1 * C::NB + b];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              float y[4] = {0.f, 0.f, 0.f, 0.f};
+              gemv::mma16816(y, f0, q[n][b][0], q[n][b][1]);
+              gemv::mma16816(y, f1, q[n][b][2], q[n][b][3]);
+              s[n][0] = fmaf(y[0], sk0, s[n][0]), s[n][1] = fmaf(y[1], sk0, s[n][1]);
+              s[n][2] = fmaf(y[2], sk1, s[n][2]), s[n][3] = fmaf(y[3], sk1, s[n][3]);
+            }
+          } else {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              gemv::mma16816(s[n], f0, q[n][b][0], q[n][b][1]);
+              gemv::mma16816(s2[n], f1, q[n][b][2], q[n][b][3]);
+            }
+          }
         }
-      }
-      // u = s + log2 vs; keys that a row does not see: -inf
-      bool up = false;
+        const float2 lvi0 = lvi_s[k0], lvi1 = lvi_s[k1];
+        float ks0 = 1.f, ks1 = 1.f;
+        if constexpr (!BLK) ks0 = ks_s[k0], ks1 = ks_s[k1];
+        // u = s + log2 vs: -inf for keys that are not there
+        bool up = false;
 #pragma unroll
-      for (int j = 0; j < C::M2; ++j) {
-        const int tok = 4 * (g >> 1) + (g & 1), base = (unit * C::M2 + j) * 16 + tok;
+        for (int n = 0; n < NT; ++n) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int i = c >> 1, col = c & 1;
-            const bool in = tok + 2 * i < seen[j] && base + 2 * i < lim[n][col];
-            s[j][n][c] = in ? fmaf(s[j][n][c], qs[n][col], lv[j][i]) : -INFINITY;
-            up |= s[j][n][c] > m[n][col] + LAZY;
+          for (int x = 0; x < 4; ++x) {
+            const float y = BLK ? s[n][x] : (s[n][x] + s2[n][x]) * (x < 2 ? ks0 : ks1);
+            s[n][x] = fmaf(y, qs[n][x & 1], x < 2 ? lvi0.x : lvi1.x);
           }
-      }
-      if (__any_sync(0xFFFFFFFFu, up)) {
+          if (p.causal && p.queries > 1) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int col = 0; col < 2; ++col) {
-            float top = m[n][col];
-#pragma unroll
-            for (int j = 0; j < C::M2; ++j) top = fmaxf(top, fmaxf(s[j][n][col], s[j][n][col + 2]));
-#pragma unroll
-            for (int q = 4; q < 32; q <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, q));
-            const float f = m[n][col] == -INFINITY ? 0.f : ex2(m[n][col] - top);
-            m[n][col] = top;
-            l[n][col] *= f;
-#pragma unroll
-            for (int i = 0; i < C::MT; ++i) o[n][i][col] *= f, o[n][i][col + 2] *= f;
+            for (int x = 0; x < 4; ++x)
+              if (first + (x < 2 ? k0 : k1) >= lim[n][x & 1]) s[n][x] = -INFINITY;
           }
-      }
+          up |= fmaxf(s[n][0], s[n][2]) > m[n][0] + LAZY || fmaxf(s[n][1], s[n][3]) > m[n][1] + LAZY;
+        }
+        if (__any_sync(0xFFFFFFFFu, up)) {
 #pragma unroll
-      for (int j = 0; j < C::M2; ++j) {
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int col = 0; col < 2; ++col) {
+              float top = fmaxf(m[n][col], fmaxf(s[n][col], s[n][col + 2]));
+#pragma unroll
+              for (int y = 4; y < 32; y <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, y));
+              const float f = m[n][col] == -INFINITY ? 0.f : ex2(m[n][col] - top);
+              m[n][col] = top;
+              l[n][col] *= f;
+#pragma unroll
+              for (int i = 0; i < C::MT; ++i) o[n][i][col] *= f, o[n][i][col + 2] *= f;
+            }
+        }
         uint32_t bp[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           float pr[4];
+          const float m0 = m[n][0] == -INFINITY ? 0.f : m[n][0] - BIAS, m1 = m[n][1] == -INFINITY ? 0.f : m[n][1] - BIAS;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const float mm = m[n][c & 1] == -INFINITY ? 0.f : m[n][c & 1] - BIAS;
-            pr[c] = ex2(s[j][n][c] - mm);
-            if (pr[c] != 0.f) l[n][c & 1] = fmaf(pr[c], iv[j][c >> 1], l[n][c & 1]);  // an unseen key's scale may be NaN
+          for (int x = 0; x < 4; ++x) {
+            pr[x] = ex2(s[n][x] - (x & 1 ? m1 : m0));
+            // an unseen key's scale may be NaN
+            if (pr[x] != 0.f) l[n][x & 1] = fmaf(pr[x], x < 2 ? lvi0.y : lvi1.y, l[n][x & 1]);
           }
           bp[n][0] = movmatrix_trans(pack_f16(pr[0], pr[1]));
           bp[n][1] = movmatrix_trans(pack_f16(pr[2], pr[3]));
         }
-        uint32_t vr[2][BLK ? C::VCH : 1];  // scales of this lane's block of values, tokens in pairs
-        if constexpr (BLK) {
-          // keys 4t .. 4t + 3 are rows 2t, 2t + 1 of the scores: key 4t + i sits in lane 8t + 4 (i & 1)
-          float inv[4];
+        // out^T += V^T p^T: rows 2t, 2t + 1 (and + 8) of the scores are this lane's four keys
+        const int kv[2] = {sb + C::key_of(2 * t), sb + C::key_of(2 * t + 1)};
+#pragma unroll
+        for (int ch = 0; ch < C::VCH; ++ch) {
+          uint32_t w[4][C::VCW];  // keys kv[0], kv[1], kv[0] + 8, kv[1] + 8
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int ex = __shfl_sync(0xFFFFFFFFu, ve[j][i >> 1], 8 * t + 4 * (i & 1) + t);
-            inv[i] = RowRef<F>::inverse(ex);
+            const int row = kv[i & 1] + 8 * (i >> 1);
+            const int at = (g + 8 * ch) * C::VCB;
+            lds<C::VCB>(vt + C::chunk(row, at >> 4) + (at & 15), w[i]);
+          }
+          uint32_t vr[2] = {0, 0};
+          if constexpr (BLK) {
+            const uint8_t *at = vr_s + (((g + 8 * ch) * C::VEC / 32) * C::T + sb + 2 * t) * 2;
+            vr[0] = *(const uint32_t *)at, vr[1] = *(const uint32_t *)(at + 16);
           }
 #pragma unroll
-          for (int c = 0; c < C::VCH; ++c)
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-              vr[i][c] = pack_f16(__uint_as_float(number(x[j].vb[2 * i][c]) << 16) * inv[2 * i],
-                                  __uint_as_float(number(x[j].vb[2 * i + 1][c]) << 16) * inv[2 * i + 1]);
-        }
-        // out^T += V^T p^T
-#pragma unroll
-        for (int c = 0; c < C::VCH; ++c)
-#pragma unroll
-          for (int w = 0; w < C::VCW; ++w) {
+          for (int y = 0; y < C::VCW; ++y) {
             constexpr int DW = 32 / C::bits;  // values of a word
-            uint32_t f[2][DW];                // [tokens (0, 1) or (2, 3)][value]
+            uint32_t f[2][DW];                // [keys of a pair][value]
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              const uint32_t w0 = x[j].v[2 * i][c * C::VCW + w], w1 = x[j].v[2 * i + 1][c * C::VCW + w];
+              const uint32_t w0 = w[2 * i][y], w1 = w[2 * i + 1][y];
               if constexpr (C::bits == 8) {
                 decode4_8bit<F>(__byte_perm(w0, w1, 0x5140), f[i][0], f[i][1]);
                 decode4_8bit<F>(__byte_perm(w0, w1, 0x7362), f[i][2], f[i][3]);
@@ -634,115 +726,122 @@ __global__ void __launch_bounds__(THREADS, D == 256 || NT == 2 ? 1 : 2) attn_ker
                 decode8_4<F>(__byte_perm(w0, w1, 0x5410), lo);
                 decode8_4<F>(__byte_perm(w0, w1, 0x7632), hi);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) f[i][q] = lo[q], f[i][q + 4] = hi[q];
+                for (int x = 0; x < 4; ++x) f[i][x] = lo[x], f[i][x + 4] = hi[x];
               } else {
                 uint32_t ev[4], od[4];
                 decode8_4<F>((w0 & 0x0F0F0F0Fu) | ((w1 << 4) & 0xF0F0F0F0u), ev);
                 decode8_4<F>(((w0 >> 4) & 0x0F0F0F0Fu) | (w1 & 0xF0F0F0F0u), od);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) f[i][2 * q] = ev[q], f[i][2 * q + 1] = od[q];
+                for (int x = 0; x < 4; ++x) f[i][2 * x] = ev[x], f[i][2 * x + 1] = od[x];
               }
               if constexpr (BLK)
 #pragma unroll
-                for (int q = 0; q < DW; ++q) f[i][q] = hmul2(f[i][q], vr[i][c]);
+                for (int x = 0; x < DW; ++x) f[i][x] = hmul2(f[i][x], vr[i]);
             }
 #pragma unroll
-            for (int q = 0; q < DW / 2; ++q) {
-              const uint32_t frag[4] = {f[0][2 * q], f[0][2 * q + 1], f[1][2 * q], f[1][2 * q + 1]};
-              const int mt = (c * C::VCW + w) * (DW / 2) + q;
+            for (int x = 0; x < DW / 2; ++x) {
+              const uint32_t frag[4] = {f[0][2 * x], f[0][2 * x + 1], f[1][2 * x], f[1][2 * x + 1]};
+              const int mt = (ch * C::VCW + y) * (DW / 2) + x;
 #pragma unroll
               for (int n = 0; n < NT; ++n) gemv::mma16816(o[n][mt], frag, bp[n][0], bp[n][1]);
             }
           }
-      }
-      if (next < to) {
-#pragma unroll
-        for (int j = 0; j < C::M2; ++j) {
-          row[j] = nrow[j], valid[j] = nvalid[j];
-          load_v<F, D, NT, BLK>(x[j], p, row[j], valid[j], g, t);
         }
       }
+      __syncwarp();
+      fill(stage);
+      read_scales();
+      stage = stage + 1 == STAGES ? 0 : stage + 1;
     }
 
-    // join the warps: numerators [row][value] of each in shared memory
+    // join the warps, half of each lane's values at a time
+    const bool whole = from == 0 && upto == real;
+    const uint32_t c0 = split ? c.seg0 / per : 0, c1 = split ? (c.seg0 + real - 1) / per : 0;  // CTAs of the segment
+    const int slot = (int)(2 * blockIdx.x + (from == 0 ? 1 : 0));
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int col = 0; col < 2; ++col) {
 #pragma unroll
-        for (int q = 4; q < 32; q <<= 1) l[n][col] += __shfl_xor_sync(0xFFFFFFFFu, l[n][col], q);
+        for (int y = 4; y < 32; y <<= 1) l[n][col] += __shfl_xor_sync(0xFFFFFFFFu, l[n][col], y);
         const int r = n * 8 + 2 * t + col;
         if (g == 0) join_m[warp * C::ROWS + r] = m[n][col], join_l[warp * C::ROWS + r] = l[n][col];
-        float *dst = join_o + (warp * C::ROWS + r) * C::ORS;
+      }
 #pragma unroll
-        for (int i = 0; i < C::MT; ++i) {
-          constexpr int PER = C::VEC / 2;  // tiles of a chunk
-          const int d = (g + 8 * (i / PER)) * C::VEC + 2 * (i % PER);
-          *reinterpret_cast<float2 *>(dst + d) = make_float2(o[n][i][col], o[n][i][col + 2]);
+    for (int half = 0; half < 2; ++half) {
+      // value of the head at place i of a pass: lane g's tiles half * MT / 2 .. + MT / 2
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int col = 0; col < 2; ++col) {
+          float *dst = join_o + (warp * C::ROWS + n * 8 + 2 * t + col) * C::ORS + g * C::MT;
+#pragma unroll
+          for (int i = 0; i < C::MT / 2; ++i)
+            *reinterpret_cast<float2 *>(dst + 2 * i) =
+                make_float2(o[n][half * (C::MT / 2) + i][col], o[n][half * (C::MT / 2) + i][col + 2]);
+        }
+      __syncthreads();
+      for (int i = tid; i < C::ROWS * (C::HALF / 4); i += THREADS) {
+        const int r = i / (C::HALF / 4), at = (i % (C::HALF / 4)) * 4;
+        const int gg = at / C::MT, place = half * C::MT + at % C::MT;  // value `place` of lane gg's
+        const int d = (gg + 8 * (place / C::VEC)) * C::VEC + place % C::VEC;
+        float M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) M = fmaxf(M, join_m[w * C::ROWS + r]);
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+          const float mw = join_m[w * C::ROWS + r], f = mw == -INFINITY ? 0.f : ex2(mw - M);
+          const float4 y = *reinterpret_cast<const float4 *>(join_o + (w * C::ROWS + r) * C::ORS + at);
+          x.x += y.x * f, x.y += y.y * f, x.z += y.z * f, x.w += y.w * f;
+          L += join_l[w * C::ROWS + r] * f;  // NaN stays NaN, also where it left m at -inf
+        }
+        if (L != L) x.x = x.y = x.z = x.w = L;
+        if (whole) {
+          if (r < n_rows) finish<T, D>(p, row_at(p, c.b, c.h, r0 + r).out, d, x, M, L);
+        } else {
+          *reinterpret_cast<float4 *>(p.ws_o + ((int64_t)slot * C::ROWS + r) * D + d) = x;
+          if (d == 0) *reinterpret_cast<float2 *>(p.ws_ml + ((int64_t)slot * C::ROWS + r) * 2) = make_float2(M, L);
         }
       }
-    __syncthreads();
-    const bool whole = from == 0 && to == units;
-    const int64_t c0 = seg0 / per, c1 = (seg1 - 1) / per;  // CTAs of the segment
-    const int slot = (int)(2 * blockIdx.x + (from == 0 ? 1 : 0));
-    for (int i = tid; i < C::ROWS * (D / 4); i += THREADS) {
-      const int r = i / (D / 4), d = (i % (D / 4)) * 4;
-      float M = -INFINITY, L = 0.f;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) M = fmaxf(M, join_m[w * C::ROWS + r]);
-      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        const float mw = join_m[w * C::ROWS + r], f = mw == -INFINITY ? 0.f : ex2(mw - M);
-        const float4 y = *reinterpret_cast<const float4 *>(join_o + (w * C::ROWS + r) * C::ORS + d);
-        a.x += y.x * f, a.y += y.y * f, a.z += y.z * f, a.w += y.w * f;
-        L += join_l[w * C::ROWS + r] * f;
-      }
-      // NaN has no order: a warp whose scores are NaN keeps m = -inf but a NaN denominator
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w)
-        if (join_l[w * C::ROWS + r] != join_l[w * C::ROWS + r]) L = a.x = a.y = a.z = a.w = __uint_as_float(0x7FC00000u);
-      if (whole) {
-        if (r < n_rows) finish<T, D>(p, row_at(p, b, h, r0 + r).out, d, a, M, L);
-      } else {
-        *reinterpret_cast<float4 *>(p.ws_o + ((int64_t)slot * C::ROWS + r) * D + d) = a;
-        if (d == 0) *reinterpret_cast<float2 *>(p.ws_ml + ((int64_t)slot * C::ROWS + r) * 2) = make_float2(M, L);
-      }
+      __syncthreads();
     }
     if (!whole) {
       __threadfence();
       __syncthreads();
-      if (tid == 0) last = atomicAdd(&p.tickets[c0], 1u) == (uint32_t)(c1 - c0);
+      if (tid == 0) last = atomicAdd(&p.tickets[c0], 1u) == c1 - c0;
       __syncthreads();
       if (last) {
         __threadfence();
         for (int i = tid; i < n_rows * (D / 4); i += THREADS) {
           const int r = i / (D / 4), d = (i % (D / 4)) * 4;
           float M = -INFINITY, L = 0.f;
-          float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-          bool nan = false;
-          for (int64_t c = c0; c <= c1; ++c) {
-            const int64_t sl = (2 * c + (c == c0 ? 1 : 0)) * C::ROWS + r;
+          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+          for (uint32_t k = c0; k <= c1; ++k) {
+            const int64_t sl = (int64_t)(2 * k + (k == c0 ? 1 : 0)) * C::ROWS + r;
             M = fmaxf(M, __ldcg((const float2 *)(p.ws_ml + sl * 2)).x);
           }
 #pragma unroll 4
-          for (int64_t c = c0; c <= c1; ++c) {
-            const int64_t sl = (2 * c + (c == c0 ? 1 : 0)) * C::ROWS + r;
+          for (uint32_t k = c0; k <= c1; ++k) {
+            const int64_t sl = (int64_t)(2 * k + (k == c0 ? 1 : 0)) * C::ROWS + r;
             const float2 ml = __ldcg((const float2 *)(p.ws_ml + sl * 2));
             const float4 y = __ldcg((const float4 *)(p.ws_o + sl * D + d));
             const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
-            a.x += y.x * f, a.y += y.y * f, a.z += y.z * f, a.w += y.w * f;
+            x.x += y.x * f, x.y += y.y * f, x.z += y.z * f, x.w += y.w * f;
             L += ml.y * f;
-            nan |= ml.y != ml.y;
           }
-          if (nan) L = a.x = a.y = a.z = a.w = __uint_as_float(0x7FC00000u);
-          finish<T, D>(p, row_at(p, b, h, r0 + r).out, d, a, M, L);
+          if (L != L) x.x = x.y = x.z = x.w = L;
+          finish<T, D>(p, row_at(p, c.b, c.h, r0 + r).out, d, x, M, L);
         }
         if (tid == 0) p.tickets[c0] = 0u;  // ready for the next call on this workspace
       }
+      __syncthreads();
     }
-    u = seg0 + to;
+    c.u = c.seg0 + to;
+    if (c.u == c.seg1) next_segment(c);
   }
+  cp_async_wait<0>();
 }
 
 // ---- per-(device, stream) workspace of split segments ---------------------------------------------
@@ -792,11 +891,16 @@ static int32_t workspace_for(cudaStream_t stream, Workspace &out) {
 
 template <typename T, int F, int D, int NT, bool BLK>
 static int32_t launch_t(Params p, cudaStream_t stream) {
-  using C = Cfg<F, D, NT>;
+  using C = Cfg<F, D, NT, BLK>;
   p.row_tiles = (p.rows + C::ROWS - 1) / C::ROWS;
   if (p.row_tiles > MAX_ENTRIES)
     return b200_set_error(B200_ERR_UNSUPPORTED, "cache_attention: too many query rows (%d of a key head)", p.rows);
-  const int at_once = MAX_ENTRIES / p.row_tiles;
+  const int64_t round = C::T * WARPS;
+  const int64_t cap = p.lengths != nullptr ? ((int64_t)p.max_pages << p.page_shift) : p.fixed;
+  const int64_t rounds = ((cap + round - 1) / round + SHORT) * p.kv_heads * p.row_tiles;  // of a request
+  if (rounds > (1 << 29)) return b200_set_error(B200_ERR_UNSUPPORTED, "cache_attention: too many keys for one launch");
+  int at_once = MAX_ENTRIES / p.row_tiles;
+  if (rounds * at_once > (1 << 29)) at_once = (int)((1 << 29) / rounds);
   if (p.batch > at_once) {  // a launch for each run of requests that the scan has room for
     const int all = p.batch;
     const Params base = p;
@@ -818,12 +922,9 @@ static int32_t launch_t(Params p, cudaStream_t stream) {
   if (int32_t rc = workspace_for(stream, w)) return rc;
   p.ws_o = w.o, p.ws_ml = w.ml, p.tickets = w.tickets;
   B200_CUDA_TRY((ensure_dynamic_smem<attn_kernel<T, F, D, NT, BLK>>(C::SMEM)));
-  // no more CTAs than there can be runs of 2 * WARPS units
-  const int64_t unit = 16 * C::M2;
-  const int64_t cap = p.lengths != nullptr ? ((int64_t)p.max_pages << p.page_shift) : p.fixed;
-  const int64_t most = entries * p.kv_heads * ((cap + unit - 1) / unit);
-  int64_t grid = (most + 2 * WARPS - 1) / (2 * WARPS);
-  const int64_t full = (D == 256 || NT == 2) ? w.grid / 2 : w.grid;
+  // no more CTAs than there can be rounds
+  int64_t grid = entries * p.kv_heads * ((cap + round - 1) / round);
+  const int64_t full = (int64_t)w.grid / 2 * C::CTAS;
   if (grid > full) grid = full;
   if (grid < 1) grid = 1;
   cudaLaunchConfig_t cfg = {};
@@ -871,7 +972,10 @@ static int32_t attention(const b200_cache_desc *c, const b200_attention_args *a,
   p.k = (const uint8_t *)c->k, p.v = (const uint8_t *)c->v, p.ks = c->k_scales, p.vs = c->v_scales;
   p.cp = c->strides[0], p.ch = c->strides[1], p.ct = c->strides[2];
   p.sp = c->scale_strides[0], p.sh = c->scale_strides[1], p.st = c->scale_strides[2];
+  p.q_vec = (uintptr_t)p.q % 16 == 0 && p.qsr % 8 == 0 && p.qsb % 8 == 0 && p.qsh % 8 == 0;
   p.e8m0 = c->scale_dtype == B200_DT_E8M0;
+  const int per_row = dim / c->block_size;  // a row's scales as one vector where they are aligned so
+  p.scale_vec = p.sp % per_row == 0 && p.sh % per_row == 0 && p.st % per_row == 0;
   p.pages = c->pages, p.kv_heads = c->kv_heads, p.group = a->heads / c->kv_heads, p.q_heads = a->heads;
   while ((1 << p.page_shift) < c->page_size) ++p.page_shift;
   p.scale = a->scale * 1.44269504088896341f;
@@ -921,8 +1025,8 @@ int32_t b200_cache_attention(const b200_cache_desc *c, const b200_attention_args
       a->prefix_length > a->prefix_pages * c->page_size)
     return b200_set_error(B200_ERR_INVALID, "cache_attention: bad table sizes");
   if (a->batch == 0 || a->queries == 0) return B200_OK;
-  if (a->batch * a->queries * a->heads > INT32_MAX || a->max_pages * c->page_size > INT32_MAX - 64 ||
-      a->prefix_pages * c->page_size > INT32_MAX - 64)
+  if (a->batch * a->queries * a->heads > INT32_MAX || a->max_pages > (INT32_MAX - 4096) / c->page_size ||
+      a->prefix_pages > (INT32_MAX - 4096) / c->page_size)
     return b200_set_error(B200_ERR_UNSUPPORTED, "cache_attention: more rows or keys than 32-bit counts hold");
   if (a->q == nullptr || a->out == nullptr || a->lengths == nullptr || (a->tables == nullptr && a->max_pages > 0) ||
       (a->prefix_length > 0 && (a->prefix == nullptr || a->scratch == nullptr)))
