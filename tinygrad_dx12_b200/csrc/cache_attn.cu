@@ -60,7 +60,9 @@ struct Params {
   int64_t qsr, qsb, qsh;  // strides of q: request, token, head
   const uint8_t *k, *v;
   const void *ks, *vs;
-  int64_t cp, ch, ct, sp, sh, st;  // strides of codes (bytes) and scales: page, head, token
+  // strides in bytes: page, head, token; a page's extent and a page stride are below 2^31
+  uint32_t cp, ct, sp, st;
+  int64_t ch, sh;
   int e8m0, scale_vec, q_vec;
   int64_t pages;
   int page_shift, kv_heads, group;
@@ -152,7 +154,7 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
 }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool in) {  // zeros where not `in`
   const int n = in ? 16 : 0;
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+  asm volatile("cp.async.cg.shared.global.L2::64B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -228,50 +230,40 @@ struct Walk {
   uint32_t seg0;
 };
 
-// NB scales of a row as bfloat16 bits.
+// The NB scales of a row in as few words as they fill.
 template <int NB>
-__device__ __forceinline__ void load_scales(const void *base, int64_t at, bool e8m0, bool vec, uint32_t (&raw)[(NB + 1) / 2]) {
+__device__ __forceinline__ void load_scales(const uint8_t *p, bool e8m0, bool vec, uint32_t (&raw)[(NB + 1) / 2]) {
   if constexpr (NB == 1) {
-    raw[0] = e8m0 ? ((const uint8_t *)base)[at] : ((const uint16_t *)base)[at];
+    raw[0] = e8m0 ? *p : *(const uint16_t *)p;
+  } else if (vec && !e8m0) {
+    lds<NB * 2>(p, raw);
+  } else if (vec) {
+    if constexpr (NB == 2) raw[0] = *(const uint16_t *)p;
+    else lds<NB>(p, raw);
   } else {
-    if (vec && !e8m0) {
 #pragma unroll
-      for (int i = 0; i < NB / 2; ++i) raw[i] = 0;
-      if constexpr (NB == 2) raw[0] = *(const uint32_t *)((const uint16_t *)base + at);
-      if constexpr (NB == 4) {
-        const uint2 x = *(const uint2 *)((const uint16_t *)base + at);
-        raw[0] = x.x, raw[1] = x.y;
-      }
-      if constexpr (NB == 8) {
-        const uint4 x = *(const uint4 *)((const uint16_t *)base + at);
-        raw[0] = x.x, raw[1] = x.y, raw[2] = x.z, raw[3] = x.w;
-      }
-    } else if (vec) {  // bytes, left as they are: scale_at() widens them
-      if constexpr (NB == 2) raw[0] = *(const uint16_t *)((const uint8_t *)base + at);
-      if constexpr (NB == 4) raw[0] = *(const uint32_t *)((const uint8_t *)base + at);
-      if constexpr (NB == 8) {
-        const uint2 x = *(const uint2 *)((const uint8_t *)base + at);
-        raw[0] = x.x, raw[1] = x.y;
-      }
-    } else {
+    for (int i = 0; i < (NB + 1) / 2; ++i) raw[i] = 0;
 #pragma unroll
-      for (int i = 0; i < (NB + 1) / 2; ++i) raw[i] = 0;
-#pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        if (e8m0) raw[i / 4] |= (uint32_t)((const uint8_t *)base)[at + i] << (8 * (i % 4));
-        else raw[i / 2] |= (uint32_t)((const uint16_t *)base)[at + i] << (16 * (i % 2));
-      }
+    for (int i = 0; i < NB; ++i) {
+      if (e8m0) raw[i / 4] |= (uint32_t)p[i] << (8 * (i % 4));
+      else raw[i / 2] |= (uint32_t)((const uint16_t *)p)[i] << (16 * (i % 2));
     }
   }
 }
-// Scale i of load_scales' words as bfloat16 bits.
+// Them as fp32: E8M0's NaN byte reads infinity, which the product with zero turns into NaN (its
+// byte 0, 2^-127, reads zero).
 template <int NB>
-__device__ __forceinline__ uint32_t scale_at(const uint32_t (&raw)[(NB + 1) / 2], int i, bool e8m0) {
+__device__ __forceinline__ void widen(const uint32_t (&raw)[(NB + 1) / 2], bool e8m0, float (&f)[NB]) {
   if (e8m0) {
-    const uint32_t b = NB == 1 ? raw[0] : (raw[i / 4] >> (8 * (i % 4))) & 0xFFu;
-    return b == 0 ? 0x40u : b == 255 ? 0x7FC0u : b << 7;
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const float x = __uint_as_float(((raw[i / 4] >> (8 * (i % 4))) & 0xFFu) << 23);
+      f[i] = fmaf(x, 0.f, x);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NB; ++i) f[i] = __uint_as_float(i % 2 ? raw[i / 2] & 0xFFFF0000u : raw[i / 2] << 16);
   }
-  return NB == 1 ? raw[0] : (raw[i / 2] >> (16 * (i % 2))) & 0xFFFFu;
 }
 
 template <typename T, int F, int D, int NT, bool BLK>
@@ -406,12 +398,16 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
   constexpr int KPL = (C::T + 31) / 32;          // keys of a lane
   constexpr int SW = (C::KNB + 1) / 2;
   Walk a = c;                                    // the unit whose pages are being read
-  int32_t page[BPU];
-  int64_t code[BPU];                             // of the unit whose scales are being read
+  uint32_t page[BPU];
+  const uint8_t *code[BPU];                      // key codes of the unit whose scales are being read
   int left = 0;                                  // its keys, none if there is no such unit
   uint32_t bad = 0;                              // its blocks on pages outside the cache
   uint32_t rk[KPL][SW], rv[KPL][SW];
   const int page_blocks = p.page_shift - 4;
+  const uint32_t in_page = (1u << page_blocks) - 1;
+  const int lr = lane / C::CPR, lc = lane % C::CPR;
+  const uint32_t lane_code = lr * p.ct + lc * 16, lane_scale = (lane & 15) * p.st;
+  const uint64_t v_of_k = (uint64_t)p.v - (uint64_t)p.k, vs_of_ks = (uint64_t)p.vs - (uint64_t)p.ks;
 
   auto read_pages = [&]() {
     if (a.u >= u_end) return;
@@ -419,38 +415,36 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
     const int32_t *table = p.tables + a.b * p.table_stride;
 #pragma unroll
     for (int j = 0; j < BPU; ++j)
-      page[j] = (first + j) * 16 < a.keys ? __ldg(table + ((first + j) >> page_blocks)) : 0;
+      page[j] = (first + j) * 16 < a.keys ? (uint32_t)__ldg(table + ((first + j) >> page_blocks)) : 0u;
   };
   auto read_scales = [&]() {  // of a's unit, whose pages are here; then a moves on and its next pages are asked for
     left = 0, bad = 0;
     if (a.u >= u_end) return;
     const int first = (int)(a.u - a.seg0) * WARPS + warp;
     left = a.keys - first * C::T;
-    int64_t at[BPU];
+    const uint8_t *kh = p.k + a.h * p.ch, *sh = (const uint8_t *)p.ks + a.h * p.sh;
 #pragma unroll
     for (int j = 0; j < BPU; ++j) {
-      const bool in = 16 * j < left;
-      const bool ok = (uint32_t)page[j] < (uint64_t)p.pages;
-      if (in && !ok) {
-        bad |= 1u << j;
-        if (lane == 0) atomicOr(&g_device_error, DEVERR_BAD_INDEX);
+      if (page[j] >= (uint64_t)p.pages) {
+        if (16 * j < left) {
+          bad |= 1u << j;
+          if (lane == 0) atomicOr(&g_device_error, DEVERR_BAD_INDEX);
+        }
+        page[j] = 0;
       }
-      const int64_t pg = in && ok ? page[j] : 0;
-      const int64_t off = (int64_t)((first * BPU + j) & ((1 << page_blocks) - 1)) << 4;
-      code[j] = pg * p.cp + a.h * p.ch + off * p.ct;
-      at[j] = pg * p.sp + a.h * p.sh + off * p.st;
+      code[j] = kh + (uint64_t)page[j] * p.cp + ((first * BPU + j) & in_page) * 16 * p.ct;
     }
 #pragma unroll
     for (int k = 0; k < KPL; ++k) {
       const int key = lane + 32 * k, j = key >> 4;
-      int64_t row = at[0];
+      uint32_t pg = page[0];
 #pragma unroll
       for (int i = 1; i < BPU; ++i)
-        if (j == i) row = at[i];
-      row += (key & 15) * p.st;
+        if (j == i) pg = page[i];
       if (key < C::T && key < left && !((bad >> j) & 1)) {
-        load_scales<C::KNB>(p.ks, row, p.e8m0, p.scale_vec, rk[k]);
-        load_scales<C::KNB>(p.vs, row, p.e8m0, p.scale_vec, rv[k]);
+        const uint8_t *at = sh + (uint64_t)pg * p.sp + ((first * BPU + j) & in_page) * 16 * p.st + lane_scale;
+        load_scales<C::KNB>(at, p.e8m0, p.scale_vec, rk[k]);
+        load_scales<C::KNB>(at + vs_of_ks, p.e8m0, p.scale_vec, rv[k]);
       }
     }
     if (++a.u == a.seg1) next_segment(a);
@@ -460,14 +454,28 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
   auto fill = [&](int s) {
     if (left > 0) {
       const uint32_t kd = smem_u32(ring + s * C::STAGE), vd = kd + C::T * C::RB;
-      const int lr = lane / C::CPR, lc = lane % C::CPR;
+      if (left >= C::T && bad == 0) {
 #pragma unroll
-      for (int i = 0; i < C::T / C::RPI; ++i) {
-        const int row = lr + i * C::RPI, j = (i * C::RPI) >> 4;
-        const bool in = row < left && !((bad >> j) & 1);
-        const int64_t src = code[j] + (int64_t)(row & 15) * p.ct + lc * 16;
-        cp_async16(kd + C::chunk(row, lc), p.k + src, in);
-        cp_async16(vd + C::chunk(row, lc), p.v + src, in);
+        for (int i = 0; i < C::T / C::RPI; ++i) {
+          const uint8_t *src = code[(i * C::RPI) >> 4] + (lane_code + ((i * C::RPI) & 15) * p.ct);
+          const int to = C::chunk(lr + i * C::RPI, lc);
+          cp_async16(kd + to, src, true);
+          cp_async16(vd + to, src + v_of_k, true);
+        }
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < C::T / C::RPI; ++i) {
+          const int row = lr + i * C::RPI, j = (i * C::RPI) >> 4;
+          const bool in = row < left && !((bad >> j) & 1);
+          const uint8_t *at = code[0];
+#pragma unroll
+          for (int x = 1; x < BPU; ++x)
+            if (j == x) at = code[x];
+          const uint8_t *src = at + (lane_code + ((i * C::RPI) & 15) * p.ct);
+          const int to = C::chunk(row, lc);
+          cp_async16(kd + to, src, in);
+          cp_async16(vd + to, src + v_of_k, in);
+        }
       }
       float2 *lvi = (float2 *)(slots + s * C::SLOT);
       float *ks = (float *)(slots + s * C::SLOT + C::LVI);
@@ -477,31 +485,29 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
         const int key = lane + 32 * k;
         if (C::T < 32 && key >= C::T) continue;
         const bool in = key < left && !((bad >> (key >> 4)) & 1);
+        float kf[C::KNB], vf[C::KNB];
+        widen<C::KNB>(rk[k], p.e8m0, kf);
+        widen<C::KNB>(rv[k], p.e8m0, vf);
         if constexpr (!BLK) {
-          float vsc = __uint_as_float(scale_at<1>(rv[k], 0, p.e8m0) << 16);
-          vsc = vsc < 0x1p-120f ? 0x1p-120f : vsc;  // a scale of zero: weight without a value
+          const float vsc = vf[0] < 0x1p-120f ? 0x1p-120f : vf[0];  // a scale of zero: weight without a value
           lvi[key] = in ? make_float2(lg2(vsc), __frcp_rn(vsc)) : make_float2(-INFINITY, 0.f);
-          ks[key] = in ? __uint_as_float(scale_at<1>(rk[k], 0, p.e8m0) << 16) : 0.f;
+          ks[key] = in ? kf[0] : 0.f;
         } else {
-          uint32_t top = 0, vb[C::NB];
-          float kb[C::NB];
+          uint32_t top = 0;  // magnitudes order as integers, NaN above all
 #pragma unroll
-          for (int i = 0; i < C::NB; ++i) {
-            vb[i] = scale_at<C::NB>(rv[k], i, p.e8m0);
-            kb[i] = in ? __uint_as_float(scale_at<C::NB>(rk[k], i, p.e8m0) << 16) : 0.f;
-            top = max(top, vb[i]);
-          }
-          const int e = RowRef<F>::exponent(top);
-          const bool nan = top > 0x7F80u;  // the row's NaN travels in its denominator, which only rows that see it take
-          lvi[key] = in ? make_float2((float)(e - 127), nan ? __uint_as_float(0x7FC00000u) : RowRef<F>::inverse(e))
+          for (int i = 0; i < C::NB; ++i) top = max(top, __float_as_uint(vf[i]) & 0x7FFFFFFFu);
+          const int e = RowRef<F>::exponent(top >> 16);
+          float inv = RowRef<F>::inverse(e);
+          // the row's NaN travels in its denominator, which only rows that see it take
+          lvi[key] = in ? make_float2((float)(e - 127), top > 0x7F800000u ? __uint_as_float(top) : inv)
                         : make_float2(-INFINITY, 0.f);
+          const bool use = in && top <= 0x7F800000u;
+          __half *vk = vr + (key & ~7) + C::row_of(key & 7);  // ratios in the order of the instruction's rows
 #pragma unroll
-          for (int i = 0; i < C::NB; ++i) {
-            ks[key * C::NB + i] = kb[i];
-            // ratios in the order of the instruction's rows
-            vr[i * C::T + (key & ~7) + C::row_of(key & 7)] =
-                __float2half_rn(in && vb[i] <= 0x7F80u && !nan ? __uint_as_float(vb[i] << 16) * RowRef<F>::inverse(e) : 0.f);
-          }
+          for (int i = 0; i < C::NB; ++i) vk[i * C::T] = __float2half_rn(use ? vf[i] * inv : 0.f);
+#pragma unroll
+          for (int i = 0; i < C::NB; i += 2)
+            *(float2 *)(ks + key * C::NB + i) = in ? make_float2(kf[i], kf[i + 1]) : make_float2(0.f, 0.f);
         }
       }
     }
@@ -606,7 +612,13 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
       for (int sb = 0; sb < C::T && first + sb < c.keys; sb += 16) {
         const int k0 = sb + C::key_of(g), k1 = k0 + 8;  // this lane's two keys
         // s^T = K q^T
-        float s[NT][4], s2[NT][4];
+        float s[NT][4], s2[NT][4], sk0[C::KNB], sk1[C::KNB];
+        lds<C::KNB * 4 < 16 ? C::KNB * 4 : 16>((const uint8_t *)(ks_s + k0 * C::KNB), (uint32_t *)sk0);
+        lds<C::KNB * 4 < 16 ? C::KNB * 4 : 16>((const uint8_t *)(ks_s + k1 * C::KNB), (uint32_t *)sk1);
+        if constexpr (C::KNB == 8) {
+          lds<16>((const uint8_t *)(ks_s + k0 * C::KNB + 4), (uint32_t *)sk0 + 4);
+          lds<16>((const uint8_t *)(ks_s + k1 * C::KNB + 4), (uint32_t *)sk1 + 4);
+        }
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -630,14 +642,13 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
           }
           const uint32_t f0[4] = {f[0][0], f[1][0], f[0][1], f[1][1]}, f1[4] = {f[0][2], f[1][2], f[0][3], f[1][3]};
           if constexpr (BLK) {
-            const float sk0 = ks_s[k0 * C::NB + b], sk1 = ks_s[k1 * C::NB + b];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               float y[4] = {0.f, 0.f, 0.f, 0.f};
               gemv::mma16816(y, f0, q[n][b][0], q[n][b][1]);
               gemv::mma16816(y, f1, q[n][b][2], q[n][b][3]);
-              s[n][0] = fmaf(y[0], sk0, s[n][0]), s[n][1] = fmaf(y[1], sk0, s[n][1]);
-              s[n][2] = fmaf(y[2], sk1, s[n][2]), s[n][3] = fmaf(y[3], sk1, s[n][3]);
+              s[n][0] = fmaf(y[0], sk0[b], s[n][0]), s[n][1] = fmaf(y[1], sk0[b], s[n][1]);
+              s[n][2] = fmaf(y[2], sk1[b], s[n][2]), s[n][3] = fmaf(y[3], sk1[b], s[n][3]);
             }
           } else {
 #pragma unroll
@@ -648,15 +659,13 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
           }
         }
         const float2 lvi0 = lvi_s[k0], lvi1 = lvi_s[k1];
-        float ks0 = 1.f, ks1 = 1.f;
-        if constexpr (!BLK) ks0 = ks_s[k0], ks1 = ks_s[k1];
         // u = s + log2 vs: -inf for keys that are not there
         bool up = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            const float y = BLK ? s[n][x] : (s[n][x] + s2[n][x]) * (x < 2 ? ks0 : ks1);
+            const float y = BLK ? s[n][x] : (s[n][x] + s2[n][x]) * (x < 2 ? sk0[0] : sk1[0]);
             s[n][x] = fmaf(y, qs[n][x & 1], x < 2 ? lvi0.x : lvi1.x);
           }
           if (p.causal && p.queries > 1) {
@@ -970,12 +979,13 @@ static int32_t attention(const b200_cache_desc *c, const b200_attention_args *a,
   p.q = a->q;
   p.qsr = a->q_strides[0], p.qsb = a->q_strides[1], p.qsh = a->q_strides[2];
   p.k = (const uint8_t *)c->k, p.v = (const uint8_t *)c->v, p.ks = c->k_scales, p.vs = c->v_scales;
-  p.cp = c->strides[0], p.ch = c->strides[1], p.ct = c->strides[2];
-  p.sp = c->scale_strides[0], p.sh = c->scale_strides[1], p.st = c->scale_strides[2];
+  const int64_t esz = c->scale_dtype == B200_DT_E8M0 ? 1 : 2;
+  p.cp = (uint32_t)c->strides[0], p.ch = c->strides[1], p.ct = (uint32_t)c->strides[2];
+  p.sp = (uint32_t)(c->scale_strides[0] * esz), p.sh = c->scale_strides[1] * esz, p.st = (uint32_t)(c->scale_strides[2] * esz);
   p.q_vec = (uintptr_t)p.q % 16 == 0 && p.qsr % 8 == 0 && p.qsb % 8 == 0 && p.qsh % 8 == 0;
   p.e8m0 = c->scale_dtype == B200_DT_E8M0;
   const int per_row = dim / c->block_size;  // a row's scales as one vector where they are aligned so
-  p.scale_vec = p.sp % per_row == 0 && p.sh % per_row == 0 && p.st % per_row == 0;
+  p.scale_vec = p.sp % (per_row * esz) == 0 && p.sh % (per_row * esz) == 0 && p.st % (per_row * esz) == 0;
   p.pages = c->pages, p.kv_heads = c->kv_heads, p.group = a->heads / c->kv_heads, p.q_heads = a->heads;
   while ((1 << p.page_shift) < c->page_size) ++p.page_shift;
   p.scale = a->scale * 1.44269504088896341f;

@@ -520,6 +520,13 @@ int32_t check_cache(const b200_cache_desc *c) {
     if (c->k == nullptr || c->v == nullptr || c->k_scales == nullptr || c->v_scales == nullptr)
       return b200_set_error(B200_ERR_INVALID, "null cache storage");
     for (int i = 0; i < 3; ++i)
+      if (c->strides[i] < 0 || c->scale_strides[i] < 0)
+        return b200_set_error(B200_ERR_INVALID, "cache strides must not be negative");
+    constexpr int64_t most = 1ll << 30;
+    if (c->strides[0] > most || c->scale_strides[0] > most || c->strides[2] > most / c->page_size ||
+        c->scale_strides[2] > most / c->page_size)
+      return b200_set_error(B200_ERR_UNSUPPORTED, "cache pages of more than 2^30 bytes, or as far apart");
+    for (int i = 0; i < 3; ++i)
       if (c->strides[i] % 16) return b200_set_error(B200_ERR_INVALID, "cache strides must be multiples of 16 bytes");
     if ((uintptr_t)c->k % 16 || (uintptr_t)c->v % 16 || (uintptr_t)c->k_scales % 16 || (uintptr_t)c->v_scales % 16)
       return b200_set_error(B200_ERR_INVALID, "cache storage must start on 16-byte boundaries");
