@@ -78,138 +78,187 @@ __device__ __forceinline__ void store_n(T *p, bool vec, const float (&f)[N]) {
   for (int i = 0; i < N; ++i) p[i] = t[i];
 }
 
+// 16 bytes of T as fp32, and back.
+template <typename T, int N>
+__device__ __forceinline__ void widen_raw(const uint4 &r, float (&f)[N]) {
+  const T *t = reinterpret_cast<const T *>(&r);
+#pragma unroll
+  for (int i = 0; i < N; ++i) f[i] = (float)t[i];
+}
+template <typename T, int N>
+__device__ __forceinline__ uint4 narrow_raw(const float (&f)[N]) {
+  uint4 r;
+  if constexpr (sizeof(T) == 4) {
+    r = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  } else {
+    alignas(16) T t[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) t[i] = from_f32<T>(f[i]);
+    r = *reinterpret_cast<const uint4 *>(t);
+  }
+  return r;
+}
+
 // ---- rotary positions ----------------------------------------------------------------------------
 // Pair (a, b) of a head becomes (a cos - b sin, b cos + a sin), the transposed map (the gradient)
 // takes -sin. Products and sums are rounded one by one (no contraction): the same bits as the
-// formula in fp32. A unit is VEC values of each side of VEC pairs (half layout), VEC values of
-// VEC / 2 pairs (interleaved), or VEC values behind the rotated part, which are copied. A thread
-// keeps its angles for HPT heads, so that the tables are read HPT times less often.
+// formula in fp32. HBM-bound: each value is read and written once, 16 bytes a lane, and a thread
+// keeps its angles for HPT heads, so that the tables (L2) are read HPT times less often.
 struct RotaryArgs {
   const void *x;
   void *y;
   int64_t xsb, xst, xsh, ysb, yst, ysh;
-  int64_t batch, tokens;
+  uint32_t batch, tokens;
   int heads, dim, rot;
   const float *cos, *sin;
   int64_t rows;
   const void *pos;
   int pos_wide, interleaved;
   float sign;
-  int hgroups, units;
+  uint32_t hgroups, units, total;
 };
 
-template <typename T, int VEC, int HPT>
-__global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs a) {
-  pdl_enter();
-  const int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int u = (int)(idx % a.units);
-  const int64_t hi = idx / a.units;
-  const int hg = (int)(hi % a.hgroups);
-  const int64_t tok = hi / a.hgroups;
-  if (tok >= a.batch * a.tokens) return;
-  const int64_t b = tok / a.tokens, t = tok - b * a.tokens;
-  const int half = a.rot / 2, ur = a.interleaved ? a.rot / VEC : half / VEC;
-  const T *x = (const T *)a.x + b * a.xsb + t * a.xst;
-  T *y = (T *)a.y + b * a.ysb + t * a.yst;
-  constexpr bool V = VEC * sizeof(T) >= 16;
-  const int h0 = hg * HPT;
-  if (u >= ur) {  // behind the rotated part
-    const int d = a.rot + (u - ur) * VEC;
-#pragma unroll
-    for (int i = 0; i < HPT; ++i)
-      if (h0 + i < a.heads) {
-        float f[VEC];
-        load_n<T, VEC>(x + (int64_t)(h0 + i) * a.xsh + d, V, f);
-        store_n<T, VEC>(y + (int64_t)(h0 + i) * a.ysh + d, V, f);
-      }
-    return;
-  }
-  const int64_t p = load_index(a.pos, tok, a.pos_wide);
+__device__ __forceinline__ bool in_table(const RotaryArgs &a, int64_t p) {
   const bool ok = p >= 0 && p < a.rows;
   if (!ok) atomicOr(&g_device_error, DEVERR_BAD_INDEX);
-  const float nan = __uint_as_float(0x7FC00000u);
-  if (!a.interleaved) {
-    const int d = u * VEC;
-    float c[VEC], s[VEC];
-    if (ok) {
-      load_n<float, VEC>(a.cos + p * half + d, V, c);
-      load_n<float, VEC>(a.sin + p * half + d, V, s);
-    }
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) c[i] = ok ? c[i] : nan, s[i] = ok ? s[i] * a.sign : nan;
-    float f[HPT][VEC], g[HPT][VEC];
-#pragma unroll
-    for (int i = 0; i < HPT; ++i)
-      if (h0 + i < a.heads) {
-        load_n<T, VEC>(x + (int64_t)(h0 + i) * a.xsh + d, V, f[i]);
-        load_n<T, VEC>(x + (int64_t)(h0 + i) * a.xsh + half + d, V, g[i]);
-      }
-#pragma unroll
-    for (int i = 0; i < HPT; ++i)
-      if (h0 + i < a.heads) {
-        float m[VEC], n[VEC];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          m[j] = __fsub_rn(__fmul_rn(f[i][j], c[j]), __fmul_rn(g[i][j], s[j]));
-          n[j] = __fadd_rn(__fmul_rn(g[i][j], c[j]), __fmul_rn(f[i][j], s[j]));
-        }
-        store_n<T, VEC>(y + (int64_t)(h0 + i) * a.ysh + d, V, m);
-        store_n<T, VEC>(y + (int64_t)(h0 + i) * a.ysh + half + d, V, n);
-      }
-  } else if constexpr (VEC >= 2) {
-    const int d = u * VEC;
-    constexpr bool VT = V && VEC * 2 >= 16;
-    float c[VEC / 2], s[VEC / 2];
-    if (ok) {
-      load_n<float, VEC / 2>(a.cos + p * half + d / 2, VT, c);
-      load_n<float, VEC / 2>(a.sin + p * half + d / 2, VT, s);
-    }
-#pragma unroll
-    for (int i = 0; i < VEC / 2; ++i) c[i] = ok ? c[i] : nan, s[i] = ok ? s[i] * a.sign : nan;
-    float f[HPT][VEC];
-#pragma unroll
-    for (int i = 0; i < HPT; ++i)
-      if (h0 + i < a.heads) load_n<T, VEC>(x + (int64_t)(h0 + i) * a.xsh + d, V, f[i]);
-#pragma unroll
-    for (int i = 0; i < HPT; ++i)
-      if (h0 + i < a.heads) {
-        float m[VEC];
-#pragma unroll
-        for (int j = 0; j < VEC; j += 2) {
-          m[j] = __fsub_rn(__fmul_rn(f[i][j], c[j / 2]), __fmul_rn(f[i][j + 1], s[j / 2]));
-          m[j + 1] = __fadd_rn(__fmul_rn(f[i][j + 1], c[j / 2]), __fmul_rn(f[i][j], s[j / 2]));
-        }
-        store_n<T, VEC>(y + (int64_t)(h0 + i) * a.ysh + d, V, m);
-      }
-  }
+  return ok;
 }
 
-template <typename T, int VEC, int HPT>
-static int32_t launch_rotary_t(RotaryArgs a, cudaStream_t stream) {
-  a.hgroups = (a.heads + HPT - 1) / HPT;
-  a.units = (a.interleaved ? a.rot / VEC : a.rot / 2 / VEC) + (a.dim - a.rot) / VEC;
-  const int64_t n = a.batch * a.tokens * a.hgroups * a.units, blocks = (n + 255) / 256;
-  if (blocks > 0x7FFFFFFF) return b200_set_error(B200_ERR_UNSUPPORTED, "rotary: too many values for one launch");
-  B200_CUDA_TRY(launch_pdl(rotary_kernel<T, VEC, HPT>, dim3((unsigned)blocks), dim3(256), stream, a));
-  return B200_OK;
+// A unit is two vectors of 16 bytes: the sides of VEC pairs (half layout), neighbours in the rotated
+// part (interleaved), or two behind it, which pass unchanged: one path for all lanes of a warp.
+template <typename T, bool INTER, int HPT>
+__global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
+  pdl_enter();
+  constexpr int VEC = 16 / sizeof(T), NA = INTER ? VEC : VEC;  // angles of a unit
+  const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
+  if (idx >= a.total) return;
+  const uint32_t hi = idx / a.units, u = idx - hi * a.units;
+  const uint32_t tok = hi / a.hgroups, hg = hi - tok * a.hgroups;
+  const uint32_t b = a.batch == 1 ? 0 : tok / a.tokens, t = tok - b * a.tokens;
+  const int half = a.rot / 2, turned = (INTER ? a.rot / 2 : half) / VEC;
+  const bool turn = (int)u < turned;
+  const int rest = (a.dim - a.rot) / 2;
+  const int d0 = INTER ? (int)u * 2 * VEC : turn ? (int)u * VEC : a.rot + ((int)u - turned) * VEC;
+  const int d1 = INTER ? d0 + VEC : turn ? d0 + half : d0 + rest;
+  const int h0 = (int)hg * HPT;
+  const T *x = (const T *)a.x + b * a.xsb + t * a.xst + (int64_t)h0 * a.xsh;
+  T *y = (T *)a.y + b * a.ysb + t * a.yst + (int64_t)h0 * a.ysh;
+  uint4 r[HPT][2];
+#pragma unroll
+  for (int i = 0; i < HPT; ++i)
+    if (h0 + i < a.heads) {
+      r[i][0] = *reinterpret_cast<const uint4 *>(x + i * a.xsh + d0);
+      r[i][1] = *reinterpret_cast<const uint4 *>(x + i * a.xsh + d1);
+    }
+  float c[NA], s[NA];
+#pragma unroll
+  for (int i = 0; i < NA; ++i) c[i] = s[i] = __uint_as_float(0x7FC00000u);
+  if (turn) {
+    const int64_t p = load_index(a.pos, tok, a.pos_wide);
+    if (in_table(a, p)) {
+      const float *ct = a.cos + p * half + (INTER ? d0 / 2 : d0), *st = a.sin + p * half + (INTER ? d0 / 2 : d0);
+#pragma unroll
+      for (int i = 0; i < NA / 4; ++i) {
+        reinterpret_cast<float4 *>(c)[i] = __ldg(reinterpret_cast<const float4 *>(ct) + i);
+        reinterpret_cast<float4 *>(s)[i] = __ldg(reinterpret_cast<const float4 *>(st) + i);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NA; ++i) s[i] *= a.sign;
+#pragma unroll
+  for (int i = 0; i < HPT; ++i)
+    if (h0 + i < a.heads) {
+      if (turn) {
+        float f[VEC], g[VEC], m[VEC], n[VEC];
+        widen_raw<T, VEC>(r[i][0], f);
+        widen_raw<T, VEC>(r[i][1], g);
+        if constexpr (INTER) {
+#pragma unroll
+          for (int j = 0; j < VEC; j += 2) {
+            const float c0 = c[j / 2], s0 = s[j / 2], c1 = c[VEC / 2 + j / 2], s1 = s[VEC / 2 + j / 2];
+            m[j] = __fsub_rn(__fmul_rn(f[j], c0), __fmul_rn(f[j + 1], s0));
+            m[j + 1] = __fadd_rn(__fmul_rn(f[j + 1], c0), __fmul_rn(f[j], s0));
+            n[j] = __fsub_rn(__fmul_rn(g[j], c1), __fmul_rn(g[j + 1], s1));
+            n[j + 1] = __fadd_rn(__fmul_rn(g[j + 1], c1), __fmul_rn(g[j], s1));
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            m[j] = __fsub_rn(__fmul_rn(f[j], c[j]), __fmul_rn(g[j], s[j]));
+            n[j] = __fadd_rn(__fmul_rn(g[j], c[j]), __fmul_rn(f[j], s[j]));
+          }
+        }
+        r[i][0] = narrow_raw<T, VEC>(m), r[i][1] = narrow_raw<T, VEC>(n);
+      }
+      *reinterpret_cast<uint4 *>(y + i * a.ysh + d0) = r[i][0];
+      *reinterpret_cast<uint4 *>(y + i * a.ysh + d1) = r[i][1];
+    }
+}
+
+// Any size and alignment: a thread a pair, or two values behind the rotated part.
+template <typename T>
+__global__ void __launch_bounds__(256) rotary_any_kernel(const RotaryArgs a) {
+  pdl_enter();
+  const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
+  if (idx >= a.total) return;
+  const uint32_t hi = idx / a.units, u = idx - hi * a.units;
+  const uint32_t tok = hi / (uint32_t)a.heads, h = hi - tok * a.heads;
+  const uint32_t b = tok / a.tokens, t = tok - b * a.tokens;
+  const int half = a.rot / 2;
+  const T *x = (const T *)a.x + b * a.xsb + t * a.xst + (int64_t)h * a.xsh;
+  T *y = (T *)a.y + b * a.ysb + t * a.yst + (int64_t)h * a.ysh;
+  if ((int)u >= half) {
+    const int d = 2 * (int)u;
+    y[d] = x[d];
+    if (d + 1 < a.dim) y[d + 1] = x[d + 1];
+    return;
+  }
+  const int d0 = a.interleaved ? 2 * (int)u : (int)u, d1 = a.interleaved ? d0 + 1 : d0 + half;
+  const int64_t p = load_index(a.pos, tok, a.pos_wide);
+  float c = __uint_as_float(0x7FC00000u), s = c;
+  if (in_table(a, p)) c = a.cos[p * half + u], s = a.sin[p * half + u] * a.sign;
+  const float f = (float)x[d0], g = (float)x[d1];
+  y[d0] = from_f32<T>(__fsub_rn(__fmul_rn(f, c), __fmul_rn(g, s)));
+  y[d1] = from_f32<T>(__fadd_rn(__fmul_rn(g, c), __fmul_rn(f, s)));
 }
 
 template <typename T>
-static int32_t launch_rotary_dt(const RotaryArgs &a, cudaStream_t stream) {
+static int32_t launch_rotary_dt(RotaryArgs a, int64_t batch, int64_t tokens, cudaStream_t stream) {
   constexpr int VEC = 16 / sizeof(T);
   auto fits = [](const void *p, int64_t sb, int64_t st, int64_t sh) {
     return (uintptr_t)p % 16 == 0 && sb % VEC == 0 && st % VEC == 0 && sh % VEC == 0;
   };
-  const int side = a.interleaved ? a.rot : a.rot / 2;
-  const bool vec = fits(a.x, a.xsb, a.xst, a.xsh) && fits(a.y, a.ysb, a.yst, a.ysh) && side % VEC == 0 &&
-                   (a.dim - a.rot) % VEC == 0 && (uintptr_t)a.cos % 16 == 0 && (uintptr_t)a.sin % 16 == 0 &&
+  const bool vec = fits(a.x, a.xsb, a.xst, a.xsh) && fits(a.y, a.ysb, a.yst, a.ysh) && a.rot % (2 * VEC) == 0 &&
+                   (a.dim - a.rot) % (2 * VEC) == 0 && (uintptr_t)a.cos % 16 == 0 && (uintptr_t)a.sin % 16 == 0 &&
                    (a.rot / 2) % 4 == 0;
-  if (!vec) return a.interleaved && (a.dim - a.rot) % 2 == 0 ? launch_rotary_t<T, 2, 1>(a, stream)
-                   : a.interleaved ? b200_set_error(B200_ERR_UNSUPPORTED, "rotary: an odd head needs the half layout")
-                                   : launch_rotary_t<T, 1, 1>(a, stream);
-  // four heads a thread once that leaves every SM its 2048 threads twice over
-  const int64_t threads = a.batch * a.tokens * ((a.heads + 3) / 4) * (a.dim / VEC);
-  return threads >= 148 * 2048 * 2 ? launch_rotary_t<T, VEC, 4>(a, stream) : launch_rotary_t<T, VEC, 1>(a, stream);
+  // two heads a thread once that leaves every SM its 2048 threads twice over
+  const bool wide = vec && batch * tokens * a.heads * (a.dim / (2 * VEC)) >= 148 * 2048 * 4;
+  a.units = vec ? a.dim / (2 * VEC) : (a.dim + 1) / 2;
+  a.hgroups = wide ? (a.heads + 1) / 2 : a.heads;
+  const int64_t per_token = (int64_t)a.units * a.hgroups;
+  if (per_token > (1 << 30)) return b200_set_error(B200_ERR_UNSUPPORTED, "rotary: a token of too many values");
+  // launches of less than 2^31 threads: runs of whole batches, or of one batch's tokens
+  const int64_t most = (1ll << 30) / per_token;
+  const int64_t nt = tokens < most ? tokens : most, nb = tokens < most ? most / tokens : 1;
+  const RotaryArgs all = a;
+  const int64_t es = sizeof(T), ps = a.pos_wide ? 8 : 4;
+  for (int64_t b = 0; b < batch; b += nb)
+    for (int64_t t = 0; t < tokens; t += nt) {
+      a.batch = (uint32_t)(batch - b < nb ? batch - b : nb);
+      a.tokens = (uint32_t)(tokens - t < nt ? tokens - t : nt);
+      a.x = (const uint8_t *)all.x + (b * a.xsb + t * a.xst) * es;
+      a.y = (uint8_t *)all.y + (b * a.ysb + t * a.yst) * es;
+      a.pos = (const uint8_t *)all.pos + (b * tokens + t) * ps;
+      a.total = (uint32_t)(a.batch * (int64_t)a.tokens * per_token);
+      const dim3 grid((a.total + 255) / 256), block(256);
+      if (!vec) B200_CUDA_TRY(launch_pdl(rotary_any_kernel<T>, grid, block, stream, a));
+      else if (a.interleaved && wide) B200_CUDA_TRY(launch_pdl(rotary_kernel<T, true, 2>, grid, block, stream, a));
+      else if (a.interleaved) B200_CUDA_TRY(launch_pdl(rotary_kernel<T, true, 1>, grid, block, stream, a));
+      else if (wide) B200_CUDA_TRY(launch_pdl(rotary_kernel<T, false, 2>, grid, block, stream, a));
+      else B200_CUDA_TRY(launch_pdl(rotary_kernel<T, false, 1>, grid, block, stream, a));
+    }
+  return B200_OK;
 }
 
 // ---- writing -------------------------------------------------------------------------------------
@@ -230,7 +279,7 @@ struct WriteArgs {
   int rot, interleaved;
   const void *pos;
   int pos_wide;
-  int qvec, kvec, vvec, tvec;
+  int qvec, kvec, vvec, tvec, page_shift;
 };
 
 template <int F>
@@ -279,6 +328,154 @@ __device__ __forceinline__ void encode8(const float (&x)[8], float inv, uint8_t 
   }
 }
 
+// A block's scale from its largest magnitude, stored at `at` when `writes`.
+template <int F>
+__device__ __forceinline__ float block_scale(float top, bool e8m0, void *scales, int64_t at, bool writes) {
+  constexpr float lo = 0x1p-100f, hi = 0x1p100f;
+  const float r = __fmul_rn(top, (float)(1.0 / CFmt<F>::qmax));
+  if (e8m0) {
+    uint32_t e = (__float_as_uint(r) + 0x7FFFFFu) >> 23;
+    e = r != r ? 255u : min(227u, max(27u, e));
+    if (writes) ((uint8_t *)scales)[at] = (uint8_t)e;
+    return e == 255u ? r : __uint_as_float(e << 23);
+  }
+  float sc = __bfloat162float(__float2bfloat16_rn(r));
+  sc = sc < lo ? lo : sc > hi ? hi : sc;
+  if (writes) ((__nv_bfloat16 *)scales)[at] = __float2bfloat16_rn(sc);
+  return sc;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN above all
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+template <int F>
+__device__ __forceinline__ void encode8_scaled(float (&y)[8], float sc, uint8_t *codes) {
+  // under a NaN scale codes are zeros: in attention the NaN then reaches only rows that see the key
+  if (sc != sc)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = 0.f;
+  encode8<F>(y, __frcp_rn(sc != sc ? 1.f : sc), codes);
+}
+
+// The usual shapes of 16-bit inputs: a lane holds the two vectors of 8 values that turn together (or
+// two that pass), dim / 16 lanes a row, so that every value is read once; four rows in flight. INTER:
+// interleaved pairs, or none to turn (cos null).
+constexpr int PT = 128, PR = 3;
+template <typename T, int F, int D, bool INTER>
+__global__ void __launch_bounds__(PT, 6) cache_write_pairs_kernel(const WriteArgs a) {
+  pdl_enter();
+  constexpr int LPR = D / 16, RPC = PT / LPR;
+  const int j = threadIdx.x % LPR, slot_row = threadIdx.x / LPR, step = RPC * gridDim.y;
+  const int kvh = a.c.kv_heads, total = a.q_heads + 2 * kvh, half = a.rot / 2;
+  const uint32_t t = blockIdx.x;
+  const int turned = INTER ? LPR : half / 8;
+  const bool mine = INTER || j < turned;
+  const int d0 = INTER || j < turned ? j * 8 : a.rot + (j - turned) * 8;
+  const int d1 = INTER ? d0 + D / 2 : mine ? d0 + half : d0 + (D - a.rot) / 2;
+  const int64_t slot = load_index(a.slots, t, a.slots_wide);
+  const int64_t cells = a.c.pages << a.page_shift;
+  if (slot >= cells && threadIdx.x == 0) atomicOr(&g_device_error, DEVERR_BAD_INDEX);
+  const bool place = slot >= 0 && slot < cells;
+  const int64_t page = place ? slot >> a.page_shift : 0, offset = place ? slot & ((1 << a.page_shift) - 1) : 0;
+  const int64_t code0 = page * a.c.strides[0] + offset * a.c.strides[2];
+  const int64_t scale0 = page * a.c.scale_strides[0] + offset * a.c.scale_strides[2];
+  const bool e8 = a.c.scale_dtype == B200_DT_E8M0;
+  const int blk = a.c.block_size, lanes = blk == D ? LPR : 4;
+  float c[8], s[8];  // half layout: of the pairs; interleaved: 4 of the first vector, 4 of the second
+  const bool turn0 = a.cos != nullptr && (INTER ? d0 < a.rot : mine), turn1 = a.cos != nullptr && (INTER ? d1 < a.rot : mine);
+  const int r_first = slot_row + blockIdx.y * RPC;
+  for (int r0 = r_first; r0 - slot_row % (32 / LPR) < total; r0 += PR * step) {  // uniform in a warp
+    uint4 x[PR][2];
+#pragma unroll
+    for (int i = 0; i < PR; ++i) {
+      const int r = r0 + i * step;
+      if (r < total) {
+        const T *src = r < a.q_heads ? (const T *)a.q + t * a.qst + r * a.qsh
+                       : r < a.q_heads + kvh ? (const T *)a.k + t * a.kst + (r - a.q_heads) * a.ksh
+                                             : (const T *)a.v + t * a.vst + (r - a.q_heads - kvh) * a.vsh;
+        x[i][0] = *reinterpret_cast<const uint4 *>(src + d0);
+        x[i][1] = *reinterpret_cast<const uint4 *>(src + d1);
+      }
+    }
+    if (r0 == r_first && a.cos != nullptr) {  // once, behind the first rows' loads
+      const int64_t p = load_index(a.pos, t, a.pos_wide);
+      const bool ok = p >= 0 && p < a.rows;
+      if (!ok && threadIdx.x == 0) atomicOr(&g_device_error, DEVERR_BAD_INDEX);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) c[i] = s[i] = __uint_as_float(0x7FC00000u);
+      const float *ct = a.cos + p * half, *st = a.sin + p * half;
+      if (ok && turn0) {
+        const int at = INTER ? d0 / 2 : d0;
+        reinterpret_cast<float4 *>(c)[0] = __ldg((const float4 *)(ct + at));
+        reinterpret_cast<float4 *>(s)[0] = __ldg((const float4 *)(st + at));
+      }
+      if (ok && turn1) {
+        const int at = INTER ? d1 / 2 : d0 + 4;
+        reinterpret_cast<float4 *>(c)[1] = __ldg((const float4 *)(ct + at));
+        reinterpret_cast<float4 *>(s)[1] = __ldg((const float4 *)(st + at));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < PR; ++i) {
+      const int r = r0 + i * step;
+      if (r - slot_row % (32 / LPR) >= total) break;  // the whole warp is done
+      const bool in = r < total, isq = r < a.q_heads, isk = r < a.q_heads + kvh;
+      float f[8], g[8];
+      widen_raw<T, 8>(x[i][0], f);
+      widen_raw<T, 8>(x[i][1], g);
+      if (isk) {
+        if constexpr (INTER) {
+          if (turn0)
+#pragma unroll
+            for (int y = 0; y < 8; y += 2) {
+              const float m = f[y], n = f[y + 1];
+              f[y] = __fsub_rn(__fmul_rn(m, c[y / 2]), __fmul_rn(n, s[y / 2]));
+              f[y + 1] = __fadd_rn(__fmul_rn(n, c[y / 2]), __fmul_rn(m, s[y / 2]));
+            }
+          if (turn1)
+#pragma unroll
+            for (int y = 0; y < 8; y += 2) {
+              const float m = g[y], n = g[y + 1];
+              g[y] = __fsub_rn(__fmul_rn(m, c[4 + y / 2]), __fmul_rn(n, s[4 + y / 2]));
+              g[y + 1] = __fadd_rn(__fmul_rn(n, c[4 + y / 2]), __fmul_rn(m, s[4 + y / 2]));
+            }
+        } else if (turn0) {
+#pragma unroll
+          for (int y = 0; y < 8; ++y) {
+            const float m = f[y], n = g[y];
+            f[y] = __fsub_rn(__fmul_rn(m, c[y]), __fmul_rn(n, s[y]));
+            g[y] = __fadd_rn(__fmul_rn(n, c[y]), __fmul_rn(m, s[y]));
+          }
+        }
+      }
+      if (isq) {
+        T *dst = (T *)a.q_out + ((int64_t)t * a.q_heads + r) * D;
+        *reinterpret_cast<uint4 *>(dst + d0) = narrow_raw<T, 8>(f);
+        *reinterpret_cast<uint4 *>(dst + d1) = narrow_raw<T, 8>(g);
+      }
+      if (__all_sync(0xFFFFFFFFu, isq)) continue;
+      float tf = 0.f, tg = 0.f;
+#pragma unroll
+      for (int y = 0; y < 8; ++y) tf = max_nan(tf, fabsf(f[y])), tg = max_nan(tg, fabsf(g[y]));
+      if (blk == D) tf = tg = max_nan(tf, tg);
+      for (int m = 1; m < lanes; m <<= 1) {
+        tf = max_nan(tf, __shfl_xor_sync(0xFFFFFFFFu, tf, m));
+        if (blk != D) tg = max_nan(tg, __shfl_xor_sync(0xFFFFFFFFu, tg, m));
+      }
+      if (!in || isq || !place) continue;
+      const int h = isk ? r - a.q_heads : r - a.q_heads - kvh;
+      void *scales = isk ? a.c.k_scales : a.c.v_scales;
+      uint8_t *codes = (uint8_t *)(isk ? a.c.k : a.c.v) + code0 + h * a.c.strides[1];
+      const int64_t at = scale0 + h * a.c.scale_strides[1];
+      const float sf = block_scale<F>(tf, e8, scales, at + d0 / blk, d0 % blk == 0);
+      const float sg = blk == D ? sf : block_scale<F>(tg, e8, scales, at + d1 / blk, d1 % blk == 0);
+      encode8_scaled<F>(f, sf, codes + d0 * CFmt<F>::bits / 8);
+      encode8_scaled<F>(g, sg, codes + d1 * CFmt<F>::bits / 8);
+    }
+  }
+}
+
 constexpr int WT = 256, WR = 4;  // threads of a CTA, rows in flight per lane
 
 template <typename T, int F, int D>
@@ -292,7 +489,7 @@ __global__ void __launch_bounds__(WT) cache_write_kernel(WriteArgs a) {
   const int64_t cells = a.c.pages * a.c.page_size;
   if (slot >= cells && threadIdx.x == 0) atomicOr(&g_device_error, DEVERR_BAD_INDEX);
   const bool place = slot >= 0 && slot < cells;
-  const int64_t page = place ? slot / a.c.page_size : 0, offset = place ? slot - page * a.c.page_size : 0;
+  const int64_t page = place ? slot >> a.page_shift : 0, offset = place ? slot - (page << a.page_shift) : 0;
   const int half = a.rot / 2;
   const bool turns = a.cos != nullptr;
   // the angles of this lane's values, and which way the other of a pair lies: half layout
@@ -371,44 +568,45 @@ __global__ void __launch_bounds__(WT) cache_write_kernel(WriteArgs a) {
       const int lanes = a.c.block_size / 8;
       for (int m = 1; m < lanes; m <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, m));
       if (in && !isq && place) {
-        constexpr float lo = 0x1p-100f, hi = 0x1p100f;
-        const float rr = __fmul_rn(__uint_as_float(top), (float)(1.0 / CFmt<F>::qmax));
         const int h = isk ? r - a.q_heads : r - a.q_heads - kvh;
         const int64_t at = scale_row(a.c, page, h, offset) + lane_d / a.c.block_size;
-        const bool writes = lane_d % a.c.block_size == 0;
-        float sc;
-        if (a.c.scale_dtype == B200_DT_E8M0) {
-          uint32_t e = (__float_as_uint(rr) + 0x7FFFFFu) >> 23;
-          e = rr != rr ? 255u : min(227u, max(27u, e));
-          sc = e == 255u ? rr : __uint_as_float(e << 23);
-          if (writes) ((uint8_t *)(isk ? a.c.k_scales : a.c.v_scales))[at] = (uint8_t)e;
-        } else {
-          sc = __bfloat162float(__float2bfloat16_rn(rr));
-          sc = sc < lo ? lo : sc > hi ? hi : sc;
-          if (writes) ((__nv_bfloat16 *)(isk ? a.c.k_scales : a.c.v_scales))[at] = __float2bfloat16_rn(sc);
-        }
-        // under a NaN scale codes are zeros: in attention the NaN then reaches only rows that see the key
-        uint8_t *codes = (uint8_t *)(isk ? a.c.k : a.c.v) + code_row(a.c, page, h, offset) + lane_d * CFmt<F>::bits / 8;
-        if (sc != sc)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) y[j] = 0.f;
-        encode8<F>(y, __frcp_rn(sc != sc ? 1.f : sc), codes);
+        const float sc = block_scale<F>(__uint_as_float(top), a.c.scale_dtype == B200_DT_E8M0,
+                                        isk ? a.c.k_scales : a.c.v_scales, at, lane_d % a.c.block_size == 0);
+        encode8_scaled<F>(y, sc, (uint8_t *)(isk ? a.c.k : a.c.v) + code_row(a.c, page, h, offset) +
+                                     lane_d * CFmt<F>::bits / 8);
       }
     }
   }
 }
 
+template <typename T, int F, int D>
+static int32_t launch_write_d(const WriteArgs &a, cudaStream_t stream) {
+  const int rows = a.q_heads + 2 * a.c.kv_heads;
+  // few tokens: a CTA for every run of rows; many: one a token, its angles loaded once
+  const bool many = a.tokens >= 148 * 8;
+  if constexpr (sizeof(T) == 2) {
+    const int blk = a.c.block_size, rest = D - a.rot;
+    const bool inter = a.cos == nullptr || a.interleaved;
+    const bool pairs = (a.q_heads == 0 || a.qvec) && a.kvec && a.vvec &&
+                       (a.cos == nullptr || (a.tvec && (inter ? a.rot % 8 == 0 : (rest / 2) % 8 == 0))) &&
+                       (inter || blk == D || ((a.rot / 2) % 32 == 0 && (rest / 2) % 32 == 0));
+    if (pairs) {
+      const int rpc = PT / (D / 16);
+      const dim3 grid((unsigned)a.tokens, (unsigned)(many ? 1 : (rows + rpc - 1) / rpc));
+      if (inter) B200_CUDA_TRY(launch_pdl(cache_write_pairs_kernel<T, F, D, true>, grid, dim3(PT), stream, a));
+      else B200_CUDA_TRY(launch_pdl(cache_write_pairs_kernel<T, F, D, false>, grid, dim3(PT), stream, a));
+      return B200_OK;
+    }
+  }
+  const int rpc = WT / (D / 8);
+  const dim3 grid((unsigned)a.tokens, (unsigned)(many ? 1 : (rows + rpc - 1) / rpc));
+  B200_CUDA_TRY(launch_pdl(cache_write_kernel<T, F, D>, grid, dim3(WT), stream, a));
+  return B200_OK;
+}
 template <typename T, int F>
 static int32_t launch_write_t(const WriteArgs &a, cudaStream_t stream) {
-  const int rows = a.q_heads + 2 * a.c.kv_heads, rpc = WT / (a.c.head_dim / 8);
-  const int need = (rows + rpc - 1) / rpc;
-  // few tokens: a CTA for every RPC rows; many: one CTA a token, its angles loaded once
-  const int split = a.tokens >= 148 * 8 ? 1 : need;
-  const dim3 grid((unsigned)a.tokens, (unsigned)split);
-  if (a.c.head_dim == 64) B200_CUDA_TRY(launch_pdl(cache_write_kernel<T, F, 64>, grid, dim3(WT), stream, a));
-  else if (a.c.head_dim == 128) B200_CUDA_TRY(launch_pdl(cache_write_kernel<T, F, 128>, grid, dim3(WT), stream, a));
-  else B200_CUDA_TRY(launch_pdl(cache_write_kernel<T, F, 256>, grid, dim3(WT), stream, a));
-  return B200_OK;
+  return a.c.head_dim == 64 ? launch_write_d<T, F, 64>(a, stream)
+         : a.c.head_dim == 128 ? launch_write_d<T, F, 128>(a, stream) : launch_write_d<T, F, 256>(a, stream);
 }
 template <typename T>
 static int32_t launch_write_f(const WriteArgs &a, cudaStream_t stream) {
@@ -422,78 +620,97 @@ static int32_t launch_write_f(const WriteArgs &a, cudaStream_t stream) {
 
 // ---- reading back --------------------------------------------------------------------------------
 // out[t, h, :] = codes * scale of slot t, one fp32 product rounded to the output type; a thread
-// gives 8 values. A negative slot reads zeros.
+// gives 16 values of the key and of the value. A negative slot reads zeros.
 struct ReadArgs {
   b200_cache_desc c;
   const void *slots;
-  int slots_wide;
-  int64_t tokens;
+  int slots_wide, page_shift;
+  uint32_t total;
   void *k_out, *v_out;
 };
 
+// 8 * W codes as fp32, W = 1 or 2 words of 4-bit codes, 2 of 8-bit.
 template <int F>
-__device__ __forceinline__ void decode8(const uint8_t *src, float (&f)[8]) {
-  uint32_t p[4];
+__device__ __forceinline__ void decode16(const uint32_t (&w)[CFmt<F>::bits / 2], float (&f)[16]) {
+  uint32_t p[8];
   if constexpr (CFmt<F>::bits == 8) {
-    const uint2 w = *reinterpret_cast<const uint2 *>(src);
-    decode4_8bit<F>(w.x, p[0], p[1]);
-    decode4_8bit<F>(w.y, p[2], p[3]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) decode4_8bit<F>(w[i], p[2 * i], p[2 * i + 1]);
   } else {
-    decode8_4<F>(*reinterpret_cast<const uint32_t *>(src), p);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) decode8_4<F>(w[i], reinterpret_cast<uint32_t(&)[4]>(p[4 * i]));
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 8; ++i) {
     const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&p[i]));
-    if constexpr (F == B200_CACHE_INT4) f[i] = v.x, f[i + 4] = v.y;
+    if constexpr (F == B200_CACHE_INT4) f[8 * (i / 4) + i % 4] = v.x, f[8 * (i / 4) + i % 4 + 4] = v.y;
     else f[2 * i] = v.x, f[2 * i + 1] = v.y;
   }
 }
 
-template <typename T, int F>
-__global__ void __launch_bounds__(256) cache_read_kernel(ReadArgs a) {
+template <typename T, int F, int D>
+__global__ void __launch_bounds__(256) cache_read_kernel(const ReadArgs a) {
   pdl_enter();
-  const int D = a.c.head_dim, lpr = D / 8;
-  const int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int d = (int)(idx % lpr) * 8;
-  const int64_t hi = idx / lpr;
-  const int h = (int)(hi % a.c.kv_heads);
-  const int64_t t = hi / a.c.kv_heads;
-  if (t >= a.tokens) return;
+  constexpr int LPR = D / 16, W = CFmt<F>::bits / 2;  // lanes of a row, words of 16 codes
+  const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
+  if (idx >= a.total) return;
+  const int d = (int)(idx % LPR) * 16;
+  const uint32_t hi = idx / LPR, kvh = a.c.kv_heads, t = hi / kvh, h = hi - t * kvh;
   const int64_t slot = load_index(a.slots, t, a.slots_wide);
-  const int64_t cells = a.c.pages * a.c.page_size;
-  const bool in = slot >= 0 && slot < cells;
+  const int64_t cells = a.c.pages << a.page_shift;
   if (slot >= cells) atomicOr(&g_device_error, DEVERR_BAD_INDEX);
-  float k[8], v[8];
+  float k[16], v[16];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) k[i] = v[i] = 0.f;
-  if (in) {
-    const int64_t page = slot / a.c.page_size;
-    const int64_t offset = slot - page * a.c.page_size;
-    const bool e8 = a.c.scale_dtype == B200_DT_E8M0;
+  for (int i = 0; i < 16; ++i) k[i] = v[i] = 0.f;
+  if (slot >= 0 && slot < cells) {
+    const int64_t page = slot >> a.page_shift, offset = slot - (page << a.page_shift);
     const int64_t at = scale_row(a.c, page, h, offset) + d / a.c.block_size;
     const int64_t cd = code_row(a.c, page, h, offset) + d * CFmt<F>::bits / 8;
+    uint32_t wk[W], wv[W];
+    if constexpr (W == 4) {
+      *reinterpret_cast<uint4 *>(wk) = *reinterpret_cast<const uint4 *>((const uint8_t *)a.c.k + cd);
+      *reinterpret_cast<uint4 *>(wv) = *reinterpret_cast<const uint4 *>((const uint8_t *)a.c.v + cd);
+    } else {
+      *reinterpret_cast<uint2 *>(wk) = *reinterpret_cast<const uint2 *>((const uint8_t *)a.c.k + cd);
+      *reinterpret_cast<uint2 *>(wv) = *reinterpret_cast<const uint2 *>((const uint8_t *)a.c.v + cd);
+    }
+    const bool e8 = a.c.scale_dtype == B200_DT_E8M0;
     const float ks = scale_f32(a.c.k_scales, at, e8), vs = scale_f32(a.c.v_scales, at, e8);
-    decode8<F>((const uint8_t *)a.c.k + cd, k);
-    decode8<F>((const uint8_t *)a.c.v + cd, v);
+    decode16<F>(wk, k);
+    decode16<F>(wv, v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) k[i] *= ks, v[i] *= vs;
+    for (int i = 0; i < 16; ++i) k[i] *= ks, v[i] *= vs;
   }
-  store_n<T, 8>((T *)a.k_out + (t * a.c.kv_heads + h) * D + d, true, k);
-  store_n<T, 8>((T *)a.v_out + (t * a.c.kv_heads + h) * D + d, true, v);
+  const int64_t to = (int64_t)hi * D + d;
+  store_n<T, 16>((T *)a.k_out + to, true, k);
+  store_n<T, 16>((T *)a.v_out + to, true, v);
 }
 
-template <typename T>
-static int32_t launch_read_t(const ReadArgs &a, cudaStream_t stream) {
-  const int64_t n = a.tokens * a.c.kv_heads * (a.c.head_dim / 8), blocks = (n + 255) / 256;
-  if (blocks > 0x7FFFFFFF) return b200_set_error(B200_ERR_UNSUPPORTED, "cache_read: too many values for one launch");
-  const dim3 grid((unsigned)blocks);
-  switch (a.c.format) {
-    case B200_CACHE_INT8: B200_CUDA_TRY(launch_pdl(cache_read_kernel<T, B200_CACHE_INT8>, grid, dim3(256), stream, a)); break;
-    case B200_CACHE_FP8E4M3: B200_CUDA_TRY(launch_pdl(cache_read_kernel<T, B200_CACHE_FP8E4M3>, grid, dim3(256), stream, a)); break;
-    case B200_CACHE_INT4: B200_CUDA_TRY(launch_pdl(cache_read_kernel<T, B200_CACHE_INT4>, grid, dim3(256), stream, a)); break;
-    default: B200_CUDA_TRY(launch_pdl(cache_read_kernel<T, B200_CACHE_FP4_E2M1>, grid, dim3(256), stream, a)); break;
+template <typename T, int F>
+static int32_t launch_read_f(ReadArgs a, int64_t tokens, cudaStream_t stream) {
+  // launches of less than 2^31 threads
+  const int64_t per_token = (int64_t)a.c.kv_heads * (a.c.head_dim / 16), most = (1ll << 30) / per_token;
+  const ReadArgs all = a;
+  for (int64_t t = 0; t < tokens; t += most) {
+    const int64_t n = tokens - t < most ? tokens - t : most, out = t * a.c.kv_heads * a.c.head_dim;
+    a.slots = (const uint8_t *)all.slots + t * (a.slots_wide ? 8 : 4);
+    a.k_out = (T *)all.k_out + out, a.v_out = (T *)all.v_out + out;
+    a.total = (uint32_t)(n * per_token);
+    const dim3 grid((a.total + 255) / 256), block(256);
+    if (a.c.head_dim == 64) B200_CUDA_TRY(launch_pdl(cache_read_kernel<T, F, 64>, grid, block, stream, a));
+    else if (a.c.head_dim == 128) B200_CUDA_TRY(launch_pdl(cache_read_kernel<T, F, 128>, grid, block, stream, a));
+    else B200_CUDA_TRY(launch_pdl(cache_read_kernel<T, F, 256>, grid, block, stream, a));
   }
   return B200_OK;
+}
+template <typename T>
+static int32_t launch_read_t(const ReadArgs &a, int64_t tokens, cudaStream_t stream) {
+  switch (a.c.format) {
+    case B200_CACHE_INT8: return launch_read_f<T, B200_CACHE_INT8>(a, tokens, stream);
+    case B200_CACHE_FP8E4M3: return launch_read_f<T, B200_CACHE_FP8E4M3>(a, tokens, stream);
+    case B200_CACHE_INT4: return launch_read_f<T, B200_CACHE_INT4>(a, tokens, stream);
+    default: return launch_read_f<T, B200_CACHE_FP4_E2M1>(a, tokens, stream);
+  }
 }
 
 static bool bad_index_dtype(int dt) { return dt != B200_DT_I32 && dt != B200_DT_I64; }
@@ -541,13 +758,13 @@ int32_t launch_rotary(const void *x, int32_t dtype, int64_t batch, int64_t token
   RotaryArgs a = {};
   a.x = x, a.y = y;
   a.xsb = xs[0], a.xst = xs[1], a.xsh = xs[2], a.ysb = ys[0], a.yst = ys[1], a.ysh = ys[2];
-  a.batch = batch, a.tokens = tokens, a.heads = heads, a.dim = head_dim, a.rot = r->rotary_dim;
+  a.heads = heads, a.dim = head_dim, a.rot = r->rotary_dim;
   a.cos = r->cos, a.sin = r->sin, a.rows = r->rows, a.pos = pos;
   a.pos_wide = pos_dtype == B200_DT_I64, a.interleaved = r->interleaved, a.sign = transpose ? -1.f : 1.f;
   switch (dtype) {
-    case B200_DT_F16: return launch_rotary_dt<__half>(a, stream);
-    case B200_DT_BF16: return launch_rotary_dt<__nv_bfloat16>(a, stream);
-    default: return launch_rotary_dt<float>(a, stream);
+    case B200_DT_F16: return launch_rotary_dt<__half>(a, batch, tokens, stream);
+    case B200_DT_BF16: return launch_rotary_dt<__nv_bfloat16>(a, batch, tokens, stream);
+    default: return launch_rotary_dt<float>(a, batch, tokens, stream);
   }
 }
 
@@ -572,6 +789,7 @@ int32_t launch_cache_write(const b200_cache_desc *c, const void *k, const void *
   a.kst = ks[0], a.ksh = ks[1], a.vst = vs[0], a.vsh = vs[1];
   if (q != nullptr) a.qst = qs[0], a.qsh = qs[1];
   a.slots = slots, a.slots_wide = slots_dtype == B200_DT_I64;
+  while ((1 << a.page_shift) < c->page_size) ++a.page_shift;
   if (r != nullptr) {
     a.cos = r->cos, a.sin = r->sin, a.rows = r->rows, a.rot = r->rotary_dim, a.interleaved = r->interleaved;
     a.pos = pos, a.pos_wide = pos_dtype == B200_DT_I64;
@@ -589,11 +807,12 @@ int32_t launch_cache_write(const b200_cache_desc *c, const void *k, const void *
 int32_t launch_cache_read(const b200_cache_desc *c, const void *slots, int32_t slots_dtype, int64_t tokens, void *k_out,
                           void *v_out, int32_t dtype, cudaStream_t stream) {
   using namespace cache;
-  ReadArgs a = {*c, slots, slots_dtype == B200_DT_I64, tokens, k_out, v_out};
+  ReadArgs a = {*c, slots, slots_dtype == B200_DT_I64, 0, 0, k_out, v_out};
+  while ((1 << a.page_shift) < c->page_size) ++a.page_shift;
   switch (dtype) {
-    case B200_DT_F16: return launch_read_t<__half>(a, stream);
-    case B200_DT_BF16: return launch_read_t<__nv_bfloat16>(a, stream);
-    default: return launch_read_t<float>(a, stream);
+    case B200_DT_F16: return launch_read_t<__half>(a, tokens, stream);
+    case B200_DT_BF16: return launch_read_t<__nv_bfloat16>(a, tokens, stream);
+    default: return launch_read_t<float>(a, tokens, stream);
   }
 }
 
