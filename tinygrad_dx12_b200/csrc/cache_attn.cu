@@ -34,8 +34,7 @@
 #include <map>
 #include <mutex>
 
-#include "cache.cuh"
-#include "kernels.h"
+#include "cache_attn.cuh"
 #include "sm100.cuh"
 
 namespace b200 {
@@ -47,44 +46,9 @@ int32_t cache_attn_device_error(unsigned int *v, bool clear) {
 
 namespace cattn {
 
-using namespace cache;
-
 constexpr int WARPS = 8, THREADS = WARPS * 32, STAGES = 2;
 constexpr int MAX_ENTRIES = 1024;    // (request, row tile) pairs of one launch
 constexpr int SHORT = 4;             // rounds that a segment is not cut below where work is scarce
-constexpr float LAZY = 4.f;          // u may pass the running maximum by this before it moves
-constexpr float BIAS = 15.f - LAZY;  // p = 2^(u - m + BIAS) uses fp16 up to 2^15, so small weights keep their bits
-
-struct Params {
-  const void *q;
-  int64_t qsr, qsb, qsh;  // strides of q: request, token, head
-  const uint8_t *k, *v;
-  const void *ks, *vs;
-  // strides in bytes: page, head, token; a page's extent and a page stride are below 2^31
-  uint32_t cp, ct, sp, st;
-  int64_t ch, sh;
-  int e8m0, scale_vec, q_vec;
-  int64_t pages;
-  int page_shift, kv_heads, group;
-  const int32_t *tables;
-  int64_t table_stride;
-  int max_pages;
-  const int32_t *lengths;  // per request, or null: `fixed` for all
-  int64_t fixed;
-  int batch, rows, queries;  // rows: query rows of a (request, key head)
-  int per_request;           // queries of a request (rows / group of them may span requests)
-  int causal;
-  float scale;  // softmax scale * log2 e
-  int row_tiles, q_heads;
-  // results: final (out, lse) or partial (po, pm, pl)
-  void *out;
-  float *lse;
-  float *po, *pm, *pl;
-  const float *fo, *fm, *fl;  // partials of the shared prefix, joined at the end
-  // split segments
-  float *ws_o, *ws_ml;
-  uint32_t *tickets;
-};
 
 template <int F, int D, int NT, bool BLK>
 struct Cfg {
@@ -129,28 +93,10 @@ struct Cfg {
   }
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float lg2(float x) {
-  float y;
-  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t *>(&h);
-}
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
   uint32_t y;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
-}
-__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
-  const __half2 r = __hmul2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
-  return *reinterpret_cast<const uint32_t *>(&r);
 }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool in) {  // zeros where not `in`
   const int n = in ? 16 : 0;
@@ -159,69 +105,6 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool i
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-template <int BYTES>
-__device__ __forceinline__ void lds(const uint8_t *p, uint32_t *w) {
-  if constexpr (BYTES == 16) {
-    const uint4 x = *reinterpret_cast<const uint4 *>(p);
-    w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
-  } else if constexpr (BYTES == 8) {
-    const uint2 x = *reinterpret_cast<const uint2 *>(p);
-    w[0] = x.x, w[1] = x.y;
-  } else {
-    w[0] = *reinterpret_cast<const uint32_t *>(p);
-  }
-}
-
-// 2^-(E - H): what a block's scale is multiplied by; 2^(E - H) is the row's scale.
-template <int F>
-struct RowRef {
-  static constexpr int H = CFmt<F>::bits == 4 ? 12 : 6;
-  // `top`: bfloat16 bits of the row's largest scale
-  __device__ static __forceinline__ int exponent(uint32_t top) { return max((int)((top >> 7) & 0xFF), H + 1) - H; }
-  __device__ static __forceinline__ float inverse(int e) { return __uint_as_float((uint32_t)(254 - e) << 23); }
-  __device__ static __forceinline__ float value(int e) { return __uint_as_float((uint32_t)e << 23); }
-};
-
-// Query row r of (entry, key head h): its offset in q, and its place among all rows of out.
-struct RowAt {
-  int64_t q, out;
-};
-__device__ __forceinline__ RowAt row_at(const Params &p, int b, int h, int r) {
-  const int tok = r / p.group, head = h * p.group + (r - tok * p.group);
-  const int rq = tok / p.per_request, qi = tok - rq * p.per_request;
-  const int64_t req = b + rq;
-  return {req * p.qsr + qi * p.qsb + head * p.qsh, (req * p.per_request + qi) * p.q_heads + head};
-}
-
-template <typename T>
-__device__ __forceinline__ float to_f32(T v) { return (float)v; }
-template <typename T> __device__ __forceinline__ T out_of(float v);
-template <> __device__ __forceinline__ __half out_of<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 out_of<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-
-// A row's result from its numerator (four values), maximum and denominator.
-template <typename T, int D>
-__device__ __forceinline__ void finish(const Params &p, int64_t row, int d, float4 o, float m, float l) {
-  if (p.po != nullptr) {
-    *reinterpret_cast<float4 *>(p.po + row * D + d) = o;
-    if (d == 0) p.pm[row] = m, p.pl[row] = l;
-    return;
-  }
-  if (p.fo != nullptr) {
-    const float pm = p.fm[row], M = fmaxf(m, pm);
-    const float a = m == -INFINITY ? 0.f : ex2(m - M), b = pm == -INFINITY ? 0.f : ex2(pm - M);
-    const float4 f = *reinterpret_cast<const float4 *>(p.fo + row * D + d);
-    o.x = o.x * a + f.x * b, o.y = o.y * a + f.y * b, o.z = o.z * a + f.z * b, o.w = o.w * a + f.w * b;
-    l = l * a + p.fl[row] * b;
-    m = M;
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;  // no key seen: zeros
-  T *dst = (T *)p.out + row * D + d;
-  alignas(8) T r[4] = {out_of<T>(o.x * inv), out_of<T>(o.y * inv), out_of<T>(o.z * inv), out_of<T>(o.w * inv)};
-  *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<const uint2 *>(r);
-  if (p.lse != nullptr && d == 0) p.lse[row] = l == 0.f ? -INFINITY : (m - BIAS + log2f(l)) * 0.69314718055994531f;
-}
-
 // A run of units of one segment, as a warp walks it.
 struct Walk {
   uint32_t u, seg1;   // the round it stands at, and where its segment ends (both in the run's numbering)
@@ -229,42 +112,6 @@ struct Walk {
   int b, keys;        // request, keys that the segment reads
   uint32_t seg0;
 };
-
-// The NB scales of a row in as few words as they fill.
-template <int NB>
-__device__ __forceinline__ void load_scales(const uint8_t *p, bool e8m0, bool vec, uint32_t (&raw)[(NB + 1) / 2]) {
-  if constexpr (NB == 1) {
-    raw[0] = e8m0 ? *p : *(const uint16_t *)p;
-  } else if (vec && !e8m0) {
-    lds<NB * 2>(p, raw);
-  } else if (vec) {
-    if constexpr (NB == 2) raw[0] = *(const uint16_t *)p;
-    else lds<NB>(p, raw);
-  } else {
-#pragma unroll
-    for (int i = 0; i < (NB + 1) / 2; ++i) raw[i] = 0;
-#pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      if (e8m0) raw[i / 4] |= (uint32_t)p[i] << (8 * (i % 4));
-      else raw[i / 2] |= (uint32_t)((const uint16_t *)p)[i] << (16 * (i % 2));
-    }
-  }
-}
-// Them as fp32: E8M0's NaN byte reads infinity, which the product with zero turns into NaN (its
-// byte 0, 2^-127, reads zero).
-template <int NB>
-__device__ __forceinline__ void widen(const uint32_t (&raw)[(NB + 1) / 2], bool e8m0, float (&f)[NB]) {
-  if (e8m0) {
-#pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      const float x = __uint_as_float(((raw[i / 4] >> (8 * (i % 4))) & 0xFFu) << 23);
-      f[i] = fmaf(x, 0.f, x);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < NB; ++i) f[i] = __uint_as_float(i % 2 ? raw[i / 2] & 0xFFFF0000u : raw[i / 2] << 16);
-  }
-}
 
 template <typename T, int F, int D, int NT, bool BLK>
 __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel(const Params p) {
@@ -921,7 +768,7 @@ static int32_t launch_t(Params p, cudaStream_t stream) {
       p.tables += b * p.table_stride, p.lengths += b;
       p.out = (T *)p.out + rows * D;
       if (p.lse != nullptr) p.lse += rows;
-      if (p.fo != nullptr) p.fo += rows * D, p.fm += rows, p.fl += rows;
+      p.row0 += rows;
       if (int32_t rc = launch_t<T, F, D, NT, BLK>(p, stream)) return rc;
     }
     return B200_OK;
@@ -992,7 +839,8 @@ static int32_t attention(const b200_cache_desc *c, const b200_attention_args *a,
   p.per_request = a->queries;
   const bool blk = c->block_size != dim;
   const int64_t all_rows = (int64_t)a->batch * a->queries * a->heads;
-  auto run = [&](const Params &q) {
+  auto run = [&](Params &q) {
+    if (mma_supported(q, dim)) return launch_mma(q, a->q_dtype, c->format, dim, blk, stream);
     return a->q_dtype == B200_DT_F16 ? launch_f<__half>(q, c->format, dim, blk, stream)
                                      : launch_f<__nv_bfloat16>(q, c->format, dim, blk, stream);
   };
@@ -1002,7 +850,7 @@ static int32_t attention(const b200_cache_desc *c, const b200_attention_args *a,
     f.fixed = a->prefix_length, f.batch = 1, f.queries = (int)(a->batch * a->queries), f.rows = f.queries * p.group;
     f.po = (float *)a->scratch, f.pm = f.po + all_rows * dim, f.pl = f.pm + all_rows;
     if (int32_t rc = run(f)) return rc;
-    p.fo = f.po, p.fm = f.pm, p.fl = f.pl;
+    p.fo = f.po, p.fm = f.pm, p.fl = f.pl, p.cuts = f.cuts;
   }
   p.tables = a->tables, p.table_stride = a->table_stride, p.max_pages = (int)a->max_pages, p.lengths = a->lengths;
   p.batch = (int)a->batch, p.queries = (int)a->queries, p.rows = p.queries * p.group, p.causal = 1;

@@ -1,0 +1,861 @@
+// cache_attn_mma.cu -- attention of many query rows over the packed key/value cache, on the tcgen05 cores.
+//
+// The mathematics is cache_attn.cu's (base 2, u = s + log2 vs, codes as fp16 operands); here a tile of
+// 128 query rows meets tiles of 128 keys: s = Q K^T (M = 128, N = 128, K = D) and O += p V (M = 128,
+// N = D, K = 128) as tcgen05.mma with accumulators in tensor memory. Rows are those that see the same
+// keys: all requests' heads of a key head over a shared prefix, or the tokens of a prompt's chunk times
+// the heads of a group. One CTA an SM, 16 warps:
+//   warps 0..7    two softmax warpgroups, a thread a row: scores from tensor memory, p back into it in
+//                 the scores' place as the second product's left operand; O stays in tensor memory and
+//                 is only touched when a row's maximum has grown by more than 2^4;
+//   warps 8..11   codes -> fp16 into swizzled tiles in shared memory: keys row by row; values eight keys
+//                 at a time, turned on the way so that keys are contiguous (pairs of keys are joined by
+//                 byte permutes before they are decoded). Codes of the next tile are in registers;
+//   warp 12       one lane issues the MMAs (13..15 are there for the registers' split).
+// Two row tiles share every decoded key tile (256 rows); with up to 128 rows both warpgroups take the
+// same rows and every other key tile each, and add up at the end. While one slot is in its softmax the
+// other's products run. What bounds it: a tile pair is 2048 cycles of MMA, as many of the special
+// function unit (one exponential a score) and about 9000 issue slots of four schedulers.
+//
+// Tiles of all (row tile, key head) segments are laid end to end and cut into equal runs, one per CTA.
+// A segment within a run is finished there; the others leave their share (numerators, maximum,
+// denominator) in the CTA's two workspace slots, and are joined by the kernel after it: the one over
+// the requests' own keys for a prefix, join_kernel for a chunk.
+#include <map>
+#include <mutex>
+
+#include "cache_attn.cuh"
+#include "sm100.cuh"
+
+namespace b200 {
+
+int32_t cache_attn_mma_device_error(unsigned int *v, bool clear) {
+  B200_CUDA_TRY(tu_device_error(v, clear));
+  return B200_OK;
+}
+
+namespace cattn {
+namespace mma {
+
+constexpr int KT = 128;                      // keys of a tile
+constexpr int WG = 128, THREADS = 4 * WG;
+constexpr int MAX_ENTRIES = 1024;
+// 128 x (2 x 176 + 104 + 56) = 512 x 128, the registers that the block is launched with
+constexpr int SOFT_REGS = 176, DECODE_REGS = 104, ISSUE_REGS = 56;
+constexpr uint64_t WAIT_NS = 2000000000ull;
+
+template <int F, int D, bool BLK>
+struct Cfg {
+  static constexpr int bits = CFmt<F>::bits;
+  static constexpr int RB = D * bits / 8;
+  static constexpr int U = 8, UD = D / U, UB = UD * bits / 8, UW = UB / 4;  // units of a row, values, bytes, words of one
+  static constexpr int NB = D / 32, KNB = BLK ? NB : 1;
+  static constexpr int QB = 128 * D * 2, KB = KT * D * 2, VB = KT * D * 2;
+  static constexpr int RING = 4;                                            // tiles of scales
+  static constexpr int SC = RING * KT * 12, RATIO = BLK ? 2 * NB * KT * 2 : 0;
+  static constexpr int SMEM = 1024 + 2 * QB + 2 * KB + 2 * VB + SC + 2 * RATIO + 256;
+};
+
+__device__ __forceinline__ float2 wide2(const Params &p, uint32_t w) {
+  if (p.q_bf16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+  return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+}
+template <int D>
+__device__ __forceinline__ void finish_any(const Params &p, int64_t row, int d, float4 o, float m, float l) {
+  if (p.q_bf16) finish<__nv_bfloat16, D>(p, row, d, o, m, l);
+  else finish<__half, D>(p, row, d, o, m, l);
+}
+
+__device__ __forceinline__ int length_of(const Params &p, int b) {
+  const int64_t cap = (int64_t)p.max_pages << p.page_shift;
+  const int64_t n = p.lengths != nullptr ? p.lengths[b] : p.fixed;
+  return (int)(n < 0 ? 0 : n > cap ? cap : n);
+}
+__device__ __forceinline__ int keys_of(const Params &p, int e, int tile_rows) {
+  const int b = p.row_tiles == 1 ? e : e / p.row_tiles, n = length_of(p, b);
+  if (!p.causal) return n;
+  const int r1 = min(p.rows, (e - b * p.row_tiles + 1) * tile_rows) - 1;
+  return max(0, n - p.queries + r1 / p.group + 1);
+}
+// Tiles of a key head before each entry (request, row tile), by the first warp.
+__device__ __forceinline__ void scan_entries(const Params &p, int tile_rows, uint32_t *prefix) {
+  const int entries = p.batch * p.row_tiles, lane = threadIdx.x & 31;
+  if (threadIdx.x < 32) {
+    uint32_t carry = 0;
+    for (int e0 = 0; e0 < entries; e0 += 32) {
+      const int e = e0 + lane;
+      const uint32_t n = e < entries ? ((uint32_t)keys_of(p, e, tile_rows) + KT - 1) / KT : 0;
+      uint32_t inc = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+        if (lane >= o) inc += v;
+      }
+      if (e < entries) prefix[e] = carry + inc - n;
+      carry += __shfl_sync(0xFFFFFFFFu, inc, 31);
+    }
+    if (lane == 0) prefix[entries] = carry;
+  }
+}
+
+// A run of tiles, segment part by segment part.
+struct Part {
+  uint32_t u, u_end;         // where the run stands, and its end
+  uint32_t seg0, tiles;      // the segment's first tile, and how many it has
+  uint32_t from, to;         // this part of it
+  int e, h, b, keys;
+};
+
+struct Bars {
+  uint64_t qfull[2], sfull[2], pfull[2], pvdone[2], kfull[2], kfree[2], vfull[2], vfree[2], scfull[4];
+  uint64_t done[3];  // one row tile: the first warpgroup's products; the second's share; that share's reading
+};
+
+template <int REGS> __device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS)); }
+template <int REGS> __device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS)); }
+// All N threads of barrier ID meet; whether every one of them is `ok`.
+template <int ID, int N>
+__device__ __forceinline__ bool meet(bool ok) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.and.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(all)
+      : "r"((uint32_t)ok), "n"(ID), "n"(N)
+      : "memory");
+  return all != 0;
+}
+
+// Byte of 16-byte chunk g (8 values) of row r in a K-major tile of `rows` rows, 64 values a swizzled row.
+__device__ __forceinline__ uint32_t tile_at(int rows, int r, int g) {
+  return (uint32_t)((g >> 3) * rows * 128 + r * 128 + (((g & 7) ^ (r & 7)) << 4));
+}
+__device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// The type of q and out is a matter of a few instructions a row: a run-time one.
+template <int F, int D, int RT, bool BLK>
+__global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
+  using C = Cfg<F, D, BLK>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t *qt = smem, *kt = qt + 2 * C::QB, *vt = kt + 2 * C::KB;
+  float *sc = (float *)(vt + 2 * C::VB);             // [RING][key scale | log2 value scale | its inverse][KT]
+  __half *kratio = (__half *)((uint8_t *)sc + C::SC), *vratio = kratio + C::RATIO / 2;  // [2][NB][KT]
+  __shared__ Bars bars;
+  __shared__ uint32_t prefix[MAX_ENTRIES + 1];
+  __shared__ float2 share_ml[RT == 1 ? 128 : 1];
+  __shared__ uint32_t tmem_slot;
+  __shared__ uint32_t abort_word;
+  volatile uint32_t *abort_flag = &abort_word;
+
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  constexpr int TR = 128 * RT;  // rows of a segment
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars.qfull[i], WG), mbar_init(&bars.sfull[i], 1), mbar_init(&bars.pfull[i], WG), mbar_init(&bars.pvdone[i], 1);
+      mbar_init(&bars.kfull[i], WG), mbar_init(&bars.kfree[i], 1), mbar_init(&bars.vfull[i], WG), mbar_init(&bars.vfree[i], 1);
+    }
+    for (int i = 0; i < 4; ++i) mbar_init(&bars.scfull[i], WG);
+    for (int i = 0; i < 3; ++i) mbar_init(&bars.done[i], WG);
+    abort_word = 0;
+    fence_mbar_init();
+  }
+  scan_entries(p, TR, prefix);
+  if (warp == 12) tmem_alloc(&tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const int entries = p.batch * p.row_tiles, heads = p.kv_heads;
+  const uint32_t total = prefix[entries] * (uint32_t)heads;
+  const bool split = p.ws_o != nullptr;
+  const uint32_t per = max(1u, (total + gridDim.x - 1) / gridDim.x);
+
+  // rows without a key: zeros (or what the prefix gave)
+  for (int e = blockIdx.x; e < entries; e += gridDim.x) {
+    if (prefix[e + 1] != prefix[e]) continue;
+    const int b = p.row_tiles == 1 ? e : e / p.row_tiles, rt = e - b * p.row_tiles;
+    const int n = min(TR, p.rows - rt * TR);
+    for (int i = tid; i < heads * n * (D / 4); i += THREADS) {
+      const int d = (i % (D / 4)) * 4, rr = i / (D / 4);
+      const RowAt at = row_at(p, b, rr / n, rt * TR + rr % n);
+      finish_any<D>(p, at.out, d, make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, 0.f);
+    }
+  }
+
+  auto enter = [&](Part &w) {  // the segment of w.e, w.h, from w.u on
+    w.tiles = prefix[w.e + 1] - prefix[w.e];
+    w.seg0 = prefix[w.e] * heads + w.h * w.tiles;
+    w.b = p.row_tiles == 1 ? w.e : w.e / p.row_tiles;
+    w.keys = keys_of(p, w.e, TR);
+    w.from = w.u - w.seg0;
+    w.to = min(w.u_end - w.seg0, w.tiles);
+  };
+  auto next = [&](Part &w) {  // on to the next part; false at the end of the run
+    do {
+      w.u = w.seg0 + w.tiles;
+      if (w.u >= w.u_end) return false;
+      if (++w.h == heads) {
+        w.h = 0;
+        do ++w.e;
+        while (prefix[w.e + 1] == prefix[w.e]);
+      }
+      enter(w);
+    } while (!split && (w.e * (uint32_t)heads + w.h) % gridDim.x != blockIdx.x);
+    return true;
+  };
+  auto begin = [&](Part &w) {
+    w.u = split ? min(total, blockIdx.x * per) : 0;
+    w.u_end = split ? min(total, w.u + per) : total;
+    if (w.u >= w.u_end) return false;
+    int lo = 0, hi = entries;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (prefix[mid] * heads <= w.u) lo = mid;
+      else hi = mid;
+    }
+    w.e = lo;
+    w.h = (int)((w.u - prefix[lo] * heads) / (prefix[lo + 1] - prefix[lo]));
+    enter(w);
+    return split || (w.e * (uint32_t)heads + w.h) % gridDim.x == blockIdx.x ? true : next(w);
+  };
+  const int page_blocks = p.page_shift - 4;
+  const uint32_t in_page = (1u << page_blocks) - 1;
+
+  if (warp < 8) {
+    // ================ softmax: thread = row of slot `slot` ================
+    reg_inc<SOFT_REGS>();
+    const int slot = warp >> 2, r = tid & 127;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + lanes + (uint32_t)slot * 128, to = tmem + lanes + 256 + slot * D;
+    uint32_t n0 = 0, ops = 0, parts = 0;  // tiles of the CTA so far; this slot's operations and parts
+    Part w;
+    bool alive = true;
+    auto wait = [&](uint64_t *bar, uint32_t parity) {  // the warp's answer: what follows is for whole warps
+      return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, abort_flag, WAIT_NS)) != 0;
+    };
+    for (bool more = begin(w); more && alive; more = next(w), ++parts) {
+      const int rt = w.e - w.b * p.row_tiles, row = rt * TR + (RT == 2 ? slot * 128 : 0) + r;
+      const bool in = row < p.rows;
+      const int len = length_of(p, w.b);
+      const int lim = !in ? 0 : p.causal ? len - p.queries + row / p.group + 1 : len;
+      const RowAt at = in ? row_at(p, w.b, w.h, row) : RowAt{0, 0};
+      const uint32_t first = RT == 2 ? w.from : w.from + ((n0 ^ slot) & 1);  // this slot's tiles: first, first + RT's step
+      constexpr uint32_t STEP = RT == 2 ? 1 : 2;
+      float m = -INFINITY, l = 0.f, qs = 0.f;
+      const uint32_t ops0 = ops;
+      if (first < w.to) {
+        // q: fp16, scaled by a power of two, in the order that the keys' codes come out decoded
+        const uint16_t *src = (const uint16_t *)p.q + at.q;
+        uint32_t raw[4];
+        float top = 0.f;
+        auto load8 = [&](int g) {
+          if (!in) raw[0] = raw[1] = raw[2] = raw[3] = 0;
+          else if (p.q_vec) lds<16>((const uint8_t *)(src + 8 * g), raw);
+          else
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              raw[i] = (uint32_t)src[8 * g + 2 * i] | ((uint32_t)src[8 * g + 2 * i + 1] << 16);
+        };
+#pragma unroll 4
+        for (int g = 0; g < D / 8; ++g) {
+          load8(g);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 v = wide2(p, raw[i]);
+            top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
+          }
+        }
+        const int ex = min(max((int)(__float_as_uint(top) >> 23), 1), 253);
+        const float down = __uint_as_float((uint32_t)(254 - ex) << 23);
+        qs = p.scale * __uint_as_float((uint32_t)ex << 23);
+        const uint32_t qa = smem_u32(qt + slot * C::QB);
+#pragma unroll 4
+        for (int g = 0; g < D / 8; ++g) {
+          load8(g);
+          float x[8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 v = wide2(p, raw[i]);
+            x[2 * i] = v.x * down, x[2 * i + 1] = v.y * down;
+          }
+          uint32_t y[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            y[i] = F == B200_CACHE_INT4 ? pack_f16(x[i], x[i + 4]) : pack_f16(x[2 * i], x[2 * i + 1]);
+          sts128(qa + tile_at(128, r, g), y[0], y[1], y[2], y[3]);
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        mbar_arrive(&bars.qfull[slot]);
+      }
+      for (uint32_t j = first; j < w.to; j += STEP, ++ops) {
+        const uint32_t n = n0 + (j - w.from);
+        alive = wait(&bars.scfull[n & 3], (n >> 2) & 1) && wait(&bars.sfull[slot], ops & 1);
+        if (!alive) break;
+        tc_fence_after();
+        const float4 *k4 = (const float4 *)(sc + (n & 3) * 3 * KT), *l4 = k4 + KT / 4, *i4 = l4 + KT / 4;
+        uint32_t u[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(ts + 32 * c, u[c]);
+        tmem_ld_wait();
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float4 k = k4[8 * c + i], a = l4[8 * c + i];
+            const float ks[4] = {k.x, k.y, k.z, k.w}, as[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const float y = fmaf(__uint_as_float(u[c][4 * i + x]) * ks[x], qs, as[x]);
+              u[c][4 * i + x] = __float_as_uint(y);
+              top[x] = fmaxf(top[x], y);
+            }
+          }
+        if (p.causal && __any_sync(0xFFFFFFFFu, (int)(j * KT + KT) > lim)) {  // keys that this row does not see
+          top[0] = top[1] = top[2] = top[3] = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              if ((int)(j * KT) + 32 * c + i >= lim) u[c][i] = 0xFF800000u;
+              top[i & 3] = fmaxf(top[i & 3], __uint_as_float(u[c][i]));
+            }
+        }
+        const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        const bool up = most > m + LAZY;
+        if (__any_sync(0xFFFFFFFFu, up)) {
+          const float f = !up || m == -INFINITY ? 1.f : ex2(m - most);
+          if (up) m = most, l *= f;
+          if (ops != ops0) {  // what O holds
+            alive = wait(&bars.pvdone[slot], (ops - 1) & 1);
+            if (!alive) break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t o[16];
+              tmem_ld_32x32b_x16(to + 16 * c, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              tmem_st_32x32b_x16(to + 16 * c, o);
+            }
+          }
+        }
+        const float mm = m == -INFINITY ? 0.f : m - BIAS;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float4 v = i4[8 * c + i];
+            const float vs[4] = {v.x, v.y, v.z, v.w};
+            float e[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              e[x] = ex2(__uint_as_float(u[c][4 * i + x]) - mm);
+              if (e[x] != 0.f) sum[x] = fmaf(e[x], vs[x], sum[x]);  // an unseen key's scale may be NaN
+            }
+            pk[2 * i] = pack_f16(e[0], e[1]), pk[2 * i + 1] = pack_f16(e[2], e[3]);
+          }
+          tmem_st_32x32b_x16(ts + 16 * c, pk);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&bars.pfull[slot]);
+      }
+      if (!alive) break;
+      n0 += w.to - w.from;
+      const bool any = ops != ops0;
+      alive = !any || wait(&bars.pvdone[slot], (ops - 1) & 1);
+      if (!alive) break;
+      tc_fence_after();
+      const bool whole = w.from == 0 && w.to == w.tiles;
+      const int64_t place = (int64_t)(2 * blockIdx.x + (w.from == 0 ? 1 : 0)) * TR + (RT == 2 ? slot * 128 : 0) + r;
+      if constexpr (RT == 2) {
+#pragma unroll 1
+        for (int c = 0; c < D / 16; ++c) {
+          uint32_t o[16];
+          tmem_ld_32x32b_x16(to + 16 * c, o);
+          tmem_ld_wait();
+          if (in)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+              float4 x = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
+              if (l != l) x = make_float4(l, l, l, l);
+              if (whole) finish_any<D>(p, at.out, 16 * c + i, x, m, l);
+              else *reinterpret_cast<float4 *>(p.ws_o + place * D + 16 * c + i) = x;
+            }
+        }
+        if (in && !whole) *reinterpret_cast<float2 *>(p.ws_ml + place * 2) = make_float2(m, l);
+      } else {
+        // the second warpgroup's share goes through its own and the first's query tile
+        float *other = (float *)qt;  // [128][D], 16 bytes a lane in rows of their own order
+        static_assert(C::QB * 2 >= 128 * D * 4, "query tiles hold the share");
+        if (slot == 0) mbar_arrive(&bars.done[0]);
+        if (slot == 1) {
+          alive = wait(&bars.done[0], parts & 1);
+          if (!alive) break;
+#pragma unroll 1
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld_32x32b_x16(to + 16 * c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+              *reinterpret_cast<float4 *>(other + (4 * c + i / 4) * 512 + r * 4) =
+                  any ? make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]))
+                      : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+          share_ml[r] = make_float2(m, l);
+          mbar_arrive(&bars.done[1]);
+        } else {
+          alive = wait(&bars.done[1], parts & 1);
+          if (!alive) break;
+          const float2 ml = share_ml[r];
+          const float M = fmaxf(m, ml.x), fa = m == -INFINITY ? 0.f : ex2(m - M), fb = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
+          const float L = l * fa + ml.y * fb;
+#pragma unroll 1
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld_32x32b_x16(to + 16 * c, o);
+            tmem_ld_wait();
+            if (in)
+#pragma unroll
+              for (int i = 0; i < 16; i += 4) {
+                const float4 y = *reinterpret_cast<const float4 *>(other + (4 * c + i / 4) * 512 + r * 4);
+                const float z = any ? fa : 0.f;
+                float4 x = make_float4(y.x * fb, y.y * fb, y.z * fb, y.w * fb);
+                if (any) {
+                  x.x += __uint_as_float(o[i]) * z, x.y += __uint_as_float(o[i + 1]) * z;
+                  x.z += __uint_as_float(o[i + 2]) * z, x.w += __uint_as_float(o[i + 3]) * z;
+                }
+                if (L != L) x = make_float4(L, L, L, L);
+                if (whole) finish_any<D>(p, at.out, 16 * c + i, x, M, L);
+                else *reinterpret_cast<float4 *>(p.ws_o + place * D + 16 * c + i) = x;
+              }
+          }
+          if (in && !whole) *reinterpret_cast<float2 *>(p.ws_ml + place * 2) = make_float2(M, L);
+          mbar_arrive(&bars.done[2]);
+        }
+        alive = wait(&bars.done[2], parts & 1);  // the query tiles are free again
+        if (!alive) break;
+      }
+      tc_fence_before();
+    }
+  } else if (warp < 12) {
+    // ================ codes to fp16 ================
+    reg_dec<DECODE_REGS>();
+    const int w4 = warp & 3, i128 = tid & 127;
+    // keys: unit kc of rows r0 + 4i; values: unit vc of keys 8 kg .. 8 kg + 7
+    const int kc = lane & 7, r0 = 32 * w4 + (lane >> 3), vc = (lane >> 3) + 4 * (w4 & 1), kg = (lane & 7) + 8 * (w4 >> 1);
+    uint32_t rawk[8][C::UW], rawv[8][C::UW];
+    uint32_t rs[(C::KNB + 1) / 2], rv[(C::KNB + 1) / 2];  // the scales of this thread's key (i128)
+    bool s_in = false;
+    uint32_t page[3] = {0, 0, 0};  // of the keys' two blocks of 16 and the values' one, of the tile that is read next
+
+    Part w;
+    bool more = begin(w);
+    uint32_t j = more ? w.from : 0;  // that tile
+    auto read_pages = [&]() {
+      if (!more) return;
+      const int32_t *table = p.tables + w.b * p.table_stride;
+      const int blk = (int)j * (KT / 16), blocks = (w.keys + 15) >> 4;
+      const int at[3] = {blk + 2 * w4, blk + 2 * w4 + 1, blk + (kg >> 1)};
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        page[i] = 0xFFFFFFFFu;
+        if (at[i] < blocks) page[i] = (uint32_t)__ldg(table + (at[i] >> page_blocks));
+      }
+    };
+    auto read = [&](uint32_t (&raw)[8][C::UW], const uint8_t *codes, bool values) {
+      const int blk = (int)j * (KT / 16), left = w.keys - (int)j * KT;
+      const uint8_t *base = codes + w.h * p.ch + (values ? vc : kc) * C::UB;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int bk = values ? blk + (kg >> 1) : blk + 2 * w4 + half;
+        const uint32_t pg = values ? page[2] : page[half];
+        const bool ok = pg < (uint64_t)p.pages;
+        const uint8_t *at = base + (uint64_t)(ok ? pg : 0) * p.cp + (bk & in_page) * 16 * p.ct;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int x = 4 * half + i, key = values ? 8 * kg + x : r0 + 4 * x;  // within the tile
+          if (ok && key < left) {
+            lds<C::UB>(at + (key & 15) * p.ct, raw[x]);
+          } else {
+#pragma unroll
+            for (int y = 0; y < C::UW; ++y) raw[x][y] = 0;
+          }
+        }
+      }
+    };
+    auto read_keys = [&]() {
+      read(rawk, p.k, false);
+      const int sb = (int)j * (KT / 16) + (i128 >> 4);
+      const uint32_t pg = lane < 16 ? page[0] : page[1];
+      const bool there = i128 < w.keys - (int)(j * KT);
+      s_in = there && pg < (uint64_t)p.pages;
+      if (there && !s_in) atomicOr(&g_device_error, DEVERR_BAD_INDEX);
+      if (s_in) {
+        const uint8_t *at = (const uint8_t *)p.ks + w.h * p.sh + (uint64_t)pg * p.sp + ((sb & in_page) * 16 + (i128 & 15)) * p.st;
+        load_scales<C::KNB>(at, p.e8m0, p.scale_vec, rs);
+        load_scales<C::KNB>(at + ((uint64_t)p.vs - (uint64_t)p.ks), p.e8m0, p.scale_vec, rv);
+      }
+    };
+    auto read_values = [&]() {  // then on to the next tile, whose pages are asked for
+      read(rawv, p.v, true);
+      if (++j == w.to) {
+        more = next(w);
+        j = w.from;
+      }
+      read_pages();
+    };
+    read_pages();
+    bool here = more;
+    if (here) {
+      read_keys();
+      read_values();
+    }
+    for (uint32_t n = 0; here; ++n) {
+      const uint32_t buf = n & 1, phase = ((n >> 1) - 1) & 1;
+      const bool again = more;  // a tile follows this one
+      const bool free_ = n < 2 || mbar_wait(&bars.kfree[buf], phase, abort_flag, WAIT_NS);
+      if (!BLK && !free_) break;
+      {
+        float kf[C::KNB], vf[C::KNB];
+        float *k_s = sc + (n & 3) * 3 * KT + i128;
+        widen<C::KNB>(rs, p.e8m0, kf);
+        widen<C::KNB>(rv, p.e8m0, vf);
+        if constexpr (!BLK) {
+          const float vsc = vf[0] < 0x1p-120f ? 0x1p-120f : vf[0];  // a scale of zero: weight without a value
+          k_s[0] = s_in ? kf[0] : 0.f, k_s[KT] = s_in ? lg2(vsc) : -INFINITY, k_s[2 * KT] = s_in ? __frcp_rn(vsc) : 0.f;
+        } else {
+          uint32_t km = 0, vm = 0;  // magnitudes order as integers, NaN above all
+#pragma unroll
+          for (int i = 0; i < C::NB; ++i)
+            km = max(km, __float_as_uint(kf[i]) & 0x7FFFFFFFu), vm = max(vm, __float_as_uint(vf[i]) & 0x7FFFFFFFu);
+          const int ke = RowRef<F>::exponent(km >> 16), ve = RowRef<F>::exponent(vm >> 16);
+          const bool kn = km > 0x7F800000u, vn = vm > 0x7F800000u;  // a row's NaN travels in its score or denominator
+          k_s[0] = !s_in ? 0.f : kn ? __uint_as_float(km) : RowRef<F>::value(ke);
+          k_s[KT] = s_in ? (float)(ve - 127) : -INFINITY;
+          k_s[2 * KT] = !s_in ? 0.f : vn ? __uint_as_float(vm) : RowRef<F>::inverse(ve);
+          const float ki = RowRef<F>::inverse(ke), vi = RowRef<F>::inverse(ve);
+#pragma unroll
+          for (int i = 0; i < C::NB; ++i) {
+            kratio[(buf * C::NB + i) * KT + i128] = __float2half_rn(s_in && !kn ? kf[i] * ki : 0.f);
+            vratio[(buf * C::NB + i) * KT + i128] = __float2half_rn(s_in && !vn ? vf[i] * vi : 0.f);
+          }
+        }
+        mbar_arrive(&bars.scfull[n & 3]);
+        if (BLK && !meet<1, WG>(free_)) break;  // the ratios are there for all
+      }
+      const uint32_t ka = smem_u32(kt + buf * C::KB);
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const int row = r0 + 4 * x;
+        uint32_t f[C::UD / 2];
+        if constexpr (C::bits == 8) {
+#pragma unroll
+          for (int y = 0; y < C::UW; ++y) decode4_8bit<F>(rawk[x][y], f[2 * y], f[2 * y + 1]);
+        } else {
+#pragma unroll
+          for (int y = 0; y < C::UW; ++y) decode8_4<F>(rawk[x][y], reinterpret_cast<uint32_t(&)[4]>(f[4 * y]));
+        }
+        if constexpr (BLK) {
+          const __half2 r2 = __half2half2(kratio[(buf * C::NB + kc * C::UD / 32) * KT + row]);
+#pragma unroll
+          for (int y = 0; y < C::UD / 2; ++y) f[y] = hmul2(f[y], *reinterpret_cast<const uint32_t *>(&r2));
+        }
+        if constexpr (C::UD == 16) {  // the upper units write their second half first: no bank twice
+          const bool sw = kc >= 4;
+          const uint32_t a0 = ka + tile_at(KT, row, 2 * kc), a1 = ka + tile_at(KT, row, 2 * kc + 1);
+          sts128(sw ? a1 : a0, sw ? f[4] : f[0], sw ? f[5] : f[1], sw ? f[6] : f[2], sw ? f[7] : f[3]);
+          sts128(sw ? a0 : a1, sw ? f[0] : f[4], sw ? f[1] : f[5], sw ? f[2] : f[6], sw ? f[3] : f[7]);
+        } else {
+          sts128(ka + tile_at(KT, row, kc), f[0], f[1], f[2], f[3]);
+        }
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&bars.kfull[buf]);
+      if (again) read_keys();
+
+      if (n >= 2 && !mbar_wait(&bars.vfree[buf], phase, abort_flag, WAIT_NS)) break;
+      const uint32_t va = smem_u32(vt + buf * C::VB);
+      uint32_t r4[4] = {0, 0, 0, 0};
+      if constexpr (BLK) lds<16>((const uint8_t *)&vratio[(buf * C::NB + vc * C::UD / 32) * KT + 8 * kg], r4);
+      constexpr int DW = 32 / C::bits;
+#pragma unroll
+      for (int y = 0; y < C::UW; ++y) {
+        uint32_t f[DW][4];  // [value][pair of keys]
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t w0 = rawv[2 * i][y], w1 = rawv[2 * i + 1][y];
+          if constexpr (C::bits == 8) {
+            decode4_8bit<F>(__byte_perm(w0, w1, 0x5140), f[0][i], f[1][i]);
+            decode4_8bit<F>(__byte_perm(w0, w1, 0x7362), f[2][i], f[3][i]);
+          } else if constexpr (F == B200_CACHE_INT4) {
+            uint32_t lo[4], hi[4];
+            decode8_4<F>(__byte_perm(w0, w1, 0x5410), lo);
+            decode8_4<F>(__byte_perm(w0, w1, 0x7632), hi);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) f[x][i] = lo[x], f[x + 4][i] = hi[x];
+          } else {
+            uint32_t ev[4], od[4];
+            decode8_4<F>((w0 & 0x0F0F0F0Fu) | ((w1 << 4) & 0xF0F0F0F0u), ev);
+            decode8_4<F>(((w0 >> 4) & 0x0F0F0F0Fu) | (w1 & 0xF0F0F0F0u), od);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) f[2 * x][i] = ev[x], f[2 * x + 1][i] = od[x];
+          }
+          if constexpr (BLK)
+#pragma unroll
+            for (int x = 0; x < DW; ++x) f[x][i] = hmul2(f[x][i], r4[i]);
+        }
+#pragma unroll
+        for (int x = 0; x < DW; ++x) {
+          const int d = vc * C::UD + y * DW + x;
+          sts128(va + tile_at(D, d, kg), f[x][0], f[x][1], f[x][2], f[x][3]);
+        }
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&bars.vfull[buf]);
+      here = again;
+      if (here) read_values();
+    }
+  } else {
+    reg_dec<ISSUE_REGS>();
+    if (warp == 12 && lane == 0) {
+    // ================ MMA issuer ================
+    constexpr uint32_t id_s = idesc_f16(0, 128, KT), id_o = idesc_f16(0, 128, D);
+    uint32_t parity = 0;  // bits: qfull[0, 1], pfull[0, 1]
+    auto wait_flip = [&](uint64_t *bar, uint32_t bit) {
+      const bool ok = mbar_wait(bar, (parity >> bit) & 1, abort_flag, WAIT_NS);
+      parity ^= 1u << bit;
+      return ok;
+    };
+    // operation o of a part: RT = 2: slot o & 1 of tile o >> 1; RT = 1: slot (n0 + o) & 1 of tile o
+    auto scores = [&](uint32_t n, uint32_t s, bool first) {
+      if (first && !wait_flip(&bars.qfull[s], s)) return false;
+      if (!mbar_wait(&bars.kfull[n & 1], (n >> 1) & 1, abort_flag, WAIT_NS)) return false;
+      tc_fence_after();
+      const uint64_t qa = sw128_kmajor_desc(qt + s * C::QB), kb = sw128_kmajor_desc(kt + (n & 1) * C::KB);
+#pragma unroll
+      for (int x = 0; x < D / 16; ++x) {  // 128 x 128 bytes a 64 values, 32 bytes a step
+        const uint64_t at = (x >> 2) * (128 * 128 / 16) + 2 * (x & 3);
+        mma_f16_ss(tmem + s * 128, qa + at, kb + at, id_s, x != 0);
+      }
+      mma_commit(&bars.sfull[s]);
+      if (RT == 1 || s == 1) mma_commit(&bars.kfree[n & 1]);
+      return true;
+    };
+    auto values = [&](uint32_t n, uint32_t s, bool first) {
+      if (!mbar_wait(&bars.vfull[n & 1], (n >> 1) & 1, abort_flag, WAIT_NS) || !wait_flip(&bars.pfull[s], 2 + s)) return false;
+      tc_fence_after();
+      const uint64_t vb = sw128_kmajor_desc(vt + (n & 1) * C::VB);
+#pragma unroll
+      for (int x = 0; x < KT / 16; ++x)
+        mma_f16_ts(tmem + 256 + s * D, tmem + s * 128 + 8 * x, vb + (x >> 2) * (D * 128 / 16) + 2 * (x & 3), id_o, !first || x != 0);
+      mma_commit(&bars.pvdone[s]);
+      if (RT == 1 || s == 1) mma_commit(&bars.vfree[n & 1]);
+      return true;
+    };
+    Part w;
+    uint32_t n0 = 0;
+    bool ok = true;
+    for (bool more = begin(w); more && ok; more = next(w)) {
+      const uint32_t count = (w.to - w.from) * RT;
+      auto step = [&](uint32_t o, bool second) {
+        const uint32_t n = n0 + (RT == 2 ? o >> 1 : o), s = RT == 2 ? o & 1 : n & 1;
+        return second ? values(n, s, o < 2) : scores(n, s, o < 2);
+      };
+      for (uint32_t o = 0; o < count + 2 && ok; ++o) {  // scores run two operations ahead of values
+        if (o >= 2) ok = step(o - 2, true);
+        if (o < count && ok) ok = step(o, false);
+      }
+      n0 += w.to - w.from;
+    }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 12) tmem_dealloc(tmem, 512);
+}
+
+// Joins the segments that were cut: a CTA takes 32 rows of one.
+template <int D>
+__global__ void __launch_bounds__(256) join_kernel(const Params p, int tile_rows, uint32_t ctas) {
+  __shared__ uint32_t prefix[MAX_ENTRIES + 1];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  scan_entries(p, tile_rows, prefix);
+  __syncthreads();
+  const int entries = p.batch * p.row_tiles, chunks = tile_rows / 32;
+  const uint32_t total = prefix[entries] * (uint32_t)p.kv_heads, per = max(1u, (total + ctas - 1) / ctas);
+  for (int x = blockIdx.x; x < entries * p.kv_heads * chunks; x += gridDim.x) {
+    const int chunk = x % chunks, s = x / chunks, e = s / p.kv_heads, h = s - e * p.kv_heads;
+    const uint32_t tiles = prefix[e + 1] - prefix[e], seg0 = prefix[e] * p.kv_heads + h * tiles;
+    if (tiles == 0) continue;
+    const uint32_t c0 = seg0 / per, c1 = (seg0 + tiles - 1) / per;
+    if (c0 == c1) continue;
+    const int b = e / p.row_tiles, rt = e - b * p.row_tiles;
+    for (int i = threadIdx.x; i < 32 * (D / 4); i += 256) {
+      const int rr = chunk * 32 + i / (D / 4), d = (i % (D / 4)) * 4, row = rt * tile_rows + rr;
+      if (row >= p.rows) continue;
+      float M = -INFINITY, L = 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+      for (uint32_t c = c0; c <= c1; ++c) {
+        const int64_t sl = (int64_t)(2 * c + (c == c0 ? 1 : 0)) * tile_rows + rr;
+        const float2 ml = *(const float2 *)(p.ws_ml + sl * 2);
+        join<D>(o, M, L, p.ws_o + sl * D + d, ml.x, ml.y);
+      }
+      if (L != L) o = make_float4(L, L, L, L);
+      finish_any<D>(p, row_at(p, b, h, row).out, d, o, M, L);
+    }
+  }
+}
+
+// ---- per-(device, stream) workspace of cut segments ------------------------------------------------
+struct Workspace {
+  float *o = nullptr, *ml = nullptr;
+};
+static std::mutex g_ws_mutex;
+static std::map<std::pair<int, cudaStream_t>, Workspace> g_ws;
+
+static int32_t workspace_for(cudaStream_t stream, int sms, Workspace &out) {
+  int dev = 0;
+  B200_CUDA_TRY(cudaGetDevice(&dev));
+  std::lock_guard<std::mutex> lock(g_ws_mutex);
+  auto it = g_ws.find({dev, stream});
+  out = Workspace();
+  if (it != g_ws.end()) {
+    out = it->second;
+    return B200_OK;
+  }
+  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+  B200_CUDA_TRY(cudaStreamIsCapturing(stream, &cs));
+  if (cs != cudaStreamCaptureStatusNone) return B200_OK;  // nothing can be allocated now: whole segments
+  const size_t rows = (size_t)sms * 2 * 256;
+  uint8_t *base = nullptr;
+  B200_CUDA_TRY(cudaMalloc((void **)&base, rows * (128 + 2) * 4));
+  Workspace w;
+  w.o = (float *)base, w.ml = (float *)(base + rows * 128 * 4);
+  g_ws[{dev, stream}] = w;
+  out = w;
+  return B200_OK;
+}
+
+template <typename K>
+static int32_t launch_pdl(K kernel, int grid, int block, size_t smem, cudaStream_t stream, const Params &p) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3((unsigned)block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  B200_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, p));
+  return B200_OK;
+}
+
+template <int F, int D, int RT, bool BLK>
+static int32_t launch_t(Params &p, cudaStream_t stream) {
+  using C = Cfg<F, D, BLK>;
+  constexpr int TR = 128 * RT;
+  int sms = 0;
+  B200_CUDA_TRY(device_sms(&sms));
+  p.row_tiles = (p.rows + TR - 1) / TR;
+  if (p.row_tiles > MAX_ENTRIES)
+    return b200_set_error(B200_ERR_UNSUPPORTED, "cache_attention: too many query rows (%d of a key head)", p.rows);
+  const int64_t cap = p.lengths != nullptr ? ((int64_t)p.max_pages << p.page_shift) : p.fixed;
+  const int64_t tiles = (cap + KT - 1) / KT * p.kv_heads * p.row_tiles;  // of a request
+  if (tiles > (1 << 30)) return b200_set_error(B200_ERR_UNSUPPORTED, "cache_attention: too many keys for one launch");
+  int at_once = MAX_ENTRIES / p.row_tiles;
+  if (tiles > 0 && tiles * at_once > (1 << 30)) at_once = (int)((1 << 30) / tiles);
+  Workspace w;
+  if (int32_t rc = workspace_for(stream, sms, w)) return rc;
+  B200_CUDA_TRY((ensure_dynamic_smem<attn_mma_kernel<F, D, RT, BLK>>(C::SMEM)));
+  const Params base = p;
+  for (int b = 0; b < base.batch; b += at_once) {  // a launch for each run of requests that the scan has room for
+    p = base;
+    p.batch = base.batch - b < at_once ? base.batch - b : at_once;
+    if (b > 0) {
+      const int64_t rows = (int64_t)b * p.per_request * p.q_heads;
+      p.q = (const uint16_t *)p.q + b * p.qsr;
+      p.tables += b * p.table_stride, p.lengths += b;
+      p.out = (uint16_t *)p.out + rows * D;
+      if (p.lse != nullptr) p.lse += rows;
+      p.row0 += rows;
+    }
+    p.ws_o = w.o, p.ws_ml = w.ml;
+    int64_t grid = tiles * p.batch;
+    if (grid > sms) grid = sms;
+    if (grid < 1) grid = 1;
+    if (int32_t rc = launch_pdl(attn_mma_kernel<F, D, RT, BLK>, (int)grid, THREADS, C::SMEM, stream, p)) return rc;
+    if (w.o == nullptr) continue;
+    if (p.po != nullptr) {  // the next kernel joins
+      const uint32_t n = (uint32_t)((p.fixed + KT - 1) / KT), total = n * (uint32_t)(p.kv_heads * p.row_tiles);
+      p.cuts = {w.o, w.ml, n, (uint32_t)((total + grid - 1) / grid), TR};
+    } else {
+      const int64_t chunks = (int64_t)p.batch * p.row_tiles * p.kv_heads * (TR / 32);
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3((unsigned)(chunks < 8 * sms ? chunks : 8 * sms));
+      cfg.blockDim = dim3(256);
+      cfg.stream = stream;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      attr[0].val.programmaticStreamSerializationAllowed = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      B200_CUDA_TRY(cudaLaunchKernelEx(&cfg, join_kernel<D>, (const Params)p, TR, (uint32_t)grid));
+    }
+  }
+  return B200_OK;
+}
+
+template <int F>
+static int32_t launch_d(Params &p, int dim, bool blk, cudaStream_t stream) {
+  const bool two = p.rows > 128;
+  if (dim == 64) {
+    if (two) return blk ? launch_t<F, 64, 2, true>(p, stream) : launch_t<F, 64, 2, false>(p, stream);
+    return blk ? launch_t<F, 64, 1, true>(p, stream) : launch_t<F, 64, 1, false>(p, stream);
+  }
+  if (two) return blk ? launch_t<F, 128, 2, true>(p, stream) : launch_t<F, 128, 2, false>(p, stream);
+  return blk ? launch_t<F, 128, 1, true>(p, stream) : launch_t<F, 128, 1, false>(p, stream);
+}
+#ifdef DEV_ONE
+static int32_t launch_f(Params &p, int fmt, int dim, bool blk, cudaStream_t stream) { return launch_t<1, 128, 2, false>(p, stream); }
+#else
+static int32_t launch_f(Params &p, int fmt, int dim, bool blk, cudaStream_t stream) {
+  switch (fmt) {
+    case B200_CACHE_INT8: return launch_d<B200_CACHE_INT8>(p, dim, blk, stream);
+    case B200_CACHE_FP8E4M3: return launch_d<B200_CACHE_FP8E4M3>(p, dim, blk, stream);
+    case B200_CACHE_INT4: return launch_d<B200_CACHE_INT4>(p, dim, blk, stream);
+    default: return launch_d<B200_CACHE_FP4_E2M1>(p, dim, blk, stream);
+  }
+}
+
+#endif
+}  // namespace mma
+
+bool mma_supported(const Params &p, int dim) { return dim <= 128 && p.rows > 16; }
+
+int32_t launch_mma(Params &p, int q_dtype, int fmt, int dim, bool blk, cudaStream_t stream) {
+  p.q_bf16 = q_dtype == B200_DT_BF16;
+  return mma::launch_f(p, fmt, dim, blk, stream);
+}
+
+}  // namespace cattn
+}  // namespace b200

@@ -307,7 +307,9 @@ int32_t b200_device_status(int32_t device, uint32_t *flags, int32_t clear) {
   unsigned int co = 0, ca = 0;
   if (int32_t rc = cache_ops_device_error(&co, clear != 0)) return rc;
   if (int32_t rc = cache_attn_device_error(&ca, clear != 0)) return rc;
-  *flags = v | u | w | z | dd | mxe | co | ca;
+  unsigned int cm = 0;
+  if (int32_t rc = cache_attn_mma_device_error(&cm, clear != 0)) return rc;
+  *flags = v | u | w | z | dd | mxe | co | ca | cm;
   if (clear != 0 && (*flags & 1u) != 0)  // a kernel gave up mid-way: its split-tile tickets may be half counted
     if (int32_t rc = mx_reset_tickets()) return rc;
   return B200_OK;

@@ -95,6 +95,7 @@ int32_t launch_wait_flag(const int32_t *flag, int32_t expect, int64_t max_spins,
 int32_t check_cache(const b200_cache_desc *c);
 int32_t cache_ops_device_error(unsigned int *v, bool clear);
 int32_t cache_attn_device_error(unsigned int *v, bool clear);
+int32_t cache_attn_mma_device_error(unsigned int *v, bool clear);
 
 }  // namespace b200
 
