@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
         widen<C::KNB>(rv[k], p.e8m0, vf);
         if constexpr (!BLK) {
           const float vsc = vf[0] < 0x1p-120f ? 0x1p-120f : vf[0];  // a scale of zero: weight without a value
-          lvi[key] = in ? make_float2(lg2(vsc), __frcp_rn(vsc)) : make_float2(-INFINITY, 0.f);
+          lvi[key] = in ? make_float2(lg2(vsc), vsc == vsc ? __frcp_rn(vsc) : 0.f) : make_float2(-INFINITY, 0.f);
           ks[key] = in ? kf[0] : 0.f;
         } else {
           uint32_t top = 0;  // magnitudes order as integers, NaN above all
@@ -345,9 +345,9 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
           for (int i = 0; i < C::NB; ++i) top = max(top, __float_as_uint(vf[i]) & 0x7FFFFFFFu);
           const int e = RowRef<F>::exponent(top >> 16);
           float inv = RowRef<F>::inverse(e);
-          // the row's NaN travels in its denominator, which only rows that see it take
-          lvi[key] = in ? make_float2((float)(e - 127), top > 0x7F800000u ? __uint_as_float(top) : inv)
-                        : make_float2(-INFINITY, 0.f);
+          // the row's NaN travels in its scores, which rows that do not see it drop
+          lvi[key] = !in ? make_float2(-INFINITY, 0.f)
+                     : top > 0x7F800000u ? make_float2(__uint_as_float(top), 0.f) : make_float2((float)(e - 127), inv);
           const bool use = in && top <= 0x7F800000u;
           __half *vk = vr + (key & ~7) + C::row_of(key & 7);  // ratios in the order of the instruction's rows
 #pragma unroll
@@ -545,8 +545,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             pr[x] = ex2(s[n][x] - (x & 1 ? m1 : m0));
-            // an unseen key's scale may be NaN
-            if (pr[x] != 0.f) l[n][x & 1] = fmaf(pr[x], x < 2 ? lvi0.y : lvi1.y, l[n][x & 1]);
+            l[n][x & 1] = fmaf(pr[x], x < 2 ? lvi0.y : lvi1.y, l[n][x & 1]);
           }
           bp[n][0] = movmatrix_trans(pack_f16(pr[0], pr[1]));
           bp[n][1] = movmatrix_trans(pack_f16(pr[2], pr[3]));

@@ -39,9 +39,9 @@ namespace mma {
 
 constexpr int KT = 128;                      // keys of a tile
 constexpr int WG = 128, THREADS = 4 * WG;
+// 128 x (2 x 168 + 120 + 56) = 512 x 128, the registers that the block is launched with
+constexpr int SOFT_REGS = 168, DECODE_REGS = 120, ISSUE_REGS = 56;
 constexpr int MAX_ENTRIES = 1024;
-// 128 x (2 x 176 + 104 + 56) = 512 x 128, the registers that the block is launched with
-constexpr int SOFT_REGS = 176, DECODE_REGS = 104, ISSUE_REGS = 56;
 constexpr uint64_t WAIT_NS = 2000000000ull;
 
 template <int F, int D, bool BLK>
@@ -52,9 +52,46 @@ struct Cfg {
   static constexpr int NB = D / 32, KNB = BLK ? NB : 1;
   static constexpr int QB = 128 * D * 2, KB = KT * D * 2, VB = KT * D * 2;
   static constexpr int RING = 4;                                            // tiles of scales
-  static constexpr int SC = RING * KT * 12, RATIO = BLK ? 2 * NB * KT * 2 : 0;
+  static constexpr int SC = RING * KT * 12, RATIO = 2 * KNB * KT * 2;
+  // scale exponents of a tile may differ by this for its codes to take them with all their bits in fp16
+  static constexpr int SPAN = bits == 4 ? 24 : 11;
+  static constexpr bool FOLD = BLK || bits == 4;                            // key codes always take their scales
   static constexpr int SMEM = 1024 + 2 * QB + 2 * KB + 2 * VB + SC + 2 * RATIO + 256;
 };
+
+// Pairs of fp32 in a register pair: one instruction for two.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t y;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ uint64_t pair(uint32_t a, uint32_t b) {
+  uint64_t y;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "r"(a), "r"(b));
+  return y;
+}
+__device__ __forceinline__ void unpair(uint64_t x, uint32_t &a, uint32_t &b) { asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(x)); }
+__device__ __forceinline__ void unpair(uint64_t x, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t y;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
+  return y;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t y;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+  return y;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t y;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+  return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
 
 __device__ __forceinline__ float2 wide2(const Params &p, uint32_t w) {
   if (p.q_bf16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
@@ -111,8 +148,6 @@ struct Bars {
   uint64_t done[3];  // one row tile: the first warpgroup's products; the second's share; that share's reading
 };
 
-template <int REGS> __device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS)); }
-template <int REGS> __device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS)); }
 // All N threads of barrier ID meet; whether every one of them is `ok`.
 template <int ID, int N>
 __device__ __forceinline__ bool meet(bool ok) {
@@ -124,6 +159,29 @@ __device__ __forceinline__ bool meet(bool ok) {
       : "r"((uint32_t)ok), "n"(ID), "n"(N)
       : "memory");
   return all != 0;
+}
+
+template <int REGS> __device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS)); }
+template <int REGS> __device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS)); }
+
+// tcgen05.mma and its commit by one lane of a converged warp.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\telect.sync _|q, 0xFFFFFFFF;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\telect.sync _|q, 0xFFFFFFFF;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t *bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\telect.sync _|q, 0xFFFFFFFF;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
+      : "memory");
 }
 
 // Byte of 16-byte chunk g (8 values) of row r in a K-major tile of `rows` rows, 64 values a swizzled row.
@@ -146,6 +204,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
   __shared__ Bars bars;
   __shared__ uint32_t prefix[MAX_ENTRIES + 1];
   __shared__ float2 share_ml[RT == 1 ? 128 : 1];
+  __shared__ float4 tile_s[C::RING];   // (key scale, log2 of the value scale, its inverse, keys differ) of a tile
+  __shared__ uint32_t span_s[2][4][5]; // of a warp's keys: largest and smallest exponents, any to be looked at one by one
   __shared__ uint32_t tmem_slot;
   __shared__ uint32_t abort_word;
   volatile uint32_t *abort_flag = &abort_word;
@@ -252,36 +312,33 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
       if (first < w.to) {
         // q: fp16, scaled by a power of two, in the order that the keys' codes come out decoded
         const uint16_t *src = (const uint16_t *)p.q + at.q;
-        uint32_t raw[4];
+        uint32_t raw[D / 8][4];
         float top = 0.f;
-        auto load8 = [&](int g) {
-          if (!in) raw[0] = raw[1] = raw[2] = raw[3] = 0;
-          else if (p.q_vec) lds<16>((const uint8_t *)(src + 8 * g), raw);
+#pragma unroll
+        for (int g = 0; g < D / 8; ++g) {
+          if (!in) raw[g][0] = raw[g][1] = raw[g][2] = raw[g][3] = 0;
+          else if (p.q_vec) lds<16>((const uint8_t *)(src + 8 * g), raw[g]);
           else
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              raw[i] = (uint32_t)src[8 * g + 2 * i] | ((uint32_t)src[8 * g + 2 * i + 1] << 16);
-        };
-#pragma unroll 4
-        for (int g = 0; g < D / 8; ++g) {
-          load8(g);
+            for (int i = 0; i < 4; ++i) raw[g][i] = (uint32_t)src[8 * g + 2 * i] | ((uint32_t)src[8 * g + 2 * i + 1] << 16);
+        }
+#pragma unroll
+        for (int g = 0; g < D / 8; ++g)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float2 v = wide2(p, raw[i]);
+            const float2 v = wide2(p, raw[g][i]);
             top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
           }
-        }
         const int ex = min(max((int)(__float_as_uint(top) >> 23), 1), 253);
-        const float down = __uint_as_float((uint32_t)(254 - ex) << 23);
-        qs = p.scale * __uint_as_float((uint32_t)ex << 23);
+        const float down = copysignf(__uint_as_float((uint32_t)(254 - ex) << 23), p.scale);
+        qs = fabsf(p.scale) * __uint_as_float((uint32_t)ex << 23);  // not negative: the largest score is the largest product's
         const uint32_t qa = smem_u32(qt + slot * C::QB);
-#pragma unroll 4
+#pragma unroll
         for (int g = 0; g < D / 8; ++g) {
-          load8(g);
           float x[8];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float2 v = wide2(p, raw[i]);
+            const float2 v = wide2(p, raw[g][i]);
             x[2 * i] = v.x * down, x[2 * i + 1] = v.y * down;
           }
           uint32_t y[4];
@@ -299,36 +356,67 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
         alive = wait(&bars.scfull[n & 3], (n >> 2) & 1) && wait(&bars.sfull[slot], ops & 1);
         if (!alive) break;
         tc_fence_after();
-        const float4 *k4 = (const float4 *)(sc + (n & 3) * 3 * KT), *l4 = k4 + KT / 4, *i4 = l4 + KT / 4;
-        uint32_t u[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(ts + 32 * c, u[c]);
-        tmem_ld_wait();
-        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float4 k = k4[8 * c + i], a = l4[8 * c + i];
-            const float ks[4] = {k.x, k.y, k.z, k.w}, as[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const float y = fmaf(__uint_as_float(u[c][4 * i + x]) * ks[x], qs, as[x]);
-              u[c][4 * i + x] = __float_as_uint(y);
-              top[x] = fmaxf(top[x], y);
-            }
+        const ulonglong2 *k4 = (const ulonglong2 *)(sc + (n & 3) * 3 * KT), *l4 = k4 + KT / 4, *i4 = l4 + KT / 4;
+        const float4 tile = tile_s[n & 3];
+        const bool edge = p.causal && __any_sync(0xFFFFFFFFu, (int)(j * KT + KT) > lim);  // keys that a row does not see
+        // keys one by one: a tile that ends early, whose scales are far apart, or that some rows see in part
+        const bool each = edge || tile.w != 0.f;
+        const float qt_s = qs * tile.x;
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, most;
+        uint32_t xa[32], xb[32];
+        // `f` on the four chunks of 32 scores, the next chunk on its way meanwhile
+        auto chunks = [&](auto f) {
+          tmem_ld_32x32b_x32(ts, xa);
+#pragma unroll 1
+          for (int c = 0; c < 4; c += 2) {
+            tmem_ld_wait();
+            tmem_ld_32x32b_x32(ts + 32 * c + 32, xb);
+            f(xa, c);
+            tmem_ld_wait();
+            if (c == 0) tmem_ld_32x32b_x32(ts + 64, xa);
+            f(xb, c + 1);
           }
-        if (p.causal && __any_sync(0xFFFFFFFFu, (int)(j * KT + KT) > lim)) {  // keys that this row does not see
-          top[0] = top[1] = top[2] = top[3] = -INFINITY;
+        };
+        auto largest = [&](const uint32_t (&x)[32]) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int i = 0; i < 32; i += 2)
+            top[(i >> 1) & 3] = max3(top[(i >> 1) & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+        };
+        if (each) {  // u of every key in its score's place
+          const uint64_t qs2 = pair(qs, qs);
+          chunks([&](uint32_t(&x)[32], int c) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              if ((int)(j * KT) + 32 * c + i >= lim) u[c][i] = 0xFF800000u;
-              top[i & 3] = fmaxf(top[i & 3], __uint_as_float(u[c][i]));
+            for (int i = 0; i < 8; ++i) {
+              const ulonglong2 k = k4[8 * c + i], a = l4[8 * c + i];
+              unpair(fma2(mul2(pair(x[4 * i], x[4 * i + 1]), k.x), qs2, a.x), x[4 * i], x[4 * i + 1]);
+              unpair(fma2(mul2(pair(x[4 * i + 2], x[4 * i + 3]), k.y), qs2, a.y), x[4 * i + 2], x[4 * i + 3]);
             }
+            if (edge)
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if ((int)(j * KT) + 32 * c + i >= lim) x[i] = 0xFF800000u;
+            largest(x);
+            tmem_st_32x32b_x32(ts + 32 * c, x);
+          });
+          tmem_st_wait();
+          most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        } else if (C::FOLD || p.e8m0) {  // one scale for all: it goes into the exponential's argument
+          chunks([&](uint32_t(&x)[32], int) { largest(x); });
+          most = fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), qt_s, tile.y);
+        } else {  // scales of 8 bits times codes of 8 would lose some in fp16: products take their key's scale
+          chunks([&](uint32_t(&x)[32], int c) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const ulonglong2 k = k4[8 * c + i];
+              unpair(mul2(pair(x[4 * i], x[4 * i + 1]), k.x), x[4 * i], x[4 * i + 1]);
+              unpair(mul2(pair(x[4 * i + 2], x[4 * i + 3]), k.y), x[4 * i + 2], x[4 * i + 3]);
+            }
+            largest(x);
+            tmem_st_32x32b_x32(ts + 32 * c, x);
+          });
+          tmem_st_wait();
+          most = fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), qt_s, tile.y);
         }
-        const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         const bool up = most > m + LAZY;
         if (__any_sync(0xFFFFFFFFu, up)) {
           const float f = !up || m == -INFINITY ? 1.f : ex2(m - most);
@@ -349,25 +437,48 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
           }
         }
         const float mm = m == -INFINITY ? 0.f : m - BIAS;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        // p of chunk c goes over the scores of chunk c / 2, which have been read
+        uint64_t sum[2] = {0, 0};
+        if (each) {
+          const uint64_t mm2 = pair(-mm, -mm);
+          chunks([&](uint32_t(&x)[32], int c) {
+            uint32_t pk[16];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t pk[16];
+            for (int i = 0; i < 8; ++i) {
+              const ulonglong2 v = i4[8 * c + i];
+              float e[4];
+              unpair(add2(pair(x[4 * i], x[4 * i + 1]), mm2), e[0], e[1]);
+              unpair(add2(pair(x[4 * i + 2], x[4 * i + 3]), mm2), e[2], e[3]);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float4 v = i4[8 * c + i];
-            const float vs[4] = {v.x, v.y, v.z, v.w};
-            float e[4];
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              e[x] = ex2(__uint_as_float(u[c][4 * i + x]) - mm);
-              if (e[x] != 0.f) sum[x] = fmaf(e[x], vs[x], sum[x]);  // an unseen key's scale may be NaN
+              for (int y = 0; y < 4; ++y) e[y] = ex2(e[y]);
+              sum[0] = fma2(pair(e[0], e[1]), v.x, sum[0]);
+              sum[1] = fma2(pair(e[2], e[3]), v.y, sum[1]);
+              pk[2 * i] = pack_f16(e[0], e[1]), pk[2 * i + 1] = pack_f16(e[2], e[3]);
             }
-            pk[2 * i] = pack_f16(e[0], e[1]), pk[2 * i + 1] = pack_f16(e[2], e[3]);
-          }
-          tmem_st_32x32b_x16(ts + 16 * c, pk);
+            tmem_st_32x32b_x16(ts + 16 * c, pk);
+          });
+        } else {
+          const uint64_t qs2 = pair(qt_s, qt_s), a2 = pair(tile.y - mm, tile.y - mm);
+          chunks([&](uint32_t(&x)[32], int c) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              float e[4];
+              unpair(fma2(pair(x[4 * i], x[4 * i + 1]), qs2, a2), e[0], e[1]);
+              unpair(fma2(pair(x[4 * i + 2], x[4 * i + 3]), qs2, a2), e[2], e[3]);
+#pragma unroll
+              for (int y = 0; y < 4; ++y) e[y] = ex2(e[y]);
+              sum[0] = add2(pair(e[0], e[1]), sum[0]);
+              sum[1] = add2(pair(e[2], e[3]), sum[1]);
+              pk[2 * i] = pack_f16(e[0], e[1]), pk[2 * i + 1] = pack_f16(e[2], e[3]);
+            }
+            tmem_st_32x32b_x16(ts + 16 * c, pk);
+          });
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        float s0, s1, s2, s3;
+        unpair(sum[0], s0, s1);
+        unpair(sum[1], s2, s3);
+        l = fmaf((s0 + s1) + (s2 + s3), each ? 1.f : tile.z, l);
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(&bars.pfull[slot]);
@@ -381,20 +492,38 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
       const bool whole = w.from == 0 && w.to == w.tiles;
       const int64_t place = (int64_t)(2 * blockIdx.x + (w.from == 0 ? 1 : 0)) * TR + (RT == 2 ? slot * 128 : 0) + r;
       if constexpr (RT == 2) {
+        const bool plain = whole && p.po == nullptr && p.fo == nullptr;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll 1
-        for (int c = 0; c < D / 16; ++c) {
-          uint32_t o[16];
-          tmem_ld_32x32b_x16(to + 16 * c, o);
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          __syncwarp();
+          tmem_ld_32x32b_x32(to + 32 * c, o);
           tmem_ld_wait();
-          if (in)
+          if (!in) {
+          } else if (plain) {
 #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
+            for (int i = 0; i < 32; i += 8) {
+              uint32_t y[4];
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const float f0 = __uint_as_float(o[i + 2 * x]) * inv, f1 = __uint_as_float(o[i + 2 * x + 1]) * inv;
+                const __nv_bfloat162 h = __floats2bfloat162_rn(f0, f1);
+                y[x] = p.q_bf16 ? *reinterpret_cast<const uint32_t *>(&h) : pack_f16(f0, f1);
+              }
+              *reinterpret_cast<uint4 *>((uint16_t *)p.out + at.out * D + 32 * c + i) = make_uint4(y[0], y[1], y[2], y[3]);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
               float4 x = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
               if (l != l) x = make_float4(l, l, l, l);
-              if (whole) finish_any<D>(p, at.out, 16 * c + i, x, m, l);
-              else *reinterpret_cast<float4 *>(p.ws_o + place * D + 16 * c + i) = x;
+              if (whole) finish_any<D>(p, at.out, 32 * c + i, x, m, l);
+              else *reinterpret_cast<float4 *>(p.ws_o + place * D + 32 * c + i) = x;
             }
+          }
         }
+        if (in && plain && p.lse != nullptr) p.lse[at.out] = l == 0.f ? -INFINITY : (m - BIAS + log2f(l)) * 0.69314718055994531f;
         if (in && !whole) *reinterpret_cast<float2 *>(p.ws_ml + place * 2) = make_float2(m, l);
       } else {
         // the second warpgroup's share goes through its own and the first's query tile
@@ -528,34 +657,56 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
       const uint32_t buf = n & 1, phase = ((n >> 1) - 1) & 1;
       const bool again = more;  // a tile follows this one
       const bool free_ = n < 2 || mbar_wait(&bars.kfree[buf], phase, abort_flag, WAIT_NS);
-      if (!BLK && !free_) break;
+      // Scales. Where the tile's exponents lie close together, key and value codes take theirs relative to the
+      // tile's (exactly, but for rounding products of 8-bit codes and bfloat16 scales to fp16) and the rows
+      // need one of each; where not, or where a key is missing or NaN, relative to their own key's, and every
+      // key leaves what the rows need of it.
+      const bool fold = C::FOLD || p.e8m0;
+      float kf[C::KNB], vf[C::KNB];
+      widen<C::KNB>(rs, p.e8m0, kf);
+      widen<C::KNB>(rv, p.e8m0, vf);
+      uint32_t km = 0, vm = 0, kl = 0x7F800000u, vl = 0x7F800000u;  // magnitudes order as integers, NaN above all
+#pragma unroll
+      for (int i = 0; i < C::KNB; ++i) {
+        const uint32_t a = __float_as_uint(kf[i]) & 0x7FFFFFFFu, b = __float_as_uint(vf[i]) & 0x7FFFFFFFu;
+        km = max(km, a), vm = max(vm, b);
+        if (a > 0x0E000000u) kl = min(kl, a);  // blocks of zeros have scales of 2^-100 and no say
+        if (b > 0x0E000000u) vl = min(vl, b);
+      }
+      const bool kn = km >= 0x7F800000u, vn = vm >= 0x7F800000u;
       {
-        float kf[C::KNB], vf[C::KNB];
+        uint32_t *sp = span_s[buf][w4];
+        const uint32_t x0 = __reduce_max_sync(0xFFFFFFFFu, s_in ? km >> 23 : 0), x1 = __reduce_min_sync(0xFFFFFFFFu, s_in ? kl >> 23 : 255);
+        const uint32_t x2 = __reduce_max_sync(0xFFFFFFFFu, s_in ? vm >> 23 : 0), x3 = __reduce_min_sync(0xFFFFFFFFu, s_in ? vl >> 23 : 255);
+        const bool any = __any_sync(0xFFFFFFFFu, !s_in || kn || vn);
+        if (lane == 0) sp[0] = x0, sp[1] = x1, sp[2] = x2, sp[3] = x3, sp[4] = any;
+      }
+      if (!meet<1, WG>(free_)) break;
+      {
+        uint32_t kx = 0, ki = 255, vx = 0, vi = 255;
+        bool each = false;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t *sp = span_s[buf][i];
+          kx = max(kx, sp[0]), ki = min(ki, sp[1]), vx = max(vx, sp[2]), vi = min(vi, sp[3]), each |= sp[4] != 0;
+        }
+        each = each || (fold && (int)(kx - ki) > C::SPAN) || (int)(vx - vi) > C::SPAN;
+        const int ke = RowRef<F>::exponent((each ? km >> 23 : kx) << 7), ve = RowRef<F>::exponent((each ? vm >> 23 : vx) << 7);
         float *k_s = sc + (n & 3) * 3 * KT + i128;
-        widen<C::KNB>(rs, p.e8m0, kf);
-        widen<C::KNB>(rv, p.e8m0, vf);
-        if constexpr (!BLK) {
-          const float vsc = vf[0] < 0x1p-120f ? 0x1p-120f : vf[0];  // a scale of zero: weight without a value
-          k_s[0] = s_in ? kf[0] : 0.f, k_s[KT] = s_in ? lg2(vsc) : -INFINITY, k_s[2 * KT] = s_in ? __frcp_rn(vsc) : 0.f;
-        } else {
-          uint32_t km = 0, vm = 0;  // magnitudes order as integers, NaN above all
+        const float ks = fold ? RowRef<F>::value(ke) : kf[0], nan = __uint_as_float(0x7FC00000u);
+        // a NaN scale: in the score, which rows that do not see the key drop
+        k_s[0] = s_in && !kn ? ks : 0.f;
+        k_s[KT] = !s_in ? -INFINITY : kn || vn ? nan : (float)(ve - 127);
+        k_s[2 * KT] = s_in && !vn ? RowRef<F>::inverse(ve) : 0.f;
+        if (i128 == 0) tile_s[n & 3] = make_float4(fold ? ks : 1.f, (float)(ve - 127), RowRef<F>::inverse(ve), each ? 1.f : 0.f);
+        const float kr = RowRef<F>::inverse(ke), vr = RowRef<F>::inverse(ve);
 #pragma unroll
-          for (int i = 0; i < C::NB; ++i)
-            km = max(km, __float_as_uint(kf[i]) & 0x7FFFFFFFu), vm = max(vm, __float_as_uint(vf[i]) & 0x7FFFFFFFu);
-          const int ke = RowRef<F>::exponent(km >> 16), ve = RowRef<F>::exponent(vm >> 16);
-          const bool kn = km > 0x7F800000u, vn = vm > 0x7F800000u;  // a row's NaN travels in its score or denominator
-          k_s[0] = !s_in ? 0.f : kn ? __uint_as_float(km) : RowRef<F>::value(ke);
-          k_s[KT] = s_in ? (float)(ve - 127) : -INFINITY;
-          k_s[2 * KT] = !s_in ? 0.f : vn ? __uint_as_float(vm) : RowRef<F>::inverse(ve);
-          const float ki = RowRef<F>::inverse(ke), vi = RowRef<F>::inverse(ve);
-#pragma unroll
-          for (int i = 0; i < C::NB; ++i) {
-            kratio[(buf * C::NB + i) * KT + i128] = __float2half_rn(s_in && !kn ? kf[i] * ki : 0.f);
-            vratio[(buf * C::NB + i) * KT + i128] = __float2half_rn(s_in && !vn ? vf[i] * vi : 0.f);
-          }
+        for (int i = 0; i < C::KNB; ++i) {
+          kratio[(buf * C::KNB + i) * KT + i128] = __float2half_rn(s_in && !kn ? kf[i] * kr : 0.f);
+          vratio[(buf * C::KNB + i) * KT + i128] = __float2half_rn(s_in && !vn ? vf[i] * vr : 0.f);
         }
         mbar_arrive(&bars.scfull[n & 3]);
-        if (BLK && !meet<1, WG>(free_)) break;  // the ratios are there for all
+        meet<2, WG>(true);  // the ratios are there for all
       }
       const uint32_t ka = smem_u32(kt + buf * C::KB);
 #pragma unroll
@@ -569,8 +720,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
 #pragma unroll
           for (int y = 0; y < C::UW; ++y) decode8_4<F>(rawk[x][y], reinterpret_cast<uint32_t(&)[4]>(f[4 * y]));
         }
-        if constexpr (BLK) {
-          const __half2 r2 = __half2half2(kratio[(buf * C::NB + kc * C::UD / 32) * KT + row]);
+        if (fold) {
+          const __half2 r2 = __half2half2(kratio[(buf * C::KNB + (BLK ? kc * C::UD / 32 : 0)) * KT + row]);
 #pragma unroll
           for (int y = 0; y < C::UD / 2; ++y) f[y] = hmul2(f[y], *reinterpret_cast<const uint32_t *>(&r2));
         }
@@ -589,8 +740,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
 
       if (n >= 2 && !mbar_wait(&bars.vfree[buf], phase, abort_flag, WAIT_NS)) break;
       const uint32_t va = smem_u32(vt + buf * C::VB);
-      uint32_t r4[4] = {0, 0, 0, 0};
-      if constexpr (BLK) lds<16>((const uint8_t *)&vratio[(buf * C::NB + vc * C::UD / 32) * KT + 8 * kg], r4);
+      uint32_t r4[4];
+      lds<16>((const uint8_t *)&vratio[(buf * C::KNB + (BLK ? vc * C::UD / 32 : 0)) * KT + 8 * kg], r4);
       constexpr int DW = 32 / C::bits;
 #pragma unroll
       for (int y = 0; y < C::UW; ++y) {
@@ -614,9 +765,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
 #pragma unroll
             for (int x = 0; x < 4; ++x) f[2 * x][i] = ev[x], f[2 * x + 1][i] = od[x];
           }
-          if constexpr (BLK)
 #pragma unroll
-            for (int x = 0; x < DW; ++x) f[x][i] = hmul2(f[x][i], r4[i]);
+          for (int x = 0; x < DW; ++x) f[x][i] = hmul2(f[x][i], r4[i]);
         }
 #pragma unroll
         for (int x = 0; x < DW; ++x) {
@@ -631,46 +781,50 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
     }
   } else {
     reg_dec<ISSUE_REGS>();
-    if (warp == 12 && lane == 0) {
-    // ================ MMA issuer ================
+    if (warp == 12) {
+      // ================ MMA issuer: the warp stays together, so that descriptors live in uniform registers ================
     constexpr uint32_t id_s = idesc_f16(0, 128, KT), id_o = idesc_f16(0, 128, D);
     uint32_t parity = 0;  // bits: qfull[0, 1], pfull[0, 1]
+    auto wait = [&](uint64_t *bar, uint32_t phase) {
+      return __all_sync(0xFFFFFFFFu, mbar_wait(bar, phase, abort_flag, WAIT_NS)) != 0;
+    };
     auto wait_flip = [&](uint64_t *bar, uint32_t bit) {
-      const bool ok = mbar_wait(bar, (parity >> bit) & 1, abort_flag, WAIT_NS);
+      const bool ok = wait(bar, (parity >> bit) & 1);
       parity ^= 1u << bit;
       return ok;
     };
+    const uint64_t q0 = sw128_kmajor_desc(qt), k0 = sw128_kmajor_desc(kt), v0 = sw128_kmajor_desc(vt);
     // operation o of a part: RT = 2: slot o & 1 of tile o >> 1; RT = 1: slot (n0 + o) & 1 of tile o
     auto scores = [&](uint32_t n, uint32_t s, bool first) {
       if (first && !wait_flip(&bars.qfull[s], s)) return false;
-      if (!mbar_wait(&bars.kfull[n & 1], (n >> 1) & 1, abort_flag, WAIT_NS)) return false;
+      if (!wait(&bars.kfull[n & 1], (n >> 1) & 1)) return false;
       tc_fence_after();
-      const uint64_t qa = sw128_kmajor_desc(qt + s * C::QB), kb = sw128_kmajor_desc(kt + (n & 1) * C::KB);
+      const uint64_t qa = q0 + s * (C::QB / 16), kb = k0 + (n & 1) * (C::KB / 16);
 #pragma unroll
       for (int x = 0; x < D / 16; ++x) {  // 128 x 128 bytes a 64 values, 32 bytes a step
         const uint64_t at = (x >> 2) * (128 * 128 / 16) + 2 * (x & 3);
-        mma_f16_ss(tmem + s * 128, qa + at, kb + at, id_s, x != 0);
+        mma_ss(tmem + s * 128, qa + at, kb + at, id_s, x != 0);
       }
-      mma_commit(&bars.sfull[s]);
-      if (RT == 1 || s == 1) mma_commit(&bars.kfree[n & 1]);
+      commit(&bars.sfull[s]);
+      if (RT == 1 || s == 1) commit(&bars.kfree[n & 1]);
       return true;
     };
     auto values = [&](uint32_t n, uint32_t s, bool first) {
-      if (!mbar_wait(&bars.vfull[n & 1], (n >> 1) & 1, abort_flag, WAIT_NS) || !wait_flip(&bars.pfull[s], 2 + s)) return false;
+      if (!wait(&bars.vfull[n & 1], (n >> 1) & 1) || !wait_flip(&bars.pfull[s], 2 + s)) return false;
       tc_fence_after();
-      const uint64_t vb = sw128_kmajor_desc(vt + (n & 1) * C::VB);
+      const uint64_t vb = v0 + (n & 1) * (C::VB / 16);
 #pragma unroll
       for (int x = 0; x < KT / 16; ++x)
-        mma_f16_ts(tmem + 256 + s * D, tmem + s * 128 + 8 * x, vb + (x >> 2) * (D * 128 / 16) + 2 * (x & 3), id_o, !first || x != 0);
-      mma_commit(&bars.pvdone[s]);
-      if (RT == 1 || s == 1) mma_commit(&bars.vfree[n & 1]);
+        mma_ts(tmem + 256 + s * D, tmem + s * 128 + 8 * x, vb + (x >> 2) * (D * 128 / 16) + 2 * (x & 3), id_o, !first || x != 0);
+      commit(&bars.pvdone[s]);
+      if (RT == 1 || s == 1) commit(&bars.vfree[n & 1]);
       return true;
     };
     Part w;
     uint32_t n0 = 0;
     bool ok = true;
     for (bool more = begin(w); more && ok; more = next(w)) {
-      const uint32_t count = (w.to - w.from) * RT;
+      const uint32_t tiles = __shfl_sync(0xFFFFFFFFu, w.to - w.from, 0), count = tiles * RT;
       auto step = [&](uint32_t o, bool second) {
         const uint32_t n = n0 + (RT == 2 ? o >> 1 : o), s = RT == 2 ? o & 1 : n & 1;
         return second ? values(n, s, o < 2) : scores(n, s, o < 2);
@@ -679,7 +833,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
         if (o >= 2) ok = step(o - 2, true);
         if (o < count && ok) ok = step(o, false);
       }
-      n0 += w.to - w.from;
+      n0 += tiles;
     }
     }
   }
@@ -836,7 +990,7 @@ static int32_t launch_d(Params &p, int dim, bool blk, cudaStream_t stream) {
   return blk ? launch_t<F, 128, 1, true>(p, stream) : launch_t<F, 128, 1, false>(p, stream);
 }
 #ifdef DEV_ONE
-static int32_t launch_f(Params &p, int fmt, int dim, bool blk, cudaStream_t stream) { return launch_t<1, 128, 2, false>(p, stream); }
+static int32_t launch_f(Params &p, int fmt, int dim, bool blk, cudaStream_t stream) { return launch_t<DEV_F, DEV_D, DEV_RT, DEV_B>(p, stream); }
 #else
 static int32_t launch_f(Params &p, int fmt, int dim, bool blk, cudaStream_t stream) {
   switch (fmt) {
