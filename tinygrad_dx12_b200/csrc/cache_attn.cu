@@ -847,9 +847,10 @@ static int32_t attention(const b200_cache_desc *c, const b200_attention_args *a,
     Params f = p;  // every row of the batch against the prefix: one request of batch * queries tokens
     f.tables = a->prefix, f.table_stride = 0, f.max_pages = (int)a->prefix_pages;
     f.fixed = a->prefix_length, f.batch = 1, f.queries = (int)(a->batch * a->queries), f.rows = f.queries * p.group;
+    f.exact_keys = a->lse != nullptr;
     f.po = (float *)a->scratch, f.pm = f.po + all_rows * dim, f.pl = f.pm + all_rows;
     if (int32_t rc = run(f)) return rc;
-    p.fo = f.po, p.fm = f.pm, p.fl = f.pl, p.cuts = f.cuts;
+    p.fo = f.po, p.fm = f.pm, p.fl = f.pl;
   }
   p.tables = a->tables, p.table_stride = a->table_stride, p.max_pages = (int)a->max_pages, p.lengths = a->lengths;
   p.batch = (int)a->batch, p.queries = (int)a->queries, p.rows = p.queries * p.group, p.causal = 1;

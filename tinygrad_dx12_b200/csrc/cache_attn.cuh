@@ -13,15 +13,6 @@ using namespace cache;
 constexpr float LAZY = 4.f;          // u may pass the running maximum by this before it moves
 constexpr float BIAS = 15.f - LAZY;  // p = 2^(u - m + BIAS) uses fp16 up to 2^15, so small weights keep their bits
 
-// How the many-row kernel cut the prefix: segment (row tile, key head) s of `tiles` tiles covers
-// tiles s * tiles .. of runs of `per`; one within a run is in fo / fm / fl, of the others run c's share
-// is in slot 2c + (it begins there), `rows` rows each.
-struct Cuts {
-  const float *o, *ml;  // null: nothing is cut
-  uint32_t tiles, per;
-  int rows;
-};
-
 struct Params {
   const void *q;
   int64_t qsr, qsb, qsh;  // strides of q: request, token, head
@@ -31,6 +22,7 @@ struct Params {
   uint32_t cp, ct, sp, st;
   int64_t ch, sh;
   int e8m0, scale_vec, q_vec, q_bf16;
+  int exact_keys;  // a prefix's share of results that come with logarithms
   int64_t pages;
   int page_shift, kv_heads, group;
   const int32_t *tables;
@@ -48,8 +40,7 @@ struct Params {
   float *lse;
   float *po, *pm, *pl;
   const float *fo, *fm, *fl;  // partials of the shared prefix, joined at the end
-  int64_t row0;               // rows before these in fo, fm, fl and cuts
-  Cuts cuts;                  // where the many-row kernel left those of prefix segments that it cut
+  int64_t row0;               // rows before these in fo, fm, fl
   // split segments
   float *ws_o, *ws_ml;
   uint32_t *tickets;
@@ -169,23 +160,7 @@ __device__ __forceinline__ void finish(const Params &p, int64_t row, int d, floa
     return;
   }
   if (p.fo != nullptr) {
-    uint32_t c0 = 0, c1 = 0, r = 0;
-    if (p.cuts.o != nullptr) {
-      const int tok = (int)((p.row0 + row) / p.q_heads), head = (int)(p.row0 + row - (int64_t)tok * p.q_heads), h = head / p.group;
-      const uint32_t pr = (uint32_t)tok * p.group + (head - h * p.group);  // among the prefix's rows of a key head
-      const uint32_t rt = pr / p.cuts.rows, s0 = (rt * p.kv_heads + h) * p.cuts.tiles;
-      r = pr - rt * p.cuts.rows, c0 = s0 / p.cuts.per, c1 = (s0 + p.cuts.tiles - 1) / p.cuts.per;
-    }
-    if (c0 == c1) {
-      join<D>(o, m, l, p.fo + (p.row0 + row) * D + d, p.fm[p.row0 + row], p.fl[p.row0 + row]);
-    } else {
-#pragma unroll 4
-      for (uint32_t c = c0; c <= c1; ++c) {
-        const int64_t sl = (int64_t)(2 * c + (c == c0 ? 1 : 0)) * p.cuts.rows + r;
-        const float2 ml = *(const float2 *)(p.cuts.ml + sl * 2);
-        join<D>(o, m, l, p.cuts.o + sl * D + d, ml.x, ml.y);
-      }
-    }
+    join<D>(o, m, l, p.fo + (p.row0 + row) * D + d, p.fm[p.row0 + row], p.fl[p.row0 + row]);
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;  // no key seen: zeros
   T *dst = (T *)p.out + row * D + d;
@@ -197,7 +172,7 @@ __device__ __forceinline__ void finish(const Params &p, int64_t row, int d, floa
 
 // The many-row kernel (cache_attn_mma.cu): rows of p in tiles of 128 or 256 on the tcgen05 cores.
 bool mma_supported(const Params &p, int dim);
-int32_t launch_mma(Params &p, int q_dtype, int fmt, int dim, bool blk, cudaStream_t stream);  // fills p.cuts
+int32_t launch_mma(Params &p, int q_dtype, int fmt, int dim, bool blk, cudaStream_t stream);
 
 }  // namespace cattn
 }  // namespace b200

@@ -19,8 +19,7 @@
 //
 // Tiles of all (row tile, key head) segments are laid end to end and cut into equal runs, one per CTA.
 // A segment within a run is finished there; the others leave their share (numerators, maximum,
-// denominator) in the CTA's two workspace slots, and are joined by the kernel after it: the one over
-// the requests' own keys for a prefix, join_kernel for a chunk.
+// denominator) in the CTA's two workspace slots, and join_kernel adds those up.
 #include <map>
 #include <mutex>
 
@@ -144,7 +143,7 @@ struct Part {
 };
 
 struct Bars {
-  uint64_t qfull[2], sfull[2], pfull[2], pvdone[2], kfull[2], kfree[2], vfull[2], vfree[2], scfull[4];
+  uint64_t qfull[2], sfull[2], pfull[2][2], pvdone[2], kfull[2], kfree[2], vfull[2], vfree[2], scfull[4];
   uint64_t done[3];  // one row tile: the first warpgroup's products; the second's share; that share's reading
 };
 
@@ -184,6 +183,14 @@ __device__ __forceinline__ void commit(uint64_t *bar) {
       : "memory");
 }
 
+// Value d (a multiple of four) of row `place` (slot * rows + row) of the shares of cut segments: four values of
+// all rows side by side, as a thread a row writes them.
+template <int D>
+__device__ __forceinline__ int64_t cut_at(int64_t place, int rows, int d) {
+  const int64_t slot = place / rows;
+  return (slot * (D / 4) + d / 4) * rows * 4 + (place - slot * rows) * 4;
+}
+
 // Byte of 16-byte chunk g (8 values) of row r in a K-major tile of `rows` rows, 64 values a swizzled row.
 __device__ __forceinline__ uint32_t tile_at(int rows, int r, int g) {
   return (uint32_t)((g >> 3) * rows * 128 + r * 128 + (((g & 7) ^ (r & 7)) << 4));
@@ -217,7 +224,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
   constexpr int TR = 128 * RT;  // rows of a segment
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bars.qfull[i], WG), mbar_init(&bars.sfull[i], 1), mbar_init(&bars.pfull[i], WG), mbar_init(&bars.pvdone[i], 1);
+      mbar_init(&bars.qfull[i], WG), mbar_init(&bars.sfull[i], 1), mbar_init(&bars.pfull[i][0], WG), mbar_init(&bars.pfull[i][1], WG), mbar_init(&bars.pvdone[i], 1);
       mbar_init(&bars.kfull[i], WG), mbar_init(&bars.kfree[i], 1), mbar_init(&bars.vfull[i], WG), mbar_init(&bars.vfree[i], 1);
     }
     for (int i = 0; i < 4; ++i) mbar_init(&bars.scfull[i], WG);
@@ -284,6 +291,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
     enter(w);
     return split || (w.e * (uint32_t)heads + w.h) % gridDim.x == blockIdx.x ? true : next(w);
   };
+  // Key codes take their scales before the products. With 8-bit codes and bfloat16 scales that rounds their
+  // 15 bits to fp16's 11, 2^-12 at random: far below a bfloat16 result's half unit of 2^-8, but not below what
+  // fp16 results and logarithms keep, whose scores take their key's scale instead.
+  const bool fold = C::FOLD || p.e8m0 || (p.q_bf16 && p.lse == nullptr && p.exact_keys == 0);
   const int page_blocks = p.page_shift - 4;
   const uint32_t in_page = (1u << page_blocks) - 1;
 
@@ -311,41 +322,44 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
       const uint32_t ops0 = ops;
       if (first < w.to) {
         // q: fp16, scaled by a power of two, in the order that the keys' codes come out decoded
-        const uint16_t *src = (const uint16_t *)p.q + at.q;
-        uint32_t raw[D / 8][4];
-        float top = 0.f;
+        // (a warp does its own 32 rows, whole rows at a time)
+        constexpr int LPR = D / 8, RPI = 32 / LPR;  // lanes of a row, rows at once
+        const int g = lane % LPR;
+        uint32_t raw[LPR][4];
 #pragma unroll
-        for (int g = 0; g < D / 8; ++g) {
-          if (!in) raw[g][0] = raw[g][1] = raw[g][2] = raw[g][3] = 0;
-          else if (p.q_vec) lds<16>((const uint8_t *)(src + 8 * g), raw[g]);
+        for (int x = 0; x < LPR; ++x) {
+          const int rr = x * RPI + lane / LPR;
+          const int64_t q0 = __shfl_sync(0xFFFFFFFFu, at.q, rr);
+          const bool there = __shfl_sync(0xFFFFFFFFu, (int)in, rr) != 0;
+          const uint16_t *src = (const uint16_t *)p.q + q0 + 8 * g;
+          if (!there) raw[x][0] = raw[x][1] = raw[x][2] = raw[x][3] = 0;
+          else if (p.q_vec) lds<16>((const uint8_t *)src, raw[x]);
           else
 #pragma unroll
-            for (int i = 0; i < 4; ++i) raw[g][i] = (uint32_t)src[8 * g + 2 * i] | ((uint32_t)src[8 * g + 2 * i + 1] << 16);
+            for (int i = 0; i < 4; ++i) raw[x][i] = (uint32_t)src[2 * i] | ((uint32_t)src[2 * i + 1] << 16);
         }
-#pragma unroll
-        for (int g = 0; g < D / 8; ++g)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 v = wide2(p, raw[g][i]);
-            top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
-          }
-        const int ex = min(max((int)(__float_as_uint(top) >> 23), 1), 253);
-        const float down = copysignf(__uint_as_float((uint32_t)(254 - ex) << 23), p.scale);
-        qs = fabsf(p.scale) * __uint_as_float((uint32_t)ex << 23);  // not negative: the largest score is the largest product's
         const uint32_t qa = smem_u32(qt + slot * C::QB);
 #pragma unroll
-        for (int g = 0; g < D / 8; ++g) {
-          float x[8];
+        for (int x = 0; x < LPR; ++x) {
+          float f[8], top = 0.f;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float2 v = wide2(p, raw[g][i]);
-            x[2 * i] = v.x * down, x[2 * i + 1] = v.y * down;
+            const float2 v = wide2(p, raw[x][i]);
+            f[2 * i] = v.x, f[2 * i + 1] = v.y;
+            top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
           }
+#pragma unroll
+          for (int y = 1; y < LPR; y <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, y));
+          const int ex = min(max((int)(__float_as_uint(top) >> 23), 1), 253);
+          const float down = copysignf(__uint_as_float((uint32_t)(254 - ex) << 23), p.scale);
+          // not negative: the largest score is the largest product's
+          const float up = __shfl_sync(0xFFFFFFFFu, fabsf(p.scale) * __uint_as_float((uint32_t)ex << 23), (lane % RPI) * LPR);
+          if (lane / RPI == x) qs = up;
           uint32_t y[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            y[i] = F == B200_CACHE_INT4 ? pack_f16(x[i], x[i + 4]) : pack_f16(x[2 * i], x[2 * i + 1]);
-          sts128(qa + tile_at(128, r, g), y[0], y[1], y[2], y[3]);
+            y[i] = F == B200_CACHE_INT4 ? pack_f16(f[i] * down, f[i + 4] * down) : pack_f16(f[2 * i] * down, f[2 * i + 1] * down);
+          sts128(qa + tile_at(128, (warp & 3) * 32 + x * RPI + lane / LPR, g), y[0], y[1], y[2], y[3]);
         }
         fence_proxy_async_smem();
         tc_fence_before();
@@ -400,10 +414,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
           });
           tmem_st_wait();
           most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-        } else if (C::FOLD || p.e8m0) {  // one scale for all: it goes into the exponential's argument
+        } else if (fold) {  // one scale for all: it goes into the exponential's argument
           chunks([&](uint32_t(&x)[32], int) { largest(x); });
           most = fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), qt_s, tile.y);
-        } else {  // scales of 8 bits times codes of 8 would lose some in fp16: products take their key's scale
+        } else {  // products take their key's scale
           chunks([&](uint32_t(&x)[32], int c) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -437,6 +451,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
           }
         }
         const float mm = m == -INFINITY ? 0.f : m - BIAS;
+        // the second product may begin with the first 64 keys
+        auto half_done = [&]() {
+          tmem_st_wait();
+          tc_fence_before();
+          mbar_arrive(&bars.pfull[slot][0]);
+        };
         // p of chunk c goes over the scores of chunk c / 2, which have been read
         uint64_t sum[2] = {0, 0};
         if (each) {
@@ -456,6 +476,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
               pk[2 * i] = pack_f16(e[0], e[1]), pk[2 * i + 1] = pack_f16(e[2], e[3]);
             }
             tmem_st_32x32b_x16(ts + 16 * c, pk);
+            if (c == 1) half_done();
           });
         } else {
           const uint64_t qs2 = pair(qt_s, qt_s), a2 = pair(tile.y - mm, tile.y - mm);
@@ -473,6 +494,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
               pk[2 * i] = pack_f16(e[0], e[1]), pk[2 * i + 1] = pack_f16(e[2], e[3]);
             }
             tmem_st_32x32b_x16(ts + 16 * c, pk);
+            if (c == 1) half_done();
           });
         }
         float s0, s1, s2, s3;
@@ -481,7 +503,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
         l = fmaf((s0 + s1) + (s2 + s3), each ? 1.f : tile.z, l);
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(&bars.pfull[slot]);
+        mbar_arrive(&bars.pfull[slot][1]);
       }
       if (!alive) break;
       n0 += w.to - w.from;
@@ -494,14 +516,14 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
       if constexpr (RT == 2) {
         const bool plain = whole && p.po == nullptr && p.fo == nullptr;
         const float inv = l == 0.f ? 0.f : 1.f / l;
+        const uint32_t rowbuf = smem_u32(qt + slot * C::QB);
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
           __syncwarp();
           tmem_ld_32x32b_x32(to + 32 * c, o);
           tmem_ld_wait();
-          if (!in) {
-          } else if (plain) {
+          if (plain) {  // through this row's place in the query tile, so that whole rows are stored
 #pragma unroll
             for (int i = 0; i < 32; i += 8) {
               uint32_t y[4];
@@ -511,17 +533,30 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
                 const __nv_bfloat162 h = __floats2bfloat162_rn(f0, f1);
                 y[x] = p.q_bf16 ? *reinterpret_cast<const uint32_t *>(&h) : pack_f16(f0, f1);
               }
-              *reinterpret_cast<uint4 *>((uint16_t *)p.out + at.out * D + 32 * c + i) = make_uint4(y[0], y[1], y[2], y[3]);
+              sts128(rowbuf + r * (D * 2) + (((4 * c + i / 8) ^ (r & (D / 8 - 1))) << 4), y[0], y[1], y[2], y[3]);
             }
-          } else {
+          } else if (in) {
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
               float4 x = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
               if (l != l) x = make_float4(l, l, l, l);
               if (whole) finish_any<D>(p, at.out, 32 * c + i, x, m, l);
-              else *reinterpret_cast<float4 *>(p.ws_o + place * D + 32 * c + i) = x;
+              else *reinterpret_cast<float4 *>(p.ws_o + cut_at<D>(place, TR, 32 * c + i)) = x;
             }
           }
+        }
+        if (plain) {
+          constexpr int LPR = D / 8, RPI = 32 / LPR;
+          __syncwarp();
+#pragma unroll 4
+          for (int x = 0; x < LPR; ++x) {
+            const int rr = x * RPI + lane / LPR, row_ = (warp & 3) * 32 + rr, g = lane % LPR;
+            const int64_t to_row = __shfl_sync(0xFFFFFFFFu, at.out, rr);
+            const bool there = __shfl_sync(0xFFFFFFFFu, (int)in, rr) != 0;
+            const uint4 y = *reinterpret_cast<const uint4 *>(qt + slot * C::QB + row_ * (D * 2) + ((g ^ (row_ & (D / 8 - 1))) << 4));
+            if (there) *reinterpret_cast<uint4 *>((uint16_t *)p.out + to_row * D + 8 * g) = y;
+          }
+          __syncwarp();
         }
         if (in && plain && p.lse != nullptr) p.lse[at.out] = l == 0.f ? -INFINITY : (m - BIAS + log2f(l)) * 0.69314718055994531f;
         if (in && !whole) *reinterpret_cast<float2 *>(p.ws_ml + place * 2) = make_float2(m, l);
@@ -569,7 +604,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
                 }
                 if (L != L) x = make_float4(L, L, L, L);
                 if (whole) finish_any<D>(p, at.out, 16 * c + i, x, M, L);
-                else *reinterpret_cast<float4 *>(p.ws_o + place * D + 16 * c + i) = x;
+                else *reinterpret_cast<float4 *>(p.ws_o + cut_at<D>(place, TR, 16 * c + i)) = x;
               }
           }
           if (in && !whole) *reinterpret_cast<float2 *>(p.ws_ml + place * 2) = make_float2(M, L);
@@ -661,7 +696,6 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
       // tile's (exactly, but for rounding products of 8-bit codes and bfloat16 scales to fp16) and the rows
       // need one of each; where not, or where a key is missing or NaN, relative to their own key's, and every
       // key leaves what the rows need of it.
-      const bool fold = C::FOLD || p.e8m0;
       float kf[C::KNB], vf[C::KNB];
       widen<C::KNB>(rs, p.e8m0, kf);
       widen<C::KNB>(rv, p.e8m0, vf);
@@ -784,7 +818,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
     if (warp == 12) {
       // ================ MMA issuer: the warp stays together, so that descriptors live in uniform registers ================
     constexpr uint32_t id_s = idesc_f16(0, 128, KT), id_o = idesc_f16(0, 128, D);
-    uint32_t parity = 0;  // bits: qfull[0, 1], pfull[0, 1]
+    uint32_t parity = 0;  // bits: qfull[0, 1], both of pfull[0], both of pfull[1]
     auto wait = [&](uint64_t *bar, uint32_t phase) {
       return __all_sync(0xFFFFFFFFu, mbar_wait(bar, phase, abort_flag, WAIT_NS)) != 0;
     };
@@ -797,7 +831,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
     // operation o of a part: RT = 2: slot o & 1 of tile o >> 1; RT = 1: slot (n0 + o) & 1 of tile o
     auto scores = [&](uint32_t n, uint32_t s, bool first) {
       if (first && !wait_flip(&bars.qfull[s], s)) return false;
-      if (!wait(&bars.kfull[n & 1], (n >> 1) & 1)) return false;
+      if ((RT == 1 || s == 0) && !wait(&bars.kfull[n & 1], (n >> 1) & 1)) return false;
       tc_fence_after();
       const uint64_t qa = q0 + s * (C::QB / 16), kb = k0 + (n & 1) * (C::KB / 16);
 #pragma unroll
@@ -810,12 +844,17 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
       return true;
     };
     auto values = [&](uint32_t n, uint32_t s, bool first) {
-      if (!wait(&bars.vfull[n & 1], (n >> 1) & 1) || !wait_flip(&bars.pfull[s], 2 + s)) return false;
-      tc_fence_after();
+      if ((RT == 1 || s == 0) && !wait(&bars.vfull[n & 1], (n >> 1) & 1)) return false;
       const uint64_t vb = v0 + (n & 1) * (C::VB / 16);
 #pragma unroll
-      for (int x = 0; x < KT / 16; ++x)
-        mma_ts(tmem + 256 + s * D, tmem + s * 128 + 8 * x, vb + (x >> 2) * (D * 128 / 16) + 2 * (x & 3), id_o, !first || x != 0);
+      for (int h = 0; h < 2; ++h) {  // 64 keys at a time
+        if (!wait(&bars.pfull[s][h], (parity >> (2 + s)) & 1)) return false;
+        tc_fence_after();
+#pragma unroll
+        for (int x = 4 * h; x < 4 * h + 4; ++x)
+          mma_ts(tmem + 256 + s * D, tmem + s * 128 + 8 * x, vb + (x >> 2) * (D * 128 / 16) + 2 * (x & 3), id_o, !first || x != 0);
+      }
+      parity ^= 4u << s;
       commit(&bars.pvdone[s]);
       if (RT == 1 || s == 1) commit(&bars.vfree[n & 1]);
       return true;
@@ -844,7 +883,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
   if (warp == 12) tmem_dealloc(tmem, 512);
 }
 
-// Joins the segments that were cut: a CTA takes 32 rows of one.
+// Joins the segments that were cut: a CTA takes 32 rows of one and as many of their values, a thread four.
 template <int D>
 __global__ void __launch_bounds__(256) join_kernel(const Params p, int tile_rows, uint32_t ctas) {
   __shared__ uint32_t prefix[MAX_ENTRIES + 1];
@@ -852,7 +891,7 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p, int tile_rows
   asm volatile("griddepcontrol.wait;" ::: "memory");
   scan_entries(p, tile_rows, prefix);
   __syncthreads();
-  const int entries = p.batch * p.row_tiles, chunks = tile_rows / 32;
+  const int entries = p.batch * p.row_tiles, chunks = tile_rows / 32 * (D / 32);
   const uint32_t total = prefix[entries] * (uint32_t)p.kv_heads, per = max(1u, (total + ctas - 1) / ctas);
   for (int x = blockIdx.x; x < entries * p.kv_heads * chunks; x += gridDim.x) {
     const int chunk = x % chunks, s = x / chunks, e = s / p.kv_heads, h = s - e * p.kv_heads;
@@ -861,20 +900,24 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p, int tile_rows
     const uint32_t c0 = seg0 / per, c1 = (seg0 + tiles - 1) / per;
     if (c0 == c1) continue;
     const int b = e / p.row_tiles, rt = e - b * p.row_tiles;
-    for (int i = threadIdx.x; i < 32 * (D / 4); i += 256) {
-      const int rr = chunk * 32 + i / (D / 4), d = (i % (D / 4)) * 4, row = rt * tile_rows + rr;
-      if (row >= p.rows) continue;
-      float M = -INFINITY, L = 0.f;
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
-      for (uint32_t c = c0; c <= c1; ++c) {
-        const int64_t sl = (int64_t)(2 * c + (c == c0 ? 1 : 0)) * tile_rows + rr;
-        const float2 ml = *(const float2 *)(p.ws_ml + sl * 2);
-        join<D>(o, M, L, p.ws_o + sl * D + d, ml.x, ml.y);
-      }
-      if (L != L) o = make_float4(L, L, L, L);
-      finish_any<D>(p, row_at(p, b, h, row).out, d, o, M, L);
+    const int rr = chunk / (D / 32) * 32 + (threadIdx.x & 31), d = chunk % (D / 32) * 32 + (threadIdx.x >> 5) * 4;
+    const int row = rt * tile_rows + rr;
+    if (row >= p.rows) continue;
+    auto place = [&](uint32_t c) { return (int64_t)(2 * c + (c == c0 ? 1 : 0)) * tile_rows + rr; };
+    float M = -INFINITY, L = 0.f;
+#pragma unroll 8
+    for (uint32_t c = c0; c <= c1; ++c) M = fmaxf(M, ((const float2 *)p.ws_ml)[place(c)].x);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (uint32_t c = c0; c <= c1; ++c) {
+      const float2 ml = ((const float2 *)p.ws_ml)[place(c)];
+      const float4 y = *(const float4 *)(p.ws_o + cut_at<D>(place(c), tile_rows, d));
+      const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
+      o.x += y.x * f, o.y += y.y * f, o.z += y.z * f, o.w += y.w * f;
+      L += ml.y * f;
     }
+    if (L != L) o = make_float4(L, L, L, L);
+    finish_any<D>(p, row_at(p, b, h, row).out, d, o, M, L);
   }
 }
 
@@ -959,22 +1002,17 @@ static int32_t launch_t(Params &p, cudaStream_t stream) {
     if (grid < 1) grid = 1;
     if (int32_t rc = launch_pdl(attn_mma_kernel<F, D, RT, BLK>, (int)grid, THREADS, C::SMEM, stream, p)) return rc;
     if (w.o == nullptr) continue;
-    if (p.po != nullptr) {  // the next kernel joins
-      const uint32_t n = (uint32_t)((p.fixed + KT - 1) / KT), total = n * (uint32_t)(p.kv_heads * p.row_tiles);
-      p.cuts = {w.o, w.ml, n, (uint32_t)((total + grid - 1) / grid), TR};
-    } else {
-      const int64_t chunks = (int64_t)p.batch * p.row_tiles * p.kv_heads * (TR / 32);
-      cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = dim3((unsigned)(chunks < 8 * sms ? chunks : 8 * sms));
-      cfg.blockDim = dim3(256);
-      cfg.stream = stream;
-      cudaLaunchAttribute attr[1];
-      attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-      attr[0].val.programmaticStreamSerializationAllowed = 1;
-      cfg.attrs = attr;
-      cfg.numAttrs = 1;
-      B200_CUDA_TRY(cudaLaunchKernelEx(&cfg, join_kernel<D>, (const Params)p, TR, (uint32_t)grid));
-    }
+    const int64_t chunks = (int64_t)p.batch * p.row_tiles * p.kv_heads * (TR / 32) * (D / 32);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(chunks < 8 * sms ? chunks : 8 * sms));
+    cfg.blockDim = dim3(256);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    B200_CUDA_TRY(cudaLaunchKernelEx(&cfg, join_kernel<D>, (const Params)p, TR, (uint32_t)grid));
   }
   return B200_OK;
 }
