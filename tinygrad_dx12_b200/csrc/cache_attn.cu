@@ -47,7 +47,7 @@ int32_t cache_attn_device_error(unsigned int *v, bool clear) {
 namespace cattn {
 
 constexpr int WARPS = 8, THREADS = WARPS * 32, STAGES = 2;
-constexpr int MAX_ENTRIES = 1024;    // (request, row tile) pairs of one launch
+constexpr int MAX_ENTRIES = 4096;    // (request, row tile) pairs of one launch
 constexpr int SHORT = 4;             // rounds that a segment is not cut below where work is scarce
 
 template <int F, int D, int NT, bool BLK>
@@ -69,10 +69,14 @@ struct Cfg {
   // scales, and in blocks the ratios of the value scales to their row's
   static constexpr int LVI = T * 8, KSB = T * KNB * 4, VRB = BLK ? T * NB * 2 : 0;
   static constexpr int SLOT = LVI + KSB + VRB;
-  static constexpr int HALF = D / 2, ORS = HALF + 4;                   // values and row pitch of a join pass
-  static constexpr int JOIN = WARPS * ROWS * ORS * 4;
-  static constexpr int SMEM = WARPS * STAGES * (STAGE + SLOT) + JOIN + 2 * WARPS * ROWS * 4;
   static constexpr int CTAS = D == 256 || NT == 2 ? 1 : 2;             // per SM
+  static constexpr int RINGS = WARPS * STAGES * (STAGE + SLOT), STATS = 2 * WARPS * ROWS * 4;
+  static constexpr int join_bytes(int passes) { return WARPS * ROWS * (D / passes + 4) * 4; }
+  static constexpr bool fits(int passes) { return CTAS * (RINGS + join_bytes(passes) + STATS + 4096) <= 227 * 1024; }
+  static constexpr int PASSES = fits(1) ? 1 : 2;                       // the warps join all of a row's values at once, or halves
+  static_assert(fits(PASSES), "shared memory");
+  static constexpr int PART = D / PASSES, ORS = PART + 4;              // values and row pitch of a pass
+  static constexpr int SMEM = RINGS + join_bytes(PASSES) + STATS;
 
   // key of a unit's 16 that row r of an instruction's first 8 rows holds (row r + 8: the same + 8),
   // chosen with chunk() so that a read of 32 lanes meets no bank twice
@@ -117,7 +121,6 @@ template <typename T, int F, int D, int NT, bool BLK>
 __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel(const Params p) {
   using C = Cfg<F, D, NT, BLK>;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint32_t prefix[MAX_ENTRIES + 1];  // rounds of a key head before each entry
   __shared__ uint32_t scan[2 * WARPS];
   __shared__ uint32_t last;
 
@@ -129,6 +132,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
   uint8_t *slots = smem + WARPS * STAGES * C::STAGE + warp * STAGES * C::SLOT;
   float *join_o = (float *)(smem + WARPS * STAGES * (C::STAGE + C::SLOT));
   float *join_m = join_o + WARPS * C::ROWS * C::ORS, *join_l = join_m + WARPS * C::ROWS;
+  uint32_t *prefix = (uint32_t *)(join_l + WARPS * C::ROWS);  // rounds of a key head before each entry
   const int entries = p.batch * p.row_tiles, heads = p.kv_heads;
   constexpr uint32_t ROUND = C::T * WARPS;
   const int64_t cap = (int64_t)p.max_pages << p.page_shift;
@@ -370,6 +374,27 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
   read_scales();
   int stage = 0;
 
+  uint32_t raw_q[NT][C::NB][4];
+  auto read_q = [&](const Walk &w) {
+    const int r0 = (w.e - w.b * p.row_tiles) * C::ROWS;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int r = r0 + n * 8 + g;
+      const bool in = r < p.rows;
+      const T *src = in ? (const T *)p.q + row_at(p, w.b, w.h, r).q + 8 * t : nullptr;
+#pragma unroll
+      for (int b = 0; b < C::NB; ++b) {
+        if (in && p.q_vec) lds<16>((const uint8_t *)(src + 32 * b), raw_q[n][b]);
+        else if (in)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            raw_q[n][b][i] = (uint32_t)*(const uint16_t *)(src + 32 * b + 2 * i) | ((uint32_t)*(const uint16_t *)(src + 32 * b + 2 * i + 1) << 16);
+        else raw_q[n][b][0] = raw_q[n][b][1] = raw_q[n][b][2] = raw_q[n][b][3] = 0;
+      }
+    }
+  };
+  if (c.u < u_end) read_q(c);
+
   while (c.u < u_end) {
     const uint32_t real = rounds_of(c.keys), from = c.u - c.seg0, to = min(u_end, c.seg1) - c.seg0;
     const uint32_t upto = min(to, real);
@@ -381,6 +406,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
       }
       c.u = c.seg0 + to;
       if (c.u == c.seg1) next_segment(c);
+      if (c.u < u_end) read_q(c);
       continue;
     }
     const int rt = c.e - c.b * p.row_tiles, r0 = rt * C::ROWS, n_rows = min(C::ROWS, p.rows - r0);
@@ -393,25 +419,14 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
     int lim[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int r = n * 8 + g;
-      const bool in = r < n_rows;
-      const T *src = in ? (const T *)p.q + row_at(p, c.b, c.h, r0 + r).q + 8 * t : nullptr;
-      uint32_t raw[C::NB][4];
       float top = 0.f;
 #pragma unroll
-      for (int b = 0; b < C::NB; ++b) {
-        if (in && p.q_vec) lds<16>((const uint8_t *)(src + 32 * b), raw[b]);
-        else if (in)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            raw[b][i] = (uint32_t)*(const uint16_t *)(src + 32 * b + 2 * i) | ((uint32_t)*(const uint16_t *)(src + 32 * b + 2 * i + 1) << 16);
-        else raw[b][0] = raw[b][1] = raw[b][2] = raw[b][3] = 0;
+      for (int b = 0; b < C::NB; ++b)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const T *v = reinterpret_cast<const T *>(&raw[b][i]);
+          const T *v = reinterpret_cast<const T *>(&raw_q[n][b][i]);
           top = fmaxf(top, fmaxf(fabsf(to_f32(v[0])), fabsf(to_f32(v[1]))));
         }
-      }
       top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
       const int ex = min(max((int)(__float_as_uint(top) >> 23), 1), 253);
@@ -421,7 +436,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
         float x[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const T *v = reinterpret_cast<const T *>(&raw[b][i]);
+          const T *v = reinterpret_cast<const T *>(&raw_q[n][b][i]);
           x[2 * i] = to_f32(v[0]) * down, x[2 * i + 1] = to_f32(v[1]) * down;
         }
 #pragma unroll
@@ -433,7 +448,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
       for (int col = 0; col < 2; ++col) {
         qs[n][col] = __shfl_sync(0xFFFFFFFFu, mine, (2 * t + col) * 4);
         const int rc = n * 8 + 2 * t + col;
-        lim[n][col] = rc >= n_rows ? 0 : p.causal ? len - p.queries + (r0 + rc) / p.group + 1 : len;
+        lim[n][col] = rc >= n_rows ? 0 : p.causal && p.queries > 1 ? len - p.queries + (r0 + rc) / p.group + 1 : len;
       }
     }
 
@@ -609,7 +624,8 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
       stage = stage + 1 == STAGES ? 0 : stage + 1;
     }
 
-    // join the warps, half of each lane's values at a time
+    // join the warps
+    Walk following = c;
     const bool whole = from == 0 && upto == real;
     const uint32_t c0 = split ? c.seg0 / per : 0, c1 = split ? (c.seg0 + real - 1) / per : 0;  // CTAs of the segment
     const int slot = (int)(2 * blockIdx.x + (from == 0 ? 1 : 0));
@@ -623,30 +639,36 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
         if (g == 0) join_m[warp * C::ROWS + r] = m[n][col], join_l[warp * C::ROWS + r] = l[n][col];
       }
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      // value of the head at place i of a pass: lane g's tiles half * MT / 2 .. + MT / 2
+    for (int pass = 0; pass < C::PASSES; ++pass) {
+      // a lane's tiles pass * MT / PASSES .. side by side: 2 * MT / PASSES values
+      constexpr int OWN = 2 * C::MT / C::PASSES;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int col = 0; col < 2; ++col) {
-          float *dst = join_o + (warp * C::ROWS + n * 8 + 2 * t + col) * C::ORS + g * C::MT;
+          float *dst = join_o + (warp * C::ROWS + n * 8 + 2 * t + col) * C::ORS + g * OWN;
 #pragma unroll
-          for (int i = 0; i < C::MT / 2; ++i)
+          for (int i = 0; i < OWN / 2; ++i)
             *reinterpret_cast<float2 *>(dst + 2 * i) =
-                make_float2(o[n][half * (C::MT / 2) + i][col], o[n][half * (C::MT / 2) + i][col + 2]);
+                make_float2(o[n][pass * (OWN / 2) + i][col], o[n][pass * (OWN / 2) + i][col + 2]);
         }
+      if (pass == C::PASSES - 1) {  // the next segment's queries are on their way while the warps meet
+        following.u = c.seg0 + to;
+        if (following.u == following.seg1) next_segment(following);
+        if (following.u < u_end) read_q(following);
+      }
       __syncthreads();
-      for (int i = tid; i < C::ROWS * (C::HALF / 4); i += THREADS) {
-        const int r = i / (C::HALF / 4), at = (i % (C::HALF / 4)) * 4;
-        const int gg = at / C::MT, place = half * C::MT + at % C::MT;  // value `place` of lane gg's
+      for (int i = tid; i < C::ROWS * (C::PART / 4); i += THREADS) {
+        const int r = i / (C::PART / 4), at = (i % (C::PART / 4)) * 4;
+        const int gg = at / OWN, place = pass * OWN + at % OWN;  // value `place` of lane gg's
         const int d = (gg + 8 * (place / C::VEC)) * C::VEC + place % C::VEC;
-        float M = -INFINITY, L = 0.f;
+        float M = -INFINITY, L = 0.f, mw[WARPS];
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) M = fmaxf(M, join_m[w * C::ROWS + r]);
+        for (int w = 0; w < WARPS; ++w) mw[w] = join_m[w * C::ROWS + r], M = fmaxf(M, mw[w]);
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
-          const float mw = join_m[w * C::ROWS + r], f = mw == -INFINITY ? 0.f : ex2(mw - M);
+          const float f = mw[w] == -INFINITY ? 0.f : ex2(mw[w] - M);
           const float4 y = *reinterpret_cast<const float4 *>(join_o + (w * C::ROWS + r) * C::ORS + at);
           x.x += y.x * f, x.y += y.y * f, x.z += y.z * f, x.w += y.w * f;
           L += join_l[w * C::ROWS + r] * f;  // NaN stays NaN, also where it left m at -inf
@@ -659,7 +681,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
           if (d == 0) *reinterpret_cast<float2 *>(p.ws_ml + ((int64_t)slot * C::ROWS + r) * 2) = make_float2(M, L);
         }
       }
-      __syncthreads();
+      if (pass + 1 < C::PASSES) __syncthreads();
     }
     if (!whole) {
       __threadfence();
@@ -691,10 +713,9 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
         }
         if (tid == 0) p.tickets[c0] = 0u;  // ready for the next call on this workspace
       }
-      __syncthreads();
     }
-    c.u = c.seg0 + to;
-    if (c.u == c.seg1) next_segment(c);
+    __syncthreads();  // the join's memory is free
+    c = following;
   }
   cp_async_wait<0>();
 }
@@ -776,7 +797,7 @@ static int32_t launch_t(Params p, cudaStream_t stream) {
   Workspace w;
   if (int32_t rc = workspace_for(stream, w)) return rc;
   p.ws_o = w.o, p.ws_ml = w.ml, p.tickets = w.tickets;
-  B200_CUDA_TRY((ensure_dynamic_smem<attn_kernel<T, F, D, NT, BLK>>(C::SMEM)));
+  B200_CUDA_TRY((ensure_dynamic_smem<attn_kernel<T, F, D, NT, BLK>>(C::SMEM + (MAX_ENTRIES + 1) * 4)));
   // no more CTAs than there can be rounds
   int64_t grid = entries * p.kv_heads * ((cap + round - 1) / round);
   const int64_t full = (int64_t)w.grid / 2 * C::CTAS;
@@ -785,7 +806,7 @@ static int32_t launch_t(Params p, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.dynamicSmemBytes = C::SMEM + (entries + 1) * 4;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -128,8 +128,8 @@ struct RowAt {
   int64_t q, out;
 };
 __device__ __forceinline__ RowAt row_at(const Params &p, int b, int h, int r) {
-  const int tok = r / p.group, head = h * p.group + (r - tok * p.group);
-  const int rq = tok / p.per_request, qi = tok - rq * p.per_request;
+  const int tok = p.rows == p.group ? 0 : r / p.group, head = h * p.group + (r - tok * p.group);
+  const int rq = p.per_request == 1 ? tok : tok / p.per_request, qi = tok - rq * p.per_request;
   const int64_t req = b + rq;
   return {req * p.qsr + qi * p.qsb + head * p.qsh, (req * p.per_request + qi) * p.q_heads + head};
 }
