@@ -11,7 +11,7 @@
 //   warps 8..11   codes -> fp16 into swizzled tiles in shared memory: keys row by row; values eight keys
 //                 at a time, turned on the way so that keys are contiguous (pairs of keys are joined by
 //                 byte permutes before they are decoded). Codes of the next tile are in registers;
-//   warp 12       one lane issues the MMAs (13..15 are there for the registers' split).
+//   warps 12, 13  one lane each issues a slot's MMAs (14, 15 are there for the registers' split).
 // Two row tiles share every decoded key tile (256 rows); with up to 128 rows both warpgroups take the
 // same rows and every other key tile each, and add up at the end. While one slot is in its softmax the
 // other's products run. What bounds it: a tile pair is 2048 cycles of MMA, as many of the special
@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars.qfull[i], WG), mbar_init(&bars.sfull[i], 1), mbar_init(&bars.pfull[i][0], WG), mbar_init(&bars.pfull[i][1], WG), mbar_init(&bars.pvdone[i], 1);
-      mbar_init(&bars.kfull[i], WG), mbar_init(&bars.kfree[i], 1), mbar_init(&bars.vfull[i], WG), mbar_init(&bars.vfree[i], 1);
+      mbar_init(&bars.kfull[i], WG), mbar_init(&bars.kfree[i], RT), mbar_init(&bars.vfull[i], WG), mbar_init(&bars.vfree[i], RT);
     }
     for (int i = 0; i < 4; ++i) mbar_init(&bars.scfull[i], WG);
     for (int i = 0; i < 3; ++i) mbar_init(&bars.done[i], WG);
@@ -815,65 +815,58 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
     }
   } else {
     reg_dec<ISSUE_REGS>();
-    if (warp == 12) {
-      // ================ MMA issuer: the warp stays together, so that descriptors live in uniform registers ================
-    constexpr uint32_t id_s = idesc_f16(0, 128, KT), id_o = idesc_f16(0, 128, D);
-    uint32_t parity = 0;  // bits: qfull[0, 1], both of pfull[0], both of pfull[1]
-    auto wait = [&](uint64_t *bar, uint32_t phase) {
-      return __all_sync(0xFFFFFFFFu, mbar_wait(bar, phase, abort_flag, WAIT_NS)) != 0;
-    };
-    auto wait_flip = [&](uint64_t *bar, uint32_t bit) {
-      const bool ok = wait(bar, (parity >> bit) & 1);
-      parity ^= 1u << bit;
-      return ok;
-    };
-    const uint64_t q0 = sw128_kmajor_desc(qt), k0 = sw128_kmajor_desc(kt), v0 = sw128_kmajor_desc(vt);
-    // operation o of a part: RT = 2: slot o & 1 of tile o >> 1; RT = 1: slot (n0 + o) & 1 of tile o
-    auto scores = [&](uint32_t n, uint32_t s, bool first) {
-      if (first && !wait_flip(&bars.qfull[s], s)) return false;
-      if ((RT == 1 || s == 0) && !wait(&bars.kfull[n & 1], (n >> 1) & 1)) return false;
-      tc_fence_after();
-      const uint64_t qa = q0 + s * (C::QB / 16), kb = k0 + (n & 1) * (C::KB / 16);
-#pragma unroll
-      for (int x = 0; x < D / 16; ++x) {  // 128 x 128 bytes a 64 values, 32 bytes a step
-        const uint64_t at = (x >> 2) * (128 * 128 / 16) + 2 * (x & 3);
-        mma_ss(tmem + s * 128, qa + at, kb + at, id_s, x != 0);
-      }
-      commit(&bars.sfull[s]);
-      if (RT == 1 || s == 1) commit(&bars.kfree[n & 1]);
-      return true;
-    };
-    auto values = [&](uint32_t n, uint32_t s, bool first) {
-      if ((RT == 1 || s == 0) && !wait(&bars.vfull[n & 1], (n >> 1) & 1)) return false;
-      const uint64_t vb = v0 + (n & 1) * (C::VB / 16);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {  // 64 keys at a time
-        if (!wait(&bars.pfull[s][h], (parity >> (2 + s)) & 1)) return false;
-        tc_fence_after();
-#pragma unroll
-        for (int x = 4 * h; x < 4 * h + 4; ++x)
-          mma_ts(tmem + 256 + s * D, tmem + s * 128 + 8 * x, vb + (x >> 2) * (D * 128 / 16) + 2 * (x & 3), id_o, !first || x != 0);
-      }
-      parity ^= 4u << s;
-      commit(&bars.pvdone[s]);
-      if (RT == 1 || s == 1) commit(&bars.vfree[n & 1]);
-      return true;
-    };
-    Part w;
-    uint32_t n0 = 0;
-    bool ok = true;
-    for (bool more = begin(w); more && ok; more = next(w)) {
-      const uint32_t tiles = __shfl_sync(0xFFFFFFFFu, w.to - w.from, 0), count = tiles * RT;
-      auto step = [&](uint32_t o, bool second) {
-        const uint32_t n = n0 + (RT == 2 ? o >> 1 : o), s = RT == 2 ? o & 1 : n & 1;
-        return second ? values(n, s, o < 2) : scores(n, s, o < 2);
+    if (warp < 14) {
+      // ================ MMA issuers: a warp a slot, so that neither waits for the other's softmax; the warp
+      // stays together, so that descriptors live in uniform registers ================
+      const uint32_t s = __shfl_sync(0xFFFFFFFFu, (uint32_t)warp - 12u, 0);
+      constexpr uint32_t id_s = idesc_f16(0, 128, KT), id_o = idesc_f16(0, 128, D), STEP = RT == 2 ? 1 : 2;
+      uint32_t qp = 0, pp = 0;  // parities of the queries' and weights' barriers
+      auto wait = [&](uint64_t *bar, uint32_t phase) {
+        return __all_sync(0xFFFFFFFFu, mbar_wait(bar, phase, abort_flag, WAIT_NS)) != 0;
       };
-      for (uint32_t o = 0; o < count + 2 && ok; ++o) {  // scores run two operations ahead of values
-        if (o >= 2) ok = step(o - 2, true);
-        if (o < count && ok) ok = step(o, false);
+      const uint64_t qa = sw128_kmajor_desc(qt) + s * (C::QB / 16), k0 = sw128_kmajor_desc(kt), v0 = sw128_kmajor_desc(vt);
+      const uint32_t ts = tmem + s * 128, to = tmem + 256 + s * D;
+      auto scores = [&](uint32_t n) {
+        if (!wait(&bars.kfull[n & 1], (n >> 1) & 1)) return false;
+        tc_fence_after();
+        const uint64_t kb = k0 + (n & 1) * (C::KB / 16);
+#pragma unroll
+        for (int x = 0; x < D / 16; ++x) {  // 128 x 128 bytes a 64 values, 32 bytes a step
+          const uint64_t at = (x >> 2) * (128 * 128 / 16) + 2 * (x & 3);
+          mma_ss(ts, qa + at, kb + at, id_s, x != 0);
+        }
+        commit(&bars.sfull[s]);
+        commit(&bars.kfree[n & 1]);
+        return true;
+      };
+      auto values = [&](uint32_t n, bool first) {
+        if (!wait(&bars.vfull[n & 1], (n >> 1) & 1)) return false;
+        const uint64_t vb = v0 + (n & 1) * (C::VB / 16);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {  // 64 keys at a time
+          if (!wait(&bars.pfull[s][h], pp)) return false;
+          tc_fence_after();
+#pragma unroll
+          for (int x = 4 * h; x < 4 * h + 4; ++x)
+            mma_ts(to, ts + 8 * x, vb + (x >> 2) * (D * 128 / 16) + 2 * (x & 3), id_o, !first || x != 0);
+        }
+        pp ^= 1;
+        commit(&bars.pvdone[s]);
+        commit(&bars.vfree[n & 1]);
+        return true;
+      };
+      Part w;
+      uint32_t n0 = 0;
+      bool ok = true;
+      for (bool more = begin(w); more && ok; more = next(w)) {
+        const uint32_t end = n0 + __shfl_sync(0xFFFFFFFFu, w.to - w.from, 0), first = RT == 2 ? n0 : n0 + ((n0 ^ s) & 1);
+        if (first < end) {
+          ok = wait(&bars.qfull[s], qp) && scores(first);
+          qp ^= 1;
+          for (uint32_t n = first; n < end && ok; n += STEP) ok = values(n, n == first) && (n + STEP >= end || scores(n + STEP));
+        }
+        n0 = end;
       }
-      n0 += tiles;
-    }
     }
   }
 
