@@ -288,22 +288,24 @@ typedef struct b200_rotary_desc {
 
 /* y = x turned by its positions: pair (a, b) becomes (a cos - b sin, b cos + a sin); `transpose`
  * takes -sin (the gradient). x, y: [batch, tokens, heads, head_dim] of F16, BF16 or F32, unit
- * stride along head_dim, element strides of the other axes in x_strides / y_strides (3 each);
+ * stride along head_dim, element strides of the other axes;
  * y may be x with equal strides. positions: batch * tokens contiguous I32 or I64. A position
  * outside the table gives NaN and sets bit 1 of b200_device_status. */
 int32_t b200_rotary(const void *x, int32_t dtype, int64_t batch, int64_t tokens, int32_t heads, int32_t head_dim,
-                    const int64_t *x_strides, void *y, const int64_t *y_strides, const b200_rotary_desc *table,
-                    const void *positions, int32_t positions_dtype, int32_t transpose, void *stream);
+                    int64_t x_stride_b, int64_t x_stride_t, int64_t x_stride_h, void *y, int64_t y_stride_b,
+                    int64_t y_stride_t, int64_t y_stride_h, const b200_rotary_desc *table, const void *positions,
+                    int32_t positions_dtype, int32_t transpose, void *stream);
 
 /* Store tokens' keys (turned first when `table` is given) and values in the cells `slots` names
  * (I32 or I64; negative: not stored; beyond the cache: not stored, bit 1 of b200_device_status).
  * k, v: [tokens, kv_heads, head_dim] with element strides (token, head), F16, BF16 or F32. With
  * `q` ([tokens, q_heads, head_dim], same type) the turned queries go to q_out (contiguous, 16-byte
  * aligned). Two tokens of one call must not name one slot. */
-int32_t b200_cache_write(const b200_cache_desc *cache, const void *k, const void *v, int32_t dtype, int64_t tokens,
-                         const int64_t *k_strides, const int64_t *v_strides, const void *slots, int32_t slots_dtype,
-                         const b200_rotary_desc *table, const void *positions, int32_t positions_dtype, const void *q,
-                         int32_t q_heads, const int64_t *q_strides, void *q_out, void *stream);
+int32_t b200_cache_write(const b200_cache_desc *cache, const void *k, int64_t k_stride_t, int64_t k_stride_h,
+                         const void *v, int64_t v_stride_t, int64_t v_stride_h, int32_t dtype, int64_t tokens,
+                         const void *slots, int32_t slots_dtype, const b200_rotary_desc *table, const void *positions,
+                         int32_t positions_dtype, const void *q, int32_t q_heads, int64_t q_stride_t, int64_t q_stride_h,
+                         void *q_out, void *stream);
 
 /* The values that the cells `slots` hold, as `dtype` (F16, BF16, F32), contiguous [tokens, kv_heads,
  * head_dim], 16-byte aligned. Negative slots and slots beyond the cache (bit 1 of

@@ -91,16 +91,14 @@ def _desc(**kw):
 def test_c_entries_check_the_cache(kw, msg):
     lib, d = _lib.lib(), _desc(**kw)
     a = A.AttentionArgs()
-    s = (ctypes.c_int64 * 2)(0, 0)
     for rc in (lib.b200_cache_attention(ctypes.byref(d), ctypes.byref(a), None),
                lib.b200_cache_read(ctypes.byref(d), None, 6, 0, None, None, 12, None),
-               lib.b200_cache_write(ctypes.byref(d), None, None, 12, 0, s, s, None, 6, None, None, 0, None, 0, None, None, None)):
+               lib.b200_cache_write(ctypes.byref(d), None, 0, 0, None, 0, 0, 12, 0, None, 6, None, None, 0, None, 0, 0, 0, None, None)):
         assert rc == _lib.ERR_INVALID and msg in _lib.last_error()
 
 
 def test_c_entries_check_arguments():
     lib, d = _lib.lib(), _desc()
-    s2, s3 = (ctypes.c_int64 * 2)(0, 0), (ctypes.c_int64 * 3)(0, 0, 0)
     ref = ctypes.byref(d)
 
     def attention(**kw):
@@ -120,12 +118,12 @@ def test_c_entries_check_arguments():
     assert lib.b200_cache_read(ref, None, 6, 1, None, None, 12, None) == _lib.ERR_INVALID
     assert lib.b200_cache_read(ref, None, 12, 0, None, None, 12, None) == _lib.ERR_INVALID
     assert lib.b200_cache_read(ref, None, 6, 0, None, None, 2, None) == _lib.ERR_INVALID
-    assert lib.b200_cache_write(ref, None, None, 12, -1, s2, s2, None, 6, None, None, 0, None, 0, None, None, None) == _lib.ERR_INVALID
-    assert lib.b200_cache_write(ref, None, None, 12, 1, s2, s2, None, 6, None, None, 0, None, 0, None, None, None) == _lib.ERR_INVALID
+    assert lib.b200_cache_write(ref, None, 0, 0, None, 0, 0, 12, -1, None, 6, None, None, 0, None, 0, 0, 0, None, None) == _lib.ERR_INVALID
+    assert lib.b200_cache_write(ref, None, 0, 0, None, 0, 0, 12, 1, None, 6, None, None, 0, None, 0, 0, 0, None, None) == _lib.ERR_INVALID
     t = A.RotaryDesc(4096, 4096, 10, 66, 0)
-    assert lib.b200_rotary(4096, 12, 1, 1, 1, 64, s3, 4096, s3, ctypes.byref(t), 4096, 6, 0, None) == _lib.ERR_INVALID
+    assert lib.b200_rotary(4096, 12, 1, 1, 1, 64, 0, 0, 0, 4096, 0, 0, 0, ctypes.byref(t), 4096, 6, 0, None) == _lib.ERR_INVALID
     assert "rotary_dim" in _lib.last_error()
-    assert lib.b200_rotary(4096, 12, 1, 1, 1, 64, s3, 4096, s3, None, 4096, 6, 0, None) == _lib.ERR_INVALID
-    assert lib.b200_rotary(None, 12, 0, 1, 1, 64, s3, None, s3, None, None, 6, 0, None) == 0
+    assert lib.b200_rotary(4096, 12, 1, 1, 1, 64, 0, 0, 0, 4096, 0, 0, 0, None, 4096, 6, 0, None) == _lib.ERR_INVALID
+    assert lib.b200_rotary(None, 12, 0, 1, 1, 64, 0, 0, 0, None, 0, 0, 0, None, None, 6, 0, None) == 0
     assert lib.b200_cache_attention_scratch(2, 3, 4, 64, 10) == 2 * 3 * 4 * 66 * 4
     assert lib.b200_cache_attention_scratch(2, 3, 4, 64, 0) == 0

@@ -491,6 +491,52 @@ def test_first_call_captured():
     assert good.shape == out.shape
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("e8", [False, True])
+@pytest.mark.parametrize("queries,prefix", [(1, 300), (40, 0), (70, 130)])
+def test_attention_without_logarithms(fmt, e8, queries, prefix):
+    """Results alone: key codes may take their scales before the products then, rounded to fp16 (2^-11 a
+    term, like a block-scaled cache's)."""
+    c = Case([200, queries, 5, 0], queries=queries, heads=16, kv=2, fmt=fmt, e8=e8, prefix=prefix, seed=90)
+    c.blocked = True
+    _, lse = c.run()
+    shared = dict(prefix=c.prefix.to(torch.int32).cuda(), prefix_length=prefix) if prefix else {}
+    out = tg.cache_attention(c.q.cuda(), c.cache, c.tables.to(torch.int32).cuda(),
+                             torch.tensor(c.lengths, dtype=torch.int32).cuda(), **shared)
+    c.check(out, lse)
+
+
+@pytest.mark.parametrize("rows", ["few", "many"])
+@pytest.mark.parametrize("fmt,blocked", [("int8", False), ("fp4_e2m1", True), ("int4", False), ("fp8e4m3", True)])
+def test_attention_outliers_that_are_not_seen(rows, fmt, blocked):
+    """Keys and values 2^40 times the others', infinite or NaN, behind what most queries see: theirs are as
+    without them."""
+    queries = 1 if rows == "few" else 24
+    c = Case([150, 150], queries=queries, heads=4, kv=1, fmt=fmt, blocked=blocked, seed=91, per=10, page=16)
+    good, _ = c.run()
+    big = torch.randn(1, 1, 128) * 2.0 ** 40
+    bad = big.clone()
+    bad[0, 0, 7], bad[0, 0, 50] = math.inf, math.nan
+    last = c.own[0][149:150].cuda()  # request 0's last key: its last query alone sees it
+    for x in (big, bad):
+        tg.cache_write(c.cache, x.cuda(), x.cuda(), last)
+        out, lse = c.run()
+        if queries > 1:
+            assert torch.equal(out[1], good[1])
+            tol = 2.0 ** -7 * good[0, :-1].abs() + 2.0 ** -9 * good[0, :-1].abs().max()  # two runs' roundings
+            assert ((out[0, :-1].float() - good[0, :-1].float()).abs() <= tol.float()).all()
+        else:  # one query sees it: beyond the length instead
+            n = torch.tensor([149, 150], dtype=torch.int32).cuda()
+            o = tg.cache_attention(c.q.cuda(), c.cache, c.tables.to(torch.int32).cuda(), n)
+            assert not o.isnan().any() and torch.equal(o[1], good[1])
+
+
+@pytest.mark.parametrize("blocked", [False, True])
+def test_attention_many_rows_value_ranges(blocked):
+    """Scales that span 2^40 from key to key under many query rows."""
+    Case([400], queries=40, heads=8, kv=2, fmt="int8", blocked=blocked, e8=True, spread=10.0, q_gain=8.0, seed=92).check()
+
+
 # ---- refusals ---------------------------------------------------------------------------------------
 def test_refusals():
     cache = make_cache("int8", 128, heads=2)

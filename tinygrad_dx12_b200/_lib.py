@@ -79,8 +79,9 @@ SIGNATURES = {
     "b200_ipc_close": ([_P], _I32),
     "b200_add_rmsnorm": ([_P, _I32, _P, _P, _I32, _I64, _I64, ctypes.c_float, _P], _I32),
     "b200_gate_mul": ([_P, _I32, _P, _I32, _I64, _I64, _P], _I32),
-    "b200_rotary": ([_P, _I32, _I64, _I64, _I32, _I32, _P, _P, _P, _P, _P, _I32, _I32, _P], _I32),
-    "b200_cache_write": ([_P, _P, _P, _I32, _I64, _P, _P, _P, _I32, _P, _P, _I32, _P, _I32, _P, _P, _P], _I32),
+    "b200_rotary": ([_P, _I32, _I64, _I64, _I32, _I32, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _I32, _I32, _P], _I32),
+    "b200_cache_write": ([_P, _P, _I64, _I64, _P, _I64, _I64, _I32, _I64, _P, _I32, _P, _P, _I32, _P, _I32, _I64, _I64, _P,
+                          _P], _I32),
     "b200_cache_read": ([_P, _P, _I32, _I64, _P, _P, _I32, _P], _I32),
     "b200_cache_attention_scratch": ([_I64, _I64, _I32, _I32, _I64], _I64),
     "b200_cache_attention": ([_P, _P, _P], _I32),

@@ -29,7 +29,7 @@ HEAD_DIMS = (64, 128, 256)
 _REAL = {torch.float16: _lib.DT["float16"], torch.bfloat16: _lib.DT["bfloat16"], torch.float32: _lib.DT["float32"]}
 _INDEX = {torch.int32: _lib.DT["int32"], torch.int64: _lib.DT["int64"]}
 _SCALES = {torch.bfloat16: _lib.DT["bfloat16"], torch.float8_e8m0fnu: _lib.DT["e8m0"]}
-_I64x2, _I64x3 = ctypes.c_int64 * 2, ctypes.c_int64 * 3
+_I64x3 = ctypes.c_int64 * 3
 
 
 class RotaryDesc(ctypes.Structure):
@@ -60,19 +60,25 @@ class AttentionArgs(ctypes.Structure):
                 ("heads", ctypes.c_int32), ("scale", ctypes.c_float), ("reserved", ctypes.c_int32)]
 
 
+_FN: dict = {}  # library functions by name
+
+
 def _call(name: str, device: torch.device, *args) -> None:
-    """A library call with the operands' device current."""
+    """A library call on the current stream of the operands' device, which is made current."""
+    fn = _FN.get(name)
+    if fn is None:
+        fn = _FN[name] = getattr(_lib.lib(), name)
     if device.index is None or device.index == torch.cuda.current_device():
-        _lib.call(name, *args, stream_ptr(device))
+        status = fn(*args, stream_ptr(device))
     else:
         with torch.cuda.device(device):
-            _lib.call(name, *args, stream_ptr(device))
+            status = fn(*args, stream_ptr(device))
+    if status < 0:
+        _lib.check(status, name)
 
 
-def _same_device(device: torch.device, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} must be on {device}, not {t.device}")
+def _elsewhere(name: str, t, device: torch.device) -> ValueError:
+    return ValueError(f"{name} must be on {device}, not {t.device}")
 
 
 # ---- rotary positions -------------------------------------------------------------------------
@@ -91,7 +97,8 @@ class RotaryTable:
         if cos.shape[1] < 1:
             raise ValueError("rotary tables need at least one pair")
         _require_cuda(cos, "rotary tables")
-        _same_device(cos.device, sin=sin)
+        if sin.device != cos.device:
+            raise _elsewhere("sin", sin, cos.device)
         self.cos, self.sin, self.layout = cos.contiguous(), sin.contiguous(), layout
         self.rotary_dim, self.rows, self.device = 2 * cos.shape[1], cos.shape[0], cos.device
         self.desc = RotaryDesc(self.cos.data_ptr(), self.sin.data_ptr(), self.rows, self.rotary_dim,
@@ -139,19 +146,11 @@ class RotaryTable:
 def _index(t: torch.Tensor, name: str, shape, device) -> torch.Tensor:
     if t.dtype not in _INDEX:
         raise ValueError(f"{name} must be int32 or int64")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
-    _same_device(device, **{name: t})
+    if t.device != device:
+        raise _elsewhere(name, t, device)
     return t if t.is_contiguous() else t.contiguous()
-
-
-def _rotary(x: torch.Tensor, table: RotaryTable, positions: torch.Tensor, out: torch.Tensor, transpose: bool) -> None:
-    four = x.dim() == 4
-    b, t = (x.shape[0], x.shape[1]) if four else (1, x.shape[0])
-    xs, ys = x.stride(), out.stride()
-    _call("b200_rotary", x.device, x.data_ptr(), _REAL[x.dtype], b, t, x.shape[-2], x.shape[-1],
-          _I64x3(xs[0] if four else 0, xs[-3], xs[-2]), out.data_ptr(), _I64x3(ys[0] if four else 0, ys[-3], ys[-2]),
-          table._ref, positions.data_ptr(), _INDEX[positions.dtype], int(transpose))
 
 
 class _Rotary(torch.autograd.Function):
@@ -184,23 +183,36 @@ def rotary(x: torch.Tensor, table: RotaryTable, positions: torch.Tensor, transpo
         raise ValueError(f"rotary takes float16, bfloat16 or float32, not {x.dtype}")
     if table.rotary_dim > x.shape[-1]:
         raise ValueError(f"a table of {table.rotary_dim} rotary dimensions does not fit heads of {x.shape[-1]}")
-    _require_cuda(x, "rotary input")
-    _same_device(x.device, table=table)
-    positions = _index(positions, "positions", x.shape[:-2], x.device)
+    device = x.device
+    if device.type != "cuda":
+        _require_cuda(x, "rotary input")
+    if table.device != device:
+        raise _elsewhere("table", table, device)
+    positions = _index(positions, "positions", x.shape[:-2], device)
     if x.requires_grad and torch.is_grad_enabled():
         if out is not None:
             raise ValueError("rotary with a gradient cannot write into out")
         return _Rotary.apply(x, table, positions, transpose)
-    if x.stride(-1) != 1:
+    xs = x.stride()
+    if xs[-1] != 1:
         x = x.contiguous()
+        xs = x.stride()
     if out is None:
-        out = torch.empty_like(x)
+        out = torch.empty_like(x)  # x's own order of axes where that is dense
         if out.stride(-1) != 1:
-            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or out.stride(-1) != 1:
-        raise ValueError("out must have x's shape, type and device, and contiguous heads")
-    if x.numel():
-        _rotary(x, table, positions, out, transpose)
+            out = torch.empty(x.shape, dtype=x.dtype, device=device)
+    elif out.shape != x.shape or out.dtype != x.dtype or out.device != device:
+        raise ValueError("out must have x's shape, type and device")
+    ys = out.stride()
+    if ys[-1] != 1:
+        raise ValueError("out must have contiguous heads")
+    shape = x.shape
+    if len(shape) == 4:
+        b, t, xb, yb = shape[0], shape[1], xs[0], ys[0]
+    else:
+        b, t, xb, yb = 1, shape[0], 0, 0
+    _call("b200_rotary", device, x.data_ptr(), _REAL[x.dtype], b, t, shape[-2], shape[-1], xb, xs[-3], xs[-2],
+          out.data_ptr(), yb, ys[-3], ys[-2], table._ref, positions.data_ptr(), _INDEX[positions.dtype], int(transpose))
     return out
 
 
@@ -341,30 +353,39 @@ def cache_write(cache: PackedCache, k: torch.Tensor, v: torch.Tensor, slots: tor
     if (table is None) != (positions is None):
         raise ValueError("table and positions go together")
     device = cache.k.device
-    _require_cuda(cache.k, "the cache")
-    _same_device(device, k=k, v=v, q=q, table=table)
-    slots = _index(slots, "slots", (n,), device)
-    out, qs, q_ptr, out_ptr, heads = None, None, None, None, 0
+    if device.type != "cuda":
+        _require_cuda(cache.k, "the cache")
+    if k.device != device or v.device != device:
+        raise _elsewhere("k and v", k if k.device != device else v, device)
+    slots = _index(slots, "slots", k.shape[:1], device)
+    out, q_ptr, out_ptr, heads, qt, qh = None, None, None, 0, 0, 0
+    if table is not None:
+        if table.device != device:
+            raise _elsewhere("table", table, device)
+        if table.rotary_dim > cache.head_dim:
+            raise ValueError(f"a table of {table.rotary_dim} rotary dimensions does not fit heads of {cache.head_dim}")
+        positions = _index(positions, "positions", k.shape[:1], device)
     if q is not None:
         if table is None:
             raise ValueError("q needs table and positions")
         q = _rows(q, "q", None, cache)
         if q.shape[0] != n:
             raise ValueError("q and k must hold the same tokens")
+        if q.device != device:
+            raise _elsewhere("q", q, device)
         heads = q.shape[1]
-        out = torch.empty((n, heads, cache.head_dim), dtype=q.dtype, device=device)
-    if table is not None:
-        positions = _index(positions, "positions", (n,), device)
-        if table.rotary_dim > cache.head_dim:
-            raise ValueError(f"a table of {table.rotary_dim} rotary dimensions does not fit heads of {cache.head_dim}")
-    if n == 0:
-        return out
-    if q is not None and heads:
-        qs, q_ptr, out_ptr = _I64x2(q.stride(0), q.stride(1)), q.data_ptr(), out.data_ptr()
-    _call("b200_cache_write", device, cache.desc(), k.data_ptr(), v.data_ptr(), _REAL[k.dtype], n,
-          _I64x2(k.stride(0), k.stride(1)), _I64x2(v.stride(0), v.stride(1)), slots.data_ptr(), _INDEX[slots.dtype],
-          None if table is None else table._ref, None if table is None else positions.data_ptr(),
-          0 if table is None else _INDEX[positions.dtype], q_ptr, heads, qs, out_ptr)
+        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        if heads:
+            qt, qh = q.stride()[:2]
+            q_ptr, out_ptr = q.data_ptr(), out.data_ptr()
+    ks, vs = k.stride(), v.stride()
+    if table is None:
+        _call("b200_cache_write", device, cache.desc(), k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
+              _REAL[k.dtype], n, slots.data_ptr(), _INDEX[slots.dtype], None, None, 0, None, 0, 0, 0, None)
+    else:
+        _call("b200_cache_write", device, cache.desc(), k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
+              _REAL[k.dtype], n, slots.data_ptr(), _INDEX[slots.dtype], table._ref, positions.data_ptr(),
+              _INDEX[positions.dtype], q_ptr, heads, qt, qh, out_ptr)
     return out
 
 
@@ -375,15 +396,17 @@ def cache_read(cache: PackedCache, slots: torch.Tensor, dtype: torch.dtype = tor
     and sets bit 1 of the device status."""
     if dtype not in _REAL:
         raise ValueError(f"cache_read gives float16, bfloat16 or float32, not {dtype}")
-    _require_cuda(cache.k, "the cache")
+    device = cache.k.device
+    if device.type != "cuda":
+        _require_cuda(cache.k, "the cache")
     if slots.dim() != 1:
         raise ValueError("slots must be one-dimensional")
-    slots = _index(slots, "slots", slots.shape, cache.k.device)
-    shape = (slots.shape[0], cache.kv_heads, cache.head_dim)
-    k, v = (torch.empty(shape, dtype=dtype, device=cache.k.device) for _ in "kv")
-    if shape[0]:
-        _call("b200_cache_read", cache.k.device, cache.desc(), slots.data_ptr(), _INDEX[slots.dtype], shape[0],
-              k.data_ptr(), v.data_ptr(), _REAL[dtype])
+    slots = _index(slots, "slots", slots.shape, device)
+    n = slots.shape[0]
+    both = torch.empty((2, n, cache.k.shape[1], cache.head_dim), dtype=dtype, device=device)
+    k, v = both.unbind(0)
+    _call("b200_cache_read", device, cache.desc(), slots.data_ptr(), _INDEX[slots.dtype], n, k.data_ptr(), v.data_ptr(),
+          _REAL[dtype])
     return k, v
 
 
@@ -416,11 +439,15 @@ def cache_attention(q: torch.Tensor, cache: PackedCache, tables: torch.Tensor, l
     if heads < 1 or heads % cache.kv_heads:
         raise ValueError(f"{heads} heads do not share {cache.kv_heads} key heads evenly")
     device = cache.k.device
-    _require_cuda(cache.k, "the cache")
-    _same_device(device, q=q, tables=tables, lengths=lengths, prefix=prefix, out=out)
+    if device.type != "cuda":
+        _require_cuda(cache.k, "the cache")
+    if q.device != device:
+        raise _elsewhere("q", q, device)
+    if tables.device != device or lengths.device != device:
+        raise _elsewhere("tables and lengths", tables if tables.device != device else lengths, device)
     if tables.dtype != torch.int32 or tables.dim() != 2 or tables.shape[0] != batch:
         raise ValueError("tables must be int32 (batch, max_pages)")
-    if lengths.dtype != torch.int32 or tuple(lengths.shape) != (batch,):
+    if lengths.dtype != torch.int32 or lengths.shape != q.shape[:1]:
         raise ValueError("lengths must be int32 (batch,)")
     if not lengths.is_contiguous():
         lengths = lengths.contiguous()
@@ -429,6 +456,8 @@ def cache_attention(q: torch.Tensor, cache: PackedCache, tables: torch.Tensor, l
     if prefix_length < 0 or (prefix_length > 0 and prefix is None):
         raise ValueError("prefix_length needs the prefix's pages")
     if prefix is not None:
+        if prefix.device != device:
+            raise _elsewhere("prefix", prefix, device)
         if prefix.dtype != torch.int32 or prefix.dim() != 1 or prefix_length > prefix.shape[0] * cache.page_size:
             raise ValueError("prefix must be int32 pages that hold prefix_length tokens")
         if not prefix.is_contiguous():
@@ -437,8 +466,8 @@ def cache_attention(q: torch.Tensor, cache: PackedCache, tables: torch.Tensor, l
         q = q.contiguous()
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=device)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
-        raise ValueError("out must be contiguous, of q's shape and type")
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != device or not out.is_contiguous():
+        raise ValueError("out must be contiguous, of q's shape, type and device")
     lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=device) if return_lse else None
     if out.numel():
         a = AttentionArgs()
@@ -451,8 +480,8 @@ def cache_attention(q: torch.Tensor, cache: PackedCache, tables: torch.Tensor, l
         if lse is not None:
             a.lse = lse.data_ptr()
         if prefix_length > 0:
-            scratch = torch.empty(_lib.lib().b200_cache_attention_scratch(batch, queries, heads, cache.head_dim, prefix_length),
-                                  dtype=torch.uint8, device=device)
+            size = _lib.lib().b200_cache_attention_scratch(batch, queries, heads, cache.head_dim, prefix_length)
+            scratch = torch.empty(size, dtype=torch.uint8, device=device)
             a.prefix, a.prefix_pages, a.prefix_length, a.scratch = (prefix.data_ptr(), prefix.shape[0], prefix_length,
                                                                     scratch.data_ptr())
         _call("b200_cache_attention", device, cache.desc(), ctypes.byref(a))

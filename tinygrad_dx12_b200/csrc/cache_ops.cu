@@ -824,26 +824,29 @@ using namespace b200;
 extern "C" {
 
 int32_t b200_rotary(const void *x, int32_t dtype, int64_t batch, int64_t tokens, int32_t heads, int32_t head_dim,
-                    const int64_t *x_strides, void *y, const int64_t *y_strides, const b200_rotary_desc *table,
-                    const void *positions, int32_t positions_dtype, int32_t transpose, void *stream) {
+                    int64_t x_stride_b, int64_t x_stride_t, int64_t x_stride_h, void *y, int64_t y_stride_b,
+                    int64_t y_stride_t, int64_t y_stride_h, const b200_rotary_desc *table, const void *positions,
+                    int32_t positions_dtype, int32_t transpose, void *stream) {
   if (int32_t rc = b200_injected()) return rc;
-  if (batch < 0 || tokens < 0 || heads < 0 || head_dim < 1 || x_strides == nullptr || y_strides == nullptr)
+  if (batch < 0 || tokens < 0 || heads < 0 || head_dim < 1)
     return b200_set_error(B200_ERR_INVALID, "rotary: bad sizes");
   if (!cache::real_dtype(dtype)) return b200_set_error(B200_ERR_INVALID, "rotary: unsupported dtype %d", dtype);
   if (batch == 0 || tokens == 0 || heads == 0) return B200_OK;
   if (int32_t rc = check_rotary(table, head_dim, positions, positions_dtype)) return rc;
   if (x == nullptr || y == nullptr) return b200_set_error(B200_ERR_INVALID, "rotary: null x or y");
-  return launch_rotary(x, dtype, batch, tokens, heads, head_dim, x_strides, y, y_strides, table, positions,
+  const int64_t xs[3] = {x_stride_b, x_stride_t, x_stride_h}, ys[3] = {y_stride_b, y_stride_t, y_stride_h};
+  return launch_rotary(x, dtype, batch, tokens, heads, head_dim, xs, y, ys, table, positions,
                        positions_dtype, transpose, (cudaStream_t)stream);
 }
 
-int32_t b200_cache_write(const b200_cache_desc *c, const void *k, const void *v, int32_t dtype, int64_t tokens,
-                         const int64_t *k_strides, const int64_t *v_strides, const void *slots, int32_t slots_dtype,
-                         const b200_rotary_desc *table, const void *positions, int32_t positions_dtype, const void *q,
-                         int32_t q_heads, const int64_t *q_strides, void *q_out, void *stream) {
+int32_t b200_cache_write(const b200_cache_desc *c, const void *k, int64_t k_stride_t, int64_t k_stride_h, const void *v,
+                         int64_t v_stride_t, int64_t v_stride_h, int32_t dtype, int64_t tokens, const void *slots,
+                         int32_t slots_dtype, const b200_rotary_desc *table, const void *positions,
+                         int32_t positions_dtype, const void *q, int32_t q_heads, int64_t q_stride_t, int64_t q_stride_h,
+                         void *q_out, void *stream) {
   if (int32_t rc = b200_injected()) return rc;
   if (int32_t rc = check_cache(c)) return rc;
-  if (tokens < 0 || k_strides == nullptr || v_strides == nullptr || (q != nullptr && (q_heads < 1 || q_heads > 65535 || q_strides == nullptr)))
+  if (tokens < 0 || (q != nullptr && (q_heads < 1 || q_heads > 65535)))
     return b200_set_error(B200_ERR_INVALID, "cache_write: bad sizes");
   if (!cache::real_dtype(dtype)) return b200_set_error(B200_ERR_INVALID, "cache_write: unsupported dtype %d", dtype);
   if (cache::bad_index_dtype(slots_dtype)) return b200_set_error(B200_ERR_INVALID, "cache_write: slots must be int32 or int64");
@@ -853,8 +856,9 @@ int32_t b200_cache_write(const b200_cache_desc *c, const void *k, const void *v,
   if (k == nullptr || v == nullptr || slots == nullptr || (q != nullptr && q_out == nullptr))
     return b200_set_error(B200_ERR_INVALID, "cache_write: null pointer");
   if ((uintptr_t)q_out % 16) return b200_set_error(B200_ERR_INVALID, "cache_write: q_out must start on a 16-byte boundary");
-  return launch_cache_write(c, k, v, dtype, tokens, k_strides, v_strides, slots, slots_dtype, table, positions,
-                            positions_dtype, q, q_heads, q_strides, q_out, (cudaStream_t)stream);
+  const int64_t ks[2] = {k_stride_t, k_stride_h}, vs[2] = {v_stride_t, v_stride_h}, qs[2] = {q_stride_t, q_stride_h};
+  return launch_cache_write(c, k, v, dtype, tokens, ks, vs, slots, slots_dtype, table, positions, positions_dtype, q,
+                            q_heads, qs, q_out, (cudaStream_t)stream);
 }
 
 int32_t b200_cache_read(const b200_cache_desc *c, const void *slots, int32_t slots_dtype, int64_t tokens, void *k_out,
