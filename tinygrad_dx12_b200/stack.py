@@ -13,8 +13,10 @@ chain the projections of a decoder layer over packed weights. One layer here:
     m   = gu[:, :I] * gu[:, I:]   fp32 product rounded to the activation dtype
     h  += allreduce(m @ Wd^T)     row-parallel, fp32
 
-There is no attention: k and v are computed and dropped (their weights stream like a real
-layer's). ``rmsnorm(h) = h * rsqrt(mean(h^2) + 1e-6)`` in fp32 keeps the synthetic activations
+Without a ``StackCache`` there is no attention: k and v are computed and dropped (their weights
+stream like a real layer's). With one, q and k are turned by their positions, k and v are quantised
+into the layer's packed cache, and o's input is the attention of q over it
+(``forward(h, cache, step)``; each rank keeps its own key heads). ``rmsnorm(h) = h * rsqrt(mean(h^2) + 1e-6)`` in fp32 keeps the synthetic activations
 bounded over 32 or 80 layers. Projections run through ``b200_packed_linear`` (fp32
 accumulation); the elementwise steps through ``b200_add_rmsnorm`` / ``b200_gate_mul``; the
 all-reduce through ``torch.distributed`` (NCCL between GPUs). Shards are cut from the full
@@ -155,6 +157,54 @@ def shard_layer(full: dict, cfg: StackConfig, rank: int, world: int) -> LayerSha
     gu = concat_rows([shard_rows(full["gate"], i0, i1), shard_rows(full["up"], i0, i1)])
     return LayerShard(qkv=qkv, o=shard_cols(full["o"], q0, q1), gu=gu, down=shard_cols(full["down"], i0, i1),
                       q_rows=q1 - q0, inter_rows=i1 - i0)
+
+
+# ---- attention between the projections -----------------------------------------------------
+@dataclasses.dataclass
+class StackStep:
+    """Where a forward pass's tokens go: ``batch`` requests of ``tokens / batch`` new tokens each, one
+    request after the other. ``slots`` and ``positions`` (tokens,), ``tables`` int32 (batch, max_pages)
+    and ``lengths`` int32 (batch,) as ``cache_write`` and ``cache_attention`` take them (lengths count
+    the new tokens); ``prefix`` pages and ``prefix_length`` are shared by the batch."""
+
+    slots: torch.Tensor
+    positions: torch.Tensor
+    tables: torch.Tensor
+    lengths: torch.Tensor
+    prefix: torch.Tensor | None = None
+    prefix_length: int = 0
+
+
+class StackCache:
+    """A packed key/value cache for every layer of one rank's shard, and the rotary table they share."""
+
+    def __init__(self, cfg: StackConfig, table, pages: int, page_size: int = 64, head_dim: int = 128, format: str = "int8",
+                 block_size: int | None = None, scale_dtype: torch.dtype = torch.bfloat16, layers: int | None = None,
+                 world: int = 1, device="cuda"):
+        from .attention import PackedCache
+
+        if cfg.q_dim % (head_dim * world) or cfg.kv_dim % (head_dim * world):
+            raise ValueError(f"heads of {head_dim} do not split over {world} ranks")
+        self.table, self.head_dim = table, head_dim
+        kv_heads = cfg.kv_dim // head_dim // world
+        self.layers = [PackedCache.empty(pages, page_size, kv_heads, head_dim, format, block_size, scale_dtype, device)
+                       for _ in range(cfg.layers if layers is None else layers)]
+
+    def attend(self, layer: int, qkv: torch.Tensor, q_rows: int, step: StackStep) -> torch.Tensor:
+        """Attention of one layer's projected tokens (tokens, q_rows + 2 * kv_rows); (tokens, q_rows)."""
+        from .attention import cache_attention, cache_write
+
+        cache, d = self.layers[layer], self.head_dim
+        rows = qkv.view(qkv.shape[0], -1, d)
+        heads, kv = q_rows // d, cache.kv_heads
+        q = cache_write(cache, rows[:, heads:heads + kv], rows[:, heads + kv:], step.slots, self.table, step.positions,
+                        q=rows[:, :heads])
+        batch = step.lengths.shape[0]
+        if batch < 1 or q.shape[0] % batch:
+            raise ValueError(f"{q.shape[0]} tokens do not split over {batch} requests")
+        out = cache_attention(q.view(batch, -1, heads, d), cache, step.tables, step.lengths, prefix=step.prefix,
+                              prefix_length=step.prefix_length)
+        return out.view(qkv.shape[0], q_rows)
 
 
 # ---- compute back-ends ----------------------------------------------------------------------
@@ -317,8 +367,11 @@ class TPStack:
                 tot += w.data.numel() + (w.scales.numel() * w.scales.element_size() if w.scales is not None else 0)
         return tot
 
-    def forward(self, h: torch.Tensor) -> torch.Tensor:
-        """h: (M, hidden) in the activation dtype, replicated on every rank; updated in place."""
+    def forward(self, h: torch.Tensor, cache: StackCache | None = None, step: StackStep | None = None) -> torch.Tensor:
+        """h: (M, hidden) in the activation dtype, replicated on every rank; updated in place. With
+        ``cache`` and ``step`` the layers attend over their cached tokens, h's among them."""
+        if (cache is None) != (step is None):
+            raise ValueError("cache and step go together")
         cfg, ops = self.cfg, self.ops
         m = h.shape[0]
         x = torch.empty_like(h)
@@ -329,9 +382,10 @@ class TPStack:
         else:
             row_reduce = getattr(ops, "row_reduce", None) or (
                 lambda w, inp, hh, xx, slot: _generic_row_reduce(ops, w, inp, hh, xx))
-        for L in self.layers:
+        for i, L in enumerate(self.layers):
             qkv = ops.linear(L.qkv, x, cfg.act)
-            row_reduce(L.o, qkv[:, :L.q_rows], h, x, 0)
+            q = qkv[:, :L.q_rows] if cache is None else cache.attend(i, qkv, L.q_rows, step)
+            row_reduce(L.o, q, h, x, 0)
             gu = ops.linear(L.gu, x, cfg.act)
             ops.gate_mul(gu, mbuf)
             row_reduce(L.down, mbuf, h, x, 1)
