@@ -301,8 +301,8 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
     if (++a.u == a.seg1) next_segment(a);
     read_pages();
   };
-  // the codes of the unit whose scales were read last, and those scales, into stage s
-  auto fill = [&](int s) {
+  // the codes of the unit whose scales were read last into stage s
+  auto issue_codes = [&](int s) {
     if (left > 0) {
       const uint32_t kd = smem_u32(ring + s * C::STAGE), vd = kd + C::T * C::RB;
       if (left >= C::T && bad == 0) {
@@ -328,6 +328,12 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
           cp_async16(vd + to, src + v_of_k, in);
         }
       }
+    }
+    cp_async_commit();
+  };
+  // what the scores need of its scales beside them
+  auto store_scales = [&](int s) {
+    if (left > 0) {
       float2 *lvi = (float2 *)(slots + s * C::SLOT);
       float *ks = (float *)(slots + s * C::SLOT + C::LVI);
       __half *vr = (__half *)(slots + s * C::SLOT + C::LVI + C::KSB);
@@ -362,17 +368,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
         }
       }
     }
-    cp_async_commit();
   };
-
-  read_pages();
-#pragma unroll
-  for (int s = 0; s < STAGES; ++s) {
-    read_scales();
-    fill(s);
-  }
-  read_scales();
-  int stage = 0;
 
   uint32_t raw_q[NT][C::NB][4];
   auto read_q = [&](const Walk &w) {
@@ -393,16 +389,25 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
       }
     }
   };
+  read_pages();
   if (c.u < u_end) read_q(c);
+  // Of the unit that is computed, stage `stage` holds codes and scales; the next one's codes are asked for
+  // first thing, and its scales, which were asked for a unit earlier, are stored last.
+  int stage = 0;
+  read_scales();
+  issue_codes(0);
+  store_scales(0);
+  read_scales();
 
   while (c.u < u_end) {
     const uint32_t real = rounds_of(c.keys), from = c.u - c.seg0, to = min(u_end, c.seg1) - c.seg0;
     const uint32_t upto = min(to, real);
     if (from >= real) {  // padding alone: the ring goes on
       for (uint32_t i = from; i < to; ++i) {
-        fill(stage);
+        stage ^= 1;
+        issue_codes(stage);
+        store_scales(stage);
         read_scales();
-        stage = stage + 1 == STAGES ? 0 : stage + 1;
       }
       c.u = c.seg0 + to;
       if (c.u == c.seg1) next_segment(c);
@@ -464,7 +469,8 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
 
     for (uint32_t round = from; round < to; ++round) {
       const int first = ((int)round * WARPS + warp) * C::T;  // the unit's first key
-      cp_async_wait<STAGES - 1>();
+      issue_codes(stage ^ 1);
+      cp_async_wait<1>();
       __syncwarp();
       const uint8_t *kt = ring + stage * C::STAGE, *vt = kt + C::T * C::RB;
       const float2 *lvi_s = (const float2 *)(slots + stage * C::SLOT);
@@ -618,10 +624,10 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
           }
         }
       }
-      __syncwarp();
-      fill(stage);
+      stage ^= 1;
+      store_scales(stage);
+      __syncwarp();  // this unit's stage may be filled again
       read_scales();
-      stage = stage + 1 == STAGES ? 0 : stage + 1;
     }
 
     // join the warps
