@@ -68,10 +68,25 @@ __device__ __forceinline__ void decode4_8bit(uint32_t w, uint32_t &p0, uint32_t 
         : "r"(w));
   }
 }
-// 8 nibbles -> 4 fp16 pairs: INT4 pairs (i, i + 4), FP4 pairs (2i, 2i + 1).
+// 8 nibbles -> 4 fp16 pairs: INT4 pairs (i, i + 4), FP4 pairs (2i, 2i + 1). INT4: with the sign bit
+// flipped a nibble under 0x64 is fp16 1024 + (c + 8), four bits higher 1024 + 16 (c + 8): mask and flip
+// are one operation.
 template <int F>
 __device__ __forceinline__ void decode8_4(uint32_t w, uint32_t (&p)[4]) {
-  gemv::decode8_4bit<F == B200_CACHE_INT4 ? B200_FMT_INT4 : B200_FMT_FP4_E2M1>(w, p);
+  if constexpr (F == B200_CACHE_INT4) {
+    const uint32_t hi = w >> 8;
+    const uint32_t h[4] = {(w & 0x000F000Fu) ^ 0x64086408u, (w & 0x00F000F0u) ^ 0x64806480u,
+                           (hi & 0x000F000Fu) ^ 0x64086408u, (hi & 0x00F000F0u) ^ 0x64806480u};
+    const __half2 one = __float2half2_rn(1032.f), sixteenth = __float2half2_rn(0.0625f), off = __float2half2_rn(-72.f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 x = *reinterpret_cast<const __half2 *>(&h[i]);
+      const __half2 r = i % 2 ? __hfma2(x, sixteenth, off) : __hsub2(x, one);
+      p[i] = *reinterpret_cast<const uint32_t *>(&r);
+    }
+  } else {
+    gemv::decode8_4bit<B200_FMT_FP4_E2M1>(w, p);
+  }
 }
 
 }  // namespace cache
