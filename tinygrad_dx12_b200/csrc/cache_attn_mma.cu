@@ -1020,9 +1020,6 @@ static int32_t launch_d(Params &p, int dim, bool blk, cudaStream_t stream) {
   if (two) return blk ? launch_t<F, 128, 2, true>(p, stream) : launch_t<F, 128, 2, false>(p, stream);
   return blk ? launch_t<F, 128, 1, true>(p, stream) : launch_t<F, 128, 1, false>(p, stream);
 }
-#ifdef DEV_ONE
-static int32_t launch_f(Params &p, int fmt, int dim, bool blk, cudaStream_t stream) { return launch_t<DEV_F, DEV_D, DEV_RT, DEV_B>(p, stream); }
-#else
 static int32_t launch_f(Params &p, int fmt, int dim, bool blk, cudaStream_t stream) {
   switch (fmt) {
     case B200_CACHE_INT8: return launch_d<B200_CACHE_INT8>(p, dim, blk, stream);
@@ -1032,7 +1029,6 @@ static int32_t launch_f(Params &p, int fmt, int dim, bool blk, cudaStream_t stre
   }
 }
 
-#endif
 }  // namespace mma
 
 bool mma_supported(const Params &p, int dim) { return dim <= 128 && p.rows > 16; }

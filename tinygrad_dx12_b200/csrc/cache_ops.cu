@@ -359,11 +359,12 @@ __device__ __forceinline__ void encode8_scaled(float (&y)[8], float sc, uint8_t 
 }
 
 // The usual shapes of 16-bit inputs: a lane holds the two vectors of 8 values that turn together (or
-// two that pass), dim / 16 lanes a row, so that every value is read once; four rows in flight. INTER:
+// two that pass), dim / 16 lanes a row, so that every value is read once; two rows in flight a lane and 8
+// CTAs an SM (one CTA a token spends its time in the chain position -> angles -> store). INTER:
 // interleaved pairs, or none to turn (cos null).
-constexpr int PT = 128, PR = 3;
+constexpr int PT = 128, PR = 2;
 template <typename T, int F, int D, bool INTER>
-__global__ void __launch_bounds__(PT, 6) cache_write_pairs_kernel(const WriteArgs a) {
+__global__ void __launch_bounds__(PT, 8) cache_write_pairs_kernel(const WriteArgs a) {
   pdl_enter();
   constexpr int LPR = D / 16, RPC = PT / LPR;
   const int j = threadIdx.x % LPR, slot_row = threadIdx.x / LPR, step = RPC * gridDim.y;
