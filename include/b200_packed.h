@@ -322,8 +322,12 @@ int32_t b200_cache_read(const b200_cache_desc *cache, const void *slots, int32_t
  * b200_device_status. q: F16 or BF16, element strides (request, token, head), unit along head_dim;
  * out: contiguous [batch, queries, heads, head_dim] of q's type; lse: fp32 [batch, queries, heads]
  * natural logarithms of the softmax sums, or NULL. `scratch` holds b200_cache_attention_scratch()
- * bytes (prefix only). Allocates a workspace (10 MiB) on the first call per (device, stream); when
- * that first call is captured into a graph it runs without one, with less parallelism. */
+ * bytes (prefix only). A NaN in a key's or value's scale makes the rows that see that key NaN, in all
+ * their values. Allocates workspaces for the life of the process on the first call per (device,
+ * stream): 5 MiB, and 38 MiB more when a key head first has over 64 query rows (queries, or batch x
+ * queries for the prefix, x heads / kv_heads); a first call that is captured into a graph runs
+ * without, with less parallelism. More than 262144 query rows of a key head, 32768 for head_dim
+ * 256: B200_ERR_UNSUPPORTED. */
 typedef struct b200_attention_args {
   const void *q;
   int64_t q_strides[3];

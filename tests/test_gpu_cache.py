@@ -531,6 +531,30 @@ def test_attention_outliers_that_are_not_seen(rows, fmt, blocked):
             assert not o.isnan().any() and torch.equal(o[1], good[1])
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("blocked,e8", [(False, False), (False, True), (True, False), (True, True)])
+@pytest.mark.parametrize("queries,heads,kv", [(17, 8, 2), (33, 12, 2)])
+def test_attention_many_rows_formats(fmt, dim, blocked, e8, queries, heads, kv):
+    """68 and 198 query rows of a key head; lengths that end inside the block, before it and behind it."""
+    Case([queries, 0, 200, 3, 129], queries=queries, heads=heads, kv=kv, dim=dim, fmt=fmt, blocked=blocked, e8=e8,
+         order="tokens" if e8 else "heads", seed=93).check()
+
+
+@pytest.mark.parametrize("queries,heads,kv", [(1, 16, 1), (1, 17, 1), (16, 4, 1), (13, 5, 1), (32, 4, 1), (43, 3, 1), (4, 16, 1)])
+@pytest.mark.parametrize("prefix", [0, 1, 131])
+def test_attention_rows_where_kernels_change(queries, heads, kv, prefix):
+    Case([queries + 2, 0, 140, 31], queries=queries, heads=heads, kv=kv, dim=64, fmt="int8", prefix=prefix, seed=94).check()
+
+
+@pytest.mark.parametrize("fmt,dim,lengths", [("int4", 64, [4096, 300]), ("int8", 128, [129, 1025, 0, 2047]), ("fp8e4m3", 256, [700])])
+def test_attention_segments_cut_to_single_rounds(fmt, dim, lengths):
+    c = Case(lengths, heads=8, kv=2, dim=dim, fmt=fmt, page=64, seed=95)
+    a, b = c.run(), c.run()
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    c.check(*a)
+
+
 @pytest.mark.parametrize("blocked", [False, True])
 def test_attention_many_rows_value_ranges(blocked):
     """Scales that span 2^40 from key to key under many query rows."""

@@ -27,10 +27,16 @@
 //
 // The units of all (request, key head, row tile) segments are laid end to end in rounds (a unit for
 // each warp) and cut into equal runs, one per CTA, from the lengths on the device: ragged batches
-// balance, and the launch (a CUDA graph) does not depend on the lengths. Where there is little work,
-// segments start on run boundaries instead, so that short ones are not cut. A CTA's warps join in
+// balance, and the launch (a CUDA graph) does not depend on the lengths. A CTA's warps join in
 // shared memory; a segment cut over several CTAs is joined by the CTA that finishes last, always in
-// the same order.
+// the same order. Cuts pay down to single rounds: segments kept whole up to four rounds took 22.7 us
+// instead of 12.2 for 4 requests of 4096 int4 keys, and 7.0 instead of 7.4 at 300 int8 keys.
+//
+// Measured (bf16, 8 key heads of 128, device time): 64 requests of 2048 to 8192 keys, 64 heads, FP4 in
+// blocks: 138 us = 2.6 TB/s. Bound by instruction issue there: about 470 warp instructions for each 16
+// keys of a key head, two thirds of them decoding and turning codes, at 0.52 an SM quarter and cycle. 32
+// requests of 8192 keys: int8 4.2 TB/s, fp8 4.6 TB/s. One request of 257 int8 keys: 8.6 us, a chain of
+// launch, lengths, page numbers, codes, two products, the warps' and the CTAs' joins.
 #include <map>
 #include <mutex>
 
@@ -48,7 +54,6 @@ namespace cattn {
 
 constexpr int WARPS = 8, THREADS = WARPS * 32, STAGES = 2;
 constexpr int MAX_ENTRIES = 4096;    // (request, row tile) pairs of one launch
-constexpr int SHORT = 4;             // rounds that a segment is not cut below where work is scarce
 
 template <int F, int D, int NT, bool BLK>
 struct Cfg {
@@ -121,7 +126,7 @@ template <typename T, int F, int D, int NT, bool BLK>
 __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel(const Params p) {
   using C = Cfg<F, D, NT, BLK>;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint32_t scan[2 * WARPS];
+  __shared__ uint32_t scan[WARPS];
   __shared__ uint32_t last;
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -151,44 +156,39 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
     return max(0, n - p.queries + r1 / p.group + 1);
   };
   auto rounds_of = [&](int keys) -> uint32_t { return ((uint32_t)keys + ROUND - 1) / ROUND; };
-  auto aligned = [&](uint32_t r) -> uint32_t { return (r + SHORT - 1) / SHORT * SHORT; };
 
-  // rounds of the entries, summed up: as they are, and with segments padded to SHORT
-  uint32_t per;
-  bool pad;
+  uint32_t per;  // rounds of a CTA; the entries' are summed up
   {
     const int each = (entries + THREADS - 1) / THREADS, e0 = tid * each;
-    uint32_t sum = 0, psum = 0;
+    uint32_t sum = 0;
     for (int i = 0; i < each; ++i)
       if (e0 + i < entries) {
         const uint32_t r = rounds_of(keys_of(e0 + i));
         prefix[e0 + i] = r;
-        sum += r, psum += aligned(r);
+        sum += r;
       }
-    uint32_t inc = sum, pinc = psum;
+    uint32_t inc = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, inc, o), w = __shfl_up_sync(0xFFFFFFFFu, pinc, o);
-      if (lane >= o) inc += v, pinc += w;
+      const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+      if (lane >= o) inc += v;
     }
-    if (lane == 31) scan[warp] = inc, scan[WARPS + warp] = pinc;
+    if (lane == 31) scan[warp] = inc;
     __syncthreads();
-    uint32_t base = 0, pbase = 0, total = 0, ptotal = 0;
+    uint32_t base = 0, total = 0;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
-      if (w < warp) base += scan[w], pbase += scan[WARPS + w];
-      total += scan[w], ptotal += scan[WARPS + w];
+      if (w < warp) base += scan[w];
+      total += scan[w];
     }
     per = (uint32_t)(((uint64_t)total * heads + gridDim.x - 1) / gridDim.x);
-    pad = split && per <= 1;
-    if (pad) per = aligned((uint32_t)(((uint64_t)ptotal * heads + gridDim.x - 1) / gridDim.x));
     if (per == 0) per = 1;
-    uint32_t run = pad ? pbase + pinc - psum : base + inc - sum;
+    uint32_t run = base + inc - sum;
     for (int i = 0; i < each; ++i)
       if (e0 + i < entries) {
         const uint32_t r = prefix[e0 + i];
         prefix[e0 + i] = run;
-        run += pad ? aligned(r) : r;
+        run += r;
         if (e0 + i == entries - 1) prefix[entries] = run;
       }
     __syncthreads();
@@ -779,7 +779,7 @@ static int32_t launch_t(Params p, cudaStream_t stream) {
     return b200_set_error(B200_ERR_UNSUPPORTED, "cache_attention: too many query rows (%d of a key head)", p.rows);
   const int64_t round = C::T * WARPS;
   const int64_t cap = p.lengths != nullptr ? ((int64_t)p.max_pages << p.page_shift) : p.fixed;
-  const int64_t rounds = ((cap + round - 1) / round + SHORT) * p.kv_heads * p.row_tiles;  // of a request
+  const int64_t rounds = ((cap + round - 1) / round) * p.kv_heads * p.row_tiles;  // of a request
   if (rounds > (1 << 29)) return b200_set_error(B200_ERR_UNSUPPORTED, "cache_attention: too many keys for one launch");
   int at_once = MAX_ENTRIES / p.row_tiles;
   if (rounds * at_once > (1 << 29)) at_once = (int)((1 << 29) / rounds);
@@ -825,7 +825,9 @@ static int32_t launch_t(Params p, cudaStream_t stream) {
 
 template <typename T, int F>
 static int32_t launch_d(const Params &p, int dim, bool blk, cudaStream_t stream) {
-  const bool two = p.rows > 8;  // 16 query rows share a pass over the keys
+  // Nine rows and more share a pass over the keys 16 at a time: two query tokens of 32 requests take 104
+  // us instead of 141; where one request leaves SMs idle (4 tokens, 8192 keys), 19.8 us instead of 17.8.
+  const bool two = p.rows > 8;
   if (dim == 64) {
     if (two) return blk ? launch_t<T, F, 64, 2, true>(p, stream) : launch_t<T, F, 64, 2, false>(p, stream);
     return blk ? launch_t<T, F, 64, 1, true>(p, stream) : launch_t<T, F, 64, 1, false>(p, stream);

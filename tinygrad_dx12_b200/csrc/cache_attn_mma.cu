@@ -15,7 +15,12 @@
 // Two row tiles share every decoded key tile (256 rows); with up to 128 rows both warpgroups take the
 // same rows and every other key tile each, and add up at the end. While one slot is in its softmax the
 // other's products run. What bounds it: a tile pair is 2048 cycles of MMA, as many of the special
-// function unit (one exponential a score) and about 9000 issue slots of four schedulers.
+// function unit (one exponential a score) and about 9000 issue slots of four schedulers. It takes some
+// 5300 cycles: a softmax (2400) and the round trip of its products (2650) follow one another in each
+// slot, and the two slots fill each other's gaps only in part.
+// Measured (bf16, 8 key heads of 128, device time): 1024 tokens of 32 heads against 8192 fp8 keys 215 us
+// = 600 TFLOP/s (the few-row kernel 1087); 128 requests of 64 heads behind 16384 int4 keys, with their
+// own 1 to 1024, 207 us (595).
 //
 // Tiles of all (row tile, key head) segments are laid end to end and cut into equal runs, one per CTA.
 // A segment within a run is finished there; the others leave their share (numerators, maximum,
@@ -1012,6 +1017,8 @@ static int32_t launch_t(Params &p, cudaStream_t stream) {
 
 template <int F>
 static int32_t launch_d(Params &p, int dim, bool blk, cudaStream_t stream) {
+  // Up to 128 rows: both softmax warpgroups on the same rows (64 rows, 8192 keys: 42.3 us, with one of
+  // them idle 46.4).
   const bool two = p.rows > 128;
   if (dim == 64) {
     if (two) return blk ? launch_t<F, 64, 2, true>(p, stream) : launch_t<F, 64, 2, false>(p, stream);
@@ -1031,7 +1038,11 @@ static int32_t launch_f(Params &p, int fmt, int dim, bool blk, cudaStream_t stre
 
 }  // namespace mma
 
-bool mma_supported(const Params &p, int dim) { return dim <= 128 && p.rows > 16; }
+// The few-row kernel reads and decodes the keys again for every 16 rows, this one for every 256, with a
+// dearer start. Device us there and here: 8192 fp8 keys, 64 rows 34.9 and 43.1, 128 rows 50.0 and 41.6;
+// 32768 keys, 64 rows 84 and 99, 128 rows 146 and 92; 16 requests of FP4 blocks, 48 rows 155 and 200, 64
+// rows 202 and 202, 80 rows 248 and 204; an int4 prefix of 16384, 64 rows 72 and 80, 96 rows 88 and 83.
+bool mma_supported(const Params &p, int dim) { return dim <= 128 && p.rows > 64; }
 
 int32_t launch_mma(Params &p, int q_dtype, int fmt, int dim, bool blk, cudaStream_t stream) {
   p.q_bf16 = q_dtype == B200_DT_BF16;
