@@ -34,9 +34,9 @@
 //
 // Measured (bf16, 8 key heads of 128, device time): 64 requests of 2048 to 8192 keys, 64 heads, FP4 in
 // blocks: 138 us = 2.6 TB/s. Bound by instruction issue there: about 470 warp instructions for each 16
-// keys of a key head, two thirds of them decoding and turning codes, at 0.52 an SM quarter and cycle. 32
-// requests of 8192 keys: int8 4.2 TB/s, fp8 4.6 TB/s. One request of 257 int8 keys: 8.6 us, a chain of
-// launch, lengths, page numbers, codes, two products, the warps' and the CTAs' joins.
+// keys of a key head, at 0.52 an SM quarter and cycle. 32 requests of 8192 keys: int8 4.2 TB/s, fp8 4.6
+// TB/s. One request of 257 int8 keys: 8.8 us, a chain of launch, lengths, page numbers, codes, two
+// products, the warps' and the CTAs' joins.
 #include <map>
 #include <mutex>
 
