@@ -555,6 +555,40 @@ def test_attention_segments_cut_to_single_rounds(fmt, dim, lengths):
     c.check(*a)
 
 
+def test_attention_prefix_over_many_launches():
+    """More requests than one launch takes, behind a prefix whose segments are cut."""
+    lengths = torch.randint(0, 20, (4500,), generator=gen(96)).tolist()
+    Case(lengths, heads=2, kv=1, dim=64, fmt="int4", prefix=600, seed=97).check()
+
+
+def test_attention_prefix_follows_its_inputs():
+    """Queries, keys and lengths that the launches right before have written: the same bits as when each
+    call waits for everything before it."""
+    c = Case([90, 33, 64, 2] * 12, heads=16, kv=2, fmt="int8", prefix=1500, seed=98)
+    tables, prefix = c.tables.to(torch.int32).cuda(), c.prefix.to(torch.int32).cuda()
+    last = torch.stack([o[n - 1] for o, n in zip(c.own, c.lengths)]).cuda()
+    qs = [torch.randn(c.q.shape, generator=gen(i)).to(c.q.dtype).cuda() for i in range(8)]
+    xs = [randn((len(c.lengths), 2, 128), 200 + i).cuda() for i in range(8)]
+    ns = [torch.tensor([max(0, n - i) for n in c.lengths], dtype=torch.int32).cuda() for i in range(8)]
+    q, n = torch.empty_like(qs[0]), torch.empty_like(ns[0])
+
+    def step(i, wait):
+        q.copy_(qs[i]), n.copy_(ns[i])
+        tg.cache_write(c.cache, xs[i], xs[i], last)
+        if wait:
+            torch.cuda.synchronize()
+        out = tg.cache_attention(q, c.cache, tables, n, prefix=prefix, prefix_length=1500)
+        if wait:
+            torch.cuda.synchronize()
+        return out
+
+    good = [step(i, True) for i in range(8)]
+    for _ in range(10):
+        fast = [step(i, False) for i in range(8)]
+        assert all(torch.equal(a, b) for a, b in zip(fast, good))
+    assert not torch.equal(good[0], good[1])
+
+
 @pytest.mark.parametrize("blocked", [False, True])
 def test_attention_many_rows_value_ranges(blocked):
     """Scales that span 2^40 from key to key under many query rows."""

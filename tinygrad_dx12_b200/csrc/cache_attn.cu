@@ -130,7 +130,8 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
   __shared__ uint32_t last;
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  auto await = []() { asm volatile("griddepcontrol.wait;" ::: "memory"); };
+  if (!p.early) await();  // else before the prefix's partials are read
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   uint8_t *ring = smem + warp * STAGES * C::STAGE;
@@ -198,6 +199,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
   // rows without a key: zeros (or what the prefix gave)
   for (int e = blockIdx.x; e < entries; e += gridDim.x) {
     if (prefix[e + 1] != prefix[e]) continue;
+    if (p.early) await();
     const int b = e / p.row_tiles, rt = e - b * p.row_tiles;
     const int n = min(C::ROWS, p.rows - rt * C::ROWS);
     for (int i = tid; i < heads * n * (D / 4); i += THREADS) {
@@ -401,19 +403,6 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
 
   while (c.u < u_end) {
     const uint32_t real = rounds_of(c.keys), from = c.u - c.seg0, to = min(u_end, c.seg1) - c.seg0;
-    const uint32_t upto = min(to, real);
-    if (from >= real) {  // padding alone: the ring goes on
-      for (uint32_t i = from; i < to; ++i) {
-        stage ^= 1;
-        issue_codes(stage);
-        store_scales(stage);
-        read_scales();
-      }
-      c.u = c.seg0 + to;
-      if (c.u == c.seg1) next_segment(c);
-      if (c.u < u_end) read_q(c);
-      continue;
-    }
     const int rt = c.e - c.b * p.row_tiles, r0 = rt * C::ROWS, n_rows = min(C::ROWS, p.rows - r0);
     const int len = length_of(c.b);
 
@@ -631,8 +620,9 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
     }
 
     // join the warps
+    if (p.early) await();
     Walk following = c;
-    const bool whole = from == 0 && upto == real;
+    const bool whole = from == 0 && to == real;
     const uint32_t c0 = split ? c.seg0 / per : 0, c1 = split ? (c.seg0 + real - 1) / per : 0;  // CTAs of the segment
     const int slot = (int)(2 * blockIdx.x + (from == 0 ? 1 : 0));
 #pragma unroll
@@ -724,6 +714,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
     c = following;
   }
   cp_async_wait<0>();
+  if (p.early) await();  // the launch behind this one takes this one's end for that of all before it
 }
 
 // ---- per-(device, stream) workspace of split segments ---------------------------------------------
@@ -795,6 +786,7 @@ static int32_t launch_t(Params p, cudaStream_t stream) {
       p.out = (T *)p.out + rows * D;
       if (p.lse != nullptr) p.lse += rows;
       p.row0 += rows;
+      if (b > 0) p.early = 0;  // these share the workspace with the launch before
       if (int32_t rc = launch_t<T, F, D, NT, BLK>(p, stream)) return rc;
     }
     return B200_OK;
@@ -872,6 +864,7 @@ static int32_t attention(const b200_cache_desc *c, const b200_attention_args *a,
     return a->q_dtype == B200_DT_F16 ? launch_f<__half>(q, c->format, dim, blk, stream)
                                      : launch_f<__nv_bfloat16>(q, c->format, dim, blk, stream);
   };
+  bool joined = false;
   if (a->prefix_length > 0) {
     Params f = p;  // every row of the batch against the prefix: one request of batch * queries tokens
     f.tables = a->prefix, f.table_stride = 0, f.max_pages = (int)a->prefix_pages;
@@ -880,10 +873,13 @@ static int32_t attention(const b200_cache_desc *c, const b200_attention_args *a,
     f.po = (float *)a->scratch, f.pm = f.po + all_rows * dim, f.pl = f.pm + all_rows;
     if (int32_t rc = run(f)) return rc;
     p.fo = f.po, p.fm = f.pm, p.fl = f.pl;
+    joined = f.ws_o != nullptr;
   }
   p.tables = a->tables, p.table_stride = a->table_stride, p.max_pages = (int)a->max_pages, p.lengths = a->lengths;
   p.batch = (int)a->batch, p.queries = (int)a->queries, p.rows = p.queries * p.group, p.causal = 1;
   p.out = a->out, p.lse = a->lse;
+  // The few-row kernel works on its first keys while the prefix's cut segments are joined.
+  p.early = joined && !mma_supported(p, dim);
   return run(p);
 }
 

@@ -41,6 +41,7 @@ struct Params {
   float *po, *pm, *pl;
   const float *fo, *fm, *fl;  // partials of the shared prefix, joined at the end
   int64_t row0;               // rows before these in fo, fm, fl
+  int early;  // the launch before is the join_kernel that completes these partials: nothing else is waited for
   // split segments
   float *ws_o, *ws_ml;
   uint32_t *tickets;

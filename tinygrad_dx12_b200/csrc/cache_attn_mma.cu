@@ -885,8 +885,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
 template <int D>
 __global__ void __launch_bounds__(256) join_kernel(const Params p, int tile_rows, uint32_t ctas) {
   __shared__ uint32_t prefix[MAX_ENTRIES + 1];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  // only now: what starts from here on finds all launches before this one complete (Params::early)
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   scan_entries(p, tile_rows, prefix);
   __syncthreads();
   const int entries = p.batch * p.row_tiles, chunks = tile_rows / 32 * (D / 32);
