@@ -33,9 +33,9 @@
 // instead of 12.2 for 4 requests of 4096 int4 keys, and 7.0 instead of 7.4 at 300 int8 keys.
 //
 // Measured (bf16, 8 key heads of 128, device time): 64 requests of 2048 to 8192 keys, 64 heads, FP4 in
-// blocks: 138 us = 2.6 TB/s. Bound by instruction issue there: about 470 warp instructions for each 16
-// keys of a key head, at 0.52 an SM quarter and cycle. 32 requests of 8192 keys: int8 4.2 TB/s, fp8 4.6
-// TB/s. One request of 257 int8 keys: 8.8 us, a chain of launch, lengths, page numbers, codes, two
+// blocks: 128 us = 2.8 TB/s. Bound by instruction issue there: about 500 warp instructions for each 16
+// keys of a key head, at 0.62 an SM quarter and cycle. 32 requests of 8192 keys: int8 4.2 TB/s, fp8 4.6
+// TB/s. One request of 257 int8 keys: 8.6 us, a chain of launch, lengths, page numbers, codes, two
 // products, the warps' and the CTAs' joins.
 #include <map>
 #include <mutex>

@@ -20,7 +20,7 @@
 // slot, and the two slots fill each other's gaps only in part.
 // Measured (bf16, 8 key heads of 128, device time): 1024 tokens of 32 heads against 8192 fp8 keys 215 us
 // = 600 TFLOP/s (the few-row kernel 1087); 128 requests of 64 heads behind 16384 int4 keys, with their
-// own 1 to 1024, 207 us (595).
+// own 1 to 1024, 197 us (595).
 //
 // Tiles of all (row tile, key head) segments are laid end to end and cut into equal runs, one per CTA.
 // A segment within a run is finished there; the others leave their share (numerators, maximum,
