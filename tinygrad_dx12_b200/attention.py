@@ -153,18 +153,45 @@ def _index(t: torch.Tensor, name: str, shape, device) -> torch.Tensor:
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _turned(x, table, positions, transpose, out=None):
+    """``rotary`` of operands that have been checked, but for ``out``."""
+    device = x.device
+    xs = x.stride()
+    if xs[-1] != 1:
+        x = x.contiguous()
+        xs = x.stride()
+    if out is None:
+        out = torch.empty_like(x)  # x's own order of axes where that is dense
+        if out.stride(-1) != 1:
+            out = torch.empty(x.shape, dtype=x.dtype, device=device)
+    elif out.shape != x.shape or out.dtype != x.dtype or out.device != device:
+        raise ValueError("out must have x's shape, type and device")
+    ys = out.stride()
+    if ys[-1] != 1:
+        raise ValueError("out must have contiguous heads")
+    shape = x.shape
+    if len(shape) == 4:
+        b, t, xb, yb = shape[0], shape[1], xs[0], ys[0]
+    else:
+        b, t, xb, yb = 1, shape[0], 0, 0
+    _call("b200_rotary", device, x.data_ptr(), _REAL[x.dtype], b, t, shape[-2], shape[-1], xb, xs[-3], xs[-2],
+          out.data_ptr(), yb, ys[-3], ys[-2], table._ref, positions.data_ptr(), _INDEX[positions.dtype], int(transpose))
+    return out
+
+
 class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, table, positions, transpose):
         ctx.table, ctx.transpose = table, transpose
         ctx.save_for_backward(positions)
-        return rotary(x, table, positions, transpose)
+        return _turned(x, table, positions, transpose)
 
     @staticmethod
     def backward(ctx, dy):
         # the map is linear: its gradient is the transposed map
         (positions,) = ctx.saved_tensors
-        return rotary(dy, ctx.table, positions, not ctx.transpose), None, None, None
+        turn = rotary if dy.requires_grad else _turned
+        return turn(dy, ctx.table, positions, not ctx.transpose), None, None, None
 
 
 def rotary(x: torch.Tensor, table: RotaryTable, positions: torch.Tensor, transpose: bool = False,
@@ -193,27 +220,7 @@ def rotary(x: torch.Tensor, table: RotaryTable, positions: torch.Tensor, transpo
         if out is not None:
             raise ValueError("rotary with a gradient cannot write into out")
         return _Rotary.apply(x, table, positions, transpose)
-    xs = x.stride()
-    if xs[-1] != 1:
-        x = x.contiguous()
-        xs = x.stride()
-    if out is None:
-        out = torch.empty_like(x)  # x's own order of axes where that is dense
-        if out.stride(-1) != 1:
-            out = torch.empty(x.shape, dtype=x.dtype, device=device)
-    elif out.shape != x.shape or out.dtype != x.dtype or out.device != device:
-        raise ValueError("out must have x's shape, type and device")
-    ys = out.stride()
-    if ys[-1] != 1:
-        raise ValueError("out must have contiguous heads")
-    shape = x.shape
-    if len(shape) == 4:
-        b, t, xb, yb = shape[0], shape[1], xs[0], ys[0]
-    else:
-        b, t, xb, yb = 1, shape[0], 0, 0
-    _call("b200_rotary", device, x.data_ptr(), _REAL[x.dtype], b, t, shape[-2], shape[-1], xb, xs[-3], xs[-2],
-          out.data_ptr(), yb, ys[-3], ys[-2], table._ref, positions.data_ptr(), _INDEX[positions.dtype], int(transpose))
-    return out
+    return _turned(x, table, positions, transpose, out)
 
 
 # ---- the cache ----------------------------------------------------------------------------------
