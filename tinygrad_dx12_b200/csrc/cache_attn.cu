@@ -6,8 +6,10 @@
 // One pass over the keys. With everything in base 2, u = s + log2 vs[t] and a running maximum m of
 // u, a key adds p * vc[t] (p = 2^(u - m + 11)) to the numerator and p / vs[t] to the denominator:
 // codes enter the matrix instructions as they are stored, exact in fp16, and no scale is multiplied
-// into them. p <= 2^15 is rounded to fp16 for the second product (11 bits down to 2^-25 of the
-// largest weight); sums, statistics and the denominator are fp32. q is scaled by a power of two per row, so that bf16 values fit fp16.
+// into them. vs is at least 2^-100 here, which stands for values of zero too, and the denominator is kept
+// as 2^-20 of itself, so that it bears any number of such keys. p <= 2^15 is rounded to fp16 for the
+// second product (11 bits down to 2^-25 of the largest weight); sums, statistics and the denominator are
+// fp32. q is scaled by a power of two per row, so that bf16 values fit fp16.
 // Blocks of 32 values with scales of their own: the codes are multiplied by scale / 2^E, with 2^E
 // just above the row's largest scale (shifted up by fp16's headroom, so that blocks down to 2^-26,
 // 8-bit 2^-20, of the largest keep their bits), and ks, vs above become 2^E.
@@ -348,8 +350,9 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
         widen<C::KNB>(rk[k], p.e8m0, kf);
         widen<C::KNB>(rv[k], p.e8m0, vf);
         if constexpr (!BLK) {
-          const float vsc = vf[0] < 0x1p-120f ? 0x1p-120f : vf[0];  // a scale of zero: weight without a value
-          lvi[key] = in ? make_float2(lg2(vsc), vsc == vsc ? __frcp_rn(vsc) : 0.f) : make_float2(-INFINITY, 0.f);
+          // values of zero, or a cell that was never written (scale 0): weight without a value
+          const float vsc = vf[0] < 0x1p-100f ? 0x1p-100f : vf[0];
+          lvi[key] = in ? make_float2(lg2(vsc), vsc == vsc ? __frcp_rn(vsc) * SUM_UNIT : 0.f) : make_float2(-INFINITY, 0.f);
           ks[key] = in ? kf[0] : 0.f;
         } else {
           uint32_t top = 0;  // magnitudes order as integers, NaN above all
@@ -359,7 +362,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
           float inv = RowRef<F>::inverse(e);
           // the row's NaN travels in its scores, which rows that do not see it drop
           lvi[key] = !in ? make_float2(-INFINITY, 0.f)
-                     : top > 0x7F800000u ? make_float2(__uint_as_float(top), 0.f) : make_float2((float)(e - 127), inv);
+                     : top > 0x7F800000u ? make_float2(__uint_as_float(top), 0.f) : make_float2((float)(e - 127), inv * SUM_UNIT);
           const bool use = in && top <= 0x7F800000u;
           __half *vk = vr + (key & ~7) + C::row_of(key & 7);  // ratios in the order of the instruction's rows
 #pragma unroll

@@ -12,6 +12,11 @@ using namespace cache;
 
 constexpr float LAZY = 4.f;          // u may pass the running maximum by this before it moves
 constexpr float BIAS = 15.f - LAZY;  // p = 2^(u - m + BIAS) uses fp16 up to 2^15, so small weights keep their bits
+// A key adds p / vs to the denominator: up to 2^15 * 2^100 where its values are zero (a block of zeros has
+// the scale 2^-100, no reference is below that), down to 2^11 / 2^100 where the largest are all that counts.
+// Sums are kept as 2^-SUM_EXP of themselves: 2^31 keys stay below 2^126, and 2^-109 is an ordinary number.
+constexpr int SUM_EXP = 20;
+constexpr float SUM_UNIT = 1.f / (1 << SUM_EXP);
 
 struct Params {
   const void *q;
@@ -78,12 +83,12 @@ __device__ __forceinline__ void lds(const uint8_t *p, uint32_t *w) {
   }
 }
 
-// 2^-(E - H): what a block's scale is multiplied by; 2^(E - H) is the row's scale.
+// 2^-(E - H): what a block's scale is multiplied by; 2^(E - H) is the row's scale, 2^-100 at least.
 template <int F>
 struct RowRef {
   static constexpr int H = CFmt<F>::bits == 4 ? 12 : 6;
   // `top`: bfloat16 bits of the row's largest scale
-  __device__ static __forceinline__ int exponent(uint32_t top) { return max((int)((top >> 7) & 0xFF), H + 1) - H; }
+  __device__ static __forceinline__ int exponent(uint32_t top) { return max((int)((top >> 7) & 0xFF) - H, 27); }
   __device__ static __forceinline__ float inverse(int e) { return __uint_as_float((uint32_t)(254 - e) << 23); }
   __device__ static __forceinline__ float value(int e) { return __uint_as_float((uint32_t)e << 23); }
 };
@@ -152,6 +157,17 @@ __device__ __forceinline__ void join(float4 &o, float &m, float &l, const float 
   m = M;
 }
 
+// What a numerator is multiplied by, one after the other: 2^-SUM_EXP / l in two parts that are ordinary numbers
+// (and so are the products) whatever the sum. No key seen: zeros.
+__device__ __forceinline__ float2 inverse_sum(float l) {
+  const bool small = l < 1.f;
+  return make_float2(l == 0.f ? 0.f : (small ? SUM_UNIT : 1.f) / l, small ? 1.f : SUM_UNIT);
+}
+// The natural logarithm of the softmax's sum.
+__device__ __forceinline__ float log_sum(float m, float l) {
+  return l == 0.f ? -INFINITY : (m - BIAS + (log2f(l) + SUM_EXP)) * 0.69314718055994531f;
+}
+
 // A row's result from its numerator (four values), maximum and denominator.
 template <typename T, int D>
 __device__ __forceinline__ void finish(const Params &p, int64_t row, int d, float4 o, float m, float l) {
@@ -163,11 +179,12 @@ __device__ __forceinline__ void finish(const Params &p, int64_t row, int d, floa
   if (p.fo != nullptr) {
     join<D>(o, m, l, p.fo + (p.row0 + row) * D + d, p.fm[p.row0 + row], p.fl[p.row0 + row]);
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;  // no key seen: zeros
+  const float2 f = inverse_sum(l);
   T *dst = (T *)p.out + row * D + d;
-  alignas(8) T r[4] = {out_of<T>(o.x * inv), out_of<T>(o.y * inv), out_of<T>(o.z * inv), out_of<T>(o.w * inv)};
+  alignas(8) T r[4] = {out_of<T>(o.x * f.x * f.y), out_of<T>(o.y * f.x * f.y), out_of<T>(o.z * f.x * f.y),
+                       out_of<T>(o.w * f.x * f.y)};
   *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<const uint2 *>(r);
-  if (p.lse != nullptr && d == 0) p.lse[row] = l == 0.f ? -INFINITY : (m - BIAS + log2f(l)) * 0.69314718055994531f;
+  if (p.lse != nullptr && d == 0) p.lse[row] = log_sum(m, l);
 }
 
 

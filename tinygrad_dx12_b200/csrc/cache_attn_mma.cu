@@ -520,7 +520,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
       const int64_t place = (int64_t)(2 * blockIdx.x + (w.from == 0 ? 1 : 0)) * TR + (RT == 2 ? slot * 128 : 0) + r;
       if constexpr (RT == 2) {
         const bool plain = whole && p.po == nullptr && p.fo == nullptr;
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const float2 inv = inverse_sum(l);
         const uint32_t rowbuf = smem_u32(qt + slot * C::QB);
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
@@ -534,7 +534,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
               uint32_t y[4];
 #pragma unroll
               for (int x = 0; x < 4; ++x) {
-                const float f0 = __uint_as_float(o[i + 2 * x]) * inv, f1 = __uint_as_float(o[i + 2 * x + 1]) * inv;
+                const float f0 = __uint_as_float(o[i + 2 * x]) * inv.x * inv.y, f1 = __uint_as_float(o[i + 2 * x + 1]) * inv.x * inv.y;
                 const __nv_bfloat162 h = __floats2bfloat162_rn(f0, f1);
                 y[x] = p.q_bf16 ? *reinterpret_cast<const uint32_t *>(&h) : pack_f16(f0, f1);
               }
@@ -563,7 +563,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
           }
           __syncwarp();
         }
-        if (in && plain && p.lse != nullptr) p.lse[at.out] = l == 0.f ? -INFINITY : (m - BIAS + log2f(l)) * 0.69314718055994531f;
+        if (in && plain && p.lse != nullptr) p.lse[at.out] = log_sum(m, l);
         if (in && !whole) *reinterpret_cast<float2 *>(p.ws_ml + place * 2) = make_float2(m, l);
       } else {
         // the second warpgroup's share goes through its own and the first's query tile
@@ -736,8 +736,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
         // a NaN scale: in the score, which rows that do not see the key drop
         k_s[0] = s_in && !kn ? ks : 0.f;
         k_s[KT] = !s_in ? -INFINITY : kn || vn ? nan : (float)(ve - 127);
-        k_s[2 * KT] = s_in && !vn ? RowRef<F>::inverse(ve) : 0.f;
-        if (i128 == 0) tile_s[n & 3] = make_float4(fold ? ks : 1.f, (float)(ve - 127), RowRef<F>::inverse(ve), each ? 1.f : 0.f);
+        k_s[2 * KT] = s_in && !vn ? RowRef<F>::inverse(ve) * SUM_UNIT : 0.f;
+        if (i128 == 0)
+          tile_s[n & 3] = make_float4(fold ? ks : 1.f, (float)(ve - 127), RowRef<F>::inverse(ve) * SUM_UNIT, each ? 1.f : 0.f);
         const float kr = RowRef<F>::inverse(ke), vr = RowRef<F>::inverse(ve);
 #pragma unroll
         for (int i = 0; i < C::KNB; ++i) {
