@@ -136,3 +136,20 @@ def test_multi_destination_epilogue():
     torch.cuda.synchronize()
     for o in outs:
         assert torch.equal(o, expect)
+
+
+@pytest.mark.parametrize("fmt", ["fp4_e2m1", "fp6_e2m3", "fp6_e3m2"])
+@pytest.mark.parametrize("kind,sdt", [("e8m0", "e8m0"), ("f16row", None), (None, None)])
+@pytest.mark.parametrize("m", [1, 5])
+def test_products_wait_for_the_codes(fmt, kind, sdt, m):
+    """Weights that come from HBM while x lies in cache: the products of every call, whatever the scales, wait
+    for the copies of their codes, so every call gives the first one's bits, which are checked."""
+    from tinygrad_dx12_b200.linalg import _packed_linear
+
+    spec = _spec(fmt, 4096, 4096, 32 if kind != "f16row" else 4096, kind, 6)
+    w, x, y0 = _run(spec, sdt, m, "bfloat16", "float32", xscale=0.25)
+    flush = torch.empty(256 << 20, dtype=torch.uint8, device=DEV)  # twice L2
+    for _ in range(20):
+        flush.zero_()
+        x.add_(0)  # x is in cache again
+        assert torch.equal(_packed_linear(w, x, torch.float32, "mx"), y0)

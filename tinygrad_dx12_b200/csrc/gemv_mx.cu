@@ -252,7 +252,8 @@ __global__ void __launch_bounds__(THREADS, 1)
           ++seg;
           if (seg >= 2 && !mbar_wait(&accempty[seg & 1], (uint32_t)((seg / 2 - 1) & 1), abort_flag)) break;
         }
-        ok = mbar_wait(&sfready[slot], round & 1u, abort_flag);  // implies the codes, pieces and scales
+        // the pieces and all scales (sfready), and the codes: with row scales or none nobody else waits for them
+        ok = mbar_wait(&sfready[slot], round & 1u, abort_flag) && mbar_wait(&full[slot], round & 1u, abort_flag);
         if (!ok) break;
         tc_fence_after();
         const uint8_t *st = ring + (size_t)slot * p.stage_bytes;
