@@ -693,10 +693,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
       read_keys();
       read_values();
     }
+    // A thread whose wait ran out leaves with all others, at meet(), or they would wait for it there.
+    bool alive = true;
     for (uint32_t n = 0; here; ++n) {
       const uint32_t buf = n & 1, phase = ((n >> 1) - 1) & 1;
       const bool again = more;  // a tile follows this one
-      const bool free_ = n < 2 || mbar_wait(&bars.kfree[buf], phase, abort_flag, WAIT_NS);
+      alive = alive && (n < 2 || mbar_wait(&bars.kfree[buf], phase, abort_flag, WAIT_NS));
       // Scales. Where the tile's exponents lie close together, key and value codes take theirs relative to the
       // tile's (exactly, but for rounding products of 8-bit codes and bfloat16 scales to fp16) and the rows
       // need one of each; where not, or where a key is missing or NaN, relative to their own key's, and every
@@ -720,7 +722,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
         const bool any = __any_sync(0xFFFFFFFFu, !s_in || kn || vn);
         if (lane == 0) sp[0] = x0, sp[1] = x1, sp[2] = x2, sp[3] = x3, sp[4] = any;
       }
-      if (!meet<1, WG>(free_)) break;
+      if (!meet<1, WG>(alive)) break;
       {
         uint32_t kx = 0, ki = 255, vx = 0, vi = 255;
         bool each = false;
@@ -778,7 +780,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
       mbar_arrive(&bars.kfull[buf]);
       if (again) read_keys();
 
-      if (n >= 2 && !mbar_wait(&bars.vfree[buf], phase, abort_flag, WAIT_NS)) break;
+      alive = n < 2 || mbar_wait(&bars.vfree[buf], phase, abort_flag, WAIT_NS);
       const uint32_t va = smem_u32(vt + buf * C::VB);
       uint32_t r4[4];
       lds<16>((const uint8_t *)&vratio[(buf * C::KNB + (BLK ? vc * C::UD / 32 : 0)) * KT + 8 * kg], r4);
