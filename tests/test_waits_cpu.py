@@ -9,7 +9,7 @@ import re
 import pytest
 
 CSRC = pathlib.Path(__file__).resolve().parent.parent / "tinygrad_dx12_b200" / "csrc"
-SOURCES = sorted(CSRC.glob("cache_*.cu"))
+SOURCES = sorted(CSRC.glob("*.cu"))
 WAIT = re.compile(r"\bmbar_wait\w*\(")
 GROUP_BARRIER = re.compile(r"\b(meet<|epi_sync\(|tmem_sync\(|consumer_sync<)")
 LEAVES = re.compile(r"\b(break|return)\b")

@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     for (int64_t i = cw; i < n && cw < p.nact; i += p.nact) {
       const int slot = (int)(i % S);
       const uint32_t round = (uint32_t)(i / S);
-      if (i >= S && !mbar_wait(&empty[slot], (round - 1u) & 1u, abort_flag)) break;
+      if (i >= S && !__all_sync(0xFFFFFFFFu, mbar_wait(&empty[slot], (round - 1u) & 1u, abort_flag))) break;
       const int s = (int)((u0 + i) % p.nst);
       const uint16_t *xs = p.x + (int64_t)s * KS + 8 * lane;
       uint8_t *stg = ring + (size_t)slot * p.stage_bytes;
@@ -303,6 +303,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       if ((slot & 1) != set) continue;
       bool ok = mbar_wait(&bready[slot], round & 1u, abort_flag);
       if (SMODE == SM_E8M0) ok = ok && mbar_wait(&full[slot], round & 1u, abort_flag);
+      ok = __all_sync(0xFFFFFFFFu, ok);
       if (!ok) break;
       const int s = (int)((u0 + i) % p.nst);
       const uint8_t *st = ring + (size_t)slot * p.stage_bytes;
@@ -327,7 +328,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t lane_base = (uint32_t)((warp - EPI_WARP0) * 32) << 16;
     const uint32_t d_col[2] = {0u, p.d1_col};
     constexpr int TOK = P == 8 ? 1 : 8;  // tokens per accumulator read: TOK * P / 8 loads of 8 columns
-    bool waited = false;
+    bool waited = false, ok = true;  // ok: this warp's waits. After one that ran out it still meets the others
     int seg = 0;
     for (int64_t i = 0; i < n;) {
       const int64_t u = u0 + i;
@@ -336,9 +337,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       const bool whole = s0 == 0 && len == p.nst;
       i += len;
       const int buf = seg & 1;
-      if (!mbar_wait(&accfull[buf], (uint32_t)((seg / 2) & 1), abort_flag)) break;  // no sleep: the tail is latency
+      // no sleep: the tail is latency
+      ok = __all_sync(0xFFFFFFFFu, ok && mbar_wait(&accfull[buf], (uint32_t)((seg / 2) & 1), abort_flag));
       tc_fence_after();
-      if (!waited) {  // y, the partials and the tickets belong to the stream order
+      if (ok && !waited) {  // y, the partials and the tickets belong to the stream order
         asm volatile("griddepcontrol.wait;" ::: "memory");
         waited = true;
       }
@@ -349,7 +351,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int e = (u0 / p.nst == t) ? 0 : 1;  // this CTA's first or last tile
       float *mypart = p.part + ((size_t)blockIdx.x * 2 + e) * p.m * TM;
       // TOK tokens at a time: P * TOK accumulator columns
-      for (int m0 = 0; m0 < p.m; m0 += TOK) {
+      for (int m0 = 0; ok && m0 < p.m; m0 += TOK) {
         float acc[TOK];
 #pragma unroll
         for (int q = 0; q < TOK; ++q) acc[q] = 0.f;
@@ -388,13 +390,13 @@ __global__ void __launch_bounds__(THREADS, 1)
         epi_sync();
         if (threadIdx.x == EPI_WARP0 * 32) {
           __threadfence();
-          unsigned int old;
-          asm volatile("atom.add.acq_rel.gpu.u32 %0, [%1], 1;" : "=r"(old) : "l"(&p.tickets[t]) : "memory");
+          unsigned int old = ~0u;  // not counted: nobody finishes the tile
+          if (ok) asm volatile("atom.add.acq_rel.gpu.u32 %0, [%1], 1;" : "=r"(old) : "l"(&p.tickets[t]) : "memory");
           *last_flag = old == (unsigned int)(cl - cf) ? 1u : 0u;
         }
         epi_sync();
         if (*last_flag) {
-          if (row < p.rows) {
+          if (ok && row < p.rows) {
             for (int m0 = 0; m0 < p.m; m0 += 8) {  // 8 tokens at a time: all their loads in flight together
               float sum[8];
 #pragma unroll

@@ -336,7 +336,7 @@ __global__ void __launch_bounds__(THREADS, 1) mxs_kernel(const __grid_constant__
       uint2 nxt[4];
       if (i + 4 < n) load_unit(t, s, nxt);
       const int r = i % SFR;
-      if (i >= SFR && !mbar_wait(&sffree[r], (uint32_t)((i / SFR - 1) & 1), abort_flag)) break;
+      if (i >= SFR && !__all_sync(0xFFFFFFFFu, mbar_wait(&sffree[r], (uint32_t)((i / SFR - 1) & 1), abort_flag))) break;
       uint8_t *atom = sfa_atoms + (size_t)r * 1024 + 16 * lane;
       *reinterpret_cast<uint4 *>(atom) = make_uint4(cur[0].x, cur[1].x, cur[2].x, cur[3].x);
       *reinterpret_cast<uint4 *>(atom + 512) = make_uint4(cur[0].y, cur[1].y, cur[2].y, cur[3].y);
@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(THREADS, 1) mxs_kernel(const __grid_constant__
     // slower: the two tickets and reductions then pile up on the same late CTAs.)
     const int r = warp * 32 + lane;  // row within the tile = tensor-memory lane
     const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
-    bool waited = false, ok = true;
+    bool waited = false, ok = true;  // ok: this warp's waits. After one that ran out it still meets the others
     const uint32_t prank = p.pair ? cluster_rank() : 0u;
     float *pairbuf = reinterpret_cast<float *>(base + p.pair_off);
     if (p.pair) {
@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(THREADS, 1) mxs_kernel(const __grid_constant__
     }
     uint32_t ph = 0;  // phase bit of accfull[issuer][buffer]
     int seg = 0;
-    for (int i = 0; i < n && ok;) {
+    for (int i = 0; i < n;) {
       const int64_t u = u0 + i;
       const int t = (int)(u / p.nst), s0 = (int)(u % p.nst);
       const int len = (p.nst - s0) < (n - i) ? (p.nst - s0) : (n - i);
@@ -430,9 +430,9 @@ __global__ void __launch_bounds__(THREADS, 1) mxs_kernel(const __grid_constant__
           ok = ok && mbar_wait(&accfull[a], (ph >> a) & 1u, abort_flag);  // no sleep: the tail is latency
           ph ^= 1u << a;
         }
-      if (!ok) break;
+      ok = __all_sync(0xFFFFFFFFu, ok);
       tc_fence_after();
-      if (!waited) {  // y, the partials and the tickets belong to the stream order
+      if (ok && !waited) {  // y, the partials and the tickets belong to the stream order
         asm volatile("griddepcontrol.wait;" ::: "memory");
         waited = true;
       }
@@ -445,7 +445,7 @@ __global__ void __launch_bounds__(THREADS, 1) mxs_kernel(const __grid_constant__
       float mine[MAX_M];
 #pragma unroll
       for (int q = 0; q < MAX_M; ++q) mine[q] = 0.f;
-      for (int mm = 0; mm < p.m; ++mm) {
+      for (int mm = 0; ok && mm < p.m; ++mm) {
         float acc = 0.f;
         for (int k = 0; k < 2; ++k)
           if (contrib >> k & 1u) {
@@ -476,9 +476,9 @@ __global__ void __launch_bounds__(THREADS, 1) mxs_kernel(const __grid_constant__
       if (p.pair) {
         // second half: publish this thread's pushes; first half: add them after its own sums
         if (prank == 1u) {
-          mbar_arrive_cluster(map_rank(smem_u32(pairbar), 0u));
+          if (ok) mbar_arrive_cluster(map_rank(smem_u32(pairbar), 0u));
         } else {
-          ok = mbar_wait_cluster(pairbar, 0u, abort_flag);
+          ok = __all_sync(0xFFFFFFFFu, ok && mbar_wait_cluster(pairbar, 0u, abort_flag));
           if (ok && row < p.rows) {
             for (int mm = 0; mm < p.m; ++mm) {
               float mv = 0.f;
@@ -500,13 +500,13 @@ __global__ void __launch_bounds__(THREADS, 1) mxs_kernel(const __grid_constant__
       epi_sync();
       if (threadIdx.x == EPI_WARP0 * 32) {
         __threadfence();
-        unsigned int old;
-        asm volatile("atom.add.acq_rel.gpu.u32 %0, [%1], 1;" : "=r"(old) : "l"(&p.tickets[t]) : "memory");
+        unsigned int old = ~0u;  // not counted: nobody finishes the tile
+        if (ok) asm volatile("atom.add.acq_rel.gpu.u32 %0, [%1], 1;" : "=r"(old) : "l"(&p.tickets[t]) : "memory");
         *last_flag = old == (unsigned int)(cl - cf) ? 1u : 0u;
       }
       epi_sync();
       if (*last_flag) {
-        if (row < p.rows) {
+        if (ok && row < p.rows) {
           float sum[MAX_M];
 #pragma unroll
           for (int q = 0; q < MAX_M; ++q) sum[q] = 0.f;
