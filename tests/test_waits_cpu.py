@@ -77,6 +77,21 @@ def test_no_thread_leaves_alone(path):
     assert not list(offences(path))
 
 
+def test_what_is_in_flight_is_waited_for():
+    """A CTA that gave up waits for its copies and products by time alone: a wait that also ends on the abort
+    flag, which is up by then, would let it exit under them."""
+    found, drains = [], 0
+    for path in SOURCES:
+        lines = path.read_text().splitlines()
+        for i, line in enumerate(lines):
+            if re.search(r"if \(\*abort_flag\) \{", line):
+                found += [f"{path.name}: {x.strip()}" for x in body(lines, i) if WAIT.search(x)]
+            if re.search(r"mbar_wait\w*\(&?(drain|done)\b(?!\[.*parts)", line):
+                found.append(f"{path.name}:{i + 1}: {line.strip()}")
+            drains += "mbar_drain(" in line
+    assert not found and drains >= 11
+
+
 def test_warps_agree_before_group_barriers():
     """In a loop with a barrier of several warps, nobody leaves on a warp's answer either: only on the barrier's."""
     found = []

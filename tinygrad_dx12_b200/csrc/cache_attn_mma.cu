@@ -150,6 +150,7 @@ struct Part {
 struct Bars {
   uint64_t qfull[2], sfull[2], pfull[2][2], pvdone[2], kfull[2], kfree[2], vfull[2], vfree[2], scfull[4];
   uint64_t done[3];  // one row tile: the first warpgroup's products; the second's share; that share's reading
+  uint64_t drain[2]; // an issuer that gave up: its products in flight
 };
 
 // All N threads of barrier ID meet; whether every one of them is `ok`.
@@ -234,6 +235,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
     }
     for (int i = 0; i < 4; ++i) mbar_init(&bars.scfull[i], WG);
     for (int i = 0; i < 3; ++i) mbar_init(&bars.done[i], WG);
+    for (int i = 0; i < 2; ++i) mbar_init(&bars.drain[i], 1);
     abort_word = 0;
     fence_mbar_init();
   }
@@ -874,6 +876,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
           for (uint32_t n = first; n < end && ok; n += STEP) ok = values(n, n == first) && (n + STEP >= end || scores(n + STEP));
         }
         n0 = end;
+      }
+      if (!ok) {  // tensor memory is freed behind the products in flight (else every one has been waited for)
+        commit(&bars.drain[s]);
+        mbar_drain(&bars.drain[s], 0, 200000000ull);
       }
     }
   }

@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           int s = idx - 1 - i;
           uint32_t q = ph;
           if (s < 0) s += STAGES, q ^= 1u;
-          mbar_wait(&full[s], q, abort_flag, 200000000ull);
+          mbar_drain(&full[s], q, 200000000ull);
         }
       }
     }
@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         mma_commit(&accfull[ab]);
       }
       mma_commit(done);
-      mbar_wait(done, 0, abort_flag, 500000000ull);
+      mbar_drain(done, 0, 500000000ull);
     }
   } else {
     const int qd = warp & 3;

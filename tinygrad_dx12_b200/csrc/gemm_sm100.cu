@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           int idx = st.idx - 1 - i;
           uint32_t ph = st.phase;
           if (idx < 0) idx += STAGES, ph ^= 1u;
-          mbar_wait(&full[idx], ph, abort_flag, 200000000ull);
+          mbar_drain(&full[idx], ph, 200000000ull);
         }
       }
     }
@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         mma_commit(&accfull[ab]);  // arrives once this tile's MMAs have completed
       }
       mma_commit(done);
-      mbar_wait(done, 0, abort_flag, 500000000ull);
+      mbar_drain(done, 0, 500000000ull);
     }
   } else if (warp < 2 + DQ_WARPS) {
     // ---------------- dequant: thread = (weight row r = TMEM lane, K quarter kq) ----------------

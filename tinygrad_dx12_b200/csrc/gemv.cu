@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(threads<NC>(), 1)
       if (*abort_flag) {  // drain copies still in flight before exiting
         const int64_t first = gs > STAGES ? gs - STAGES : 0;
         for (int64_t q = first; q < gs; ++q)
-          mbar_wait(&full[q % STAGES], (uint32_t)((q / STAGES) & 1), abort_flag, 200000000ull);
+          mbar_drain(&full[q % STAGES], (uint32_t)((q / STAGES) & 1), 200000000ull);
       }
     }
     return;

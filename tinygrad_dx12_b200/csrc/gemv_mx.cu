@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       if (*abort_flag) {  // let this thread's copies in flight land before the CTA exits
         for (int64_t q = warp; q < (i < n ? i : n); q += p.nact)
-          if (q + S >= i) mbar_wait(&full[q % S], (uint32_t)((q / S) & 1), abort_flag, 200000000ull);
+          if (q + S >= i) mbar_drain(&full[q % S], (uint32_t)((q / S) & 1), 200000000ull);
       }
     }
   } else if (warp >= CONV_WARP0 && warp < CONV_WARP0 + CONV_WARPS) {
@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       // every MMA issued has completed before the CTA frees its tensor memory
       mma_commit(drain);
-      mbar_wait(drain, 0, abort_flag, 200000000ull);
+      mbar_drain(drain, 0, 200000000ull);
     }
   } else if (warp >= SF_WARP0 && warp < SF_WARP0 + 8) {
     // ---------------- scale factors -> tensor memory (one lane quarter per warp) ----------------

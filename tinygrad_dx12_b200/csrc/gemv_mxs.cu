@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(THREADS, 1) mxs_kernel(const __grid_constant__
       }
       if (*abort_flag) {  // let this thread's copies in flight land before the CTA exits
         for (int q = pw; q < (i < n ? i : n); q += nact)
-          if (q + S >= i) mbar_wait(&full[q % S], (uint32_t)((q / S) & 1), abort_flag, 200000000ull);
+          if (q + S >= i) mbar_drain(&full[q % S], (uint32_t)((q / S) & 1), 200000000ull);
       }
     }
     if (p.pair) {
@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(THREADS, 1) mxs_kernel(const __grid_constant__
       }
       // every MMA issued has completed before the CTA frees its tensor memory
       mma_commit(&drain[k]);
-      mbar_wait(&drain[k], 0, abort_flag, 200000000ull);
+      mbar_drain(&drain[k], 0, 200000000ull);
     }
   }
   if (warp < 4) {

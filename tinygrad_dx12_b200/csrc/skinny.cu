@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(threads<NT, SK>(), ctas_per_sm<NT>())
           int s = slot - 1 - i;
           uint32_t q = ph;
           if (s < 0) s += STAGES, q ^= 1u;
-          mbar_wait(&full[s], q, abort_flag, 200000000ull);
+          mbar_drain(&full[s], q, 200000000ull);
         }
       }
     }

@@ -107,6 +107,14 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, volati
   }
 }
 
+// Wait, before a CTA that gave up exits, for what it has in flight (copies into its shared memory, MMAs on its
+// tensor memory): bounded by time alone, since the abort flag is up already.
+__device__ __forceinline__ void mbar_drain(uint64_t *bar, uint32_t parity, uint64_t budget_ns) {
+  const uint64_t t0 = globaltimer();
+  while (!mbar_try_wait(bar, parity) && globaltimer() - t0 <= budget_ns) {
+  }
+}
+
 // Make generic-proxy shared-memory writes visible to the async proxy (TMA / tensor core).
 __device__ __forceinline__ void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
