@@ -1,0 +1,108 @@
+"""Recorded steps own the memory that their kernels leave partial results in: two recordings of one stream,
+replayed on two streams at once beside eager calls on the stream that recorded them, give each the bits of an
+eager call; recordings that are gone give their memory back to later ones; a capture needs no call before it."""
+
+from __future__ import annotations
+
+import gc
+import time
+
+import pytest
+import torch
+
+import tinygrad_dx12_b200 as tg
+from tests.test_gpu_cache import Case
+
+pytestmark = pytest.mark.gpu
+
+# lengths, queries, prefix: few rows cut over many CTAs, many rows, a prefix of few and of many rows
+KINDS = {"few": ([20000, 1, 333], 1, 0), "many": ([3000, 90], 75, 0), "one tile": ([6000], 20, 0),
+         "prefix": ([400, 70, 900], 1, 5000), "prefix of many": ([300] * 40, 1, 3000)}
+
+
+def call(kind, seed):
+    """A step over its own cache: a function of its own inputs, and the eager result."""
+    lengths, queries, prefix = KINDS[kind]
+    c = Case(lengths, queries=queries, heads=8, kv=2, fmt="int8", page=64, prefix=prefix, seed=seed)
+    q, tables = c.q.cuda(), c.tables.to(torch.int32).cuda()
+    n = torch.tensor(lengths, dtype=torch.int32).cuda()
+    shared = dict(prefix=c.prefix.to(torch.int32).cuda(), prefix_length=prefix) if prefix else {}
+
+    def step():
+        return tg.cache_attention(q, c.cache, tables, n, **shared)
+
+    return step, step()
+
+
+def record(step, stream):
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        out = step()
+    return graph, out
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+def test_recordings_of_one_stream_replayed_at_once(kind):
+    (a, want_a), (b, want_b), (c, want_c) = call(kind, 400), call(kind, 410), call(kind, 420)
+    side, one, two = (torch.cuda.Stream() for _ in range(3))
+    assert len({side.cuda_stream, one.cuda_stream, two.cuda_stream}) == 3
+    (ga, out_a), (gb, out_b) = record(a, side), record(b, side)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        out_a.zero_(), out_b.zero_()
+        torch.cuda.synchronize()
+        eager = []
+        for _ in range(5):
+            with torch.cuda.stream(one):
+                ga.replay()
+            with torch.cuda.stream(two):
+                gb.replay()
+            with torch.cuda.stream(side):
+                eager.append(c())
+        torch.cuda.synchronize()
+        assert torch.equal(out_a, want_a) and torch.equal(out_b, want_b)
+        assert all(torch.equal(e, want_c) for e in eager)
+
+
+def test_recordings_give_their_memory_back():
+    step, want = call("many", 430)  # 38 MiB a recording
+    side = torch.cuda.Stream()
+
+    def free():
+        gc.collect()
+        torch.cuda.synchronize()
+        time.sleep(0.2)
+        torch.cuda.empty_cache()
+        return torch.cuda.mem_get_info()[0]
+
+    kept, out_kept = record(step, side)
+    record(step, side)
+    before = free()
+    for _ in range(30):
+        graph, out = record(step, side)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        del graph, out
+        torch.cuda.synchronize()
+        time.sleep(0.02)
+    assert before - free() < 200 << 20  # 30 blocks would be 1.1 GiB
+    out_kept.zero_()
+    kept.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out_kept, want)
+
+
+@pytest.mark.parametrize("queries,heads", [(1, 8), (13, 10), (26, 10), (60, 10)])  # 4, 65, 130 and 300 rows of a key head
+@pytest.mark.parametrize("prefix", [0, 500])
+def test_first_calls_captured(queries, heads, prefix):
+    c = Case([2000, queries, 0, 130], queries=queries, heads=heads, kv=2, fmt="fp8e4m3", page=64, prefix=prefix, seed=440)
+    good, lse = c.run()
+    q, t, n = c.q.cuda(), c.tables.to(torch.int32).cuda(), torch.tensor(c.lengths, dtype=torch.int32).cuda()
+    shared = dict(prefix=c.prefix.to(torch.int32).cuda(), prefix_length=prefix) if prefix else {}
+    graph, (out, out_lse) = record(lambda: tg.cache_attention(q, c.cache, t, n, return_lse=True, **shared), torch.cuda.Stream())
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, good) and torch.equal(out_lse, lse)
+    c.check(out, out_lse)

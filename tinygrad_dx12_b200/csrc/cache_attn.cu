@@ -39,9 +39,6 @@
 // keys of a key head, at 0.62 an SM quarter and cycle. 32 requests of 8192 keys: int8 4.2 TB/s, fp8 4.6
 // TB/s. One request of 257 int8 keys: 8.6 us, a chain of launch, lengths, page numbers, codes, two
 // products, the warps' and the CTAs' joins.
-#include <map>
-#include <mutex>
-
 #include "cache_attn.cuh"
 #include "sm100.cuh"
 
@@ -144,7 +141,6 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
   const int entries = p.batch * p.row_tiles, heads = p.kv_heads;
   constexpr uint32_t ROUND = C::T * WARPS;
   const int64_t cap = (int64_t)p.max_pages << p.page_shift;
-  const bool split = p.ws_o != nullptr;
 
   auto length_of = [&](int b) -> int {
     const int64_t n = p.lengths != nullptr ? p.lengths[b] : p.fixed;
@@ -211,8 +207,8 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
     }
   }
 
-  // this CTA's run of rounds; without a workspace, whole segments in turn
-  const uint32_t u0 = split ? min(total, blockIdx.x * per) : 0, u_end = split ? min(total, u0 + per) : total;
+  // this CTA's run of rounds
+  const uint32_t u0 = min(total, blockIdx.x * per), u_end = min(total, u0 + per);
 
   auto enter = [&](Walk &w) {  // reads the segment that w.e, w.h name
     const uint32_t n = prefix[w.e + 1] - prefix[w.e];
@@ -222,16 +218,14 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
     w.keys = keys_of(w.e);
   };
   auto next_segment = [&](Walk &w) {  // w.u stands at its end
-    do {
-      w.u = w.seg1;
-      if (w.u >= u_end) return;
-      if (++w.h == heads) {
-        w.h = 0;
-        do ++w.e;
-        while (prefix[w.e + 1] == prefix[w.e]);
-      }
-      enter(w);
-    } while (!split && (w.e * (uint32_t)heads + w.h) % gridDim.x != blockIdx.x);
+    w.u = w.seg1;
+    if (w.u >= u_end) return;
+    if (++w.h == heads) {
+      w.h = 0;
+      do ++w.e;
+      while (prefix[w.e + 1] == prefix[w.e]);
+    }
+    enter(w);
   };
   Walk c;
   c.u = u0, c.e = 0, c.h = 0;
@@ -245,7 +239,6 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
     c.e = lo;
     c.h = (int)((u0 - prefix[lo] * heads) / (prefix[lo + 1] - prefix[lo]));
     enter(c);
-    if (!split && (c.e * (uint32_t)heads + c.h) % gridDim.x != blockIdx.x) next_segment(c);
   }
 
   // ---- what is on its way: pages of one unit, scales of the one before, codes of the one before that
@@ -626,7 +619,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
     if (p.early) await();
     Walk following = c;
     const bool whole = from == 0 && to == real;
-    const uint32_t c0 = split ? c.seg0 / per : 0, c1 = split ? (c.seg0 + real - 1) / per : 0;  // CTAs of the segment
+    const uint32_t c0 = c.seg0 / per, c1 = (c.seg0 + real - 1) / per;  // CTAs of the segment
     const int slot = (int)(2 * blockIdx.x + (from == 0 ? 1 : 0));
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -720,48 +713,15 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
   if (p.early) await();  // the launch behind this one takes this one's end for that of all before it
 }
 
-// ---- per-(device, stream) workspace of split segments ---------------------------------------------
-struct Workspace {
-  float *o = nullptr, *ml = nullptr;
-  uint32_t *tickets = nullptr;
-  int grid = 0;
-};
+// ---- workspace of split segments -------------------------------------------------------------------
 constexpr int MAX_ROWS_D = 16 * 128;  // ROWS * D of every variant is at most this
 
-static std::mutex g_ws_mutex;
-static std::map<std::pair<int, cudaStream_t>, Workspace> g_ws;
-
-static int32_t workspace_for(cudaStream_t stream, Workspace &out) {
-  int dev = 0, sms = 0;
-  B200_CUDA_TRY(cudaGetDevice(&dev));
-  B200_CUDA_TRY(device_sms(&sms));
-  std::lock_guard<std::mutex> lock(g_ws_mutex);
-  auto it = g_ws.find({dev, stream});
-  if (it != g_ws.end()) {
-    out = it->second;
-    return B200_OK;
-  }
-  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-  B200_CUDA_TRY(cudaStreamIsCapturing(stream, &cs));
-  Workspace w;
-  w.grid = 2 * sms;
-  if (cs != cudaStreamCaptureStatusNone) {  // nothing can be allocated while capturing: whole segments
-    out = w;
-    return B200_OK;
-  }
-  const size_t slots = 2 * (size_t)w.grid;
-  const size_t o_bytes = slots * MAX_ROWS_D * 4, ml_bytes = slots * 16 * 2 * 4, t_bytes = (size_t)w.grid * 4;
+// Two slots for each of the `grid` CTAs that a launch has at most, and their tickets, first.
+static int32_t workspace_for(cudaStream_t stream, int grid, Params &p) {
+  const size_t slots = 2 * (size_t)grid, t_bytes = ((size_t)grid * 4 + 255) / 256 * 256, o_bytes = slots * MAX_ROWS_D * 4;
   uint8_t *base = nullptr;
-  B200_CUDA_TRY(cudaMalloc((void **)&base, o_bytes + ml_bytes + t_bytes));
-  w.o = (float *)base, w.ml = (float *)(base + o_bytes), w.tickets = (uint32_t *)(base + o_bytes + ml_bytes);
-  // on the caller's stream, the only one that uses this workspace
-  cudaError_t err = cudaMemsetAsync(w.tickets, 0, t_bytes, stream);
-  if (err != cudaSuccess) {
-    cudaFree(base);
-    return b200_set_error(B200_ERR_CUDA, "cache_attention workspace: %s", cudaGetErrorString(err));
-  }
-  g_ws[{dev, stream}] = w;
-  out = w;
+  if (int32_t rc = workspace_of(WS_ATTENTION, t_bytes + o_bytes + slots * 16 * 2 * 4, t_bytes, stream, &base)) return rc;
+  p.tickets = (uint32_t *)base, p.ws_o = (float *)(base + t_bytes), p.ws_ml = (float *)(base + t_bytes + o_bytes);
   return B200_OK;
 }
 
@@ -795,13 +755,13 @@ static int32_t launch_t(Params p, cudaStream_t stream) {
     return B200_OK;
   }
   const int64_t entries = (int64_t)p.batch * p.row_tiles;
-  Workspace w;
-  if (int32_t rc = workspace_for(stream, w)) return rc;
-  p.ws_o = w.o, p.ws_ml = w.ml, p.tickets = w.tickets;
+  int sms = 0;
+  B200_CUDA_TRY(device_sms(&sms));
+  if (int32_t rc = workspace_for(stream, 2 * sms, p)) return rc;
   B200_CUDA_TRY((ensure_dynamic_smem<attn_kernel<T, F, D, NT, BLK>>(C::SMEM + (MAX_ENTRIES + 1) * 4)));
   // no more CTAs than there can be rounds
   int64_t grid = entries * p.kv_heads * ((cap + round - 1) / round);
-  const int64_t full = (int64_t)w.grid / 2 * C::CTAS;
+  const int64_t full = (int64_t)sms * C::CTAS;
   if (grid > full) grid = full;
   if (grid < 1) grid = 1;
   cudaLaunchConfig_t cfg = {};
@@ -876,12 +836,12 @@ static int32_t attention(const b200_cache_desc *c, const b200_attention_args *a,
     f.po = (float *)a->scratch, f.pm = f.po + all_rows * dim, f.pl = f.pm + all_rows;
     if (int32_t rc = run(f)) return rc;
     p.fo = f.po, p.fm = f.pm, p.fl = f.pl;
-    joined = f.ws_o != nullptr;
+    joined = mma_supported(f, dim);
   }
   p.tables = a->tables, p.table_stride = a->table_stride, p.max_pages = (int)a->max_pages, p.lengths = a->lengths;
   p.batch = (int)a->batch, p.queries = (int)a->queries, p.rows = p.queries * p.group, p.causal = 1;
   p.out = a->out, p.lse = a->lse;
-  // The few-row kernel works on its first keys while the prefix's cut segments are joined.
+  // The few-row kernel works on its first keys while the many-row kernel's cut segments of the prefix are joined.
   p.early = joined && !mma_supported(p, dim);
   return run(p);
 }

@@ -25,9 +25,6 @@
 // Tiles of all (row tile, key head) segments are laid end to end and cut into equal runs, one per CTA.
 // A segment within a run is finished there; the others leave their share (numerators, maximum,
 // denominator) in the CTA's two workspace slots, and join_kernel adds those up.
-#include <map>
-#include <mutex>
-
 #include "cache_attn.cuh"
 #include "sm100.cuh"
 
@@ -247,7 +244,6 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
   const uint32_t tmem = tmem_slot;
   const int entries = p.batch * p.row_tiles, heads = p.kv_heads;
   const uint32_t total = prefix[entries] * (uint32_t)heads;
-  const bool split = p.ws_o != nullptr;
   const uint32_t per = max(1u, (total + gridDim.x - 1) / gridDim.x);
 
   // rows without a key: zeros (or what the prefix gave)
@@ -271,21 +267,19 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
     w.to = min(w.u_end - w.seg0, w.tiles);
   };
   auto next = [&](Part &w) {  // on to the next part; false at the end of the run
-    do {
-      w.u = w.seg0 + w.tiles;
-      if (w.u >= w.u_end) return false;
-      if (++w.h == heads) {
-        w.h = 0;
-        do ++w.e;
-        while (prefix[w.e + 1] == prefix[w.e]);
-      }
-      enter(w);
-    } while (!split && (w.e * (uint32_t)heads + w.h) % gridDim.x != blockIdx.x);
+    w.u = w.seg0 + w.tiles;
+    if (w.u >= w.u_end) return false;
+    if (++w.h == heads) {
+      w.h = 0;
+      do ++w.e;
+      while (prefix[w.e + 1] == prefix[w.e]);
+    }
+    enter(w);
     return true;
   };
   auto begin = [&](Part &w) {
-    w.u = split ? min(total, blockIdx.x * per) : 0;
-    w.u_end = split ? min(total, w.u + per) : total;
+    w.u = min(total, blockIdx.x * per);
+    w.u_end = min(total, w.u + per);
     if (w.u >= w.u_end) return false;
     int lo = 0, hi = entries;
     while (hi - lo > 1) {
@@ -296,7 +290,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_mma_kernel(const Params p) {
     w.e = lo;
     w.h = (int)((w.u - prefix[lo] * heads) / (prefix[lo + 1] - prefix[lo]));
     enter(w);
-    return split || (w.e * (uint32_t)heads + w.h) % gridDim.x == blockIdx.x ? true : next(w);
+    return true;
   };
   // Key codes take their scales before the products. With 8-bit codes and bfloat16 scales that rounds their
   // 15 bits to fp16's 11, 2^-12 at random: far below a bfloat16 result's half unit of 2^-8, but not below what
@@ -929,36 +923,6 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p, int tile_rows
   }
 }
 
-// ---- per-(device, stream) workspace of cut segments ------------------------------------------------
-struct Workspace {
-  float *o = nullptr, *ml = nullptr;
-};
-static std::mutex g_ws_mutex;
-static std::map<std::pair<int, cudaStream_t>, Workspace> g_ws;
-
-static int32_t workspace_for(cudaStream_t stream, int sms, Workspace &out) {
-  int dev = 0;
-  B200_CUDA_TRY(cudaGetDevice(&dev));
-  std::lock_guard<std::mutex> lock(g_ws_mutex);
-  auto it = g_ws.find({dev, stream});
-  out = Workspace();
-  if (it != g_ws.end()) {
-    out = it->second;
-    return B200_OK;
-  }
-  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-  B200_CUDA_TRY(cudaStreamIsCapturing(stream, &cs));
-  if (cs != cudaStreamCaptureStatusNone) return B200_OK;  // nothing can be allocated now: whole segments
-  const size_t rows = (size_t)sms * 2 * 256;
-  uint8_t *base = nullptr;
-  B200_CUDA_TRY(cudaMalloc((void **)&base, rows * (128 + 2) * 4));
-  Workspace w;
-  w.o = (float *)base, w.ml = (float *)(base + rows * 128 * 4);
-  g_ws[{dev, stream}] = w;
-  out = w;
-  return B200_OK;
-}
-
 template <typename K>
 static int32_t launch_pdl(K kernel, int grid, int block, size_t smem, cudaStream_t stream, const Params &p) {
   cudaLaunchConfig_t cfg = {};
@@ -989,8 +953,10 @@ static int32_t launch_t(Params &p, cudaStream_t stream) {
   if (tiles > (1 << 30)) return b200_set_error(B200_ERR_UNSUPPORTED, "cache_attention: too many keys for one launch");
   int at_once = MAX_ENTRIES / p.row_tiles;
   if (tiles > 0 && tiles * at_once > (1 << 30)) at_once = (int)((1 << 30) / tiles);
-  Workspace w;
-  if (int32_t rc = workspace_for(stream, sms, w)) return rc;
+  const size_t rows = (size_t)sms * 2 * 256;  // two shares a CTA
+  uint8_t *ws = nullptr;
+  if (int32_t rc = workspace_of(WS_ATTENTION_MMA, rows * (128 + 2) * 4, 0, stream, &ws)) return rc;
+  p.ws_o = (float *)ws, p.ws_ml = (float *)(ws + rows * 128 * 4);
   B200_CUDA_TRY((ensure_dynamic_smem<attn_mma_kernel<F, D, RT, BLK>>(C::SMEM)));
   const Params base = p;
   for (int b = 0; b < base.batch; b += at_once) {  // a launch for each run of requests that the scan has room for
@@ -1004,12 +970,10 @@ static int32_t launch_t(Params &p, cudaStream_t stream) {
       if (p.lse != nullptr) p.lse += rows;
       p.row0 += rows;
     }
-    p.ws_o = w.o, p.ws_ml = w.ml;
     int64_t grid = tiles * p.batch;
     if (grid > sms) grid = sms;
     if (grid < 1) grid = 1;
     if (int32_t rc = launch_pdl(attn_mma_kernel<F, D, RT, BLK>, (int)grid, THREADS, C::SMEM, stream, p)) return rc;
-    if (w.o == nullptr) continue;
     const int64_t chunks = (int64_t)p.batch * p.row_tiles * p.kv_heads * (TR / 32) * (D / 32);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(chunks < 8 * sms ? chunks : 8 * sms));

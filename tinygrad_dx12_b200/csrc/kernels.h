@@ -90,6 +90,11 @@ int32_t stackops_device_error(unsigned int *v, bool clear);
 int32_t launch_gate_mul(const void *gu, int gdt, void *out, int odt, int64_t M, int64_t I, cudaStream_t stream);
 int32_t launch_wait_flag(const int32_t *flag, int32_t expect, int64_t max_spins, int32_t *status, cudaStream_t stream);
 
+// `bytes` of device memory for partial results and tickets of kernels on `stream`: the same block for all calls
+// of a kind on a stream, one of its own for those of a capture, the first `zeroed` bytes zero when it is handed
+// out first (workspace.cu).
+enum WorkspaceKind { WS_ATTENTION, WS_ATTENTION_MMA };
+int32_t workspace_of(WorkspaceKind kind, size_t bytes, size_t zeroed, cudaStream_t stream, uint8_t **base);
 
 // packed key/value cache: rotary positions, writing, reading (cache_ops.cu), attention (cache_attn.cu)
 int32_t check_cache(const b200_cache_desc *c);
