@@ -16,8 +16,11 @@
  *   - b200_last_error() copies the calling thread's last error message;
  *   - all pointers to tensors are device pointers owned by the caller. The compute entry
  *     points allocate nothing, with one exception: b200_packed_linear on a few tokens
- *     (3 <= m <= 64) splits K across CTAs and, on its first such call on a (device, stream),
- *     allocates a 16 MiB split-K workspace kept for the life of the process
+ *     (3 <= m <= 64) splits K across CTAs and keeps a 16 MiB split-K workspace, its block-scaled
+ *     kernel one of 10 MiB, b200_cache_attention others (see there). The first such call on a
+ *     (device, stream) allocates it for the life of the process; the calls of a stream capture
+ *     have one of their own, which the graph owns: recorded graphs can be replayed on any streams,
+ *     beside one another and beside direct calls (but not several executables of one graph at once)
  *     (b200_packed_linear_noalloc is the allocation-free form). Other allocations are the
  *     explicit b200_malloc / b200_stream_create / b200_event_create calls;
  *   - `stream` is a cudaStream_t passed as void* (NULL = legacy default stream);
@@ -323,11 +326,9 @@ int32_t b200_cache_read(const b200_cache_desc *cache, const void *slots, int32_t
  * out: contiguous [batch, queries, heads, head_dim] of q's type; lse: fp32 [batch, queries, heads]
  * natural logarithms of the softmax sums, or NULL. `scratch` holds b200_cache_attention_scratch()
  * bytes (prefix only). A NaN in a key's or value's scale makes the rows that see that key NaN, in all
- * their values. Allocates workspaces for the life of the process on the first call per (device,
- * stream): 5 MiB, and 38 MiB more when a key head first has over 64 query rows (queries, or batch x
- * queries for the prefix, x heads / kv_heads); a first call that is captured into a graph runs
- * without, with less parallelism. More than 262144 query rows of a key head, 32768 for head_dim
- * 256: B200_ERR_UNSUPPORTED. */
+ * their values. Workspaces: 5 MiB per (device, stream) or capture, and 38 MiB more when a key head
+ * has over 64 query rows (queries, or batch x queries for the prefix, x heads / kv_heads). More
+ * than 262144 query rows of a key head, 32768 for head_dim 256: B200_ERR_UNSUPPORTED. */
 typedef struct b200_attention_args {
   const void *q;
   int64_t q_strides[3];

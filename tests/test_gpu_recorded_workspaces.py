@@ -7,11 +7,15 @@ from __future__ import annotations
 import gc
 import time
 
+import numpy as np
 import pytest
 import torch
 
 import tinygrad_dx12_b200 as tg
+from oracle import packed_ref
+from tests.helpers import to_device
 from tests.test_gpu_cache import Case
+from tinygrad_dx12_b200.linalg import _packed_linear
 
 pytestmark = pytest.mark.gpu
 
@@ -20,8 +24,24 @@ KINDS = {"few": ([20000, 1, 333], 1, 0), "many": ([3000, 90], 75, 0), "one tile"
          "prefix": ([400, 70, 900], 1, 5000), "prefix of many": ([300] * 40, 1, 3000)}
 
 
+# packed products whose tiles several CTAs share: rows, columns, tokens, path
+PRODUCTS = {"split K": (4096, 4096, 8, "gemv"), "shared tiles": (9600, 1024, 1, "mx"), "shared tiles, 16 tokens": (8192, 2048, 16, "mx")}
+
+
 def call(kind, seed):
-    """A step over its own cache: a function of its own inputs, and the eager result."""
+    """A step over its own operands, and the eager result."""
+    if kind in PRODUCTS:
+        rows, cols, m, path = PRODUCTS[kind]
+        w = to_device(packed_ref.make_packed(np.random.default_rng(seed), "fp4_e2m1", rows, cols, 32, "e8m0"), "cuda:0", "e8m0")
+        x = torch.randn((m, cols), generator=torch.Generator().manual_seed(seed)).to(torch.bfloat16).cuda()
+
+        def product():
+            y = _packed_linear(w, x, torch.float32, path)
+            for _ in range(3):
+                y = torch.maximum(y, _packed_linear(w, x, torch.float32, path))
+            return y
+
+        return product, product()
     lengths, queries, prefix = KINDS[kind]
     c = Case(lengths, queries=queries, heads=8, kv=2, fmt="int8", page=64, prefix=prefix, seed=seed)
     q, tables = c.q.cuda(), c.tables.to(torch.int32).cuda()
@@ -42,7 +62,7 @@ def record(step, stream):
     return graph, out
 
 
-@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("kind", [*KINDS, *PRODUCTS])
 def test_recordings_of_one_stream_replayed_at_once(kind):
     (a, want_a), (b, want_b), (c, want_c) = call(kind, 400), call(kind, 410), call(kind, 420)
     side, one, two = (torch.cuda.Stream() for _ in range(3))
@@ -92,6 +112,16 @@ def test_recordings_give_their_memory_back():
     kept.replay()
     torch.cuda.synchronize()
     assert torch.equal(out_kept, want)
+
+
+@pytest.mark.parametrize("kind", list(PRODUCTS))
+def test_first_products_captured(kind):
+    """The kernel and the bits of a direct call."""
+    step, want = call(kind, 450)
+    graph, out = record(step, torch.cuda.Stream())
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
 
 
 @pytest.mark.parametrize("queries,heads", [(1, 8), (13, 10), (26, 10), (60, 10)])  # 4, 65, 130 and 300 rows of a key head

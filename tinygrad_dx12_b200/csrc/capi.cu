@@ -134,13 +134,12 @@ static bool fill_linear(const b200_packed_desc *w, const void *x, int32_t x_dtyp
   return x_stride_k == 1;
 }
 
-// Kernel for these operands. `mx_ok` = false leaves the block-scaled decode kernel out (its
-// workspace cannot be allocated during a stream capture).
-static int32_t plan(const LinearArgs &a, bool kstride_ok, int32_t path, bool mx_ok = true) {
+// Kernel for these operands.
+static int32_t plan(const LinearArgs &a, bool kstride_ok, int32_t path) {
   if (!kstride_ok) return B200_ERR_UNSUPPORTED;
   path &= 0xFF;  // flag bits (B200_FLAG_*) do not select a kernel
   const bool tc = gemv_tc_supported(a) || skinny_supported(a), gm = gemm_supported(a), simt = simt_supported(a);
-  const bool mx = mx_ok && mx_supported(a);
+  const bool mx = mx_supported(a);
   switch (path) {
     case B200_PATH_MX: return mx ? B200_PATH_MX : B200_ERR_UNSUPPORTED;
     case B200_PATH_AUTO:
@@ -177,7 +176,7 @@ int32_t b200_packed_linear(const b200_packed_desc *w, const void *x, int32_t x_d
   const bool ks = fill_linear(w, x, x_dtype, m, x_stride_m, x_stride_k, y, y_dtype, y_stride_m, y_stride_n, a);
   a.flags = path & ~0xFF;
   cudaStream_t s = (cudaStream_t)stream;
-  const int32_t p = plan(a, ks, path, mx_ready(s));
+  const int32_t p = plan(a, ks, path);
   switch (p) {
     case B200_PATH_MX: return launch_mx(a, s);
     case B200_PATH_GEMV:
@@ -329,7 +328,7 @@ int32_t b200_packed_linear_multi(const b200_packed_desc *w, const void *x, int32
   const bool ks = fill_linear(w, x, x_dtype, m, x_stride_m, 1, y[0], y_dtype, y_stride_m, 1, a);
   a.flags = flags & ~0xFF;
   cudaStream_t s = (cudaStream_t)stream;
-  const int32_t p = plan(a, ks, flags, mx_ready(s));  // the low byte selects a path, as in b200_packed_linear
+  const int32_t p = plan(a, ks, flags);  // the low byte selects a path, as in b200_packed_linear
   if (p == B200_PATH_MX || (p == B200_PATH_GEMV && a.m <= 2)) {  // these epilogues write every destination
     a.ncopy = n_y - 1;
     for (int i = 1; i < n_y; ++i) a.ycopy[i - 1] = y[i];

@@ -37,9 +37,6 @@
 // into one of two fp32 accumulators; warps 4-7 read the accumulators (tcgen05.ld) and finish
 // the rows.
 // Every wait is bounded (sm100.cuh); on give-up the kernel flags the device error word.
-#include <map>
-#include <mutex>
-
 #include "mx.cuh"
 
 namespace b200 {
@@ -432,35 +429,16 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (warp == MMA_WARP) tmem_dealloc(tmem, p.tmem_cols);
 }
 
-// ---- per-(device, stream) workspace: fp32 partials of shared tiles and their tickets ----------
-
-static std::mutex g_ws_mutex;
-static std::map<std::pair<int, cudaStream_t>, Workspace> g_ws;
-
-int32_t workspace_for(cudaStream_t stream, bool may_allocate, Workspace *&out) {
-  int dev = 0;
-  B200_CUDA_TRY(cudaGetDevice(&dev));
-  std::lock_guard<std::mutex> lock(g_ws_mutex);
-  auto it = g_ws.find({dev, stream});
-  if (it != g_ws.end()) {
-    out = &it->second;
-    return B200_OK;
-  }
-  out = nullptr;
-  if (!may_allocate) return B200_OK;
-  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-  B200_CUDA_TRY(cudaStreamIsCapturing(stream, &cs));
-  if (cs != cudaStreamCaptureStatusNone) return B200_OK;  // no allocation while capturing
+// ---- workspace: tickets of shared tiles and their fp32 partials ----------------------------------
+static int32_t workspace_for(cudaStream_t stream, Workspace &out) {
   int sms = 0;
   B200_CUDA_TRY(device_sms(&sms));
-  Workspace w;
-  w.part_bytes = (size_t)sms * 2 * 64 * TM * sizeof(float);
-  w.tickets_n = TICKETS;
-  B200_CUDA_TRY(cudaMalloc((void **)&w.part, w.part_bytes));
-  B200_CUDA_TRY(cudaMalloc((void **)&w.tickets, w.tickets_n * sizeof(unsigned int)));
-  B200_CUDA_TRY(cudaMemset(w.tickets, 0, w.tickets_n * sizeof(unsigned int)));
-  B200_CUDA_TRY(cudaDeviceSynchronize());
-  out = &(g_ws[{dev, stream}] = w);
+  const size_t t_bytes = TICKETS * sizeof(unsigned int);
+  out.part_bytes = (size_t)sms * 2 * 64 * TM * sizeof(float);
+  uint8_t *base = nullptr;
+  if (int32_t rc = workspace_of(WS_MX, t_bytes + out.part_bytes, t_bytes, stream, &base)) return rc;
+  out.tickets = reinterpret_cast<unsigned int *>(base);
+  out.part = reinterpret_cast<float *>(base + t_bytes);
   return B200_OK;
 }
 
@@ -589,7 +567,7 @@ static int32_t dispatch(const LinearArgs &a, const Workspace &w, cudaStream_t st
 
 }  // namespace mx
 
-// Shapes the block-scaled kernel takes (independent of whether its workspace exists yet).
+// Shapes the block-scaled kernel takes.
 bool mx_supported(const LinearArgs &a) {
   using namespace mx;
   if (!(a.fmt == B200_FMT_FP4_E2M1 || a.fmt == B200_FMT_FP6_E2M3 || a.fmt == B200_FMT_FP6_E3M2)) return false;
@@ -614,48 +592,25 @@ bool mx_supported(const LinearArgs &a) {
   return true;
 }
 
-// Runs the kernel if its workspace exists or can be allocated now; B200_ERR_UNSUPPORTED otherwise
-// (a first call inside a stream capture), so the caller can take another kernel.
 int32_t launch_mx(const LinearArgs &a, cudaStream_t stream) {
   using namespace mx;
-  Workspace *w = nullptr;
-  if (int32_t rc = workspace_for(stream, true, w)) return rc;
-  if (w == nullptr) return b200_set_error(B200_ERR_UNSUPPORTED, "mx decode: no workspace while capturing");
+  Workspace w;
+  if (int32_t rc = workspace_for(stream, w)) return rc;
   int sms = 0;
   B200_CUDA_TRY(device_sms(&sms));
-  if ((size_t)sms * 2 * a.m * TM * sizeof(float) > w->part_bytes)
+  if ((size_t)sms * 2 * a.m * TM * sizeof(float) > w.part_bytes)
     return b200_set_error(B200_ERR_UNSUPPORTED, "mx decode: shape beyond the workspace");
-  if (mxs_supported(a)) return launch_mxs(a, *w, stream);
+  if (mxs_supported(a)) return launch_mxs(a, w, stream);
   switch (a.fmt) {
-    case B200_FMT_FP4_E2M1: return dispatch<B200_FMT_FP4_E2M1>(a, *w, stream);
-    case B200_FMT_FP6_E2M3: return dispatch<B200_FMT_FP6_E2M3>(a, *w, stream);
-    case B200_FMT_FP6_E3M2: return dispatch<B200_FMT_FP6_E3M2>(a, *w, stream);
+    case B200_FMT_FP4_E2M1: return dispatch<B200_FMT_FP4_E2M1>(a, w, stream);
+    case B200_FMT_FP6_E2M3: return dispatch<B200_FMT_FP6_E2M3>(a, w, stream);
+    case B200_FMT_FP6_E3M2: return dispatch<B200_FMT_FP6_E3M2>(a, w, stream);
   }
   return b200_set_error(B200_ERR_UNSUPPORTED, "mx decode: format %d", a.fmt);
 }
 
 // Zero the tile tickets of every workspace on the current device: after a kernel gave up on a
 // bounded wait (device status bit set), a split tile may have been left half counted.
-int32_t mx_reset_tickets() {
-  using namespace mx;
-  int dev = 0;
-  B200_CUDA_TRY(cudaGetDevice(&dev));
-  std::lock_guard<std::mutex> lock(g_ws_mutex);
-  for (auto &kv : g_ws)
-    if (kv.first.first == dev) B200_CUDA_TRY(cudaMemset(kv.second.tickets, 0, kv.second.tickets_n * sizeof(unsigned int)));
-  B200_CUDA_TRY(cudaDeviceSynchronize());
-  return B200_OK;
-}
-
-// Whether a call on `stream` could run now: the workspace exists, or may be allocated (not capturing).
-bool mx_ready(cudaStream_t stream) {
-  using namespace mx;
-  Workspace *w = nullptr;
-  if (workspace_for(stream, false, w) != B200_OK) return false;
-  if (w != nullptr) return true;
-  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-  if (cudaStreamIsCapturing(stream, &cs) != cudaSuccess) return false;
-  return cs == cudaStreamCaptureStatusNone;
-}
+int32_t mx_reset_tickets() { return workspace_zero(WS_MX); }
 
 }  // namespace b200

@@ -62,7 +62,6 @@ int32_t launch_skinny_noalloc(const LinearArgs &a, cudaStream_t stream);
 // block-scaled tcgen05 decode kernel (kind::mxf8f6f4) for FP4 / FP6 weights and 1..64 tokens
 // (gemv_mx.cu): the packed codes are the MMA's A operand, x is split into exact E4M3 pieces
 bool mx_supported(const LinearArgs &a);
-bool mx_ready(cudaStream_t stream);  // its workspace exists or can be allocated now
 int32_t launch_mx(const LinearArgs &a, cudaStream_t stream);
 int32_t mx_device_error(unsigned int *v, bool clear);
 int32_t mx_reset_tickets();  // after a device error: zero the split-tile tickets on this device
@@ -93,8 +92,9 @@ int32_t launch_wait_flag(const int32_t *flag, int32_t expect, int64_t max_spins,
 // `bytes` of device memory for partial results and tickets of kernels on `stream`: the same block for all calls
 // of a kind on a stream, one of its own for those of a capture, the first `zeroed` bytes zero when it is handed
 // out first (workspace.cu).
-enum WorkspaceKind { WS_ATTENTION, WS_ATTENTION_MMA };
+enum WorkspaceKind { WS_SPLIT_K, WS_MX, WS_ATTENTION, WS_ATTENTION_MMA };
 int32_t workspace_of(WorkspaceKind kind, size_t bytes, size_t zeroed, cudaStream_t stream, uint8_t **base);
+int32_t workspace_zero(WorkspaceKind kind);  // that part again, of every block on the current device; synchronous
 
 // packed key/value cache: rotary positions, writing, reading (cache_ops.cu), attention (cache_attn.cu)
 int32_t check_cache(const b200_cache_desc *c);

@@ -219,14 +219,13 @@ inline int scale_mode(const LinearArgs &a) {
 }
 
 // The fp32 partials of split tiles ([SMs][2][<= 64 tokens][128 rows]) and one ticket per 128-row
-// tile, per (device, stream); allocated on first use outside stream capture (gemv_mx.cu).
+// tile.
 struct Workspace {
   float *part = nullptr;
   unsigned int *tickets = nullptr;
-  size_t part_bytes = 0, tickets_n = 0;
+  size_t part_bytes = 0;
 };
 constexpr size_t TICKETS = 16384;  // 128-row tiles: N <= 2M rows
-int32_t workspace_for(cudaStream_t stream, bool may_allocate, Workspace *&out);
 
 }  // namespace mx
 

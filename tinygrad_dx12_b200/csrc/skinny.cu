@@ -514,44 +514,9 @@ static size_t smem_bytes(int esz) {
   return 1024 + (size_t)stages<NT>(esz) * slot_bytes<NT>(esz) + 2 * 4 * 8 + 16 + 4 * 8 * NT * 4;
 }
 
-// ---- per-(device, stream) split-K workspace --------------------------------------------------
-struct Workspace {
-  float *ws = nullptr;
-  unsigned int *tickets = nullptr;
-  size_t ws_bytes = 0, tickets_n = 0;
-};
+// ---- split-K workspace: tickets of row blocks, then fp32 partials --------------------------------
 constexpr size_t WS_BYTES = 16u << 20;  // fp32 partials (max splits x M x N)
 constexpr size_t TICKETS = 16384;       // row blocks (N up to 2M rows)
-
-static std::mutex g_ws_mutex;
-static std::map<std::pair<int, cudaStream_t>, Workspace> g_ws;
-
-static int32_t workspace_for(cudaStream_t stream, Workspace *&out) {
-  int dev = 0;
-  B200_CUDA_TRY(cudaGetDevice(&dev));
-  std::lock_guard<std::mutex> lock(g_ws_mutex);
-  auto it = g_ws.find({dev, stream});
-  if (it != g_ws.end()) {
-    out = &it->second;
-    return B200_OK;
-  }
-  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-  B200_CUDA_TRY(cudaStreamIsCapturing(stream, &cs));
-  if (cs != cudaStreamCaptureStatusNone) {  // no allocation while capturing: run unsplit
-    out = nullptr;
-    return B200_OK;
-  }
-  Workspace w;
-  B200_CUDA_TRY(cudaMalloc((void **)&w.ws, WS_BYTES));
-  B200_CUDA_TRY(cudaMalloc((void **)&w.tickets, TICKETS * sizeof(unsigned int)));
-  // on the caller's stream, the only one that uses this workspace: ordered before its kernels
-  // even when that stream does not synchronise with the legacy default stream
-  B200_CUDA_TRY(cudaMemsetAsync(w.tickets, 0, TICKETS * sizeof(unsigned int), stream));
-  w.ws_bytes = WS_BYTES;
-  w.tickets_n = TICKETS;
-  out = &(g_ws[{dev, stream}] = w);
-  return B200_OK;
-}
 
 template <int FMT, int NT, int SK, bool XBF16>
 static int32_t launch_t(const LinearArgs &a, int splits, float *ws, unsigned int *tickets, cudaStream_t stream) {
@@ -715,16 +680,16 @@ int32_t launch_skinny(const LinearArgs &a, cudaStream_t stream) {
   float *ws = nullptr;
   unsigned int *tickets = nullptr;
   if (splits > 1) {
-    Workspace *w = nullptr;
-    if (int32_t rc = workspace_for(stream, w)) return rc;
     const int64_t nrb = (a.rows + RB - 1) / RB;
-    const size_t per_split = (size_t)a.m * a.rows * sizeof(float);
-    if (w == nullptr || (size_t)nrb > w->tickets_n) {
+    const size_t per_split = (size_t)a.m * a.rows * sizeof(float), t_bytes = TICKETS * sizeof(unsigned int);
+    if ((size_t)nrb > TICKETS) {
       splits = 1;
     } else {
-      while (splits > 1 && (size_t)splits * per_split > w->ws_bytes) --splits;
-      ws = w->ws;
-      tickets = w->tickets;
+      uint8_t *base = nullptr;
+      if (int32_t rc = workspace_of(WS_SPLIT_K, t_bytes + WS_BYTES, t_bytes, stream, &base)) return rc;
+      while (splits > 1 && (size_t)splits * per_split > WS_BYTES) --splits;
+      tickets = reinterpret_cast<unsigned int *>(base);
+      ws = reinterpret_cast<float *>(base + t_bytes);
     }
   }
   const int sk = gemv::scale_kind(a);

@@ -63,7 +63,7 @@ void CUDART_CB graph_is_gone(void *block) {  // no CUDA call may be made here
 
 }  // namespace
 
-int32_t workspace_of(WorkspaceKind kind, size_t bytes, size_t zeroed, cudaStream_t stream, uint8_t **base) {
+static int32_t find_or_make(WorkspaceKind kind, size_t bytes, size_t zeroed, cudaStream_t stream, uint8_t **base) {
   int dev = 0;
   B200_CUDA_TRY(cudaGetDevice(&dev));
   unsigned long long id = (unsigned long long)(uintptr_t)stream, capture = 0;
@@ -130,6 +130,26 @@ int32_t workspace_of(WorkspaceKind kind, size_t bytes, size_t zeroed, cudaStream
   }
   if (e != cudaSuccess) return b200_set_error(B200_ERR_CUDA, "workspace: %s", cudaGetErrorString(e));
   *base = b->base;
+  return B200_OK;
+}
+
+int32_t workspace_of(WorkspaceKind kind, size_t bytes, size_t zeroed, cudaStream_t stream, uint8_t **base) {
+  try {
+    return find_or_make(kind, bytes, zeroed, stream, base);
+  } catch (...) {
+    return b200_set_error(B200_ERR_CUDA, "workspace: out of host memory");
+  }
+}
+
+int32_t workspace_zero(WorkspaceKind kind) {
+  int dev = 0;
+  B200_CUDA_TRY(cudaGetDevice(&dev));
+  State &s = state();
+  B200_CUDA_TRY(cudaDeviceSynchronize());
+  std::lock_guard<std::mutex> making(s.making);
+  std::lock_guard<std::mutex> lock(s.mutex);  // spare blocks are zeroed when they are handed out again
+  for (auto &kv : s.used)
+    if (std::get<0>(kv.first) == kind && std::get<1>(kv.first) == dev) B200_CUDA_TRY(zero(kv.second->base, kv.second->zeroed));
   return B200_OK;
 }
 

@@ -25,7 +25,8 @@ class GraphStep:
     keeps static copies of them and captures ``fn(*static_inputs)`` after ``warmup`` eager runs
     on a side stream. A call copies each new input into its static buffer unless it is that
     buffer, replays on the current stream and returns the static outputs (overwritten by the
-    next call). ``wait=True`` synchronises and returns ``(outputs, seconds)`` of the replay.
+    next call). Every step has workspaces of its own: steps can be replayed on several streams at
+    once, each on one at a time. ``wait=True`` synchronises and returns ``(outputs, seconds)`` of the replay.
     Host inputs are rewritten only after the previous replay has finished reading them."""
 
     def __init__(self, fn, *inputs: torch.Tensor, warmup: int = 2):
