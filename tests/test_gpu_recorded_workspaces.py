@@ -136,3 +136,39 @@ def test_first_calls_captured(queries, heads, prefix):
     torch.cuda.synchronize()
     assert torch.equal(out, good) and torch.equal(out_lse, lse)
     c.check(out, out_lse)
+
+
+@pytest.mark.parametrize("order", ["row", "column"])  # the lean decode call, and the general one
+def test_recorded_host_operands(order):
+    """Recorded steps with pinned host tokens own the buffers these are staged in: later calls on the recording's
+    stream, larger ones too, leave them alone, and two recordings of one stream can be replayed at once."""
+    w = to_device(packed_ref.make_packed(np.random.default_rng(460), "fp4_e2m1", 1024, 4096, 32, "e8m0"), "cuda:0", "e8m0")
+    side, one, two = (torch.cuda.Stream() for _ in range(3))
+
+    def token(seed, m=2):
+        x = torch.randn((m, 4096), generator=torch.Generator().manual_seed(seed)).to(torch.bfloat16)
+        return x.pin_memory().t() if order == "row" else x.t().contiguous().pin_memory()
+
+    def product(x):
+        return tg.matmul(w, x, dtype=torch.bfloat16)
+
+    a, b = token(461), token(462)
+    want_a, want_b = product(a).clone(), product(b).clone()
+    (ga, out_a), (gb, out_b) = record(lambda: product(a), side), record(lambda: product(b), side)
+    with torch.cuda.stream(side):
+        big = token(463, 40)
+        want_big = product(big).clone()
+        others = [torch.full((1 << 14,), 7.0, device="cuda", dtype=torch.bfloat16) for _ in range(64)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        out_a.zero_(), out_b.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(one):
+            ga.replay()
+        with torch.cuda.stream(two):
+            gb.replay()
+        with torch.cuda.stream(side):
+            got = product(big)
+        torch.cuda.synchronize()
+        assert torch.equal(out_a, want_a) and torch.equal(out_b, want_b) and torch.equal(got, want_big)
+    assert all((t == 7).all() for t in others)

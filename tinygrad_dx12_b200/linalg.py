@@ -236,6 +236,19 @@ _HOST_Y_PLANS = ("gemv", "mx", "simt")
 _STAGING: dict = {}  # (device, stream, dtype) -> device buffer reused by every staged call on that stream
 
 
+def _staging(n: int, dtype: torch.dtype, device: torch.device, stream: int) -> torch.Tensor:
+    """A device buffer of at least ``n`` values for host operands of calls on ``stream``. A call that is
+    being recorded has its own, in the recording's memory: the graph may run on another stream, and
+    beside calls on this one, which may outgrow and replace theirs."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(n, device=device, dtype=dtype)
+    key = (device.index, stream, dtype)
+    buf = _STAGING.get(key)
+    if buf is None or buf.numel() < n:
+        buf = _STAGING[key] = torch.empty(max(n, 1 << 14), device=device, dtype=dtype)
+    return buf
+
+
 def _stage_host(t: torch.Tensor, device: torch.device) -> torch.Tensor:
     """A pinned host tensor on ``device``: for 16/32-bit floats laid out row- or column-major, the
     library's copy kernel reads it over the host link (for a decode step's few KB this costs a
@@ -249,13 +262,8 @@ def _stage_host(t: torch.Tensor, device: torch.device) -> torch.Tensor:
     if src is None or t.dtype not in FUSED_IO:
         return t.to(device, non_blocking=True)
     stream = stream_ptr(device)
-    key = (device.index, stream, src.dtype)
-    buf = _STAGING.get(key)
     n = src.numel()
-    if buf is None or buf.numel() < n:
-        buf = torch.empty(max(n, 1 << 14), device=device, dtype=src.dtype)
-        _STAGING[key] = buf
-    dst = buf[:n].view(src.shape)
+    dst = _staging(n, src.dtype, device, stream)[:n].view(src.shape)
     code = _lib.DT[D.name(src.dtype)]
     _lib.call("b200_cast", src.data_ptr(), code, dst.data_ptr(), code, n, stream)
     return dst if src is t else dst.t()
@@ -288,11 +296,7 @@ def _host_decode_step(a: PackedTensor, b: torch.Tensor, dtype, out):
         raise ValueError("host matrix operands must be in pinned memory (torch.Tensor.pin_memory())")
     device = a.data.device
     stream = stream_ptr(device)
-    key = (device.index, stream, b.dtype)
-    buf = _STAGING.get(key)
-    if buf is None or buf.numel() < m * kdim:
-        buf = torch.empty(max(m * kdim, 1 << 14), device=device, dtype=b.dtype)
-        _STAGING[key] = buf
+    buf = _staging(m * kdim, b.dtype, device, stream)
     xcode, ycode = _lib.DT[D.name(b.dtype)], _lib.DT[D.name(dtype)]
     _lib.call("b200_cast", b.data_ptr(), xcode, buf.data_ptr(), xcode, m * kdim, stream)
     y = torch.empty((m, n), device=device, dtype=dtype) if out is None else out
