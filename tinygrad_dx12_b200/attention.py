@@ -18,6 +18,7 @@ import math
 from dataclasses import dataclass
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from . import dtypes as D
@@ -179,19 +180,49 @@ def _turned(x, table, positions, transpose, out=None):
     return out
 
 
+def _tracked(x: torch.Tensor) -> bool:
+    """Whether a gradient, a forward-mode tangent or a transform of torch.func goes through x (which may wrap
+    the tensor there: only autograd's own call takes it out)."""
+    if (x.requires_grad and torch.is_grad_enabled()) or torch._C._are_functorch_transforms_active():
+        return True
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None
+
+
+class _Turn:
+    """The linear map that rotary() applies: what autograd carries beside x, closed to torch.func's wrapping."""
+
+    __slots__ = ("table", "positions", "version", "transpose")
+
+    def __init__(self, table, positions, transpose):
+        self.table, self.positions, self.transpose = table, positions, transpose
+        self.version = None if positions.is_inference() else positions._version
+
+    def of(self, x: torch.Tensor, back: bool) -> torch.Tensor:
+        if self.version is not None and self.positions._version != self.version:
+            raise RuntimeError("the positions of a rotary() were changed in place before its gradient was computed")
+        transpose = self.transpose != back
+        if _tracked(x):
+            return _Rotary.apply(x, _Turn(self.table, self.positions, transpose))
+        return _turned(x, self.table, self.positions, transpose)
+
+
 class _Rotary(torch.autograd.Function):
+    # the map is linear: its gradient is the transposed map, a tangent goes through the map itself
     @staticmethod
-    def forward(ctx, x, table, positions, transpose):
-        ctx.table, ctx.transpose = table, transpose
-        ctx.save_for_backward(positions)
-        return _turned(x, table, positions, transpose)
+    def forward(x, turn):
+        return _turned(x, turn.table, turn.positions, turn.transpose)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        ctx.turn = inputs[1]
 
     @staticmethod
     def backward(ctx, dy):
-        # the map is linear: its gradient is the transposed map
-        (positions,) = ctx.saved_tensors
-        turn = rotary if dy.requires_grad else _turned
-        return turn(dy, ctx.table, positions, not ctx.transpose), None, None, None
+        return ctx.turn.of(dy, back=True), None
+
+    @staticmethod
+    def jvp(ctx, tangent, _):
+        return ctx.turn.of(tangent, back=False)
 
 
 def rotary(x: torch.Tensor, table: RotaryTable, positions: torch.Tensor, transpose: bool = False,
@@ -203,7 +234,7 @@ def rotary(x: torch.Tensor, table: RotaryTable, positions: torch.Tensor, transpo
     gradient's. x has three or four axes of any strides (a copy is made when head_dim is not
     contiguous); ``positions`` (int32 or int64) has x's shape without the last two. ``out`` may be x
     itself. A position outside the table gives NaN and sets bit 1 of the device status.
-    Differentiable in x."""
+    Differentiable in x, any number of times, in reverse and in forward mode."""
     if x.dim() not in (3, 4):
         raise ValueError("rotary takes (tokens, heads, head_dim) or (batch, tokens, heads, head_dim)")
     if x.dtype not in _REAL:
@@ -216,10 +247,10 @@ def rotary(x: torch.Tensor, table: RotaryTable, positions: torch.Tensor, transpo
     if table.device != device:
         raise _elsewhere("table", table, device)
     positions = _index(positions, "positions", x.shape[:-2], device)
-    if x.requires_grad and torch.is_grad_enabled():
+    if _tracked(x):
         if out is not None:
             raise ValueError("rotary with a gradient cannot write into out")
-        return _Rotary.apply(x, table, positions, transpose)
+        return _Rotary.apply(x, _Turn(table, positions, bool(transpose)))
     return _turned(x, table, positions, transpose, out)
 
 
