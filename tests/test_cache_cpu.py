@@ -54,6 +54,11 @@ def test_cache_parts_must_agree():
             tg.PackedCache(*bad)
 
 
+def test_caches_compare_by_identity():
+    a, b = cache(), cache()
+    assert a == a and a != b and len({a, b, a}) == 2 and [b, a].index(a) == 1
+
+
 def test_no_cpu_path():
     c = cache()
     x = torch.zeros(1, 2, 64)

@@ -255,7 +255,7 @@ def rotary(x: torch.Tensor, table: RotaryTable, positions: torch.Tensor, transpo
 
 
 # ---- the cache ----------------------------------------------------------------------------------
-@dataclass(frozen=True)
+@dataclass(frozen=True, eq=False)  # a cache equals itself: comparing storage would read the device
 class PackedCache:
     """Keys and values of cached tokens as low-bit codes with block scales, in pages.
 
