@@ -74,3 +74,18 @@ def test_tensor_parallel_two_gloo_ranks(name, tmp_path):
     y0, y1 = np.load(tmp_path / "rank0.npy"), np.load(tmp_path / "rank1.npy")
     np.testing.assert_array_equal(y0, y1)  # h is replicated after every all-reduce
     _close(y0, r, cfg.act)
+
+
+def test_stack_cache_splits_key_heads():
+    """Each rank keeps its own key heads; sizes that do not split are refused."""
+    import dataclasses
+
+    from tests.stack_helpers import SMALL_INT4
+
+    cfg = dataclasses.replace(SMALL_INT4, q_dim=512, kv_dim=256)
+    for world, heads in ((1, 4), (2, 2), (4, 1)):
+        c = S.StackCache(cfg, None, pages=3, page_size=16, head_dim=64, format="int4", world=world, layers=2, device="cpu")
+        assert [x.kv_heads for x in c.layers] == [heads, heads] and c.layers[0].k.shape == (3, heads, 16, 32)
+    for world in (3, 8):
+        with pytest.raises(ValueError, match="do not split"):
+            S.StackCache(cfg, None, pages=3, page_size=16, head_dim=64, world=world, layers=1, device="cpu")
