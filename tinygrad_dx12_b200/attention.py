@@ -180,10 +180,13 @@ def _turned(x, table, positions, transpose, out=None):
     return out
 
 
+_transforms = torch._C._are_functorch_transforms_active
+
+
 def _tracked(x: torch.Tensor) -> bool:
     """Whether a gradient, a forward-mode tangent or a transform of torch.func goes through x (which may wrap
     the tensor there: only autograd's own call takes it out)."""
-    if (x.requires_grad and torch.is_grad_enabled()) or torch._C._are_functorch_transforms_active():
+    if (x.requires_grad and torch.is_grad_enabled()) or _transforms():
         return True
     return forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None
 
@@ -202,19 +205,16 @@ class _Turn:
             raise RuntimeError("the positions of a rotary() were changed in place before its gradient was computed")
         transpose = self.transpose != back
         if _tracked(x):
-            return _Rotary.apply(x, _Turn(self.table, self.positions, transpose))
+            return _apply(x, _Turn(self.table, self.positions, transpose))
         return _turned(x, self.table, self.positions, transpose)
 
 
 class _Rotary(torch.autograd.Function):
     # the map is linear: its gradient is the transposed map, a tangent goes through the map itself
     @staticmethod
-    def forward(x, turn):
+    def forward(ctx, x, turn):
+        ctx.turn = turn
         return _turned(x, turn.table, turn.positions, turn.transpose)
-
-    @staticmethod
-    def setup_context(ctx, inputs, output):
-        ctx.turn = inputs[1]
 
     @staticmethod
     def backward(ctx, dy):
@@ -223,6 +223,22 @@ class _Rotary(torch.autograd.Function):
     @staticmethod
     def jvp(ctx, tangent, _):
         return ctx.turn.of(tangent, back=False)
+
+
+class _RotaryTransformed(_Rotary):
+    """The form that torch.func's transforms take; elsewhere a training step's call is 115 us in it, 87 in the other."""
+
+    @staticmethod
+    def forward(x, turn):
+        return _turned(x, turn.table, turn.positions, turn.transpose)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        ctx.turn = inputs[1]
+
+
+def _apply(x, turn):
+    return (_RotaryTransformed if _transforms() else _Rotary).apply(x, turn)
 
 
 def rotary(x: torch.Tensor, table: RotaryTable, positions: torch.Tensor, transpose: bool = False,
@@ -250,7 +266,7 @@ def rotary(x: torch.Tensor, table: RotaryTable, positions: torch.Tensor, transpo
     if _tracked(x):
         if out is not None:
             raise ValueError("rotary with a gradient cannot write into out")
-        return _Rotary.apply(x, _Turn(table, positions, bool(transpose)))
+        return _apply(x, _Turn(table, positions, bool(transpose)))
     return _turned(x, table, positions, transpose, out)
 
 
