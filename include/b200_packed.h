@@ -19,9 +19,9 @@
  *     (3 <= m <= 64) splits K across CTAs and keeps a 16 MiB split-K workspace, its block-scaled
  *     kernel one of 10 MiB, b200_cache_attention others (see there). The first such call on a
  *     (device, stream) allocates it for the life of the process; the calls of a stream capture
- *     have one of their own, which the graph owns: recorded graphs can be replayed on any streams,
- *     beside one another and beside direct calls (but not several executables of one graph at once)
- *     (b200_packed_linear_noalloc is the allocation-free form). Other allocations are the
+ *     have one of their own: recorded graphs can be replayed on any streams, beside one another
+ *     and beside direct calls (but not several executables of one graph at once); see
+ *     b200_capture_release (b200_packed_linear_noalloc is the allocation-free form). Other allocations are the
  *     explicit b200_malloc / b200_stream_create / b200_event_create calls;
  *   - `stream` is a cudaStream_t passed as void* (NULL = legacy default stream);
  *     all compute entry points are asynchronous on that stream.
@@ -200,6 +200,13 @@ int32_t b200_device_wait_flag(const int32_t *flag, int32_t expect, int64_t max_s
 int32_t b200_packed_linear_multi(const b200_packed_desc *w, const void *x, int32_t x_dtype, int64_t m,
                                  int64_t x_stride_m, void *const *y, int32_t n_y, int32_t y_dtype, int64_t y_stride_m,
                                  int32_t flags, void *stream);
+
+/* Workspaces of recorded calls. b200_capture_id: the capture that `stream` is in, 0 if none.
+ * b200_capture_release: what was recorded in capture `id` is gone, its replays have been launched for
+ * the last time; its workspaces serve captures that begin once those replays have completed. Without this call they
+ * stay for the life of the process. No counterpart in the reference. */
+int32_t b200_capture_id(void *stream, uint64_t *id);
+int32_t b200_capture_release(uint64_t id);
 
 /* Allocation-free form of b200_packed_linear for a few tokens (3 <= m <= 32, 4-bit formats,
  * the split-K decode GEMM). No counterpart in the reference. Same arguments and result as

@@ -132,3 +132,11 @@ def test_c_entries_check_arguments():
     assert lib.b200_rotary(None, 12, 0, 1, 1, 64, 0, 0, 0, None, 0, 0, 0, None, None, 6, 0, None) == 0
     assert lib.b200_cache_attention_scratch(2, 3, 4, 64, 10) == 2 * 3 * 4 * 66 * 4
     assert lib.b200_cache_attention_scratch(2, 3, 4, 64, 0) == 0
+
+
+def test_c_entries_of_captures():
+    lib = _lib.lib()
+    assert lib.b200_capture_release(0) == 0 and lib.b200_capture_release(12345) == 0
+    assert lib.b200_capture_id(None, None) == _lib.ERR_INVALID and "null" in _lib.last_error()
+    n = ctypes.c_uint64(7)
+    assert lib.b200_capture_id(None, ctypes.byref(n)) == 0 and n.value == 0  # the legacy stream is never captured

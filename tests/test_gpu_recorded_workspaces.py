@@ -1,11 +1,10 @@
 """Recorded steps own the memory that their kernels leave partial results in: two recordings of one stream,
 replayed on two streams at once beside eager calls on the stream that recorded them, give each the bits of an
-eager call; recordings that are gone give their memory back to later ones; a capture needs no call before it."""
+eager call; steps that are gone give their memory back to later ones; a capture needs no call before it."""
 
 from __future__ import annotations
 
 import gc
-import time
 
 import numpy as np
 import pytest
@@ -85,33 +84,39 @@ def test_recordings_of_one_stream_replayed_at_once(kind):
         assert all(torch.equal(e, want_c) for e in eager)
 
 
-def test_recordings_give_their_memory_back():
-    step, want = call("many", 430)  # 38 MiB a recording
-    side = torch.cuda.Stream()
+def test_steps_give_their_memory_back():
+    run, want = call("many", 430)  # 38 MiB a recording
+    x = torch.zeros(1, device="cuda")
+
+    def step():
+        return tg.GraphStep(lambda _: run(), x)
 
     def free():
         gc.collect()
         torch.cuda.synchronize()
-        time.sleep(0.2)
         torch.cuda.empty_cache()
         return torch.cuda.mem_get_info()[0]
 
-    kept, out_kept = record(step, side)
-    record(step, side)
+    for _ in range(40):  # every stream of torch's pool has its workspace for direct calls
+        step()
+    kept = step()
     before = free()
     for _ in range(30):
-        graph, out = record(step, side)
-        graph.replay()
-        torch.cuda.synchronize()
-        assert torch.equal(out, want)
-        del graph, out
-        torch.cuda.synchronize()
-        time.sleep(0.02)
+        other = step()
+        assert torch.equal(other(), want)
+        del other
     assert before - free() < 200 << 20  # 30 blocks would be 1.1 GiB
-    out_kept.zero_()
-    kept.replay()
-    torch.cuda.synchronize()
-    assert torch.equal(out_kept, want)
+    kept.outputs.zero_()
+    assert torch.equal(kept(), want)
+    with pytest.raises(RuntimeError, match="on purpose"):  # a recording that fails gives its memory back, too
+        tg.GraphStep(lambda _: failing(run), x)
+    assert torch.equal(step()(), want) and torch.equal(kept(), want)
+
+
+def failing(run):
+    run()
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("on purpose")
 
 
 @pytest.mark.parametrize("kind", list(PRODUCTS))

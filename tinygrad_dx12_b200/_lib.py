@@ -85,6 +85,8 @@ SIGNATURES = {
     "b200_cache_read": ([_P, _P, _I32, _I64, _P, _P, _I32, _P], _I32),
     "b200_cache_attention_scratch": ([_I64, _I64, _I32, _I32, _I64], _I64),
     "b200_cache_attention": ([_P, _P, _P], _I32),
+    "b200_capture_id": ([_P, ctypes.POINTER(ctypes.c_uint64)], _I32),
+    "b200_capture_release": ([ctypes.c_uint64], _I32),
     "b200_device_status": ([_I32, ctypes.POINTER(ctypes.c_uint32), _I32], _I32),
 }
 

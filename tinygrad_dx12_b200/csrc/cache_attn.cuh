@@ -161,7 +161,8 @@ __device__ __forceinline__ void join(float4 &o, float &m, float &l, const float 
 // (and so are the products) whatever the sum. No key seen: zeros.
 __device__ __forceinline__ float2 inverse_sum(float l) {
   const bool small = l < 1.f;
-  return make_float2(l == 0.f ? 0.f : (small ? SUM_UNIT : 1.f) / l, small ? 1.f : SUM_UNIT);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  return make_float2(small ? inv * SUM_UNIT : inv, small ? 1.f : SUM_UNIT);
 }
 // The natural logarithm of the softmax's sum.
 __device__ __forceinline__ float log_sum(float m, float l) {

@@ -3,9 +3,9 @@
 // Calls on one stream follow one another, so they share a block per (kernel family, device, stream), allocated
 // on the first call and kept for the life of the process. A recorded graph runs on whatever stream replays it,
 // beside calls on the stream that recorded it and beside other recordings: the calls of a capture share a block
-// of their own, which the graph owns (a user object) and which goes back to a list, for later recordings, when
-// the graph and everything instantiated from it are gone. It is allocated outside the graph while that is being
-// captured: a recorded step has no allocation nodes.
+// of their own, until whoever holds the graph says that it is gone (b200_capture_release); then it serves a later
+// capture. It is allocated outside the graph while that is being captured: a recorded step has no allocation
+// nodes. (A user object, by which the graph would say so itself, costs 2 to 3 us of every replay.)
 #include <map>
 #include <mutex>
 #include <tuple>
@@ -27,9 +27,9 @@ struct State {
   std::mutex mutex;   // of the members below
   std::mutex making;  // one block is made at a time; never taken while `mutex` is held
   std::map<Key, Block *> used;
-  std::vector<Block *> spare;  // of recordings that are gone
+  std::vector<Block *> spare;  // of recordings that are gone; their tickets are zero, as kernels leave them
 };
-State &state() {  // never destroyed: graphs may outlive static objects
+State &state() {  // never destroyed: a recording may be released after static objects
   static State *s = new State;
   return *s;
 }
@@ -52,13 +52,16 @@ cudaError_t zero(uint8_t *p, size_t n) {
   return e;
 }
 
-void CUDART_CB graph_is_gone(void *block) {  // no CUDA call may be made here
-  Block *b = static_cast<Block *>(block);
-  State &s = state();
-  std::lock_guard<std::mutex> lock(s.mutex);
-  auto it = s.used.find(b->key);
-  if (it != s.used.end() && it->second == b) s.used.erase(it);
-  s.spare.push_back(b);
+// The capture that `stream` is in, 0 if none.
+int32_t capture_of(cudaStream_t stream, unsigned long long *id) {
+  *id = 0;
+  if (stream == nullptr || stream == cudaStreamLegacy) return B200_OK;  // cannot be captured
+  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+  B200_CUDA_TRY(cudaStreamIsCapturing(stream, &cs));
+  if (cs == cudaStreamCaptureStatusNone) return B200_OK;
+  B200_CUDA_TRY(cudaStreamGetCaptureInfo_v2(stream, &cs, id, nullptr, nullptr, nullptr));
+  if (cs != cudaStreamCaptureStatusActive) return b200_set_error(B200_ERR_CUDA, "the stream's capture is invalid");
+  return B200_OK;
 }
 
 }  // namespace
@@ -67,69 +70,40 @@ static int32_t find_or_make(WorkspaceKind kind, size_t bytes, size_t zeroed, cud
   int dev = 0;
   B200_CUDA_TRY(cudaGetDevice(&dev));
   unsigned long long id = (unsigned long long)(uintptr_t)stream, capture = 0;
-  cudaGraph_t graph = nullptr;
   if (stream == cudaStreamLegacy) id = 0;
   if (stream == cudaStreamPerThread) B200_CUDA_TRY(cudaStreamGetId(stream, &id));  // one handle for every thread's
-  if (id != 0) {  // the legacy stream cannot be captured
-    cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-    B200_CUDA_TRY(cudaStreamIsCapturing(stream, &cs));
-    if (cs != cudaStreamCaptureStatusNone) {
-      B200_CUDA_TRY(cudaStreamGetCaptureInfo_v2(stream, &cs, &capture, &graph, nullptr, nullptr));
-      if (cs != cudaStreamCaptureStatusActive) return b200_set_error(B200_ERR_CUDA, "workspace: the stream's capture is invalid");
-    }
-  }
+  if (int32_t rc = capture_of(stream, &capture)) return rc;
   const Key key(kind, dev, id, capture);
   State &s = state();
-  auto found = [&]() {
+  auto found = [&](bool spare) {
     std::lock_guard<std::mutex> lock(s.mutex);
     auto it = s.used.find(key);
+    if (it == s.used.end() && spare)
+      for (size_t i = 0; i < s.spare.size(); ++i)
+        if (std::get<0>(s.spare[i]->key) == kind && std::get<1>(s.spare[i]->key) == dev) {
+          s.spare[i]->key = key;
+          it = s.used.emplace(key, s.spare[i]).first;
+          s.spare.erase(s.spare.begin() + i);
+          break;
+        }
     if (it != s.used.end()) *base = it->second->base;
     return it != s.used.end();
   };
-  if (found()) return B200_OK;
+  if (found(false)) return B200_OK;
   std::lock_guard<std::mutex> making(s.making);
-  if (found()) return B200_OK;
-  Block *b = nullptr;
-  if (capture != 0) {
-    std::lock_guard<std::mutex> lock(s.mutex);
-    for (size_t i = 0; i < s.spare.size() && b == nullptr; ++i)
-      if (std::get<0>(s.spare[i]->key) == kind && std::get<1>(s.spare[i]->key) == dev) {
-        b = s.spare[i];
-        s.spare.erase(s.spare.begin() + i);
-      }
-  }
+  if (found(capture != 0)) return B200_OK;
   Relaxed relaxed;
-  if (b == nullptr) {
-    b = new Block{key, nullptr, zeroed};
-    const cudaError_t e = cudaMalloc((void **)&b->base, bytes);
-    if (e != cudaSuccess) {
-      delete b;
-      cudaGetLastError();
-      return b200_set_error(B200_ERR_CUDA, "workspace of %zu bytes: %s", bytes, cudaGetErrorString(e));
-    }
+  uint8_t *p = nullptr;
+  cudaError_t e = cudaMalloc((void **)&p, bytes);
+  if (e == cudaSuccess) e = zero(p, zeroed);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    if (p != nullptr) cudaFree(p);
+    return b200_set_error(B200_ERR_CUDA, "workspace of %zu bytes: %s", bytes, cudaGetErrorString(e));
   }
-  b->key = key;
-  cudaError_t e = zero(b->base, zeroed);
-  if (e == cudaSuccess && capture != 0) {
-    {
-      std::lock_guard<std::mutex> lock(s.mutex);
-      s.used[key] = b;
-    }
-    cudaUserObject_t object = nullptr;
-    e = cudaUserObjectCreate(&object, b, graph_is_gone, 1, cudaUserObjectNoDestructorSync);
-    if (e != cudaSuccess) {
-      graph_is_gone(b);
-    } else {
-      e = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove);
-      if (e != cudaSuccess) cudaUserObjectRelease(object, 1);  // calls graph_is_gone
-    }
-  } else {
-    std::lock_guard<std::mutex> lock(s.mutex);
-    if (e == cudaSuccess) s.used[key] = b;
-    else s.spare.push_back(b);
-  }
-  if (e != cudaSuccess) return b200_set_error(B200_ERR_CUDA, "workspace: %s", cudaGetErrorString(e));
-  *base = b->base;
+  std::lock_guard<std::mutex> lock(s.mutex);
+  s.used[key] = new Block{key, p, zeroed};
+  *base = p;
   return B200_OK;
 }
 
@@ -147,10 +121,45 @@ int32_t workspace_zero(WorkspaceKind kind) {
   State &s = state();
   B200_CUDA_TRY(cudaDeviceSynchronize());
   std::lock_guard<std::mutex> making(s.making);
-  std::lock_guard<std::mutex> lock(s.mutex);  // spare blocks are zeroed when they are handed out again
-  for (auto &kv : s.used)
-    if (std::get<0>(kv.first) == kind && std::get<1>(kv.first) == dev) B200_CUDA_TRY(zero(kv.second->base, kv.second->zeroed));
+  std::lock_guard<std::mutex> lock(s.mutex);
+  std::vector<Block *> all(s.spare);
+  for (auto &kv : s.used) all.push_back(kv.second);
+  for (Block *b : all)
+    if (std::get<0>(b->key) == kind && std::get<1>(b->key) == dev) B200_CUDA_TRY(zero(b->base, b->zeroed));
   return B200_OK;
 }
 
 }  // namespace b200
+
+using namespace b200;
+
+extern "C" {
+
+int32_t b200_capture_id(void *stream, uint64_t *id) {
+  if (id == nullptr) return b200_set_error(B200_ERR_INVALID, "capture_id: null pointer");
+  unsigned long long c = 0;
+  if (int32_t rc = capture_of((cudaStream_t)stream, &c)) return rc;
+  *id = c;
+  return B200_OK;
+}
+
+int32_t b200_capture_release(uint64_t id) {
+  if (id == 0) return B200_OK;
+  try {
+    State &s = state();
+    std::lock_guard<std::mutex> lock(s.mutex);
+    for (auto it = s.used.begin(); it != s.used.end();) {
+      if (std::get<3>(it->first) == id) {
+        s.spare.push_back(it->second);
+        it = s.used.erase(it);
+      } else {
+        ++it;
+      }
+    }
+  } catch (...) {
+    return b200_set_error(B200_ERR_CUDA, "capture_release: out of host memory");
+  }
+  return B200_OK;
+}
+
+}  // extern "C"

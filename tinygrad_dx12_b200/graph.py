@@ -14,8 +14,15 @@ from __future__ import annotations
 
 import ctypes
 import time
+import weakref
 
 import torch
+
+from . import _lib
+
+
+def _release(capture: ctypes.c_uint64) -> None:
+    _lib.lib().b200_capture_release(capture.value)
 
 
 class GraphStep:
@@ -55,7 +62,12 @@ class GraphStep:
         torch.cuda.current_stream(self.device).wait_stream(side)
         torch.cuda.synchronize(self.device)
         self.graph = torch.cuda.CUDAGraph()
+        # the recording's workspaces go to a later one when this step is gone (a later capture begins with a
+        # device synchronisation, behind the last replay)
+        capture = ctypes.c_uint64()
+        weakref.finalize(self, _release, capture).atexit = False
         with torch.cuda.graph(self.graph, stream=side):
+            _lib.call("b200_capture_id", side.cuda_stream, ctypes.byref(capture))
             self.outputs = fn(*self.static)
         torch.cuda.synchronize(self.device)
         self._done = torch.cuda.Event()
