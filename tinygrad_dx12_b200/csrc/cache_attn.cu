@@ -716,12 +716,12 @@ __global__ void __launch_bounds__(THREADS, Cfg<F, D, NT, BLK>::CTAS) attn_kernel
 // ---- workspace of split segments -------------------------------------------------------------------
 constexpr int MAX_ROWS_D = 16 * 128;  // ROWS * D of every variant is at most this
 
-// Two slots for each of the `grid` CTAs that a launch has at most, and their tickets, first.
+// Two slots for each of the `grid` CTAs that a launch has at most, and their tickets.
 static int32_t workspace_for(cudaStream_t stream, int grid, Params &p) {
-  const size_t slots = 2 * (size_t)grid, t_bytes = ((size_t)grid * 4 + 255) / 256 * 256, o_bytes = slots * MAX_ROWS_D * 4;
+  const size_t slots = 2 * (size_t)grid, o_bytes = slots * MAX_ROWS_D * 4, bytes = o_bytes + slots * 16 * 2 * 4;
   uint8_t *base = nullptr;
-  if (int32_t rc = workspace_of(WS_ATTENTION, t_bytes + o_bytes + slots * 16 * 2 * 4, t_bytes, stream, &base)) return rc;
-  p.tickets = (uint32_t *)base, p.ws_o = (float *)(base + t_bytes), p.ws_ml = (float *)(base + t_bytes + o_bytes);
+  if (int32_t rc = workspace_of(WS_ATTENTION, bytes, (size_t)grid * 4, stream, &base)) return rc;
+  p.ws_o = (float *)base, p.ws_ml = (float *)(base + o_bytes), p.tickets = (uint32_t *)(base + bytes);
   return B200_OK;
 }
 

@@ -429,16 +429,15 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (warp == MMA_WARP) tmem_dealloc(tmem, p.tmem_cols);
 }
 
-// ---- workspace: tickets of shared tiles and their fp32 partials ----------------------------------
+// ---- workspace: fp32 partials of shared tiles, then their tickets --------------------------------
 static int32_t workspace_for(cudaStream_t stream, Workspace &out) {
   int sms = 0;
   B200_CUDA_TRY(device_sms(&sms));
-  const size_t t_bytes = TICKETS * sizeof(unsigned int);
   out.part_bytes = (size_t)sms * 2 * 64 * TM * sizeof(float);
   uint8_t *base = nullptr;
-  if (int32_t rc = workspace_of(WS_MX, t_bytes + out.part_bytes, t_bytes, stream, &base)) return rc;
-  out.tickets = reinterpret_cast<unsigned int *>(base);
-  out.part = reinterpret_cast<float *>(base + t_bytes);
+  if (int32_t rc = workspace_of(WS_MX, out.part_bytes, TICKETS * sizeof(unsigned int), stream, &base)) return rc;
+  out.part = reinterpret_cast<float *>(base);
+  out.tickets = reinterpret_cast<unsigned int *>(base + out.part_bytes);
   return B200_OK;
 }
 

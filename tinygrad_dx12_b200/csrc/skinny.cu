@@ -514,7 +514,7 @@ static size_t smem_bytes(int esz) {
   return 1024 + (size_t)stages<NT>(esz) * slot_bytes<NT>(esz) + 2 * 4 * 8 + 16 + 4 * 8 * NT * 4;
 }
 
-// ---- split-K workspace: tickets of row blocks, then fp32 partials --------------------------------
+// ---- split-K workspace: fp32 partials, then tickets of row blocks --------------------------------
 constexpr size_t WS_BYTES = 16u << 20;  // fp32 partials (max splits x M x N)
 constexpr size_t TICKETS = 16384;       // row blocks (N up to 2M rows)
 
@@ -681,15 +681,15 @@ int32_t launch_skinny(const LinearArgs &a, cudaStream_t stream) {
   unsigned int *tickets = nullptr;
   if (splits > 1) {
     const int64_t nrb = (a.rows + RB - 1) / RB;
-    const size_t per_split = (size_t)a.m * a.rows * sizeof(float), t_bytes = TICKETS * sizeof(unsigned int);
+    const size_t per_split = (size_t)a.m * a.rows * sizeof(float);
     if ((size_t)nrb > TICKETS) {
       splits = 1;
     } else {
       uint8_t *base = nullptr;
-      if (int32_t rc = workspace_of(WS_SPLIT_K, t_bytes + WS_BYTES, t_bytes, stream, &base)) return rc;
+      if (int32_t rc = workspace_of(WS_SPLIT_K, WS_BYTES, TICKETS * sizeof(unsigned int), stream, &base)) return rc;
       while (splits > 1 && (size_t)splits * per_split > WS_BYTES) --splits;
-      tickets = reinterpret_cast<unsigned int *>(base);
-      ws = reinterpret_cast<float *>(base + t_bytes);
+      ws = reinterpret_cast<float *>(base);
+      tickets = reinterpret_cast<unsigned int *>(base + WS_BYTES);
     }
   }
   const int sk = gemv::scale_kind(a);

@@ -21,7 +21,7 @@ using Key = std::tuple<int, int, unsigned long long, unsigned long long>;  // ki
 struct Block {
   Key key;
   uint8_t *base;
-  size_t zeroed;
+  size_t bytes, tickets;
 };
 struct State {
   std::mutex mutex;   // of the members below
@@ -66,7 +66,7 @@ int32_t capture_of(cudaStream_t stream, unsigned long long *id) {
 
 }  // namespace
 
-static int32_t find_or_make(WorkspaceKind kind, size_t bytes, size_t zeroed, cudaStream_t stream, uint8_t **base) {
+static int32_t find_or_make(WorkspaceKind kind, size_t bytes, size_t tickets, cudaStream_t stream, uint8_t **base) {
   int dev = 0;
   B200_CUDA_TRY(cudaGetDevice(&dev));
   unsigned long long id = (unsigned long long)(uintptr_t)stream, capture = 0;
@@ -94,22 +94,22 @@ static int32_t find_or_make(WorkspaceKind kind, size_t bytes, size_t zeroed, cud
   if (found(capture != 0)) return B200_OK;
   Relaxed relaxed;
   uint8_t *p = nullptr;
-  cudaError_t e = cudaMalloc((void **)&p, bytes);
-  if (e == cudaSuccess) e = zero(p, zeroed);
+  cudaError_t e = cudaMalloc((void **)&p, bytes + tickets);
+  if (e == cudaSuccess && tickets > 0) e = zero(p + bytes, tickets);
   if (e != cudaSuccess) {
     cudaGetLastError();
     if (p != nullptr) cudaFree(p);
-    return b200_set_error(B200_ERR_CUDA, "workspace of %zu bytes: %s", bytes, cudaGetErrorString(e));
+    return b200_set_error(B200_ERR_CUDA, "workspace of %zu bytes: %s", bytes + tickets, cudaGetErrorString(e));
   }
   std::lock_guard<std::mutex> lock(s.mutex);
-  s.used[key] = new Block{key, p, zeroed};
+  s.used[key] = new Block{key, p, bytes, tickets};
   *base = p;
   return B200_OK;
 }
 
-int32_t workspace_of(WorkspaceKind kind, size_t bytes, size_t zeroed, cudaStream_t stream, uint8_t **base) {
+int32_t workspace_of(WorkspaceKind kind, size_t bytes, size_t tickets, cudaStream_t stream, uint8_t **base) {
   try {
-    return find_or_make(kind, bytes, zeroed, stream, base);
+    return find_or_make(kind, bytes, tickets, stream, base);
   } catch (...) {
     return b200_set_error(B200_ERR_CUDA, "workspace: out of host memory");
   }
@@ -125,7 +125,7 @@ int32_t workspace_zero(WorkspaceKind kind) {
   std::vector<Block *> all(s.spare);
   for (auto &kv : s.used) all.push_back(kv.second);
   for (Block *b : all)
-    if (std::get<0>(b->key) == kind && std::get<1>(b->key) == dev) B200_CUDA_TRY(zero(b->base, b->zeroed));
+    if (std::get<0>(b->key) == kind && std::get<1>(b->key) == dev) B200_CUDA_TRY(zero(b->base + b->bytes, b->tickets));
   return B200_OK;
 }
 
