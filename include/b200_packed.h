@@ -21,8 +21,8 @@
  *     (device, stream) allocates it for the life of the process; the calls of a stream capture
  *     have one of their own: recorded graphs can be replayed on any streams, beside one another
  *     and beside direct calls (but not several executables of one graph at once); see
- *     b200_capture_release (b200_packed_linear_noalloc is the allocation-free form). Other allocations are the
- *     explicit b200_malloc / b200_stream_create / b200_event_create calls;
+ *     b200_capture_release. b200_packed_linear_noalloc is the allocation-free form. Other
+ *     allocations are the explicit b200_malloc / b200_stream_create / b200_event_create calls;
  *   - `stream` is a cudaStream_t passed as void* (NULL = legacy default stream);
  *     all compute entry points are asynchronous on that stream.
  *   - thread-safe: no global mutable state on the compute paths except the per-thread
@@ -202,9 +202,9 @@ int32_t b200_packed_linear_multi(const b200_packed_desc *w, const void *x, int32
                                  int32_t flags, void *stream);
 
 /* Workspaces of recorded calls. b200_capture_id: the capture that `stream` is in, 0 if none.
- * b200_capture_release: what was recorded in capture `id` is gone, its replays have been launched for
- * the last time; its workspaces serve captures that begin once those replays have completed. Without this call they
- * stay for the life of the process. No counterpart in the reference. */
+ * b200_capture_release: what was recorded in capture `id` is gone; its workspaces go to later
+ * captures, which must not begin before its last replay has completed. Without this call they stay
+ * for the life of the process. No counterpart in the reference. */
 int32_t b200_capture_id(void *stream, uint64_t *id);
 int32_t b200_capture_release(uint64_t id);
 
@@ -331,7 +331,9 @@ int32_t b200_cache_read(const b200_cache_desc *cache, const void *slots, int32_t
  * (lse: -inf). A page outside the cache counts as absent keys and sets bit 1 of
  * b200_device_status. q: F16 or BF16, element strides (request, token, head), unit along head_dim;
  * out: contiguous [batch, queries, heads, head_dim] of q's type; lse: fp32 [batch, queries, heads]
- * natural logarithms of the softmax sums, or NULL. `scratch` holds b200_cache_attention_scratch()
+ * natural logarithms of the softmax sums, or NULL (over 8-bit codes with a bfloat16 scale a row,
+ * under more than 64 query rows of a key head, asking for them keeps keys' scales in fp32, and
+ * bfloat16 results differ in their last bits). `scratch` holds b200_cache_attention_scratch()
  * bytes (prefix only). A NaN in a key's or value's scale makes the rows that see that key NaN, in all
  * their values. Workspaces: 5 MiB per (device, stream) or capture, and 38 MiB more when a key head
  * has over 64 query rows (queries, or batch x queries for the prefix, x heads / kv_heads). More

@@ -5,6 +5,7 @@ eager call; steps that are gone give their memory back to later ones; a capture 
 from __future__ import annotations
 
 import gc
+import threading
 
 import numpy as np
 import pytest
@@ -177,3 +178,29 @@ def test_recorded_host_operands(order):
         torch.cuda.synchronize()
         assert torch.equal(out_a, want_a) and torch.equal(out_b, want_b) and torch.equal(got, want_big)
     assert all((t == 7).all() for t in others)
+
+
+def test_streams_of_threads(monkeypatch):
+    """The handle that stands for a stream of each thread's own: two threads at once, each with its workspace."""
+    from tinygrad_dx12_b200 import attention
+
+    per_thread = 2  # cudaStreamPerThread
+    steps = [call("few", 470), call("few", 480)]
+    monkeypatch.setattr(attention, "stream_ptr", lambda device: per_thread)
+    torch.cuda.synchronize()
+    start = threading.Barrier(2)
+    got = [[], []]
+
+    def work(i):
+        torch.cuda.set_device(0)
+        start.wait()
+        got[i] += [steps[i][0]() for _ in range(40)]
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for outs, (_, want) in zip(got, steps):
+        assert len(outs) == 40 and all(torch.equal(o, want) for o in outs)

@@ -480,10 +480,14 @@ def cache_attention(q: torch.Tensor, cache: PackedCache, tables: torch.Tensor, l
     batch shares: they are read once and multiplied with all requests' queries together.
 
     A query that sees no key gives zeros, with a logarithm of -inf. ``return_lse`` also returns the
-    natural logarithms of the softmax sums, float32 of q's shape without head_dim. Lengths beyond the
+    natural logarithms of the softmax sums, float32 of q's shape without head_dim; with over 64 query
+    rows of a key head over int8 or fp8e4m3 codes with a bfloat16 scale a row, bfloat16 results then
+    differ in their last bits from those without (keys' scales stay in fp32). Lengths beyond the
     table count as the table's; a page outside the cache counts as no keys and sets bit 1 of the
     device status. The launch does not depend on the lengths, so it can be recorded in a
-    ``GraphStep``. No gradients."""
+    ``GraphStep``. At most 262144 query rows of a key head (queries, or batch * queries for the prefix,
+    times heads / kv_heads), 32768 for a head_dim of 256: longer prompts are called in parts. No
+    gradients."""
     single = q.dim() == 3
     if q.dim() not in (3, 4) or q.shape[-1] != cache.head_dim:
         raise ValueError(f"q must have shape (batch, [queries,] heads, {cache.head_dim})")

@@ -26,8 +26,6 @@ template <> struct CFmt<B200_CACHE_FP8E4M3> { static constexpr int bits = 8; sta
 template <> struct CFmt<B200_CACHE_INT4> { static constexpr int bits = 4; static constexpr double qmax = 7.0; };
 template <> struct CFmt<B200_CACHE_FP4_E2M1> { static constexpr int bits = 4; static constexpr double qmax = 6.0; };
 
-__host__ __device__ inline int cache_bits(int f) { return f == B200_CACHE_INT8 || f == B200_CACHE_FP8E4M3 ? 8 : 4; }
-
 // Scale `i` of an array as the bits of a bfloat16 (an E8M0 byte b is bfloat16 2^(b-127) exactly).
 __device__ __forceinline__ uint32_t scale_bits(const void *p, int64_t i, bool e8m0) {
   if (e8m0) {

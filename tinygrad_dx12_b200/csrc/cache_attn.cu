@@ -21,11 +21,12 @@
 // its scale in fp32. For V^T a lane reads its D / 8 neighbouring values of four keys; pairs of keys
 // are joined by byte permutes before the codes become fp16. p is turned with movmatrix.
 //
-// Every warp works alone: it copies units of 16 to 64 keys (4 KB of codes) into a ring of its own
-// with cp.async, 16 bytes a lane, two units ahead, chunks xor-ed by their row so that both operands'
-// reads spread over the banks; a lane loads the scales of one key three units ahead and leaves what
-// the scores need of them beside the ring. Page numbers are read one unit earlier still. 16 warps of
-// an SM keep up to 128 KB in flight, and no barrier stands between a segment's units.
+// Every warp works alone: it copies units of 16 to 64 keys (4 KB of codes, 8 KB for 256 values of 8 bits)
+// into a ring of two of its own with cp.async, 16 bytes a lane, one unit ahead, chunks xor-ed by their row so
+// that both operands' reads spread over the banks; a lane asks for the scales of a key two units ahead and
+// leaves what the scores need of them beside the ring, and page numbers are asked for three units ahead.
+// While a unit is computed the SM's 16 warps have 64 KB of codes on their way (8 warps 32 KB where 16 query
+// rows share a pass), and no barrier stands between a segment's units.
 //
 // The units of all (request, key head, row tile) segments are laid end to end in rounds (a unit for
 // each warp) and cut into equal runs, one per CTA, from the lengths on the device: ragged batches
@@ -35,10 +36,10 @@
 // instead of 12.2 for 4 requests of 4096 int4 keys, and 7.0 instead of 7.4 at 300 int8 keys.
 //
 // Measured (bf16, 8 key heads of 128, device time): 64 requests of 2048 to 8192 keys, 64 heads, FP4 in
-// blocks: 128 us = 2.8 TB/s. Bound by instruction issue there: about 500 warp instructions for each 16
-// keys of a key head, at 0.62 an SM quarter and cycle. 32 requests of 8192 keys: int8 4.2 TB/s, fp8 4.6
-// TB/s. One request of 257 int8 keys: 8.6 us, a chain of launch, lengths, page numbers, codes, two
-// products, the warps' and the CTAs' joins.
+// blocks: 127 us = 2.8 TB/s. Bound by instruction issue there: about 500 warp instructions for each 16
+// keys of a key head, at 0.62 an SM quarter and cycle. 32 requests of 8192 keys, a scale a row: int8 116 us
+// = 4.7 TB/s, fp8 104 us = 5.3 TB/s. One request of 257 int8 keys: 8.4 us, a chain of launch, lengths, page
+// numbers, codes, two products, the warps' and the CTAs' joins.
 #include "cache_attn.cuh"
 #include "sm100.cuh"
 

@@ -15,6 +15,8 @@ constexpr float BIAS = 15.f - LAZY;  // p = 2^(u - m + BIAS) uses fp16 up to 2^1
 // A key adds p / vs to the denominator: up to 2^15 * 2^100 where its values are zero (a block of zeros has
 // the scale 2^-100, no reference is below that), down to 2^11 / 2^100 where the largest are all that counts.
 // Sums are kept as 2^-SUM_EXP of themselves: 2^31 keys stay below 2^126, and 2^-109 is an ordinary number.
+// p below 2^-126 is flushed to zero: beside values whose scale is 2^13 (fp16's largest) a key of zeros counts
+// down to 2^-24 of their weight, and fully, at equal scores, up to scales of 2^37.
 constexpr int SUM_EXP = 20;
 constexpr float SUM_UNIT = 1.f / (1 << SUM_EXP);
 

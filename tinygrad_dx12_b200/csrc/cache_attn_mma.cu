@@ -20,7 +20,7 @@
 // slot, and the two slots fill each other's gaps only in part.
 // Measured (bf16, 8 key heads of 128, device time): 1024 tokens of 32 heads against 8192 fp8 keys 215 us
 // = 600 TFLOP/s (the few-row kernel 1087); 128 requests of 64 heads behind 16384 int4 keys, with their
-// own 1 to 1024, 197 us (595).
+// own 1 to 1024, 193 us (595).
 //
 // Tiles of all (row tile, key head) segments are laid end to end and cut into equal runs, one per CTA.
 // A segment within a run is finished there; the others leave their share (numerators, maximum,
@@ -1016,6 +1016,9 @@ static int32_t launch_f(Params &p, int fmt, int dim, bool blk, cudaStream_t stre
 // dearer start. Device us there and here: 8192 fp8 keys, 64 rows 34.9 and 43.1, 128 rows 50.0 and 41.6;
 // 32768 keys, 64 rows 84 and 99, 128 rows 146 and 92; 16 requests of FP4 blocks, 48 rows 155 and 200, 64
 // rows 202 and 202, 80 rows 248 and 204; an int4 prefix of 16384, 64 rows 72 and 80, 96 rows 88 and 83.
+// The rule does not look at the number of keys, and over few of them the few-row kernel would be faster: 512
+// fp8 keys, 96 rows 13.7 and 22.0, 128 rows 13.8 and 21.9, 192 rows 22.0 and 21.5, 256 rows 12.3 and 22.9; 64
+// requests behind a prefix of 1024 keys 56.7 and 65.6.
 bool mma_supported(const Params &p, int dim) { return dim <= 128 && p.rows > 64; }
 
 int32_t launch_mma(Params &p, int q_dtype, int fmt, int dim, bool blk, cudaStream_t stream) {

@@ -1,10 +1,12 @@
 // cache_ops.cu -- rotary positions, and the packed key/value cache's writing and reading back.
 //
 // All three move each value once and compute little: their floor is HBM bandwidth for prompts and
-// the launch for single tokens. The reference has no attention; these feed cache_attn.cu. Measured
-// (device time): rotary over 8192 x 64 heads of 128 bf16 values 46 us = 5.9 TB/s, one token 1.8 us; 32768
-// tokens of 8 + 8 heads and 32 query heads turned and written as fp8 and read back, 209 us of a floor of
-// 146; 1999 tokens of 64 query heads with FP4 blocks 26 us of 13; 16 tokens 5.2 us.
+// the launch for single tokens. Rotary is at 90 % of it; writing and reading back wait for chains of
+// loads (a token's slot, position, angles and rows, then its codes) that the warps of an SM do not cover.
+// The reference has no attention; these feed cache_attn.cu. Measured (device time): rotary over 8192 x 64
+// heads of 128 bf16 values 46 us = 5.9 TB/s, one token 2.1 us; 32768 tokens of 8 + 8 heads and 32 query
+// heads turned and written as fp8 and read back, 209 us of a floor of 146; 1999 tokens of 64 query heads
+// with FP4 blocks 26 us of 13; 16 tokens 5.2 us.
 #include "cache.cuh"
 #include "kernels.h"
 #include "sm100.cuh"
@@ -132,13 +134,13 @@ __device__ __forceinline__ bool in_table(const RotaryArgs &a, int64_t p) {
 template <typename T, bool INTER, int HPT>
 __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
   pdl_enter();
-  constexpr int VEC = 16 / sizeof(T), NA = INTER ? VEC : VEC;  // angles of a unit
+  constexpr int VEC = 16 / sizeof(T), NA = VEC;  // angles of a unit
   const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
   if (idx >= a.total) return;
   const uint32_t hi = idx / a.units, u = idx - hi * a.units;
   const uint32_t tok = hi / a.hgroups, hg = hi - tok * a.hgroups;
   const uint32_t b = a.batch == 1 ? 0 : tok / a.tokens, t = tok - b * a.tokens;
-  const int half = a.rot / 2, turned = (INTER ? a.rot / 2 : half) / VEC;
+  const int half = a.rot / 2, turned = half / VEC;
   const bool turn = (int)u < turned;
   const int rest = (a.dim - a.rot) / 2;
   const int d0 = INTER ? (int)u * 2 * VEC : turn ? (int)u * VEC : a.rot + ((int)u - turned) * VEC;
