@@ -92,3 +92,29 @@ def test_zero_values_beside_small_and_large_ones(fmt, blocked, queries, size):
     tol = ref.tolerance(r, spread, torch.bfloat16, 128, blocked) - 2.0 ** -24
     assert ((out[0].cpu().double() - r).abs() <= tol).all()
     assert ((lse[0].cpu().double() - rl).abs() <= 2.0 ** -9).all() and math.isfinite(lse.sum().item())
+
+
+@pytest.mark.parametrize("fmt,blocked", [("int8", False), ("fp4_e2m1", True)])
+@pytest.mark.parametrize("rows", ["few", "many"])
+@pytest.mark.parametrize("zero", [False, True])
+def test_two_million_keys(fmt, blocked, rows, zero):
+    """One page named 2^15 times: the result of the page alone, its logarithm larger by that of 2^15."""
+    page, times = 64, 1 << 15
+    cache = tg.PackedCache.empty(2, page, 1, 128, fmt, block_size=32 if blocked else 128)
+    k, v = randn((page, 1, 128), 310).cuda(), randn((page, 1, 128), 311).cuda() * (0.0 if zero else 1.0)
+    tg.cache_write(cache, k, v, torch.arange(page, 2 * page).cuda())
+    batch = 2 if rows == "few" else 40
+    q = randn((batch, 4, 128), 312, torch.bfloat16).cuda()
+    one = torch.ones((batch, times), dtype=torch.int32, device="cuda")
+    none = torch.zeros(batch, dtype=torch.int32, device="cuda")
+
+    def attend(n):
+        if rows == "few":
+            return tg.cache_attention(q, cache, one, none + n, return_lse=True)
+        return tg.cache_attention(q, cache, one, none, prefix=one[0], prefix_length=n, return_lse=True)
+
+    (a, la), (b, lb) = attend(page), attend(page * times)
+    # both round once to bfloat16 (2^-8); sums of up to 2^14 terms a lane in fp32 (2^-24 each)
+    assert ((a.double() - b.double()).abs() <= 2.0 ** -7 * a.double().abs() + 2.0 ** -9 * a.double().abs().max()).all()
+    assert ((lb.double() - la.double() - math.log(times)).abs() <= 2.0 ** -9).all()
+    assert not zero or (b == 0).all()
