@@ -359,6 +359,114 @@ int64_t b200_cache_attention_scratch(int64_t batch, int64_t queries, int32_t hea
                                      int64_t prefix_length);
 int32_t b200_cache_attention(const b200_cache_desc *cache, const b200_attention_args *args, void *stream);
 
+/* ---- 8-bit activations between packed projections ---------------------------------------
+ * No counterpart in the reference, whose packed path ends at one matmul. Activations are held as
+ * E4M3 codes with a power of two (E8M0 byte) for every 32 values of a row, which is how the tensor
+ * cores read them beside FP4 / FP6 weights:
+ *   codes [rows, cols], scales [rows, cols / 32], both contiguous; cols a multiple of 32.
+ * A block's scale is the smallest power of two not below max|x| * (1 / 448), held within
+ * [2^-100, 2^100]; x is stored as the E4M3 value nearest to x / scale, ties to even, held at 448. A
+ * NaN makes its block's scale NaN (byte 255) and its codes zero. */
+
+/* Rows of x, with `residual` added when given: total = x + residual rounded to `total_dtype`, the
+ * residual's own type (total may be residual itself); t is total, or x without a residual. With
+ * `normalize`, t * rsqrt(mean(t^2) + eps) * weight, else t. All in fp32, rounded once to y_dtype (F16,
+ * BF16, F32), or quantised when y_dtype is B200_DT_F8E4M3 (y codes, y_scales scales). Strides in
+ * elements between rows, unit along them. */
+typedef struct b200_norm_args {
+  const void *x;
+  const void *residual; /* or NULL                                                        */
+  void *total;          /* with residual                                                  */
+  const void *weight;   /* [cols] F16, BF16 or F32, or NULL: ones                         */
+  void *y;              /* contiguous                                                     */
+  void *y_scales;       /* 8-bit y only                                                   */
+  int64_t rows, cols;
+  int64_t x_stride, residual_stride, total_stride;
+  int32_t x_dtype, total_dtype, weight_dtype, y_dtype;
+  int32_t normalize;
+  float eps;
+} b200_norm_args;
+int32_t b200_rms_norm(const b200_norm_args *args, void *stream);
+
+/* The values of block-scaled rows as `dtype` (F16, BF16, F32): code times scale, rounded once. */
+int32_t b200_scaled_values(const void *codes, const void *scales, int64_t rows, int64_t cols, void *out, int32_t dtype,
+                           void *stream);
+
+/* Products of block-scaled rows with packed weights (FP4 or FP6 codes, E8M0 scales in blocks of 32,
+ * cols a multiple of 32), fp32 sums, and what follows them:
+ *   v = x W^T + bias;  gated: W's rows are [gate; up] and v = act(v_gate) * v_up, else v = act(v);
+ *   v + residual, rounded to y_dtype (F16, BF16, F32) or quantised (F8E4M3; the columns of y must then
+ *   be a multiple of 32).
+ * With `experts` > 0 the weights are `experts` matrices of w->rows / experts rows each, and rows of x
+ * go through them by a plan (b200_expert_plan): pair p = token * fan + j, in the order `order`, those
+ * of expert e at offsets[e] .. offsets[e + 1]. A pair reads row p / fan of x, or row p when
+ * `per_pair`, and gives row p of y; rows of pairs that no expert has are zeros. bias is [experts,
+ * rows] then, residual must be NULL. cols a multiple of 128 and weights on a 32-byte boundary run on
+ * the tensor cores, other calls on a general kernel, for which `scratch` (b200_scaled_linear_scratch
+ * bytes, 0 for the former) is needed. Workspace: 38 MiB per (device, stream) or capture. */
+#define B200_ACT_NONE 0
+#define B200_ACT_RELU 1
+#define B200_ACT_SILU 2
+#define B200_ACT_GELU 3      /* v * (1 + erf(v / sqrt 2)) / 2                              */
+#define B200_ACT_GELU_TANH 4 /* its form with a hyperbolic tangent                        */
+typedef struct b200_scaled_args {
+  const void *x, *x_scales;
+  int64_t rows;           /* of y: tokens, or tokens * fan pairs                           */
+  const void *bias;       /* F16, BF16 or F32, or NULL                                     */
+  const void *residual;   /* [rows, columns of y], or NULL                                 */
+  int64_t residual_stride;
+  void *y;                /* contiguous                                                    */
+  void *y_scales;
+  void *scratch;
+  const int32_t *offsets; /* [experts + 1]                                                 */
+  const int32_t *order;   /* [rows]                                                        */
+  int64_t experts;        /* 0: one matrix for all rows                                    */
+  int32_t fan, per_pair;
+  int32_t bias_dtype, residual_dtype, y_dtype;
+  int32_t activation, gated;
+  int32_t general;        /* nonzero: the general kernel whatever the operands             */
+} b200_scaled_args;
+int64_t b200_scaled_linear_scratch(const b200_packed_desc *w, const b200_scaled_args *args);
+int32_t b200_scaled_linear(const b200_packed_desc *w, const b200_scaled_args *args, void *stream);
+
+/* Routing of rows (tokens) to experts by their logits (F16, BF16 or F32, at most 1024 of a row).
+ * scores: softmax (0) or sigmoid (1) of the logits. choice: scores + bias when given, the scores when
+ * group_best is 2, else the logits; in 64 bits wherever scores decide. Groups of experts / groups
+ * consecutive experts (at most 32 groups) are ranked by their best choice or the sum of their best two (group_best);
+ * of the experts of the top_groups best groups the k best are chosen (at most 32), best first; ties go to the
+ * lowest index. A logit of NaN or -inf, or a bias of these, keeps an expert from being chosen; larger
+ * ones count as the largest finite value. weights: the chosen experts' scores without bias, divided by their sum
+ * with `renormalize`, times `scale`. Where fewer than k can be chosen, and in rows from *live on when
+ * given, indices are -1 and weights 0. */
+typedef struct b200_route_args {
+  const void *logits;
+  const float *bias;    /* [experts] or NULL                                              */
+  const int32_t *live;  /* or NULL                                                        */
+  int32_t *indices;     /* [rows, k]                                                      */
+  float *weights;       /* [rows, k]                                                      */
+  int32_t *offsets;     /* [experts + 1], as b200_expert_plan                             */
+  int32_t *order;       /* [rows * k]                                                     */
+  void *scratch;        /* b200_expert_plan_scratch(rows * k, experts) bytes              */
+  int64_t rows, stride;
+  int32_t dtype, experts, k, sigmoid, groups, top_groups, group_best, renormalize;
+  float scale;
+} b200_route_args;
+int32_t b200_route_experts(const b200_route_args *args, void *stream);
+
+/* The pairs 0 .. pairs - 1 in the order of the experts that `indices` names for them, equal ones in
+ * their own order: offsets[e] .. offsets[e + 1] are the places of expert first + e (e < experts <=
+ * 1024); pairs of other experts (indices below `first`, -1 among them, or beyond) come behind. */
+int64_t b200_expert_plan_scratch(int64_t pairs, int32_t experts);
+int32_t b200_expert_plan(const int32_t *indices, int64_t pairs, int32_t first, int32_t experts, int32_t *offsets,
+                         int32_t *order, void *scratch, void *stream);
+
+/* out[t] = residual[t] + sum over j of weights[t, j] * y[t * fan + j], over the pairs whose index lies
+ * in first .. first + experts - 1, in fp32 and the order of j, rounded once to out_dtype (F16, BF16,
+ * F32). y: F16, BF16 or F32 [tokens * fan, cols], out: [tokens, cols], contiguous. */
+int32_t b200_expert_combine(const void *y, int32_t y_dtype, const float *weights, const int32_t *indices, int32_t first,
+                            int32_t experts, int32_t fan, int64_t tokens, int64_t cols, const void *residual,
+                            int32_t residual_dtype, int64_t residual_stride, void *out, int32_t out_dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

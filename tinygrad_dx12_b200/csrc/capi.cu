@@ -308,9 +308,13 @@ int32_t b200_device_status(int32_t device, uint32_t *flags, int32_t clear) {
   if (int32_t rc = cache_attn_device_error(&ca, clear != 0)) return rc;
   unsigned int cm = 0;
   if (int32_t rc = cache_attn_mma_device_error(&cm, clear != 0)) return rc;
-  *flags = v | u | w | z | dd | mxe | co | ca | cm;
-  if (clear != 0 && (*flags & 1u) != 0)  // a kernel gave up mid-way: its split-tile tickets may be half counted
+  unsigned int sm = 0;
+  if (int32_t rc = scaled_mma_device_error(&sm, clear != 0)) return rc;
+  *flags = v | u | w | z | dd | mxe | co | ca | cm | sm;
+  if (clear != 0 && (*flags & 1u) != 0) {  // a kernel gave up mid-way: its split-tile tickets may be half counted
     if (int32_t rc = mx_reset_tickets()) return rc;
+    if (int32_t rc = scaled_mma_reset_tickets()) return rc;
+  }
   return B200_OK;
 }
 

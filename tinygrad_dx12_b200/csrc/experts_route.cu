@@ -1,0 +1,535 @@
+// experts_route.cu -- which experts a row goes to, the order in which experts read their rows, and the
+// sum of what they give back.
+//
+// Routing: a warp a row, expert e in lane e % 32. Choices become whole numbers that order like them (0:
+// cannot be chosen), 32 bits where the logits decide and 64 where scores do, so a round of the k best is
+// a warp-wide maximum, and a tie a warp-wide minimum of the index: no sort, and the same choice whatever
+// else runs. Scores that decide are computed in 64 bits: two experts whose scores differ by less than
+// fp32 resolves are ordered as their definition has it.
+// Plan: a stable counting sort of the pairs by expert. CTAs count their chunk's pairs, one warp an expert
+// sums the counts over the chunks, and each CTA places its chunk: warps own consecutive pieces of it, so a
+// pair's place is what lies before it in earlier chunks, earlier warps, earlier rounds and lower lanes.
+// No atomics on places: the order is the same every time. Few pairs take one launch of one CTA.
+// Bound by the launches up to some ten thousand pairs, then by HBM (logits).
+#include "kernels.h"
+#include "common.cuh"
+
+namespace b200 {
+namespace route {
+
+constexpr int MAX_EXPERTS = 1024, MAX_K = 32, MAX_GROUPS = 32;
+constexpr int PLAN_WARPS = 16, PLAN_THREADS = 32 * PLAN_WARPS;
+
+struct RouteParams {
+  b200_route_args a;
+};
+
+// Whole numbers that order like the values; 0 stands for what cannot be chosen (and orders below all).
+__device__ __forceinline__ uint32_t order32(float v) {
+  const uint32_t u = __float_as_uint(v);
+  return u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
+}
+__device__ __forceinline__ uint64_t order64(double v) {
+  const uint64_t u = (uint64_t)__double_as_longlong(v);
+  return u ^ ((u >> 63) ? ~0ull : 1ull << 63);
+}
+__device__ __forceinline__ double value64(uint64_t k) {
+  return __longlong_as_double((long long)(k ^ ((k >> 63) ? 1ull << 63 : ~0ull)));
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ uint32_t warp_max(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
+__device__ __forceinline__ uint64_t warp_max(uint64_t v) {
+  const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32));
+  const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
+  return (uint64_t)hi << 32 | lo;
+}
+
+// N experts a lane. Key: uint32_t (logits decide) or uint64_t (scores decide).
+template <int N, typename Key>
+__global__ void __launch_bounds__(128) route_kernel(const __grid_constant__ RouteParams rp) {
+  const b200_route_args &a = rp.a;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= a.rows) return;
+  int32_t *indices = a.indices + row * a.k;
+  float *weights = a.weights + row * a.k;
+  if (a.live != nullptr && row >= *a.live) {
+    if (lane < a.k) indices[lane] = -1, weights[lane] = 0.f;
+    return;
+  }
+  constexpr bool WIDE = sizeof(Key) == 8;
+  // logits; -inf for what cannot be chosen by them
+  float x[N];
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int e = lane + 32 * i;
+    float v = -INFINITY;
+    if (e < a.experts) {
+      v = load_as_f32(a.logits, row * a.stride + e, a.dtype);
+      v = v != v ? -INFINITY : fminf(v, 3.402823466e38f);
+    }
+    x[i] = v;
+    top = fmaxf(top, v);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  // the softmax's denominator, over all experts with a logit
+  float total = 0.f;
+  if (!a.sigmoid) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) total += x[i] == -INFINITY ? 0.f : expf(x[i] - top);
+    total = warp_sum(total);
+  }
+  Key key[N];
+  if constexpr (WIDE) {
+    double all = 1.0;
+    if (!a.sigmoid) {
+      all = 0.0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) all += x[i] == -INFINITY ? 0.0 : exp((double)x[i] - (double)top);
+      all = warp_sum(all);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      key[i] = 0;
+      if (x[i] == -INFINITY) continue;
+      double c = a.sigmoid ? 1.0 / (1.0 + exp(-(double)x[i])) : exp((double)x[i] - (double)top) / all;
+      if (a.bias != nullptr) {
+        const float b = a.bias[lane + 32 * i];
+        if (b != b || b == -INFINITY) continue;
+        c += (double)fminf(b, 3.402823466e38f);
+      }
+      key[i] = order64(c == 0.0 ? 0.0 : c);  // one zero
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) key[i] = x[i] == -INFINITY ? 0u : order32(x[i] == 0.f ? 0.f : x[i]);
+  }
+  if (a.groups > 1) {
+    const int size = a.experts / a.groups;
+    Key mine = 0;  // lane g: the rank of group g
+    for (int g = 0; g < a.groups; ++g) {
+      Key best = 0;
+      int at = -1;  // this lane's own best
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int e = lane + 32 * i;
+        if (e >= g * size && e < (g + 1) * size && key[i] > best) best = key[i], at = i;
+      }
+      Key first = warp_max(best);
+      if constexpr (WIDE) {
+        if (a.group_best == 2 && first != 0) {
+          const uint32_t has = __ballot_sync(0xffffffffu, best == first);
+          Key second = best;
+          if (lane == __ffs(has) - 1) {  // one lane gives up its best for its next
+            second = 0;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+              const int e = lane + 32 * i;
+              if (i != at && e >= g * size && e < (g + 1) * size && key[i] > second) second = key[i];
+            }
+          }
+          second = warp_max(second);
+          if (second != 0) {
+            const double sum = value64(first) + value64(second);
+            first = order64(sum == 0.0 ? 0.0 : sum);
+          }
+        }
+      }
+      if (lane == g) mine = first;
+    }
+    uint32_t kept = 0;
+    for (int r = 0; r < a.top_groups; ++r) {
+      const Key best = warp_max(mine);
+      if (best == 0) break;
+      const int g = __ffs(__ballot_sync(0xffffffffu, mine == best)) - 1;
+      kept |= 1u << g;
+      if (lane == g) mine = 0;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int e = lane + 32 * i;
+      if (e < a.experts && !(kept >> (e / size) & 1u)) key[i] = 0;
+    }
+  }
+  // the k best, round by round: lane j keeps the j-th
+  int chosen = -1;
+  float logit = -INFINITY;
+  for (int j = 0; j < a.k; ++j) {
+    Key best = 0;
+    float value = 0.f;
+    uint32_t index = 0xFFFFFFFFu;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (key[i] > best) best = key[i], value = x[i], index = lane + 32 * i;  // the lower index on a tie
+    const Key first = warp_max(best);
+    if (first == 0) break;
+    const uint32_t at = __reduce_min_sync(0xffffffffu, best == first ? index : 0xFFFFFFFFu);
+    value = __shfl_sync(0xffffffffu, value, at & 31);
+    if (lane == j) chosen = (int)at, logit = value;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if ((int)at == lane + 32 * i) key[i] = 0;
+  }
+  float w = 0.f;
+  if (a.renormalize) {
+    // scores over their sum, both divided by the largest softmax numerator of the chosen (exp(min(0, the
+    // largest logit)) for sigmoids): neither vanishes, however small the scores are
+    float most = logit;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (chosen >= 0) {
+      if (!a.sigmoid) w = expf(logit - most);
+      else if (most >= 0.f) w = 1.f / (1.f + expf(-logit));
+      else w = expf(logit - most) / (1.f + expf(logit));
+    }
+    const float sum = warp_sum(w);
+    w = chosen >= 0 ? w / sum : 0.f;
+  } else if (chosen >= 0) {
+    w = a.sigmoid ? 1.f / (1.f + expf(-logit)) : expf(logit - top) / total;
+  }
+  if (lane < a.k) indices[lane] = chosen, weights[lane] = w * a.scale;
+}
+
+// ---- the plan -------------------------------------------------------------------------------------
+struct PlanParams {
+  const int32_t *indices;
+  int64_t pairs;
+  int first, experts;
+  int32_t *offsets, *order;
+  int32_t *counts;  // [experts + 1][chunks]: pairs of a chunk, then those of earlier chunks
+  int32_t *totals;  // [experts + 1]
+  int64_t chunk;    // pairs a chunk, a multiple of PLAN_THREADS
+  int chunks;
+};
+
+__device__ __forceinline__ int bin_of(const PlanParams &p, int64_t i) {
+  const uint32_t e = (uint32_t)p.indices[i] - (uint32_t)p.first;  // below `first`: wraps far beyond
+  return p.indices[i] >= p.first && e < (uint32_t)p.experts ? (int)e : p.experts;
+}
+
+// Pairs [begin, end) of each warp of CTA `c`: consecutive pieces of whole rounds of 32.
+__device__ __forceinline__ void piece(const PlanParams &p, int c, int warp, int64_t &begin, int64_t &end) {
+  const int64_t per = p.chunk / PLAN_WARPS;
+  begin = c * p.chunk + warp * per;
+  end = begin + per < p.pairs ? begin + per : p.pairs;
+}
+
+// hist[warp][bin] = pairs of each bin in the warp's piece.
+__device__ __forceinline__ void count_pieces(const PlanParams &p, int c, int32_t *hist) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, bins = p.experts + 1;
+  for (int i = threadIdx.x; i < PLAN_WARPS * bins; i += PLAN_THREADS) hist[i] = 0;
+  __syncthreads();
+  int64_t begin, end;
+  piece(p, c, warp, begin, end);
+  for (int64_t i = begin + lane; i < end; i += 32) atomicAdd(&hist[warp * bins + bin_of(p, i)], 1);
+  __syncthreads();
+}
+
+// base[bin] = where the bin begins, from the totals in `base`: an exclusive sum in place (bins <= 1056).
+__device__ __forceinline__ void exclusive(int32_t *base, int bins) {
+  __shared__ int32_t part[PLAN_WARPS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int carry = 0;
+  for (int first = 0; first < bins; first += PLAN_THREADS) {
+    const int i = first + threadIdx.x;
+    const int own = i < bins ? base[i] : 0;
+    int v = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    if (lane == 31) part[warp] = v;
+    __syncthreads();
+    int before = carry, all = 0;
+    for (int w = 0; w < PLAN_WARPS; ++w) {
+      if (w < warp) before += part[w];
+      all += part[w];
+    }
+    if (i < bins) base[i] = before + v - own;
+    carry += all;
+    __syncthreads();
+  }
+}
+
+// Places the warps' pieces: base[bin] is where the chunk's pairs of a bin begin, hist the pieces' counts.
+__device__ __forceinline__ void place_pieces(const PlanParams &p, int c, int32_t *hist, const int32_t *base) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, bins = p.experts + 1;
+  for (int b = threadIdx.x; b < bins; b += PLAN_THREADS) {
+    int at = base[b];
+    for (int w = 0; w < PLAN_WARPS; ++w) {
+      const int n = hist[w * bins + b];
+      hist[w * bins + b] = at;
+      at += n;
+    }
+  }
+  __syncthreads();
+  int64_t begin, end;
+  piece(p, c, warp, begin, end);
+  int32_t *next = hist + warp * bins;
+  for (int64_t i = begin; i < end; i += 32) {
+    const bool live = i + lane < end;
+    const int b = live ? bin_of(p, i + lane) : -1;
+    const uint32_t same = __match_any_sync(0xffffffffu, b);
+    const int at = live ? next[b] : 0;
+    __syncwarp();
+    if (live) {
+      p.order[at + __popc(same & ((1u << lane) - 1))] = (int32_t)(i + lane);
+      if ((same >> lane) == 1u) next[b] = at + __popc(same);  // the last of them
+    }
+    __syncwarp();
+  }
+}
+
+__global__ void __launch_bounds__(PLAN_THREADS) plan_whole_kernel(const PlanParams p) {
+  extern __shared__ int32_t smem[];
+  const int bins = p.experts + 1;
+  int32_t *base = smem, *hist = smem + bins;
+  count_pieces(p, 0, hist);
+  for (int b = threadIdx.x; b < bins; b += PLAN_THREADS) {
+    int n = 0;
+    for (int w = 0; w < PLAN_WARPS; ++w) n += hist[w * bins + b];
+    base[b] = n;
+  }
+  __syncthreads();
+  exclusive(base, bins);
+  for (int b = threadIdx.x; b < bins; b += PLAN_THREADS) p.offsets[b] = base[b];
+  place_pieces(p, 0, hist, base);
+}
+
+__global__ void __launch_bounds__(PLAN_THREADS) plan_count_kernel(const PlanParams p) {
+  extern __shared__ int32_t smem[];
+  const int bins = p.experts + 1;
+  count_pieces(p, blockIdx.x, smem);
+  for (int b = threadIdx.x; b < bins; b += PLAN_THREADS) {
+    int n = 0;
+    for (int w = 0; w < PLAN_WARPS; ++w) n += smem[w * bins + b];
+    p.counts[(int64_t)b * p.chunks + blockIdx.x] = n;
+  }
+}
+
+// A warp a bin: counts over the chunks become those of earlier chunks.
+__global__ void __launch_bounds__(128) plan_sum_kernel(const PlanParams p) {
+  const int b = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (b > p.experts) return;
+  int32_t *row = p.counts + (int64_t)b * p.chunks;
+  int carry = 0;
+  for (int first = 0; first < p.chunks; first += 32) {
+    const int c = first + lane;
+    const int own = c < p.chunks ? row[c] : 0;
+    int v = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    if (c < p.chunks) row[c] = carry + v - own;
+    carry += __shfl_sync(0xffffffffu, v, 31);
+  }
+  if (lane == 0) p.totals[b] = carry;
+}
+
+__global__ void __launch_bounds__(PLAN_THREADS) plan_place_kernel(const PlanParams p) {
+  extern __shared__ int32_t smem[];
+  const int bins = p.experts + 1;
+  int32_t *base = smem, *hist = smem + bins;
+  for (int b = threadIdx.x; b < bins; b += PLAN_THREADS) base[b] = p.totals[b];
+  __syncthreads();
+  exclusive(base, bins);
+  if (blockIdx.x == 0)
+    for (int b = threadIdx.x; b < bins; b += PLAN_THREADS) p.offsets[b] = base[b];
+  __syncthreads();
+  for (int b = threadIdx.x; b < bins; b += PLAN_THREADS) base[b] += p.counts[(int64_t)b * p.chunks + blockIdx.x];
+  __syncthreads();
+  count_pieces(p, blockIdx.x, hist);
+  place_pieces(p, blockIdx.x, hist, base);
+}
+
+// Up to this many pairs one CTA does it all.
+constexpr int64_t WHOLE = 8192;
+constexpr int MAX_CHUNKS = 256;
+
+static int64_t chunk_of(int64_t pairs) {
+  if (pairs <= WHOLE) return (pairs + PLAN_THREADS - 1) / PLAN_THREADS * PLAN_THREADS;
+  int64_t c = (pairs + MAX_CHUNKS - 1) / MAX_CHUNKS;
+  c = c < 2048 ? 2048 : c;
+  return (c + PLAN_THREADS - 1) / PLAN_THREADS * PLAN_THREADS;
+}
+
+static int32_t plan(const int32_t *indices, int64_t pairs, int first, int experts, int32_t *offsets, int32_t *order,
+                    void *scratch, cudaStream_t stream) {
+  PlanParams p{indices, pairs, first, experts, offsets, order, nullptr, nullptr, chunk_of(pairs), 1};
+  const int bins = experts + 1;
+  const size_t smem = (size_t)(PLAN_WARPS + 1) * bins * 4;  // at most 70 KB
+  if (pairs <= WHOLE) {
+    B200_CUDA_TRY((ensure_dynamic_smem<plan_whole_kernel>(72 * 1024)));
+    plan_whole_kernel<<<1, PLAN_THREADS, smem, stream>>>(p);
+  } else {
+    p.chunks = (int)((pairs + p.chunk - 1) / p.chunk);
+    p.counts = (int32_t *)scratch;
+    p.totals = p.counts + (int64_t)bins * p.chunks;
+    B200_CUDA_TRY((ensure_dynamic_smem<plan_count_kernel>(72 * 1024)));
+    B200_CUDA_TRY((ensure_dynamic_smem<plan_place_kernel>(72 * 1024)));
+    plan_count_kernel<<<p.chunks, PLAN_THREADS, smem, stream>>>(p);
+    B200_LAUNCH_CHECK();
+    plan_sum_kernel<<<(bins + 3) / 4, 128, 0, stream>>>(p);
+    B200_LAUNCH_CHECK();
+    plan_place_kernel<<<p.chunks, PLAN_THREADS, smem, stream>>>(p);
+  }
+  B200_LAUNCH_CHECK();
+  return B200_OK;
+}
+
+template <int N>
+static int32_t launch_route(const RouteParams &rp, bool wide, cudaStream_t stream) {
+  const unsigned ctas = (unsigned)((rp.a.rows + 3) / 4);
+  if (wide) route_kernel<N, uint64_t><<<ctas, 128, 0, stream>>>(rp);
+  else route_kernel<N, uint32_t><<<ctas, 128, 0, stream>>>(rp);
+  B200_LAUNCH_CHECK();
+  return B200_OK;
+}
+
+// ---- the weighted sum -------------------------------------------------------------------------------
+struct CombineParams {
+  const void *y;
+  const float *weights;
+  const int32_t *indices;
+  const void *residual;
+  void *out;
+  int64_t cols, rstride;
+  int first, experts, fan, ydt, rdt, odt;
+};
+
+// VEC neighbouring columns a thread.
+template <int VEC>
+__global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ CombineParams p) {
+  const int64_t t = blockIdx.y, c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * VEC;
+  if (c >= p.cols) return;
+  float sum[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) sum[i] = 0.f;
+  for (int j = 0; j < p.fan; ++j) {
+    const int64_t pair = t * p.fan + j;
+    const int32_t e = p.indices[pair];
+    if (e < p.first || e - p.first >= p.experts) continue;
+    const float w = p.weights[pair];
+    float v[VEC];
+    if constexpr (VEC == 4) {
+      if (p.ydt == B200_DT_F32) {
+        const float4 u = *reinterpret_cast<const float4 *>((const float *)p.y + pair * p.cols + c);
+        v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
+      } else {
+        const uint2 u = *reinterpret_cast<const uint2 *>((const uint16_t *)p.y + pair * p.cols + c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint16_t h = (uint16_t)((i & 2 ? u.y : u.x) >> (16 * (i & 1)));
+          v[i] = p.ydt == B200_DT_F16 ? __half2float(__ushort_as_half(h)) : __uint_as_float((uint32_t)h << 16);
+        }
+      }
+    } else {
+      v[0] = load_as_f32(p.y, pair * p.cols + c, p.ydt);
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) sum[i] = fmaf(w, v[i], sum[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    if (p.residual != nullptr) sum[i] += load_as_f32(p.residual, t * p.rstride + c + i, p.rdt);
+    store_f32(p.out, t * p.cols + c + i, p.odt, sum[i]);
+  }
+}
+
+static bool real(int dt) { return dt == B200_DT_F16 || dt == B200_DT_BF16 || dt == B200_DT_F32; }
+
+}  // namespace route
+}  // namespace b200
+
+using namespace b200;
+using namespace b200::route;
+
+extern "C" {
+
+int64_t b200_expert_plan_scratch(int64_t pairs, int32_t experts) {
+  if (pairs <= WHOLE || experts < 1 || experts > MAX_EXPERTS) return 0;
+  const int64_t chunks = (pairs + chunk_of(pairs) - 1) / chunk_of(pairs);
+  return (chunks + 1) * (experts + 1) * 4;
+}
+
+int32_t b200_expert_plan(const int32_t *indices, int64_t pairs, int32_t first, int32_t experts, int32_t *offsets,
+                         int32_t *order, void *scratch, void *stream) {
+  if (int32_t rc = b200_injected()) return rc;
+  if (pairs < 0 || first < 0 || experts < 1 || experts > MAX_EXPERTS || pairs > 0x7FFFFFFF)
+    return b200_set_error(B200_ERR_INVALID, "expert_plan: 1 to %d experts and fewer than 2^31 pairs", MAX_EXPERTS);
+  if (offsets == nullptr || (pairs > 0 && (indices == nullptr || order == nullptr)) || (pairs > WHOLE && scratch == nullptr))
+    return b200_set_error(B200_ERR_INVALID, "expert_plan: null pointer");
+  return plan(indices, pairs, first, experts, offsets, order, scratch, (cudaStream_t)stream);
+}
+
+int32_t b200_route_experts(const b200_route_args *a, void *stream) {
+  if (int32_t rc = b200_injected()) return rc;
+  if (a == nullptr) return b200_set_error(B200_ERR_INVALID, "route_experts: null arguments");
+  if (!real(a->dtype) || a->rows < 0 || a->experts < 1 || a->experts > MAX_EXPERTS || a->k < 1 || a->k > MAX_K || a->k > a->experts)
+    return b200_set_error(B200_ERR_INVALID, "route_experts: k of at most %d out of 1 to %d experts, float16, bfloat16 or float32",
+                          MAX_K, MAX_EXPERTS);
+  if (a->groups < 1 || a->groups > MAX_GROUPS || a->experts % a->groups != 0 || a->top_groups < 1 || a->top_groups > a->groups ||
+      (a->group_best != 1 && a->group_best != 2) || a->k > a->experts / a->groups * a->top_groups)
+    return b200_set_error(B200_ERR_INVALID, "route_experts: groups do not divide the experts, or leave fewer than k");
+  if (a->rows * a->k > 0x7FFFFFFF) return b200_set_error(B200_ERR_UNSUPPORTED, "route_experts: 2^31 pairs or more");
+  if (a->offsets == nullptr || (a->rows > 0 && (a->logits == nullptr || a->indices == nullptr || a->weights == nullptr || a->order == nullptr)))
+    return b200_set_error(B200_ERR_INVALID, "route_experts: null pointer");
+  if (a->rows * a->k > WHOLE && a->scratch == nullptr) return b200_set_error(B200_ERR_INVALID, "route_experts: null scratch");
+  cudaStream_t s = (cudaStream_t)stream;
+  const RouteParams rp{*a};
+  const bool wide = a->bias != nullptr || (a->groups > 1 && a->group_best == 2);
+  if (a->rows > 0) {
+    int32_t rc;
+    if (a->experts <= 64) rc = launch_route<2>(rp, wide, s);
+    else if (a->experts <= 128) rc = launch_route<4>(rp, wide, s);
+    else if (a->experts <= 256) rc = launch_route<8>(rp, wide, s);
+    else if (a->experts <= 512) rc = launch_route<16>(rp, wide, s);
+    else rc = launch_route<32>(rp, wide, s);
+    if (rc != B200_OK) return rc;
+  }
+  return plan(a->indices, a->rows * a->k, 0, a->experts, a->offsets, a->order, a->scratch, s);
+}
+
+int32_t b200_expert_combine(const void *y, int32_t y_dtype, const float *weights, const int32_t *indices, int32_t first,
+                            int32_t experts, int32_t fan, int64_t tokens, int64_t cols, const void *residual,
+                            int32_t residual_dtype, int64_t residual_stride, void *out, int32_t out_dtype, void *stream) {
+  if (int32_t rc = b200_injected()) return rc;
+  if (!real(y_dtype) || !real(out_dtype) || (residual != nullptr && !real(residual_dtype)) || fan < 1 || tokens < 0 || cols < 0)
+    return b200_set_error(B200_ERR_INVALID, "expert_combine: float16, bfloat16 or float32 rows");
+  if (tokens == 0 || cols == 0) return B200_OK;
+  if (y == nullptr || weights == nullptr || indices == nullptr || out == nullptr)
+    return b200_set_error(B200_ERR_INVALID, "expert_combine: null pointer");
+  cudaStream_t s = (cudaStream_t)stream;
+  CombineParams p{y, weights, indices, residual, out, cols, residual_stride, first, experts, fan, y_dtype, residual_dtype, out_dtype};
+  const bool vec = cols % 4 == 0 && (uintptr_t)y % 16 == 0;
+  for (int64_t t0 = 0; t0 < tokens; t0 += 65535) {  // the grid's second axis
+    const int64_t n = tokens - t0 < 65535 ? tokens - t0 : 65535;
+    CombineParams q = p;
+    q.y = (const uint8_t *)y + t0 * fan * cols * dt_size(y_dtype);
+    q.weights += t0 * fan;
+    q.indices += t0 * fan;
+    if (residual != nullptr) q.residual = (const uint8_t *)residual + t0 * residual_stride * dt_size(residual_dtype);
+    q.out = (uint8_t *)out + t0 * cols * dt_size(out_dtype);
+    if (vec) combine_kernel<4><<<dim3((unsigned)((cols + 1023) / 1024), (unsigned)n), 256, 0, s>>>(q);
+    else combine_kernel<1><<<dim3((unsigned)((cols + 255) / 256), (unsigned)n), 256, 0, s>>>(q);
+    B200_LAUNCH_CHECK();
+  }
+  return B200_OK;
+}
+
+}  // extern "C"

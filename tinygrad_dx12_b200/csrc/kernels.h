@@ -93,7 +93,7 @@ int32_t launch_wait_flag(const int32_t *flag, int32_t expect, int64_t max_spins,
 // zero at first. The same block for all calls of a kind on a stream, one of its own for those of a capture
 // (workspace.cu). The partial results lie on the block's own alignment: a ticket array before them (1280
 // bytes) cost a cut attention call of 257 keys 0.3 of 8.3 us.
-enum WorkspaceKind { WS_SPLIT_K, WS_MX, WS_ATTENTION, WS_ATTENTION_MMA };
+enum WorkspaceKind { WS_SPLIT_K, WS_MX, WS_ATTENTION, WS_ATTENTION_MMA, WS_SCALED };
 int32_t workspace_of(WorkspaceKind kind, size_t bytes, size_t tickets, cudaStream_t stream, uint8_t **base);
 int32_t workspace_zero(WorkspaceKind kind);  // the tickets again, of every block on the current device; synchronous
 
@@ -102,6 +102,13 @@ int32_t check_cache(const b200_cache_desc *c);
 int32_t cache_ops_device_error(unsigned int *v, bool clear);
 int32_t cache_attn_device_error(unsigned int *v, bool clear);
 int32_t cache_attn_mma_device_error(unsigned int *v, bool clear);
+
+// products of block-scaled activations with packed weights: on the tensor cores (scaled_mma.cu), in general (scaled_general.cu)
+bool scaled_mma_takes(const b200_packed_desc *w, const b200_scaled_args *a);
+int32_t launch_scaled_mma(const b200_packed_desc *w, const b200_scaled_args *a, cudaStream_t stream);
+int32_t launch_scaled_general(const b200_packed_desc *w, const b200_scaled_args *a, cudaStream_t stream);
+int32_t scaled_mma_device_error(unsigned int *v, bool clear);
+int32_t scaled_mma_reset_tickets();
 
 }  // namespace b200
 

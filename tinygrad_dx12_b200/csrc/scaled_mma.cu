@@ -1,0 +1,601 @@
+// scaled_mma.cu -- products of block-scaled 8-bit activations with packed FP4 / FP6 weights on the
+// 5th-generation tensor cores, dense or through experts.
+//
+//   v[t, n] = sum_k x[t, k] 2^(xs[t, k/32]) w[n, k] 2^(ws[n, k/32]),  then bias, activation, gate, residual
+//
+// tcgen05.mma kind::mxf8f6f4 reads both sides as they are stored: E4M3 codes of x, FP4 / FP6 codes of w
+// (TMA lays each 16 of them into a 16-byte slot), and a power of two for every 32 of either. No code is
+// decoded on the CUDA cores, for one token or for thousands; products are exact and sums fp32.
+//
+// A tile is R x 128 weight rows (the MMA's M; R = 2 when gated: 128 gate rows and the 128 up rows that go
+// with them, in two accumulators, so both are in one thread's hands) times up to NT tokens (its N, a
+// multiple of 16, so an expert with few tokens costs few columns). K advances 128 codes a stage.
+//   warps 0-3    epilogue: tcgen05.ld (lane = weight row, column = token), bias, activation, gate,
+//                residual; a warp's 32 rows are 32 neighbouring columns of y, a block of the 8-bit output,
+//                whose largest value is one warp-wide maximum
+//   warps 4-7    cp.async of x's codes (token rows found through the plan's order when there are experts)
+//                and of both sides' scale bytes, four of a row at a time, into the layout that
+//                tcgen05.cp takes; a stage is announced when its copies, some stages back, have landed
+//   warp 8       one thread: tcgen05.cp of the scales into tensor memory, four MMAs a stage and
+//                accumulator; commit frees the stage
+//   warps 9-11   one thread each: TMA of the weight codes (a thread issues a box in several hundred
+//                cycles, so three take turns)
+// Two accumulators of a tile's width, so that the epilogue of one tile runs under the products of the
+// next: 2 x 224 columns, and four rotating sets of scale columns beside them.
+//
+// Work split: units are (tile, K stage), laid end to end over experts, weight rows and token tiles; each of
+// G CTAs takes an equal run of them, whatever the matrix or the routing, so that every SM streams as many
+// bytes as the others. The units of experts are counted on the device from the plan's offsets: a recorded
+// launch fits every routing. A tile that a run's border cuts is finished by the last of its CTAs to arrive
+// (acquire-release ticket), which adds the fp32 parts in the order of the CTAs: the same bits every time.
+// No CTA waits for another. Every wait is bounded (sm100.cuh).
+#include <string.h>
+
+#include "kernels.h"
+#include "mx.cuh"
+#include "scaled_epilogue.cuh"
+
+namespace b200 {
+
+int32_t scaled_mma_device_error(unsigned int *v, bool clear) {
+  B200_CUDA_TRY(tu_device_error(v, clear));
+  return B200_OK;
+}
+int32_t scaled_mma_reset_tickets() { return workspace_zero(WS_SCALED); }
+
+namespace scaled {
+
+constexpr int TM = 128, KS = 128;            // weight rows of an MMA, codes of a stage
+constexpr int EPI_WARPS = 4, LOAD_WARP0 = 4, LOAD_WARPS = 4, MMA_WARP = 8, W_WARP0 = 9, W_WARPS = 3;
+constexpr int THREADS = 12 * 32;           // three warps a scheduler: up to 168 registers
+constexpr int ACC_COLS = 224;                // columns of an accumulator set: R * NT at most
+constexpr int SF_SETS = 4;
+constexpr int MAX_STAGES = 12;
+constexpr int MAX_EXPERTS = 1024;
+constexpr int MIN_UNITS = 4;                 // a CTA's run is no shorter: its start costs more than its work otherwise
+constexpr size_t TICKETS = 4096;             // one a CTA
+constexpr int SMEM_LIMIT = 227 * 1024;
+
+struct Params {
+  const uint8_t *x, *xs, *ws;
+  const int32_t *offsets, *order;
+  int64_t rows, n;        // rows of y, weight rows of one matrix
+  int64_t wrows;          // of all matrices
+  int64_t nblk;           // scale bytes of a row
+  int64_t cols;
+  int experts, fan, per_pair;
+  int nst;                // K stages
+  int wtiles;             // tiles of weight rows of one matrix
+  int nt;                 // tokens of a tile, at most
+  int grid, stages, lag;
+  uint32_t stage_bytes, b_off, sfa_off, sfb_off, sfb_bytes;
+  uint32_t tx;
+  uint32_t acc_width, sf_col, tmem_cols;
+  uint32_t idesc;
+  float *part;            // [grid][2][R][nt][128]
+  unsigned int *tickets;  // [grid]: of the tile that the CTA's run ends in
+};
+
+__device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+__device__ __forceinline__ void cp_async16(void *dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async4(void *dst, const void *src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Shared-memory descriptor of a scale atom (32 rows of 16 bytes, no swizzle), tcgen05.cp's source, and the
+// copy into 4 columns of every lane quarter.
+__device__ __forceinline__ uint64_t sf_desc(const void *atom) {
+  const uint64_t addr = smem_u32(atom);
+  return ((addr & 0x3FFFFull) >> 4) | ((uint64_t)(128 >> 4) << 16) | ((uint64_t)(128 >> 4) << 32) | (1ull << 46);
+}
+__device__ __forceinline__ void sf_copy(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+// What a tile is: expert, first weight row within its matrix, place of its first row, rows.
+struct Tile {
+  int e;
+  int64_t w0, first;
+  int rows, width;  // width: rows rounded up to the MMA's N
+};
+
+// Token tiles of `count` rows: as few as hold them, equally full.
+__device__ __forceinline__ int tiles_of(const Params &p, int count) { return (count + p.nt - 1) / p.nt; }
+
+__device__ __forceinline__ Tile tile_at(const Params &p, const int32_t *before, const int32_t *start, int64_t tile) {
+  int e = 0;
+  int64_t first = 0, count = p.rows, at = tile;
+  if (p.experts > 0) {
+    int lo = 0, hi = p.experts;  // before[lo] <= tile < before[hi]; empty experts have no tiles
+    const int32_t t = (int32_t)(tile / p.wtiles);
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (before[mid] <= t) lo = mid;
+      else hi = mid;
+    }
+    e = lo;
+    at = tile - (int64_t)before[e] * p.wtiles;
+    first = start[e];
+    count = start[e + 1] - start[e];
+  }
+  const int tt = tiles_of(p, (int)count);
+  const int per = ((int)(count + tt - 1) / tt + 15) / 16 * 16;
+  const int w = (int)(at / tt), t = (int)(at - (int64_t)w * tt);
+  Tile r;
+  r.e = e;
+  r.w0 = (int64_t)w * TM;
+  r.first = first + (int64_t)t * per;
+  r.rows = (int)(count - (int64_t)t * per < per ? count - (int64_t)t * per : per);
+  r.width = (r.rows + 15) / 16 * 16;
+  return r;
+}
+
+// The CTA's run of units and how it falls into tiles.
+struct Run {
+  int64_t units, u0, u1;
+  int ctas;  // that have one
+  __device__ __forceinline__ int64_t start(int64_t c) const { return c * units / ctas; }
+};
+
+template <typename T>
+__device__ __forceinline__ T to_out(float v) {
+  if constexpr (std::is_same<T, __half>::value) return __float2half_rn(v);
+  else if constexpr (std::is_same<T, __nv_bfloat16>::value) return __float2bfloat16_rn(v);
+  else return v;
+}
+struct E4M3 {};
+
+// One weight row's products with 32 tokens, column `c` of y (live: c is one): finished and stored. `at` is
+// the row of y of token j in lane j.
+template <int R, typename OUT>
+__device__ __forceinline__ void finish32(const Epilogue &ep, float (&v)[R][32], const float (&bias)[R], int64_t c, bool live,
+                                         int64_t at, int count) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) v[0][j] += bias[0];
+  if (ep.activation != B200_ACT_NONE) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[0][j] = activate(v[0][j], ep.activation);
+  }
+  if constexpr (R == 2) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[0][j] = __fmul_rn(v[0][j], v[1][j] + bias[1]);
+  }
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    if (j >= count) break;
+    const int64_t row = __shfl_sync(0xffffffffu, at, j);
+    float f = v[0][j];
+    if (ep.residual != nullptr && live) f += load_as_f32(ep.residual, row * ep.rstride + c, ep.rdt);
+    if constexpr (std::is_same<OUT, E4M3>::value) {  // y's columns are whole blocks: a warp's are all live or none
+      const uint32_t byte = rows8::scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(f) & 0x7FFFFFFFu));
+      if (live) {
+        ((uint8_t *)ep.y)[row * ep.cols + c] = (uint8_t)rows8::codes2(f, 0.f, rows8::inverse(byte), byte == 255u);
+        if (lane == 0) ep.ys[row * (ep.cols >> 5) + (c >> 5)] = (uint8_t)byte;
+      }
+    } else if (live) {
+      ((OUT *)ep.y)[row * ep.cols + c] = to_out<OUT>(f);
+    }
+  }
+}
+
+template <int R, typename OUT>
+__global__ void __launch_bounds__(THREADS, 1)
+    scaled_kernel(const __grid_constant__ CUtensorMap tmw, const __grid_constant__ Params p, const __grid_constant__ Epilogue ep) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *ring = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  const int S = p.stages;
+  uint64_t *fullw = reinterpret_cast<uint64_t *>(ring + (size_t)S * p.stage_bytes);
+  uint64_t *fullx = fullw + S;
+  uint64_t *empty = fullx + S;
+  uint64_t *accfull = empty + S;
+  uint64_t *accempty = accfull + 2;
+  uint64_t *drain = accempty + 2;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
+  volatile uint32_t *abort_flag = tmem_slot + 1;
+  volatile uint32_t *last_flag = tmem_slot + 2;
+  int32_t *start = reinterpret_cast<int32_t *>(tmem_slot + 4);  // [experts + 1] the plan's offsets
+  int32_t *before = start + p.experts + 1;                      // [experts + 1] token tiles of earlier experts
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&fullw[s], 1);
+      mbar_init(&fullx[s], LOAD_WARPS);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&accfull[b], 1);
+      mbar_init(&accempty[b], EPI_WARPS);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    prefetch_tmap(&tmw);
+  }
+  for (int e = threadIdx.x; e <= p.experts && p.experts > 0; e += THREADS) start[e] = p.offsets[e];
+  if (warp == MMA_WARP) tmem_alloc(tmem_slot, p.tmem_cols);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0 && p.experts > 0) {  // token tiles of the experts before each
+    int carry = 0;
+    for (int first = 0; first < p.experts; first += 32) {
+      const int e = first + lane;
+      const int own = e < p.experts ? tiles_of(p, start[e + 1] - start[e]) : 0;
+      int v = own;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
+      }
+      if (e < p.experts) before[e] = carry + v - own;
+      carry += __shfl_sync(0xffffffffu, v, 31);
+    }
+    if (lane == 0) before[p.experts] = carry;
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  Run run;
+  run.units = (p.experts > 0 ? (int64_t)before[p.experts] : (int64_t)tiles_of(p, (int)p.rows)) * p.wtiles * p.nst;
+  run.ctas = (int)(run.units / MIN_UNITS < p.grid ? (run.units / MIN_UNITS < 1 ? 1 : run.units / MIN_UNITS) : p.grid);
+  run.u0 = (int)blockIdx.x < run.ctas ? run.start(blockIdx.x) : 0;
+  run.u1 = (int)blockIdx.x < run.ctas ? run.start(blockIdx.x + 1) : 0;
+  const int64_t n = run.u1 - run.u0;
+
+  if (warp >= W_WARP0) {
+    // ---------------- TMA of weight codes: warp w takes the stages i = w (mod W_WARPS) ----------------
+    if (lane == 0) {
+      const int turn = warp - W_WARP0, turns = S < W_WARPS ? S : W_WARPS;
+      int64_t i = turn, tile = (run.u0 + turn) / p.nst;
+      int s = (int)((run.u0 + turn) % p.nst);
+      int slot = turn;
+      uint32_t round = 0;
+      int64_t row = 0, known = -1;
+      for (; i < n && turn < turns; i += turns) {
+        if (tile != known) {
+          const Tile t = tile_at(p, before, start, tile);
+          row = t.e * p.n + t.w0;
+          known = tile;
+        }
+        if (round > 0 && !mbar_wait(&empty[slot], (round - 1u) & 1u, abort_flag)) break;
+        uint8_t *st = ring + (size_t)slot * p.stage_bytes;
+        mbar_arrive_expect_tx(&fullw[slot], p.tx);
+        tma_load_2d(st, &tmw, s * KS, (int32_t)row, &fullw[slot]);
+        if constexpr (R == 2) tma_load_2d(st + TM * KS, &tmw, s * KS, (int32_t)(row + ep.cols), &fullw[slot]);
+        for (s += turns; s >= p.nst; s -= p.nst) ++tile;
+        if ((slot += turns) >= S) slot -= S, ++round;
+      }
+      if (*abort_flag) {  // this thread's copies in flight land before the CTA exits
+        for (int64_t q = turn; q < (i < n ? i : n); q += turns)
+          if (q + S >= i) mbar_drain(&fullw[q % S], (uint32_t)((q / S) & 1), 200000000ull);
+      }
+    }
+  } else if (warp >= LOAD_WARP0 && warp < LOAD_WARP0 + LOAD_WARPS) {
+    // ---------------- cp.async of x's codes and of all scale bytes ----------------
+    const int th = threadIdx.x - LOAD_WARP0 * 32;
+    const int chunk = th & 7, r0 = th >> 3;  // 16 bytes of a row's 128; rows r0, r0 + 16, ...
+    constexpr int PASSES = ACC_COLS / R / 16;
+    int64_t done = 0;  // stages announced
+    int slot = 0, dslot = 0;
+    uint32_t round = 0;
+    auto announce = [&]() {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&fullx[dslot]);
+      if (++dslot == S) dslot = 0;
+      ++done;
+    };
+    int64_t i = 0;
+    bool ok = true;
+    while (i < n && ok) {
+      const int64_t u = run.u0 + i;
+      const Tile t = tile_at(p, before, start, u / p.nst);
+      int s = (int)(u % p.nst);
+      const int64_t len = p.nst - s < n - i ? p.nst - s : n - i;
+      // rows of x: where this thread's begin
+      auto xrow = [&](int r) -> int64_t {
+        const int64_t at = t.first + r;
+        if (p.experts == 0) return at;
+        const int32_t pair = p.order[at];
+        return p.per_pair ? pair : pair / p.fan;
+      };
+      uint32_t rows[PASSES];
+#pragma unroll
+      for (int q = 0; q < PASSES; ++q) rows[q] = r0 + 16 * q < t.rows ? (uint32_t)xrow(r0 + 16 * q) : 0u;
+      const uint8_t *sx[2], *sw[R];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) sx[q] = th + 128 * q < t.rows ? p.xs + xrow(th + 128 * q) * p.nblk : nullptr;
+#pragma unroll
+      for (int q = 0; q < R; ++q) {
+        int64_t wrow = t.e * p.n + q * ep.cols + t.w0 + th;
+        if (wrow >= p.wrows) wrow = p.wrows - 1;  // rows behind the last: not stored
+        sw[q] = p.ws + wrow * p.nblk;
+      }
+      const uint32_t sf_at = (uint32_t)(th & 31) * 16 + (uint32_t)(th >> 5) * 4;
+      for (int64_t j = 0; j < len; ++j, ++i, ++s) {
+        if (round > 0) ok = __all_sync(0xffffffffu, mbar_wait(&empty[slot], (round - 1u) & 1u, abort_flag));
+        if (!ok) break;
+        uint8_t *st = ring + (size_t)slot * p.stage_bytes;
+        const int64_t k = (int64_t)s * KS + chunk * 16;
+#pragma unroll
+        for (int q = 0; q < PASSES; ++q) {
+          const int r = r0 + 16 * q;
+          if (r < t.rows) cp_async16(st + p.b_off + r * 128 + ((chunk ^ (r & 7)) << 4), p.x + (int64_t)rows[q] * p.cols + k);
+        }
+#pragma unroll
+        for (int q = 0; q < R; ++q) cp_async4(st + p.sfa_off + q * 512 + sf_at, sw[q] + 4 * s);
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+          if (sx[q] != nullptr) cp_async4(st + p.sfb_off + q * 512 + sf_at, sx[q] + 4 * s);
+        cp_commit();
+        if (++slot == S) slot = 0, ++round;
+        if (i + 1 - done > p.lag) {  // the stage `lag` back has landed
+          if (p.lag == 4) cp_wait<4>();
+          else cp_wait<2>();
+          announce();
+        }
+      }
+    }
+    cp_wait<0>();
+    while (ok && done < n) announce();
+  } else if (warp == MMA_WARP) {
+    // ---------------- MMA issuer ----------------
+    if (lane == 0) {
+      int slot = 0, set = 0, seg = -1;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int64_t i = 0; i < n && ok;) {
+        const int64_t u = run.u0 + i;
+        const Tile t = tile_at(p, before, start, u / p.nst);
+        const int s0 = (int)(u % p.nst);
+        const int64_t len = p.nst - s0 < n - i ? p.nst - s0 : n - i;
+        i += len;
+        ++seg;
+        if (seg >= 2 && !mbar_wait(&accempty[seg & 1], (uint32_t)((seg / 2 - 1) & 1), abort_flag)) break;
+        tc_fence_after();
+        const uint32_t acc = tmem + (uint32_t)(seg & 1) * R * p.acc_width;
+        const uint32_t idesc = p.idesc | ((uint32_t)(t.width >> 3) << 17);
+        for (int64_t j = 0; j < len; ++j) {
+          ok = mbar_wait(&fullw[slot], phase, abort_flag) && mbar_wait(&fullx[slot], phase, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          const uint8_t *st = ring + (size_t)slot * p.stage_bytes;
+          const uint32_t sf = tmem + p.sf_col + 12u * (uint32_t)set;
+          const uint32_t sfb = sf + 4u * R;
+#pragma unroll
+          for (int q = 0; q < R; ++q) sf_copy(sf + 4u * q, sf_desc(st + p.sfa_off + q * 512));
+          sf_copy(sfb, sf_desc(st + p.sfb_off));
+          if (R == 1 && t.width > 128) sf_copy(sfb + 4u, sf_desc(st + p.sfb_off + 512));
+          const uint64_t bd = sw128_kmajor_desc(st + p.b_off);
+#pragma unroll
+          for (int q = 0; q < R; ++q) {
+            const uint64_t ad = sw128_kmajor_desc(st + q * TM * KS);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)  // K = 32 each: 32 bytes further along the rows, scale byte k
+              mx::mma_mx(acc + (uint32_t)q * p.acc_width, ad + (uint64_t)(2 * k), bd + (uint64_t)(2 * k),
+                         idesc | ((uint32_t)k << 4) | ((uint32_t)k << 29), (j | k) != 0 ? 1u : 0u,
+                         (sf + 4u * q) | ((uint32_t)k << 30), sfb | ((uint32_t)k << 30));
+          }
+          mma_commit(&empty[slot]);
+          if (++slot == S) slot = 0, phase ^= 1u;
+          if (++set == SF_SETS) set = 0;
+        }
+        if (ok) mma_commit(&accfull[seg & 1]);
+      }
+      // every MMA issued has completed before the CTA frees its tensor memory
+      mma_commit(drain);
+      mbar_drain(drain, 0, 200000000ull);
+    }
+  } else if (warp < EPI_WARPS) {
+    // ---------------- epilogue: weight row = tensor-memory lane, token = column ----------------
+    const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
+    bool ok = true;  // this warp's waits; after one that ran out it still meets the others
+    int seg = 0;
+    for (int64_t i = 0; i < n; ++seg) {
+      const int64_t u = run.u0 + i, tile = u / p.nst;
+      const int s0 = (int)(u % p.nst);
+      const int64_t len = p.nst - s0 < n - i ? p.nst - s0 : n - i;
+      const bool whole = s0 == 0 && len == p.nst;
+      const Tile t = tile_at(p, before, start, tile);
+      const int64_t c = t.w0 + warp * 32 + lane;  // column of y
+      const bool live = c < ep.cols;
+      float bias[R];
+#pragma unroll
+      for (int q = 0; q < R; ++q)
+        bias[q] = ep.bias != nullptr && live ? load_as_f32(ep.bias, t.e * p.n + q * ep.cols + c, ep.bdt) : 0.f;
+      ok = __all_sync(0xffffffffu, ok && mbar_wait(&accfull[seg & 1], (uint32_t)((seg / 2) & 1), abort_flag));
+      tc_fence_after();
+      const uint32_t acc = tmem + lane_base + (uint32_t)(seg & 1) * R * p.acc_width;
+      // partial sums: of the CTA's first tile in place 0, of its last in place 1
+      const size_t place = (size_t)R * p.nt * TM;
+      float *mine = p.part + ((size_t)blockIdx.x * 2 + (i == 0 ? 0 : 1)) * place + warp * 32 + lane;
+      for (int j0 = 0; j0 < t.rows; j0 += 32) {
+        float v[R][32];
+#pragma unroll
+        for (int q = 0; q < R; ++q) {
+          uint32_t raw[32];
+          tmem_ld_32x32b_x32(acc + (uint32_t)q * p.acc_width + (uint32_t)j0, raw);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[q][j] = __uint_as_float(raw[j]);
+        }
+        if (j0 + 32 >= t.rows) {  // the last columns are read: the accumulator may be used again
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&accempty[seg & 1]);
+        }
+        const int count = t.rows - j0 < 32 ? t.rows - j0 : 32;
+        if (whole) {
+          if (ok) {
+            int64_t at = t.first + j0 + (lane < count ? lane : 0);
+            if (p.experts > 0) at = p.order[at];
+            finish32<R, OUT>(ep, v, bias, c, live, at, count);
+          }
+        } else {
+#pragma unroll
+          for (int q = 0; q < R; ++q)
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j < count) __stcg(mine + ((size_t)q * p.nt + j0 + j) * TM, v[q][j]);
+        }
+      }
+      if (!whole) {
+        // the CTAs whose runs hold the tile's first and last unit; the tile's ticket is the first one's
+        const int64_t a = tile * p.nst, b = a + p.nst - 1;
+        int cf = (int)(a * run.ctas / run.units), cl = (int)(b * run.ctas / run.units);
+        while (cf > 0 && run.start(cf) > a) --cf;
+        while (cf + 1 < run.ctas && run.start(cf + 1) <= a) ++cf;
+        while (cl > 0 && run.start(cl) > b) --cl;
+        while (cl + 1 < run.ctas && run.start(cl + 1) <= b) ++cl;
+        epi_sync();  // orders all parts' stores before the fence, which publishes them
+        if (threadIdx.x == 0) {
+          __threadfence();
+          unsigned int old = ~0u;  // not counted: nobody finishes the tile
+          if (ok && !*abort_flag) asm volatile("atom.add.acq_rel.gpu.u32 %0, [%1], 1;" : "=r"(old) : "l"(&p.tickets[cf]) : "memory");
+          *last_flag = old == (unsigned int)(cl - cf) ? 1u : 0u;
+        }
+        epi_sync();
+        if (*last_flag) {
+          if (ok) {
+            for (int j0 = 0; j0 < t.rows; j0 += 32) {
+              const int count = t.rows - j0 < 32 ? t.rows - j0 : 32;
+              float v[R][32];
+#pragma unroll
+              for (int q = 0; q < R; ++q)
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[q][j] = 0.f;
+              for (int cc = cf; cc <= cl; ++cc) {
+                const int64_t first = run.start(cc) / p.nst;
+                const float *src = p.part + ((size_t)cc * 2 + (first == tile ? 0 : 1)) * place + warp * 32 + lane;
+#pragma unroll
+                for (int q = 0; q < R; ++q)
+#pragma unroll
+                  for (int j = 0; j < 32; ++j)
+                    if (j < count) v[q][j] += __ldcg(src + ((size_t)q * p.nt + j0 + j) * TM);
+              }
+              int64_t at = t.first + j0 + (lane < count ? lane : 0);
+              if (p.experts > 0) at = p.order[at];
+              finish32<R, OUT>(ep, v, bias, c, live, at, count);
+            }
+          }
+          if (threadIdx.x == 0) p.tickets[cf] = 0u;  // ready for the next call
+        }
+        epi_sync();
+      }
+      i += len;
+    }
+    // rows of pairs that no expert has are zeros
+    if (p.experts > 0) {
+      const int64_t size = std::is_same<OUT, E4M3>::value ? 1 : sizeof(OUT), bytes = ep.cols * size;
+      for (int64_t r = start[p.experts] + blockIdx.x; r < p.rows; r += gridDim.x) {
+        const int64_t row = p.order[r];
+        uint8_t *y = (uint8_t *)ep.y + row * bytes;
+        for (int64_t o = threadIdx.x; o < bytes / size; o += EPI_WARPS * 32) {
+          if (size == 4) ((uint32_t *)y)[o] = 0u;
+          else if (size == 2) ((uint16_t *)y)[o] = 0u;
+          else y[o] = 0u;
+        }
+        if constexpr (std::is_same<OUT, E4M3>::value)
+          for (int64_t o = threadIdx.x; o < ep.cols >> 5; o += EPI_WARPS * 32) ep.ys[row * (ep.cols >> 5) + o] = 27u;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == MMA_WARP) tmem_dealloc(tmem, p.tmem_cols);
+}
+
+template <int R, typename OUT>
+static int32_t launch_t(const b200_packed_desc *w, const b200_scaled_args *a, cudaStream_t stream) {
+  int sms = 0;
+  B200_CUDA_TRY(device_sms(&sms));
+  const int bits = fmt_bits(w->format);
+  Params p;
+  memset(&p, 0, sizeof(p));
+  p.x = (const uint8_t *)a->x, p.xs = (const uint8_t *)a->x_scales, p.ws = (const uint8_t *)w->scales;
+  p.offsets = a->offsets, p.order = a->order;
+  p.rows = a->rows;
+  p.n = a->experts > 0 ? w->rows / a->experts : w->rows;
+  p.wrows = w->rows;
+  p.cols = w->cols;
+  p.nblk = w->cols / 32;
+  p.experts = (int)a->experts, p.fan = a->experts > 0 ? a->fan : 1, p.per_pair = a->per_pair;
+  p.nst = (int)(w->cols / KS);
+  const Epilogue ep = epilogue_of(w, a);
+  p.wtiles = (int)((ep.cols + TM - 1) / TM);
+  // tokens of a tile: no more than an expert can have, equally full tiles
+  const int64_t most = a->experts > 0 ? (a->rows + a->fan - 1) / a->fan : a->rows;
+  const int64_t limit = ACC_COLS / R;
+  const int64_t tt = (most + limit - 1) / limit;
+  p.nt = (int)(((most + tt - 1) / tt + 15) / 16 * 16);
+  if (a->experts > 0 && tt > 1) p.nt = (int)limit;
+  p.b_off = (uint32_t)(R * TM * KS);
+  p.sfa_off = p.b_off + (uint32_t)((p.nt * KS + 1023) / 1024 * 1024);
+  p.sfb_off = p.sfa_off + R * 512;
+  p.sfb_bytes = 1024;
+  p.stage_bytes = (p.sfb_off + p.sfb_bytes + 1023) / 1024 * 1024;
+  const size_t tail = 8 * (3 * MAX_STAGES + 5) + 16 + 8 * ((size_t)p.experts + 1) + 16;
+  int stages = (int)((SMEM_LIMIT - 1024 - tail) / p.stage_bytes);
+  p.stages = stages < MAX_STAGES ? stages : MAX_STAGES;
+  p.lag = p.stages >= 6 ? 4 : 2;
+  p.tx = (uint32_t)(R * TM * KS * bits / 8);  // codes as they lie in global memory
+  p.acc_width = (uint32_t)p.nt;
+  p.sf_col = 2 * R * p.acc_width;
+  p.tmem_cols = 32;
+  while (p.tmem_cols < p.sf_col + 12 * SF_SETS) p.tmem_cols *= 2;
+  const uint32_t fmt = w->format == B200_FMT_FP4_E2M1 ? 5u : w->format == B200_FMT_FP6_E2M3 ? 3u : 4u;
+  p.idesc = (fmt << 7) | (0u << 10) | (1u << 23) | ((uint32_t)(TM >> 4) << 24);  // B: E4M3; E8M0 scales
+  p.grid = sms;
+  const size_t part = (size_t)sms * 2 * ACC_COLS * TM * sizeof(float);
+  uint8_t *base = nullptr;
+  if (int32_t rc = workspace_of(WS_SCALED, part, TICKETS * sizeof(unsigned int), stream, &base)) return rc;
+  p.part = reinterpret_cast<float *>(base);
+  p.tickets = reinterpret_cast<unsigned int *>(base + part);
+
+  CUtensorMap tmw;
+  const uint64_t row_bytes = (uint64_t)w->cols * bits / 8;
+  if (int32_t rc = make_tma_2d(&tmw, bits == 4 ? CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B : CU_TENSOR_MAP_DATA_TYPE_16U6_ALIGN16B,
+                               w->data, (uint64_t)w->cols, (uint64_t)w->rows, row_bytes, KS, TM, CU_TENSOR_MAP_SWIZZLE_128B))
+    return rc;
+  const size_t smem = 1024 + (size_t)p.stages * p.stage_bytes + tail;
+  B200_CUDA_TRY((ensure_dynamic_smem<scaled_kernel<R, OUT>>(SMEM_LIMIT)));
+  scaled_kernel<R, OUT><<<p.grid, THREADS, smem, stream>>>(tmw, p, ep);
+  B200_LAUNCH_CHECK();
+  return B200_OK;
+}
+
+template <int R>
+static int32_t dispatch(const b200_packed_desc *w, const b200_scaled_args *a, cudaStream_t stream) {
+  switch (a->y_dtype) {
+    case B200_DT_F16: return launch_t<R, __half>(w, a, stream);
+    case B200_DT_BF16: return launch_t<R, __nv_bfloat16>(w, a, stream);
+    case B200_DT_F32: return launch_t<R, float>(w, a, stream);
+    default: return launch_t<R, E4M3>(w, a, stream);
+  }
+}
+
+}  // namespace scaled
+
+// What the checks of the entry have left: whole stages, and the alignment that TMA and cp.async ask for.
+bool scaled_mma_takes(const b200_packed_desc *w, const b200_scaled_args *a) {
+  if (w->cols % scaled::KS != 0 || w->cols > (1 << 24) || w->rows > (1ll << 31) - 256) return false;
+  if ((uintptr_t)w->data % 32 != 0 || (uintptr_t)w->scales % 4 != 0) return false;
+  if ((uintptr_t)a->x % 16 != 0 || (uintptr_t)a->x_scales % 4 != 0) return false;
+  return a->experts <= scaled::MAX_EXPERTS;
+}
+
+int32_t launch_scaled_mma(const b200_packed_desc *w, const b200_scaled_args *a, cudaStream_t stream) {
+  return a->gated ? scaled::dispatch<2>(w, a, stream) : scaled::dispatch<1>(w, a, stream);
+}
+
+}  // namespace b200

@@ -1,0 +1,297 @@
+"""8-bit activations between packed projections: block-scaled rows, the RMS norm that makes them, and
+products of them with packed weights.
+
+tinygrad-dx12 has no counterpart: its packed path ends at one matmul (``src/tinygrad_dx12/codegen/
+linalg.py:136-223``). ``matmul`` takes 16-bit activations and decodes the weights; here both sides stay
+as they are stored, E4M3 codes of the activations beside FP4 / FP6 codes of the weights, each with a power
+of two for every 32 values, and the tensor cores multiply them so:
+
+    x8, h = rms_norm(y, weight, residual=h, dtype=torch.float8_e4m3fn)      add, norm, quantise
+    m8    = scaled_linear(x8, gate_up, activation="silu", gated=True, dtype=torch.float8_e4m3fn)
+    h     = scaled_linear(m8, down, residual=h)
+
+Everything runs in the library's kernels on the current stream; there is no CPU path. No gradients.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib
+from .attention import _REAL, _call, _elsewhere
+from .packed import PackedTensor, _require_cuda
+
+BLOCK = 32
+ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+SCALED_FORMATS = ("fp4_e2m1", "fp6_e2m3", "fp6_e3m2")
+_E4M3, _E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+_RESULTS = {**_REAL, _E4M3: _lib.DT["fp8e4m3"]}
+
+
+class NormArgs(ctypes.Structure):
+    """``b200_norm_args``."""
+
+    _fields_ = [("x", ctypes.c_void_p), ("residual", ctypes.c_void_p), ("total", ctypes.c_void_p),
+                ("weight", ctypes.c_void_p), ("y", ctypes.c_void_p), ("y_scales", ctypes.c_void_p),
+                ("rows", ctypes.c_int64), ("cols", ctypes.c_int64), ("x_stride", ctypes.c_int64),
+                ("residual_stride", ctypes.c_int64), ("total_stride", ctypes.c_int64), ("x_dtype", ctypes.c_int32),
+                ("total_dtype", ctypes.c_int32), ("weight_dtype", ctypes.c_int32), ("y_dtype", ctypes.c_int32),
+                ("normalize", ctypes.c_int32), ("eps", ctypes.c_float)]
+
+
+class ScaledArgs(ctypes.Structure):
+    """``b200_scaled_args``."""
+
+    _fields_ = [("x", ctypes.c_void_p), ("x_scales", ctypes.c_void_p), ("rows", ctypes.c_int64),
+                ("bias", ctypes.c_void_p), ("residual", ctypes.c_void_p), ("residual_stride", ctypes.c_int64),
+                ("y", ctypes.c_void_p), ("y_scales", ctypes.c_void_p), ("scratch", ctypes.c_void_p),
+                ("offsets", ctypes.c_void_p), ("order", ctypes.c_void_p), ("experts", ctypes.c_int64),
+                ("fan", ctypes.c_int32), ("per_pair", ctypes.c_int32), ("bias_dtype", ctypes.c_int32),
+                ("residual_dtype", ctypes.c_int32), ("y_dtype", ctypes.c_int32), ("activation", ctypes.c_int32),
+                ("gated", ctypes.c_int32), ("general", ctypes.c_int32)]
+
+
+@dataclass(frozen=True, eq=False)  # compared by identity, as caches are
+class BlockScaled:
+    """Rows of 8-bit values: ``codes`` float8_e4m3fn (..., dim) and ``scales`` float8_e8m0fnu (..., dim / 32),
+    a power of two for every 32 values along the last axis. ``quantize`` and ``rms_norm`` make them."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    def __post_init__(self) -> None:
+        if self.codes.dtype != _E4M3 or self.scales.dtype != _E8M0:
+            raise ValueError("block-scaled rows are float8_e4m3fn codes with float8_e8m0fnu scales")
+        if self.codes.dim() < 1 or self.codes.shape[-1] % BLOCK:
+            raise ValueError(f"block-scaled rows are whole blocks of {BLOCK}")
+        expected = (*self.codes.shape[:-1], self.codes.shape[-1] // BLOCK)
+        if tuple(self.scales.shape) != expected:
+            raise ValueError(f"scales must have shape {expected}")
+        if self.scales.device != self.codes.device:
+            raise _elsewhere("scales", self.scales, self.codes.device)
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.codes.shape
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def values(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """What the codes stand for, rounded once (bfloat16 and float32 hold every value whose scale lies in
+        [2^-100, 2^100])."""
+        if dtype not in _REAL:
+            raise ValueError(f"values are float16, bfloat16 or float32, not {dtype}")
+        _require_cuda(self.codes, "block-scaled rows")
+        codes, scales = _dense(self)
+        out = torch.empty(codes.shape, dtype=dtype, device=self.device)
+        if out.numel():
+            cols = codes.shape[-1]
+            _call("b200_scaled_values", self.device, codes.data_ptr(), scales.data_ptr(), codes.numel() // cols, cols,
+                  out.data_ptr(), _REAL[dtype])
+        return out
+
+
+def _dense(x: BlockScaled):
+    """x's codes and scales, contiguous and on the boundaries that the kernels ask for."""
+    codes, scales = x.codes, x.scales
+    if not codes.is_contiguous() or codes.data_ptr() % 16:
+        codes = codes.clone(memory_format=torch.contiguous_format)
+    if not scales.is_contiguous() or scales.data_ptr() % 4:
+        scales = scales.clone(memory_format=torch.contiguous_format)
+    return codes, scales
+
+
+def _flat(t: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
+    """t (..., cols) as (rows, cols) with contiguous rows; a copy where its axes do not fold."""
+    if t.dim() != 2:
+        t = t.reshape(rows, cols)
+    return t if t.stride(1) == 1 or cols == 1 else t.contiguous()
+
+
+def _blocks(shape, device) -> BlockScaled:
+    return BlockScaled(torch.empty(shape, dtype=_E4M3, device=device),
+                       torch.empty((*shape[:-1], shape[-1] // BLOCK), dtype=_E8M0, device=device))
+
+
+def _norm(x, weight, eps, residual, total, dtype, normalize):
+    device, shape = x.device, x.shape
+    cols = shape[-1]
+    rows = x.numel() // cols if cols else 0
+    y = _blocks(shape, device) if dtype == _E4M3 else torch.empty(shape, dtype=dtype, device=device)
+    if x.numel():
+        a = NormArgs()
+        flat = _flat(x, rows, cols)
+        a.x, a.x_stride, a.x_dtype, a.rows, a.cols = flat.data_ptr(), flat.stride(0), _REAL[x.dtype], rows, cols
+        if residual is not None:
+            r, t = _flat(residual, rows, cols), total.view(rows, cols)
+            a.residual, a.residual_stride = r.data_ptr(), r.stride(0)
+            a.total, a.total_stride, a.total_dtype = t.data_ptr(), t.stride(0), _REAL[residual.dtype]
+        if weight is not None:
+            a.weight, a.weight_dtype = weight.data_ptr(), _REAL[weight.dtype]
+        if dtype == _E4M3:
+            a.y, a.y_scales = y.codes.data_ptr(), y.scales.data_ptr()
+        else:
+            a.y = y.data_ptr()
+        a.y_dtype, a.normalize, a.eps = _RESULTS[dtype], normalize, eps
+        _call("b200_rms_norm", device, ctypes.byref(a))
+    return y
+
+
+def quantize(x: torch.Tensor) -> BlockScaled:
+    """``x`` (..., dim), float16, bfloat16 or float32, in 8 bits; dim a multiple of 32.
+
+    A block of 32 values along the last axis gets the smallest power of two that is not below max|x| / 448 as
+    its scale, held within [2^-100, 2^100], and each value the E4M3 code nearest to x / scale, ties to even,
+    held at 448. A NaN makes its block's scale NaN."""
+    if x.dtype not in _REAL or x.dim() < 1:
+        raise ValueError(f"quantize takes float16, bfloat16 or float32 rows, not {x.dtype}")
+    if x.shape[-1] % BLOCK:
+        raise ValueError(f"block-scaled rows are whole blocks of {BLOCK}, not {x.shape[-1]} values")
+    _require_cuda(x, "quantize's input")
+    return _norm(x, None, 0.0, None, None, _E4M3, 0)
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6, residual: torch.Tensor | None = None,
+             dtype: torch.dtype | None = None, total: torch.Tensor | None = None):
+    """``x * rsqrt(mean(x^2) + eps) * weight`` over the last axis, in fp32, rounded once.
+
+    x (..., dim): float16, bfloat16 or float32, any strides. ``weight`` (dim,) of one of these types.
+    ``dtype``: the result's, x's by default; ``torch.float8_e4m3fn`` gives ``BlockScaled`` rows, quantised from
+    fp32 as ``quantize`` does (dim a multiple of 32).
+
+    With ``residual`` (x's shape) the norm is of ``residual + x``, rounded to the residual's type, which comes back
+    too: ``y, total``. It is written into ``total`` when given (contiguous, of the residual's shape and type; it
+    may be the residual itself). No gradients."""
+    if x.dtype not in _REAL or x.dim() < 1:
+        raise ValueError(f"rms_norm takes float16, bfloat16 or float32 rows, not {x.dtype}")
+    dtype = x.dtype if dtype is None else dtype
+    if dtype not in _RESULTS:
+        raise ValueError(f"rms_norm gives float16, bfloat16, float32 or float8_e4m3fn, not {dtype}")
+    if dtype == _E4M3 and x.shape[-1] % BLOCK:
+        raise ValueError(f"block-scaled rows are whole blocks of {BLOCK}, not {x.shape[-1]} values")
+    device = x.device
+    if device.type != "cuda":
+        _require_cuda(x, "rms_norm's input")
+    if weight is not None:
+        if weight.dtype not in _REAL or weight.shape != x.shape[-1:]:
+            raise ValueError(f"weight must be float16, bfloat16 or float32 of shape ({x.shape[-1]},)")
+        if weight.device != device:
+            raise _elsewhere("weight", weight, device)
+        if not weight.is_contiguous():
+            weight = weight.contiguous()
+    if residual is None:
+        if total is not None:
+            raise ValueError("total needs a residual")
+        return _norm(x, weight, eps, None, None, dtype, 1)
+    if residual.dtype not in _REAL or residual.shape != x.shape:
+        raise ValueError("residual must be float16, bfloat16 or float32 of x's shape")
+    if residual.device != device:
+        raise _elsewhere("residual", residual, device)
+    if total is None:
+        total = torch.empty(residual.shape, dtype=residual.dtype, device=device)
+    elif total.shape != residual.shape or total.dtype != residual.dtype or total.device != device or not total.is_contiguous():
+        raise ValueError("total must be contiguous, of the residual's shape, type and device")
+    return _norm(x, weight, eps, residual, total, dtype, 1), total
+
+
+def _check_weights(w: PackedTensor, dims: int, what: str) -> None:
+    if not isinstance(w, PackedTensor) or len(w.shape) != dims:
+        raise ValueError(f"{what} takes a PackedTensor of {dims} dimensions")
+    if w.format not in SCALED_FORMATS:
+        raise ValueError(f"{what} takes FP4 or FP6 weights, not {w.format}")
+    if w.scales is None or w.scales.dtype != _E8M0 or w.block_size != BLOCK or w.cols < 1 or w.cols % BLOCK:
+        raise ValueError(f"{what} takes weights with float8_e8m0fnu scales in whole blocks of {BLOCK}")
+    if w.device.type != "cuda":
+        _require_cuda(w.data, "packed data")
+
+
+def _check_product(x, w, activation, gated, dtype, what):
+    """Columns of the result."""
+    if not isinstance(x, BlockScaled):
+        raise ValueError(f"{what} takes BlockScaled activations (quantize, rms_norm)")
+    if x.shape[-1] != w.cols:
+        raise ValueError(f"activations of {x.shape[-1]} values do not fit weights of {w.cols}")
+    if x.device != w.device:
+        raise _elsewhere("activations", x, w.device)
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"unknown activation {activation!r}")
+    if dtype not in _RESULTS:
+        raise ValueError(f"{what} gives float16, bfloat16, float32 or float8_e4m3fn, not {dtype}")
+    cols = w.shape[-2]
+    if gated:
+        if cols % 2:
+            raise ValueError("gated weights hold as many gate rows as up rows")
+        cols //= 2
+    if dtype == _E4M3 and cols % BLOCK:
+        raise ValueError(f"block-scaled rows are whole blocks of {BLOCK}, not {cols} values")
+    return cols
+
+
+def _check_bias(bias, shape, device, name="bias"):
+    if bias is None:
+        return None
+    if bias.dtype not in _REAL or tuple(bias.shape) != tuple(shape):
+        raise ValueError(f"{name} must be float16, bfloat16 or float32 of shape {tuple(shape)}")
+    if bias.device != device:
+        raise _elsewhere(name, bias, device)
+    return bias if bias.is_contiguous() else bias.contiguous()
+
+
+def _product(x, w, y, rows, bias, activation, gated, residual=None, plan=None, fan=1, per_pair=0, general=False):
+    """Launches one product of checked operands into y."""
+    codes, scales = _dense(x)
+    a = ScaledArgs()
+    a.x, a.x_scales, a.rows = codes.data_ptr(), scales.data_ptr(), rows
+    if bias is not None:
+        a.bias, a.bias_dtype = bias.data_ptr(), _REAL[bias.dtype]
+    if residual is not None:
+        a.residual, a.residual_stride, a.residual_dtype = residual.data_ptr(), residual.stride(0), _REAL[residual.dtype]
+    if isinstance(y, BlockScaled):
+        a.y, a.y_scales, a.y_dtype = y.codes.data_ptr(), y.scales.data_ptr(), _RESULTS[_E4M3]
+    else:
+        a.y, a.y_dtype = y.data_ptr(), _REAL[y.dtype]
+    if plan is not None:
+        a.offsets, a.order, a.experts = plan.offsets.data_ptr(), plan.rows.data_ptr(), w.shape[0]
+        a.fan, a.per_pair = fan, per_pair
+    a.activation, a.gated, a.general = ACTIVATIONS[activation], int(gated), int(general)
+    desc = w.desc()
+    if general or w.cols % 128 or desc.data % 32 or desc.scales % 4:  # not on the tensor cores
+        size = _lib.lib().b200_scaled_linear_scratch(ctypes.byref(desc), ctypes.byref(a))
+        scratch = torch.empty(size, dtype=torch.uint8, device=x.device)
+        a.scratch = scratch.data_ptr()
+    _call("b200_scaled_linear", x.device, ctypes.byref(desc), ctypes.byref(a))
+
+
+def scaled_linear(x: BlockScaled, w: PackedTensor, bias: torch.Tensor | None = None, activation: str | None = None,
+                  gated: bool = False, residual: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16,
+                  _general: bool = False):
+    """``act(x W^T + bias) + residual``: products of 8-bit rows with packed weights and what follows them.
+
+    x (..., K); ``w`` (N, K) FP4 or FP6 with E8M0 scales in blocks of 32 (K a multiple of 32; of 128, and data on a
+    32-byte boundary, for the tensor cores: other calls run, slowly, on a general kernel). Both are multiplied
+    as stored, sums are fp32. ``activation``: None, "relu", "silu", "gelu" or "gelu_tanh". ``gated``: w's rows are
+    [gate; up], N / 2 each, and the result is act(gate) * up. ``bias`` (N,). ``residual`` (..., columns of the
+    result) is added behind the activation. ``dtype``: float16, bfloat16 or float32, rounded once, or float8_e4m3fn for
+    ``BlockScaled`` rows quantised from fp32 (columns a multiple of 32). No gradients."""
+    _check_weights(w, 2, "scaled_linear")
+    cols = _check_product(x, w, activation, gated, dtype, "scaled_linear")
+    device = x.device
+    bias = _check_bias(bias, w.shape[:1], device)
+    shape = (*x.shape[:-1], cols)
+    rows = math.prod(x.shape[:-1])
+    if residual is not None:
+        if residual.dtype not in _REAL or tuple(residual.shape) != shape:
+            raise ValueError(f"residual must be float16, bfloat16 or float32 of shape {shape}")
+        if residual.device != device:
+            raise _elsewhere("residual", residual, device)
+        residual = _flat(residual, rows, cols)
+    y = _blocks(shape, device) if dtype == _E4M3 else torch.empty(shape, dtype=dtype, device=device)
+    if rows and cols:
+        _product(x, w, y, rows, bias, activation, gated, residual, general=_general)
+    return y
