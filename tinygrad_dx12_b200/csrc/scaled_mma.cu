@@ -10,15 +10,15 @@
 // A tile is R x 128 weight rows (the MMA's M; R = 2 when gated: 128 gate rows and the 128 up rows that go
 // with them, in two accumulators, so both are in one thread's hands) times up to NT tokens (its N, a
 // multiple of 16, so an expert with few tokens costs few columns). K advances 128 codes a stage.
-//   warps 0-3    epilogue: tcgen05.ld (lane = weight row, column = token), bias, activation, gate,
-//                residual; a warp's 32 rows are 32 neighbouring columns of y, a block of the 8-bit output,
-//                whose largest value is one warp-wide maximum
-//   warps 4-7    cp.async of x's codes (token rows found through the plan's order when there are experts)
+//   warps 0-7    epilogue, two groups of four that take turns at 16 or 32 tokens: tcgen05.ld (lane = weight
+//                row, column = token), bias, activation, gate, residual; a warp's 32 rows are 32 neighbouring
+//                columns of y, a block of the 8-bit output, whose largest value is one warp-wide maximum
+//   warps 8-11   cp.async of x's codes (token rows found through the plan's order when there are experts)
 //                and of both sides' scale bytes, four of a row at a time, into the layout that
-//                tcgen05.cp takes; a stage is announced when its copies, some stages back, have landed
-//   warp 8       one thread: tcgen05.cp of the scales into tensor memory, four MMAs a stage and
+//                tcgen05.cp takes; the copies themselves arrive at the stage's barrier when they land
+//   warp 12      one thread: tcgen05.cp of the scales into tensor memory, four MMAs a stage and
 //                accumulator; commit frees the stage
-//   warps 9-11   one thread each: TMA of the weight codes (a thread issues a box in several hundred
+//   warps 13-15  one thread each: TMA of the weight codes (a thread issues a box in several hundred
 //                cycles, so three take turns)
 // Two accumulators of a tile's width, so that the epilogue of one tile runs under the products of the
 // next: 2 x 224 columns, and four rotating sets of scale columns beside them.
@@ -46,8 +46,8 @@ int32_t scaled_mma_reset_tickets() { return workspace_zero(WS_SCALED); }
 namespace scaled {
 
 constexpr int TM = 128, KS = 128;            // weight rows of an MMA, codes of a stage
-constexpr int EPI_WARPS = 4, LOAD_WARP0 = 4, LOAD_WARPS = 4, MMA_WARP = 8, W_WARP0 = 9, W_WARPS = 3;
-constexpr int THREADS = 12 * 32;           // three warps a scheduler: up to 168 registers
+constexpr int EPI_WARPS = 8, LOAD_WARP0 = 8, LOAD_WARPS = 4, MMA_WARP = 12, W_WARP0 = 13, W_WARPS = 3;
+constexpr int THREADS = 16 * 32, LOADERS = LOAD_WARPS * 32;
 constexpr int ACC_COLS = 224;                // columns of an accumulator set: R * NT at most
 constexpr int SF_SETS = 4;
 constexpr int MAX_STAGES = 12;
@@ -67,7 +67,7 @@ struct Params {
   int nst;                // K stages
   int wtiles;             // tiles of weight rows of one matrix
   int nt;                 // tokens of a tile, at most
-  int grid, stages, lag;
+  int grid, stages;
   uint32_t stage_bytes, b_off, sfa_off, sfb_off, sfb_bytes;
   uint32_t tx;
   uint32_t acc_width, sf_col, tmem_cols;
@@ -76,7 +76,7 @@ struct Params {
   unsigned int *tickets;  // [grid]: of the tile that the CTA's run ends in
 };
 
-__device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, %0;" ::"n"(EPI_WARPS * 32) : "memory"); }
 
 __device__ __forceinline__ void cp_async16(void *dst, const void *src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
@@ -84,11 +84,11 @@ __device__ __forceinline__ void cp_async16(void *dst, const void *src) {
 __device__ __forceinline__ void cp_async4(void *dst, const void *src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// Arrives at `bar` when the copies that this thread has issued so far have landed.
+__device__ __forceinline__ void cp_arrive(uint64_t *bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+__device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // Shared-memory descriptor of a scale atom (32 rows of 16 bytes, no swizzle), tcgen05.cp's source, and the
 // copy into 4 columns of every lane quarter.
@@ -153,36 +153,72 @@ __device__ __forceinline__ T to_out(float v) {
 }
 struct E4M3 {};
 
-// One weight row's products with 32 tokens, column `c` of y (live: c is one): finished and stored. `at` is
+template <int N>
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[N]) {
+  uint32_t (&r)[N] = reinterpret_cast<uint32_t (&)[N]>(v);
+  if constexpr (N == 32) tmem_ld_32x32b_x32(taddr, r);
+  else tmem_ld_32x32b_x16(taddr, r);
+}
+
+// One weight row's products with CH tokens, column `c` of y (live: c is one): finished and stored. `at` is
 // the row of y of token j in lane j.
-template <int R, typename OUT>
-__device__ __forceinline__ void finish32(const Epilogue &ep, float (&v)[R][32], const float (&bias)[R], int64_t c, bool live,
-                                         int64_t at, int count) {
+template <int R, typename OUT, int CH>
+__device__ __forceinline__ void finish(const Epilogue &ep, float (&v)[R][CH], const float (&bias)[R], int c, bool live,
+                                       int at, int count) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int j = 0; j < 32; ++j) v[0][j] += bias[0];
-  if (ep.activation != B200_ACT_NONE) {
+  for (int j = 0; j < CH; ++j) v[0][j] += bias[0];
+  switch (ep.activation) {  // outside the loop: a column's functions run side by side
+    case B200_ACT_RELU:
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[0][j] = activate(v[0][j], ep.activation);
+      for (int j = 0; j < CH; ++j) v[0][j] = activate<B200_ACT_RELU>(v[0][j]);
+      break;
+    case B200_ACT_SILU:
+#pragma unroll
+      for (int j = 0; j < CH; ++j) v[0][j] = activate<B200_ACT_SILU>(v[0][j]);
+      break;
+    case B200_ACT_GELU:
+#pragma unroll
+      for (int j = 0; j < CH; ++j) v[0][j] = activate<B200_ACT_GELU>(v[0][j]);
+      break;
+    case B200_ACT_GELU_TANH:
+#pragma unroll
+      for (int j = 0; j < CH; ++j) v[0][j] = activate<B200_ACT_GELU_TANH>(v[0][j]);
+      break;
   }
   if constexpr (R == 2) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[0][j] = __fmul_rn(v[0][j], v[1][j] + bias[1]);
+    for (int j = 0; j < CH; ++j) v[0][j] = __fmul_rn(v[0][j], v[1][j] + bias[1]);
   }
+  const int cols = (int)ep.cols;
+  if (ep.residual != nullptr) {
 #pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    if (j >= count) break;
-    const int64_t row = __shfl_sync(0xffffffffu, at, j);
-    float f = v[0][j];
-    if (ep.residual != nullptr && live) f += load_as_f32(ep.residual, row * ep.rstride + c, ep.rdt);
-    if constexpr (std::is_same<OUT, E4M3>::value) {  // y's columns are whole blocks: a warp's are all live or none
-      const uint32_t byte = rows8::scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(f) & 0x7FFFFFFFu));
-      if (live) {
-        ((uint8_t *)ep.y)[row * ep.cols + c] = (uint8_t)rows8::codes2(f, 0.f, rows8::inverse(byte), byte == 255u);
-        if (lane == 0) ep.ys[row * (ep.cols >> 5) + (c >> 5)] = (uint8_t)byte;
-      }
-    } else if (live) {
-      ((OUT *)ep.y)[row * ep.cols + c] = to_out<OUT>(f);
+    for (int j = 0; j < CH; ++j) {
+      const int row = __shfl_sync(0xffffffffu, at, j);
+      if (live && j < count) v[0][j] += load_as_f32(ep.residual, row * ep.rstride + c, ep.rdt);
+    }
+  }
+  if constexpr (std::is_same<OUT, E4M3>::value) {  // y's columns are whole blocks: a warp's are all live or none
+    uint32_t top = 0;  // of token j in lane j, which finds the scale for all
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+      const uint32_t t = __reduce_max_sync(0xffffffffu, __float_as_uint(v[0][j]) & 0x7FFFFFFFu);
+      if (lane == j) top = t;
+    }
+    const uint32_t byte = rows8::scale_byte(top);
+    const float inv = rows8::inverse(byte);
+    if (live && lane < count) ep.ys[(int64_t)at * (cols >> 5) + (c >> 5)] = (uint8_t)byte;
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+      const int row = __shfl_sync(0xffffffffu, at, j);
+      const float s = __shfl_sync(0xffffffffu, inv, j);
+      if (live && j < count) ((uint8_t *)ep.y)[(int64_t)row * cols + c] = (uint8_t)rows8::codes2(v[0][j], 0.f, s, s == 0.f);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+      const int row = __shfl_sync(0xffffffffu, at, j);
+      if (live && j < count) ((OUT *)ep.y)[(int64_t)row * cols + c] = to_out<OUT>(v[0][j]);
     }
   }
 }
@@ -209,7 +245,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(&fullw[s], 1);
-      mbar_init(&fullx[s], LOAD_WARPS);
+      mbar_init(&fullx[s], LOADERS);
       mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -284,16 +320,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int th = threadIdx.x - LOAD_WARP0 * 32;
     const int chunk = th & 7, r0 = th >> 3;  // 16 bytes of a row's 128; rows r0, r0 + 16, ...
     constexpr int PASSES = ACC_COLS / R / 16;
-    int64_t done = 0;  // stages announced
-    int slot = 0, dslot = 0;
+    int slot = 0;
     uint32_t round = 0;
-    auto announce = [&]() {
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&fullx[dslot]);
-      if (++dslot == S) dslot = 0;
-      ++done;
-    };
     int64_t i = 0;
     bool ok = true;
     while (i < n && ok) {
@@ -336,17 +364,11 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
         for (int q = 0; q < 2; ++q)
           if (sx[q] != nullptr) cp_async4(st + p.sfb_off + q * 512 + sf_at, sx[q] + 4 * s);
-        cp_commit();
+        cp_arrive(&fullx[slot]);
         if (++slot == S) slot = 0, ++round;
-        if (i + 1 - done > p.lag) {  // the stage `lag` back has landed
-          if (p.lag == 4) cp_wait<4>();
-          else cp_wait<2>();
-          announce();
-        }
       }
     }
-    cp_wait<0>();
-    while (ok && done < n) announce();
+    cp_wait_all();
   } else if (warp == MMA_WARP) {
     // ---------------- MMA issuer ----------------
     if (lane == 0) {
@@ -367,6 +389,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int64_t j = 0; j < len; ++j) {
           ok = mbar_wait(&fullw[slot], phase, abort_flag) && mbar_wait(&fullx[slot], phase, abort_flag);
           if (!ok) break;
+          fence_proxy_async_smem();  // cp.async wrote by the generic proxy, the tensor core reads by the other
           tc_fence_after();
           const uint8_t *st = ring + (size_t)slot * p.stage_bytes;
           const uint32_t sf = tmem + p.sf_col + 12u * (uint32_t)set;
@@ -397,7 +420,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   } else if (warp < EPI_WARPS) {
     // ---------------- epilogue: weight row = tensor-memory lane, token = column ----------------
-    const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
+    const int quarter = warp & 3, group = warp >> 2;
+    const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+    constexpr int CH = R == 2 ? 16 : 32;  // tokens at a time: R * CH accumulators in registers
     bool ok = true;  // this warp's waits; after one that ran out it still meets the others
     int seg = 0;
     for (int64_t i = 0; i < n; ++seg) {
@@ -406,45 +431,43 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int64_t len = p.nst - s0 < n - i ? p.nst - s0 : n - i;
       const bool whole = s0 == 0 && len == p.nst;
       const Tile t = tile_at(p, before, start, tile);
-      const int64_t c = t.w0 + warp * 32 + lane;  // column of y
+      const int c = (int)t.w0 + quarter * 32 + lane;  // column of y
       const bool live = c < ep.cols;
       float bias[R];
 #pragma unroll
       for (int q = 0; q < R; ++q)
         bias[q] = ep.bias != nullptr && live ? load_as_f32(ep.bias, t.e * p.n + q * ep.cols + c, ep.bdt) : 0.f;
+      auto row_of = [&](int j0, int count) -> int {  // of y, of token j0 + lane
+        const int64_t at = t.first + j0 + (lane < count ? lane : 0);
+        return p.experts > 0 ? p.order[at] : (int)at;
+      };
       ok = __all_sync(0xffffffffu, ok && mbar_wait(&accfull[seg & 1], (uint32_t)((seg / 2) & 1), abort_flag));
       tc_fence_after();
       const uint32_t acc = tmem + lane_base + (uint32_t)(seg & 1) * R * p.acc_width;
       // partial sums: of the CTA's first tile in place 0, of its last in place 1
       const size_t place = (size_t)R * p.nt * TM;
-      float *mine = p.part + ((size_t)blockIdx.x * 2 + (i == 0 ? 0 : 1)) * place + warp * 32 + lane;
-      for (int j0 = 0; j0 < t.rows; j0 += 32) {
-        float v[R][32];
+      float *mine = p.part + ((size_t)blockIdx.x * 2 + (i == 0 ? 0 : 1)) * place + quarter * 32 + lane;
+      const int last = (t.rows - 1) / CH;  // chunk; the groups take turns
+      if (group > last && lane == 0) mbar_arrive(&accempty[seg & 1]);
+      for (int ch = group; ch <= last; ch += 2) {
+        const int j0 = ch * CH, count = t.rows - j0 < CH ? t.rows - j0 : CH;
+        float v[R][CH];
 #pragma unroll
-        for (int q = 0; q < R; ++q) {
-          uint32_t raw[32];
-          tmem_ld_32x32b_x32(acc + (uint32_t)q * p.acc_width + (uint32_t)j0, raw);
-          tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[q][j] = __uint_as_float(raw[j]);
-        }
-        if (j0 + 32 >= t.rows) {  // the last columns are read: the accumulator may be used again
+        for (int q = 0; q < R; ++q) tmem_ld<CH>(acc + (uint32_t)q * p.acc_width + (uint32_t)j0, v[q]);
+        tmem_ld_wait();
+        if (ch + 2 > last) {  // the group's last columns are read: the accumulator may be used again
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&accempty[seg & 1]);
         }
-        const int count = t.rows - j0 < 32 ? t.rows - j0 : 32;
+        if (!ok) continue;
         if (whole) {
-          if (ok) {
-            int64_t at = t.first + j0 + (lane < count ? lane : 0);
-            if (p.experts > 0) at = p.order[at];
-            finish32<R, OUT>(ep, v, bias, c, live, at, count);
-          }
+          finish<R, OUT, CH>(ep, v, bias, c, live, row_of(j0, count), count);
         } else {
 #pragma unroll
           for (int q = 0; q < R; ++q)
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
+            for (int j = 0; j < CH; ++j)
               if (j < count) __stcg(mine + ((size_t)q * p.nt + j0 + j) * TM, v[q][j]);
         }
       }
@@ -465,27 +488,23 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         epi_sync();
         if (*last_flag) {
-          if (ok) {
-            for (int j0 = 0; j0 < t.rows; j0 += 32) {
-              const int count = t.rows - j0 < 32 ? t.rows - j0 : 32;
-              float v[R][32];
+          for (int ch = group; ch <= last; ch += 2) {
+            const int j0 = ch * CH, count = t.rows - j0 < CH ? t.rows - j0 : CH;
+            float v[R][CH];
+#pragma unroll
+            for (int q = 0; q < R; ++q)
+#pragma unroll
+              for (int j = 0; j < CH; ++j) v[q][j] = 0.f;
+            for (int cc = cf; cc <= cl; ++cc) {
+              const int64_t first = run.start(cc) / p.nst;
+              const float *src = p.part + ((size_t)cc * 2 + (first == tile ? 0 : 1)) * place + quarter * 32 + lane;
 #pragma unroll
               for (int q = 0; q < R; ++q)
 #pragma unroll
-                for (int j = 0; j < 32; ++j) v[q][j] = 0.f;
-              for (int cc = cf; cc <= cl; ++cc) {
-                const int64_t first = run.start(cc) / p.nst;
-                const float *src = p.part + ((size_t)cc * 2 + (first == tile ? 0 : 1)) * place + warp * 32 + lane;
-#pragma unroll
-                for (int q = 0; q < R; ++q)
-#pragma unroll
-                  for (int j = 0; j < 32; ++j)
-                    if (j < count) v[q][j] += __ldcg(src + ((size_t)q * p.nt + j0 + j) * TM);
-              }
-              int64_t at = t.first + j0 + (lane < count ? lane : 0);
-              if (p.experts > 0) at = p.order[at];
-              finish32<R, OUT>(ep, v, bias, c, live, at, count);
+                for (int j = 0; j < CH; ++j)
+                  if (j < count) v[q][j] += __ldcg(src + ((size_t)q * p.nt + j0 + j) * TM);
             }
+            finish<R, OUT, CH>(ep, v, bias, c, live, row_of(j0, count), count);
           }
           if (threadIdx.x == 0) p.tickets[cf] = 0u;  // ready for the next call
         }
@@ -547,7 +566,6 @@ static int32_t launch_t(const b200_packed_desc *w, const b200_scaled_args *a, cu
   const size_t tail = 8 * (3 * MAX_STAGES + 5) + 16 + 8 * ((size_t)p.experts + 1) + 16;
   int stages = (int)((SMEM_LIMIT - 1024 - tail) / p.stage_bytes);
   p.stages = stages < MAX_STAGES ? stages : MAX_STAGES;
-  p.lag = p.stages >= 6 ? 4 : 2;
   p.tx = (uint32_t)(R * TM * KS * bits / 8);  // codes as they lie in global memory
   p.acc_width = (uint32_t)p.nt;
   p.sf_col = 2 * R * p.acc_width;
