@@ -16,10 +16,11 @@
 //   warps 8-11   cp.async of x's codes (token rows found through the plan's order when there are experts)
 //                and of both sides' scale bytes, four of a row at a time, into the layout that
 //                tcgen05.cp takes; the copies themselves arrive at the stage's barrier when they land
-//   warp 12      one thread: tcgen05.cp of the scales into tensor memory, four MMAs a stage and
-//                accumulator; commit frees the stage
-//   warps 13-15  one thread each: TMA of the weight codes (a thread issues a box in several hundred
-//                cycles, so three take turns)
+//   warp 13      waits for all of a stage, then tcgen05.cp of its scales into one of four sets of tensor-memory
+//                columns; commit announces the stage to warp 12
+//   warp 12      four MMAs a stage and accumulator; commit frees the stage and its set. (One warp for both
+//                took 0.5 us a stage: copies, waits and MMAs cost an issuing thread 25 to 45 ns each)
+//   warps 14-15  one thread each: TMA of the weight codes
 // Two accumulators of a tile's width, so that the epilogue of one tile runs under the products of the
 // next: 2 x 224 columns, and four rotating sets of scale columns beside them.
 //
@@ -46,7 +47,7 @@ int32_t scaled_mma_reset_tickets() { return workspace_zero(WS_SCALED); }
 namespace scaled {
 
 constexpr int TM = 128, KS = 128;            // weight rows of an MMA, codes of a stage
-constexpr int EPI_WARPS = 8, LOAD_WARP0 = 8, LOAD_WARPS = 4, MMA_WARP = 12, W_WARP0 = 13, W_WARPS = 3;
+constexpr int EPI_WARPS = 8, LOAD_WARP0 = 8, LOAD_WARPS = 4, MMA_WARP = 12, SF_WARP = 13, W_WARP0 = 14, W_WARPS = 2;
 constexpr int THREADS = 16 * 32, LOADERS = LOAD_WARPS * 32;
 constexpr int ACC_COLS = 224;                // columns of an accumulator set: R * NT at most
 constexpr int SF_SETS = 4;
@@ -78,11 +79,24 @@ struct Params {
 
 __device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, %0;" ::"n"(EPI_WARPS * 32) : "memory"); }
 
-__device__ __forceinline__ void cp_async16(void *dst, const void *src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+// Whether the phase is over, without waiting.
+__device__ __forceinline__ bool mbar_over(uint64_t *bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
 }
-__device__ __forceinline__ void cp_async4(void *dst, const void *src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void *src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 // Arrives at `bar` when the copies that this thread has issued so far have landed.
 __device__ __forceinline__ void cp_arrive(uint64_t *bar) {
@@ -90,14 +104,39 @@ __device__ __forceinline__ void cp_arrive(uint64_t *bar) {
 }
 __device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// Shared-memory descriptor of a scale atom (32 rows of 16 bytes, no swizzle), tcgen05.cp's source, and the
-// copy into 4 columns of every lane quarter.
+// Shared-memory descriptor of a scale atom: 32 rows of 16 bytes, no swizzle.
 __device__ __forceinline__ uint64_t sf_desc(const void *atom) {
   const uint64_t addr = smem_u32(atom);
   return ((addr & 0x3FFFFull) >> 4) | ((uint64_t)(128 >> 4) << 16) | ((uint64_t)(128 >> 4) << 32) | (1ull << 46);
 }
+// The tensor core's work is issued by one lane of a converged warp: descriptors stay in uniform registers.
+// An atom into 4 columns of every lane quarter:
 __device__ __forceinline__ void sf_copy(uint32_t taddr, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  asm volatile(
+      "{\n\t.reg .pred q;\n\telect.sync _|q, 0xFFFFFFFF;\n\t"
+      "@q tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(taddr), "l"(desc) : "memory");
+}
+// The four products of a stage (K = 32 each: 32 bytes further along the rows, scale byte k): D (+)= A B^T.
+__device__ __forceinline__ void mma_stage(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t sfa,
+                                          uint32_t sfb) {
+  constexpr uint32_t ID = (1u << 4) | (1u << 29), SF = 1u << 30;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\telect.sync _|q, 0xFFFFFFFF;\n\tsetp.ne.b32 p, %1, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale [%0], %2, %6, %10, [%14], [%18], p;\n\t"
+      "setp.eq.b32 p, 0, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale [%0], %3, %7, %11, [%15], [%19], p;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale [%0], %4, %8, %12, [%16], [%20], p;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale [%0], %5, %9, %13, [%17], [%21], p;\n\t}" ::"r"(d),
+      "r"(acc), "l"(a), "l"(a + 2), "l"(a + 4), "l"(a + 6), "l"(b), "l"(b + 2), "l"(b + 4), "l"(b + 6), "r"(idesc),
+      "r"(idesc + ID), "r"(idesc + 2 * ID), "r"(idesc + 3 * ID), "r"(sfa), "r"(sfa + SF), "r"(sfa + 2 * SF), "r"(sfa + 3 * SF),
+      "r"(sfb), "r"(sfb + SF), "r"(sfb + 2 * SF), "r"(sfb + 3 * SF)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t *bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\telect.sync _|q, 0xFFFFFFFF;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
+      : "memory");
 }
 
 // What a tile is: expert, first weight row within its matrix, place of its first row, rows.
@@ -225,17 +264,18 @@ __device__ __forceinline__ void finish(const Epilogue &ep, float (&v)[R][CH], co
 
 template <int R, typename OUT>
 __global__ void __launch_bounds__(THREADS, 1)
-    scaled_kernel(const __grid_constant__ CUtensorMap tmw, const __grid_constant__ Params p, const __grid_constant__ Epilogue ep) {
+    scaled_kernel(const __grid_constant__ CUtensorMap tmw, const __grid_constant__ CUtensorMap tmx, const __grid_constant__ Params p, const __grid_constant__ Epilogue ep) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t *ring = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const int S = p.stages;
   uint64_t *fullw = reinterpret_cast<uint64_t *>(ring + (size_t)S * p.stage_bytes);
   uint64_t *fullx = fullw + S;
   uint64_t *empty = fullx + S;
-  uint64_t *accfull = empty + S;
+  uint64_t *sfready = empty + S;
+  uint64_t *accfull = sfready + SF_SETS;
   uint64_t *accempty = accfull + 2;
   uint64_t *drain = accempty + 2;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 2);
   volatile uint32_t *abort_flag = tmem_slot + 1;
   volatile uint32_t *last_flag = tmem_slot + 2;
   int32_t *start = reinterpret_cast<int32_t *>(tmem_slot + 4);  // [experts + 1] the plan's offsets
@@ -248,11 +288,13 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(&fullx[s], LOADERS);
       mbar_init(&empty[s], 1);
     }
+    for (int b = 0; b < SF_SETS; ++b) mbar_init(&sfready[b], 1);
     for (int b = 0; b < 2; ++b) {
       mbar_init(&accfull[b], 1);
       mbar_init(&accempty[b], EPI_WARPS);
     }
     mbar_init(drain, 1);
+    mbar_init(drain + 1, 1);
     *abort_flag = 0;
     fence_mbar_init();
     prefetch_tmap(&tmw);
@@ -295,11 +337,12 @@ __global__ void __launch_bounds__(THREADS, 1)
       int s = (int)((run.u0 + turn) % p.nst);
       int slot = turn;
       uint32_t round = 0;
-      int64_t row = 0, known = -1;
+      int64_t row = 0, first = 0, known = -1;
       for (; i < n && turn < turns; i += turns) {
         if (tile != known) {
           const Tile t = tile_at(p, before, start, tile);
           row = t.e * p.n + t.w0;
+          first = t.first;
           known = tile;
         }
         if (round > 0 && !mbar_wait(&empty[slot], (round - 1u) & 1u, abort_flag)) break;
@@ -307,6 +350,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         mbar_arrive_expect_tx(&fullw[slot], p.tx);
         tma_load_2d(st, &tmw, s * KS, (int32_t)row, &fullw[slot]);
         if constexpr (R == 2) tma_load_2d(st + TM * KS, &tmw, s * KS, (int32_t)(row + ep.cols), &fullw[slot]);
+        if (p.experts == 0) tma_load_2d(st + p.b_off, &tmx, s * KS, (int32_t)first, &fullw[slot]);
         for (s += turns; s >= p.nst; s -= p.nst) ++tile;
         if ((slot += turns) >= S) slot -= S, ++round;
       }
@@ -316,108 +360,144 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     }
   } else if (warp >= LOAD_WARP0 && warp < LOAD_WARP0 + LOAD_WARPS) {
-    // ---------------- cp.async of x's codes and of all scale bytes ----------------
+    // ---------------- cp.async of all scale bytes and, through experts, of x's codes ----------------
+    // A stage is worth some 450 cycles, and one warp's dependent instructions take 4 to 6 each: pointers are
+    // kept and moved on, so that a copy is one instruction.
     const int th = threadIdx.x - LOAD_WARP0 * 32;
-    const int chunk = th & 7, r0 = th >> 3;  // 16 bytes of a row's 128; rows r0, r0 + 16, ...
+    const int chunk = th & 7, r0 = th >> 3;  // 16 bytes of a row's 128; rows r0, r0 + 16, ... (r & 7 the same in all)
     constexpr int PASSES = ACC_COLS / R / 16;
+    const uint32_t base = smem_u32(ring);
+    const uint32_t bdst = base + p.b_off + (uint32_t)(r0 * 128 + ((chunk ^ (r0 & 7)) << 4));
+    const uint32_t sdst = base + p.sfa_off + (uint32_t)((th & 31) * 16 + (th >> 5) * 4);
+    const uint32_t to_b = p.sfb_off - p.sfa_off;
     int slot = 0;
-    uint32_t round = 0;
-    int64_t i = 0;
+    uint32_t round = 0, off = 0;
     bool ok = true;
-    while (i < n && ok) {
+    for (int64_t i = 0; i < n && ok;) {
       const int64_t u = run.u0 + i;
       const Tile t = tile_at(p, before, start, u / p.nst);
-      int s = (int)(u % p.nst);
-      const int64_t len = p.nst - s < n - i ? p.nst - s : n - i;
-      // rows of x: where this thread's begin
-      auto xrow = [&](int r) -> int64_t {
+      const int s = (int)(u % p.nst);
+      const int len = (int)(p.nst - s < n - i ? p.nst - s : n - i);
+      i += len;
+      auto xrow = [&](int r) -> int64_t {  // row of x
         const int64_t at = t.first + r;
         if (p.experts == 0) return at;
         const int32_t pair = p.order[at];
         return p.per_pair ? pair : pair / p.fan;
       };
-      uint32_t rows[PASSES];
+      const uint8_t *src[PASSES], *sx[2], *sw[R];
+      const int passes = p.experts > 0 ? (t.rows - r0 + 15) / 16 : 0;  // this thread's; the warp's most are the tile's
+      const int most = p.experts > 0 ? (t.rows + 15) / 16 : 0;
 #pragma unroll
-      for (int q = 0; q < PASSES; ++q) rows[q] = r0 + 16 * q < t.rows ? (uint32_t)xrow(r0 + 16 * q) : 0u;
-      const uint8_t *sx[2], *sw[R];
+      for (int q = 0; q < PASSES; ++q)
+        src[q] = q < passes ? p.x + xrow(r0 + 16 * q) * p.cols + (int64_t)s * KS + chunk * 16 : p.x;
 #pragma unroll
-      for (int q = 0; q < 2; ++q) sx[q] = th + 128 * q < t.rows ? p.xs + xrow(th + 128 * q) * p.nblk : nullptr;
+      for (int q = 0; q < 2; ++q) sx[q] = th + 128 * q < t.rows ? p.xs + xrow(th + 128 * q) * p.nblk + 4 * s : nullptr;
 #pragma unroll
       for (int q = 0; q < R; ++q) {
         int64_t wrow = t.e * p.n + q * ep.cols + t.w0 + th;
         if (wrow >= p.wrows) wrow = p.wrows - 1;  // rows behind the last: not stored
-        sw[q] = p.ws + wrow * p.nblk;
+        sw[q] = p.ws + wrow * p.nblk + 4 * s;
       }
-      const uint32_t sf_at = (uint32_t)(th & 31) * 16 + (uint32_t)(th >> 5) * 4;
-      for (int64_t j = 0; j < len; ++j, ++i, ++s) {
+      for (int j = 0; j < len; ++j) {
         if (round > 0) ok = __all_sync(0xffffffffu, mbar_wait(&empty[slot], (round - 1u) & 1u, abort_flag));
         if (!ok) break;
-        uint8_t *st = ring + (size_t)slot * p.stage_bytes;
-        const int64_t k = (int64_t)s * KS + chunk * 16;
 #pragma unroll
-        for (int q = 0; q < PASSES; ++q) {
-          const int r = r0 + 16 * q;
-          if (r < t.rows) cp_async16(st + p.b_off + r * 128 + ((chunk ^ (r & 7)) << 4), p.x + (int64_t)rows[q] * p.cols + k);
+        for (int q = 0; q < R; ++q) {
+          cp_async4(sdst + off + q * 512, sw[q]);
+          sw[q] += 4;
         }
 #pragma unroll
-        for (int q = 0; q < R; ++q) cp_async4(st + p.sfa_off + q * 512 + sf_at, sw[q] + 4 * s);
-#pragma unroll
         for (int q = 0; q < 2; ++q)
-          if (sx[q] != nullptr) cp_async4(st + p.sfb_off + q * 512 + sf_at, sx[q] + 4 * s);
+          if (sx[q] != nullptr) {
+            cp_async4(sdst + to_b + off + q * 512, sx[q]);
+            sx[q] += 4;
+          }
+#pragma unroll
+        for (int q = 0; q < PASSES; ++q) {
+          if (q >= most) break;
+          if (q < passes) cp_async16(bdst + off + q * 2048, src[q]);
+          src[q] += KS;
+        }
         cp_arrive(&fullx[slot]);
-        if (++slot == S) slot = 0, ++round;
+        off += p.stage_bytes;
+        if (++slot == S) slot = 0, off = 0, ++round;
       }
     }
     cp_wait_all();
   } else if (warp == MMA_WARP) {
-    // ---------------- MMA issuer ----------------
-    if (lane == 0) {
-      int slot = 0, set = 0, seg = -1;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int64_t i = 0; i < n && ok;) {
-        const int64_t u = run.u0 + i;
-        const Tile t = tile_at(p, before, start, u / p.nst);
-        const int s0 = (int)(u % p.nst);
-        const int64_t len = p.nst - s0 < n - i ? p.nst - s0 : n - i;
-        i += len;
-        ++seg;
-        if (seg >= 2 && !mbar_wait(&accempty[seg & 1], (uint32_t)((seg / 2 - 1) & 1), abort_flag)) break;
+    // ---------------- MMA issuer: the whole warp, one lane of it elected ----------------
+    const uint64_t ad = sw128_kmajor_desc(ring), bd = sw128_kmajor_desc(ring + p.b_off);  // the slots' follow: address / 16
+    int slot = 0, set = 0, seg = -1;
+    uint64_t off = 0;
+    uint32_t phase = 0;  // of the scale set
+    bool ok = true, over = false;
+    for (int64_t i = 0; i < n && ok;) {
+      const int64_t u = run.u0 + i;
+      const Tile t = tile_at(p, before, start, u / p.nst);
+      const int s0 = (int)(u % p.nst);
+      const int len = (int)(p.nst - s0 < n - i ? p.nst - s0 : n - i);
+      i += len;
+      ++seg;
+      if (seg >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&accempty[seg & 1], (uint32_t)((seg / 2 - 1) & 1), abort_flag));
+      if (!ok) break;
+      const uint32_t acc = tmem + (uint32_t)(seg & 1) * R * p.acc_width;
+      const uint32_t idesc = p.idesc | ((uint32_t)(t.width >> 3) << 17);
+      for (int j = 0; j < len; ++j) {
+        if (!over) ok = __all_sync(0xffffffffu, mbar_wait(&sfready[set], phase, abort_flag));
+        if (!ok) break;
         tc_fence_after();
-        const uint32_t acc = tmem + (uint32_t)(seg & 1) * R * p.acc_width;
-        const uint32_t idesc = p.idesc | ((uint32_t)(t.width >> 3) << 17);
-        for (int64_t j = 0; j < len; ++j) {
-          ok = mbar_wait(&fullw[slot], phase, abort_flag) && mbar_wait(&fullx[slot], phase, abort_flag);
-          if (!ok) break;
-          fence_proxy_async_smem();  // cp.async wrote by the generic proxy, the tensor core reads by the other
-          tc_fence_after();
-          const uint8_t *st = ring + (size_t)slot * p.stage_bytes;
-          const uint32_t sf = tmem + p.sf_col + 12u * (uint32_t)set;
-          const uint32_t sfb = sf + 4u * R;
+        const uint32_t sf = tmem + p.sf_col + 12u * (uint32_t)set;
+        if (++set == SF_SETS) set = 0, phase ^= 1u;
+        over = __all_sync(0xffffffffu, mbar_over(&sfready[set], phase));  // asked for before the MMAs are issued
 #pragma unroll
-          for (int q = 0; q < R; ++q) sf_copy(sf + 4u * q, sf_desc(st + p.sfa_off + q * 512));
-          sf_copy(sfb, sf_desc(st + p.sfb_off));
-          if (R == 1 && t.width > 128) sf_copy(sfb + 4u, sf_desc(st + p.sfb_off + 512));
-          const uint64_t bd = sw128_kmajor_desc(st + p.b_off);
-#pragma unroll
-          for (int q = 0; q < R; ++q) {
-            const uint64_t ad = sw128_kmajor_desc(st + q * TM * KS);
-#pragma unroll
-            for (int k = 0; k < 4; ++k)  // K = 32 each: 32 bytes further along the rows, scale byte k
-              mx::mma_mx(acc + (uint32_t)q * p.acc_width, ad + (uint64_t)(2 * k), bd + (uint64_t)(2 * k),
-                         idesc | ((uint32_t)k << 4) | ((uint32_t)k << 29), (j | k) != 0 ? 1u : 0u,
-                         (sf + 4u * q) | ((uint32_t)k << 30), sfb | ((uint32_t)k << 30));
-          }
-          mma_commit(&empty[slot]);
-          if (++slot == S) slot = 0, phase ^= 1u;
-          if (++set == SF_SETS) set = 0;
-        }
-        if (ok) mma_commit(&accfull[seg & 1]);
+        for (int q = 0; q < R; ++q)
+          mma_stage(acc + (uint32_t)q * p.acc_width, ad + off + (uint64_t)(q * (TM * KS >> 4)), bd + off, idesc, (uint32_t)j, sf + 4u * q,
+                    sf + 4u * R);
+        commit(&empty[slot]);
+        off += p.stage_bytes >> 4;
+        if (++slot == S) slot = 0, off = 0;
       }
-      // every MMA issued has completed before the CTA frees its tensor memory
-      mma_commit(drain);
-      mbar_drain(drain, 0, 200000000ull);
+      if (ok) commit(&accfull[seg & 1]);
     }
+    // every MMA issued has completed before the CTA frees its tensor memory
+    commit(&drain[0]);
+    if (lane == 0) mbar_drain(&drain[0], 0, 200000000ull);
+    __syncwarp();
+  } else if (warp == SF_WARP) {
+    // ---------------- scales into tensor memory, once all of a stage has landed ----------------
+    const uint64_t da = sf_desc(ring + p.sfa_off), db = sf_desc(ring + p.sfb_off);
+    uint64_t off = 0;
+    int slot = 0, set = 0, back = 0;  // back: the slot of the stage SF_SETS before
+    uint32_t phase = 0, bphase = 0;
+    bool ok = true;
+    for (int64_t i = 0; i < n; ++i) {
+      const bool reuse = i >= SF_SETS;  // the MMAs that read the set are done
+      bool over = mbar_over(&fullx[slot], phase) & mbar_over(&fullw[slot], phase);
+      if (reuse) over = over & mbar_over(&empty[back], bphase);
+      if (!__all_sync(0xffffffffu, over)) {
+        ok = mbar_wait(&fullx[slot], phase, abort_flag) && mbar_wait(&fullw[slot], phase, abort_flag);
+        ok = __all_sync(0xffffffffu, ok && (!reuse || mbar_wait(&empty[back], bphase, abort_flag)));
+        if (!ok) break;
+      }
+      fence_proxy_async_smem();  // cp.async wrote by the generic proxy, the tensor core reads by the other
+      tc_fence_after();
+      const uint32_t sf = tmem + p.sf_col + 12u * (uint32_t)set;
+#pragma unroll
+      for (int q = 0; q < R; ++q) sf_copy(sf + 4u * q, da + off + 32u * q);
+      sf_copy(sf + 4u * R, db + off);
+      if (R == 1 && p.nt > 128) sf_copy(sf + 8u, db + off + 32u);
+      commit(&sfready[set]);
+      off += p.stage_bytes >> 4;
+      if (++slot == S) slot = 0, off = 0, phase ^= 1u;
+      if (++set == SF_SETS) set = 0;
+      if (reuse && ++back == S) back = 0, bphase ^= 1u;
+    }
+    // its copies have completed before the tensor memory is freed: the last MMAs followed them, but after a
+    // wait that ran out they may not have
+    commit(&drain[1]);
+    if (lane == 0) mbar_drain(&drain[1], 0, 200000000ull);
+    __syncwarp();
   } else if (warp < EPI_WARPS) {
     // ---------------- epilogue: weight row = tensor-memory lane, token = column ----------------
     const int quarter = warp & 3, group = warp >> 2;
@@ -563,7 +643,7 @@ static int32_t launch_t(const b200_packed_desc *w, const b200_scaled_args *a, cu
   p.sfb_off = p.sfa_off + R * 512;
   p.sfb_bytes = 1024;
   p.stage_bytes = (p.sfb_off + p.sfb_bytes + 1023) / 1024 * 1024;
-  const size_t tail = 8 * (3 * MAX_STAGES + 5) + 16 + 8 * ((size_t)p.experts + 1) + 16;
+  const size_t tail = 8 * (3 * MAX_STAGES + SF_SETS + 6) + 16 + 8 * ((size_t)p.experts + 1) + 16;
   int stages = (int)((SMEM_LIMIT - 1024 - tail) / p.stage_bytes);
   p.stages = stages < MAX_STAGES ? stages : MAX_STAGES;
   p.tx = (uint32_t)(R * TM * KS * bits / 8);  // codes as they lie in global memory
@@ -585,9 +665,16 @@ static int32_t launch_t(const b200_packed_desc *w, const b200_scaled_args *a, cu
   if (int32_t rc = make_tma_2d(&tmw, bits == 4 ? CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B : CU_TENSOR_MAP_DATA_TYPE_16U6_ALIGN16B,
                                w->data, (uint64_t)w->cols, (uint64_t)w->rows, row_bytes, KS, TM, CU_TENSOR_MAP_SWIZZLE_128B))
     return rc;
+  CUtensorMap tmx = tmw;
+  if (p.experts == 0) {  // rows of x side by side: whole tiles of them
+    p.tx += (uint32_t)(p.nt * KS);
+    if (int32_t rc = make_tma_2d(&tmx, CU_TENSOR_MAP_DATA_TYPE_UINT8, a->x, (uint64_t)w->cols, (uint64_t)a->rows, (uint64_t)w->cols, KS,
+                                 (uint32_t)p.nt, CU_TENSOR_MAP_SWIZZLE_128B))
+      return rc;
+  }
   const size_t smem = 1024 + (size_t)p.stages * p.stage_bytes + tail;
   B200_CUDA_TRY((ensure_dynamic_smem<scaled_kernel<R, OUT>>(SMEM_LIMIT)));
-  scaled_kernel<R, OUT><<<p.grid, THREADS, smem, stream>>>(tmw, p, ep);
+  scaled_kernel<R, OUT><<<p.grid, THREADS, smem, stream>>>(tmw, tmx, p, ep);
   B200_LAUNCH_CHECK();
   return B200_OK;
 }
