@@ -403,7 +403,7 @@ int32_t b200_scaled_values(const void *codes, const void *scales, int64_t rows, 
  * `per_pair`, and gives row p of y; rows of pairs that no expert has are zeros. bias is [experts,
  * rows] then, residual must be NULL. cols a multiple of 128 and weights on a 32-byte boundary run on
  * the tensor cores, other calls on a general kernel, for which `scratch` (b200_scaled_linear_scratch
- * bytes, 0 for the former) is needed. Workspace: 38 MiB per (device, stream) or capture. */
+ * bytes, 0 for the former) is needed. Workspace: 65 MiB per (device, stream) or capture. */
 #define B200_ACT_NONE 0
 #define B200_ACT_RELU 1
 #define B200_ACT_SILU 2

@@ -13,20 +13,23 @@
 //   warps 0-7    epilogue, two groups of four that take turns at 16 or 32 tokens: tcgen05.ld (lane = weight
 //                row, column = token), bias, activation, gate, residual; a warp's 32 rows are 32 neighbouring
 //                columns of y, a block of the 8-bit output, whose largest value is one warp-wide maximum
-//   warps 8-11   cp.async of x's codes (token rows found through the plan's order when there are experts)
-//                and of both sides' scale bytes, four of a row at a time, into the layout that
-//                tcgen05.cp takes; the copies themselves arrive at the stage's barrier when they land
-//   warp 13      waits for all of a stage, then tcgen05.cp of its scales into one of four sets of tensor-memory
-//                columns; commit announces the stage to warp 12
-//   warp 12      four MMAs a stage and accumulator; commit frees the stage and its set. (One warp for both
-//                took 0.5 us a stage: copies, waits and MMAs cost an issuing thread 25 to 45 ns each)
-//   warps 14-15  one thread each: TMA of the weight codes
+//   warps 8-9    cp.async of both sides' scale bytes, four of a row at a time, into the layout that
+//                tcgen05.cp takes, up to 12 stages ahead
+//   warp 13      tcgen05.cp of a stage's scales into one of four sets of tensor-memory columns; commit
+//                announces them to warp 12
+//   warps 10-11  through experts, cp.async of x's codes: token rows are found through the plan's order. The
+//                copies themselves arrive at the stage's barrier when they land
+//   warps 14-15  one thread each: TMA of the weight codes and, without experts, of x's
+//   warp 12      four MMAs a stage and accumulator; commit frees the stage and its set. (One warp for
+//                scales and MMAs took 0.5 us a stage: copies, waits and MMAs cost an issuing thread 25 to 45 ns each)
 // Two accumulators of a tile's width, so that the epilogue of one tile runs under the products of the
 // next: 2 x 224 columns, and four rotating sets of scale columns beside them.
 //
 // Work split: units are (tile, K stage), laid end to end over experts, weight rows and token tiles; each of
-// G CTAs takes an equal run of them, whatever the matrix or the routing, so that every SM streams as many
-// bytes as the others. The units of experts are counted on the device from the plan's offsets: a recorded
+// G CTAs takes an equal run of them, whatever the matrix or the routing, so that every SM works as long as
+// the others. CTAs so stand at different K, which L2 likes: with whole tiles handed out in turn, so that
+// neighbours read the same rows of x at the same time, 4096 tokens x 1024 x 16384 took 324 us, not 112, and
+// 128 tokens x 57344 x 8192 161, not 106. The units of experts are counted on the device from the plan's offsets: a recorded
 // launch fits every routing. A tile that a run's border cuts is finished by the last of its CTAs to arrive
 // (acquire-release ticket), which adds the fp32 parts in the order of the CTAs: the same bits every time.
 // No CTA waits for another. Every wait is bounded (sm100.cuh).
@@ -48,7 +51,9 @@ namespace scaled {
 
 constexpr int TM = 128, KS = 128;            // weight rows of an MMA, codes of a stage
 constexpr int EPI_WARPS = 8, LOAD_WARP0 = 8, LOAD_WARPS = 4, MMA_WARP = 12, SF_WARP = 13, W_WARP0 = 14, W_WARPS = 2;
-constexpr int THREADS = 16 * 32, LOADERS = LOAD_WARPS * 32;
+constexpr int THREADS = 16 * 32;
+constexpr int LOADERS = LOAD_WARPS / 2 * 32;  // threads that copy scales, and as many that copy x's codes
+constexpr int SLOTS = 12;                    // stages whose scales wait for tensor memory
 constexpr int ACC_COLS = 224;                // columns of an accumulator set: R * NT at most
 constexpr int SF_SETS = 4;
 constexpr int MAX_STAGES = 12;
@@ -62,16 +67,20 @@ struct Params {
   const int32_t *offsets, *order;
   int64_t rows, n;        // rows of y, weight rows of one matrix
   int64_t wrows;          // of all matrices
+  int64_t second;         // the tile's other weight rows: up rows of a gate's, or the next 128
   int64_t nblk;           // scale bytes of a row
   int64_t cols;
   int experts, fan, per_pair;
   int nst;                // K stages
-  int wtiles;             // tiles of weight rows of one matrix
+  int wtiles, tile_rows;  // tiles of weight rows of one matrix, columns of y in each
   int nt;                 // tokens of a tile, at most
   int grid, stages;
-  uint32_t stage_bytes, b_off, sfa_off, sfb_off, sfb_bytes;
+  int sets;               // of scale columns in turn: no more than stages, whose barriers guard them
+  uint32_t stage_bytes, b_off;        // weight codes, then x's
+  uint32_t scale_bytes, sfb_off;      // of a slot: weight scales, then x's
   uint32_t tx;
-  uint32_t acc_width, sf_col, tmem_cols;
+  int bufs;               // accumulators that take turns: 2, or 1 of twice the width
+  uint32_t acc_width, sf_col, sf_width, tmem_cols;
   uint32_t idesc;
   float *part;            // [grid][2][R][nt][128]
   unsigned int *tickets;  // [grid]: of the tile that the CTA's run ends in
@@ -170,19 +179,32 @@ __device__ __forceinline__ Tile tile_at(const Params &p, const int32_t *before, 
   const int w = (int)(at / tt), t = (int)(at - (int64_t)w * tt);
   Tile r;
   r.e = e;
-  r.w0 = (int64_t)w * TM;
+  r.w0 = (int64_t)w * p.tile_rows;
   r.first = first + (int64_t)t * per;
   r.rows = (int)(count - (int64_t)t * per < per ? count - (int64_t)t * per : per);
   r.width = (r.rows + 15) / 16 * 16;
   return r;
 }
 
-// The CTA's run of units and how it falls into tiles.
+// The CTA's run of units, of all that are shared out among `ctas`.
 struct Run {
   int64_t units, u0, u1;
-  int ctas;  // that have one
+  int ctas;
   __device__ __forceinline__ int64_t start(int64_t c) const { return c * units / ctas; }
 };
+struct Seg {
+  int64_t tile;
+  int s0, len;  // K stages
+};
+// The next part of a tile in the run; `u` goes through its units.
+__device__ __forceinline__ bool next_seg(const Params &p, const Run &run, int64_t &u, Seg &g) {
+  if (u >= run.u1) return false;
+  g.tile = u / p.nst;
+  g.s0 = (int)(u - g.tile * p.nst);
+  g.len = (int)(p.nst - g.s0 < run.u1 - u ? p.nst - g.s0 : run.u1 - u);
+  u += g.len;
+  return true;
+}
 
 template <typename T>
 __device__ __forceinline__ T to_out(float v) {
@@ -199,49 +221,50 @@ __device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[N]) {
   else tmem_ld_32x32b_x16(taddr, r);
 }
 
-// One weight row's products with CH tokens, column `c` of y (live: c is one): finished and stored. `at` is
-// the row of y of token j in lane j.
-template <int R, typename OUT, int CH>
-__device__ __forceinline__ void finish(const Epilogue &ep, float (&v)[R][CH], const float (&bias)[R], int c, bool live,
-                                       int at, int count) {
+// A gate of two products: the second one's values times the first one's, which the activation has been
+// applied to. `up` is not read without one.
+template <bool GATED, typename OUT, int CH>
+__device__ __forceinline__ void finish_column(const Epilogue &ep, float (&v)[CH], float bias, const float (&up)[CH], float up_bias, int c,
+                                              int at, int count) {
   const int lane = threadIdx.x & 31;
+  const bool live = c < ep.cols;
 #pragma unroll
-  for (int j = 0; j < CH; ++j) v[0][j] += bias[0];
+  for (int j = 0; j < CH; ++j) v[j] += bias;
   switch (ep.activation) {  // outside the loop: a column's functions run side by side
     case B200_ACT_RELU:
 #pragma unroll
-      for (int j = 0; j < CH; ++j) v[0][j] = activate<B200_ACT_RELU>(v[0][j]);
+      for (int j = 0; j < CH; ++j) v[j] = activate<B200_ACT_RELU>(v[j]);
       break;
     case B200_ACT_SILU:
 #pragma unroll
-      for (int j = 0; j < CH; ++j) v[0][j] = activate<B200_ACT_SILU>(v[0][j]);
+      for (int j = 0; j < CH; ++j) v[j] = activate<B200_ACT_SILU>(v[j]);
       break;
     case B200_ACT_GELU:
 #pragma unroll
-      for (int j = 0; j < CH; ++j) v[0][j] = activate<B200_ACT_GELU>(v[0][j]);
+      for (int j = 0; j < CH; ++j) v[j] = activate<B200_ACT_GELU>(v[j]);
       break;
     case B200_ACT_GELU_TANH:
 #pragma unroll
-      for (int j = 0; j < CH; ++j) v[0][j] = activate<B200_ACT_GELU_TANH>(v[0][j]);
+      for (int j = 0; j < CH; ++j) v[j] = activate<B200_ACT_GELU_TANH>(v[j]);
       break;
   }
-  if constexpr (R == 2) {
+  if constexpr (GATED) {
 #pragma unroll
-    for (int j = 0; j < CH; ++j) v[0][j] = __fmul_rn(v[0][j], v[1][j] + bias[1]);
+    for (int j = 0; j < CH; ++j) v[j] = __fmul_rn(v[j], up[j] + up_bias);
   }
   const int cols = (int)ep.cols;
   if (ep.residual != nullptr) {
 #pragma unroll
     for (int j = 0; j < CH; ++j) {
       const int row = __shfl_sync(0xffffffffu, at, j);
-      if (live && j < count) v[0][j] += load_as_f32(ep.residual, row * ep.rstride + c, ep.rdt);
+      if (live && j < count) v[j] += load_as_f32(ep.residual, row * ep.rstride + c, ep.rdt);
     }
   }
   if constexpr (std::is_same<OUT, E4M3>::value) {  // y's columns are whole blocks: a warp's are all live or none
     uint32_t top = 0;  // of token j in lane j, which finds the scale for all
 #pragma unroll
     for (int j = 0; j < CH; ++j) {
-      const uint32_t t = __reduce_max_sync(0xffffffffu, __float_as_uint(v[0][j]) & 0x7FFFFFFFu);
+      const uint32_t t = __reduce_max_sync(0xffffffffu, __float_as_uint(v[j]) & 0x7FFFFFFFu);
       if (lane == j) top = t;
     }
     const uint32_t byte = rows8::scale_byte(top);
@@ -251,27 +274,37 @@ __device__ __forceinline__ void finish(const Epilogue &ep, float (&v)[R][CH], co
     for (int j = 0; j < CH; ++j) {
       const int row = __shfl_sync(0xffffffffu, at, j);
       const float s = __shfl_sync(0xffffffffu, inv, j);
-      if (live && j < count) ((uint8_t *)ep.y)[(int64_t)row * cols + c] = (uint8_t)rows8::codes2(v[0][j], 0.f, s, s == 0.f);
+      if (live && j < count) ((uint8_t *)ep.y)[(int64_t)row * cols + c] = (uint8_t)rows8::codes2(v[j], 0.f, s, s == 0.f);
     }
   } else {
 #pragma unroll
     for (int j = 0; j < CH; ++j) {
       const int row = __shfl_sync(0xffffffffu, at, j);
-      if (live && j < count) ((OUT *)ep.y)[(int64_t)row * cols + c] = to_out<OUT>(v[0][j]);
+      if (live && j < count) ((OUT *)ep.y)[(int64_t)row * cols + c] = to_out<OUT>(v[j]);
     }
   }
 }
 
-template <int R, typename OUT>
+// Weight rows' products with CH tokens, column `c` of y and, with two accumulators and no gate, c + 128:
+// finished and stored. `at` is the row of y of token j in lane j.
+template <int R, bool GATED, typename OUT, int CH>
+__device__ __forceinline__ void finish(const Epilogue &ep, float (&v)[R][CH], const float (&bias)[R], int c, int at, int count) {
+  finish_column<GATED, OUT, CH>(ep, v[0], bias[0], v[R - 1], bias[R - 1], c, at, count);
+  if constexpr (R == 2 && !GATED) finish_column<false, OUT, CH>(ep, v[1], bias[1], v[1], 0.f, c + TM, at, count);
+}
+
+template <int R, bool GATED, typename OUT>
 __global__ void __launch_bounds__(THREADS, 1)
     scaled_kernel(const __grid_constant__ CUtensorMap tmw, const __grid_constant__ CUtensorMap tmx, const __grid_constant__ Params p, const __grid_constant__ Epilogue ep) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t *ring = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const int S = p.stages;
-  uint64_t *fullw = reinterpret_cast<uint64_t *>(ring + (size_t)S * p.stage_bytes);
+  uint8_t *scales = ring + (size_t)S * p.stage_bytes;
+  uint64_t *fullw = reinterpret_cast<uint64_t *>(scales + (size_t)SLOTS * p.scale_bytes);
   uint64_t *fullx = fullw + S;
   uint64_t *empty = fullx + S;
-  uint64_t *sfready = empty + S;
+  uint64_t *fulls = empty + S, *frees = fulls + SLOTS;  // scales landed, scales in tensor memory
+  uint64_t *sfready = frees + SLOTS;
   uint64_t *accfull = sfready + SF_SETS;
   uint64_t *accempty = accfull + 2;
   uint64_t *drain = accempty + 2;
@@ -288,6 +321,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(&fullx[s], LOADERS);
       mbar_init(&empty[s], 1);
     }
+    for (int b = 0; b < SLOTS; ++b) {
+      mbar_init(&fulls[b], LOADERS);
+      mbar_init(&frees[b], 1);
+    }
     for (int b = 0; b < SF_SETS; ++b) mbar_init(&sfready[b], 1);
     for (int b = 0; b < 2; ++b) {
       mbar_init(&accfull[b], 1);
@@ -299,6 +336,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     fence_mbar_init();
     prefetch_tmap(&tmw);
   }
+  // The next kernel's CTAs may start as this one's leave. The weights are no result of the kernel before: their
+  // first stages are asked for at once, everything else waits for it (through experts the plan, hence all).
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (p.experts > 0) asm volatile("griddepcontrol.wait;" ::: "memory");
   for (int e = threadIdx.x; e <= p.experts && p.experts > 0; e += THREADS) start[e] = p.offsets[e];
   if (warp == MMA_WARP) tmem_alloc(tmem_slot, p.tmem_cols);
   tc_fence_before();
@@ -323,35 +364,52 @@ __global__ void __launch_bounds__(THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   Run run;
-  run.units = (p.experts > 0 ? (int64_t)before[p.experts] : (int64_t)tiles_of(p, (int)p.rows)) * p.wtiles * p.nst;
-  run.ctas = (int)(run.units / MIN_UNITS < p.grid ? (run.units / MIN_UNITS < 1 ? 1 : run.units / MIN_UNITS) : p.grid);
-  run.u0 = (int)blockIdx.x < run.ctas ? run.start(blockIdx.x) : 0;
-  run.u1 = (int)blockIdx.x < run.ctas ? run.start(blockIdx.x + 1) : 0;
-  const int64_t n = run.u1 - run.u0;
+  {
+    run.units = (p.experts > 0 ? (int64_t)before[p.experts] : (int64_t)tiles_of(p, (int)p.rows)) * p.wtiles * p.nst;
+    const int64_t most = run.units / MIN_UNITS;
+    run.ctas = (int)(most < 1 ? 1 : most < p.grid ? most : p.grid);
+    run.u0 = (int)blockIdx.x < run.ctas ? run.start(blockIdx.x) : 0;
+    run.u1 = (int)blockIdx.x < run.ctas ? run.start(blockIdx.x + 1) : 0;
+  }
+  const int64_t n = run.u1 - run.u0;  // stages
 
   if (warp >= W_WARP0) {
     // ---------------- TMA of weight codes: warp w takes the stages i = w (mod W_WARPS) ----------------
     if (lane == 0) {
       const int turn = warp - W_WARP0, turns = S < W_WARPS ? S : W_WARPS;
-      int64_t i = turn, tile = (run.u0 + turn) / p.nst;
-      int s = (int)((run.u0 + turn) % p.nst);
-      int slot = turn;
+      int64_t i = turn, u = run.u0, row = 0, first = 0;
+      int s = turn, slot = turn;  // s: stages into the segment, behind its end until the next is taken
+      Seg g = {0, 0, 0};
       uint32_t round = 0;
-      int64_t row = 0, first = 0, known = -1;
+      int early_x[MAX_STAGES / W_WARPS + 1], early_row[MAX_STAGES / W_WARPS + 1], early_slot[MAX_STAGES / W_WARPS + 1], held = 0;
       for (; i < n && turn < turns; i += turns) {
-        if (tile != known) {
-          const Tile t = tile_at(p, before, start, tile);
+        while (s >= g.len) {
+          s -= g.len;
+          if (!next_seg(p, run, u, g)) break;
+          const Tile t = tile_at(p, before, start, g.tile);
           row = t.e * p.n + t.w0;
           first = t.first;
-          known = tile;
         }
         if (round > 0 && !mbar_wait(&empty[slot], (round - 1u) & 1u, abort_flag)) break;
         uint8_t *st = ring + (size_t)slot * p.stage_bytes;
         mbar_arrive_expect_tx(&fullw[slot], p.tx);
-        tma_load_2d(st, &tmw, s * KS, (int32_t)row, &fullw[slot]);
-        if constexpr (R == 2) tma_load_2d(st + TM * KS, &tmw, s * KS, (int32_t)(row + ep.cols), &fullw[slot]);
-        if (p.experts == 0) tma_load_2d(st + p.b_off, &tmx, s * KS, (int32_t)first, &fullw[slot]);
-        for (s += turns; s >= p.nst; s -= p.nst) ++tile;
+        const int x = (g.s0 + s) * KS;
+        tma_load_2d(st, &tmw, x, (int32_t)row, &fullw[slot]);
+        if constexpr (R == 2) tma_load_2d(st + TM * KS, &tmw, x, (int32_t)(row + p.second), &fullw[slot]);
+        if (p.experts == 0) {
+          if (round > 0) {
+            tma_load_2d(st + p.b_off, &tmx, x, (int32_t)first, &fullw[slot]);
+          } else {  // the ring's first round: x's boxes behind all the weights'
+            early_x[held] = x, early_row[held] = (int32_t)first, early_slot[held] = slot;
+            ++held;
+            if (i + turns >= n || slot + turns >= S) {
+              asm volatile("griddepcontrol.wait;" ::: "memory");
+              for (int q = 0; q < held; ++q)
+                tma_load_2d(ring + (size_t)early_slot[q] * p.stage_bytes + p.b_off, &tmx, early_x[q], early_row[q], &fullw[early_slot[q]]);
+            }
+          }
+        }
+        s += turns;
         if ((slot += turns) >= S) slot -= S, ++round;
       }
       if (*abort_flag) {  // this thread's copies in flight land before the CTA exits
@@ -360,68 +418,86 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     }
   } else if (warp >= LOAD_WARP0 && warp < LOAD_WARP0 + LOAD_WARPS) {
-    // ---------------- cp.async of all scale bytes and, through experts, of x's codes ----------------
     // A stage is worth some 450 cycles, and one warp's dependent instructions take 4 to 6 each: pointers are
     // kept and moved on, so that a copy is one instruction.
-    const int th = threadIdx.x - LOAD_WARP0 * 32;
-    const int chunk = th & 7, r0 = th >> 3;  // 16 bytes of a row's 128; rows r0, r0 + 16, ... (r & 7 the same in all)
-    constexpr int PASSES = ACC_COLS / R / 16;
-    const uint32_t base = smem_u32(ring);
-    const uint32_t bdst = base + p.b_off + (uint32_t)(r0 * 128 + ((chunk ^ (r0 & 7)) << 4));
-    const uint32_t sdst = base + p.sfa_off + (uint32_t)((th & 31) * 16 + (th >> 5) * 4);
-    const uint32_t to_b = p.sfb_off - p.sfa_off;
-    int slot = 0;
-    uint32_t round = 0, off = 0;
+    const int th = (threadIdx.x - LOAD_WARP0 * 32) & (LOADERS - 1);
+    auto xrow = [&](const Tile &t, int r) -> int64_t {  // row of x
+      const int64_t at = t.first + r;
+      if (p.experts == 0) return at;
+      const int32_t pair = p.order[at];
+      return p.per_pair ? pair : pair / p.fan;
+    };
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     bool ok = true;
-    for (int64_t i = 0; i < n && ok;) {
-      const int64_t u = run.u0 + i;
-      const Tile t = tile_at(p, before, start, u / p.nst);
-      const int s = (int)(u % p.nst);
-      const int len = (int)(p.nst - s < n - i ? p.nst - s : n - i);
-      i += len;
-      auto xrow = [&](int r) -> int64_t {  // row of x
-        const int64_t at = t.first + r;
-        if (p.experts == 0) return at;
-        const int32_t pair = p.order[at];
-        return p.per_pair ? pair : pair / p.fan;
-      };
-      const uint8_t *src[PASSES], *sx[2], *sw[R];
-      const int passes = p.experts > 0 ? (t.rows - r0 + 15) / 16 : 0;  // this thread's; the warp's most are the tile's
-      const int most = p.experts > 0 ? (t.rows + 15) / 16 : 0;
+    uint32_t round = 0, off = 0;
+    int slot = 0;
+    int64_t u = run.u0;
+    Seg g;
+    if (warp < LOAD_WARP0 + LOAD_WARPS / 2) {
+      // ---------------- cp.async of scale bytes ----------------
+      constexpr int WR = R * TM / LOADERS, XR = (ACC_COLS + LOADERS - 1) / LOADERS;  // rows a thread
+      const uint32_t base = smem_u32(scales), to_b = p.sfb_off;
+      // row r's place in its atom: (r % 32) * 16 + (r / 32) * 4; an atom is 128 rows
+      auto place = [&](int r) -> uint32_t { return (uint32_t)((r >> 7) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4); };
+      while (ok && next_seg(p, run, u, g)) {
+        const Tile t = tile_at(p, before, start, g.tile);
+        const int s = g.s0, len = g.len;
+        const uint8_t *sw[WR], *sx[XR];
 #pragma unroll
-      for (int q = 0; q < PASSES; ++q)
-        src[q] = q < passes ? p.x + xrow(r0 + 16 * q) * p.cols + (int64_t)s * KS + chunk * 16 : p.x;
-#pragma unroll
-      for (int q = 0; q < 2; ++q) sx[q] = th + 128 * q < t.rows ? p.xs + xrow(th + 128 * q) * p.nblk + 4 * s : nullptr;
-#pragma unroll
-      for (int q = 0; q < R; ++q) {
-        int64_t wrow = t.e * p.n + q * ep.cols + t.w0 + th;
-        if (wrow >= p.wrows) wrow = p.wrows - 1;  // rows behind the last: not stored
-        sw[q] = p.ws + wrow * p.nblk + 4 * s;
-      }
-      for (int j = 0; j < len; ++j) {
-        if (round > 0) ok = __all_sync(0xffffffffu, mbar_wait(&empty[slot], (round - 1u) & 1u, abort_flag));
-        if (!ok) break;
-#pragma unroll
-        for (int q = 0; q < R; ++q) {
-          cp_async4(sdst + off + q * 512, sw[q]);
-          sw[q] += 4;
+        for (int q = 0; q < WR; ++q) {
+          const int r = th + q * LOADERS;
+          int64_t wrow = t.e * p.n + (r >> 7) * p.second + t.w0 + (r & 127);
+          if (wrow >= p.wrows) wrow = p.wrows - 1;  // rows behind the last: not stored
+          sw[q] = p.ws + wrow * p.nblk + 4 * s;
         }
+        const int mine = (t.rows - th + LOADERS - 1) / LOADERS, most = (t.rows + LOADERS - 1) / LOADERS;
 #pragma unroll
-        for (int q = 0; q < 2; ++q)
-          if (sx[q] != nullptr) {
-            cp_async4(sdst + to_b + off + q * 512, sx[q]);
-            sx[q] += 4;
+        for (int q = 0; q < XR; ++q) sx[q] = q < mine ? p.xs + xrow(t, th + q * LOADERS) * p.nblk + 4 * s : p.xs;
+        for (int j = 0; j < len; ++j) {
+          if (round > 0) ok = __all_sync(0xffffffffu, mbar_wait(&frees[slot], (round - 1u) & 1u, abort_flag));
+          if (!ok) break;
+#pragma unroll
+          for (int q = 0; q < WR; ++q) {
+            cp_async4(base + off + place(th + q * LOADERS), sw[q]);
+            sw[q] += 4;
           }
 #pragma unroll
-        for (int q = 0; q < PASSES; ++q) {
-          if (q >= most) break;
-          if (q < passes) cp_async16(bdst + off + q * 2048, src[q]);
-          src[q] += KS;
+          for (int q = 0; q < XR; ++q) {
+            if (q >= most) break;
+            if (q < mine) cp_async4(base + off + to_b + place(th + q * LOADERS), sx[q]);
+            sx[q] += 4;
+          }
+          cp_arrive(&fulls[slot]);
+          off += p.scale_bytes;
+          if (++slot == SLOTS) slot = 0, off = 0, ++round;
         }
-        cp_arrive(&fullx[slot]);
-        off += p.stage_bytes;
-        if (++slot == S) slot = 0, off = 0, ++round;
+      }
+    } else if (p.experts > 0) {
+      // ---------------- cp.async of x's codes ----------------
+      const int chunk = th & 7, r0 = th >> 3;  // 16 bytes of a row's 128; rows r0, r0 + 8, ... (r & 7 the same in all)
+      constexpr int STEP = LOADERS / 8, PASSES = ACC_COLS / STEP;
+      const uint32_t dst = smem_u32(ring) + p.b_off + (uint32_t)(r0 * 128 + ((chunk ^ (r0 & 7)) << 4));
+      while (ok && next_seg(p, run, u, g)) {
+        const Tile t = tile_at(p, before, start, g.tile);
+        const int s = g.s0, len = g.len;
+        const int mine = (t.rows - r0 + STEP - 1) / STEP, most = (t.rows + STEP - 1) / STEP;
+        const uint8_t *src[PASSES];
+#pragma unroll
+        for (int q = 0; q < PASSES; ++q)
+          src[q] = q < mine ? p.x + xrow(t, r0 + STEP * q) * p.cols + (int64_t)s * KS + chunk * 16 : p.x;
+        for (int j = 0; j < len; ++j) {
+          if (round > 0) ok = __all_sync(0xffffffffu, mbar_wait(&empty[slot], (round - 1u) & 1u, abort_flag));
+          if (!ok) break;
+#pragma unroll
+          for (int q = 0; q < PASSES; ++q) {
+            if (q >= most) break;
+            if (q < mine) cp_async16(dst + off + q * STEP * 128, src[q]);
+            src[q] += KS;
+          }
+          cp_arrive(&fullx[slot]);
+          off += p.stage_bytes;
+          if (++slot == S) slot = 0, off = 0, ++round;
+        }
       }
     }
     cp_wait_all();
@@ -430,67 +506,78 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint64_t ad = sw128_kmajor_desc(ring), bd = sw128_kmajor_desc(ring + p.b_off);  // the slots' follow: address / 16
     int slot = 0, set = 0, seg = -1;
     uint64_t off = 0;
-    uint32_t phase = 0;  // of the scale set
+    uint32_t phase = 0, sphase = 0;  // of the scale set, of the stage
     bool ok = true, over = false;
-    for (int64_t i = 0; i < n && ok;) {
-      const int64_t u = run.u0 + i;
-      const Tile t = tile_at(p, before, start, u / p.nst);
-      const int s0 = (int)(u % p.nst);
-      const int len = (int)(p.nst - s0 < n - i ? p.nst - s0 : n - i);
-      i += len;
+    int64_t u = run.u0;
+    Seg g;
+    while (ok && next_seg(p, run, u, g)) {
+      const Tile t = tile_at(p, before, start, g.tile);
+      const int len = g.len;
       ++seg;
-      if (seg >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&accempty[seg & 1], (uint32_t)((seg / 2 - 1) & 1), abort_flag));
+      const int buf = p.bufs == 2 ? seg & 1 : 0;
+      const uint32_t turn = (uint32_t)(p.bufs == 2 ? seg >> 1 : seg);  // uses of the accumulator before
+      if (turn > 0) ok = __all_sync(0xffffffffu, mbar_wait(&accempty[buf], (turn - 1u) & 1u, abort_flag));
       if (!ok) break;
-      const uint32_t acc = tmem + (uint32_t)(seg & 1) * R * p.acc_width;
+      tc_fence_after();
+      const uint32_t acc = tmem + (uint32_t)buf * R * p.acc_width;
       const uint32_t idesc = p.idesc | ((uint32_t)(t.width >> 3) << 17);
       for (int j = 0; j < len; ++j) {
-        if (!over) ok = __all_sync(0xffffffffu, mbar_wait(&sfready[set], phase, abort_flag));
+        if (!over) {
+          ok = mbar_wait(&sfready[set], phase, abort_flag) && mbar_wait(&fullw[slot], sphase, abort_flag);
+          ok = __all_sync(0xffffffffu, ok && (p.experts == 0 || mbar_wait(&fullx[slot], sphase, abort_flag)));
+        }
         if (!ok) break;
+        if (p.experts > 0) fence_proxy_async_smem();  // cp.async wrote by the generic proxy, the tensor core reads by the other
         tc_fence_after();
-        const uint32_t sf = tmem + p.sf_col + 12u * (uint32_t)set;
-        if (++set == SF_SETS) set = 0, phase ^= 1u;
-        over = __all_sync(0xffffffffu, mbar_over(&sfready[set], phase));  // asked for before the MMAs are issued
+        const uint32_t sf = tmem + p.sf_col + p.sf_width * (uint32_t)set;
+        if (++set == p.sets) set = 0, phase ^= 1u;
+        const int now = slot;
+        if (++slot == S) slot = 0, sphase ^= 1u;
+        // the next stage is asked for before this one's MMAs are issued
+        over = mbar_over(&sfready[set], phase) & mbar_over(&fullw[slot], sphase);
+        if (p.experts > 0) over = over & mbar_over(&fullx[slot], sphase);
+        over = __all_sync(0xffffffffu, over);
 #pragma unroll
         for (int q = 0; q < R; ++q)
           mma_stage(acc + (uint32_t)q * p.acc_width, ad + off + (uint64_t)(q * (TM * KS >> 4)), bd + off, idesc, (uint32_t)j, sf + 4u * q,
                     sf + 4u * R);
-        commit(&empty[slot]);
-        off += p.stage_bytes >> 4;
-        if (++slot == S) slot = 0, off = 0;
+        commit(&empty[now]);
+        off = slot == 0 ? 0 : off + (p.stage_bytes >> 4);
       }
-      if (ok) commit(&accfull[seg & 1]);
+      if (ok) commit(&accfull[buf]);
     }
     // every MMA issued has completed before the CTA frees its tensor memory
     commit(&drain[0]);
     if (lane == 0) mbar_drain(&drain[0], 0, 200000000ull);
     __syncwarp();
   } else if (warp == SF_WARP) {
-    // ---------------- scales into tensor memory, once all of a stage has landed ----------------
-    const uint64_t da = sf_desc(ring + p.sfa_off), db = sf_desc(ring + p.sfb_off);
+    // ---------------- scales into tensor memory ----------------
+    const uint64_t da = sf_desc(scales), db = sf_desc(scales + p.sfb_off);
     uint64_t off = 0;
-    int slot = 0, set = 0, back = 0;  // back: the slot of the stage SF_SETS before
+    int slot = 0, set = 0, back = 0;  // back: the ring slot of the stage p.sets before, whose MMAs read the set
     uint32_t phase = 0, bphase = 0;
     bool ok = true;
     for (int64_t i = 0; i < n; ++i) {
-      const bool reuse = i >= SF_SETS;  // the MMAs that read the set are done
-      bool over = mbar_over(&fullx[slot], phase) & mbar_over(&fullw[slot], phase);
+      const bool reuse = i >= p.sets;
+      bool over = mbar_over(&fulls[slot], phase);
       if (reuse) over = over & mbar_over(&empty[back], bphase);
       if (!__all_sync(0xffffffffu, over)) {
-        ok = mbar_wait(&fullx[slot], phase, abort_flag) && mbar_wait(&fullw[slot], phase, abort_flag);
-        ok = __all_sync(0xffffffffu, ok && (!reuse || mbar_wait(&empty[back], bphase, abort_flag)));
+        ok = mbar_wait(&fulls[slot], phase, abort_flag) && (!reuse || mbar_wait(&empty[back], bphase, abort_flag));
+        ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
       }
-      fence_proxy_async_smem();  // cp.async wrote by the generic proxy, the tensor core reads by the other
+      fence_proxy_async_smem();  // as the MMA warp's
       tc_fence_after();
-      const uint32_t sf = tmem + p.sf_col + 12u * (uint32_t)set;
+      const uint32_t sf = tmem + p.sf_col + p.sf_width * (uint32_t)set;
 #pragma unroll
       for (int q = 0; q < R; ++q) sf_copy(sf + 4u * q, da + off + 32u * q);
       sf_copy(sf + 4u * R, db + off);
-      if (R == 1 && p.nt > 128) sf_copy(sf + 8u, db + off + 32u);
+      if (p.nt > 128) sf_copy(sf + 4u * R + 4u, db + off + 32u);
       commit(&sfready[set]);
-      off += p.stage_bytes >> 4;
-      if (++slot == S) slot = 0, off = 0, phase ^= 1u;
-      if (++set == SF_SETS) set = 0;
+      commit(&frees[slot]);
+      off += p.scale_bytes >> 4;
+      if (++slot == SLOTS) slot = 0, off = 0, phase ^= 1u;
+      if (++set == p.sets) set = 0;
       if (reuse && ++back == S) back = 0, bphase ^= 1u;
     }
     // its copies have completed before the tensor memory is freed: the last MMAs followed them, but after a
@@ -500,35 +587,37 @@ __global__ void __launch_bounds__(THREADS, 1)
     __syncwarp();
   } else if (warp < EPI_WARPS) {
     // ---------------- epilogue: weight row = tensor-memory lane, token = column ----------------
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // bias, y, parts and tickets
     const int quarter = warp & 3, group = warp >> 2;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     constexpr int CH = R == 2 ? 16 : 32;  // tokens at a time: R * CH accumulators in registers
     bool ok = true;  // this warp's waits; after one that ran out it still meets the others
     int seg = 0;
-    for (int64_t i = 0; i < n; ++seg) {
-      const int64_t u = run.u0 + i, tile = u / p.nst;
-      const int s0 = (int)(u % p.nst);
-      const int64_t len = p.nst - s0 < n - i ? p.nst - s0 : n - i;
-      const bool whole = s0 == 0 && len == p.nst;
-      const Tile t = tile_at(p, before, start, tile);
-      const int c = (int)t.w0 + quarter * 32 + lane;  // column of y
-      const bool live = c < ep.cols;
+    int64_t u = run.u0;
+    Seg g;
+    for (; next_seg(p, run, u, g); ++seg) {
+      const bool whole = g.len == p.nst;
+      const Tile t = tile_at(p, before, start, g.tile);
+      const int c = (int)t.w0 + quarter * 32 + lane;  // column of y; ungated, the second accumulator's is c + 128
       float bias[R];
 #pragma unroll
-      for (int q = 0; q < R; ++q)
-        bias[q] = ep.bias != nullptr && live ? load_as_f32(ep.bias, t.e * p.n + q * ep.cols + c, ep.bdt) : 0.f;
+      for (int q = 0; q < R; ++q) {
+        const int64_t row = q * p.second + c;
+        bias[q] = ep.bias != nullptr && row < p.n ? load_as_f32(ep.bias, t.e * p.n + row, ep.bdt) : 0.f;
+      }
       auto row_of = [&](int j0, int count) -> int {  // of y, of token j0 + lane
         const int64_t at = t.first + j0 + (lane < count ? lane : 0);
         return p.experts > 0 ? p.order[at] : (int)at;
       };
-      ok = __all_sync(0xffffffffu, ok && mbar_wait(&accfull[seg & 1], (uint32_t)((seg / 2) & 1), abort_flag));
+      const int buf = p.bufs == 2 ? seg & 1 : 0;
+      ok = __all_sync(0xffffffffu, ok && mbar_wait(&accfull[buf], (uint32_t)((p.bufs == 2 ? seg >> 1 : seg) & 1), abort_flag));
       tc_fence_after();
-      const uint32_t acc = tmem + lane_base + (uint32_t)(seg & 1) * R * p.acc_width;
-      // partial sums: of the CTA's first tile in place 0, of its last in place 1
+      const uint32_t acc = tmem + lane_base + (uint32_t)buf * R * p.acc_width;
+      // partial sums: of the first of the CTA's shared tiles in place 0, of the last in place 1
       const size_t place = (size_t)R * p.nt * TM;
-      float *mine = p.part + ((size_t)blockIdx.x * 2 + (i == 0 ? 0 : 1)) * place + quarter * 32 + lane;
+      float *mine = p.part + ((size_t)blockIdx.x * 2 + (u - g.len == run.u0 ? 0 : 1)) * place + quarter * 32 + lane;
       const int last = (t.rows - 1) / CH;  // chunk; the groups take turns
-      if (group > last && lane == 0) mbar_arrive(&accempty[seg & 1]);
+      if (group > last && lane == 0) mbar_arrive(&accempty[buf]);
       for (int ch = group; ch <= last; ch += 2) {
         const int j0 = ch * CH, count = t.rows - j0 < CH ? t.rows - j0 : CH;
         float v[R][CH];
@@ -538,11 +627,11 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (ch + 2 > last) {  // the group's last columns are read: the accumulator may be used again
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&accempty[seg & 1]);
+          if (lane == 0) mbar_arrive(&accempty[buf]);
         }
         if (!ok) continue;
         if (whole) {
-          finish<R, OUT, CH>(ep, v, bias, c, live, row_of(j0, count), count);
+          finish<R, GATED, OUT, CH>(ep, v, bias, c, row_of(j0, count), count);
         } else {
 #pragma unroll
           for (int q = 0; q < R; ++q)
@@ -553,7 +642,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       if (!whole) {
         // the CTAs whose runs hold the tile's first and last unit; the tile's ticket is the first one's
-        const int64_t a = tile * p.nst, b = a + p.nst - 1;
+        const int64_t tile = g.tile, a = tile * p.nst, b = a + p.nst - 1;
         int cf = (int)(a * run.ctas / run.units), cl = (int)(b * run.ctas / run.units);
         while (cf > 0 && run.start(cf) > a) --cf;
         while (cf + 1 < run.ctas && run.start(cf + 1) <= a) ++cf;
@@ -584,13 +673,12 @@ __global__ void __launch_bounds__(THREADS, 1)
                 for (int j = 0; j < CH; ++j)
                   if (j < count) v[q][j] += __ldcg(src + ((size_t)q * p.nt + j0 + j) * TM);
             }
-            finish<R, OUT, CH>(ep, v, bias, c, live, row_of(j0, count), count);
+            finish<R, GATED, OUT, CH>(ep, v, bias, c, row_of(j0, count), count);
           }
           if (threadIdx.x == 0) p.tickets[cf] = 0u;  // ready for the next call
         }
         epi_sync();
       }
-      i += len;
     }
     // rows of pairs that no expert has are zeros
     if (p.experts > 0) {
@@ -614,8 +702,18 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (warp == MMA_WARP) tmem_dealloc(tmem, p.tmem_cols);
 }
 
-template <int R, typename OUT>
-static int32_t launch_t(const b200_packed_desc *w, const b200_scaled_args *a, cudaStream_t stream) {
+// Rows that meet one matrix: all, or an expert's share.
+static int64_t rows_of_one(const b200_scaled_args *a) {
+  return a->experts > 0 ? (a->rows + a->experts - 1) / a->experts : a->rows;
+}
+// Gated, 113 to 224 tokens: accumulators of twice the width that do not take turns, so that the weights
+// are read once (200 tokens x 57344 x 8192 146 us, with two tiles of tokens 155).
+static bool single(const b200_scaled_args *a) {
+  return a->experts == 0 && a->rows > ACC_COLS / 2 && a->rows <= ACC_COLS;
+}
+
+template <int R, bool GATED, typename OUT>
+static int32_t launch_t(const b200_packed_desc *w, const b200_scaled_args *a, int bufs, cudaStream_t stream) {
   int sms = 0;
   B200_CUDA_TRY(device_sms(&sms));
   const int bits = fmt_bits(w->format);
@@ -631,30 +729,39 @@ static int32_t launch_t(const b200_packed_desc *w, const b200_scaled_args *a, cu
   p.experts = (int)a->experts, p.fan = a->experts > 0 ? a->fan : 1, p.per_pair = a->per_pair;
   p.nst = (int)(w->cols / KS);
   const Epilogue ep = epilogue_of(w, a);
-  p.wtiles = (int)((ep.cols + TM - 1) / TM);
-  // tokens of a tile: no more than an expert can have, equally full tiles
-  const int64_t most = a->experts > 0 ? (a->rows + a->fan - 1) / a->fan : a->rows;
-  const int64_t limit = ACC_COLS / R;
+  p.second = GATED ? ep.cols : TM;
+  p.tile_rows = R == 2 && !GATED ? 2 * TM : TM;
+  p.wtiles = (int)((ep.cols + p.tile_rows - 1) / p.tile_rows);
+  p.bufs = bufs;
+  // tokens of a tile: equally full tiles; an expert's are as many as three times its share, in reason (fewer
+  // leave room for more stages, and who has more takes several tiles)
+  const int64_t limit = bufs == 2 ? ACC_COLS / R : ACC_COLS;
+  int64_t most = a->rows;
+  if (a->experts > 0) {
+    const int64_t tokens = (a->rows + a->fan - 1) / a->fan, share = 3 * rows_of_one(a);
+    most = share < 32 ? 32 : share;
+    most = most < tokens ? most : tokens;
+  }
   const int64_t tt = (most + limit - 1) / limit;
-  p.nt = (int)(((most + tt - 1) / tt + 15) / 16 * 16);
-  if (a->experts > 0 && tt > 1) p.nt = (int)limit;
+  p.nt = a->experts > 0 && tt > 1 ? (int)limit : (int)(((most + tt - 1) / tt + 15) / 16 * 16);
   p.b_off = (uint32_t)(R * TM * KS);
-  p.sfa_off = p.b_off + (uint32_t)((p.nt * KS + 1023) / 1024 * 1024);
-  p.sfb_off = p.sfa_off + R * 512;
-  p.sfb_bytes = 1024;
-  p.stage_bytes = (p.sfb_off + p.sfb_bytes + 1023) / 1024 * 1024;
-  const size_t tail = 8 * (3 * MAX_STAGES + SF_SETS + 6) + 16 + 8 * ((size_t)p.experts + 1) + 16;
-  int stages = (int)((SMEM_LIMIT - 1024 - tail) / p.stage_bytes);
+  p.stage_bytes = p.b_off + (uint32_t)((p.nt * KS + 1023) / 1024 * 1024);
+  p.sfb_off = R * 512;
+  p.scale_bytes = p.sfb_off + (p.nt > 128 ? 1024 : 512);
+  const size_t tail = 8 * (3 * MAX_STAGES + 2 * SLOTS + SF_SETS + 6) + 16 + 8 * ((size_t)p.experts + 1) + 16;
+  int stages = (int)((SMEM_LIMIT - 1024 - tail - SLOTS * p.scale_bytes) / p.stage_bytes);
   p.stages = stages < MAX_STAGES ? stages : MAX_STAGES;
+  p.sets = p.stages < SF_SETS ? p.stages : SF_SETS;
   p.tx = (uint32_t)(R * TM * KS * bits / 8);  // codes as they lie in global memory
   p.acc_width = (uint32_t)p.nt;
-  p.sf_col = 2 * R * p.acc_width;
+  p.sf_col = (uint32_t)bufs * R * p.acc_width;
+  p.sf_width = 4 * R + (p.nt > 128 ? 8 : 4);
   p.tmem_cols = 32;
-  while (p.tmem_cols < p.sf_col + 12 * SF_SETS) p.tmem_cols *= 2;
+  while (p.tmem_cols < p.sf_col + p.sf_width * SF_SETS) p.tmem_cols *= 2;
   const uint32_t fmt = w->format == B200_FMT_FP4_E2M1 ? 5u : w->format == B200_FMT_FP6_E2M3 ? 3u : 4u;
   p.idesc = (fmt << 7) | (0u << 10) | (1u << 23) | ((uint32_t)(TM >> 4) << 24);  // B: E4M3; E8M0 scales
   p.grid = sms;
-  const size_t part = (size_t)sms * 2 * ACC_COLS * TM * sizeof(float);
+  const size_t part = (size_t)sms * 2 * 2 * ACC_COLS * TM * sizeof(float);
   uint8_t *base = nullptr;
   if (int32_t rc = workspace_of(WS_SCALED, part, TICKETS * sizeof(unsigned int), stream, &base)) return rc;
   p.part = reinterpret_cast<float *>(base);
@@ -672,20 +779,29 @@ static int32_t launch_t(const b200_packed_desc *w, const b200_scaled_args *a, cu
                                  (uint32_t)p.nt, CU_TENSOR_MAP_SWIZZLE_128B))
       return rc;
   }
-  const size_t smem = 1024 + (size_t)p.stages * p.stage_bytes + tail;
-  B200_CUDA_TRY((ensure_dynamic_smem<scaled_kernel<R, OUT>>(SMEM_LIMIT)));
-  scaled_kernel<R, OUT><<<p.grid, THREADS, smem, stream>>>(tmw, tmx, p, ep);
-  B200_LAUNCH_CHECK();
+  const size_t smem = 1024 + (size_t)p.stages * p.stage_bytes + SLOTS * p.scale_bytes + tail;
+  B200_CUDA_TRY((ensure_dynamic_smem<scaled_kernel<R, GATED, OUT>>(SMEM_LIMIT)));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)p.grid);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  B200_CUDA_TRY(cudaLaunchKernelEx(&cfg, scaled_kernel<R, GATED, OUT>, tmw, tmx, p, ep));
   return B200_OK;
 }
 
-template <int R>
-static int32_t dispatch(const b200_packed_desc *w, const b200_scaled_args *a, cudaStream_t stream) {
+template <int R, bool GATED>
+static int32_t dispatch(const b200_packed_desc *w, const b200_scaled_args *a, int bufs, cudaStream_t stream) {
   switch (a->y_dtype) {
-    case B200_DT_F16: return launch_t<R, __half>(w, a, stream);
-    case B200_DT_BF16: return launch_t<R, __nv_bfloat16>(w, a, stream);
-    case B200_DT_F32: return launch_t<R, float>(w, a, stream);
-    default: return launch_t<R, E4M3>(w, a, stream);
+    case B200_DT_F16: return launch_t<R, GATED, __half>(w, a, bufs, stream);
+    case B200_DT_BF16: return launch_t<R, GATED, __nv_bfloat16>(w, a, bufs, stream);
+    case B200_DT_F32: return launch_t<R, GATED, float>(w, a, bufs, stream);
+    default: return launch_t<R, GATED, E4M3>(w, a, bufs, stream);
   }
 }
 
@@ -700,7 +816,13 @@ bool scaled_mma_takes(const b200_packed_desc *w, const b200_scaled_args *a) {
 }
 
 int32_t launch_scaled_mma(const b200_packed_desc *w, const b200_scaled_args *a, cudaStream_t stream) {
-  return a->gated ? scaled::dispatch<2>(w, a, stream) : scaled::dispatch<1>(w, a, stream);
+  // Two accumulators of 112 tokens halve a decode step's stages (57344 x 8192, us: one token 66.1 / 56.1, 33 tokens
+  // 76.8 / 70.5) and load less for many (4096 x 1024 x 16384 113 / 88); between, one of 224 reads the weights once
+  // (128 tokens 110 / 133, 200 tokens 152 / 156, 300 tokens 209 / 220).
+  const int64_t rows = scaled::rows_of_one(a);
+  if (a->gated) return scaled::dispatch<2, true>(w, a, scaled::single(a) ? 1 : 2, stream);
+  if (rows <= scaled::ACC_COLS / 2 || rows > 2 * scaled::ACC_COLS) return scaled::dispatch<2, false>(w, a, 2, stream);
+  return scaled::dispatch<1, false>(w, a, 2, stream);
 }
 
 }  // namespace b200
