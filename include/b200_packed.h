@@ -399,11 +399,18 @@ int32_t b200_scaled_values(const void *codes, const void *scales, int64_t rows, 
  *   be a multiple of 32).
  * With `experts` > 0 the weights are `experts` matrices of w->rows / experts rows each, and rows of x
  * go through them by a plan (b200_expert_plan): pair p = token * fan + j, in the order `order`, those
- * of expert e at offsets[e] .. offsets[e + 1]. A pair reads row p / fan of x, or row p when
- * `per_pair`, and gives row p of y; rows of pairs that no expert has are zeros. bias is [experts,
- * rows] then, residual must be NULL. cols a multiple of 128 and weights on a 32-byte boundary run on
- * the tensor cores, other calls on a general kernel, for which `scratch` (b200_scaled_linear_scratch
- * bytes, 0 for the former) is needed. Workspace: 65 MiB per (device, stream) or capture. */
+ * of expert e at offsets[e] .. offsets[e + 1]. x_rows says what x's rows are: tokens (a pair reads row
+ * p / fan), pairs (row p), or places of the plan; y_rows, whether y's are pairs (those of pairs that no
+ * expert has are zeros) or places of the plan (those behind offsets[experts] are not written). bias is
+ * [experts, rows] then, residual must be NULL. cols a multiple of 128 and weights on a 32-byte boundary
+ * run on the tensor cores, other calls on a general kernel. `scratch`: b200_scaled_linear_scratch bytes,
+ * for the general kernel's sums, or rows of x in the plan's order. Workspace: 65 MiB per (device,
+ * stream) or capture. The kernels may start while the one before them ends (programmatic dependent
+ * launch): they read weights and their scales at once, so no kernel that is launched to start others
+ * early may write these. */
+#define B200_ROWS_TOKENS 0
+#define B200_ROWS_PAIRS 1
+#define B200_ROWS_PLAN 2
 #define B200_ACT_NONE 0
 #define B200_ACT_RELU 1
 #define B200_ACT_SILU 2
@@ -421,10 +428,12 @@ typedef struct b200_scaled_args {
   const int32_t *offsets; /* [experts + 1]                                                 */
   const int32_t *order;   /* [rows]                                                        */
   int64_t experts;        /* 0: one matrix for all rows                                    */
-  int32_t fan, per_pair;
+  int32_t fan;
+  int32_t x_rows, y_rows; /* B200_ROWS_*; y_rows: pairs or plan                            */
   int32_t bias_dtype, residual_dtype, y_dtype;
   int32_t activation, gated;
   int32_t general;        /* nonzero: the general kernel whatever the operands             */
+  int32_t reserved;
 } b200_scaled_args;
 int64_t b200_scaled_linear_scratch(const b200_packed_desc *w, const b200_scaled_args *args);
 int32_t b200_scaled_linear(const b200_packed_desc *w, const b200_scaled_args *args, void *stream);

@@ -105,6 +105,7 @@ int32_t cache_attn_mma_device_error(unsigned int *v, bool clear);
 
 // products of block-scaled activations with packed weights: on the tensor cores (scaled_mma.cu), in general (scaled_general.cu)
 bool scaled_mma_takes(const b200_packed_desc *w, const b200_scaled_args *a);
+bool scaled_gathers(const b200_scaled_args *a);  // that kernel puts x's rows in the plan's order first, in scratch
 int32_t launch_scaled_mma(const b200_packed_desc *w, const b200_scaled_args *a, cudaStream_t stream);
 int32_t launch_scaled_general(const b200_packed_desc *w, const b200_scaled_args *a, cudaStream_t stream);
 int32_t scaled_mma_device_error(unsigned int *v, bool clear);

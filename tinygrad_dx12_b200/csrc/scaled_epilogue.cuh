@@ -30,7 +30,17 @@ template <int ACT>
 __device__ __forceinline__ float activate(float v) {
   if constexpr (ACT == B200_ACT_RELU) return v > 0.f ? v : v != v ? v : 0.f;
   if constexpr (ACT == B200_ACT_SILU) return times_sigmoid(v, v);
-  if constexpr (ACT == B200_ACT_GELU) return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
+  if constexpr (ACT == B200_ACT_GELU) {
+    // erf by Abramowitz and Stegun's 7.1.26 (within 1.5e-7): without a branch, so that a warp's columns run side
+    // by side (CUDA's erff does not: 4096 tokens x 14336 x 4096 456 us)
+    const float z = fabsf(v) * 0.70710678118654752f, t = __fdividef(1.f, fmaf(0.3275911f, z, 1.f));
+    float q = fmaf(1.061405429f, t, -1.453152027f);
+    q = fmaf(q, t, 1.421413741f);
+    q = fmaf(q, t, -0.284496736f);
+    q = fmaf(q, t, 0.254829592f);
+    const float tail = q * t * __expf(-z * z);  // 1 - erf(z)
+    return 0.5f * v * (v < 0.f ? tail : 2.f - tail);
+  }
   // (1 + tanh(z)) / 2 is the sigmoid of 2z
   if constexpr (ACT == B200_ACT_GELU_TANH) return times_sigmoid(v, 1.5957691216057307f * fmaf(0.044715f * v, v * v, v));
   return v;

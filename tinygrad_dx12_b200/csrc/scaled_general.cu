@@ -19,7 +19,7 @@ struct GeneralParams {
   float *raw;           // [rows][n]
   const int32_t *offsets, *order;
   int64_t rows, n, cols;  // rows of y, weight rows of one matrix
-  int experts, fan, per_pair;
+  int experts, fan, x_rows, y_rows;
 };
 
 // The pair at place i of the plan and its expert; -1 without one.
@@ -46,8 +46,9 @@ __global__ void __launch_bounds__(256) product_kernel(const __grid_constant__ Ge
     if (p.experts > 0) {
       const int e = expert_at(p.offsets, p.experts, i);
       if (e < 0) break;  // the pairs without an expert are the last
-      yrow = p.order[i];
-      xrow = p.per_pair ? yrow : yrow / p.fan;
+      const int64_t pair = p.order[i];
+      yrow = p.y_rows == B200_ROWS_PLAN ? i : pair;
+      xrow = p.x_rows == B200_ROWS_PLAN ? i : p.x_rows == B200_ROWS_PAIRS ? pair : pair / p.fan;
       wrow = e * p.n + n;
     }
     const uint8_t *w = p.w + wrow * nblk * BYTES, *x = p.x + xrow * p.cols;
@@ -80,7 +81,8 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Gen
     int e = 0;
     if (p.experts > 0) {
       e = expert_at(p.offsets, p.experts, i);
-      yrow = p.order[i];
+      if (p.y_rows == B200_ROWS_PLAN && e < 0) break;  // not written: they are the last
+      yrow = p.y_rows == B200_ROWS_PLAN ? i : p.order[i];
     }
     float v = 0.f;
     if (c < ep.cols && e >= 0) {
@@ -125,7 +127,7 @@ int32_t launch_scaled_general(const b200_packed_desc *w, const b200_scaled_args 
   p.raw = (float *)a->scratch;
   p.offsets = a->offsets, p.order = a->order;
   p.rows = a->rows, p.n = a->experts > 0 ? w->rows / a->experts : w->rows, p.cols = w->cols;
-  p.experts = (int)a->experts, p.fan = a->fan, p.per_pair = a->per_pair;
+  p.experts = (int)a->experts, p.fan = a->fan, p.x_rows = a->x_rows, p.y_rows = a->y_rows;
   int32_t rc;
   switch (w->format) {
     case B200_FMT_FP4_E2M1: rc = products<B200_FMT_FP4_E2M1>(p, stream); break;
@@ -156,6 +158,8 @@ static int32_t check_scaled(const b200_packed_desc *w, const b200_scaled_args *a
     return b200_set_error(B200_ERR_INVALID, "scaled_linear: rows or experts out of range");
   if (a->experts > 0 && (w->rows % a->experts != 0 || a->fan < 1 || a->residual != nullptr))
     return b200_set_error(B200_ERR_INVALID, "scaled_linear: experts of equal rows, a fan, and no residual");
+  if (a->experts > 0 && (a->x_rows < B200_ROWS_TOKENS || a->x_rows > B200_ROWS_PLAN || (a->y_rows != B200_ROWS_PAIRS && a->y_rows != B200_ROWS_PLAN)))
+    return b200_set_error(B200_ERR_INVALID, "scaled_linear: unknown kind of rows");
   const int64_t n = a->experts > 0 ? w->rows / a->experts : w->rows;
   if (a->activation < B200_ACT_NONE || a->activation > B200_ACT_GELU_TANH || (a->gated && n % 2 != 0))
     return b200_set_error(B200_ERR_INVALID, "scaled_linear: unknown activation, or a gate over an odd number of rows");
@@ -175,7 +179,7 @@ extern "C" {
 
 int64_t b200_scaled_linear_scratch(const b200_packed_desc *w, const b200_scaled_args *a) {
   if (w == nullptr || a == nullptr || a->rows < 0 || a->experts < 0) return 0;
-  if (!a->general && scaled_mma_takes(w, a)) return 0;
+  if (!a->general && scaled_mma_takes(w, a)) return scaled_gathers(a) ? a->rows * w->cols : 0;
   return a->rows * (a->experts > 0 ? w->rows / a->experts : w->rows) * 4;
 }
 
@@ -183,8 +187,10 @@ int32_t b200_scaled_linear(const b200_packed_desc *w, const b200_scaled_args *a,
   if (int32_t rc = b200_injected()) return rc;
   if (int32_t rc = check_scaled(w, a)) return rc;
   if (a->rows == 0 || w->rows == 0) return B200_OK;
-  if (!a->general && scaled_mma_takes(w, a)) return launch_scaled_mma(w, a, (cudaStream_t)stream);
-  if (a->scratch == nullptr) return b200_set_error(B200_ERR_INVALID, "scaled_linear: this call needs scratch");
+  const bool mma = !a->general && scaled_mma_takes(w, a);
+  if ((!mma || scaled_gathers(a)) && (a->scratch == nullptr || (uintptr_t)a->scratch % 16 != 0))
+    return b200_set_error(B200_ERR_INVALID, "scaled_linear: this call needs scratch on a 16-byte boundary");
+  if (mma) return launch_scaled_mma(w, a, (cudaStream_t)stream);
   return launch_scaled_general(w, a, (cudaStream_t)stream);
 }
 

@@ -13,13 +13,13 @@
 //   warps 0-7    epilogue, two groups of four that take turns at 16 or 32 tokens: tcgen05.ld (lane = weight
 //                row, column = token), bias, activation, gate, residual; a warp's 32 rows are 32 neighbouring
 //                columns of y, a block of the 8-bit output, whose largest value is one warp-wide maximum
-//   warps 8-9    cp.async of both sides' scale bytes, four of a row at a time, into the layout that
-//                tcgen05.cp takes, up to 12 stages ahead
+//   warps 8-11   both sides' scale bytes, up to 12 stages ahead: a warp takes an atom (128 rows, four bytes a
+//                stage) and loads 16 bytes of each row, four stages, which leave its registers as four atoms in the
+//                layout that tcgen05.cp takes
 //   warp 13      tcgen05.cp of a stage's scales into one of four sets of tensor-memory columns; commit
 //                announces them to warp 12
-//   warps 10-11  through experts, cp.async of x's codes: token rows are found through the plan's order. The
-//                copies themselves arrive at the stage's barrier when they land
-//   warps 14-15  one thread each: TMA of the weight codes and, without experts, of x's
+//   warps 14-15  one thread each: TMA of the codes, the weights' and x's. Through experts x's rows lie in the
+//                plan's order (gathered before, or written so by the product before), so a tile of tokens is a box
 //   warp 12      four MMAs a stage and accumulator; commit frees the stage and its set. (One warp for
 //                scales and MMAs took 0.5 us a stage: copies, waits and MMAs cost an issuing thread 25 to 45 ns each)
 // Two accumulators of a tile's width, so that the epilogue of one tile runs under the products of the
@@ -50,9 +50,8 @@ int32_t scaled_mma_reset_tickets() { return workspace_zero(WS_SCALED); }
 namespace scaled {
 
 constexpr int TM = 128, KS = 128;            // weight rows of an MMA, codes of a stage
-constexpr int EPI_WARPS = 8, LOAD_WARP0 = 8, LOAD_WARPS = 4, MMA_WARP = 12, SF_WARP = 13, W_WARP0 = 14, W_WARPS = 2;
+constexpr int EPI_WARPS = 8, SCALE_WARP0 = 8, SCALE_WARPS = 4, MMA_WARP = 12, SF_WARP = 13, W_WARP0 = 14, W_WARPS = 2;
 constexpr int THREADS = 16 * 32;
-constexpr int LOADERS = LOAD_WARPS / 2 * 32;  // threads that copy scales, and as many that copy x's codes
 constexpr int SLOTS = 12;                    // stages whose scales wait for tensor memory
 constexpr int ACC_COLS = 224;                // columns of an accumulator set: R * NT at most
 constexpr int SF_SETS = 4;
@@ -70,7 +69,12 @@ struct Params {
   int64_t second;         // the tile's other weight rows: up rows of a gate's, or the next 128
   int64_t nblk;           // scale bytes of a row
   int64_t cols;
-  int experts, fan, per_pair;
+  int experts, fan;
+  int xs_rows;            // x's scales: B200_ROWS_* (its codes lie in the plan's order)
+  int y_pairs;            // y's rows are pairs; else they lie in the plan's order (or there is no plan)
+  int single_row;         // x is one token's row
+  int vector;             // scale rows are whole 16 bytes
+  int scale_warps;
   int nst;                // K stages
   int wtiles, tile_rows;  // tiles of weight rows of one matrix, columns of y in each
   int nt;                 // tokens of a tile, at most
@@ -100,18 +104,6 @@ __device__ __forceinline__ bool mbar_over(uint64_t *bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void *src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-// Arrives at `bar` when the copies that this thread has issued so far have landed.
-__device__ __forceinline__ void cp_arrive(uint64_t *bar) {
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // Shared-memory descriptor of a scale atom: 32 rows of 16 bytes, no swizzle.
 __device__ __forceinline__ uint64_t sf_desc(const void *atom) {
@@ -184,6 +176,13 @@ __device__ __forceinline__ Tile tile_at(const Params &p, const int32_t *before, 
   r.rows = (int)(count - (int64_t)t * per < per ? count - (int64_t)t * per : per);
   r.width = (r.rows + 15) / 16 * 16;
   return r;
+}
+
+// The row of x's scales of place `at`.
+__device__ __forceinline__ int64_t scale_row(const Params &p, int64_t at) {
+  if (p.xs_rows == B200_ROWS_PLAN) return at;
+  const int32_t pair = p.order[at];
+  return p.xs_rows == B200_ROWS_PAIRS ? pair : pair / p.fan;
 }
 
 // The CTA's run of units, of all that are shared out among `ctas`.
@@ -300,9 +299,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint8_t *ring = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const int S = p.stages;
   uint8_t *scales = ring + (size_t)S * p.stage_bytes;
-  uint64_t *fullw = reinterpret_cast<uint64_t *>(scales + (size_t)SLOTS * p.scale_bytes);
-  uint64_t *fullx = fullw + S;
-  uint64_t *empty = fullx + S;
+  uint64_t *full = reinterpret_cast<uint64_t *>(scales + (size_t)SLOTS * p.scale_bytes);
+  uint64_t *empty = full + S;
   uint64_t *fulls = empty + S, *frees = fulls + SLOTS;  // scales landed, scales in tensor memory
   uint64_t *sfready = frees + SLOTS;
   uint64_t *accfull = sfready + SF_SETS;
@@ -317,12 +315,11 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
-      mbar_init(&fullw[s], 1);
-      mbar_init(&fullx[s], LOADERS);
+      mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < SLOTS; ++b) {
-      mbar_init(&fulls[b], LOADERS);
+      mbar_init(&fulls[b], p.scale_warps);
       mbar_init(&frees[b], 1);
     }
     for (int b = 0; b < SF_SETS; ++b) mbar_init(&sfready[b], 1);
@@ -388,25 +385,23 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (!next_seg(p, run, u, g)) break;
           const Tile t = tile_at(p, before, start, g.tile);
           row = t.e * p.n + t.w0;
-          first = t.first;
+          first = p.single_row ? 0 : t.first;
         }
         if (round > 0 && !mbar_wait(&empty[slot], (round - 1u) & 1u, abort_flag)) break;
         uint8_t *st = ring + (size_t)slot * p.stage_bytes;
-        mbar_arrive_expect_tx(&fullw[slot], p.tx);
+        mbar_arrive_expect_tx(&full[slot], p.tx);
         const int x = (g.s0 + s) * KS;
-        tma_load_2d(st, &tmw, x, (int32_t)row, &fullw[slot]);
-        if constexpr (R == 2) tma_load_2d(st + TM * KS, &tmw, x, (int32_t)(row + p.second), &fullw[slot]);
-        if (p.experts == 0) {
-          if (round > 0) {
-            tma_load_2d(st + p.b_off, &tmx, x, (int32_t)first, &fullw[slot]);
-          } else {  // the ring's first round: x's boxes behind all the weights'
-            early_x[held] = x, early_row[held] = (int32_t)first, early_slot[held] = slot;
-            ++held;
-            if (i + turns >= n || slot + turns >= S) {
-              asm volatile("griddepcontrol.wait;" ::: "memory");
-              for (int q = 0; q < held; ++q)
-                tma_load_2d(ring + (size_t)early_slot[q] * p.stage_bytes + p.b_off, &tmx, early_x[q], early_row[q], &fullw[early_slot[q]]);
-            }
+        tma_load_2d(st, &tmw, x, (int32_t)row, &full[slot]);
+        if constexpr (R == 2) tma_load_2d(st + TM * KS, &tmw, x, (int32_t)(row + p.second), &full[slot]);
+        if (round > 0) {
+          tma_load_2d(st + p.b_off, &tmx, x, (int32_t)first, &full[slot]);
+        } else {  // the ring's first round: x's boxes behind all the weights'
+          early_x[held] = x, early_row[held] = (int32_t)first, early_slot[held] = slot;
+          ++held;
+          if (i + turns >= n || slot + turns >= S) {
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            for (int q = 0; q < held; ++q)
+              tma_load_2d(ring + (size_t)early_slot[q] * p.stage_bytes + p.b_off, &tmx, early_x[q], early_row[q], &full[early_slot[q]]);
           }
         }
         s += turns;
@@ -414,93 +409,69 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       if (*abort_flag) {  // this thread's copies in flight land before the CTA exits
         for (int64_t q = turn; q < (i < n ? i : n); q += turns)
-          if (q + S >= i) mbar_drain(&fullw[q % S], (uint32_t)((q / S) & 1), 200000000ull);
+          if (q + S >= i) mbar_drain(&full[q % S], (uint32_t)((q / S) & 1), 200000000ull);
       }
     }
-  } else if (warp >= LOAD_WARP0 && warp < LOAD_WARP0 + LOAD_WARPS) {
-    // A stage is worth some 450 cycles, and one warp's dependent instructions take 4 to 6 each: pointers are
-    // kept and moved on, so that a copy is one instruction.
-    const int th = (threadIdx.x - LOAD_WARP0 * 32) & (LOADERS - 1);
-    auto xrow = [&](const Tile &t, int r) -> int64_t {  // row of x
-      const int64_t at = t.first + r;
-      if (p.experts == 0) return at;
-      const int32_t pair = p.order[at];
-      return p.per_pair ? pair : pair / p.fan;
-    };
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    bool ok = true;
-    uint32_t round = 0, off = 0;
+  } else if (warp >= SCALE_WARP0 && warp < SCALE_WARP0 + p.scale_warps) {
+    // ---------------- scale bytes: one atom a warp, R of the weights, then one or two of x ----------------
+    const int atom = warp - SCALE_WARP0;
+    const bool mine = atom < R;  // weights, which are no result of the kernel before
+    if (!mine) asm volatile("griddepcontrol.wait;" ::: "memory");
+    uint8_t *dst = scales + atom * 512 + lane * 16;
     int slot = 0;
+    uint32_t round = 0;
     int64_t u = run.u0;
     Seg g;
-    if (warp < LOAD_WARP0 + LOAD_WARPS / 2) {
-      // ---------------- cp.async of scale bytes ----------------
-      constexpr int WR = R * TM / LOADERS, XR = (ACC_COLS + LOADERS - 1) / LOADERS;  // rows a thread
-      const uint32_t base = smem_u32(scales), to_b = p.sfb_off;
-      // row r's place in its atom: (r % 32) * 16 + (r / 32) * 4; an atom is 128 rows
-      auto place = [&](int r) -> uint32_t { return (uint32_t)((r >> 7) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4); };
-      while (ok && next_seg(p, run, u, g)) {
-        const Tile t = tile_at(p, before, start, g.tile);
-        const int s = g.s0, len = g.len;
-        const uint8_t *sw[WR], *sx[XR];
+    bool ok = true;
+    while (ok && next_seg(p, run, u, g)) {
+      const Tile t = tile_at(p, before, start, g.tile);
+      const uint8_t *src[4];  // of rows lane, lane + 32, ...: null where there are none
 #pragma unroll
-        for (int q = 0; q < WR; ++q) {
-          const int r = th + q * LOADERS;
-          int64_t wrow = t.e * p.n + (r >> 7) * p.second + t.w0 + (r & 127);
-          if (wrow >= p.wrows) wrow = p.wrows - 1;  // rows behind the last: not stored
-          sw[q] = p.ws + wrow * p.nblk + 4 * s;
-        }
-        const int mine = (t.rows - th + LOADERS - 1) / LOADERS, most = (t.rows + LOADERS - 1) / LOADERS;
-#pragma unroll
-        for (int q = 0; q < XR; ++q) sx[q] = q < mine ? p.xs + xrow(t, th + q * LOADERS) * p.nblk + 4 * s : p.xs;
-        for (int j = 0; j < len; ++j) {
-          if (round > 0) ok = __all_sync(0xffffffffu, mbar_wait(&frees[slot], (round - 1u) & 1u, abort_flag));
-          if (!ok) break;
-#pragma unroll
-          for (int q = 0; q < WR; ++q) {
-            cp_async4(base + off + place(th + q * LOADERS), sw[q]);
-            sw[q] += 4;
-          }
-#pragma unroll
-          for (int q = 0; q < XR; ++q) {
-            if (q >= most) break;
-            if (q < mine) cp_async4(base + off + to_b + place(th + q * LOADERS), sx[q]);
-            sx[q] += 4;
-          }
-          cp_arrive(&fulls[slot]);
-          off += p.scale_bytes;
-          if (++slot == SLOTS) slot = 0, off = 0, ++round;
+      for (int q = 0; q < 4; ++q) {
+        const int r = lane + 32 * q;
+        if (mine) {
+          const int64_t row = t.e * p.n + atom * p.second + t.w0 + r;
+          src[q] = row < p.wrows ? p.ws + row * p.nblk : nullptr;
+        } else {
+          const int at = (atom - R) * 128 + r;
+          src[q] = at < t.rows ? p.xs + scale_row(p, t.first + at) * p.nblk : nullptr;
         }
       }
-    } else if (p.experts > 0) {
-      // ---------------- cp.async of x's codes ----------------
-      const int chunk = th & 7, r0 = th >> 3;  // 16 bytes of a row's 128; rows r0, r0 + 8, ... (r & 7 the same in all)
-      constexpr int STEP = LOADERS / 8, PASSES = ACC_COLS / STEP;
-      const uint32_t dst = smem_u32(ring) + p.b_off + (uint32_t)(r0 * 128 + ((chunk ^ (r0 & 7)) << 4));
-      while (ok && next_seg(p, run, u, g)) {
-        const Tile t = tile_at(p, before, start, g.tile);
-        const int s = g.s0, len = g.len;
-        const int mine = (t.rows - r0 + STEP - 1) / STEP, most = (t.rows + STEP - 1) / STEP;
-        const uint8_t *src[PASSES];
+      // four stages' bytes of each row, from a multiple of four on
+      auto load = [&](int s, uint32_t (&v)[4][4]) {
 #pragma unroll
-        for (int q = 0; q < PASSES; ++q)
-          src[q] = q < mine ? p.x + xrow(t, r0 + STEP * q) * p.cols + (int64_t)s * KS + chunk * 16 : p.x;
-        for (int j = 0; j < len; ++j) {
-          if (round > 0) ok = __all_sync(0xffffffffu, mbar_wait(&empty[slot], (round - 1u) & 1u, abort_flag));
-          if (!ok) break;
+        for (int q = 0; q < 4; ++q) {
+          if (p.vector && src[q] != nullptr) {
+            const uint4 w = *reinterpret_cast<const uint4 *>(src[q] + 4 * s);
+            v[q][0] = w.x, v[q][1] = w.y, v[q][2] = w.z, v[q][3] = w.w;
+          } else {
 #pragma unroll
-          for (int q = 0; q < PASSES; ++q) {
-            if (q >= most) break;
-            if (q < mine) cp_async16(dst + off + q * STEP * 128, src[q]);
-            src[q] += KS;
+            for (int j = 0; j < 4; ++j)
+              v[q][j] = src[q] != nullptr && s + j < p.nst ? *reinterpret_cast<const uint32_t *>(src[q] + 4 * (s + j)) : 0u;
           }
-          cp_arrive(&fullx[slot]);
-          off += p.stage_bytes;
-          if (++slot == S) slot = 0, off = 0, ++round;
+        }
+      };
+      const int end = g.s0 + g.len;
+      uint32_t now[4][4], next[4][4];
+      load(g.s0 & ~3, next);
+      for (int s = g.s0 & ~3; s < end && ok; s += 4) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) now[q][j] = next[q][j];
+        if (s + 4 < end) load(s + 4, next);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (s + j < g.s0 || s + j >= end || !ok) continue;
+          if (round > 0) ok = __all_sync(0xffffffffu, mbar_wait(&frees[slot], (round - 1u) & 1u, abort_flag));
+          if (!ok) continue;
+          *reinterpret_cast<uint4 *>(dst + slot * p.scale_bytes) = make_uint4(now[0][j], now[1][j], now[2][j], now[3][j]);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&fulls[slot]);
+          if (++slot == SLOTS) slot = 0, ++round;
         }
       }
     }
-    cp_wait_all();
   } else if (warp == MMA_WARP) {
     // ---------------- MMA issuer: the whole warp, one lane of it elected ----------------
     const uint64_t ad = sw128_kmajor_desc(ring), bd = sw128_kmajor_desc(ring + p.b_off);  // the slots' follow: address / 16
@@ -523,20 +494,17 @@ __global__ void __launch_bounds__(THREADS, 1)
       const uint32_t idesc = p.idesc | ((uint32_t)(t.width >> 3) << 17);
       for (int j = 0; j < len; ++j) {
         if (!over) {
-          ok = mbar_wait(&sfready[set], phase, abort_flag) && mbar_wait(&fullw[slot], sphase, abort_flag);
-          ok = __all_sync(0xffffffffu, ok && (p.experts == 0 || mbar_wait(&fullx[slot], sphase, abort_flag)));
+          ok = mbar_wait(&sfready[set], phase, abort_flag) && mbar_wait(&full[slot], sphase, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
         }
         if (!ok) break;
-        if (p.experts > 0) fence_proxy_async_smem();  // cp.async wrote by the generic proxy, the tensor core reads by the other
         tc_fence_after();
         const uint32_t sf = tmem + p.sf_col + p.sf_width * (uint32_t)set;
         if (++set == p.sets) set = 0, phase ^= 1u;
         const int now = slot;
         if (++slot == S) slot = 0, sphase ^= 1u;
         // the next stage is asked for before this one's MMAs are issued
-        over = mbar_over(&sfready[set], phase) & mbar_over(&fullw[slot], sphase);
-        if (p.experts > 0) over = over & mbar_over(&fullx[slot], sphase);
-        over = __all_sync(0xffffffffu, over);
+        over = __all_sync(0xffffffffu, mbar_over(&sfready[set], phase) & mbar_over(&full[slot], sphase));
 #pragma unroll
         for (int q = 0; q < R; ++q)
           mma_stage(acc + (uint32_t)q * p.acc_width, ad + off + (uint64_t)(q * (TM * KS >> 4)), bd + off, idesc, (uint32_t)j, sf + 4u * q,
@@ -566,7 +534,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
       }
-      fence_proxy_async_smem();  // as the MMA warp's
+      fence_proxy_async_smem();  // threads wrote by the generic proxy, the tensor core reads by the other
       tc_fence_after();
       const uint32_t sf = tmem + p.sf_col + p.sf_width * (uint32_t)set;
 #pragma unroll
@@ -607,7 +575,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       auto row_of = [&](int j0, int count) -> int {  // of y, of token j0 + lane
         const int64_t at = t.first + j0 + (lane < count ? lane : 0);
-        return p.experts > 0 ? p.order[at] : (int)at;
+        return p.y_pairs ? p.order[at] : (int)at;
       };
       const int buf = p.bufs == 2 ? seg & 1 : 0;
       ok = __all_sync(0xffffffffu, ok && mbar_wait(&accfull[buf], (uint32_t)((p.bufs == 2 ? seg >> 1 : seg) & 1), abort_flag));
@@ -681,7 +649,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     }
     // rows of pairs that no expert has are zeros
-    if (p.experts > 0) {
+    if (p.y_pairs) {
       const int64_t size = std::is_same<OUT, E4M3>::value ? 1 : sizeof(OUT), bytes = ep.cols * size;
       for (int64_t r = start[p.experts] + blockIdx.x; r < p.rows; r += gridDim.x) {
         const int64_t row = p.order[r];
@@ -700,6 +668,38 @@ __global__ void __launch_bounds__(THREADS, 1)
   __syncthreads();
   tc_fence_after();
   if (warp == MMA_WARP) tmem_dealloc(tmem, p.tmem_cols);
+}
+
+// x's codes in the plan's order, 16 bytes a thread: a tile of an expert's tokens is one box then. It costs a
+// write and a read of rows x cols bytes (32008 x 4096: 30 us beside 1000 us of products); copying the rows
+// with cp.async within the product kept its load/store unit busy for longer than a stage takes.
+__global__ void __launch_bounds__(256) gather_kernel(const uint8_t *x, uint8_t *out, const int32_t *offsets, const int32_t *order,
+                                                     int experts, int fan, int pairs, int64_t cols) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int per_row = (int)(cols >> 4);
+  const int64_t all = (int64_t)offsets[experts] * per_row;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const int64_t at = i / per_row;
+    const int32_t pair = order[at];
+    const int64_t row = pairs ? pair : pair / fan;
+    reinterpret_cast<uint4 *>(out)[i] = reinterpret_cast<const uint4 *>(x)[row * per_row + (i - at * per_row)];
+  }
+}
+
+template <typename... KArgs, typename... Args>
+static cudaError_t launch_dependent(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 // Rows that meet one matrix: all, or an expert's share.
@@ -726,8 +726,11 @@ static int32_t launch_t(const b200_packed_desc *w, const b200_scaled_args *a, in
   p.wrows = w->rows;
   p.cols = w->cols;
   p.nblk = w->cols / 32;
-  p.experts = (int)a->experts, p.fan = a->experts > 0 ? a->fan : 1, p.per_pair = a->per_pair;
   p.nst = (int)(w->cols / KS);
+  p.experts = (int)a->experts, p.fan = a->experts > 0 ? a->fan : 1;
+  p.xs_rows = a->experts > 0 ? a->x_rows : B200_ROWS_PLAN;
+  p.y_pairs = a->experts > 0 && a->y_rows != B200_ROWS_PLAN;
+  p.vector = p.nst % 4 == 0 && (uintptr_t)a->x_scales % 16 == 0 && (uintptr_t)w->scales % 16 == 0;
   const Epilogue ep = epilogue_of(w, a);
   p.second = GATED ? ep.cols : TM;
   p.tile_rows = R == 2 && !GATED ? 2 * TM : TM;
@@ -748,7 +751,9 @@ static int32_t launch_t(const b200_packed_desc *w, const b200_scaled_args *a, in
   p.stage_bytes = p.b_off + (uint32_t)((p.nt * KS + 1023) / 1024 * 1024);
   p.sfb_off = R * 512;
   p.scale_bytes = p.sfb_off + (p.nt > 128 ? 1024 : 512);
-  const size_t tail = 8 * (3 * MAX_STAGES + 2 * SLOTS + SF_SETS + 6) + 16 + 8 * ((size_t)p.experts + 1) + 16;
+  p.scale_warps = R + (p.nt > 128 ? 2 : 1);
+  static_assert(R + 2 <= SCALE_WARPS, "a warp for each atom");
+  const size_t tail = 8 * (2 * MAX_STAGES + 2 * SLOTS + SF_SETS + 6) + 16 + 8 * ((size_t)p.experts + 1) + 16;
   int stages = (int)((SMEM_LIMIT - 1024 - tail - SLOTS * p.scale_bytes) / p.stage_bytes);
   p.stages = stages < MAX_STAGES ? stages : MAX_STAGES;
   p.sets = p.stages < SF_SETS ? p.stages : SF_SETS;
@@ -772,26 +777,26 @@ static int32_t launch_t(const b200_packed_desc *w, const b200_scaled_args *a, in
   if (int32_t rc = make_tma_2d(&tmw, bits == 4 ? CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B : CU_TENSOR_MAP_DATA_TYPE_16U6_ALIGN16B,
                                w->data, (uint64_t)w->cols, (uint64_t)w->rows, row_bytes, KS, TM, CU_TENSOR_MAP_SWIZZLE_128B))
     return rc;
-  CUtensorMap tmx = tmw;
-  if (p.experts == 0) {  // rows of x side by side: whole tiles of them
-    p.tx += (uint32_t)(p.nt * KS);
-    if (int32_t rc = make_tma_2d(&tmx, CU_TENSOR_MAP_DATA_TYPE_UINT8, a->x, (uint64_t)w->cols, (uint64_t)a->rows, (uint64_t)w->cols, KS,
-                                 (uint32_t)p.nt, CU_TENSOR_MAP_SWIZZLE_128B))
-      return rc;
+  const uint8_t *xcodes = (const uint8_t *)a->x;
+  int64_t xrows = a->rows;
+  if (scaled_gathers(a)) {
+    const int64_t ctas = (a->rows * (w->cols / 16) + 255) / 256;
+    B200_CUDA_TRY(launch_dependent(gather_kernel, dim3((unsigned)(ctas < 8 * sms ? ctas : 8 * sms)), dim3(256), 0, stream, xcodes,
+                                   (uint8_t *)a->scratch, a->offsets, a->order, (int)a->experts, (int)a->fan,
+                                   (int)(a->x_rows == B200_ROWS_PAIRS), w->cols));
+    xcodes = (const uint8_t *)a->scratch;
+  } else if (a->experts > 0 && a->x_rows != B200_ROWS_PLAN) {
+    p.single_row = 1;
+    xrows = 1;
   }
+  p.tx += (uint32_t)(p.nt * KS);
+  CUtensorMap tmx;
+  if (int32_t rc = make_tma_2d(&tmx, CU_TENSOR_MAP_DATA_TYPE_UINT8, xcodes, (uint64_t)w->cols, (uint64_t)xrows, (uint64_t)w->cols, KS,
+                               (uint32_t)p.nt, CU_TENSOR_MAP_SWIZZLE_128B))
+    return rc;
   const size_t smem = 1024 + (size_t)p.stages * p.stage_bytes + SLOTS * p.scale_bytes + tail;
   B200_CUDA_TRY((ensure_dynamic_smem<scaled_kernel<R, GATED, OUT>>(SMEM_LIMIT)));
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)p.grid);
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  B200_CUDA_TRY(cudaLaunchKernelEx(&cfg, scaled_kernel<R, GATED, OUT>, tmw, tmx, p, ep));
+  B200_CUDA_TRY(launch_dependent(scaled_kernel<R, GATED, OUT>, dim3((unsigned)p.grid), dim3(THREADS), smem, stream, tmw, tmx, p, ep));
   return B200_OK;
 }
 
@@ -806,6 +811,11 @@ static int32_t dispatch(const b200_packed_desc *w, const b200_scaled_args *a, in
 }
 
 }  // namespace scaled
+
+// Rows of x that are no tile as they lie: tokens' or pairs' rows, unless they are one.
+bool scaled_gathers(const b200_scaled_args *a) {
+  return a->experts > 0 && a->x_rows != B200_ROWS_PLAN && !(a->x_rows == B200_ROWS_TOKENS && a->rows <= a->fan) && a->rows > 1;
+}
 
 // What the checks of the entry have left: whole stages, and the alignment that TMA and cp.async ask for.
 bool scaled_mma_takes(const b200_packed_desc *w, const b200_scaled_args *a) {

@@ -19,7 +19,7 @@ import torch
 from . import _lib
 from .attention import _REAL, _call, _elsewhere
 from .packed import PackedTensor, _require_cuda
-from .scaled import _E4M3, BlockScaled, _blocks, _check_bias, _check_product, _check_weights, _flat, _product
+from .scaled import ROWS_PAIRS, ROWS_PLAN, ROWS_TOKENS, _E4M3, BlockScaled, _blocks, _check_bias, _check_product, _check_weights, _flat, _product
 
 MAX_EXPERTS, MAX_K, MAX_GROUPS = 1024, 32, 32
 
@@ -198,7 +198,8 @@ def expert_linear(x: BlockScaled, w: PackedTensor, routing: Routing, bias: torch
     bias = _check_bias(bias, w.shape[:2], x.device)
     y = _blocks((pairs, cols), x.device) if dtype == _E4M3 else torch.empty((pairs, cols), dtype=dtype, device=x.device)
     if pairs and cols:
-        _product(x, w, y, pairs, bias, activation, gated, None, routing, routing.k, int(x.shape[0] == pairs), _general)
+        _product(x, w, y, pairs, bias, activation, gated, None, routing, ROWS_TOKENS if x.shape[0] == routing.tokens else ROWS_PAIRS,
+                 ROWS_PAIRS, _general)
     return y
 
 
@@ -237,8 +238,8 @@ def expert_mlp(x: BlockScaled, up: PackedTensor, down: PackedTensor, routing: Ro
         return out
     y = torch.empty((pairs, cols), dtype=torch.float32, device=device)
     h = _blocks((pairs, inner), device)
-    _product(x, up, h, pairs, up_bias, activation, gated, None, routing, routing.k, int(tokens == pairs), _general)
-    _product(h, down, y, pairs, down_bias, None, False, None, routing, routing.k, 1, _general)
+    _product(x, up, h, pairs, up_bias, activation, gated, None, routing, ROWS_TOKENS, ROWS_PLAN, _general)
+    _product(h, down, y, pairs, down_bias, None, False, None, routing, ROWS_PLAN, ROWS_PAIRS, _general)
     r = residual
     _call("b200_expert_combine", device, y.data_ptr(), _REAL[y.dtype], routing.weights.data_ptr(), routing.indices.data_ptr(),
           routing.first, routing.experts, routing.k, tokens, cols, None if r is None else r.data_ptr(),

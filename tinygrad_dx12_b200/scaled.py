@@ -27,6 +27,7 @@ from .packed import PackedTensor, _require_cuda
 
 BLOCK = 32
 ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+ROWS_TOKENS, ROWS_PAIRS, ROWS_PLAN = 0, 1, 2  # B200_ROWS_*
 SCALED_FORMATS = ("fp4_e2m1", "fp6_e2m3", "fp6_e3m2")
 _E4M3, _E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 _RESULTS = {**_REAL, _E4M3: _lib.DT["fp8e4m3"]}
@@ -50,9 +51,9 @@ class ScaledArgs(ctypes.Structure):
                 ("bias", ctypes.c_void_p), ("residual", ctypes.c_void_p), ("residual_stride", ctypes.c_int64),
                 ("y", ctypes.c_void_p), ("y_scales", ctypes.c_void_p), ("scratch", ctypes.c_void_p),
                 ("offsets", ctypes.c_void_p), ("order", ctypes.c_void_p), ("experts", ctypes.c_int64),
-                ("fan", ctypes.c_int32), ("per_pair", ctypes.c_int32), ("bias_dtype", ctypes.c_int32),
+                ("fan", ctypes.c_int32), ("x_rows", ctypes.c_int32), ("y_rows", ctypes.c_int32), ("bias_dtype", ctypes.c_int32),
                 ("residual_dtype", ctypes.c_int32), ("y_dtype", ctypes.c_int32), ("activation", ctypes.c_int32),
-                ("gated", ctypes.c_int32), ("general", ctypes.c_int32)]
+                ("gated", ctypes.c_int32), ("general", ctypes.c_int32), ("reserved", ctypes.c_int32)]
 
 
 @dataclass(frozen=True, eq=False)  # compared by identity, as caches are
@@ -243,7 +244,7 @@ def _check_bias(bias, shape, device, name="bias"):
     return bias if bias.is_contiguous() else bias.contiguous()
 
 
-def _product(x, w, y, rows, bias, activation, gated, residual=None, plan=None, fan=1, per_pair=0, general=False):
+def _product(x, w, y, rows, bias, activation, gated, residual=None, plan=None, x_rows=0, y_rows=1, general=False):
     """Launches one product of checked operands into y."""
     codes, scales = _dense(x)
     a = ScaledArgs()
@@ -258,10 +259,11 @@ def _product(x, w, y, rows, bias, activation, gated, residual=None, plan=None, f
         a.y, a.y_dtype = y.data_ptr(), _REAL[y.dtype]
     if plan is not None:
         a.offsets, a.order, a.experts = plan.offsets.data_ptr(), plan.rows.data_ptr(), w.shape[0]
-        a.fan, a.per_pair = fan, per_pair
+        a.fan, a.x_rows, a.y_rows = plan.k, x_rows, y_rows
     a.activation, a.gated, a.general = ACTIVATIONS[activation], int(gated), int(general)
     desc = w.desc()
-    if general or w.cols % 128 or desc.data % 32 or desc.scales % 4:  # not on the tensor cores
+    # not on the tensor cores, or rows that have to be put in the plan's order first
+    if general or w.cols % 128 or desc.data % 32 or desc.scales % 4 or (plan is not None and x_rows != ROWS_PLAN):
         size = _lib.lib().b200_scaled_linear_scratch(ctypes.byref(desc), ctypes.byref(a))
         scratch = torch.empty(size, dtype=torch.uint8, device=x.device)
         a.scratch = scratch.data_ptr()
