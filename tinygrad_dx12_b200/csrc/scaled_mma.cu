@@ -10,7 +10,7 @@
 // A tile is R x 128 weight rows (the MMA's M; R = 2 when gated: 128 gate rows and the 128 up rows that go
 // with them, in two accumulators, so both are in one thread's hands) times up to NT tokens (its N, a
 // multiple of 16, so an expert with few tokens costs few columns). K advances 128 codes a stage.
-//   warps 0-7    epilogue, two groups of four that take turns at 16 or 32 tokens: tcgen05.ld (lane = weight
+//   warps 0-7    epilogue, two groups of four that take turns at 16 tokens: tcgen05.ld (lane = weight
 //                row, column = token), bias, activation, gate, residual; a warp's 32 rows are 32 neighbouring
 //                columns of y, a block of the 8-bit output, whose largest value is one warp-wide maximum
 //   warps 8-11   both sides' scale bytes, up to 12 stages ahead: a warp takes an atom (128 rows, four bytes a
@@ -59,6 +59,7 @@ constexpr int MAX_STAGES = 12;
 constexpr int MAX_EXPERTS = 1024;
 constexpr int MIN_UNITS = 4;                 // a CTA's run is no shorter: its start costs more than its work otherwise
 constexpr size_t TICKETS = 4096;             // one a CTA
+constexpr int CH = 16;                       // tokens of an epilogue step: more unrolled code does not stay in the instruction cache
 constexpr int SMEM_LIMIT = 227 * 1024;
 
 struct Params {
@@ -213,18 +214,11 @@ __device__ __forceinline__ T to_out(float v) {
 }
 struct E4M3 {};
 
-template <int N>
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[N]) {
-  uint32_t (&r)[N] = reinterpret_cast<uint32_t (&)[N]>(v);
-  if constexpr (N == 32) tmem_ld_32x32b_x32(taddr, r);
-  else tmem_ld_32x32b_x16(taddr, r);
-}
-
-// A gate of two products: the second one's values times the first one's, which the activation has been
-// applied to. `up` is not read without one.
-template <bool GATED, typename OUT, int CH>
-__device__ __forceinline__ void finish_column(const Epilogue &ep, float (&v)[CH], float bias, const float (&up)[CH], float up_bias, int c,
-                                              int at, int count) {
+// One weight row's products with CH tokens, column `c` of y: finished and stored. `up`, with a gate: the products
+// that the activated ones multiply. `at` is the row of y of token j in lane j (pairs: of any order).
+template <bool GATED, typename OUT>
+__device__ __forceinline__ void finish(const Epilogue &ep, float (&v)[CH], float bias, const float (&up)[CH], float up_bias, int c,
+                                       int at, int count, bool pairs) {
   const int lane = threadIdx.x & 31;
   const bool live = c < ep.cols;
 #pragma unroll
@@ -251,12 +245,12 @@ __device__ __forceinline__ void finish_column(const Epilogue &ep, float (&v)[CH]
 #pragma unroll
     for (int j = 0; j < CH; ++j) v[j] = __fmul_rn(v[j], up[j] + up_bias);
   }
-  const int cols = (int)ep.cols;
+  const int cols = (int)ep.cols, lim = live ? count : 0;
   if (ep.residual != nullptr) {
 #pragma unroll
     for (int j = 0; j < CH; ++j) {
       const int row = __shfl_sync(0xffffffffu, at, j);
-      if (live && j < count) v[j] += load_as_f32(ep.residual, row * ep.rstride + c, ep.rdt);
+      if (j < lim) v[j] += load_as_f32(ep.residual, row * ep.rstride + c, ep.rdt);
     }
   }
   if constexpr (std::is_same<OUT, E4M3>::value) {  // y's columns are whole blocks: a warp's are all live or none
@@ -268,28 +262,25 @@ __device__ __forceinline__ void finish_column(const Epilogue &ep, float (&v)[CH]
     }
     const uint32_t byte = rows8::scale_byte(top);
     const float inv = rows8::inverse(byte);
-    if (live && lane < count) ep.ys[(int64_t)at * (cols >> 5) + (c >> 5)] = (uint8_t)byte;
+    if (lane < lim) ep.ys[(int64_t)at * (cols >> 5) + (c >> 5)] = (uint8_t)byte;
 #pragma unroll
     for (int j = 0; j < CH; ++j) {
       const int row = __shfl_sync(0xffffffffu, at, j);
       const float s = __shfl_sync(0xffffffffu, inv, j);
-      if (live && j < count) ((uint8_t *)ep.y)[(int64_t)row * cols + c] = (uint8_t)rows8::codes2(v[j], 0.f, s, s == 0.f);
+      if (j < lim) ((uint8_t *)ep.y)[(int64_t)row * cols + c] = (uint8_t)rows8::codes2(v[j], 0.f, s, s == 0.f);
     }
+  } else if (!pairs) {  // rows side by side
+    OUT *y = (OUT *)ep.y + (int64_t)__shfl_sync(0xffffffffu, at, 0) * cols + c;
+#pragma unroll
+    for (int j = 0; j < CH; ++j, y += cols)
+      if (j < lim) *y = to_out<OUT>(v[j]);
   } else {
 #pragma unroll
     for (int j = 0; j < CH; ++j) {
       const int row = __shfl_sync(0xffffffffu, at, j);
-      if (live && j < count) ((OUT *)ep.y)[(int64_t)row * cols + c] = to_out<OUT>(v[j]);
+      if (j < lim) ((OUT *)ep.y)[(int64_t)row * cols + c] = to_out<OUT>(v[j]);
     }
   }
-}
-
-// Weight rows' products with CH tokens, column `c` of y and, with two accumulators and no gate, c + 128:
-// finished and stored. `at` is the row of y of token j in lane j.
-template <int R, bool GATED, typename OUT, int CH>
-__device__ __forceinline__ void finish(const Epilogue &ep, float (&v)[R][CH], const float (&bias)[R], int c, int at, int count) {
-  finish_column<GATED, OUT, CH>(ep, v[0], bias[0], v[R - 1], bias[R - 1], c, at, count);
-  if constexpr (R == 2 && !GATED) finish_column<false, OUT, CH>(ep, v[1], bias[1], v[1], 0.f, c + TM, at, count);
 }
 
 template <int R, bool GATED, typename OUT>
@@ -556,9 +547,9 @@ __global__ void __launch_bounds__(THREADS, 1)
   } else if (warp < EPI_WARPS) {
     // ---------------- epilogue: weight row = tensor-memory lane, token = column ----------------
     asm volatile("griddepcontrol.wait;" ::: "memory");  // bias, y, parts and tickets
+    constexpr int TOGETHER = GATED ? 2 : 1, PARTS = R / TOGETHER;
     const int quarter = warp & 3, group = warp >> 2;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-    constexpr int CH = R == 2 ? 16 : 32;  // tokens at a time: R * CH accumulators in registers
     bool ok = true;  // this warp's waits; after one that ran out it still meets the others
     int seg = 0;
     int64_t u = run.u0;
@@ -584,28 +575,30 @@ __global__ void __launch_bounds__(THREADS, 1)
       // partial sums: of the first of the CTA's shared tiles in place 0, of the last in place 1
       const size_t place = (size_t)R * p.nt * TM;
       float *mine = p.part + ((size_t)blockIdx.x * 2 + (u - g.len == run.u0 ? 0 : 1)) * place + quarter * 32 + lane;
-      const int last = (t.rows - 1) / CH;  // chunk; the groups take turns
-      if (group > last && lane == 0) mbar_arrive(&accempty[buf]);
-      for (int ch = group; ch <= last; ch += 2) {
-        const int j0 = ch * CH, count = t.rows - j0 < CH ? t.rows - j0 : CH;
-        float v[R][CH];
+      // steps of CH tokens, of one accumulator or of a gate's two; the groups take turns at them
+      const int steps = PARTS * ((t.rows + CH - 1) / CH);
+      if (group >= steps && lane == 0) mbar_arrive(&accempty[buf]);
+#pragma unroll 1
+      for (int step = group; step < steps; step += 2) {
+        const int part = step % PARTS, j0 = step / PARTS * CH, count = t.rows - j0 < CH ? t.rows - j0 : CH;
+        float v[TOGETHER][CH];
 #pragma unroll
-        for (int q = 0; q < R; ++q) tmem_ld<CH>(acc + (uint32_t)q * p.acc_width + (uint32_t)j0, v[q]);
+        for (int q = 0; q < TOGETHER; ++q) tmem_ld_32x32b_x16(acc + (uint32_t)(part + q) * p.acc_width + (uint32_t)j0, reinterpret_cast<uint32_t (&)[CH]>(v[q]));
         tmem_ld_wait();
-        if (ch + 2 > last) {  // the group's last columns are read: the accumulator may be used again
+        if (step + 2 >= steps) {  // the group's last columns are read: the accumulator may be used again
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&accempty[buf]);
         }
         if (!ok) continue;
         if (whole) {
-          finish<R, GATED, OUT, CH>(ep, v, bias, c, row_of(j0, count), count);
+          finish<GATED, OUT>(ep, v[0], part == 0 ? bias[0] : bias[R - 1], v[TOGETHER - 1], bias[R - 1], c + part * TM, row_of(j0, count), count, p.y_pairs);
         } else {
 #pragma unroll
-          for (int q = 0; q < R; ++q)
+          for (int q = 0; q < TOGETHER; ++q)
 #pragma unroll
             for (int j = 0; j < CH; ++j)
-              if (j < count) __stcg(mine + ((size_t)q * p.nt + j0 + j) * TM, v[q][j]);
+              if (j < count) __stcg(mine + ((size_t)(part + q) * p.nt + j0 + j) * TM, v[q][j]);
         }
       }
       if (!whole) {
@@ -625,23 +618,24 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         epi_sync();
         if (*last_flag) {
-          for (int ch = group; ch <= last; ch += 2) {
-            const int j0 = ch * CH, count = t.rows - j0 < CH ? t.rows - j0 : CH;
-            float v[R][CH];
+#pragma unroll 1
+          for (int step = group; step < steps; step += 2) {
+            const int part = step % PARTS, j0 = step / PARTS * CH, count = t.rows - j0 < CH ? t.rows - j0 : CH;
+            float v[TOGETHER][CH];
 #pragma unroll
-            for (int q = 0; q < R; ++q)
+            for (int q = 0; q < TOGETHER; ++q)
 #pragma unroll
               for (int j = 0; j < CH; ++j) v[q][j] = 0.f;
             for (int cc = cf; cc <= cl; ++cc) {
               const int64_t first = run.start(cc) / p.nst;
               const float *src = p.part + ((size_t)cc * 2 + (first == tile ? 0 : 1)) * place + quarter * 32 + lane;
 #pragma unroll
-              for (int q = 0; q < R; ++q)
+              for (int q = 0; q < TOGETHER; ++q)
 #pragma unroll
                 for (int j = 0; j < CH; ++j)
-                  if (j < count) v[q][j] += __ldcg(src + ((size_t)q * p.nt + j0 + j) * TM);
+                  if (j < count) v[q][j] += __ldcg(src + ((size_t)(part + q) * p.nt + j0 + j) * TM);
             }
-            finish<R, GATED, OUT, CH>(ep, v, bias, c, row_of(j0, count), count);
+            finish<GATED, OUT>(ep, v[0], part == 0 ? bias[0] : bias[R - 1], v[TOGETHER - 1], bias[R - 1], c + part * TM, row_of(j0, count), count, p.y_pairs);
           }
           if (threadIdx.x == 0) p.tickets[cf] = 0u;  // ready for the next call
         }
@@ -826,12 +820,12 @@ bool scaled_mma_takes(const b200_packed_desc *w, const b200_scaled_args *a) {
 }
 
 int32_t launch_scaled_mma(const b200_packed_desc *w, const b200_scaled_args *a, cudaStream_t stream) {
-  // Two accumulators of 112 tokens halve a decode step's stages (57344 x 8192, us: one token 66.1 / 56.1, 33 tokens
-  // 76.8 / 70.5) and load less for many (4096 x 1024 x 16384 113 / 88); between, one of 224 reads the weights once
-  // (128 tokens 110 / 133, 200 tokens 152 / 156, 300 tokens 209 / 220).
+  // Two accumulators of 112 tokens halve a decode step's stages (one token x 57344 x 8192, us: 60 with one, 48 with
+  // two) and load less for many tokens (4096 x 1024 x 16384 93 / 66); between, one of 224 goes over the weights
+  // half as often (128 tokens x 57344 x 8192 85 / 108, 300 tokens 172 / 189, 600 tokens 284 / 356).
   const int64_t rows = scaled::rows_of_one(a);
   if (a->gated) return scaled::dispatch<2, true>(w, a, scaled::single(a) ? 1 : 2, stream);
-  if (rows <= scaled::ACC_COLS / 2 || rows > 2 * scaled::ACC_COLS) return scaled::dispatch<2, false>(w, a, 2, stream);
+  if (rows <= scaled::ACC_COLS / 2 || rows > 1024) return scaled::dispatch<2, false>(w, a, 2, stream);
   return scaled::dispatch<1, false>(w, a, 2, stream);
 }
 
