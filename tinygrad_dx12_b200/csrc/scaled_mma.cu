@@ -25,11 +25,11 @@
 // Two accumulators of a tile's width, so that the epilogue of one tile runs under the products of the
 // next: 2 x 224 columns, and four rotating sets of scale columns beside them.
 //
-// Work split: units are (tile, K stage), laid end to end over experts, weight rows and token tiles; each of
-// G CTAs takes an equal run of them, whatever the matrix or the routing, so that every SM works as long as
-// the others. CTAs so stand at different K, which L2 likes: with whole tiles handed out in turn, so that
-// neighbours read the same rows of x at the same time, 4096 tokens x 1024 x 16384 took 324 us, not 112, and
-// 128 tokens x 57344 x 8192 161, not 106. The units of experts are counted on the device from the plan's offsets: a recorded
+// Work split: G CTAs take the tiles in turn, in the order of experts, weight rows and tokens, so that those
+// of one time share their weights in L2 (64 experts' would not fit). Neighbours read the same rows of x and of the
+// weights, but not at the same time: each CTA begins at a K of its own and goes round (all at the same K, 4096 tokens
+// x 1024 x 16384 took 324 us, not 112). The tiles of the last, partial wave are cut into units, (tile, K stage),
+// laid end to end and shared out equally. The tiles of experts are counted on the device from the plan's offsets: a recorded
 // launch fits every routing. A tile that a run's border cuts is finished by the last of its CTAs to arrive
 // (acquire-release ticket), which adds the fp32 parts in the order of the CTAs: the same bits every time.
 // No CTA waits for another. Every wait is bounded (sm100.cuh).
@@ -80,6 +80,7 @@ struct Params {
   int wtiles, tile_rows;  // tiles of weight rows of one matrix, columns of y in each
   int nt;                 // tokens of a tile, at most
   int grid, stages;
+  int join;               // stages that the joining of a cut tile's parts takes as long as
   int sets;               // of scale columns in turn: no more than stages, whose barriers guard them
   uint32_t stage_bytes, b_off;        // weight codes, then x's
   uint32_t scale_bytes, sfb_off;      // of a slot: weight scales, then x's
@@ -186,21 +187,29 @@ __device__ __forceinline__ int64_t scale_row(const Params &p, int64_t at) {
   return p.xs_rows == B200_ROWS_PAIRS ? pair : pair / p.fan;
 }
 
-// The CTA's run of units, of all that are shared out among `ctas`.
+// The CTA's work: `whole` tiles blockIdx, blockIdx + grid, ..., then units u0 .. u1 of the tiles behind `tiles`,
+// the `units` of which are shared out among `ctas`.
 struct Run {
-  int64_t units, u0, u1;
-  int ctas;
+  int64_t tiles, units, u0, u1;
+  int whole, ctas, turn;
   __device__ __forceinline__ int64_t start(int64_t c) const { return c * units / ctas; }
 };
 struct Seg {
   int64_t tile;
-  int s0, len;  // K stages
+  int s0, len;  // K stages s0, s0 + 1, ... (a whole tile's go on at 0 behind the last)
 };
-// The next part of a tile in the run; `u` goes through its units.
-__device__ __forceinline__ bool next_seg(const Params &p, const Run &run, int64_t &u, Seg &g) {
+// The k-th part of the CTA's work; `u` goes through the shared units.
+__device__ __forceinline__ bool next_seg(const Params &p, const Run &run, int &k, int64_t &u, Seg &g) {
+  if (k < run.whole) {
+    g.tile = blockIdx.x + (int64_t)k * p.grid;
+    g.s0 = run.turn, g.len = p.nst;
+    ++k;
+    return true;
+  }
   if (u >= run.u1) return false;
-  g.tile = u / p.nst;
-  g.s0 = (int)(u - g.tile * p.nst);
+  const int64_t t = u / p.nst;
+  g.tile = run.tiles + t;
+  g.s0 = (int)(u - t * p.nst);
   g.len = (int)(p.nst - g.s0 < run.u1 - u ? p.nst - g.s0 : run.u1 - u);
   u += g.len;
   return true;
@@ -353,27 +362,34 @@ __global__ void __launch_bounds__(THREADS, 1)
   const uint32_t tmem = *tmem_slot;
   Run run;
   {
-    run.units = (p.experts > 0 ? (int64_t)before[p.experts] : (int64_t)tiles_of(p, (int)p.rows)) * p.wtiles * p.nst;
+    const int64_t all = (p.experts > 0 ? (int64_t)before[p.experts] : (int64_t)tiles_of(p, (int)p.rows)) * p.wtiles;
+    const int waves = (int)(all / p.grid), rest = (int)(all % p.grid);
+    // The tiles of the last, partial wave: cut up if that is worth the joining of parts
+    const bool cut = p.nst - (int)((int64_t)rest * p.nst / p.grid) > p.join;
+    run.whole = waves + (!cut && (int)blockIdx.x < rest ? 1 : 0);
+    run.tiles = (int64_t)waves * p.grid;
+    run.units = cut ? (int64_t)rest * p.nst : 0;
+    run.turn = (int)((int64_t)blockIdx.x * p.nst / p.grid);
     const int64_t most = run.units / MIN_UNITS;
     run.ctas = (int)(most < 1 ? 1 : most < p.grid ? most : p.grid);
     run.u0 = (int)blockIdx.x < run.ctas ? run.start(blockIdx.x) : 0;
     run.u1 = (int)blockIdx.x < run.ctas ? run.start(blockIdx.x + 1) : 0;
   }
-  const int64_t n = run.u1 - run.u0;  // stages
+  const int64_t n = (int64_t)run.whole * p.nst + run.u1 - run.u0;  // stages
 
   if (warp >= W_WARP0) {
     // ---------------- TMA of weight codes: warp w takes the stages i = w (mod W_WARPS) ----------------
     if (lane == 0) {
       const int turn = warp - W_WARP0, turns = S < W_WARPS ? S : W_WARPS;
       int64_t i = turn, u = run.u0, row = 0, first = 0;
-      int s = turn, slot = turn;  // s: stages into the segment, behind its end until the next is taken
+      int s = turn, k = 0, slot = turn;  // s: stages into the segment, behind its end until the next is taken
       Seg g = {0, 0, 0};
       uint32_t round = 0;
       int early_x[MAX_STAGES / W_WARPS + 1], early_row[MAX_STAGES / W_WARPS + 1], early_slot[MAX_STAGES / W_WARPS + 1], held = 0;
       for (; i < n && turn < turns; i += turns) {
         while (s >= g.len) {
           s -= g.len;
-          if (!next_seg(p, run, u, g)) break;
+          if (!next_seg(p, run, k, u, g)) break;
           const Tile t = tile_at(p, before, start, g.tile);
           row = t.e * p.n + t.w0;
           first = p.single_row ? 0 : t.first;
@@ -381,7 +397,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (round > 0 && !mbar_wait(&empty[slot], (round - 1u) & 1u, abort_flag)) break;
         uint8_t *st = ring + (size_t)slot * p.stage_bytes;
         mbar_arrive_expect_tx(&full[slot], p.tx);
-        const int x = (g.s0 + s) * KS;
+        const int x = (g.s0 + s < p.nst ? g.s0 + s : g.s0 + s - p.nst) * KS;
         tma_load_2d(st, &tmw, x, (int32_t)row, &full[slot]);
         if constexpr (R == 2) tma_load_2d(st + TM * KS, &tmw, x, (int32_t)(row + p.second), &full[slot]);
         if (round > 0) {
@@ -409,12 +425,12 @@ __global__ void __launch_bounds__(THREADS, 1)
     const bool mine = atom < R;  // weights, which are no result of the kernel before
     if (!mine) asm volatile("griddepcontrol.wait;" ::: "memory");
     uint8_t *dst = scales + atom * 512 + lane * 16;
-    int slot = 0;
+    int slot = 0, k = 0;
     uint32_t round = 0;
     int64_t u = run.u0;
     Seg g;
     bool ok = true;
-    while (ok && next_seg(p, run, u, g)) {
+    while (ok && next_seg(p, run, k, u, g)) {
       const Tile t = tile_at(p, before, start, g.tile);
       const uint8_t *src[4];  // of rows lane, lane + 32, ...: null where there are none
 #pragma unroll
@@ -442,18 +458,22 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
         }
       };
-      const int end = g.s0 + g.len;
+      // stages begin .. end - 1, and behind the last those before the first
+      int begin = g.s0, end = g.s0 + g.len < p.nst ? g.s0 + g.len : p.nst, left = g.len;
       uint32_t now[4][4], next[4][4];
-      load(g.s0 & ~3, next);
-      for (int s = g.s0 & ~3; s < end && ok; s += 4) {
+      load(begin & ~3, next);
+      for (int s = begin & ~3; left > 0 && ok; s += 4) {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
 #pragma unroll
           for (int j = 0; j < 4; ++j) now[q][j] = next[q][j];
-        if (s + 4 < end) load(s + 4, next);
+        const int first = begin, behind = end, at = s;
+        left -= (at + 4 < behind ? at + 4 : behind) - (at > first ? at : first);
+        if (s + 4 >= end) s = -4, begin = 0, end = left;  // from the first stage on
+        if (left > 0) load(s + 4, next);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if (s + j < g.s0 || s + j >= end || !ok) continue;
+          if (at + j < first || at + j >= behind || !ok) continue;
           if (round > 0) ok = __all_sync(0xffffffffu, mbar_wait(&frees[slot], (round - 1u) & 1u, abort_flag));
           if (!ok) continue;
           *reinterpret_cast<uint4 *>(dst + slot * p.scale_bytes) = make_uint4(now[0][j], now[1][j], now[2][j], now[3][j]);
@@ -470,9 +490,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint64_t off = 0;
     uint32_t phase = 0, sphase = 0;  // of the scale set, of the stage
     bool ok = true, over = false;
+    int k = 0;
     int64_t u = run.u0;
     Seg g;
-    while (ok && next_seg(p, run, u, g)) {
+    while (ok && next_seg(p, run, k, u, g)) {
       const Tile t = tile_at(p, before, start, g.tile);
       const int len = g.len;
       ++seg;
@@ -551,10 +572,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int quarter = warp & 3, group = warp >> 2;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     bool ok = true;  // this warp's waits; after one that ran out it still meets the others
-    int seg = 0;
+    int seg = 0, k = 0;
     int64_t u = run.u0;
     Seg g;
-    for (; next_seg(p, run, u, g); ++seg) {
+    for (; next_seg(p, run, k, u, g); ++seg) {
       const bool whole = g.len == p.nst;
       const Tile t = tile_at(p, before, start, g.tile);
       const int c = (int)t.w0 + quarter * 32 + lane;  // column of y; ungated, the second accumulator's is c + 128
@@ -574,7 +595,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       const uint32_t acc = tmem + lane_base + (uint32_t)buf * R * p.acc_width;
       // partial sums: of the first of the CTA's shared tiles in place 0, of the last in place 1
       const size_t place = (size_t)R * p.nt * TM;
-      float *mine = p.part + ((size_t)blockIdx.x * 2 + (u - g.len == run.u0 ? 0 : 1)) * place + quarter * 32 + lane;
+      // four tokens of a row side by side
+      float4 *mine = reinterpret_cast<float4 *>(p.part + ((size_t)blockIdx.x * 2 + (u - g.len == run.u0 ? 0 : 1)) * place) + quarter * 32 + lane;
       // steps of CH tokens, of one accumulator or of a gate's two; the groups take turns at them
       const int steps = PARTS * ((t.rows + CH - 1) / CH);
       if (group >= steps && lane == 0) mbar_arrive(&accempty[buf]);
@@ -597,13 +619,13 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
           for (int q = 0; q < TOGETHER; ++q)
 #pragma unroll
-            for (int j = 0; j < CH; ++j)
-              if (j < count) __stcg(mine + ((size_t)(part + q) * p.nt + j0 + j) * TM, v[q][j]);
+            for (int j = 0; j < CH / 4; ++j)
+              __stcg(mine + ((part + q) * p.nt + j0 + 4 * j) / 4 * TM, make_float4(v[q][4 * j], v[q][4 * j + 1], v[q][4 * j + 2], v[q][4 * j + 3]));
         }
       }
       if (!whole) {
         // the CTAs whose runs hold the tile's first and last unit; the tile's ticket is the first one's
-        const int64_t tile = g.tile, a = tile * p.nst, b = a + p.nst - 1;
+        const int64_t tile = g.tile - run.tiles, a = tile * p.nst, b = a + p.nst - 1;
         int cf = (int)(a * run.ctas / run.units), cl = (int)(b * run.ctas / run.units);
         while (cf > 0 && run.start(cf) > a) --cf;
         while (cf + 1 < run.ctas && run.start(cf + 1) <= a) ++cf;
@@ -626,14 +648,29 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int q = 0; q < TOGETHER; ++q)
 #pragma unroll
               for (int j = 0; j < CH; ++j) v[q][j] = 0.f;
-            for (int cc = cf; cc <= cl; ++cc) {
-              const int64_t first = run.start(cc) / p.nst;
-              const float *src = p.part + ((size_t)cc * 2 + (first == tile ? 0 : 1)) * place + quarter * 32 + lane;
+            for (int cc = cf; cc <= cl; cc += 2) {  // two parts' loads in flight together, added in turn
+              float4 w[2][TOGETHER][CH / 4];
 #pragma unroll
-              for (int q = 0; q < TOGETHER; ++q)
+              for (int h = 0; h < 2; ++h) {
+                const int64_t first = run.start(cc + h < cl ? cc + h : cl) / p.nst;
+                const float4 *src = reinterpret_cast<const float4 *>(p.part + ((size_t)(cc + h < cl ? cc + h : cl) * 2 + (first == tile ? 0 : 1)) * place) +
+                                    quarter * 32 + lane;
 #pragma unroll
-                for (int j = 0; j < CH; ++j)
-                  if (j < count) v[q][j] += __ldcg(src + ((size_t)(part + q) * p.nt + j0 + j) * TM);
+                for (int q = 0; q < TOGETHER; ++q)
+#pragma unroll
+                  for (int j = 0; j < CH / 4; ++j) w[h][q][j] = __ldcg(src + ((part + q) * p.nt + j0 + 4 * j) / 4 * TM);
+              }
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                if (cc + h > cl) break;
+#pragma unroll
+                for (int q = 0; q < TOGETHER; ++q)
+#pragma unroll
+                  for (int j = 0; j < CH / 4; ++j) {
+                    v[q][4 * j] += w[h][q][j].x, v[q][4 * j + 1] += w[h][q][j].y;
+                    v[q][4 * j + 2] += w[h][q][j].z, v[q][4 * j + 3] += w[h][q][j].w;
+                  }
+              }
             }
             finish<GATED, OUT>(ep, v[0], part == 0 ? bias[0] : bias[R - 1], v[TOGETHER - 1], bias[R - 1], c + part * TM, row_of(j0, count), count, p.y_pairs);
           }
@@ -760,6 +797,7 @@ static int32_t launch_t(const b200_packed_desc *w, const b200_scaled_args *a, in
   const uint32_t fmt = w->format == B200_FMT_FP4_E2M1 ? 5u : w->format == B200_FMT_FP6_E2M3 ? 3u : 4u;
   p.idesc = (fmt << 7) | (0u << 10) | (1u << 23) | ((uint32_t)(TM >> 4) << 24);  // B: E4M3; E8M0 scales
   p.grid = sms;
+  p.join = 8 + p.nt * R / 16;
   const size_t part = (size_t)sms * 2 * 2 * ACC_COLS * TM * sizeof(float);
   uint8_t *base = nullptr;
   if (int32_t rc = workspace_of(WS_SCALED, part, TICKETS * sizeof(unsigned int), stream, &base)) return rc;
