@@ -26,7 +26,8 @@
 // next: 2 x 224 columns, and four rotating sets of scale columns beside them.
 //
 // Work split: G CTAs take the tiles in turn, in the order of experts, weight rows and tokens, so that those
-// of one time share their weights in L2 (64 experts' would not fit). Neighbours read the same rows of x and of the
+// of one time share their weights in L2 (64 experts' would not fit; in equal runs of neighbouring tiles 4001 tokens
+// through them took 1730 us, not 1270). Neighbours read the same rows of x and of the
 // weights, but not at the same time: each CTA begins at a K of its own and goes round (all at the same K, 4096 tokens
 // x 1024 x 16384 took 324 us, not 112). The tiles of the last, partial wave are cut into units, (tile, K stage),
 // laid end to end and shared out equally. The tiles of experts are counted on the device from the plan's offsets: a recorded
@@ -57,7 +58,6 @@ constexpr int ACC_COLS = 224;                // columns of an accumulator set: R
 constexpr int SF_SETS = 4;
 constexpr int MAX_STAGES = 12;
 constexpr int MAX_EXPERTS = 1024;
-constexpr int MIN_UNITS = 4;                 // a CTA's run is no shorter: its start costs more than its work otherwise
 constexpr size_t TICKETS = 4096;             // one a CTA
 constexpr int CH = 16;                       // tokens of an epilogue step: more unrolled code does not stay in the instruction cache
 constexpr int SMEM_LIMIT = 227 * 1024;
@@ -80,7 +80,8 @@ struct Params {
   int wtiles, tile_rows;  // tiles of weight rows of one matrix, columns of y in each
   int nt;                 // tokens of a tile, at most
   int grid, stages;
-  int join;               // stages that the joining of a cut tile's parts takes as long as
+  int once;               // an expert's rows are one tile, most often
+  int join, join_part;    // what joining a cut tile costs, in stages, and 16 times that for each part
   int sets;               // of scale columns in turn: no more than stages, whose barriers guard them
   uint32_t stage_bytes, b_off;        // weight codes, then x's
   uint32_t scale_bytes, sfb_off;      // of a slot: weight scales, then x's
@@ -364,14 +365,33 @@ __global__ void __launch_bounds__(THREADS, 1)
   {
     const int64_t all = (p.experts > 0 ? (int64_t)before[p.experts] : (int64_t)tiles_of(p, (int)p.rows)) * p.wtiles;
     const int waves = (int)(all / p.grid), rest = (int)(all % p.grid);
-    // The tiles of the last, partial wave: cut up if that is worth the joining of parts
-    const bool cut = p.nst - (int)((int64_t)rest * p.nst / p.grid) > p.join;
-    run.whole = waves + (!cut && (int)blockIdx.x < rest ? 1 : 0);
-    run.tiles = (int64_t)waves * p.grid;
-    run.units = cut ? (int64_t)rest * p.nst : 0;
     run.turn = (int)((int64_t)blockIdx.x * p.nst / p.grid);
-    const int64_t most = run.units / MIN_UNITS;
-    run.ctas = (int)(most < 1 ? 1 : most < p.grid ? most : p.grid);
+    run.tiles = (int64_t)waves * p.grid;
+    // The tiles of the last, partial wave go whole to as many CTAs, or are cut up among more of them, whichever
+    // ends sooner by what joining the parts costs
+    int least = p.nst;
+    run.ctas = 0;
+    for (int i = 0; i < 10 && rest > 0; ++i) {
+      const int pieces = i == 0 ? 0 : i < 4 ? i + 1 : i < 7 ? 2 * i - 2 : 8 * i - 40;  // all CTAs; 2, 3, 4, 6, 8, 10, 16, 24, 32 a tile
+      const int ctas = i == 0 ? p.grid : rest * pieces;
+      if (ctas > p.grid || ctas <= rest) continue;
+      const int parts = i == 0 ? p.grid / rest + 2 : pieces;
+      const int cost = (rest * p.nst + ctas - 1) / ctas + p.join + parts * p.join_part / 16;
+      if (cost < least) least = cost, run.ctas = ctas;
+    }
+    run.whole = waves + (run.ctas == 0 && (int)blockIdx.x < rest ? 1 : 0);
+    run.units = run.ctas > 0 ? (int64_t)rest * p.nst : 0;
+    // Weights that only one tile of tokens reads gain nothing from tiles in turn: equal runs of all of them, whose first
+    // and last tiles are cut (33 tokens gated, 224 tiles: 58 us; a tile each, then parts of 76: 66), if that ends sooner
+    // than a wave of the rest
+    const int64_t equal = (all * p.nst + p.grid - 1) / p.grid + p.join + 3 * p.join_part / 16;
+    if (p.once && waves > 0 && rest > 0 && equal < (int64_t)(waves + 1) * p.nst) {
+      run.whole = 0;
+      run.tiles = 0;
+      run.units = all * p.nst;
+      run.ctas = p.grid;
+    }
+    if (run.ctas == 0) run.ctas = 1;
     run.u0 = (int)blockIdx.x < run.ctas ? run.start(blockIdx.x) : 0;
     run.u1 = (int)blockIdx.x < run.ctas ? run.start(blockIdx.x + 1) : 0;
   }
@@ -797,7 +817,10 @@ static int32_t launch_t(const b200_packed_desc *w, const b200_scaled_args *a, in
   const uint32_t fmt = w->format == B200_FMT_FP4_E2M1 ? 5u : w->format == B200_FMT_FP6_E2M3 ? 3u : 4u;
   p.idesc = (fmt << 7) | (0u << 10) | (1u << 23) | ((uint32_t)(TM >> 4) << 24);  // B: E4M3; E8M0 scales
   p.grid = sms;
-  p.join = 8 + p.nt * R / 16;
+  // 200 tokens x 4096 x 4096, each tile cut in five: 38 us, 30 of them for the joining; a stage takes 0.45
+  p.once = rows_of_one(a) <= p.nt;
+  p.join = 6;
+  p.join_part = p.nt * R * 14 / 16;
   const size_t part = (size_t)sms * 2 * 2 * ACC_COLS * TM * sizeof(float);
   uint8_t *base = nullptr;
   if (int32_t rc = workspace_of(WS_SCALED, part, TICKETS * sizeof(unsigned int), stream, &base)) return rc;
