@@ -54,13 +54,10 @@ __device__ __forceinline__ uint64_t warp_max(uint64_t v) {
   return (uint64_t)hi << 32 | lo;
 }
 
-// N experts a lane. Key: uint32_t (logits decide) or uint64_t (scores decide).
+// One row, by a warp. N experts a lane. Key: uint32_t (logits decide) or uint64_t (scores decide).
 template <int N, typename Key>
-__global__ void __launch_bounds__(128) route_kernel(const __grid_constant__ RouteParams rp) {
-  const b200_route_args &a = rp.a;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+__device__ __forceinline__ void route_row(const b200_route_args &a, int64_t row) {
   const int lane = threadIdx.x & 31;
-  if (row >= a.rows) return;
   int32_t *indices = a.indices + row * a.k;
   float *weights = a.weights + row * a.k;
   if (a.live != nullptr && row >= *a.live) {
@@ -202,6 +199,12 @@ __global__ void __launch_bounds__(128) route_kernel(const __grid_constant__ Rout
   if (lane < a.k) indices[lane] = chosen, weights[lane] = w * a.scale;
 }
 
+template <int N, typename Key>
+__global__ void __launch_bounds__(128) route_kernel(const __grid_constant__ RouteParams rp) {
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (row < rp.a.rows) route_row<N, Key>(rp.a, row);
+}
+
 // ---- the plan -------------------------------------------------------------------------------------
 struct PlanParams {
   const int32_t *indices;
@@ -293,8 +296,7 @@ __device__ __forceinline__ void place_pieces(const PlanParams &p, int c, int32_t
   }
 }
 
-__global__ void __launch_bounds__(PLAN_THREADS) plan_whole_kernel(const PlanParams p) {
-  extern __shared__ int32_t smem[];
+__device__ __forceinline__ void plan_whole(const PlanParams &p, int32_t *smem) {
   const int bins = p.experts + 1;
   int32_t *base = smem, *hist = smem + bins;
   count_pieces(p, 0, hist);
@@ -307,6 +309,20 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_whole_kernel(const PlanPara
   exclusive(base, bins);
   for (int b = threadIdx.x; b < bins; b += PLAN_THREADS) p.offsets[b] = base[b];
   place_pieces(p, 0, hist, base);
+}
+
+__global__ void __launch_bounds__(PLAN_THREADS) plan_whole_kernel(const PlanParams p) {
+  extern __shared__ int32_t smem[];
+  plan_whole(p, smem);
+}
+
+// A few rows and their plan in one launch of one CTA.
+template <int N, typename Key>
+__global__ void __launch_bounds__(PLAN_THREADS) route_whole_kernel(const __grid_constant__ RouteParams rp, const PlanParams p) {
+  extern __shared__ int32_t smem[];
+  for (int64_t row = threadIdx.x >> 5; row < rp.a.rows; row += PLAN_WARPS) route_row<N, Key>(rp.a, row);
+  __syncthreads();  // the indices are this CTA's own
+  plan_whole(p, smem);
 }
 
 __global__ void __launch_bounds__(PLAN_THREADS) plan_count_kernel(const PlanParams p) {
@@ -392,13 +408,27 @@ static int32_t plan(const int32_t *indices, int64_t pairs, int first, int expert
   return B200_OK;
 }
 
+// Up to this many rows (two a warp) routing and plan are one launch: 4.5 us for one row, in two launches 7.
+constexpr int64_t FEW_ROWS = 2 * PLAN_WARPS;
+
+template <int N, typename Key>
+static int32_t launch_keyed(const RouteParams &rp, cudaStream_t stream) {
+  if (rp.a.rows <= FEW_ROWS && rp.a.rows * rp.a.k <= WHOLE) {
+    const int64_t pairs = rp.a.rows * rp.a.k;
+    const PlanParams p{rp.a.indices, pairs, 0, rp.a.experts, rp.a.offsets, rp.a.order, nullptr, nullptr, chunk_of(pairs), 1};
+    B200_CUDA_TRY((ensure_dynamic_smem<route_whole_kernel<N, Key>>(72 * 1024)));
+    route_whole_kernel<N, Key><<<1, PLAN_THREADS, (size_t)(PLAN_WARPS + 1) * (rp.a.experts + 1) * 4, stream>>>(rp, p);
+    B200_LAUNCH_CHECK();
+    return B200_OK;
+  }
+  route_kernel<N, Key><<<(unsigned)((rp.a.rows + 3) / 4), 128, 0, stream>>>(rp);
+  B200_LAUNCH_CHECK();
+  return plan(rp.a.indices, rp.a.rows * rp.a.k, 0, rp.a.experts, rp.a.offsets, rp.a.order, rp.a.scratch, stream);
+}
+
 template <int N>
 static int32_t launch_route(const RouteParams &rp, bool wide, cudaStream_t stream) {
-  const unsigned ctas = (unsigned)((rp.a.rows + 3) / 4);
-  if (wide) route_kernel<N, uint64_t><<<ctas, 128, 0, stream>>>(rp);
-  else route_kernel<N, uint32_t><<<ctas, 128, 0, stream>>>(rp);
-  B200_LAUNCH_CHECK();
-  return B200_OK;
+  return wide ? launch_keyed<N, uint64_t>(rp, stream) : launch_keyed<N, uint32_t>(rp, stream);
 }
 
 // ---- the weighted sum -------------------------------------------------------------------------------
@@ -493,16 +523,12 @@ int32_t b200_route_experts(const b200_route_args *a, void *stream) {
   cudaStream_t s = (cudaStream_t)stream;
   const RouteParams rp{*a};
   const bool wide = a->bias != nullptr || (a->groups > 1 && a->group_best == 2);
-  if (a->rows > 0) {
-    int32_t rc;
-    if (a->experts <= 64) rc = launch_route<2>(rp, wide, s);
-    else if (a->experts <= 128) rc = launch_route<4>(rp, wide, s);
-    else if (a->experts <= 256) rc = launch_route<8>(rp, wide, s);
-    else if (a->experts <= 512) rc = launch_route<16>(rp, wide, s);
-    else rc = launch_route<32>(rp, wide, s);
-    if (rc != B200_OK) return rc;
-  }
-  return plan(a->indices, a->rows * a->k, 0, a->experts, a->offsets, a->order, a->scratch, s);
+  if (a->rows == 0) return plan(a->indices, 0, 0, a->experts, a->offsets, a->order, a->scratch, s);
+  if (a->experts <= 64) return launch_route<2>(rp, wide, s);
+  if (a->experts <= 128) return launch_route<4>(rp, wide, s);
+  if (a->experts <= 256) return launch_route<8>(rp, wide, s);
+  if (a->experts <= 512) return launch_route<16>(rp, wide, s);
+  return launch_route<32>(rp, wide, s);
 }
 
 int32_t b200_expert_combine(const void *y, int32_t y_dtype, const float *weights, const int32_t *indices, int32_t first,

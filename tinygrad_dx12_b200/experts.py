@@ -68,6 +68,13 @@ class Routing:
             if not t.is_contiguous():
                 raise ValueError(f"{name} must be contiguous")
 
+    @classmethod
+    def _made(cls, indices, weights, offsets, rows, experts, first=0) -> "Routing":
+        """Of tensors that are known to fit."""
+        r = object.__new__(cls)
+        r.__dict__.update(indices=indices, weights=weights, offsets=offsets, rows=rows, experts=experts, first=first)
+        return r
+
     @property
     def device(self) -> torch.device:
         return self.indices.device
@@ -135,20 +142,12 @@ def route_experts(logits: torch.Tensor, k: int, scores: str = "softmax", bias: t
     offsets = torch.empty(experts + 1, dtype=torch.int32, device=device)
     rows = torch.empty(tokens * k, dtype=torch.int32, device=device)
     scratch = _scratch(tokens * k, experts, device)
-    a = RouteArgs()
-    a.logits, a.stride, a.rows, a.dtype, a.experts, a.k = (logits.data_ptr(), logits.stride(0), tokens, _REAL[logits.dtype],
-                                                           experts, k)
-    a.indices, a.weights, a.offsets, a.order = indices.data_ptr(), weights.data_ptr(), offsets.data_ptr(), rows.data_ptr()
-    if bias is not None:
-        a.bias = bias.data_ptr()
-    if live is not None:
-        a.live = live.data_ptr()
-    if scratch is not None:
-        a.scratch = scratch.data_ptr()
-    a.sigmoid, a.groups, a.top_groups, a.group_best = int(scores == "sigmoid"), groups, top_groups, group_best
-    a.renormalize, a.scale = int(renormalize), scale
+    a = RouteArgs(logits.data_ptr(), None if bias is None else bias.data_ptr(), None if live is None else live.data_ptr(),
+                  indices.data_ptr(), weights.data_ptr(), offsets.data_ptr(), rows.data_ptr(),
+                  None if scratch is None else scratch.data_ptr(), tokens, logits.stride(0), _REAL[logits.dtype], experts, k,
+                  int(scores == "sigmoid"), groups, top_groups, group_best, int(renormalize), scale)
     _call("b200_route_experts", device, ctypes.byref(a))
-    return Routing(indices, weights, offsets, rows, experts)
+    return Routing._made(indices, weights, offsets, rows, experts)
 
 
 def plan_experts(indices: torch.Tensor, weights: torch.Tensor, experts: int, first: int = 0) -> Routing:
@@ -172,7 +171,7 @@ def plan_experts(indices: torch.Tensor, weights: torch.Tensor, experts: int, fir
     scratch = _scratch(pairs, experts, device)
     _call("b200_expert_plan", device, indices.data_ptr(), pairs, first, experts, offsets.data_ptr(), rows.data_ptr(),
           None if scratch is None else scratch.data_ptr())
-    return Routing(indices, weights, offsets, rows, experts, first)
+    return Routing._made(indices, weights, offsets, rows, experts, first)
 
 
 def _check_routing(w: PackedTensor, routing: Routing, what: str) -> None:

@@ -75,6 +75,13 @@ class BlockScaled:
         if self.scales.device != self.codes.device:
             raise _elsewhere("scales", self.scales, self.codes.device)
 
+    @classmethod
+    def _made(cls, codes: torch.Tensor, scales: torch.Tensor) -> "BlockScaled":
+        """Of tensors that are known to fit (the checks are a third of a small call's host time)."""
+        x = object.__new__(cls)
+        x.__dict__.update(codes=codes, scales=scales)
+        return x
+
     @property
     def shape(self) -> torch.Size:
         return self.codes.shape
@@ -116,8 +123,8 @@ def _flat(t: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
 
 
 def _blocks(shape, device) -> BlockScaled:
-    return BlockScaled(torch.empty(shape, dtype=_E4M3, device=device),
-                       torch.empty((*shape[:-1], shape[-1] // BLOCK), dtype=_E8M0, device=device))
+    return BlockScaled._made(torch.empty(shape, dtype=_E4M3, device=device),
+                             torch.empty((*shape[:-1], shape[-1] // BLOCK), dtype=_E8M0, device=device))
 
 
 def _norm(x, weight, eps, residual, total, dtype, normalize):
@@ -125,21 +132,21 @@ def _norm(x, weight, eps, residual, total, dtype, normalize):
     cols = shape[-1]
     rows = x.numel() // cols if cols else 0
     y = _blocks(shape, device) if dtype == _E4M3 else torch.empty(shape, dtype=dtype, device=device)
-    if x.numel():
-        a = NormArgs()
+    if rows and cols:
         flat = _flat(x, rows, cols)
-        a.x, a.x_stride, a.x_dtype, a.rows, a.cols = flat.data_ptr(), flat.stride(0), _REAL[x.dtype], rows, cols
+        r = t = r_ptr = t_ptr = w_ptr = ys_ptr = None
+        r_stride = t_stride = t_dtype = w_dtype = 0
         if residual is not None:
             r, t = _flat(residual, rows, cols), total.view(rows, cols)
-            a.residual, a.residual_stride = r.data_ptr(), r.stride(0)
-            a.total, a.total_stride, a.total_dtype = t.data_ptr(), t.stride(0), _REAL[residual.dtype]
+            r_ptr, r_stride, t_ptr, t_stride, t_dtype = r.data_ptr(), r.stride(0), t.data_ptr(), cols, _REAL[residual.dtype]
         if weight is not None:
-            a.weight, a.weight_dtype = weight.data_ptr(), _REAL[weight.dtype]
+            w_ptr, w_dtype = weight.data_ptr(), _REAL[weight.dtype]
         if dtype == _E4M3:
-            a.y, a.y_scales = y.codes.data_ptr(), y.scales.data_ptr()
+            y_ptr, ys_ptr = y.codes.data_ptr(), y.scales.data_ptr()
         else:
-            a.y = y.data_ptr()
-        a.y_dtype, a.normalize, a.eps = _RESULTS[dtype], normalize, eps
+            y_ptr = y.data_ptr()
+        a = NormArgs(flat.data_ptr(), r_ptr, t_ptr, w_ptr, y_ptr, ys_ptr, rows, cols, flat.stride(0), r_stride, t_stride,
+                     _REAL[x.dtype], t_dtype, w_dtype, _RESULTS[dtype], normalize, eps)
         _call("b200_rms_norm", device, ctypes.byref(a))
     return y
 
@@ -247,20 +254,20 @@ def _check_bias(bias, shape, device, name="bias"):
 def _product(x, w, y, rows, bias, activation, gated, residual=None, plan=None, x_rows=0, y_rows=1, general=False):
     """Launches one product of checked operands into y."""
     codes, scales = _dense(x)
-    a = ScaledArgs()
-    a.x, a.x_scales, a.rows = codes.data_ptr(), scales.data_ptr(), rows
+    b_ptr = r_ptr = ys_ptr = o_ptr = p_ptr = None
+    b_dtype = r_dtype = r_stride = experts = fan = 0
     if bias is not None:
-        a.bias, a.bias_dtype = bias.data_ptr(), _REAL[bias.dtype]
+        b_ptr, b_dtype = bias.data_ptr(), _REAL[bias.dtype]
     if residual is not None:
-        a.residual, a.residual_stride, a.residual_dtype = residual.data_ptr(), residual.stride(0), _REAL[residual.dtype]
-    if isinstance(y, BlockScaled):
-        a.y, a.y_scales, a.y_dtype = y.codes.data_ptr(), y.scales.data_ptr(), _RESULTS[_E4M3]
+        r_ptr, r_stride, r_dtype = residual.data_ptr(), residual.stride(0), _REAL[residual.dtype]
+    if type(y) is BlockScaled:
+        y_ptr, ys_ptr, y_dtype = y.codes.data_ptr(), y.scales.data_ptr(), _RESULTS[_E4M3]
     else:
-        a.y, a.y_dtype = y.data_ptr(), _REAL[y.dtype]
+        y_ptr, y_dtype = y.data_ptr(), _REAL[y.dtype]
     if plan is not None:
-        a.offsets, a.order, a.experts = plan.offsets.data_ptr(), plan.rows.data_ptr(), w.shape[0]
-        a.fan, a.x_rows, a.y_rows = plan.k, x_rows, y_rows
-    a.activation, a.gated, a.general = ACTIVATIONS[activation], int(gated), int(general)
+        o_ptr, p_ptr, experts, fan = plan.offsets.data_ptr(), plan.rows.data_ptr(), w.shape[0], plan.k
+    a = ScaledArgs(codes.data_ptr(), scales.data_ptr(), rows, b_ptr, r_ptr, r_stride, y_ptr, ys_ptr, None, o_ptr, p_ptr, experts, fan,
+                   x_rows, y_rows, b_dtype, r_dtype, y_dtype, ACTIVATIONS[activation], int(gated), int(general), 0)
     desc = w.desc()
     # not on the tensor cores, or rows that have to be put in the plan's order first
     if general or w.cols % 128 or desc.data % 32 or desc.scales % 4 or (plan is not None and x_rows != ROWS_PLAN):
@@ -283,7 +290,7 @@ def scaled_linear(x: BlockScaled, w: PackedTensor, bias: torch.Tensor | None = N
     ``BlockScaled`` rows quantised from fp32 (columns a multiple of 32). No gradients."""
     _check_weights(w, 2, "scaled_linear")
     cols = _check_product(x, w, activation, gated, dtype, "scaled_linear")
-    device = x.device
+    device = x.codes.device
     bias = _check_bias(bias, w.shape[:1], device)
     shape = (*x.shape[:-1], cols)
     rows = math.prod(x.shape[:-1])
