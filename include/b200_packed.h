@@ -472,9 +472,21 @@ int32_t b200_expert_plan(const int32_t *indices, int64_t pairs, int32_t first, i
 /* out[t] = residual[t] + sum over j of weights[t, j] * y[t * fan + j], over the pairs whose index lies
  * in first .. first + experts - 1, in fp32 and the order of j, rounded once to out_dtype (F16, BF16,
  * F32). y: F16, BF16 or F32 [tokens * fan, cols], out: [tokens, cols], contiguous. */
-int32_t b200_expert_combine(const void *y, int32_t y_dtype, const float *weights, const int32_t *indices, int32_t first,
-                            int32_t experts, int32_t fan, int64_t tokens, int64_t cols, const void *residual,
-                            int32_t residual_dtype, int64_t residual_stride, void *out, int32_t out_dtype, void *stream);
+typedef struct b200_combine_args {
+  const void *y;
+  const float *weights;
+  const int32_t *indices;
+  const void *residual; /* or NULL                                                        */
+  void *out;
+  int64_t tokens, cols, residual_stride;
+  int32_t y_dtype, residual_dtype, out_dtype;
+  int32_t first, experts, fan;
+} b200_combine_args;
+int32_t b200_expert_combine(const b200_combine_args *args, void *stream);
+
+/* The three in turn: the first product's y is the second one's x, whose y the sum takes. */
+int32_t b200_expert_mlp(const b200_packed_desc *up, const b200_scaled_args *first, const b200_packed_desc *down,
+                        const b200_scaled_args *second, const b200_combine_args *combine, void *stream);
 
 #ifdef __cplusplus
 }

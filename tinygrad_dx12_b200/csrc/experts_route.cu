@@ -531,31 +531,40 @@ int32_t b200_route_experts(const b200_route_args *a, void *stream) {
   return launch_route<32>(rp, wide, s);
 }
 
-int32_t b200_expert_combine(const void *y, int32_t y_dtype, const float *weights, const int32_t *indices, int32_t first,
-                            int32_t experts, int32_t fan, int64_t tokens, int64_t cols, const void *residual,
-                            int32_t residual_dtype, int64_t residual_stride, void *out, int32_t out_dtype, void *stream) {
+int32_t b200_expert_combine(const b200_combine_args *a, void *stream) {
   if (int32_t rc = b200_injected()) return rc;
-  if (!real(y_dtype) || !real(out_dtype) || (residual != nullptr && !real(residual_dtype)) || fan < 1 || tokens < 0 || cols < 0)
+  if (a == nullptr || !real(a->y_dtype) || !real(a->out_dtype) || (a->residual != nullptr && !real(a->residual_dtype)) || a->fan < 1 ||
+      a->tokens < 0 || a->cols < 0)
     return b200_set_error(B200_ERR_INVALID, "expert_combine: float16, bfloat16 or float32 rows");
+  const int64_t tokens = a->tokens, cols = a->cols;
   if (tokens == 0 || cols == 0) return B200_OK;
-  if (y == nullptr || weights == nullptr || indices == nullptr || out == nullptr)
+  if (a->y == nullptr || a->weights == nullptr || a->indices == nullptr || a->out == nullptr)
     return b200_set_error(B200_ERR_INVALID, "expert_combine: null pointer");
+  const int32_t fan = a->fan;
   cudaStream_t s = (cudaStream_t)stream;
-  CombineParams p{y, weights, indices, residual, out, cols, residual_stride, first, experts, fan, y_dtype, residual_dtype, out_dtype};
-  const bool vec = cols % 4 == 0 && (uintptr_t)y % 16 == 0;
+  const CombineParams p{a->y, a->weights, a->indices, a->residual, a->out, cols, a->residual_stride, a->first, a->experts, fan, a->y_dtype,
+                        a->residual_dtype, a->out_dtype};
+  const bool vec = cols % 4 == 0 && (uintptr_t)a->y % 16 == 0;
   for (int64_t t0 = 0; t0 < tokens; t0 += 65535) {  // the grid's second axis
     const int64_t n = tokens - t0 < 65535 ? tokens - t0 : 65535;
     CombineParams q = p;
-    q.y = (const uint8_t *)y + t0 * fan * cols * dt_size(y_dtype);
+    q.y = (const uint8_t *)a->y + t0 * fan * cols * dt_size(a->y_dtype);
     q.weights += t0 * fan;
     q.indices += t0 * fan;
-    if (residual != nullptr) q.residual = (const uint8_t *)residual + t0 * residual_stride * dt_size(residual_dtype);
-    q.out = (uint8_t *)out + t0 * cols * dt_size(out_dtype);
+    if (a->residual != nullptr) q.residual = (const uint8_t *)a->residual + t0 * a->residual_stride * dt_size(a->residual_dtype);
+    q.out = (uint8_t *)a->out + t0 * cols * dt_size(a->out_dtype);
     if (vec) combine_kernel<4><<<dim3((unsigned)((cols + 1023) / 1024), (unsigned)n), 256, 0, s>>>(q);
     else combine_kernel<1><<<dim3((unsigned)((cols + 255) / 256), (unsigned)n), 256, 0, s>>>(q);
     B200_LAUNCH_CHECK();
   }
   return B200_OK;
+}
+
+int32_t b200_expert_mlp(const b200_packed_desc *up, const b200_scaled_args *first, const b200_packed_desc *down,
+                        const b200_scaled_args *second, const b200_combine_args *combine, void *stream) {
+  if (int32_t rc = b200_scaled_linear(up, first, stream)) return rc;
+  if (int32_t rc = b200_scaled_linear(down, second, stream)) return rc;
+  return b200_expert_combine(combine, stream);
 }
 
 }  // extern "C"

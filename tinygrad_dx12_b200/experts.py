@@ -19,7 +19,8 @@ import torch
 from . import _lib
 from .attention import _REAL, _call, _elsewhere
 from .packed import PackedTensor, _require_cuda
-from .scaled import ROWS_PAIRS, ROWS_PLAN, ROWS_TOKENS, _E4M3, BlockScaled, _blocks, _check_bias, _check_product, _check_weights, _flat, _product
+from .scaled import (_E4M3, _RESULTS, BLOCK, ROWS_PAIRS, ROWS_PLAN, ROWS_TOKENS, BlockScaled, _args, _check_bias, _check_product,
+                     _check_weights, _flat, _product, _scratch_bytes)
 
 MAX_EXPERTS, MAX_K, MAX_GROUPS = 1024, 32, 32
 
@@ -34,6 +35,15 @@ class RouteArgs(ctypes.Structure):
                 ("k", ctypes.c_int32), ("sigmoid", ctypes.c_int32), ("groups", ctypes.c_int32),
                 ("top_groups", ctypes.c_int32), ("group_best", ctypes.c_int32), ("renormalize", ctypes.c_int32),
                 ("scale", ctypes.c_float)]
+
+
+class CombineArgs(ctypes.Structure):
+    """``b200_combine_args``."""
+
+    _fields_ = [("y", ctypes.c_void_p), ("weights", ctypes.c_void_p), ("indices", ctypes.c_void_p), ("residual", ctypes.c_void_p),
+                ("out", ctypes.c_void_p), ("tokens", ctypes.c_int64), ("cols", ctypes.c_int64),
+                ("residual_stride", ctypes.c_int64), ("y_dtype", ctypes.c_int32), ("residual_dtype", ctypes.c_int32),
+                ("out_dtype", ctypes.c_int32), ("first", ctypes.c_int32), ("experts", ctypes.c_int32), ("fan", ctypes.c_int32)]
 
 
 @dataclass(frozen=True, eq=False)
@@ -195,10 +205,10 @@ def expert_linear(x: BlockScaled, w: PackedTensor, routing: Routing, bias: torch
     if len(x.shape) != 2 or x.shape[0] not in (routing.tokens, pairs):
         raise ValueError(f"activations must have {routing.tokens} rows, one a token, or {pairs}, one a pair")
     bias = _check_bias(bias, w.shape[:2], x.device)
-    y = _blocks((pairs, cols), x.device) if dtype == _E4M3 else torch.empty((pairs, cols), dtype=dtype, device=x.device)
+    y = BlockScaled._empty((pairs, cols), x.device) if dtype == _E4M3 else torch.empty((pairs, cols), dtype=dtype, device=x.device)
     if pairs and cols:
         _product(x, w, y, pairs, bias, activation, gated, None, routing, ROWS_TOKENS if x.shape[0] == routing.tokens else ROWS_PAIRS,
-                 ROWS_PAIRS, _general)
+                 _general)
     return y
 
 
@@ -235,12 +245,26 @@ def expert_mlp(x: BlockScaled, up: PackedTensor, down: PackedTensor, routing: Ro
     out = torch.empty((tokens, cols), dtype=dtype, device=device)
     if not out.numel():
         return out
-    y = torch.empty((pairs, cols), dtype=torch.float32, device=device)
-    h = _blocks((pairs, inner), device)
-    _product(x, up, h, pairs, up_bias, activation, gated, None, routing, ROWS_TOKENS, ROWS_PLAN, _general)
-    _product(h, down, y, pairs, down_bias, None, False, None, routing, ROWS_PLAN, ROWS_PAIRS, _general)
+    # what lies between, in one allocation: the first product's codes and scales, the pairs' results, scratch
+    codes, scales, keep = x._pointers()
+    f32 = _REAL[torch.float32]
+    first = _args(codes, scales, pairs, 0, 0, _RESULTS[_E4M3], up_bias, activation, gated, None, routing, ROWS_TOKENS, ROWS_PLAN, _general)
+    second = _args(16, 4, pairs, 0, None, f32, down_bias, None, False, None, routing, ROWS_PLAN, ROWS_PAIRS, _general)
+    up_desc, down_desc = up.desc(), down.desc()
+    scratch = max(_scratch_bytes(up_desc, first, up), _scratch_bytes(down_desc, second, down))
+    at, sizes = 0, (pairs * inner, pairs * inner // BLOCK, pairs * cols * 4, scratch)
+    places = []
+    for size in sizes:
+        places.append(at)
+        at += -(-size // 256) * 256
+    work = torch.empty(at, dtype=torch.uint8, device=device)
+    h, hs, y, spare = (work.data_ptr() + place for place in places)
+    first.y, first.y_scales, first.scratch = h, hs, spare
+    second.x, second.x_scales, second.y, second.scratch = h, hs, y, spare
     r = residual
-    _call("b200_expert_combine", device, y.data_ptr(), _REAL[y.dtype], routing.weights.data_ptr(), routing.indices.data_ptr(),
-          routing.first, routing.experts, routing.k, tokens, cols, None if r is None else r.data_ptr(),
-          0 if r is None else _REAL[r.dtype], 0 if r is None else r.stride(0), out.data_ptr(), _REAL[dtype])
+    combine = CombineArgs(y, routing.weights.data_ptr(), routing.indices.data_ptr(), None if r is None else r.data_ptr(), out.data_ptr(),
+                          tokens, cols, 0 if r is None else r.stride(0), f32, 0 if r is None else _REAL[r.dtype], _REAL[dtype],
+                          routing.first, routing.experts, routing.k)
+    _call("b200_expert_mlp", device, ctypes.byref(up_desc), ctypes.byref(first), ctypes.byref(down_desc), ctypes.byref(second),
+          ctypes.byref(combine))
     return out

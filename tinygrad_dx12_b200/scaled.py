@@ -17,7 +17,6 @@ from __future__ import annotations
 
 import ctypes
 import math
-from dataclasses import dataclass
 
 import torch
 
@@ -56,63 +55,75 @@ class ScaledArgs(ctypes.Structure):
                 ("gated", ctypes.c_int32), ("general", ctypes.c_int32), ("reserved", ctypes.c_int32)]
 
 
-@dataclass(frozen=True, eq=False)  # compared by identity, as caches are
 class BlockScaled:
     """Rows of 8-bit values: ``codes`` float8_e4m3fn (..., dim) and ``scales`` float8_e8m0fnu (..., dim / 32),
     a power of two for every 32 values along the last axis. ``quantize`` and ``rms_norm`` make them."""
 
-    codes: torch.Tensor
-    scales: torch.Tensor
+    __slots__ = ("_codes", "_scales", "_raw", "shape", "device")
 
-    def __post_init__(self) -> None:
-        if self.codes.dtype != _E4M3 or self.scales.dtype != _E8M0:
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        if codes.dtype != _E4M3 or scales.dtype != _E8M0:
             raise ValueError("block-scaled rows are float8_e4m3fn codes with float8_e8m0fnu scales")
-        if self.codes.dim() < 1 or self.codes.shape[-1] % BLOCK:
+        if codes.dim() < 1 or codes.shape[-1] % BLOCK:
             raise ValueError(f"block-scaled rows are whole blocks of {BLOCK}")
-        expected = (*self.codes.shape[:-1], self.codes.shape[-1] // BLOCK)
-        if tuple(self.scales.shape) != expected:
+        expected = (*codes.shape[:-1], codes.shape[-1] // BLOCK)
+        if tuple(scales.shape) != expected:
             raise ValueError(f"scales must have shape {expected}")
-        if self.scales.device != self.codes.device:
-            raise _elsewhere("scales", self.scales, self.codes.device)
+        if scales.device != codes.device:
+            raise _elsewhere("scales", scales, codes.device)
+        self._codes, self._scales, self._raw, self.shape, self.device = codes, scales, None, codes.shape, codes.device
 
     @classmethod
-    def _made(cls, codes: torch.Tensor, scales: torch.Tensor) -> "BlockScaled":
-        """Of tensors that are known to fit (the checks are a third of a small call's host time)."""
+    def _empty(cls, shape, device) -> "BlockScaled":
+        """Codes and, behind them, scales in one allocation, which a small call's host time is made of; the tensors
+        are made when asked for. (Scales begin on a multiple of 32 bytes, as codes are whole blocks.)"""
         x = object.__new__(cls)
-        x.__dict__.update(codes=codes, scales=scales)
+        n = math.prod(shape)
+        x._raw = torch.empty(n + n // BLOCK, dtype=torch.uint8, device=device)
+        x._codes, x._scales, x.shape, x.device = None, None, torch.Size(shape), x._raw.device
         return x
 
     @property
-    def shape(self) -> torch.Size:
-        return self.codes.shape
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            self._codes = self._raw[: math.prod(self.shape)].view(_E4M3).view(self.shape)
+        return self._codes
 
     @property
-    def device(self) -> torch.device:
-        return self.codes.device
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            self._scales = self._raw[math.prod(self.shape):].view(_E8M0).view(*self.shape[:-1], self.shape[-1] // BLOCK)
+        return self._scales
+
+    def __repr__(self) -> str:
+        return f"BlockScaled(shape={tuple(self.shape)}, device={self.device})"
+
+    def _pointers(self):
+        """Addresses of contiguous codes and scales on the boundaries that the kernels ask for, and what keeps them."""
+        if self._raw is not None:
+            codes = self._raw.data_ptr()
+            return codes, codes + math.prod(self.shape), None
+        codes, scales = self._codes, self._scales
+        if not codes.is_contiguous() or codes.data_ptr() % 16:
+            codes = codes.clone(memory_format=torch.contiguous_format)
+        if not scales.is_contiguous() or scales.data_ptr() % 4:
+            scales = scales.clone(memory_format=torch.contiguous_format)
+        return codes.data_ptr(), scales.data_ptr(), (codes, scales)
 
     def values(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """What the codes stand for, rounded once (bfloat16 and float32 hold every value whose scale lies in
         [2^-100, 2^100])."""
         if dtype not in _REAL:
             raise ValueError(f"values are float16, bfloat16 or float32, not {dtype}")
-        _require_cuda(self.codes, "block-scaled rows")
-        codes, scales = _dense(self)
-        out = torch.empty(codes.shape, dtype=dtype, device=self.device)
-        if out.numel():
-            cols = codes.shape[-1]
-            _call("b200_scaled_values", self.device, codes.data_ptr(), scales.data_ptr(), codes.numel() // cols, cols,
-                  out.data_ptr(), _REAL[dtype])
+        if self.device.type != "cuda":
+            _require_cuda(self.codes, "block-scaled rows")
+        out = torch.empty(self.shape, dtype=dtype, device=self.device)
+        n = math.prod(self.shape)
+        if n:
+            codes, scales, keep = self._pointers()
+            cols = self.shape[-1]
+            _call("b200_scaled_values", self.device, codes, scales, n // cols, cols, out.data_ptr(), _REAL[dtype])
         return out
-
-
-def _dense(x: BlockScaled):
-    """x's codes and scales, contiguous and on the boundaries that the kernels ask for."""
-    codes, scales = x.codes, x.scales
-    if not codes.is_contiguous() or codes.data_ptr() % 16:
-        codes = codes.clone(memory_format=torch.contiguous_format)
-    if not scales.is_contiguous() or scales.data_ptr() % 4:
-        scales = scales.clone(memory_format=torch.contiguous_format)
-    return codes, scales
 
 
 def _flat(t: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
@@ -122,27 +133,22 @@ def _flat(t: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
     return t if t.stride(1) == 1 or cols == 1 else t.contiguous()
 
 
-def _blocks(shape, device) -> BlockScaled:
-    return BlockScaled._made(torch.empty(shape, dtype=_E4M3, device=device),
-                             torch.empty((*shape[:-1], shape[-1] // BLOCK), dtype=_E8M0, device=device))
-
-
 def _norm(x, weight, eps, residual, total, dtype, normalize):
     device, shape = x.device, x.shape
     cols = shape[-1]
     rows = x.numel() // cols if cols else 0
-    y = _blocks(shape, device) if dtype == _E4M3 else torch.empty(shape, dtype=dtype, device=device)
+    y = BlockScaled._empty(shape, device) if dtype == _E4M3 else torch.empty(shape, dtype=dtype, device=device)
     if rows and cols:
         flat = _flat(x, rows, cols)
-        r = t = r_ptr = t_ptr = w_ptr = ys_ptr = None
+        r = r_ptr = t_ptr = w_ptr = ys_ptr = None
         r_stride = t_stride = t_dtype = w_dtype = 0
         if residual is not None:
-            r, t = _flat(residual, rows, cols), total.view(rows, cols)
-            r_ptr, r_stride, t_ptr, t_stride, t_dtype = r.data_ptr(), r.stride(0), t.data_ptr(), cols, _REAL[residual.dtype]
+            r = _flat(residual, rows, cols)
+            r_ptr, r_stride, t_ptr, t_stride, t_dtype = r.data_ptr(), r.stride(0), total.data_ptr(), cols, _REAL[residual.dtype]
         if weight is not None:
             w_ptr, w_dtype = weight.data_ptr(), _REAL[weight.dtype]
         if dtype == _E4M3:
-            y_ptr, ys_ptr = y.codes.data_ptr(), y.scales.data_ptr()
+            y_ptr, ys_ptr, _ = y._pointers()
         else:
             y_ptr = y.data_ptr()
         a = NormArgs(flat.data_ptr(), r_ptr, t_ptr, w_ptr, y_ptr, ys_ptr, rows, cols, flat.stride(0), r_stride, t_stride,
@@ -251,27 +257,40 @@ def _check_bias(bias, shape, device, name="bias"):
     return bias if bias.is_contiguous() else bias.contiguous()
 
 
-def _product(x, w, y, rows, bias, activation, gated, residual=None, plan=None, x_rows=0, y_rows=1, general=False):
-    """Launches one product of checked operands into y."""
-    codes, scales = _dense(x)
-    b_ptr = r_ptr = ys_ptr = o_ptr = p_ptr = None
+def _args(x, xs, rows, y, ys, y_dtype, bias, activation, gated, residual=None, plan=None, x_rows=0, y_rows=1, general=False,
+          scratch=None) -> ScaledArgs:
+    """Arguments of one product: pointers of x and y, checked operands."""
+    b_ptr = r_ptr = o_ptr = p_ptr = None
     b_dtype = r_dtype = r_stride = experts = fan = 0
     if bias is not None:
         b_ptr, b_dtype = bias.data_ptr(), _REAL[bias.dtype]
     if residual is not None:
         r_ptr, r_stride, r_dtype = residual.data_ptr(), residual.stride(0), _REAL[residual.dtype]
-    if type(y) is BlockScaled:
-        y_ptr, ys_ptr, y_dtype = y.codes.data_ptr(), y.scales.data_ptr(), _RESULTS[_E4M3]
-    else:
-        y_ptr, y_dtype = y.data_ptr(), _REAL[y.dtype]
     if plan is not None:
-        o_ptr, p_ptr, experts, fan = plan.offsets.data_ptr(), plan.rows.data_ptr(), w.shape[0], plan.k
-    a = ScaledArgs(codes.data_ptr(), scales.data_ptr(), rows, b_ptr, r_ptr, r_stride, y_ptr, ys_ptr, None, o_ptr, p_ptr, experts, fan,
-                   x_rows, y_rows, b_dtype, r_dtype, y_dtype, ACTIVATIONS[activation], int(gated), int(general), 0)
+        o_ptr, p_ptr, experts, fan = plan.offsets.data_ptr(), plan.rows.data_ptr(), plan.experts, plan.indices.shape[1]
+    return ScaledArgs(x, xs, rows, b_ptr, r_ptr, r_stride, y, ys, scratch, o_ptr, p_ptr, experts, fan, x_rows, y_rows, b_dtype,
+                      r_dtype, y_dtype, ACTIVATIONS[activation], int(gated), int(general), 0)
+
+
+def _scratch_bytes(desc, a: ScaledArgs, w: PackedTensor) -> int:
+    """What the product needs besides: the general kernel's sums, or rows in the plan's order."""
+    if a.general or w.shape[-1] % 128 or desc.data % 32 or desc.scales % 4 or (a.experts and a.x_rows != ROWS_PLAN):
+        return _lib.lib().b200_scaled_linear_scratch(ctypes.byref(desc), ctypes.byref(a))
+    return 0
+
+
+def _product(x, w, y, rows, bias, activation, gated, residual=None, plan=None, x_rows=0, general=False):
+    """Launches one product of checked operands into y."""
+    codes, scales, keep = x._pointers()
+    if type(y) is BlockScaled:
+        y_ptr, ys_ptr, _ = y._pointers()
+        y_dtype = _RESULTS[_E4M3]
+    else:
+        y_ptr, ys_ptr, y_dtype = y.data_ptr(), None, _REAL[y.dtype]
+    a = _args(codes, scales, rows, y_ptr, ys_ptr, y_dtype, bias, activation, gated, residual, plan, x_rows, ROWS_PAIRS, general)
     desc = w.desc()
-    # not on the tensor cores, or rows that have to be put in the plan's order first
-    if general or w.cols % 128 or desc.data % 32 or desc.scales % 4 or (plan is not None and x_rows != ROWS_PLAN):
-        size = _lib.lib().b200_scaled_linear_scratch(ctypes.byref(desc), ctypes.byref(a))
+    size = _scratch_bytes(desc, a, w)
+    if size:
         scratch = torch.empty(size, dtype=torch.uint8, device=x.device)
         a.scratch = scratch.data_ptr()
     _call("b200_scaled_linear", x.device, ctypes.byref(desc), ctypes.byref(a))
@@ -290,7 +309,7 @@ def scaled_linear(x: BlockScaled, w: PackedTensor, bias: torch.Tensor | None = N
     ``BlockScaled`` rows quantised from fp32 (columns a multiple of 32). No gradients."""
     _check_weights(w, 2, "scaled_linear")
     cols = _check_product(x, w, activation, gated, dtype, "scaled_linear")
-    device = x.codes.device
+    device = x.device
     bias = _check_bias(bias, w.shape[:1], device)
     shape = (*x.shape[:-1], cols)
     rows = math.prod(x.shape[:-1])
@@ -300,7 +319,7 @@ def scaled_linear(x: BlockScaled, w: PackedTensor, bias: torch.Tensor | None = N
         if residual.device != device:
             raise _elsewhere("residual", residual, device)
         residual = _flat(residual, rows, cols)
-    y = _blocks(shape, device) if dtype == _E4M3 else torch.empty(shape, dtype=dtype, device=device)
+    y = BlockScaled._empty(shape, device) if dtype == _E4M3 else torch.empty(shape, dtype=dtype, device=device)
     if rows and cols:
         _product(x, w, y, rows, bias, activation, gated, residual, general=_general)
     return y
