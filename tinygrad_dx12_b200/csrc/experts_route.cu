@@ -4,13 +4,15 @@
 // Routing: a warp a row, expert e in lane e % 32. Choices become whole numbers that order like them (0:
 // cannot be chosen), 32 bits where the logits decide and 64 where scores do, so a round of the k best is
 // a warp-wide maximum, and a tie a warp-wide minimum of the index: no sort, and the same choice whatever
-// else runs. Scores that decide are computed in 64 bits: two experts whose scores differ by less than
-// fp32 resolves are ordered as their definition has it.
+// else runs. Scores that decide are compared in 64 bits wherever 32 are not sure of the order: two experts
+// whose scores differ by less than fp32 resolves are ordered as their definition has it.
 // Plan: a stable counting sort of the pairs by expert. CTAs count their chunk's pairs, one warp an expert
 // sums the counts over the chunks, and each CTA places its chunk: warps own consecutive pieces of it, so a
 // pair's place is what lies before it in earlier chunks, earlier warps, earlier rounds and lower lanes.
 // No atomics on places: the order is the same every time. Few pairs take one launch of one CTA.
 // Bound by the launches up to some ten thousand pairs, then by HBM (logits).
+#include <type_traits>
+
 #include "kernels.h"
 #include "common.cuh"
 
@@ -18,7 +20,7 @@ namespace b200 {
 namespace route {
 
 constexpr int MAX_EXPERTS = 1024, MAX_K = 32, MAX_GROUPS = 32;
-constexpr int PLAN_WARPS = 16, PLAN_THREADS = 32 * PLAN_WARPS;
+constexpr int PLAN_WARPS = 32, PLAN_THREADS = 32 * PLAN_WARPS;
 
 struct RouteParams {
   b200_route_args a;
@@ -33,8 +35,35 @@ __device__ __forceinline__ uint64_t order64(double v) {
   const uint64_t u = (uint64_t)__double_as_longlong(v);
   return u ^ ((u >> 63) ? ~0ull : 1ull << 63);
 }
+__device__ __forceinline__ float value32(uint32_t k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu)); }
+// The same of a 16-bit logit that was widened: 16 bits, never 0.
+__device__ __forceinline__ uint32_t packed16(uint32_t k, int dtype) {
+  if (dtype == B200_DT_BF16) return k >> 16;
+  const uint32_t h = (uint32_t)__half_as_ushort(__float2half_rz(value32(k)));  // exact, but for what stood for infinity
+  return h ^ ((h >> 15) ? 0xFFFFu : 0x8000u);
+}
 __device__ __forceinline__ double value64(uint64_t k) {
   return __longlong_as_double((long long)(k ^ ((k >> 63) ? 1ull << 63 : ~0ull)));
+}
+
+// Launched behind a kernel that lets its followers start early: everything waits for it, and lets others start.
+__device__ __forceinline__ void follow() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+template <typename... KArgs, typename... Args>
+static cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -47,24 +76,40 @@ __device__ __forceinline__ double warp_sum(double v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-__device__ __forceinline__ uint32_t warp_max(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
-__device__ __forceinline__ uint64_t warp_max(uint64_t v) {
-  const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32));
-  const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
-  return (uint64_t)hi << 32 | lo;
+// The lanes that hold the warp's largest key; empty if it is 0 everywhere. The low half is only compared where
+// the high halves tie.
+__device__ __forceinline__ uint32_t holders(uint32_t v) {
+  const uint32_t top = __reduce_max_sync(0xffffffffu, v);
+  return __ballot_sync(0xffffffffu, v == top && top != 0);
+}
+__device__ __forceinline__ uint32_t holders(uint64_t v) {
+  const uint32_t hi = (uint32_t)(v >> 32), top = __reduce_max_sync(0xffffffffu, hi);
+  uint32_t who = __ballot_sync(0xffffffffu, hi == top && v != 0);
+  if (who & (who - 1)) {
+    const uint32_t low = __reduce_max_sync(0xffffffffu, (who >> (threadIdx.x & 31) & 1u) ? (uint32_t)v : 0u);
+    who &= __ballot_sync(0xffffffffu, (uint32_t)v == low);
+  }
+  return who;
 }
 
-// One row, by a warp. N experts a lane. Key: uint32_t (logits decide) or uint64_t (scores decide).
-template <int N, typename Key>
-__device__ __forceinline__ void route_row(const b200_route_args &a, int64_t row) {
+// What a key is made of: a 16-bit logit and the index below it (one maximum a round finds both); a logit; a score
+// in 32 bits; a score in 64 bits.
+enum Mode { PACKED, LOGIT, QUICK, EXACT };
+
+// One row, by a warp, N experts a lane. Scores that decide are compared in 32 bits first: where two neighbours in the
+// order of what is chosen, or the last chosen and the next, lie closer than 32 bits are sure of, the answer is false
+// and the row is done again in 64 (a row of 256 experts in 64 bits takes 4500 instructions, half of them exponentials).
+template <int N, Mode MODE>
+__device__ __forceinline__ bool route_row(const b200_route_args &a, int64_t row) {
+  constexpr bool WIDE = MODE == EXACT, SCORES = MODE == EXACT || MODE == QUICK;
+  using Key = typename std::conditional<WIDE, uint64_t, uint32_t>::type;
   const int lane = threadIdx.x & 31;
   int32_t *indices = a.indices + row * a.k;
   float *weights = a.weights + row * a.k;
   if (a.live != nullptr && row >= *a.live) {
     if (lane < a.k) indices[lane] = -1, weights[lane] = 0.f;
-    return;
+    return true;
   }
-  constexpr bool WIDE = sizeof(Key) == 8;
   // logits; -inf for what cannot be chosen by them
   float x[N];
   float top = -INFINITY;
@@ -73,7 +118,9 @@ __device__ __forceinline__ void route_row(const b200_route_args &a, int64_t row)
     const int e = lane + 32 * i;
     float v = -INFINITY;
     if (e < a.experts) {
-      v = load_as_f32(a.logits, row * a.stride + e, a.dtype);
+      v = a.dtype == B200_DT_F32    ? ((const float *)a.logits)[row * a.stride + e]
+          : a.dtype == B200_DT_F16 ? __half2float(((const __half *)a.logits)[row * a.stride + e])
+                                   : __bfloat162float(((const __nv_bfloat16 *)a.logits)[row * a.stride + e]);
       v = v != v ? -INFINITY : fminf(v, 3.402823466e38f);
     }
     x[i] = v;
@@ -81,14 +128,15 @@ __device__ __forceinline__ void route_row(const b200_route_args &a, int64_t row)
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  // the softmax's denominator, over all experts with a logit
+  // the softmax's denominator, over all experts with a logit; weights over their sum do without
   float total = 0.f;
-  if (!a.sigmoid) {
+  if (!a.sigmoid && (!a.renormalize || MODE == QUICK)) {
 #pragma unroll
     for (int i = 0; i < N; ++i) total += x[i] == -INFINITY ? 0.f : expf(x[i] - top);
     total = warp_sum(total);
   }
   Key key[N];
+  float span = 0.f;  // the largest |bias|
   if constexpr (WIDE) {
     double all = 1.0;
     if (!a.sigmoid) {
@@ -109,48 +157,89 @@ __device__ __forceinline__ void route_row(const b200_route_args &a, int64_t row)
       }
       key[i] = order64(c == 0.0 ? 0.0 : c);  // one zero
     }
+  } else if constexpr (MODE == QUICK) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      key[i] = 0;
+      if (x[i] == -INFINITY) continue;
+      float c = a.sigmoid ? 1.f / (1.f + expf(-x[i])) : expf(x[i] - top) / total;
+      if (a.bias != nullptr) {
+        const float b = a.bias[lane + 32 * i];
+        if (b != b || b == -INFINITY) continue;
+        c += fminf(b, 3.402823466e38f);
+        span = fmaxf(span, fabsf(b));
+      }
+      key[i] = order32(c == 0.f ? 0.f : c);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) span = fmaxf(span, __shfl_xor_sync(0xffffffffu, span, o));
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) key[i] = x[i] == -INFINITY ? 0u : order32(x[i] == 0.f ? 0.f : x[i]);
+    for (int i = 0; i < N; ++i) {
+      key[i] = x[i] == -INFINITY ? 0u : order32(x[i] == 0.f ? 0.f : x[i]);
+      if (MODE == PACKED && key[i] != 0) key[i] = (packed16(key[i], a.dtype) << 16) | (0xFFFFu - (uint32_t)(lane + 32 * i));
+    }
   }
+  // A score's error in 32 bits is below 2e-6 of it (the exponential's, its sum's, the division's), and a score is at
+  // most |choice| + the largest |bias|: two choices or sums that differ by this or less may be in either order.
+  auto close = [&](float higher, float lower) { return higher - lower <= 8e-6f * (fabsf(higher) + span); };
   if (a.groups > 1) {
     const int size = a.experts / a.groups;
     Key mine = 0;  // lane g: the rank of group g
     for (int g = 0; g < a.groups; ++g) {
+      const int low = g * size, high = low + size;
       Key best = 0;
       int at = -1;  // this lane's own best
 #pragma unroll
       for (int i = 0; i < N; ++i) {
+        if (32 * i + 31 < low || 32 * i >= high) continue;  // no lane's
         const int e = lane + 32 * i;
-        if (e >= g * size && e < (g + 1) * size && key[i] > best) best = key[i], at = i;
+        if (e >= low && e < high && key[i] > best) best = key[i], at = i;
       }
-      Key first = warp_max(best);
-      if constexpr (WIDE) {
-        if (a.group_best == 2 && first != 0) {
-          const uint32_t has = __ballot_sync(0xffffffffu, best == first);
+      const uint32_t who = holders(best);
+      if (who == 0) continue;
+      const int src = __ffs(who) - 1;
+      Key first = __shfl_sync(0xffffffffu, best, src);
+      if constexpr (SCORES) {
+        if (a.group_best == 2) {
           Key second = best;
-          if (lane == __ffs(has) - 1) {  // one lane gives up its best for its next
+          if (lane == src) {  // one lane gives up its best for its next
             second = 0;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
               const int e = lane + 32 * i;
-              if (i != at && e >= g * size && e < (g + 1) * size && key[i] > second) second = key[i];
+              if (i != at && e >= low && e < high && key[i] > second) second = key[i];
             }
           }
-          second = warp_max(second);
-          if (second != 0) {
-            const double sum = value64(first) + value64(second);
-            first = order64(sum == 0.0 ? 0.0 : sum);
+          const uint32_t next = holders(second);
+          if (next != 0) {
+            const Key other = __shfl_sync(0xffffffffu, second, __ffs(next) - 1);
+            if constexpr (WIDE) {
+              const double sum = value64(first) + value64(other);
+              first = order64(sum == 0.0 ? 0.0 : sum);
+            } else {
+              const float sum = value32(first) + value32(other);
+              first = order32(sum == 0.f ? 0.f : sum);
+            }
           }
         }
       }
       if (lane == g) mine = first;
     }
     uint32_t kept = 0;
-    for (int r = 0; r < a.top_groups; ++r) {
-      const Key best = warp_max(mine);
-      if (best == 0) break;
-      const int g = __ffs(__ballot_sync(0xffffffffu, mine == best)) - 1;
+    float before = 0.f;
+    for (int r = 0; r < a.top_groups + (MODE == QUICK ? 1 : 0); ++r) {
+      const uint32_t who = holders(mine);
+      if (who == 0) break;
+      const int g = __ffs(who) - 1;  // the lowest on a tie
+      if constexpr (MODE == QUICK) {  // which groups, not in what order
+        const float score = value32(__shfl_sync(0xffffffffu, mine, g));
+        if (r == a.top_groups) {
+          if (close(before, score)) return false;
+          break;
+        }
+        before = score;
+      }
       kept |= 1u << g;
       if (lane == g) mine = 0;
     }
@@ -162,17 +251,30 @@ __device__ __forceinline__ void route_row(const b200_route_args &a, int64_t row)
   }
   // the k best, round by round: lane j keeps the j-th
   int chosen = -1;
-  float logit = -INFINITY;
-  for (int j = 0; j < a.k; ++j) {
+  float logit = -INFINITY, before = 0.f;
+  for (int j = 0; j < a.k + (MODE == QUICK ? 1 : 0); ++j) {
     Key best = 0;
     float value = 0.f;
-    uint32_t index = 0xFFFFFFFFu;
+    uint32_t index = 0xFFFFFFFFu, at;
 #pragma unroll
     for (int i = 0; i < N; ++i)
       if (key[i] > best) best = key[i], value = x[i], index = lane + 32 * i;  // the lower index on a tie
-    const Key first = warp_max(best);
-    if (first == 0) break;
-    const uint32_t at = __reduce_min_sync(0xffffffffu, best == first ? index : 0xFFFFFFFFu);
+    if constexpr (MODE == PACKED) {
+      const uint32_t first = __reduce_max_sync(0xffffffffu, best);
+      if (first == 0) break;
+      at = 0xFFFFu - (first & 0xFFFFu);
+    } else {
+      const uint32_t who = holders(best);
+      if (who == 0) break;
+      at = __shfl_sync(0xffffffffu, index, __ffs(who) - 1);
+      if (who & (who - 1)) at = __reduce_min_sync(0xffffffffu, (who >> lane & 1u) ? index : 0xFFFFFFFFu);
+      if constexpr (MODE == QUICK) {
+        const float choice = value32(__shfl_sync(0xffffffffu, best, __ffs(who) - 1));
+        if (j > 0 && close(before, choice)) return false;
+        if (j == a.k) break;
+        before = choice;
+      }
+    }
     value = __shfl_sync(0xffffffffu, value, at & 31);
     if (lane == j) chosen = (int)at, logit = value;
 #pragma unroll
@@ -184,8 +286,12 @@ __device__ __forceinline__ void route_row(const b200_route_args &a, int64_t row)
     // scores over their sum, both divided by the largest softmax numerator of the chosen (exp(min(0, the
     // largest logit)) for sigmoids): neither vanishes, however small the scores are
     float most = logit;
+    if constexpr (SCORES) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    } else {
+      most = __shfl_sync(0xffffffffu, most, 0);  // by logits the first chosen has the largest
+    }
     if (chosen >= 0) {
       if (!a.sigmoid) w = expf(logit - most);
       else if (most >= 0.f) w = 1.f / (1.f + expf(-logit));
@@ -197,12 +303,20 @@ __device__ __forceinline__ void route_row(const b200_route_args &a, int64_t row)
     w = a.sigmoid ? 1.f / (1.f + expf(-logit)) : expf(logit - top) / total;
   }
   if (lane < a.k) indices[lane] = chosen, weights[lane] = w * a.scale;
+  return true;
 }
 
-template <int N, typename Key>
+template <int N, Mode MODE>
+__device__ __forceinline__ void route_rows(const b200_route_args &a, int64_t row, int64_t step) {
+  for (; row < a.rows; row += step)
+    if (!route_row<N, MODE>(a, row)) route_row<N, EXACT>(a, row);
+}
+
+template <int N, Mode MODE>
 __global__ void __launch_bounds__(128) route_kernel(const __grid_constant__ RouteParams rp) {
+  follow();
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (row < rp.a.rows) route_row<N, Key>(rp.a, row);
+  route_rows<N, MODE>(rp.a, row, rp.a.rows);
 }
 
 // ---- the plan -------------------------------------------------------------------------------------
@@ -236,6 +350,7 @@ __device__ __forceinline__ void count_pieces(const PlanParams &p, int c, int32_t
   __syncthreads();
   int64_t begin, end;
   piece(p, c, warp, begin, end);
+#pragma unroll 4
   for (int64_t i = begin + lane; i < end; i += 32) atomicAdd(&hist[warp * bins + bin_of(p, i)], 1);
   __syncthreads();
 }
@@ -282,9 +397,11 @@ __device__ __forceinline__ void place_pieces(const PlanParams &p, int c, int32_t
   int64_t begin, end;
   piece(p, c, warp, begin, end);
   int32_t *next = hist + warp * bins;
+  int coming = begin + lane < end ? bin_of(p, begin + lane) : -1;
   for (int64_t i = begin; i < end; i += 32) {
-    const bool live = i + lane < end;
-    const int b = live ? bin_of(p, i + lane) : -1;
+    const int b = coming;
+    const bool live = b >= 0;
+    coming = i + 32 + lane < end ? bin_of(p, i + 32 + lane) : -1;
     const uint32_t same = __match_any_sync(0xffffffffu, b);
     const int at = live ? next[b] : 0;
     __syncwarp();
@@ -313,20 +430,23 @@ __device__ __forceinline__ void plan_whole(const PlanParams &p, int32_t *smem) {
 
 __global__ void __launch_bounds__(PLAN_THREADS) plan_whole_kernel(const PlanParams p) {
   extern __shared__ int32_t smem[];
+  follow();
   plan_whole(p, smem);
 }
 
 // A few rows and their plan in one launch of one CTA.
-template <int N, typename Key>
+template <int N, Mode MODE>
 __global__ void __launch_bounds__(PLAN_THREADS) route_whole_kernel(const __grid_constant__ RouteParams rp, const PlanParams p) {
   extern __shared__ int32_t smem[];
-  for (int64_t row = threadIdx.x >> 5; row < rp.a.rows; row += PLAN_WARPS) route_row<N, Key>(rp.a, row);
+  follow();
+  route_rows<N, MODE>(rp.a, threadIdx.x >> 5, PLAN_WARPS);
   __syncthreads();  // the indices are this CTA's own
   plan_whole(p, smem);
 }
 
 __global__ void __launch_bounds__(PLAN_THREADS) plan_count_kernel(const PlanParams p) {
   extern __shared__ int32_t smem[];
+  follow();
   const int bins = p.experts + 1;
   count_pieces(p, blockIdx.x, smem);
   for (int b = threadIdx.x; b < bins; b += PLAN_THREADS) {
@@ -338,6 +458,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_count_kernel(const PlanPara
 
 // A warp a bin: counts over the chunks become those of earlier chunks.
 __global__ void __launch_bounds__(128) plan_sum_kernel(const PlanParams p) {
+  follow();
   const int b = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (b > p.experts) return;
   int32_t *row = p.counts + (int64_t)b * p.chunks;
@@ -359,6 +480,7 @@ __global__ void __launch_bounds__(128) plan_sum_kernel(const PlanParams p) {
 
 __global__ void __launch_bounds__(PLAN_THREADS) plan_place_kernel(const PlanParams p) {
   extern __shared__ int32_t smem[];
+  follow();
   const int bins = p.experts + 1;
   int32_t *base = smem, *hist = smem + bins;
   for (int b = threadIdx.x; b < bins; b += PLAN_THREADS) base[b] = p.totals[b];
@@ -374,13 +496,13 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_place_kernel(const PlanPara
 }
 
 // Up to this many pairs one CTA does it all.
-constexpr int64_t WHOLE = 8192;
+constexpr int64_t WHOLE = 4096;
 constexpr int MAX_CHUNKS = 256;
 
 static int64_t chunk_of(int64_t pairs) {
   if (pairs <= WHOLE) return (pairs + PLAN_THREADS - 1) / PLAN_THREADS * PLAN_THREADS;
   int64_t c = (pairs + MAX_CHUNKS - 1) / MAX_CHUNKS;
-  c = c < 2048 ? 2048 : c;
+  c = c < 1024 ? 1024 : c;
   return (c + PLAN_THREADS - 1) / PLAN_THREADS * PLAN_THREADS;
 }
 
@@ -388,47 +510,43 @@ static int32_t plan(const int32_t *indices, int64_t pairs, int first, int expert
                     void *scratch, cudaStream_t stream) {
   PlanParams p{indices, pairs, first, experts, offsets, order, nullptr, nullptr, chunk_of(pairs), 1};
   const int bins = experts + 1;
-  const size_t smem = (size_t)(PLAN_WARPS + 1) * bins * 4;  // at most 70 KB
+  const size_t smem = (size_t)(PLAN_WARPS + 1) * bins * 4;  // at most 135 KB
   if (pairs <= WHOLE) {
-    B200_CUDA_TRY((ensure_dynamic_smem<plan_whole_kernel>(72 * 1024)));
-    plan_whole_kernel<<<1, PLAN_THREADS, smem, stream>>>(p);
+    B200_CUDA_TRY((ensure_dynamic_smem<plan_whole_kernel>(140 * 1024)));
+    B200_CUDA_TRY(launch(plan_whole_kernel, dim3(1), PLAN_THREADS, smem, stream, p));
   } else {
     p.chunks = (int)((pairs + p.chunk - 1) / p.chunk);
     p.counts = (int32_t *)scratch;
     p.totals = p.counts + (int64_t)bins * p.chunks;
-    B200_CUDA_TRY((ensure_dynamic_smem<plan_count_kernel>(72 * 1024)));
-    B200_CUDA_TRY((ensure_dynamic_smem<plan_place_kernel>(72 * 1024)));
-    plan_count_kernel<<<p.chunks, PLAN_THREADS, smem, stream>>>(p);
-    B200_LAUNCH_CHECK();
-    plan_sum_kernel<<<(bins + 3) / 4, 128, 0, stream>>>(p);
-    B200_LAUNCH_CHECK();
-    plan_place_kernel<<<p.chunks, PLAN_THREADS, smem, stream>>>(p);
+    B200_CUDA_TRY((ensure_dynamic_smem<plan_count_kernel>(140 * 1024)));
+    B200_CUDA_TRY((ensure_dynamic_smem<plan_place_kernel>(140 * 1024)));
+    B200_CUDA_TRY(launch(plan_count_kernel, dim3((unsigned)p.chunks), PLAN_THREADS, smem, stream, p));
+    B200_CUDA_TRY(launch(plan_sum_kernel, dim3((unsigned)(bins + 3) / 4), 128, 0, stream, p));
+    B200_CUDA_TRY(launch(plan_place_kernel, dim3((unsigned)p.chunks), PLAN_THREADS, smem, stream, p));
   }
-  B200_LAUNCH_CHECK();
   return B200_OK;
 }
 
 // Up to this many rows (two a warp) routing and plan are one launch: 4.5 us for one row, in two launches 7.
 constexpr int64_t FEW_ROWS = 2 * PLAN_WARPS;
 
-template <int N, typename Key>
+template <int N, Mode MODE>
 static int32_t launch_keyed(const RouteParams &rp, cudaStream_t stream) {
   if (rp.a.rows <= FEW_ROWS && rp.a.rows * rp.a.k <= WHOLE) {
     const int64_t pairs = rp.a.rows * rp.a.k;
     const PlanParams p{rp.a.indices, pairs, 0, rp.a.experts, rp.a.offsets, rp.a.order, nullptr, nullptr, chunk_of(pairs), 1};
-    B200_CUDA_TRY((ensure_dynamic_smem<route_whole_kernel<N, Key>>(72 * 1024)));
-    route_whole_kernel<N, Key><<<1, PLAN_THREADS, (size_t)(PLAN_WARPS + 1) * (rp.a.experts + 1) * 4, stream>>>(rp, p);
-    B200_LAUNCH_CHECK();
+    B200_CUDA_TRY((ensure_dynamic_smem<route_whole_kernel<N, MODE>>(140 * 1024)));
+    B200_CUDA_TRY(launch(route_whole_kernel<N, MODE>, dim3(1), PLAN_THREADS, (size_t)(PLAN_WARPS + 1) * (rp.a.experts + 1) * 4, stream, rp, p));
     return B200_OK;
   }
-  route_kernel<N, Key><<<(unsigned)((rp.a.rows + 3) / 4), 128, 0, stream>>>(rp);
-  B200_LAUNCH_CHECK();
+  B200_CUDA_TRY(launch(route_kernel<N, MODE>, dim3((unsigned)((rp.a.rows + 3) / 4)), 128, 0, stream, rp));
   return plan(rp.a.indices, rp.a.rows * rp.a.k, 0, rp.a.experts, rp.a.offsets, rp.a.order, rp.a.scratch, stream);
 }
 
 template <int N>
 static int32_t launch_route(const RouteParams &rp, bool wide, cudaStream_t stream) {
-  return wide ? launch_keyed<N, uint64_t>(rp, stream) : launch_keyed<N, uint32_t>(rp, stream);
+  if (wide) return launch_keyed<N, QUICK>(rp, stream);
+  return rp.a.dtype == B200_DT_F32 ? launch_keyed<N, LOGIT>(rp, stream) : launch_keyed<N, PACKED>(rp, stream);
 }
 
 // ---- the weighted sum -------------------------------------------------------------------------------
@@ -445,6 +563,7 @@ struct CombineParams {
 // VEC neighbouring columns a thread.
 template <int VEC>
 __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ CombineParams p) {
+  follow();
   const int64_t t = blockIdx.y, c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * VEC;
   if (c >= p.cols) return;
   float sum[VEC];
@@ -553,9 +672,8 @@ int32_t b200_expert_combine(const b200_combine_args *a, void *stream) {
     q.indices += t0 * fan;
     if (a->residual != nullptr) q.residual = (const uint8_t *)a->residual + t0 * a->residual_stride * dt_size(a->residual_dtype);
     q.out = (uint8_t *)a->out + t0 * cols * dt_size(a->out_dtype);
-    if (vec) combine_kernel<4><<<dim3((unsigned)((cols + 1023) / 1024), (unsigned)n), 256, 0, s>>>(q);
-    else combine_kernel<1><<<dim3((unsigned)((cols + 255) / 256), (unsigned)n), 256, 0, s>>>(q);
-    B200_LAUNCH_CHECK();
+    if (vec) B200_CUDA_TRY(launch(combine_kernel<4>, dim3((unsigned)((cols + 1023) / 1024), (unsigned)n), 256, 0, s, q));
+    else B200_CUDA_TRY(launch(combine_kernel<1>, dim3((unsigned)((cols + 255) / 256), (unsigned)n), 256, 0, s, q));
   }
   return B200_OK;
 }

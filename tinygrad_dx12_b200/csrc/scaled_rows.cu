@@ -15,6 +15,25 @@
 namespace b200 {
 namespace rows8 {
 
+// Launched behind a kernel that lets its followers start early: everything waits for it, and lets others start.
+__device__ __forceinline__ void follow() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+template <typename... KArgs, typename... Args>
+static cudaError_t launch(void (*kernel)(KArgs...), int64_t ctas, int threads, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 struct NormParams {
   const void *x, *residual, *weight;
   void *total, *y;
@@ -90,6 +109,7 @@ struct E4M3 {};  // y in 8 bits
 // Types: TX of x, TR of the residual and total (TX without one), TY of y. V vectors of 8 values a thread.
 template <typename TX, typename TR, typename TY, int V, bool RESIDUAL, bool NORMALIZE>
 __global__ void __launch_bounds__(1024) norm_kernel(const __grid_constant__ NormParams p) {
+  follow();
   const int64_t row = blockIdx.x;
   const int nvec = (int)(p.cols >> 3);
   float v[V][8];
@@ -166,6 +186,7 @@ __global__ void __launch_bounds__(1024) norm_kernel(const __grid_constant__ Norm
 // Any width, alignment and mix of types: a CTA a row, the row read again after the reduction (from total
 // where there is one). A warp holds 32 neighbouring values, so a block's largest is one warp's.
 __global__ void __launch_bounds__(256) norm_general_kernel(const NormParams p, int xdt, int tdt, int ydt, int normalize) {
+  follow();
   const int64_t row = blockIdx.x;
   const int lane = threadIdx.x & 31;
   float sum = 0.f;
@@ -203,9 +224,8 @@ __global__ void __launch_bounds__(256) norm_general_kernel(const NormParams p, i
 
 template <typename TX, typename TR, typename TY, int V, bool RESIDUAL>
 static int32_t launch_norm(const NormParams &p, int64_t rows, int threads, bool normalize, cudaStream_t stream) {
-  if (normalize) norm_kernel<TX, TR, TY, V, RESIDUAL, true><<<(unsigned)rows, threads, 0, stream>>>(p);
-  else norm_kernel<TX, TR, TY, V, RESIDUAL, false><<<(unsigned)rows, threads, 0, stream>>>(p);
-  B200_LAUNCH_CHECK();
+  if (normalize) B200_CUDA_TRY(launch(norm_kernel<TX, TR, TY, V, RESIDUAL, true>, rows, threads, stream, p));
+  else B200_CUDA_TRY(launch(norm_kernel<TX, TR, TY, V, RESIDUAL, false>, rows, threads, stream, p));
   return B200_OK;
 }
 
@@ -234,6 +254,7 @@ static int32_t typed_norm(const NormParams &p, int64_t rows, int ydt, bool norma
 
 // 16 codes a thread. The product of a code and a power of two is exact but for what `dtype` cannot hold.
 __global__ void __launch_bounds__(256) values_kernel(const uint8_t *codes, const uint8_t *scales, void *out, int dt, int64_t n16) {
+  follow();
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n16; i += (int64_t)gridDim.x * 256) {
     const uint4 u = reinterpret_cast<const uint4 *>(codes)[i];
     const float s = e8m0_to_f32(scales[i >> 1]);
@@ -290,8 +311,7 @@ int32_t b200_rms_norm(const b200_norm_args *a, void *stream) {
     if (a->x_dtype == B200_DT_F16) return typed_norm<__half>(p, a->rows, a->y_dtype, a->normalize != 0, s);
     return typed_norm<__nv_bfloat16>(p, a->rows, a->y_dtype, a->normalize != 0, s);
   }
-  norm_general_kernel<<<(unsigned)a->rows, 256, 0, s>>>(p, a->x_dtype, a->total_dtype, a->y_dtype, a->normalize);
-  B200_LAUNCH_CHECK();
+  B200_CUDA_TRY(launch(norm_general_kernel, a->rows, 256, s, p, (int)a->x_dtype, (int)a->total_dtype, (int)a->y_dtype, (int)a->normalize));
   return B200_OK;
 }
 
@@ -305,9 +325,10 @@ int32_t b200_scaled_values(const void *codes, const void *scales, int64_t rows, 
     return b200_set_error(B200_ERR_INVALID, "scaled_values: null or unaligned pointer");
   const int64_t n16 = rows * cols / 16;
   const int64_t ctas = (n16 + 255) / 256;
-  values_kernel<<<(unsigned)(ctas < 148 * 64 ? ctas : 148 * 64), 256, 0, (cudaStream_t)stream>>>(
-      (const uint8_t *)codes, (const uint8_t *)scales, out, dtype, n16);
-  B200_LAUNCH_CHECK();
+  int sms = 0;
+  B200_CUDA_TRY(device_sms(&sms));
+  B200_CUDA_TRY(launch(values_kernel, ctas < 64 * sms ? ctas : 64 * sms, 256, (cudaStream_t)stream, (const uint8_t *)codes,
+                       (const uint8_t *)scales, out, (int)dtype, n16));
   return B200_OK;
 }
 

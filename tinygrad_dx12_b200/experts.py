@@ -100,7 +100,7 @@ class Routing:
 
 def _scratch(pairs: int, experts: int, device):
     """Memory for the plan's counts; None where one CTA makes it."""
-    if pairs <= 8192:
+    if pairs <= 4096:
         return None
     return torch.empty(_lib.lib().b200_expert_plan_scratch(pairs, experts), dtype=torch.uint8, device=device)
 
