@@ -99,8 +99,9 @@ enum Mode { PACKED, LOGIT, QUICK, EXACT };
 // One row, by a warp, N experts a lane. Scores that decide are compared in 32 bits first: where two neighbours in the
 // order of what is chosen, or the last chosen and the next, lie closer than 32 bits are sure of, the answer is false
 // and the row is done again in 64 (a row of 256 experts in 64 bits takes 4500 instructions, half of them exponentials).
+// `smem` holds the warp's keys where there are groups: lane g goes through group g's.
 template <int N, Mode MODE>
-__device__ __forceinline__ bool route_row(const b200_route_args &a, int64_t row) {
+__device__ __forceinline__ bool route_row(const b200_route_args &a, int64_t row, void *smem) {
   constexpr bool WIDE = MODE == EXACT, SCORES = MODE == EXACT || MODE == QUICK;
   using Key = typename std::conditional<WIDE, uint64_t, uint32_t>::type;
   const int lane = threadIdx.x & 31;
@@ -118,9 +119,9 @@ __device__ __forceinline__ bool route_row(const b200_route_args &a, int64_t row)
     const int e = lane + 32 * i;
     float v = -INFINITY;
     if (e < a.experts) {
-      v = a.dtype == B200_DT_F32    ? ((const float *)a.logits)[row * a.stride + e]
-          : a.dtype == B200_DT_F16 ? __half2float(((const __half *)a.logits)[row * a.stride + e])
-                                   : __bfloat162float(((const __nv_bfloat16 *)a.logits)[row * a.stride + e]);
+      if (a.dtype == B200_DT_F32) v = ((const float *)a.logits)[row * a.stride + e];
+      else if (a.dtype == B200_DT_F16) v = __half2float(((const __half *)a.logits)[row * a.stride + e]);
+      else v = __bfloat162float(((const __nv_bfloat16 *)a.logits)[row * a.stride + e]);
       v = v != v ? -INFINITY : fminf(v, 3.402823466e38f);
     }
     x[i] = v;
@@ -162,7 +163,7 @@ __device__ __forceinline__ bool route_row(const b200_route_args &a, int64_t row)
     for (int i = 0; i < N; ++i) {
       key[i] = 0;
       if (x[i] == -INFINITY) continue;
-      float c = a.sigmoid ? 1.f / (1.f + expf(-x[i])) : expf(x[i] - top) / total;
+      float c = a.sigmoid ? __fdividef(1.f, 1.f + expf(-x[i])) : __fdividef(expf(x[i] - top), total);
       if (a.bias != nullptr) {
         const float b = a.bias[lane + 32 * i];
         if (b != b || b == -INFINITY) continue;
@@ -185,46 +186,33 @@ __device__ __forceinline__ bool route_row(const b200_route_args &a, int64_t row)
   auto close = [&](float higher, float lower) { return higher - lower <= 8e-6f * (fabsf(higher) + span); };
   if (a.groups > 1) {
     const int size = a.experts / a.groups;
-    Key mine = 0;  // lane g: the rank of group g
-    for (int g = 0; g < a.groups; ++g) {
-      const int low = g * size, high = low + size;
-      Key best = 0;
-      int at = -1;  // this lane's own best
+    Key *keys = (Key *)smem;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        if (32 * i + 31 < low || 32 * i >= high) continue;  // no lane's
-        const int e = lane + 32 * i;
-        if (e >= low && e < high && key[i] > best) best = key[i], at = i;
+    for (int i = 0; i < N; ++i)
+      if (lane + 32 * i < a.experts) keys[lane + 32 * i] = key[i];
+    __syncwarp();
+    // lane g: group g's best and next best, from a place of its own on, so that lanes read different banks
+    Key mine = 0, next = 0;
+    if (lane < a.groups) {
+      const Key *group = keys + lane * size;
+      int at = lane % size;
+      for (int j = 0; j < size; ++j) {
+        const Key v = group[at];
+        at = at + 1 == size ? 0 : at + 1;
+        next = max(next, min(mine, v));
+        mine = max(mine, v);
       }
-      const uint32_t who = holders(best);
-      if (who == 0) continue;
-      const int src = __ffs(who) - 1;
-      Key first = __shfl_sync(0xffffffffu, best, src);
       if constexpr (SCORES) {
-        if (a.group_best == 2) {
-          Key second = best;
-          if (lane == src) {  // one lane gives up its best for its next
-            second = 0;
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-              const int e = lane + 32 * i;
-              if (i != at && e >= low && e < high && key[i] > second) second = key[i];
-            }
-          }
-          const uint32_t next = holders(second);
-          if (next != 0) {
-            const Key other = __shfl_sync(0xffffffffu, second, __ffs(next) - 1);
-            if constexpr (WIDE) {
-              const double sum = value64(first) + value64(other);
-              first = order64(sum == 0.0 ? 0.0 : sum);
-            } else {
-              const float sum = value32(first) + value32(other);
-              first = order32(sum == 0.f ? 0.f : sum);
-            }
+        if (a.group_best == 2 && next != 0) {
+          if constexpr (WIDE) {
+            const double sum = value64(mine) + value64(next);
+            mine = order64(sum == 0.0 ? 0.0 : sum);
+          } else {
+            const float sum = value32(mine) + value32(next);
+            mine = order32(sum == 0.f ? 0.f : sum);
           }
         }
       }
-      if (lane == g) mine = first;
     }
     uint32_t kept = 0;
     float before = 0.f;
@@ -243,11 +231,18 @@ __device__ __forceinline__ bool route_row(const b200_route_args &a, int64_t row)
       kept |= 1u << g;
       if (lane == g) mine = 0;
     }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int e = lane + 32 * i;
-      if (e < a.experts && !(kept >> (e / size) & 1u)) key[i] = 0;
+    if (lane < a.groups && !(kept >> lane & 1u)) {
+      int at = lane % size;
+      for (int j = 0; j < size; ++j) {
+        keys[lane * size + at] = 0;
+        at = at + 1 == size ? 0 : at + 1;
+      }
     }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (lane + 32 * i < a.experts) key[i] = keys[lane + 32 * i];
+    __syncwarp();
   }
   // the k best, round by round: lane j keeps the j-th
   int chosen = -1;
@@ -306,17 +301,19 @@ __device__ __forceinline__ bool route_row(const b200_route_args &a, int64_t row)
   return true;
 }
 
-template <int N, Mode MODE>
-__device__ __forceinline__ void route_rows(const b200_route_args &a, int64_t row, int64_t step) {
-  for (; row < a.rows; row += step)
-    if (!route_row<N, MODE>(a, row)) route_row<N, EXACT>(a, row);
+// (the exact one's code apart: a kernel of much straight code waits for its instructions)
+template <int N>
+__device__ __noinline__ void route_row_exactly(const b200_route_args &a, int64_t row, void *smem) {
+  route_row<N, EXACT>(a, row, smem);
 }
 
 template <int N, Mode MODE>
 __global__ void __launch_bounds__(128) route_kernel(const __grid_constant__ RouteParams rp) {
+  __shared__ __align__(8) uint8_t keys[4][N * 32 * 8];
   follow();
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  route_rows<N, MODE>(rp.a, row, rp.a.rows);
+  const int warp = threadIdx.x >> 5;
+  const int64_t row = (int64_t)blockIdx.x * 4 + warp;
+  if (row < rp.a.rows && !route_row<N, MODE>(rp.a, row, keys[warp])) route_row_exactly<N>(rp.a, row, keys[warp]);
 }
 
 // ---- the plan -------------------------------------------------------------------------------------
@@ -439,7 +436,10 @@ template <int N, Mode MODE>
 __global__ void __launch_bounds__(PLAN_THREADS) route_whole_kernel(const __grid_constant__ RouteParams rp, const PlanParams p) {
   extern __shared__ int32_t smem[];
   follow();
-  route_rows<N, MODE>(rp.a, threadIdx.x >> 5, PLAN_WARPS);
+  const int warp = threadIdx.x >> 5;
+  uint8_t *keys = reinterpret_cast<uint8_t *>(smem) + warp * (N * 32 * 8);  // the plan's counts come after
+  for (int64_t row = warp; row < rp.a.rows; row += PLAN_WARPS)
+    if (!route_row<N, MODE>(rp.a, row, keys)) route_row_exactly<N>(rp.a, row, keys);
   __syncthreads();  // the indices are this CTA's own
   plan_whole(p, smem);
 }
@@ -532,12 +532,15 @@ constexpr int64_t FEW_ROWS = 2 * PLAN_WARPS;
 
 template <int N, Mode MODE>
 static int32_t launch_keyed(const RouteParams &rp, cudaStream_t stream) {
-  if (rp.a.rows <= FEW_ROWS && rp.a.rows * rp.a.k <= WHOLE) {
-    const int64_t pairs = rp.a.rows * rp.a.k;
-    const PlanParams p{rp.a.indices, pairs, 0, rp.a.experts, rp.a.offsets, rp.a.order, nullptr, nullptr, chunk_of(pairs), 1};
-    B200_CUDA_TRY((ensure_dynamic_smem<route_whole_kernel<N, MODE>>(140 * 1024)));
-    B200_CUDA_TRY(launch(route_whole_kernel<N, MODE>, dim3(1), PLAN_THREADS, (size_t)(PLAN_WARPS + 1) * (rp.a.experts + 1) * 4, stream, rp, p));
-    return B200_OK;
+  if constexpr (N <= 8) {
+    if (rp.a.rows <= FEW_ROWS) {  // at most 2048 pairs
+      const int64_t pairs = rp.a.rows * rp.a.k;
+      const PlanParams p{rp.a.indices, pairs, 0, rp.a.experts, rp.a.offsets, rp.a.order, nullptr, nullptr, chunk_of(pairs), 1};
+      const size_t counts = (size_t)(PLAN_WARPS + 1) * (rp.a.experts + 1) * 4, keys = (size_t)PLAN_WARPS * N * 32 * 8;
+      B200_CUDA_TRY((ensure_dynamic_smem<route_whole_kernel<N, MODE>>(140 * 1024)));
+      B200_CUDA_TRY(launch(route_whole_kernel<N, MODE>, dim3(1), PLAN_THREADS, counts > keys ? counts : keys, stream, rp, p));
+      return B200_OK;
+    }
   }
   B200_CUDA_TRY(launch(route_kernel<N, MODE>, dim3((unsigned)((rp.a.rows + 3) / 4)), 128, 0, stream, rp));
   return plan(rp.a.indices, rp.a.rows * rp.a.k, 0, rp.a.experts, rp.a.offsets, rp.a.order, rp.a.scratch, stream);
@@ -560,7 +563,8 @@ struct CombineParams {
   int first, experts, fan, ydt, rdt, odt;
 };
 
-// VEC neighbouring columns a thread.
+// VEC neighbouring columns a thread; four pairs' rows are asked for together and added in their order (one after
+// another a token's four took 4 us).
 template <int VEC>
 __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ CombineParams p) {
   follow();
@@ -569,35 +573,43 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Co
   float sum[VEC];
 #pragma unroll
   for (int i = 0; i < VEC; ++i) sum[i] = 0.f;
-  for (int j = 0; j < p.fan; ++j) {
-    const int64_t pair = t * p.fan + j;
-    const int32_t e = p.indices[pair];
-    if (e < p.first || e - p.first >= p.experts) continue;
-    const float w = p.weights[pair];
-    float v[VEC];
-    if constexpr (VEC == 4) {
-      if (p.ydt == B200_DT_F32) {
-        const float4 u = *reinterpret_cast<const float4 *>((const float *)p.y + pair * p.cols + c);
-        v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
-      } else {
-        const uint2 u = *reinterpret_cast<const uint2 *>((const uint16_t *)p.y + pair * p.cols + c);
+  for (int j0 = 0; j0 < p.fan; j0 += 4) {
+    float w[4], v[4][VEC];
+    bool has[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint16_t h = (uint16_t)((i & 2 ? u.y : u.x) >> (16 * (i & 1)));
-          v[i] = p.ydt == B200_DT_F16 ? __half2float(__ushort_as_half(h)) : __uint_as_float((uint32_t)h << 16);
-        }
-      }
-    } else {
-      v[0] = load_as_f32(p.y, pair * p.cols + c, p.ydt);
+    for (int j = 0; j < 4; ++j) {
+      const int64_t pair = t * p.fan + (j0 + j < p.fan ? j0 + j : p.fan - 1);
+      const int32_t e = p.indices[pair];
+      has[j] = j0 + j < p.fan && e >= p.first && e - p.first < p.experts;
+      w[j] = p.weights[pair];
     }
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) sum[i] = fmaf(w, v[i], sum[i]);
+    for (int j = 0; j < 4; ++j) {
+      const int64_t pair = t * p.fan + j0 + j;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[j][i] = 0.f;
+      if (!has[j]) continue;
+      if constexpr (VEC == 4) {
+        if (p.ydt == B200_DT_F32) {
+          const float4 u = *reinterpret_cast<const float4 *>((const float *)p.y + pair * p.cols + c);
+          v[j][0] = u.x, v[j][1] = u.y, v[j][2] = u.z, v[j][3] = u.w;
+          continue;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[j][i] = load_as_f32(p.y, pair * p.cols + c + i, p.ydt);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        if (has[j]) sum[i] = fmaf(w[j], v[j][i], sum[i]);
   }
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) {
+  for (int i = 0; i < VEC; ++i)
     if (p.residual != nullptr) sum[i] += load_as_f32(p.residual, t * p.rstride + c + i, p.rdt);
-    store_f32(p.out, t * p.cols + c + i, p.odt, sum[i]);
-  }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) store_f32(p.out, t * p.cols + c + i, p.odt, sum[i]);
 }
 
 static bool real(int dt) { return dt == B200_DT_F16 || dt == B200_DT_BF16 || dt == B200_DT_F32; }
