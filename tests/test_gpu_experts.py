@@ -249,6 +249,20 @@ def test_expert_token_counts(tg, count):
         H.check(tg.expert_linear(x, w, r, dtype=torch.float32, **kw), v, tol)
 
 
+@pytest.mark.parametrize("tokens,k,experts,n,cols", [(900, 4, 12, 2048, 384), (2000, 1, 3, 4096, 640), (130, 8, 100, 512, 256)])
+def test_expert_waves(tg, tokens, k, experts, n, cols):
+    """Several tiles of tokens an expert and several tiles a CTA."""
+    g = H.generator(tokens)
+    r = some_routing(tg, tokens, k, experts, g, holes=False)
+    w = H.make_weights((experts, n, cols), "fp4_e2m1", g)
+    x = tg.quantize(torch.randn((tokens, cols), device="cuda", generator=g))
+    xx = H.values(x.codes, x.scales)
+    for kw in (dict(), dict(gated=True, activation="silu")):
+        y = tg.expert_linear(x, w, r, dtype=torch.float32, **kw)
+        H.check(y, *pairs64(xx, w, r, None, **kw))
+        assert torch.equal(y, tg.expert_linear(x, w, r, dtype=torch.float32, **kw))
+
+
 def mlp64(x, up, down, r, activation, gated, up_bias, down_bias, residual):
     """(result, tolerance). What lies between is quantised from values known to ``tol``: a code lies within half a step
     (2^-4 of the value, 2^-10 scales) of them, on either side, so the second product is of the 64-bit values and

@@ -134,6 +134,21 @@ def test_norm_weights_and_types(tg, wdtype):
     H.check8(y, want, norm_tol(want, 512))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("cols", [256, 8192, 1000])
+def test_norm_of_sums_in_32_bits(tg, dtype, cols):
+    """fp32 partial sums added into a 16-bit stream, in place."""
+    g = H.generator(cols)
+    x, h = rows((21, cols), g, torch.float32, 3.0), rows((21, cols), g, dtype)
+    t = (x + h.float()).to(dtype)
+    for out in [dtype] + ([E4M3] if cols % 32 == 0 else []):
+        into = h.clone()
+        y, total = tg.rms_norm(x, residual=into, total=into, dtype=out)
+        assert total is into and torch.equal(into, t)
+        want = norm64(t.double(), None, 1e-6)
+        (H.check8 if out == E4M3 else H.check)(y, want, norm_tol(want, cols))
+
+
 def test_norm_in_place_and_views(tg):
     g = H.generator(5)
     x, h = rows((33, 4096), g, torch.bfloat16), rows((33, 4096), g, torch.bfloat16)
@@ -201,6 +216,45 @@ def test_linear_splits(tg, n, k, m):
     x, w = activations(tg, m, k, g), H.make_weights((n, k), "fp6_e3m2", g)
     a = run(tg, x, w, dtype=torch.float32)
     assert torch.equal(a, tg.scaled_linear(x, w, dtype=torch.float32))
+
+
+@pytest.mark.parametrize("m,n,k", [(300, 20032, 640), (40, 30016, 384), (1100, 9472, 1152), (230, 9600, 896), (20, 38016, 128)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_linear_waves(tg, m, n, k, gated):
+    """Several tiles a CTA, each begun at another K; stages that are no multiple of four."""
+    g = H.generator(m + n)
+    x, w = activations(tg, m, k, g), H.make_weights((n, k), "fp6_e2m3", g)
+    a = run(tg, x, w, dtype=torch.float32, gated=gated)
+    assert torch.equal(a, tg.scaled_linear(x, w, dtype=torch.float32, gated=gated))
+    run(tg, x, w, dtype=E4M3, gated=gated, activation="silu")
+
+
+def test_chain_of_dependent_launches(tg):
+    """Norms and products that start as the ones before them end give what they give one by one."""
+    g = H.generator(17)
+    up, down = H.make_weights((1024, 512), "fp4_e2m1", g), H.make_weights((512, 1024), "fp4_e2m1", g)
+    h0 = rows((30, 512), g, torch.bfloat16)
+
+    def layers(wait):
+        h = h0
+        for _ in range(25):
+            x = tg.rms_norm(h, dtype=E4M3)
+            wait()
+            m = tg.scaled_linear(x, up, activation="gelu", dtype=E4M3)
+            wait()
+            h = tg.scaled_linear(m, down, residual=h)
+            wait()
+        return h
+
+    want = layers(torch.cuda.synchronize)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        a = layers(lambda: None)
+        with torch.cuda.stream(side):
+            b = layers(lambda: None)
+        torch.cuda.synchronize()
+        assert torch.equal(a, want) and torch.equal(b, want)
 
 
 @pytest.mark.parametrize("general", [False, True])

@@ -494,6 +494,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if (at + j < first || at + j >= behind || !ok) continue;
+          if (round == 1 && slot == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
           if (round > 0) ok = __all_sync(0xffffffffu, mbar_wait(&frees[slot], (round - 1u) & 1u, abort_flag));
           if (!ok) continue;
           *reinterpret_cast<uint4 *>(dst + slot * p.scale_bytes) = make_uint4(now[0][j], now[1][j], now[2][j], now[3][j]);
@@ -505,6 +506,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   } else if (warp == MMA_WARP) {
     // ---------------- MMA issuer: the whole warp, one lane of it elected ----------------
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // x comes behind it: the bound of a wait does not run until then
     const uint64_t ad = sw128_kmajor_desc(ring), bd = sw128_kmajor_desc(ring + p.b_off);  // the slots' follow: address / 16
     int slot = 0, set = 0, seg = -1;
     uint64_t off = 0;
@@ -552,6 +554,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     __syncwarp();
   } else if (warp == SF_WARP) {
     // ---------------- scales into tensor memory ----------------
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint64_t da = sf_desc(scales), db = sf_desc(scales + p.sfb_off);
     uint64_t off = 0;
     int slot = 0, set = 0, back = 0;  // back: the ring slot of the stage p.sets before, whose MMAs read the set

@@ -271,6 +271,13 @@ __global__ void __launch_bounds__(256) values_kernel(const uint8_t *codes, const
   }
 }
 
+// fp32 x into a 16-bit residual: a projection's partial sums into the stream.
+template <typename TR>
+static int32_t mixed_norm(const NormParams &p, int64_t rows, int ydt, bool normalize, cudaStream_t stream) {
+  return ydt == B200_DT_F8E4M3 ? sized_norm<float, TR, E4M3, true>(p, rows, normalize, stream)
+                               : sized_norm<float, TR, TR, true>(p, rows, normalize, stream);
+}
+
 static bool real(int dt) { return dt == B200_DT_F16 || dt == B200_DT_BF16 || dt == B200_DT_F32; }
 static bool aligned(const void *p, int64_t stride, int64_t rows, int dt) {
   return (uintptr_t)p % 16 == 0 && (rows <= 1 || stride * dt_size(dt) % 16 == 0);
@@ -299,14 +306,18 @@ int32_t b200_rms_norm(const b200_norm_args *a, void *stream) {
   NormParams p{a->x, a->residual, a->normalize ? a->weight : nullptr, a->total, a->y, (uint8_t *)a->y_scales,
                a->cols, a->x_stride, a->residual_stride, a->total_stride, a->weight_dtype, a->eps};
   const bool res = a->residual != nullptr;
-  // rows in registers: one type throughout, whole vectors, at most 32768 values
+  // rows in registers: one type throughout (or fp32 x beside a 16-bit stream), whole vectors, at most 32768 values
+  const int tdt = res ? a->total_dtype : a->x_dtype;
+  const bool mixed = tdt != a->x_dtype;
   const bool fits = a->cols % 8 == 0 && a->cols <= 32768 && aligned(a->x, a->x_stride, a->rows, a->x_dtype) &&
-                    (!res || (a->total_dtype == a->x_dtype && aligned(a->residual, a->residual_stride, a->rows, a->x_dtype) &&
-                              aligned(a->total, a->total_stride, a->rows, a->x_dtype))) &&
+                    (!mixed || a->x_dtype == B200_DT_F32) &&
+                    (!res || (aligned(a->residual, a->residual_stride, a->rows, tdt) && aligned(a->total, a->total_stride, a->rows, tdt))) &&
                     (p.weight == nullptr || (uintptr_t)p.weight % 16 == 0) &&
-                    (eight ? (uintptr_t)a->y % 8 == 0 : a->y_dtype == a->x_dtype && (uintptr_t)a->y % 16 == 0);
+                    (eight ? (uintptr_t)a->y % 8 == 0 : a->y_dtype == tdt && (uintptr_t)a->y % 16 == 0);
   cudaStream_t s = (cudaStream_t)stream;
   if (fits) {
+    if (mixed) return tdt == B200_DT_F16 ? mixed_norm<__half>(p, a->rows, a->y_dtype, a->normalize != 0, s)
+                                         : mixed_norm<__nv_bfloat16>(p, a->rows, a->y_dtype, a->normalize != 0, s);
     if (a->x_dtype == B200_DT_F32) return typed_norm<float>(p, a->rows, a->y_dtype, a->normalize != 0, s);
     if (a->x_dtype == B200_DT_F16) return typed_norm<__half>(p, a->rows, a->y_dtype, a->normalize != 0, s);
     return typed_norm<__nv_bfloat16>(p, a->rows, a->y_dtype, a->normalize != 0, s);

@@ -12,7 +12,6 @@ linalg.py:136-223``). Nothing here reads the routing back to the host, so a step
 from __future__ import annotations
 
 import ctypes
-from dataclasses import dataclass
 
 import torch
 
@@ -46,43 +45,24 @@ class CombineArgs(ctypes.Structure):
                 ("out_dtype", ctypes.c_int32), ("first", ctypes.c_int32), ("experts", ctypes.c_int32), ("fan", ctypes.c_int32)]
 
 
-@dataclass(frozen=True, eq=False)
 class Routing:
-    """Which experts each token goes to, and the order in which the experts read them.
+    """Which experts each token goes to, and the order in which the experts read them; ``route_experts`` and
+    ``plan_experts`` make them.
 
     ``indices`` int32 and ``weights`` float32 (tokens, k): a token's experts and what multiplies their results; an
     index outside ``first`` .. ``first + experts - 1`` (such as -1) stands for no expert here. ``rows`` int32
     (tokens * k): pairs token * k + j in the order of their experts, those of expert first + e at
-    ``offsets[e]`` .. ``offsets[e + 1]`` (int32, experts + 1 of them). ``route_experts`` and ``plan_experts`` make them."""
+    ``offsets[e]`` .. ``offsets[e + 1]`` (int32, experts + 1 of them). The kernels go by offsets and rows as they find them."""
 
-    indices: torch.Tensor
-    weights: torch.Tensor
-    offsets: torch.Tensor
-    rows: torch.Tensor
-    experts: int
-    first: int = 0
+    __slots__ = ("indices", "weights", "offsets", "rows", "experts", "first")
 
-    def __post_init__(self) -> None:
-        if self.indices.dim() != 2 or self.indices.dtype != torch.int32:
-            raise ValueError("indices must be int32 (tokens, k)")
-        if self.weights.shape != self.indices.shape or self.weights.dtype != torch.float32:
-            raise ValueError("weights must be float32 of indices' shape")
-        if self.offsets.shape != (self.experts + 1,) or self.offsets.dtype != torch.int32:
-            raise ValueError(f"offsets must be int32 ({self.experts + 1},)")
-        if self.rows.shape != (self.indices.numel(),) or self.rows.dtype != torch.int32:
-            raise ValueError(f"rows must be int32 ({self.indices.numel()},)")
-        for name in ("indices", "weights", "offsets", "rows"):
-            t = getattr(self, name)
-            if t.device != self.indices.device:
-                raise _elsewhere(name, t, self.indices.device)
-            if not t.is_contiguous():
-                raise ValueError(f"{name} must be contiguous")
+    def __init__(self):
+        raise TypeError("route_experts and plan_experts make routings")
 
     @classmethod
     def _made(cls, indices, weights, offsets, rows, experts, first=0) -> "Routing":
-        """Of tensors that are known to fit."""
         r = object.__new__(cls)
-        r.__dict__.update(indices=indices, weights=weights, offsets=offsets, rows=rows, experts=experts, first=first)
+        r.indices, r.weights, r.offsets, r.rows, r.experts, r.first = indices, weights, offsets, rows, experts, first
         return r
 
     @property
@@ -188,7 +168,7 @@ def _check_routing(w: PackedTensor, routing: Routing, what: str) -> None:
     _check_weights(w, 3, what)
     if w.shape[0] != routing.experts:
         raise ValueError(f"weights of {w.shape[0]} experts do not fit a routing over {routing.experts}")
-    if routing.device != w.device:
+    if routing.indices.device != w.device:
         raise _elsewhere("routing", routing, w.device)
 
 

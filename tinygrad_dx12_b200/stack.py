@@ -18,7 +18,7 @@ stream like a real layer's). With one, q and k are turned by their positions, k 
 into the layer's packed cache, and o's input is the attention of q over it
 (``forward(h, cache, step)``; each rank keeps its own key heads). ``rmsnorm(h) = h * rsqrt(mean(h^2) + 1e-6)`` in fp32 keeps the synthetic activations
 bounded over 32 or 80 layers. Projections run through ``b200_packed_linear`` (fp32
-accumulation); the elementwise steps through ``b200_add_rmsnorm`` / ``b200_gate_mul``; the
+accumulation), or with ``ScaledOps`` on 8-bit activations (``b200_scaled_linear``); the elementwise steps through ``b200_add_rmsnorm`` / ``b200_gate_mul``; the
 all-reduce through ``torch.distributed`` (NCCL between GPUs). Shards are cut from the full
 matrices on the device: rows for column-parallel weights, K columns for row-parallel ones
 (a K shard must start on a byte and scale-block boundary).
@@ -243,6 +243,40 @@ class CudaOps:
         self.add_rmsnorm(h, p, x)
 
 
+class _Rows:
+    """The projections' input of ``ScaledOps``: block-scaled rows, replaced by every norm."""
+
+    value = None
+
+
+class ScaledOps(CudaOps):
+    """CudaOps with 8-bit activations: the norms quantise their rows and the projections multiply them as stored
+    (``rms_norm``, ``scaled_linear``), the gate's product in the epilogue of gate and up. For FP4 and FP6 stacks with
+    E8M0 scales in blocks of 32 (config c5)."""
+
+    def rows(self, h: torch.Tensor) -> _Rows:
+        return _Rows()
+
+    def linear(self, w: PackedTensor, x, out_dtype: torch.dtype) -> torch.Tensor:
+        from .scaled import BlockScaled, quantize, scaled_linear
+
+        x = x.value if isinstance(x, _Rows) else x
+        return scaled_linear(x if isinstance(x, BlockScaled) else quantize(x), w, dtype=out_dtype)
+
+    def gated(self, w: PackedTensor, x: _Rows, out: torch.Tensor, act: torch.dtype):
+        from .scaled import scaled_linear
+
+        return scaled_linear(x.value, w, gated=True, dtype=torch.float8_e4m3fn)
+
+    def add_rmsnorm(self, h: torch.Tensor, partial: torch.Tensor | None, x: _Rows) -> None:
+        from .scaled import rms_norm
+
+        if partial is None:
+            x.value = rms_norm(h, eps=EPS, dtype=torch.float8_e4m3fn)
+        else:
+            x.value, _ = rms_norm(partial, eps=EPS, residual=h, total=h, dtype=torch.float8_e4m3fn)
+
+
 class PeerReducer:
     """Partial buffers shared by all ranks through CUDA IPC, and the fused one-shot reduction.
 
@@ -374,9 +408,10 @@ class TPStack:
             raise ValueError("cache and step go together")
         cfg, ops = self.cfg, self.ops
         m = h.shape[0]
-        x = torch.empty_like(h)
+        x = ops.rows(h) if hasattr(ops, "rows") else torch.empty_like(h)
         mbuf = torch.empty((m, self.layers[0].inter_rows if self.layers else 0), dtype=cfg.act, device=h.device)
         ops.add_rmsnorm(h, None, x)
+        gated = getattr(ops, "gated", None) or (lambda w, xx, out, act: _gated(ops, w, xx, out, act))
         if self.world == 1:  # unsharded: nothing to reduce whatever the process group holds
             row_reduce = lambda w, inp, hh, xx, slot: _local_row_reduce(ops, w, inp, hh, xx)  # noqa: E731
         else:
@@ -386,10 +421,13 @@ class TPStack:
             qkv = ops.linear(L.qkv, x, cfg.act)
             q = qkv[:, :L.q_rows] if cache is None else cache.attend(i, qkv, L.q_rows, step)
             row_reduce(L.o, q, h, x, 0)
-            gu = ops.linear(L.gu, x, cfg.act)
-            ops.gate_mul(gu, mbuf)
-            row_reduce(L.down, mbuf, h, x, 1)
+            row_reduce(L.down, gated(L.gu, x, mbuf, cfg.act), h, x, 1)
         return h
+
+
+def _gated(ops, w, x, out, act):
+    ops.gate_mul(ops.linear(w, x, act), out)
+    return out
 
 
 def _local_row_reduce(ops, w, inp, h, x) -> None:
