@@ -143,42 +143,40 @@ __device__ __forceinline__ void commit(uint64_t *bar) {
       : "memory");
 }
 
-// What a tile is: expert, first weight row within its matrix, place of its first row, rows.
+// What a tile is: expert, first weight row within its matrix, place of its first row, rows; width: rows rounded
+// up to the MMA's N.
 struct Tile {
-  int e;
-  int64_t w0, first;
-  int rows, width;  // width: rows rounded up to the MMA's N
+  int e, w0, first, rows, width;
 };
 
 // Token tiles of `count` rows: as few as hold them, equally full.
-__device__ __forceinline__ int tiles_of(const Params &p, int count) { return (count + p.nt - 1) / p.nt; }
+__device__ __forceinline__ uint32_t tiles_of(const Params &p, int count) { return ((uint32_t)count + p.nt - 1) / (uint32_t)p.nt; }
 
-__device__ __forceinline__ Tile tile_at(const Params &p, const int32_t *before, const int32_t *start, int64_t tile) {
-  int e = 0;
-  int64_t first = 0, count = p.rows, at = tile;
-  if (p.experts > 0) {
-    int lo = 0, hi = p.experts;  // before[lo] <= tile < before[hi]; empty experts have no tiles
-    const int32_t t = (int32_t)(tile / p.wtiles);
+// One copy of it for all warps, in 32 bits: every role asks for every tile, and code of its own that runs once a
+// tile would come from L2 each time (inlined it took the scales' warps 4 us a tile).
+__device__ __noinline__ uint4 find_tile(uint32_t tile, const int32_t *before, const int32_t *start, uint32_t experts, uint32_t rows,
+                                        uint32_t wtiles, uint32_t nt) {
+  uint32_t e = 0, first = 0, count = rows, at = tile;
+  if (experts > 0) {
+    const int32_t t = (int32_t)(tile / wtiles);
+    uint32_t lo = 0, hi = experts;  // before[lo] <= t < before[hi]; empty experts have no tiles
     while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
+      const uint32_t mid = (lo + hi) >> 1;
       if (before[mid] <= t) lo = mid;
       else hi = mid;
     }
     e = lo;
-    at = tile - (int64_t)before[e] * p.wtiles;
-    first = start[e];
-    count = start[e + 1] - start[e];
+    at = tile - (uint32_t)before[e] * wtiles;
+    first = (uint32_t)start[e];
+    count = (uint32_t)start[e + 1] - first;
   }
-  const int tt = tiles_of(p, (int)count);
-  const int per = ((int)(count + tt - 1) / tt + 15) / 16 * 16;
-  const int w = (int)(at / tt), t = (int)(at - (int64_t)w * tt);
-  Tile r;
-  r.e = e;
-  r.w0 = (int64_t)w * p.tile_rows;
-  r.first = first + (int64_t)t * per;
-  r.rows = (int)(count - (int64_t)t * per < per ? count - (int64_t)t * per : per);
-  r.width = (r.rows + 15) / 16 * 16;
-  return r;
+  const uint32_t tt = (count + nt - 1) / nt, per = ((count + tt - 1) / tt + 15) / 16 * 16;
+  const uint32_t w = at / tt, t = at - w * tt;
+  return make_uint4(e, w, first + t * per, count - t * per < per ? count - t * per : per);
+}
+__device__ __forceinline__ Tile tile_at(const Params &p, const int32_t *before, const int32_t *start, int64_t tile) {
+  const uint4 f = find_tile((uint32_t)tile, before, start, (uint32_t)p.experts, (uint32_t)p.rows, (uint32_t)p.wtiles, (uint32_t)p.nt);
+  return Tile{(int)f.x, (int)f.y * p.tile_rows, (int)f.z, (int)f.w, ((int)f.w + 15) / 16 * 16};
 }
 
 // The row of x's scales of place `at`.
@@ -346,7 +344,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     int carry = 0;
     for (int first = 0; first < p.experts; first += 32) {
       const int e = first + lane;
-      const int own = e < p.experts ? tiles_of(p, start[e + 1] - start[e]) : 0;
+      const int own = e < p.experts ? (int)tiles_of(p, start[e + 1] - start[e]) : 0;
       int v = own;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -411,7 +409,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           s -= g.len;
           if (!next_seg(p, run, k, u, g)) break;
           const Tile t = tile_at(p, before, start, g.tile);
-          row = t.e * p.n + t.w0;
+          row = (int64_t)t.e * p.n + t.w0;
           first = p.single_row ? 0 : t.first;
         }
         if (round > 0 && !mbar_wait(&empty[slot], (round - 1u) & 1u, abort_flag)) break;
@@ -457,7 +455,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int q = 0; q < 4; ++q) {
         const int r = lane + 32 * q;
         if (mine) {
-          const int64_t row = t.e * p.n + atom * p.second + t.w0 + r;
+          const int64_t row = (int64_t)t.e * p.n + atom * p.second + t.w0 + r;
           src[q] = row < p.wrows ? p.ws + row * p.nblk : nullptr;
         } else {
           const int at = (atom - R) * 128 + r;
@@ -606,11 +604,11 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
       for (int q = 0; q < R; ++q) {
         const int64_t row = q * p.second + c;
-        bias[q] = ep.bias != nullptr && row < p.n ? load_as_f32(ep.bias, t.e * p.n + row, ep.bdt) : 0.f;
+        bias[q] = ep.bias != nullptr && row < p.n ? load_as_f32(ep.bias, (int64_t)t.e * p.n + row, ep.bdt) : 0.f;
       }
       auto row_of = [&](int j0, int count) -> int {  // of y, of token j0 + lane
-        const int64_t at = t.first + j0 + (lane < count ? lane : 0);
-        return p.y_pairs ? p.order[at] : (int)at;
+        const int at = t.first + j0 + (lane < count ? lane : 0);
+        return p.y_pairs ? p.order[at] : at;
       };
       const int buf = p.bufs == 2 ? seg & 1 : 0;
       ok = __all_sync(0xffffffffu, ok && mbar_wait(&accfull[buf], (uint32_t)((p.bufs == 2 ? seg >> 1 : seg) & 1), abort_flag));
@@ -880,6 +878,9 @@ bool scaled_mma_takes(const b200_packed_desc *w, const b200_scaled_args *a) {
   if (w->cols % scaled::KS != 0 || w->cols > (1 << 24) || w->rows > (1ll << 31) - 256) return false;
   if ((uintptr_t)w->data % 32 != 0 || (uintptr_t)w->scales % 4 != 0) return false;
   if ((uintptr_t)a->x % 16 != 0 || (uintptr_t)a->x_scales % 4 != 0) return false;
+  // tiles are counted in 31 bits: rows of y / 16 and some for the experts' last ones, times 128 rows of weights
+  const int64_t n = a->experts > 0 ? w->rows / a->experts : w->rows;
+  if ((a->rows / 16 + a->experts + 1) * (n / scaled::TM + 1) >= 1ll << 31) return false;
   return a->experts <= scaled::MAX_EXPERTS;
 }
 
