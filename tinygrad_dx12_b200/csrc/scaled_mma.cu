@@ -450,30 +450,37 @@ __global__ void __launch_bounds__(THREADS, 1)
     bool ok = true;
     while (ok && next_seg(p, run, k, u, g)) {
       const Tile t = tile_at(p, before, start, g.tile);
-      const uint8_t *src[4];  // of rows lane, lane + 32, ...: null where there are none
+      // rows lane, lane + 32, ... of the atom, `has` of them: side by side, or where the plan says
+      const int64_t row = mine ? (int64_t)t.e * p.n + atom * p.second + t.w0 + lane : t.first + (atom - R) * 128 + lane;
+      const int64_t rest = mine ? p.wrows - row : (int64_t)t.rows - (atom - R) * 128 - lane;
+      const int has = rest >= 97 ? 4 : rest <= 0 ? 0 : (int)((rest + 31) >> 5);
+      const uint8_t *src[4];
+      src[0] = (mine ? p.ws : p.xs) + row * p.nblk;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int r = lane + 32 * q;
-        if (mine) {
-          const int64_t row = (int64_t)t.e * p.n + atom * p.second + t.w0 + r;
-          src[q] = row < p.wrows ? p.ws + row * p.nblk : nullptr;
-        } else {
-          const int at = (atom - R) * 128 + r;
-          src[q] = at < t.rows ? p.xs + scale_row(p, t.first + at) * p.nblk : nullptr;
-        }
+      for (int q = 1; q < 4; ++q) src[q] = src[q - 1] + 32 * p.nblk;
+      if (!mine && p.xs_rows != B200_ROWS_PLAN) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (q < has) src[q] = p.xs + scale_row(p, row + 32 * q) * p.nblk;
       }
       // four stages' bytes of each row, from a multiple of four on
       auto load = [&](int s, uint32_t (&v)[4][4]) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          if (p.vector && src[q] != nullptr) {
-            const uint4 w = *reinterpret_cast<const uint4 *>(src[q] + 4 * s);
-            v[q][0] = w.x, v[q][1] = w.y, v[q][2] = w.z, v[q][3] = w.w;
-          } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              v[q][j] = src[q] != nullptr && s + j < p.nst ? *reinterpret_cast<const uint32_t *>(src[q] + 4 * (s + j)) : 0u;
+          uint4 w = make_uint4(0u, 0u, 0u, 0u);
+          if (q < has) {
+            const uint8_t *from = src[q] + 4 * s;
+            if (p.vector) {
+              w = *reinterpret_cast<const uint4 *>(from);
+            } else {
+              const uint32_t *word = reinterpret_cast<const uint32_t *>(from);
+              w.x = word[0];
+              if (s + 1 < p.nst) w.y = word[1];
+              if (s + 2 < p.nst) w.z = word[2];
+              if (s + 3 < p.nst) w.w = word[3];
+            }
           }
+          v[q][0] = w.x, v[q][1] = w.y, v[q][2] = w.z, v[q][3] = w.w;
         }
       };
       // stages begin .. end - 1, and behind the last those before the first
