@@ -15,9 +15,9 @@
  *   - every function returns int32 status: 0 = ok, < 0 = error (B200_ERR_*);
  *   - b200_last_error() copies the calling thread's last error message;
  *   - all pointers to tensors are device pointers owned by the caller. The compute entry
- *     points allocate nothing, with one exception: b200_packed_linear on a few tokens
+ *     points allocate nothing, with these exceptions: b200_packed_linear on a few tokens
  *     (3 <= m <= 64) splits K across CTAs and keeps a 16 MiB split-K workspace, its block-scaled
- *     kernel one of 10 MiB, b200_cache_attention others (see there). The first such call on a
+ *     kernel one of 10 MiB, b200_cache_attention and b200_scaled_linear others (see there). The first such call on a
  *     (device, stream) allocates it for the life of the process; the calls of a stream capture
  *     have one of their own: recorded graphs can be replayed on any streams, beside one another
  *     and beside direct calls (but not several executables of one graph at once); see

@@ -150,6 +150,8 @@ def args(**kw):
     ({}, dict(y_dtype=_lib.DT["float64"]), _lib.ERR_INVALID, "float16"),
     (dict(rows=48), dict(y_dtype=_lib.DT["fp8e4m3"]), _lib.ERR_INVALID, "whole blocks"),
     ({}, dict(x=None), _lib.ERR_INVALID, "null"),
+    ({}, dict(y=4097), _lib.ERR_INVALID, "boundary"),
+    ({}, dict(bias=4097, bias_dtype=_lib.DT["float32"]), _lib.ERR_INVALID, "boundary"),
     ({}, dict(general=1), _lib.ERR_INVALID, "scratch"),
     (dict(format=0), {}, _lib.ERR_UNSUPPORTED, "FP4 or FP6"),
     (dict(block_size=64), {}, _lib.ERR_UNSUPPORTED, "blocks of 32"),

@@ -172,6 +172,10 @@ static int32_t check_scaled(const b200_packed_desc *w, const b200_scaled_args *a
   if (a->x == nullptr || a->x_scales == nullptr || a->y == nullptr || (eight && a->y_scales == nullptr) || w->data == nullptr ||
       w->scales == nullptr || (a->experts > 0 && (a->offsets == nullptr || a->order == nullptr)))
     return b200_set_error(B200_ERR_INVALID, "scaled_linear: null pointer");
+  auto off = [](const void *p, int size) { return p != nullptr && (uintptr_t)p % size != 0; };
+  if (off(a->y, dt_size(a->y_dtype)) || off(a->bias, a->bias != nullptr ? dt_size(a->bias_dtype) : 1) ||
+      off(a->residual, a->residual != nullptr ? dt_size(a->residual_dtype) : 1) || (a->experts > 0 && (off(a->offsets, 4) || off(a->order, 4))))
+    return b200_set_error(B200_ERR_INVALID, "scaled_linear: a tensor off its elements' boundary");
   return B200_OK;
 }
 

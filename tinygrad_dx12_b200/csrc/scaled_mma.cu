@@ -34,11 +34,16 @@
 // launch fits every routing. A tile that a run's border cuts is finished by the last of its CTAs to arrive
 // (acquire-release ticket), which adds the fp32 parts in the order of the CTAs: the same bits every time.
 // No CTA waits for another. Every wait is bounded (sm100.cuh).
+//
+// Measured: 57344 x 8192 FP4, one token 50 us = 5.0 TB/s, bound by the stages' instructions (0.5 us for 16 KB an SM:
+// issue, scales, barriers) and the ring's depth; 4096 x 14336 x 4096 218 us = 2209 TFLOP/s, bound by shared memory (MMA
+// operands, codes in 16-byte slots, x); 64 tokens through 8 of 128 experts 116 + 77 us = 75 and 55 % of HBM.
 #include <string.h>
 
+#include "common.cuh"
 #include "kernels.h"
-#include "mx.cuh"
 #include "scaled_epilogue.cuh"
+#include "sm100.cuh"
 
 namespace b200 {
 
@@ -54,7 +59,7 @@ constexpr int TM = 128, KS = 128;            // weight rows of an MMA, codes of 
 constexpr int EPI_WARPS = 8, SCALE_WARP0 = 8, SCALE_WARPS = 4, MMA_WARP = 12, SF_WARP = 13, W_WARP0 = 14, W_WARPS = 2;
 constexpr int THREADS = 16 * 32;
 constexpr int SLOTS = 12;                    // stages whose scales wait for tensor memory
-constexpr int ACC_COLS = 224;                // columns of an accumulator set: R * NT at most
+constexpr int ACC_COLS = 224;                // columns of a set of accumulators that take turns: R * NT at most
 constexpr int SF_SETS = 4;
 constexpr int MAX_STAGES = 12;
 constexpr int MAX_EXPERTS = 1024;
