@@ -158,6 +158,25 @@ def test_route_odd_logits(tg):
     check_route(tg, x, 6, bias=b)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_route_odd_logits_of_16_bits(tg, dtype):
+    """Infinities above the type's largest value, zeros of both signs, subnormals, equal rows."""
+    f = torch.finfo(dtype)
+    x = torch.zeros((8, 70), device="cuda", dtype=dtype)
+    x[0, 3], x[0, 60] = f.max, math.inf
+    x[1, 3], x[1, 60], x[1, 61] = math.inf, f.max, -math.inf
+    x[2], x[2, 5] = -f.max, -math.inf
+    x[3, ::2] = -0.0
+    x[4] = torch.arange(70, device="cuda") * f.smallest_normal / 128
+    x[5] = -x[4]
+    x[6, 10:] = math.nan
+    x[7, 69], x[7, 0] = 1.0, 1.0
+    for scores in ("softmax", "sigmoid"):
+        for kw in (dict(), dict(renormalize=False), dict(groups=7, top_groups=3), dict(groups=7, top_groups=3, group_best=2),
+                   dict(bias=torch.linspace(0, 1e-3, 70, device="cuda"))):
+            check_route(tg, x, 6, scores=scores, **kw)
+
+
 @pytest.mark.parametrize("live", [0, 1, 77, 100, 500])
 def test_route_live(tg, live):
     g = H.generator(live)

@@ -36,10 +36,11 @@ __device__ __forceinline__ uint64_t order64(double v) {
   return u ^ ((u >> 63) ? ~0ull : 1ull << 63);
 }
 __device__ __forceinline__ float value32(uint32_t k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu)); }
-// The same of a 16-bit logit that was widened: 16 bits, never 0.
+// The same of a 16-bit logit that was widened: 16 bits, never 0. What stood for infinity stays above the type's
+// largest value.
 __device__ __forceinline__ uint32_t packed16(uint32_t k, int dtype) {
-  if (dtype == B200_DT_BF16) return k >> 16;
-  const uint32_t h = (uint32_t)__half_as_ushort(__float2half_rz(value32(k)));  // exact, but for what stood for infinity
+  if (dtype == B200_DT_BF16) return (k >> 16) + (k == order32(3.402823466e38f) ? 1u : 0u);
+  const uint32_t h = (uint32_t)__half_as_ushort(__float2half_ru(value32(k)));
   return h ^ ((h >> 15) ? 0xFFFFu : 0x8000u);
 }
 __device__ __forceinline__ double value64(uint64_t k) {
