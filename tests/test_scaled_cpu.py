@@ -73,6 +73,7 @@ def test_no_cpu_path():
     (lambda: tg.route_experts(torch.zeros(2, 8), 2, groups=4, group_best=3), "groups"),
     (lambda: tg.route_experts(torch.zeros(2, 8), 3, groups=4, top_groups=1), "do not hold"),
     (lambda: tg.plan_experts(torch.zeros(4, dtype=torch.int32), torch.zeros(4), 4), "tokens, k"),
+    (lambda: tg.plan_experts(torch.zeros(4, 0, dtype=torch.int32), torch.zeros(4, 0), 4), "at least 1"),
     (lambda: tg.plan_experts(torch.zeros(4, 1, dtype=torch.int64), torch.zeros(4, 1), 4), "int32"),
     (lambda: tg.plan_experts(torch.zeros(4, 1, dtype=torch.int32), torch.zeros(4, 2), 4), "weights"),
     (lambda: tg.plan_experts(torch.zeros(4, 1, dtype=torch.int32), torch.zeros(4, 1), 0), "1 to"),

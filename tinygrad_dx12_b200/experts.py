@@ -143,8 +143,8 @@ def route_experts(logits: torch.Tensor, k: int, scores: str = "softmax", bias: t
 def plan_experts(indices: torch.Tensor, weights: torch.Tensor, experts: int, first: int = 0) -> Routing:
     """The ``Routing`` of given ``indices`` int32 and ``weights`` float32 (tokens, k), for the experts ``first`` ..
     ``first + experts - 1``: all of a model's, or those that this rank holds. Others' indices stand for no expert here."""
-    if indices.dim() != 2 or indices.dtype != torch.int32:
-        raise ValueError("indices must be int32 (tokens, k)")
+    if indices.dim() != 2 or indices.dtype != torch.int32 or indices.shape[1] < 1:
+        raise ValueError("indices must be int32 (tokens, k), k at least 1")
     if weights.shape != indices.shape or weights.dtype != torch.float32:
         raise ValueError("weights must be float32 of indices' shape")
     if not 1 <= experts <= MAX_EXPERTS or first < 0 or first + experts > 1 << 30:
