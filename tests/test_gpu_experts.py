@@ -254,6 +254,25 @@ def test_expert_linear(tg, fmt, tokens, k, experts, n, cols, general):
         H.check(E.expert_linear(x, w, r, dtype=torch.bfloat16, _general=general), v, tol)
 
 
+@pytest.mark.parametrize("general", [True, False])
+@pytest.mark.parametrize("indices", [[[2, 2, 5]], [[1] * 20], [[0, 3, 0, -1, 3, 3]], [[2, 2], [2, 1]], [[4]]])
+def test_the_same_expert_twice(tg, indices, general):
+    """A token may name an expert more than once: each of its pairs is answered."""
+    from tinygrad_dx12_b200 import experts as E
+
+    g = H.generator(len(indices[0]))
+    at = torch.tensor(indices, dtype=torch.int32, device="cuda")
+    r = tg.plan_experts(at, torch.rand(at.shape, device="cuda", generator=g), 6)
+    up, down = H.make_weights((6, 256, 256), "fp4_e2m1", g), H.make_weights((6, 256, 128), "fp6_e2m3", g)
+    x = tg.quantize(torch.randn((len(indices), 256), device="cuda", generator=g))
+    xx = H.values(x.codes, x.scales)
+    for kw in (dict(), dict(gated=True, activation="silu")):
+        v, tol = pairs64(xx, up, r, None, **kw)
+        H.check(E.expert_linear(x, up, r, dtype=torch.float32, _general=general, **kw), v, tol)
+    y = E.expert_mlp(x, up, down, r, dtype=torch.float32, _general=general)
+    H.check(y, *mlp64(xx, up, down, r, "silu", True, None, None, None))
+
+
 @pytest.mark.parametrize("count", [0, 1, 15, 16, 17, 112, 113, 224, 225, 500])
 def test_expert_token_counts(tg, count):
     """One expert has ``count`` tokens, its neighbours none or the others."""

@@ -638,8 +638,14 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int part = step % PARTS, j0 = step / PARTS * CH, count = t.rows - j0 < CH ? t.rows - j0 : CH;
         float v[TOGETHER][CH];
 #pragma unroll
-        for (int q = 0; q < TOGETHER; ++q) tmem_ld_32x32b_x16(acc + (uint32_t)(part + q) * p.acc_width + (uint32_t)j0, reinterpret_cast<uint32_t (&)[CH]>(v[q]));
+        for (int q = 0; q < TOGETHER; ++q) tmem_ld_32x32b_x16(acc + (uint32_t)(part + q) * p.acc_width + (uint32_t)(p.single_row ? 0 : j0), reinterpret_cast<uint32_t (&)[CH]>(v[q]));
         tmem_ld_wait();
+        if (p.single_row) {  // a token that names an expert twice: its row is the first column's
+#pragma unroll
+          for (int q = 0; q < TOGETHER; ++q)
+#pragma unroll
+            for (int j = 1; j < CH; ++j) v[q][j] = v[q][0];
+        }
         if (step + 2 >= steps) {  // the group's last columns are read: the accumulator may be used again
           tc_fence_before();
           __syncwarp();
