@@ -300,6 +300,13 @@ def test_linear_operands_of_any_layout(tg):
     assert tg.scaled_linear(tg.quantize(rows((0, 256), g)), w).shape == (0, 192)
 
 
+@pytest.mark.parametrize("k", [1 << 24, (1 << 24) + 128])
+def test_linear_of_very_long_rows(tg, k):
+    """The last width of the tensor cores' kernel, and the first behind it."""
+    g = H.generator(17)
+    run(tg, activations(tg, 2, k, g), H.make_weights((3, k), "fp4_e2m1", g), dtype=torch.float32)
+
+
 def test_nan_stays_in_its_row(tg):
     """A NaN scale of a token or of a weight row reaches that row or column alone."""
     g = H.generator(12)

@@ -274,7 +274,7 @@ def _args(x, xs, rows, y, ys, y_dtype, bias, activation, gated, residual=None, p
 
 def _scratch_bytes(desc, a: ScaledArgs, w: PackedTensor) -> int:
     """What the product needs besides: the general kernel's sums, or rows in the plan's order."""
-    if a.general or w.shape[-1] % 128 or desc.data % 32 or desc.scales % 4 or (a.experts and a.x_rows != ROWS_PLAN):
+    if a.general or w.shape[-1] % 128 or w.shape[-1] > 1 << 24 or desc.data % 32 or desc.scales % 4 or (a.experts and a.x_rows != ROWS_PLAN):
         return _lib.lib().b200_scaled_linear_scratch(ctypes.byref(desc), ctypes.byref(a))
     return 0
 
