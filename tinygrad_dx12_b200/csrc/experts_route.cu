@@ -182,9 +182,14 @@ __device__ __forceinline__ bool route_row(const b200_route_args &a, int64_t row,
       if (MODE == PACKED && key[i] != 0) key[i] = (packed16(key[i], a.dtype) << 16) | (0xFFFFu - (uint32_t)(lane + 32 * i));
     }
   }
-  // A score's error in 32 bits is below 2e-6 of it (the exponential's, its sum's, the division's), and a score is at
-  // most |choice| + the largest |bias|: two choices or sums that differ by this or less may be in either order.
-  auto close = [&](float higher, float lower) { return higher - lower <= 8e-6f * (fabsf(higher) + span); };
+  // What 32 bits are not sure of. A score c = e^(x - top) / total is off by E c: the subtraction's rounding is up to 2^-18
+  // of an exponent (x - top beyond -64), the total's up to (N + 5) 2^-24 <= 2^-18.8 (lanes' terms, then the tree), exponentials
+  // and division 5 ulp: 9e-6 in all; a sigmoid has only the last, 8e-7. A choice is c + bias, a group's sum two of them, so the
+  // scores in it add up to at most |sum| + 2 span, and two sums that differ by more than 2 E (|higher| + 2 span) and what the
+  // additions round (2^-24 of the same) are in order. Below 2^-126 a score is off by steps of 2^-149 whatever its size, and the fast
+  // division gives zero: 2^-100 covers that. What is no number (infinite sums) is not sure either.
+  const float unsure = a.sigmoid ? 4e-6f : 2e-5f;
+  auto close = [&](float higher, float lower) { return !(higher - lower > fmaf(unsure, fabsf(higher) + 2.f * span, 7.9e-31f)); };
   if (a.groups > 1) {
     const int size = a.experts / a.groups;
     Key *keys = (Key *)smem;
