@@ -3,7 +3,7 @@
 // do not begin on a 32-byte boundary.
 //
 // A warp computes one output: lane l takes the blocks of 32 columns l, l + 32, ..., decodes 32 codes of
-// each side exactly, sums their products in fp32 and multiplies by the two powers of two. Raw sums go to
+// each side exactly, sums their products in fp32 and multiplies by the product of the two powers of two. Raw sums go to
 // scratch; a second launch applies bias, activation, gate and residual, and rounds or quantises (a warp
 // holds 32 neighbouring columns, a block). Bound by the decoding: some 0.1 TFLOP/s. It is there so that
 // every call has an answer, not for speed.
@@ -32,6 +32,12 @@ __device__ __forceinline__ int expert_at(const int32_t *offsets, int experts, in
     else hi = mid;
   }
   return lo;
+}
+
+// part * 2^(a - 127) * 2^(b - 127), rounded once: by the exponents' sum, as the tensor cores have it. (One factor after the other
+// overflows or loses bits on the way where the scales lie far apart.)
+__device__ __forceinline__ float scaled_sum(float part, int a, int b) {
+  return a == 255 || b == 255 ? __uint_as_float(0x7FC00000u) : ldexpf(part, a + b - 254);
 }
 
 template <int FMT>
@@ -63,7 +69,7 @@ __global__ void __launch_bounds__(256) product_kernel(const __grid_constant__ Ge
         for (int j = 0; j < 4; ++j)
           part = fmaf(decode_fp<FMT>((word >> (j * BITS)) & ((1u << BITS) - 1)), rows8::code_value(x[b * 32 + g * 4 + j]), part);
       }
-      sum += part * e8m0_to_f32(p.ws[wrow * nblk + b]) * e8m0_to_f32(p.xs[xrow * nblk + b]);
+      sum += scaled_sum(part, p.ws[wrow * nblk + b], p.xs[xrow * nblk + b]);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
