@@ -21,10 +21,13 @@ inline Epilogue epilogue_of(const b200_packed_desc *w, const b200_scaled_args *a
                   a->bias_dtype, a->residual_dtype, a->y_dtype, a->activation, a->gated};
 }
 
-// v / (1 + e^(-z)) by the fast exponential and division, each within 2 ulp for |z| up to 16: fp32 results of 33 x 8192 gated
-// columns over 8192 are 8.8e-8 off 64 bits, as with the exact functions, which cost a prompt 5 %. A sum above 2^126
-// divides to zero, which is the value's limit.
-__device__ __forceinline__ float times_sigmoid(float v, float z) { return __fdividef(v, 1.f + __expf(-z)); }
+// v times the sigmoid of z, by t = e^-|z|: 1 / (1 + t) or t / (1 + t). The denominator lies in [1, 2], where the fast division
+// is within 2 ulp, and t keeps its relative precision until it is subnormal, so a tail is exact to 6 ulp of itself. The
+// exponential is the full one: __expf's error grows with |z| (20 ulp at 16), and its 1 + e^-z left nothing of z below -87.
+__device__ __forceinline__ float times_sigmoid(float v, float z) {
+  const float t = expf(-fabsf(z));
+  return __fdividef(z < 0.f ? v * t : v, 1.f + t);
+}
 
 template <int ACT>
 __device__ __forceinline__ float activate(float v) {
