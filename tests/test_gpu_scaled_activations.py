@@ -38,7 +38,11 @@ def relative(v, name):
     rel = torch.full_like(v, (12 if name == "gelu" else 8) * ulp)
     if name == "gelu_tanh":
         rel = rel + 2.5 * ulp * 2 * math.sqrt(2 / math.pi) * (v.abs() + 0.044715 * v.abs() ** 3)
-    return rel, (2 * v.abs().clamp(max=200) + 2) * 2.0 ** -149
+    least = (2 * v.abs().clamp(max=200) + 2) * 2.0 ** -149
+    if name == "gelu":
+        rel = rel + ulp * v.square() / 18
+        least = least + v.abs().clamp(max=15) * 2.0 ** -127
+    return rel, least
 
 
 def exactly(v, name):
@@ -64,7 +68,7 @@ def activated(tg, bias, general, rows=17, **kw):
 
 
 @pytest.mark.parametrize("general", [True, False])
-@pytest.mark.parametrize("name", ["relu", "silu", "gelu_tanh"])
+@pytest.mark.parametrize("name", ["relu", "silu", "gelu", "gelu_tanh"])
 def test_activation_by_its_own_size(tg, name, general):
     v = grid()
     want = exactly(v.double(), name)
@@ -75,7 +79,7 @@ def test_activation_by_its_own_size(tg, name, general):
 
 
 @pytest.mark.parametrize("general", [True, False])
-@pytest.mark.parametrize("name", ["relu", "silu", "gelu_tanh"])
+@pytest.mark.parametrize("name", ["relu", "silu", "gelu", "gelu_tanh"])
 def test_gate_by_its_own_size(tg, name, general):
     """A tail times a large number is no tail."""
     v = grid()
@@ -91,7 +95,7 @@ def test_gate_by_its_own_size(tg, name, general):
 
 
 @pytest.mark.parametrize("general", [True, False])
-@pytest.mark.parametrize("name", [None, "relu", "silu", "gelu_tanh"])
+@pytest.mark.parametrize("name", [None, "relu", "silu", "gelu", "gelu_tanh"])
 def test_infinities_nan_and_large_values(tg, name, general):
     """What the formula gives for them in 64 bits, as fp32 holds it."""
     v = torch.tensor([-math.inf, -3e38, -1.5, -0.0, 0.0, 2.0, 3e38, math.inf, math.nan], device="cuda")
