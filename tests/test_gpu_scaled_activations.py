@@ -27,22 +27,24 @@ def grid():
 
 
 def relative(v, name):
-    """How far fp32 may take an activation of v from its value, relative to it, and absolutely where it is subnormal.
+    """How far fp32 may take an activation of v from its value, relative to it, and absolutely where it vanishes.
 
-    A sigmoid by t = e^-|z| <= 1: the exponential 2 ulp, 1 + t half of one, the division 2, two products one: 5.5 ulp, at most
-    2^-23 each; 8 are allowed. gelu by e^(-v^2/2) times a polynomial in 1 / (1 + p|v|): its eight steps and its fit 3.3
-    (its terms add up to 2.3 times its value), the exponential and its correction 2.5, the division 2, products and the
-    subtraction 2: 12. tanh's form: its argument has 5 roundings of half an ulp, each of which moves the exponential by
-    |z| of it. A subnormal exponential is off by up to 2 steps of 2^-149, which v multiplies."""
-    ulp = 2.0 ** -23
-    rel = torch.full_like(v, (12 if name == "gelu" else 8) * ulp)
-    if name == "gelu_tanh":
-        rel = rel + 2.5 * ulp * 2 * math.sqrt(2 / math.pi) * (v.abs() + 0.044715 * v.abs() ** 3)
-    least = (2 * v.abs().clamp(max=200) + 2) * 2.0 ** -149
+    A sigmoid by t = e^-|z| <= 1 as a power of two: the power 2 ulp and its correction half of one, 1 + t another half, the
+    division 2, two products one: 6 ulp, at most 2^-23 each; 8 are allowed. log2(e) as a number of fp32 is off by 1.4e-8 of
+    itself, which moves the power by |z| times that, |z| / 8 ulp; a power below 2^-126 is zero, and v multiplies it. tanh's
+    form: its argument has 5 roundings of half an ulp, each of which moves the power by |z| of it.
+    gelu by 2^(-v^2 log2(e) / 2) times a polynomial in 1 / (1 + p|v|): its eight steps and its fit 3.3 (its terms add up to 2.3
+    times its value), the power 2 and its correction half of one, the division 2, products and the subtraction 2: 10, and 12 are
+    allowed; log2(e) / 2 moves the power by v^2 / 18 ulp; below 2^-126 it is zero, and half of v multiplies it."""
+    ulp, a = 2.0 ** -23, v.abs()
+    z = {"silu": a, "gelu_tanh": 2 * math.sqrt(2 / math.pi) * (a + 0.044715 * a ** 3)}.get(name, torch.zeros_like(a))
+    rel = ((12 if name == "gelu" else 8) + z / 8) * ulp
+    least = (2 * a.clamp(max=200) + 2) * 2.0 ** -149
     if name == "gelu":
-        rel = rel + ulp * v.square() / 18
-        least = least + v.abs().clamp(max=15) * 2.0 ** -127
-    return rel, least
+        return rel + ulp * a.square() / 18, least + a.clamp(max=15) * 2.0 ** -127
+    if name == "gelu_tanh":
+        rel = rel + 2.5 * ulp * z
+    return rel, least + a.clamp(max=128) * 2.0 ** -126
 
 
 def exactly(v, name):

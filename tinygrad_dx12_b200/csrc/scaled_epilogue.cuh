@@ -22,10 +22,15 @@ inline Epilogue epilogue_of(const b200_packed_desc *w, const b200_scaled_args *a
 }
 
 // v times the sigmoid of z, by t = e^-|z|: 1 / (1 + t) or t / (1 + t). The denominator lies in [1, 2], where the fast division
-// is within 2 ulp, and t keeps its relative precision until it is subnormal, so a tail is exact to 6 ulp of itself. The
-// exponential is the full one: __expf's error grows with |z| (20 ulp at 16), and its 1 + e^-z left nothing of z below -87.
+// is within 2 ulp, and t keeps its relative precision, so a tail is exact to 6 + |z| / 8 ulp of itself down to t = 2^-126,
+// where it becomes zero (z = -87.3). The power of two takes |z| log2(e) with what it rounds off; without that it is off by
+// |z| ulp. 4096 tokens x 14336 x 4096, us: gated 241, FP6 with a bias 279; with CUDA's full exponential 248 and 302, with its
+// fast one 236 and 270.
 __device__ __forceinline__ float times_sigmoid(float v, float z) {
-  const float t = expf(-fabsf(z));
+  const float a = fminf(fabsf(z), 128.f), h = a * -1.44269504f;
+  float t;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(h));
+  t = fmaf(t * 0.69314718f, fmaf(a, -1.44269504f, -h), t);
   return __fdividef(z < 0.f ? v * t : v, 1.f + t);
 }
 
