@@ -888,12 +888,13 @@ bool scaled_mma_takes(const b200_packed_desc *w, const b200_scaled_args *a) {
 }
 
 int32_t launch_scaled_mma(const b200_packed_desc *w, const b200_scaled_args *a, cudaStream_t stream) {
-  // Two accumulators of 112 tokens halve a decode step's stages (one token x 57344 x 8192, us: 60 with one, 48 with
-  // two) and load less for many tokens (4096 x 1024 x 16384 93 / 66); between, one of 224 goes over the weights
-  // half as often (128 tokens x 57344 x 8192 85 / 108, 300 tokens 172 / 189, 600 tokens 284 / 356).
-  const int64_t rows = scaled::rows_of_one(a);
+  // Two accumulators of 112 tokens halve a decode step's stages (one token x 57344 x 8192, us, with two / one: 48 / 60) and
+  // load less for many tokens (2560 x 8192 x 8192 157 / 175, 4096 x 1024 x 16384 67 / 90); between, one of 224 goes over the weights
+  // half as often (128 tokens x 57344 x 8192 97 / 82, 800 x 4096 x 14336 60 / 55, 1600 x 8192 x 8192 117 / 106, 2048 x 14336 x 4096
+  // 132 / 127). Experts' tiles are seldom full, whatever their width: two at every share (224 tokens each x 4096 x 2048 64 / 77,
+  // 500 118 / 137, 1100 259 / 264; of 2048 x 4096 128 tokens each 43 / 40, 500 97 / 102, 2500 401 / 462).
   if (a->gated) return scaled::dispatch<2, true>(w, a, scaled::single(a) ? 1 : 2, stream);
-  if (rows <= scaled::ACC_COLS / 2 || rows > 1024) return scaled::dispatch<2, false>(w, a, 2, stream);
+  if (a->experts > 0 || a->rows <= scaled::ACC_COLS / 2 || a->rows > 2304) return scaled::dispatch<2, false>(w, a, 2, stream);
   return scaled::dispatch<1, false>(w, a, 2, stream);
 }
 
