@@ -406,8 +406,8 @@ int32_t b200_scaled_values(const void *codes, const void *scales, int64_t rows, 
  * run on the tensor cores, other calls on a general kernel. `scratch`: b200_scaled_linear_scratch bytes,
  * for the general kernel's sums, or rows of x in the plan's order. Workspace: 65 MiB per (device,
  * stream) or capture. The kernels may start while the one before them ends (programmatic dependent
- * launch): they read weights and their scales at once, so no kernel that is launched to start others
- * early may write these. */
+ * launch), and read and write nothing until it has. Activations are exact to a few units in the last place of
+ * their own result, which becomes zero where a sigmoid or gelu's tail falls below 2^-126. */
 #define B200_ROWS_TOKENS 0
 #define B200_ROWS_PAIRS 1
 #define B200_ROWS_PLAN 2

@@ -10,7 +10,7 @@
 // sums the counts over the chunks, and each CTA places its chunk: warps own consecutive pieces of it, so a
 // pair's place is what lies before it in earlier chunks, earlier warps, earlier rounds and lower lanes.
 // No atomics on places: the order is the same every time. Few pairs take one launch of one CTA.
-// Bound by the launches up to some ten thousand pairs, then by HBM (logits).
+// Bound by the launches up to some ten thousand pairs, then by the routing's instructions (32768 rows of 64 experts: issue 64 %).
 #include <type_traits>
 
 #include "kernels.h"
@@ -533,7 +533,7 @@ static int32_t plan(const int32_t *indices, int64_t pairs, int first, int expert
   return B200_OK;
 }
 
-// Up to this many rows (two a warp) routing and plan are one launch: 4.5 us for one row, in two launches 7.
+// Up to this many rows (two a warp) routing and plan are one launch: 5.7 us for one row, in two launches 6.8.
 constexpr int64_t FEW_ROWS = 2 * PLAN_WARPS;
 
 template <int N, Mode MODE>

@@ -68,7 +68,7 @@ constexpr int CH = 16;                       // tokens of an epilogue step: more
 constexpr int SMEM_LIMIT = 227 * 1024;
 
 struct Params {
-  const uint8_t *x, *xs, *ws;
+  const uint8_t *xs, *ws;
   const int32_t *offsets, *order;
   int64_t rows, n;        // rows of y, weight rows of one matrix
   int64_t wrows;          // of all matrices
@@ -774,7 +774,7 @@ static int32_t launch_t(const b200_packed_desc *w, const b200_scaled_args *a, in
   const int bits = fmt_bits(w->format);
   Params p;
   memset(&p, 0, sizeof(p));
-  p.x = (const uint8_t *)a->x, p.xs = (const uint8_t *)a->x_scales, p.ws = (const uint8_t *)w->scales;
+  p.xs = (const uint8_t *)a->x_scales, p.ws = (const uint8_t *)w->scales;
   p.offsets = a->offsets, p.order = a->order;
   p.rows = a->rows;
   p.n = a->experts > 0 ? w->rows / a->experts : w->rows;
@@ -876,7 +876,7 @@ bool scaled_gathers(const b200_scaled_args *a) {
   return a->experts > 0 && a->x_rows != B200_ROWS_PLAN && !(a->x_rows == B200_ROWS_TOKENS && a->rows <= a->fan) && a->rows > 1;
 }
 
-// What the checks of the entry have left: whole stages, and the alignment that TMA and cp.async ask for.
+// What the checks of the entry have left: whole stages, and the alignment that TMA and the loads of scales ask for.
 bool scaled_mma_takes(const b200_packed_desc *w, const b200_scaled_args *a) {
   if (w->cols % scaled::KS != 0 || w->cols > (1 << 24) || w->rows > (1ll << 31) - 256) return false;
   if ((uintptr_t)w->data % 32 != 0 || (uintptr_t)w->scales % 4 != 0) return false;

@@ -252,7 +252,8 @@ class _Rows:
 class ScaledOps(CudaOps):
     """CudaOps with 8-bit activations: the norms quantise their rows and the projections multiply them as stored
     (``rms_norm``, ``scaled_linear``), the gate's product in the epilogue of gate and up. For FP4 and FP6 stacks with
-    E8M0 scales in blocks of 32 (config c5)."""
+    E8M0 scales in blocks of 32 (config c5). Over ranks the partial sums are reduced by ``all_reduce`` (not by
+    ``PeerOps``' kernel), and a shard whose K is no multiple of 128 takes ``scaled_linear``'s general kernel."""
 
     def rows(self, h: torch.Tensor) -> _Rows:
         return _Rows()
@@ -409,9 +410,11 @@ class TPStack:
         cfg, ops = self.cfg, self.ops
         m = h.shape[0]
         x = ops.rows(h) if hasattr(ops, "rows") else torch.empty_like(h)
-        mbuf = torch.empty((m, self.layers[0].inter_rows if self.layers else 0), dtype=cfg.act, device=h.device)
+        gated, mbuf = getattr(ops, "gated", None), None  # a gate of its own allocates its result
+        if gated is None:
+            mbuf = torch.empty((m, self.layers[0].inter_rows if self.layers else 0), dtype=cfg.act, device=h.device)
+            gated = lambda w, xx, out, act: _gated(ops, w, xx, out, act)  # noqa: E731
         ops.add_rmsnorm(h, None, x)
-        gated = getattr(ops, "gated", None) or (lambda w, xx, out, act: _gated(ops, w, xx, out, act))
         if self.world == 1:  # unsharded: nothing to reduce whatever the process group holds
             row_reduce = lambda w, inp, hh, xx, slot: _local_row_reduce(ops, w, inp, hh, xx)  # noqa: E731
         else:
