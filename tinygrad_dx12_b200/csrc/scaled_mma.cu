@@ -35,9 +35,9 @@
 // (acquire-release ticket), which adds the fp32 parts in the order of the CTAs: the same bits every time.
 // No CTA waits for another. Every wait is bounded (sm100.cuh).
 //
-// Measured: 57344 x 8192 FP4, one token 50 us = 5.0 TB/s, bound by the stages' instructions (0.5 us for 16 KB an SM:
-// issue, scales, barriers) and the ring's depth; 4096 x 14336 x 4096 218 us = 2209 TFLOP/s, bound by shared memory (MMA
-// operands, codes in 16-byte slots, x); 64 tokens through 8 of 128 experts 116 + 77 us = 75 and 55 % of HBM.
+// Measured: 57344 x 8192 FP4, one token 52 us = 4.8 TB/s, bound by the stages' instructions (0.5 us for 16 KB an SM:
+// issue, scales, barriers) and the ring's depth; 4096 x 14336 x 4096 238 us = 2021 TFLOP/s, bound by shared memory (MMA
+// operands, codes in 16-byte slots, x); 64 tokens through 8 of 128 experts 114 + 73 us = 76 and 58 % of HBM.
 #include <string.h>
 
 #include "common.cuh"
@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     run.whole = waves + (run.ctas == 0 && (int)blockIdx.x < rest ? 1 : 0);
     run.units = run.ctas > 0 ? (int64_t)rest * p.nst : 0;
     // Weights that only one tile of tokens reads gain nothing from tiles in turn: equal runs of all of them, whose first
-    // and last tiles are cut (33 tokens gated, 224 tiles: 58 us; a tile each, then parts of 76: 66), if that ends sooner
+    // and last tiles are cut (33 tokens gated, 224 tiles: 66 us; a tile each, then parts of 76: 72), if that ends sooner
     // than a wave of the rest
     const int64_t equal = (all * p.nst + p.grid - 1) / p.grid + p.join + 3 * p.join_part / 16;
     if (p.once && waves > 0 && rest > 0 && equal < (int64_t)(waves + 1) * p.nst) {
@@ -762,7 +762,7 @@ static int64_t rows_of_one(const b200_scaled_args *a) {
   return a->experts > 0 ? (a->rows + a->experts - 1) / a->experts : a->rows;
 }
 // Gated, 113 to 224 tokens: accumulators of twice the width that do not take turns, so that the weights
-// are read once (200 tokens x 57344 x 8192 146 us, with two tiles of tokens 155).
+// are read once (200 tokens x 57344 x 8192 112 us, with two tiles of tokens 122).
 static bool single(const b200_scaled_args *a) {
   return a->experts == 0 && a->rows > ACC_COLS / 2 && a->rows <= ACC_COLS;
 }

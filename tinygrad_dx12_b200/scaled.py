@@ -14,7 +14,8 @@ Everything runs in the library's kernels on the current stream; there is no CPU 
 none, whatever their operands ask for.
 
 Which product to take: ``scaled_linear`` for many tokens (several times ``matmul``'s rate), for an epilogue and for
-experts; at one to four tokens ``matmul`` streams the weights at least as fast, on 16-bit activations.
+experts; at one or two tokens ``matmul`` streams the weights as fast or faster, on 16-bit activations (one token x 57344 x
+8192 49 us and 52, x 8192 x 8192 11 and 18; eight 83 and 52, 18 and 18).
 """
 
 from __future__ import annotations
